@@ -41,7 +41,12 @@ typedef enum {
     RLH_ERR_UNSUPPORTED = 6   /* arch is not gfx950, or a dtype the reference does not offload either */
 } rlh_status;
 
-typedef enum { RLH_F16 = 0, RLH_F32 = 1 } rlh_dtype;   /* TensorDType (src/tensor.rs:50-54) */
+/* TensorDType (src/tensor.rs:50-54).  RLH_Q4 (K4BitQuantization, which the reference names and leaves unimplemented) and RLH_I32
+ * (token ids) are taken by the calls that say so; every other call refuses them with RLH_ERR_UNSUPPORTED.
+ * A 4-bit tensor [rows x cols], cols a multiple of 32, is one buffer of rows * cols / 32 * 20 bytes: first the codes, row after row,
+ * two to a byte (the even column in the low half), then for each row and each group of 32 columns a pair of f16 numbers (scale,
+ * lowest).  A value is lowest + code * scale. */
+typedef enum { RLH_F16 = 0, RLH_F32 = 1, RLH_Q4 = 2, RLH_I32 = 3 } rlh_dtype;
 
 /* Weight names: src/transformer.rs:297-304, 405-412, 490-503, 595-614; src/embedding.rs:18 */
 typedef enum {
@@ -292,6 +297,64 @@ int  rlh_attn_prefill(rlh_tensor *out, const rlh_tensor *qkv, rlh_tensor *cache_
  * is the largest scaled logit (lowest id among equal ones); once it is not (a scaled logit above ln(FLT_MAX), a NaN, or
  * the sum itself overflowing) every probability is 0 or NaN and the pick is token 0. */
 int  rlh_argmax_greedy(const rlh_tensor *logits, float temperature, int32_t *token);
+
+/* ------------------------------------------------------------------------------------------------
+ * Long contexts and drafted tokens (no reference counterpart): the attention block over caches of 16, 32 or 4 bits with grouped
+ * heads, several sequences and a sliding window, and the choice of tokens from rows of logits.  All work is queued on the
+ * context's stream; no call here waits for it, and none allocates device memory except where it says so.
+ *
+ * Rows and positions.  A call takes n rows of each of n_seqs sequences (1..256): row b * n + i of its tensors is sequence b's
+ * row at position start_pos[b] + i.  A negative position is padding (rows on the left of a short prompt, an idle slot of a batch):
+ * it is neither written nor looked at, and its rows of the results are zeros.
+ * Cache planes are two tensors [n_seqs * n_kv_heads * max_seq_len x head_dim] of one dtype (f16, f32 or Q4), head_dim 32, 64 or
+ * 128; row (b * n_kv_heads + g) * max_seq_len + r.  Query head h reads key and value head h / (n_heads / n_kv_heads).
+ * Position t is kept in row t while t < max_seq_len.  Later positions, which need a window, replace the oldest ones behind the
+ * first `sinks`: row sinks + (t - sinks) % (max_seq_len - sinks).  Both calls below take the same `sinks`.
+ * ---------------------------------------------------------------------------------------------- */
+/* A tensor over device memory that the caller owns (another library's, on this device; 16-byte aligned): nothing is copied, and
+ * rlh_tensor_free frees only the handle, when the context's queued work is done.  The memory has to outlive the handle.  Work that the
+ * caller queued on a stream of its own is not seen: order it with the two calls below. */
+int  rlh_tensor_wrap(rlh_ctx *ctx, void *device_memory, int rows, int cols, int dtype, rlh_tensor **out);
+/* The context's later work waits for what is queued on `stream` (a hipStream_t; NULL = the default stream) by now ... */
+int  rlh_wait_stream(rlh_ctx *ctx, void *stream);
+/* ... and later work on `stream` for what is queued on the context by now.  Neither makes the host wait. */
+int  rlh_release_stream(rlh_ctx *ctx, void *stream);
+/* dst = src between f16, f32 and Q4 tensors of one shape.  To Q4, per group of 32 columns: lowest = f16(min), scale =
+ * f16((max - lowest) / 15), code = round((x - lowest) / scale), ties to even, within 0..15 (scale 0: code 0).  A group with a value
+ * that is not finite, or whose lowest or scale f16 cannot hold, reads as NaN throughout. */
+int  rlh_convert(rlh_tensor *dst, const rlh_tensor *src);
+/* The angles of positions 0 .. rows - 1, freqs f32 [rows x head_dim]: pairs (cos, sin) of position * theta^(-2j / head_dim), formed in
+ * 64 bits on the host and rounded (compute_freqs_cis, src/transformer.rs:858-885, with theta 10000).  Waits for the upload. */
+int  rlh_rope_table(rlh_tensor *freqs, double theta);
+/* A projection's rows into the caches, in one pass: qkv [n_seqs * n x (n_heads + 2 n_kv_heads) head_dim] f16 or f32, columns of the
+ * queries, then keys, then values.  Queries and keys are normalised per head (x / sqrt(mean x^2 + eps) * weight; q_norm and k_norm
+ * f32 [1 x head_dim], NULL = left out) and rotated by their position's row of freqs (f32, a row for every position; halves = 0: columns
+ * 2j and 2j + 1 are a pair, as in the reference; 1: columns j and j + head_dim / 2); queries go to q [n_seqs * n x n_heads head_dim]
+ * (dtype of qkv), keys and values into the planes.  Arithmetic in f32, one rounding to each result's type. */
+int  rlh_qkv_append(rlh_tensor *q, const rlh_tensor *qkv, const rlh_tensor *q_norm, const rlh_tensor *k_norm, double eps, const rlh_tensor *freqs,
+                    int halves, rlh_tensor *cache_k, rlh_tensor *cache_v, int n_heads, int n_kv_heads, int max_seq_len, int sinks,
+                    const int32_t *start_pos, int n_seqs);
+/* Attention of the rows over the planes, which hold the rows' own positions already: the row at position p sees the positions
+ * t <= p with t < sinks or t > p - window (window 0: all of them), out = softmax(q K^T / sqrt(head_dim)) V.  q and out
+ * [n_seqs * n x n_heads head_dim], both f16 or both f32.  f32: f32 arithmetic throughout.  f16: f16 operands with f32 sums; values of
+ * 4 bits and the softmax's weights are rounded to f16 in front of the products.  Rows and keys outside what is seen may hold anything,
+ * NaN included.  Positions beyond max_seq_len need window > 0 and sinks + window + n - 1 <= max_seq_len.
+ * The first call of a size allocates work memory that stays with the context (partial results of a sequence that is cut). */
+int  rlh_attn_window(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *cache_k, const rlh_tensor *cache_v, int n_heads, int n_kv_heads,
+                     int max_seq_len, const int32_t *start_pos, int n_seqs, int window, int sinks);
+/* Probabilities of rows of logits: probs f32 [n x vocab] = softmax(logits / temperature), logits f16 or f32.  temperature 0: 1 at the
+ * first of the largest logits, 0 elsewhere.  A row of nothing but -infinity gives zeros; a row with a NaN or +infinity gives NaN. */
+int  rlh_softmax_rows(rlh_tensor *probs, const rlh_tensor *logits, float temperature);
+/* Verification of drafted tokens (speculative sampling), for each of n_seqs sequences: target f32 [n_seqs * (k + 1) x vocab], the
+ * model's probabilities behind the text and behind each drafted token; draft f32 [n_seqs * k x vocab], the probabilities that the
+ * tokens were drawn from (NULL: each was certain); drafted i32 [n_seqs x k]; uniforms f32 [n_seqs x (k + 1)] in [0, 1).
+ * Token i is accepted while uniforms[i] * q_i(token) < p_i(token).  At the first refusal one token is drawn from max(p_i - q_i, 0); behind
+ * k accepted ones, or where an id lies outside the vocabulary (a draft that ends early), from p_i.  out i32 [n_seqs x (k + 2)]: how many
+ * were accepted, those, the drawn one, and -1 after it.
+ * The draw: weights are whole numbers round(min(p, 1) * 2^31), the variate m = floor(uniforms[k] * 2^24), and the token is the first one whose
+ * running sum exceeds floor(sum * m / 2^24): the same whatever order the sums are formed in.  Where nothing is left of max(p - q, 0) the
+ * weights are p's; where p has no positive entry either, the drawn token is -1. */
+int  rlh_verify_draft(rlh_tensor *out, const rlh_tensor *target, const rlh_tensor *draft, const rlh_tensor *drafted, const rlh_tensor *uniforms);
 
 /* ------------------------------------------------------------------------------------------------
  * Measurement aids (no reference counterpart; src/benches/benchmark.rs times the CPU/OpenCL ops with criterion).

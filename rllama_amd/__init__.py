@@ -25,9 +25,12 @@ TOK_EMB, WQ, WK, WV, WO, W1, W2, W3, ATTN_NORM, FFN_NORM, NORM, OUTPUT = range(1
 
 
 class TensorDType:
-    """TensorDType of src/tensor.rs:50-54 (the 4-bit variant is unimplemented in the reference too)."""
+    """TensorDType of src/tensor.rs:50-54 (the reference names the 4-bit variant and leaves it unimplemented; here cache planes and
+    convert() take it), and whole numbers (token ids)."""
     Float16 = 0
     Float32 = 1
+    K4BitQuantization = 2
+    Int32 = 3
 
 
 def llama_ffn_hidden(dim: int, multiple_of: int = 256) -> int:
@@ -60,6 +63,14 @@ class Context:
         hbm = C.c_uint64()
         check(self._lib.rlh_device_info(self._h, name, 256, C.byref(cus), C.byref(hbm)))
         return {"name": name.value.decode(), "compute_units": cus.value, "hbm_bytes": hbm.value}
+
+    def wait_stream(self, stream: int) -> None:
+        """Work queued here from now on waits for what is queued on the HIP stream (its handle; 0 = the default stream) by now."""
+        check(self._lib.rlh_wait_stream(self._h, stream))
+
+    def release_stream(self, stream: int) -> None:
+        """Work queued on the HIP stream from now on waits for what is queued here by now."""
+        check(self._lib.rlh_release_stream(self._h, stream))
 
     def event(self) -> "Event":
         h = C.c_void_p()
@@ -300,11 +311,13 @@ class Tensor:
     # constructors
     @staticmethod
     def from_numpy(ctx: Context, arr: np.ndarray) -> "Tensor":
-        """to_gpu_inplace (src/tensor.rs:2127-2147): uint16 arrays are f16 bits, float32 arrays are f32."""
+        """to_gpu_inplace (src/tensor.rs:2127-2147): uint16 arrays are f16 bits, float32 arrays are f32, int32 arrays are whole numbers."""
         if arr.dtype == np.uint16:
             dt = TensorDType.Float16
         elif arr.dtype == np.float32:
             dt = TensorDType.Float32
+        elif arr.dtype == np.int32:
+            dt = TensorDType.Int32
         elif arr.dtype == np.float16:
             arr, dt = arr.view(np.uint16), TensorDType.Float16
         else:
@@ -322,6 +335,14 @@ class Tensor:
         check(ctx._lib.rlh_tensor_alloc(ctx._h, rows, cols, dtype, C.byref(h)))
         return Tensor(ctx, h, rows, cols, dtype)
 
+    @staticmethod
+    def from_device(ctx: Context, device_pointer: int, rows: int, cols: int, dtype: int) -> "Tensor":
+        """A tensor over device memory that the caller owns and keeps (another library's tensor); nothing is copied.  Order the work
+        of other streams with Context.wait_stream and release_stream."""
+        h = C.c_void_p()
+        check(ctx._lib.rlh_tensor_wrap(ctx._h, device_pointer, rows, cols, dtype, C.byref(h)))
+        return Tensor(ctx, h, rows, cols, dtype)
+
     def rows(self) -> int:
         return self._rows
 
@@ -332,7 +353,13 @@ class Tensor:
         return self._dtype
 
     def to_numpy(self) -> np.ndarray:
-        """to_cpu_inplace (src/tensor.rs:2150-2166): f16 tensors come back as float16 arrays."""
+        """to_cpu_inplace (src/tensor.rs:2150-2166): f16 tensors come back as float16 arrays, whole numbers as int32; of a 4-bit tensor the
+        buffer as bytes (convert() gives the values)."""
+        if self._dtype in (TensorDType.K4BitQuantization, TensorDType.Int32):
+            shape, kind = ((self._rows, self._cols), np.int32) if self._dtype == TensorDType.Int32 else (self._rows * self._cols // 32 * 20, np.uint8)
+            out = np.empty(shape, dtype=kind)
+            check(self._lib.rlh_tensor_download(self._h, out.ctypes.data_as(C.c_void_p), self._cols, None))
+            return out
         out = np.empty((self._rows, self._cols), dtype=np.uint16 if self._dtype == TensorDType.Float16 else np.float32)
         check(self._lib.rlh_tensor_download(self._h, out.ctypes.data_as(C.c_void_p), self._cols, None))
         return out.view(np.float16) if self._dtype == TensorDType.Float16 else out
@@ -420,6 +447,46 @@ class Tensor:
         """self = qkv f16 [n x 3 dim]: RoPE, cache write and causal attention of a prompt (src/transformer.rs:704-796) -> f16 [n x dim]."""
         out = Tensor.zeros(self.ctx, self._rows, self._cols // 3, TensorDType.Float16)
         check(self._lib.rlh_attn_prefill(out._h, self._h, cache_k._h, cache_v._h, n_heads, max_seq_len))
+        return out
+
+    # long contexts and drafted tokens
+    def convert(self, dtype: Optional[int] = None, out: Optional["Tensor"] = None) -> "Tensor":
+        """The same values as f16, f32 or 4 bits."""
+        out = out or Tensor.zeros(self.ctx, self._rows, self._cols, dtype)
+        check(self._lib.rlh_convert(out._h, self._h))
+        return out
+
+    def rope_table(self, theta: float = 10000.0) -> "Tensor":
+        """self f32 [positions x head_dim] becomes the table of angles that qkv_append takes."""
+        check(self._lib.rlh_rope_table(self._h, theta))
+        return self
+
+    def qkv_append(self, q: "Tensor", cache_k: "Tensor", cache_v: "Tensor", freqs: "Tensor", n_heads: int, n_kv_heads: int, max_seq_len: int,
+                   start_pos: Sequence[int], q_norm: Optional["Tensor"] = None, k_norm: Optional["Tensor"] = None, eps: float = 1e-6, halves: bool = False,
+                   sinks: int = 0) -> "Tensor":
+        """self = qkv [rows x (n_heads + 2 n_kv_heads) head_dim]: norms per head, rotation, keys and values into the planes; queries to q."""
+        check(self._lib.rlh_qkv_append(q._h, self._h, q_norm._h if q_norm else None, k_norm._h if k_norm else None, eps, freqs._h, 1 if halves else 0,
+                                       cache_k._h, cache_v._h, n_heads, n_kv_heads, max_seq_len, sinks, (C.c_int32 * len(start_pos))(*start_pos), len(start_pos)))
+        return q
+
+    def attn_window(self, cache_k: "Tensor", cache_v: "Tensor", n_heads: int, n_kv_heads: int, max_seq_len: int, start_pos: Sequence[int], window: int = 0,
+                    sinks: int = 0, out: Optional["Tensor"] = None) -> "Tensor":
+        """self = q [rows x n_heads head_dim] after qkv_append: attention of the rows over the planes, window 0 = the whole text."""
+        out = out or self._like()
+        check(self._lib.rlh_attn_window(out._h, self._h, cache_k._h, cache_v._h, n_heads, n_kv_heads, max_seq_len, (C.c_int32 * len(start_pos))(*start_pos),
+                                        len(start_pos), window, sinks))
+        return out
+
+    def softmax_rows(self, temperature: float = 1.0, out: Optional["Tensor"] = None) -> "Tensor":
+        """self = logits [n x vocab]: probabilities f32; temperature 0 puts all of it on the first of the largest."""
+        out = out or Tensor.zeros(self.ctx, self._rows, self._cols, TensorDType.Float32)
+        check(self._lib.rlh_softmax_rows(out._h, self._h, temperature))
+        return out
+
+    def verify_draft(self, target: "Tensor", draft: Optional["Tensor"], uniforms: "Tensor", out: Optional["Tensor"] = None) -> "Tensor":
+        """self = drafted ids i32 [n_seqs x k]: i32 [n_seqs x (k + 2)] of how many are accepted, those, the token drawn behind them, -1 after it."""
+        out = out or Tensor.zeros(self.ctx, self._rows, self._cols + 2, TensorDType.Int32)
+        check(self._lib.rlh_verify_draft(out._h, target._h, draft._h if draft else None, self._h, uniforms._h))
         return out
 
     def argmax_greedy(self, temperature: float = 1.0) -> int:

@@ -95,6 +95,15 @@ SIGNATURES = {
     "rlh_attn_decode_noalloc": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     "rlh_attn_prefill": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int]),
     "rlh_argmax_greedy": (C.c_int, [_vp, C.c_float, _i32p]),
+    "rlh_tensor_wrap": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _vpp]),
+    "rlh_wait_stream": (C.c_int, [_vp, _vp]),
+    "rlh_release_stream": (C.c_int, [_vp, _vp]),
+    "rlh_convert": (C.c_int, [_vp, _vp]),
+    "rlh_rope_table": (C.c_int, [_vp, C.c_double]),
+    "rlh_qkv_append": (C.c_int, [_vp, _vp, _vp, _vp, C.c_double, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _i32p, C.c_int]),
+    "rlh_attn_window": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _i32p, C.c_int, C.c_int, C.c_int]),
+    "rlh_softmax_rows": (C.c_int, [_vp, _vp, C.c_float]),
+    "rlh_verify_draft": (C.c_int, [_vp, _vp, _vp, _vp, _vp]),
     "rlh_model_time_kernel": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _fp, C.POINTER(C.c_uint64)]),
     "rlh_time_gemv": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _fp]),
     "rlh_probe_gemv_phases": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, _fp]),

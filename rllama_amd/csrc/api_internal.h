@@ -37,6 +37,10 @@ struct OpScratch {
     int32_t *token = nullptr;      // one id
     void *gemm_ws = nullptr;       // partial sums of products cut along K and the parts of an fp32 operand (gemm_work_reserve)
     size_t gemm_ws_bytes = 0;
+    float *window_ws = nullptr;    // rlh_attn_window: partial results of sequences that are cut
+    size_t window_ws_floats = 0;
+    unsigned *window_tickets = nullptr; // ... and how many pieces have arrived; zero between launches
+    size_t window_tickets_count = 0;
 };
 constexpr int kOpMaxHeads = 1024;
 
@@ -91,8 +95,11 @@ struct rlh_tensor {
     // an operation of another context has read or written the buffer: work on that context's stream may still be queued when the tensor
     // is freed, so the buffer is not handed out again but freed, which waits for the device
     mutable std::atomic<bool> lent{false};
-    size_t esize() const { return dtype == RLH_F16 ? 2 : 4; }
+    bool wrapped = false; // the memory is the caller's
+    size_t esize() const { return dtype == RLH_F16 ? 2 : 4; } // (not of RLH_Q4, which has no whole bytes per element)
     size_t count() const { return (size_t)rows * cols; }
+    size_t bytes() const { return dtype == RLH_Q4 ? count() / 32 * 20 : count() * esize(); }
+    bool is_float() const { return dtype == RLH_F16 || dtype == RLH_F32; }
 };
 
 struct rlh_event {

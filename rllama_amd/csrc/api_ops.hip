@@ -4,6 +4,7 @@
 #include "api_internal.h"
 #include "split3_plan.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -15,7 +16,8 @@ using namespace rlh;
 // op level
 // ------------------------------------------------------------------------------------------------
 extern "C" int rlh_tensor_alloc(rlh_ctx *ctx, int rows, int cols, int dtype, rlh_tensor **out) {
-    if (!ctx || !out || rows <= 0 || cols <= 0 || (dtype != RLH_F16 && dtype != RLH_F32)) return fail(RLH_ERR_INVALID, "rlh_tensor_alloc: bad argument");
+    if (!ctx || !out || rows <= 0 || cols <= 0 || dtype < RLH_F16 || dtype > RLH_I32) return fail(RLH_ERR_INVALID, "rlh_tensor_alloc: bad argument");
+    if (dtype == RLH_Q4 && cols % 32 != 0) return fail(RLH_ERR_INVALID, "rlh_tensor_alloc: %d columns of 4 bits: a multiple of 32 is needed", cols);
     *out = nullptr;
     CtxLock lock(ctx);
     rlh_tensor *t = new rlh_tensor();
@@ -23,7 +25,7 @@ extern "C" int rlh_tensor_alloc(rlh_ctx *ctx, int rows, int cols, int dtype, rlh
     t->rows = rows;
     t->cols = cols;
     t->dtype = dtype;
-    const size_t bytes = t->count() * t->esize();
+    const size_t bytes = t->bytes();
     t->p = ctx->pool.take(bytes, &t->capacity);
     hipError_t e = hipSuccess;
     if (!t->p) {
@@ -42,6 +44,7 @@ extern "C" int rlh_tensor_alloc(rlh_ctx *ctx, int rows, int cols, int dtype, rlh
 
 extern "C" int rlh_tensor_upload(rlh_ctx *ctx, const void *host, int rows, int cols, int cols_capacity, int dtype, rlh_tensor **out) {
     if (!host || cols_capacity < cols) return fail(RLH_ERR_INVALID, "rlh_tensor_upload: bad argument");
+    if (dtype == RLH_Q4 && cols_capacity != cols) return fail(RLH_ERR_UNSUPPORTED, "rlh_tensor_upload: a 4-bit tensor travels as its whole buffer (cols_capacity = cols)");
     int rc = rlh_tensor_alloc(ctx, rows, cols, dtype, out);
     if (rc != RLH_OK) return rc;
     CtxLock lock(ctx);
@@ -49,7 +52,7 @@ extern "C" int rlh_tensor_upload(rlh_ctx *ctx, const void *host, int rows, int c
     const size_t es = t->esize();
     // (rows without padding are one linear copy, which the runtime moves several times faster from pageable memory)
     hipError_t e = cols == cols_capacity
-                       ? hipMemcpyAsync(t->p, host, t->count() * es, hipMemcpyHostToDevice, ctx->stream)
+                       ? hipMemcpyAsync(t->p, host, t->bytes(), hipMemcpyHostToDevice, ctx->stream)
                        : hipMemcpy2DAsync(t->p, (size_t)cols * es, host, (size_t)cols_capacity * es, (size_t)cols * es, (size_t)rows, hipMemcpyHostToDevice, ctx->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream); // the host buffer is the caller's again on return
     if (e != hipSuccess) {
@@ -62,13 +65,14 @@ extern "C" int rlh_tensor_upload(rlh_ctx *ctx, const void *host, int rows, int c
 
 extern "C" int rlh_tensor_download(rlh_tensor *t, void *host, int cols_capacity, rlh_event **ev) {
     if (!t || !host || cols_capacity < t->cols) return fail(RLH_ERR_INVALID, "rlh_tensor_download: bad argument");
+    if (t->dtype == RLH_Q4 && cols_capacity != t->cols) return fail(RLH_ERR_UNSUPPORTED, "rlh_tensor_download: a 4-bit tensor travels as its whole buffer (cols_capacity = cols)");
     CtxLock lock(t->ctx);
     const size_t es = t->esize();
     if (t->cols == cols_capacity && !ev) { // (with an event the caller's memory is written after this call returns)
-        HIP_TRY(stage_download(t->ctx, host, t->p, t->count() * es));
+        HIP_TRY(stage_download(t->ctx, host, t->p, t->bytes()));
         return RLH_OK;
     }
-    if (t->cols == cols_capacity) HIP_TRY(hipMemcpyAsync(host, t->p, t->count() * es, hipMemcpyDeviceToHost, t->ctx->stream));
+    if (t->cols == cols_capacity) HIP_TRY(hipMemcpyAsync(host, t->p, t->bytes(), hipMemcpyDeviceToHost, t->ctx->stream));
     else
         HIP_TRY(hipMemcpy2DAsync(host, (size_t)cols_capacity * es, t->p, (size_t)t->cols * es, (size_t)t->cols * es, (size_t)t->rows, hipMemcpyDeviceToHost,
                                  t->ctx->stream));
@@ -85,7 +89,9 @@ extern "C" void rlh_tensor_free(rlh_tensor *t) {
     if (!t) return;
     CtxLock lock(t->ctx);
     TensorPool &pool = t->ctx->pool;
-    if (t->p && TensorPool::keeps(t->capacity) && !t->lent.load(std::memory_order_relaxed)) {
+    if (t->wrapped) {
+        (void)hipStreamSynchronize(t->ctx->stream); // the memory is the caller's again
+    } else if (t->p && TensorPool::keeps(t->capacity) && !t->lent.load(std::memory_order_relaxed)) {
         if (!pool.room(t->capacity)) {
             (void)hipStreamSynchronize(t->ctx->stream);
             while (!pool.room(t->capacity)) (void)hipFree(pool.drop());
@@ -146,12 +152,17 @@ extern "C" void rlh_event_free(rlh_event *ev) {
 
 static int same_shape(const rlh_tensor *a, const rlh_tensor *b) { return a->rows == b->rows && a->cols == b->cols && a->dtype == b->dtype; }
 
+// The ops below read f16 or f32 elements.
+#define FLOATS_ONLY(name, t) \
+    if (!(t)->is_float()) return fail(RLH_ERR_UNSUPPORTED, name ": f16 and f32 tensors only")
+
 extern "C" int rlh_copy_inplace(rlh_tensor *dst, const rlh_tensor *src) {
     if (!dst || !src || !same_shape(dst, src)) return fail(RLH_ERR_INVALID, "rlh_copy_inplace: shape/dtype mismatch");
     CtxLock lock(dst->ctx);
     lend(dst->ctx, {src});
     // a plain copy kernel (the reference's copy_inplace is a kernel too); also the calibration point for HBM counters
-    HIP_TRY(launch_convert(dst->p, dst->dtype == RLH_F16, src->p, src->dtype == RLH_F16, dst->count(), dst->ctx->stream));
+    if (!dst->is_float()) HIP_TRY(launch_convert(dst->p, 0, src->p, 0, dst->bytes() / 4, dst->ctx->stream)); // as 32-bit words
+    else HIP_TRY(launch_convert(dst->p, dst->dtype == RLH_F16, src->p, src->dtype == RLH_F16, dst->count(), dst->ctx->stream));
     return RLH_OK;
 }
 
@@ -159,6 +170,7 @@ extern "C" int rlh_transpose_from(rlh_tensor *dst, const rlh_tensor *src) {
     if (!dst || !src || dst->rows != src->cols || dst->cols != src->rows || dst->dtype != src->dtype) {
         return fail(RLH_ERR_INVALID, "rlh_transpose_from: shape/dtype mismatch");
     }
+    FLOATS_ONLY("rlh_transpose_from", src);
     CtxLock lock(dst->ctx);
     lend(dst->ctx, {src});
     HIP_TRY(launch_transpose(dst->p, src->p, src->rows, src->cols, src->dtype == RLH_F16, dst->ctx->stream));
@@ -167,6 +179,7 @@ extern "C" int rlh_transpose_from(rlh_tensor *dst, const rlh_tensor *src) {
 
 extern "C" int rlh_hadamard_product_inplace(rlh_tensor *dst, const rlh_tensor *src) {
     if (!dst || !src || !same_shape(dst, src)) return fail(RLH_ERR_INVALID, "rlh_hadamard_product_inplace: shape/dtype mismatch");
+    FLOATS_ONLY("rlh_hadamard_product_inplace", dst);
     CtxLock lock(dst->ctx);
     lend(dst->ctx, {src});
     HIP_TRY(launch_hadamard(dst->p, src->p, dst->count(), dst->dtype == RLH_F16, dst->ctx->stream));
@@ -175,6 +188,7 @@ extern "C" int rlh_hadamard_product_inplace(rlh_tensor *dst, const rlh_tensor *s
 
 extern "C" int rlh_silu_inplace(rlh_tensor *t) {
     if (!t) return fail(RLH_ERR_INVALID, "rlh_silu_inplace: NULL tensor");
+    FLOATS_ONLY("rlh_silu_inplace", t);
     CtxLock lock(t->ctx);
     HIP_TRY(launch_silu(t->p, t->count(), t->dtype == RLH_F16, t->ctx->stream));
     return RLH_OK;
@@ -184,6 +198,7 @@ extern "C" int rlh_gemv(rlh_tensor *y, const rlh_tensor *w, const rlh_tensor *x,
     if (!y || !w || !x) return fail(RLH_ERR_INVALID, "rlh_gemv: NULL argument");
     if (x->dtype != RLH_F32 || y->dtype != RLH_F32) return fail(RLH_ERR_INVALID, "rlh_gemv: x and y must be f32");
     if (x->rows != 1 || y->rows != 1 || x->cols != w->cols || y->cols != w->rows) return fail(RLH_ERR_INVALID, "rlh_gemv: shape mismatch");
+    FLOATS_ONLY("rlh_gemv", w);
     const int vec = w->dtype == RLH_F16 ? 8 : 4;
     if (w->cols % vec != 0) return fail(RLH_ERR_UNSUPPORTED, "rlh_gemv: k must be a multiple of %d", vec);
     CtxLock lock(y->ctx);
@@ -209,6 +224,7 @@ extern "C" int rlh_matrix_mul_inplace_transposed(rlh_tensor *dst, const rlh_tens
     if (src->dtype != other->dtype || dst->dtype != src->dtype) return fail(RLH_ERR_INVALID, "Invalid matrix multiplication, different dtypes");
     if (dst->rows != src->rows) return fail(RLH_ERR_INVALID, "Invalid matrix multiplication, different number of rows");
     if (dst->cols != other->rows) return fail(RLH_ERR_INVALID, "Invalid matrix multiplication, different number of cols");
+    FLOATS_ONLY("rlh_matrix_mul_inplace_transposed", src);
     const int f16 = src->dtype == RLH_F16;
     if (src->cols % (f16 ? 8 : 4) != 0) return fail(RLH_ERR_UNSUPPORTED, "rlh_matrix_mul_inplace_transposed: k must be a multiple of %d", f16 ? 8 : 4);
     CtxLock lock(dst->ctx);
@@ -308,6 +324,7 @@ extern "C" int rlh_add(rlh_tensor *dst, const rlh_tensor *a, const rlh_tensor *b
 
 extern "C" int rlh_silu_mul(rlh_tensor *dst, const rlh_tensor *gate, const rlh_tensor *up) {
     if (!dst || !gate || !up || !same_shape(dst, gate) || !same_shape(dst, up)) return fail(RLH_ERR_INVALID, "rlh_silu_mul: shape/dtype mismatch");
+    FLOATS_ONLY("rlh_silu_mul", dst);
     CtxLock lock(dst->ctx);
     lend(dst->ctx, {gate, up});
     if (dst->dtype == RLH_F16) HIP_TRY(launch_silu_mul_f16(gate->p, up->p, dst->p, dst->count(), dst->ctx->stream));
@@ -358,11 +375,11 @@ extern "C" int rlh_ffn_gate(rlh_tensor *dst, const rlh_tensor *x, const rlh_tens
 }
 
 // (cos, sin) of compute_freqs_cis (transformer.rs:858-885) for positions first .. first + n - 1, as f32 like :836-837
-static std::vector<float2> rope_table(int head_dim, int first, int n) {
+static std::vector<float2> rope_table(int head_dim, int first, int n, double theta = 10000.0) {
     std::vector<float2> tab((size_t)n * (head_dim / 2));
     for (int i = 0; i < n; i++) {
         for (int j = 0; j < head_dim / 2; j++) {
-            const double freq = 1.0 / std::pow(10000.0, (double)j * 2.0 / (double)head_dim);
+            const double freq = 1.0 / std::pow(theta, (double)j * 2.0 / (double)head_dim);
             const double ang = freq * (double)(first + i);
             tab[(size_t)i * (head_dim / 2) + j] = make_float2((float)std::cos(ang), (float)std::sin(ang));
         }
@@ -370,9 +387,23 @@ static std::vector<float2> rope_table(int head_dim, int first, int n) {
     return tab;
 }
 
+extern "C" int rlh_rope_table(rlh_tensor *freqs, double theta) {
+    if (!freqs || freqs->dtype != RLH_F32 || freqs->cols % 2 != 0) return fail(RLH_ERR_INVALID, "rlh_rope_table: an f32 tensor [positions x head_dim], head_dim even, is needed");
+    if (!(theta > 0.0) || std::isinf(theta)) return fail(RLH_ERR_INVALID, "rlh_rope_table: theta must be positive");
+    CtxLock lock(freqs->ctx);
+    constexpr int kChunk = 4096; // positions formed and sent at a time
+    for (int first = 0; first < freqs->rows; first += kChunk) {
+        const int n = std::min(kChunk, freqs->rows - first);
+        const std::vector<float2> tab = rope_table(freqs->cols, first, n, theta);
+        HIP_TRY(hipMemcpyAsync((float *)freqs->p + (size_t)first * freqs->cols, tab.data(), tab.size() * sizeof(float2), hipMemcpyHostToDevice, freqs->ctx->stream));
+        HIP_TRY(hipStreamSynchronize(freqs->ctx->stream)); // the host table goes out of scope
+    }
+    return RLH_OK;
+}
+
 // Checks one layer's pair of cache planes [n_heads * max_seq_len x head_dim] and returns head_dim (0 on a mismatch).
 static int cache_planes_head_dim(const rlh_tensor *ck, const rlh_tensor *cv, int n_heads, int max_seq_len) {
-    if (!ck || !cv || n_heads <= 0 || max_seq_len <= 0 || !same_shape(ck, cv)) return 0;
+    if (!ck || !cv || n_heads <= 0 || max_seq_len <= 0 || !same_shape(ck, cv) || !ck->is_float()) return 0;
     if ((int64_t)ck->rows != (int64_t)n_heads * max_seq_len) return 0;
     const int hd = ck->cols;
     return (hd == 16 || hd == 32 || hd == 64 || hd == 128) ? hd : 0;
@@ -494,7 +525,7 @@ hipError_t gemm_work_reserve(rlh_ctx *ctx, void **p, size_t *bytes, size_t need)
 void ops_release(rlh_ctx *ctx) {
     pool_release(ctx);
     OpScratch &o = ctx->ops;
-    void *all[] = {o.state, o.attn_ws, o.tickets, o.token, o.gemm_ws};
+    void *all[] = {o.state, o.attn_ws, o.tickets, o.token, o.gemm_ws, o.window_ws, o.window_tickets};
     for (void *b : all)
         if (b) (void)hipFree(b);
     o = OpScratch();

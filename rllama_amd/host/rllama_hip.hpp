@@ -34,7 +34,7 @@ inline void check(int rc) {
     if (rc != RLH_OK) throw Error(rc, rlh_last_error());
 }
 
-enum class TensorDType { Float16 = RLH_F16, Float32 = RLH_F32 }; // src/tensor.rs:50-54
+enum class TensorDType { Float16 = RLH_F16, Float32 = RLH_F32, K4BitQuantization = RLH_Q4, Int32 = RLH_I32 }; // src/tensor.rs:50-54
 
 // OpenCL::new(verbose, nth_device) (src/tensor_opencl_support.rs:86)
 class OpenCL {

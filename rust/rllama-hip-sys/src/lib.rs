@@ -41,6 +41,8 @@ pub const RLH_ERR_UNSUPPORTED: c_int = 6;
 // rlh_dtype
 pub const RLH_F16: c_int = 0;
 pub const RLH_F32: c_int = 1;
+pub const RLH_Q4: c_int = 2;
+pub const RLH_I32: c_int = 3;
 
 // rlh_tensor_kind
 pub const RLH_TOK_EMB: c_int = 0;
@@ -134,6 +136,15 @@ extern "C" {
     pub fn rlh_attn_decode_noalloc(out: *mut rlh_tensor, q: *const rlh_tensor, cache_k: *const rlh_tensor, cache_v: *const rlh_tensor, n_heads: c_int, max_seq_len: c_int, T: c_int, n_splits: c_int, round_out: c_int) -> c_int;
     pub fn rlh_attn_prefill(out: *mut rlh_tensor, qkv: *const rlh_tensor, cache_k: *mut rlh_tensor, cache_v: *mut rlh_tensor, n_heads: c_int, max_seq_len: c_int) -> c_int;
     pub fn rlh_argmax_greedy(logits: *const rlh_tensor, temperature: c_float, token: *mut i32) -> c_int;
+    pub fn rlh_tensor_wrap(ctx: *mut rlh_ctx, device_memory: *mut c_void, rows: c_int, cols: c_int, dtype: c_int, out: *mut *mut rlh_tensor) -> c_int;
+    pub fn rlh_wait_stream(ctx: *mut rlh_ctx, stream: *mut c_void) -> c_int;
+    pub fn rlh_release_stream(ctx: *mut rlh_ctx, stream: *mut c_void) -> c_int;
+    pub fn rlh_convert(dst: *mut rlh_tensor, src: *const rlh_tensor) -> c_int;
+    pub fn rlh_rope_table(freqs: *mut rlh_tensor, theta: c_double) -> c_int;
+    pub fn rlh_qkv_append(q: *mut rlh_tensor, qkv: *const rlh_tensor, q_norm: *const rlh_tensor, k_norm: *const rlh_tensor, eps: c_double, freqs: *const rlh_tensor, halves: c_int, cache_k: *mut rlh_tensor, cache_v: *mut rlh_tensor, n_heads: c_int, n_kv_heads: c_int, max_seq_len: c_int, sinks: c_int, start_pos: *const i32, n_seqs: c_int) -> c_int;
+    pub fn rlh_attn_window(out: *mut rlh_tensor, q: *const rlh_tensor, cache_k: *const rlh_tensor, cache_v: *const rlh_tensor, n_heads: c_int, n_kv_heads: c_int, max_seq_len: c_int, start_pos: *const i32, n_seqs: c_int, window: c_int, sinks: c_int) -> c_int;
+    pub fn rlh_softmax_rows(probs: *mut rlh_tensor, logits: *const rlh_tensor, temperature: c_float) -> c_int;
+    pub fn rlh_verify_draft(out: *mut rlh_tensor, target: *const rlh_tensor, draft: *const rlh_tensor, drafted: *const rlh_tensor, uniforms: *const rlh_tensor) -> c_int;
     pub fn rlh_model_time_kernel(model: *mut rlh_model, caches: *mut rlh_caches, which: c_int, T: c_int, iters: c_int, us_per_launch: *mut c_float, bytes_per_launch: *mut u64) -> c_int;
     pub fn rlh_time_gemv(ctx: *mut rlh_ctx, rows: c_int, k: c_int, w_dtype: c_int, round_x: c_int, round_y: c_int, n_buffers: c_int, iters: c_int, us_per_launch: *mut c_float) -> c_int;
     pub fn rlh_probe_gemv_phases(ctx: *mut rlh_ctx, rows: c_int, k: c_int, n_buffers: c_int, launches: c_int, out_us: *mut c_float) -> c_int;

@@ -39,8 +39,6 @@ struct OpScratch {
     size_t gemm_ws_bytes = 0;
     float *window_ws = nullptr;    // rlh_attn_window: partial results of sequences that are cut
     size_t window_ws_floats = 0;
-    unsigned *window_tickets = nullptr; // ... and how many pieces have arrived; zero between launches
-    size_t window_tickets_count = 0;
 };
 constexpr int kOpMaxHeads = 1024;
 

@@ -143,30 +143,17 @@ extern "C" int rlh_qkv_append(rlh_tensor *q, const rlh_tensor *qkv, const rlh_te
 }
 
 // Work memory of rlh_attn_window; growing it waits for the context's stream.
-static hipError_t window_work_reserve(rlh_ctx *ctx, size_t floats, size_t tickets) {
+static hipError_t window_work_reserve(rlh_ctx *ctx, size_t floats) {
     OpScratch &o = ctx->ops;
-    hipError_t e = hipSuccess;
-    if (floats > o.window_ws_floats) {
-        if (o.window_ws) {
-            (void)hipStreamSynchronize(ctx->stream);
-            (void)hipFree(o.window_ws);
-            o.window_ws = nullptr;
-            o.window_ws_floats = 0;
-        }
-        if ((e = device_alloc(ctx, (void **)&o.window_ws, floats * sizeof(float))) != hipSuccess) return e;
-        o.window_ws_floats = floats;
+    if (floats <= o.window_ws_floats) return hipSuccess;
+    if (o.window_ws) {
+        (void)hipStreamSynchronize(ctx->stream);
+        (void)hipFree(o.window_ws);
+        o.window_ws = nullptr;
+        o.window_ws_floats = 0;
     }
-    if (tickets > o.window_tickets_count) {
-        if (o.window_tickets) {
-            (void)hipStreamSynchronize(ctx->stream);
-            (void)hipFree(o.window_tickets);
-            o.window_tickets = nullptr;
-            o.window_tickets_count = 0;
-        }
-        if ((e = device_alloc(ctx, (void **)&o.window_tickets, tickets * sizeof(unsigned))) != hipSuccess) return e;
-        if ((e = launch_fill_u32(o.window_tickets, tickets, 0u, ctx->stream)) != hipSuccess) return e;
-        o.window_tickets_count = tickets;
-    }
+    const hipError_t e = device_alloc(ctx, (void **)&o.window_ws, floats * sizeof(float));
+    if (e == hipSuccess) o.window_ws_floats = floats;
     return e;
 }
 
@@ -204,11 +191,9 @@ extern "C" int rlh_attn_window(rlh_tensor *out, const rlh_tensor *q, const rlh_t
     p.window = window;
     p.sinks = sinks;
     for (int b = 0; b < n_seqs; b++) p.start[b] = start_pos[b];
-    size_t floats = 0, tickets = 0;
     const int cus = ctx->prop.multiProcessorCount;
-    attn_window_work(p, cus, &floats, &tickets);
-    HIP_TRY(window_work_reserve(ctx, floats, tickets));
-    HIP_TRY(launch_attn_window(p, cus, ctx->ops.window_ws, ctx->ops.window_tickets, ctx->stream));
+    HIP_TRY(window_work_reserve(ctx, attn_window_work_floats(p, cus)));
+    HIP_TRY(launch_attn_window(p, cus, ctx->ops.window_ws, ctx->stream));
     return RLH_OK;
 }
 

@@ -525,7 +525,7 @@ hipError_t gemm_work_reserve(rlh_ctx *ctx, void **p, size_t *bytes, size_t need)
 void ops_release(rlh_ctx *ctx) {
     pool_release(ctx);
     OpScratch &o = ctx->ops;
-    void *all[] = {o.state, o.attn_ws, o.tickets, o.token, o.gemm_ws, o.window_ws, o.window_tickets};
+    void *all[] = {o.state, o.attn_ws, o.tickets, o.token, o.gemm_ws, o.window_ws};
     for (void *b : all)
         if (b) (void)hipFree(b);
     o = OpScratch();

@@ -18,8 +18,7 @@
 // unit in the eleventh bit, and neither adds up over a text).  32 bits: everything in f32 through v_mfma_f32_16x16x4_f32; also taken where f16
 // queries meet an f32 cache, whose values f16 may not hold.
 //
-// A text is cut into pieces when there are few rows: every workgroup leaves its (m, sum, O) in work memory and the last one to
-// arrive joins them, in the order of the pieces.
+// A text is cut into pieces when there are few rows: every workgroup leaves its (m, sum, O) in work memory and a second launch joins them.
 #include "kernels.h"
 #include "longctx.h"
 
@@ -30,21 +29,28 @@ namespace rlh {
 constexpr int kAwWaves = 8;
 constexpr int kAwThreads = kAwWaves * kWave;
 constexpr int kAwRows = 16; // rows per workgroup
+constexpr int kAwMaxPieces = 64;
 
-// What one workgroup's rows look at: steps of kStep positions, first the tokens that stay visible, then the window.
+// What one workgroup's rows look at, in steps of kStep positions that lie side by side in the cache: the first tokens that stay visible,
+// the window up to the end of the ring, the rest of the window from the ring's beginning.
 struct Span {
-    int first_end;   // positions 0 .. first_end - 1 are looked at through `sinks`
-    int low, last;   // and low .. last
-    int first_steps, steps;
+    int first_end;  // positions 0 .. first_end - 1 are looked at through `sinks`
+    int low, last;  // and low .. last
+    int row, turn;  // row of position low; the first position behind the ring's end (last + 1 if none is)
+    int steps0, steps1, steps;
 };
 template <int kStep>
-__host__ __device__ inline Span span_of(int p0, int p1, int window, int sinks) { // positions of the first and the last row that is no padding
+__device__ inline Span span_of(int p0, int p1, int window, int sinks, int max_seq_len) { // positions of the first and the last row that is no padding
     Span s;
-    s.low = window > 0 ? (p0 - window + 1 > 0 ? p0 - window + 1 : 0) : 0;
+    s.low = window > 0 ? max(0, p0 - window + 1) : 0;
     s.last = p1;
-    s.first_end = sinks < s.low ? sinks : s.low;
-    s.first_steps = (s.first_end + kStep - 1) / kStep;
-    s.steps = s.first_steps + (s.last - s.low + kStep) / kStep;
+    s.first_end = min(sinks, s.low);
+    s.row = cache_row(s.low, max_seq_len, sinks);
+    const int room = max_seq_len - s.row; // (all of low .. last fit the ring, so they pass its end once at most)
+    s.turn = s.last - s.low < room ? s.last + 1 : s.low + room;
+    s.steps0 = (s.first_end + kStep - 1) / kStep;
+    s.steps1 = s.steps0 + (s.turn - s.low + kStep - 1) / kStep;
+    s.steps = s.steps1 + (s.last + 1 - s.turn + kStep - 1) / kStep;
     return s;
 }
 
@@ -57,21 +63,65 @@ __device__ __forceinline__ float col_sum(float v) {
     return v + __shfl_xor(v, 32, kWave);
 }
 
+// Masks and exponent bits of the conversion below, kept in registers: masking and setting the exponent are one instruction then, which takes
+// no literals and one scalar register at most.
+struct Q4Bits {
+    uint32_t even = 0x000f000fu, odd = 0x00f000f0u, exponent = 0x64006400u;
+    __device__ Q4Bits() {
+        asm("" : "+s"(even));
+        asm("" : "+s"(odd));
+        asm("" : "+v"(exponent));
+    }
+};
 // eight codes of a word as f16 numbers lowest + code * scale: pairs (0, 4), (1, 5), (2, 6), (3, 7).  1024 + c is the f16 number with c in its
 // last bits (0x6400 | c); 1024 + 16 c likewise, which saves half of the shifts.  The difference to 1024 is exact, the multiply-add rounds once.
-__device__ __forceinline__ void q4_pairs_f16(uint32_t w, half2_t scale, half2_t scale16, half2_t low, half2_t (&out)[4]) {
+__device__ __forceinline__ void q4_pairs_f16(const Q4Bits &bits, uint32_t w, half2_t scale, half2_t scale16, half2_t low, half2_t (&out)[4]) {
     const half2_t k1024 = {(half_t)1024.0f, (half_t)1024.0f};
 #pragma unroll
     for (int s = 0; s < 2; s++) {
         const uint32_t x = w >> (8 * s);
-        const half2_t a = __builtin_bit_cast(half2_t, (x & 0x000f000fu) | 0x64006400u) - k1024;
-        const half2_t b = __builtin_bit_cast(half2_t, (x & 0x00f000f0u) | 0x64006400u) - k1024;
+        const half2_t a = __builtin_bit_cast(half2_t, (x & bits.even) | bits.exponent) - k1024;
+        const half2_t b = __builtin_bit_cast(half2_t, (x & bits.odd) | bits.exponent) - k1024;
         out[2 * s] = __builtin_elementwise_fma(a, scale, low);
         out[2 * s + 1] = __builtin_elementwise_fma(b, scale16, low);
     }
 }
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
 constexpr uint32_t kLoHalves = 0x05040100u, kHiHalves = 0x07060302u; // of (first, second): perm(second, first, .)
+
+// Loads through a buffer descriptor of the step's rows: offsets per lane that never change, one scalar base per step, and rows past the step's
+// last one read as zeros by the hardware's bounds check, whatever memory holds there.
+typedef __amdgpu_buffer_rsrc_t buffer_t;
+__device__ __forceinline__ buffer_t buffer_of(const void *data, size_t offset, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(reinterpret_cast<const char *>(data)) + offset, 0, bytes, 0x00027000);
+}
+template <int kWords>
+__device__ __forceinline__ void load_words(uint32_t (&dst)[kWords], buffer_t src, int offset) {
+    if constexpr (kWords % 4 == 0) {
+#pragma unroll
+        for (int w = 0; w < kWords; w += 4) {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b128(src, offset + 4 * w, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) dst[w + i] = x[i];
+        }
+    } else if constexpr (kWords == 2) {
+        const auto x = __builtin_amdgcn_raw_buffer_load_b64(src, offset, 0, 0);
+        dst[0] = x[0];
+        dst[1] = x[1];
+    } else {
+        static_assert(kWords == 1, "1, 2 or a multiple of 4");
+        dst[0] = __builtin_amdgcn_raw_buffer_load_b32(src, offset, 0, 0);
+    }
+}
+// the codes of kN elements (2, 4 or 8)
+template <int kN>
+__device__ __forceinline__ uint32_t load_codes(buffer_t src, int offset) {
+    if constexpr (kN == 8) return __builtin_amdgcn_raw_buffer_load_b32(src, offset, 0, 0);
+    else if constexpr (kN == 4) return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(src, offset, 0, 0);
+    else return (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(src, offset, 0, 0);
+}
+template <typename CT>
+constexpr int kElementBits = std::is_same_v<CT, Quant4> ? 4 : (int)sizeof(CT) * 8;
 
 // The operands of one step, and the two products on them.  AC: half_t or float, the arithmetic.
 template <typename AC, typename CT, int HD>
@@ -85,7 +135,10 @@ struct Step<half_t, CT, HD> {
     static constexpr int kKs = HD / 32;         // MFMAs per score tile
     static constexpr int kDims = HD / 16;       // neighbouring dims of V per lane = tiles of O^T
     static constexpr bool kQ4 = std::is_same_v<CT, Quant4>;
-    half8_t q[kKs];
+    static constexpr int kBits = kElementBits<CT>;
+    struct Queries {
+        half8_t q[kKs];
+    };
     uint32_t k[kTiles][kQ4 ? HD / 32 : HD / 8 /* words: a quarter of a row */];
     uint32_t kp[kTiles];
     uint32_t v[8][kQ4 ? 1 : kDims / 2];
@@ -93,61 +146,35 @@ struct Step<half_t, CT, HD> {
 
     // lane (row = l % 16, h): dims h * HD / 4 + 8 c .. + 7, in the order of the codes of a word where K has 4 bits
     template <typename QT>
-    __device__ void load_q(const QT *row, int h) {
+    __device__ static void load_q(Queries &to, const QT *row, int h) {
 #pragma unroll
         for (int c = 0; c < kKs; c++) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int d = kQ4 ? (i >> 1) + 4 * (i & 1) : i;
-                q[c][i] = (half_t)(float)row[h * (HD / 4) + 8 * c + d];
+                to.q[c][i] = (half_t)(float)row[h * (HD / 4) + 8 * c + d];
             }
         }
     }
-    template <int kWords>
-    __device__ static void load_words(uint32_t (&dst)[kWords], const void *src) {
-        if constexpr (kWords % 4 == 0) {
-#pragma unroll
-            for (int w = 0; w < kWords; w += 4) {
-                const uint4_t x = *reinterpret_cast<const uint4_t *>(reinterpret_cast<const uint32_t *>(src) + w);
-#pragma unroll
-                for (int i = 0; i < 4; i++) dst[w + i] = x[i];
-            }
-        } else if constexpr (kWords == 2) {
-            const uint2 x = *reinterpret_cast<const uint2 *>(src);
-            dst[0] = x.x;
-            dst[1] = x.y;
-        } else {
-            dst[0] = *reinterpret_cast<const uint32_t *>(src);
-        }
-    }
-    // row_of(j): the plane's row of the step's position j
-    template <typename F>
-    __device__ void load(const PlaneRef &ck, const PlaneRef &cv, int lane, F row_of) {
+    __device__ void load(buffer_t ck, buffer_t ckp, buffer_t cv, buffer_t cvp, int lane) {
         const int m = lane & 15, h = lane >> 4;
 #pragma unroll
         for (int t = 0; t < kTiles; t++) {
-            const size_t at = (size_t)row_of(16 * t + m) * HD + h * (HD / 4);
-            if constexpr (kQ4) {
-                load_words(k[t], reinterpret_cast<const char *>(ck.data) + at / 2);
-                kp[t] = ck.pairs[at / 32];
-            } else {
-                load_words(k[t], reinterpret_cast<const char *>(ck.data) + at * 2);
-            }
+            load_words(k[t], ck, (m * HD + h * (HD / 4)) * kBits / 8 + 16 * t * HD * kBits / 8);
+            if constexpr (kQ4) kp[t] = __builtin_amdgcn_raw_buffer_load_b32(ckp, (m * HD + h * (HD / 4)) / 32 * 4 + 16 * t * HD / 8, 0, 0);
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const size_t at = (size_t)row_of(j < 4 ? 4 * h + j : 12 + 4 * h + j) * HD + m * kDims;
+            const int row = j < 4 ? j : 12 + j; // + 4 h
             if constexpr (kQ4) {
-                v[j][0] = kDims == 8   ? reinterpret_cast<const uint32_t *>(cv.data)[at / 8]
-                          : kDims == 4 ? (uint32_t)reinterpret_cast<const uint16_t *>(cv.data)[at / 4]
-                                       : (uint32_t)reinterpret_cast<const uint8_t *>(cv.data)[at / 2];
-                vp[j] = cv.pairs[at / 32];
+                v[j][0] = load_codes<kDims>(cv, (4 * h * HD + m * kDims) / 2 + row * HD / 2);
+                vp[j] = __builtin_amdgcn_raw_buffer_load_b32(cvp, (4 * h * HD + m * kDims) / 32 * 4 + row * HD / 8, 0, 0);
             } else {
-                load_words(v[j], reinterpret_cast<const char *>(cv.data) + at * 2);
+                load_words(v[j], cv, (4 * h * HD + m * kDims) * 2 + row * HD * 2);
             }
         }
     }
-    __device__ void scores(float4_t (&s)[kTiles]) const {
+    __device__ void scores(const Queries &of, const Q4Bits &bits, float4_t (&s)[kTiles]) const {
 #pragma unroll
         for (int t = 0; t < kTiles; t++) {
             s[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -162,7 +189,7 @@ struct Step<half_t, CT, HD> {
                 half8_t a;
                 if constexpr (kQ4) {
                     half2_t x[4];
-                    q4_pairs_f16(k[t][c], scale, scale16, low, x);
+                    q4_pairs_f16(bits, k[t][c], scale, scale16, low, x);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         a[2 * i] = x[i][0];
@@ -171,12 +198,12 @@ struct Step<half_t, CT, HD> {
                 } else {
                     a = __builtin_bit_cast(half8_t, uint4_t{k[t][4 * c], k[t][4 * c + 1], k[t][4 * c + 2], k[t][4 * c + 3]});
                 }
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[c], s[t], 0, 0, 0);
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, of.q[c], s[t], 0, 0, 0);
             }
         }
     }
     // w[t][i]: weights of positions 16 t + 4 h + i
-    __device__ void values(const float4_t (&w)[kTiles], float4_t (&o)[kDims]) const {
+    __device__ void values(const float4_t (&w)[kTiles], const Q4Bits &bits, float4_t (&o)[kDims]) const {
         half8_t b;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -194,7 +221,7 @@ struct Step<half_t, CT, HD> {
 #pragma unroll
                 for (int part = 0; part < (kDims + 3) / 4; part++) {
                     half2_t y[4];
-                    q4_pairs_f16(perm(v[j + 1][0], v[j][0], part ? kHiHalves : kLoHalves), scale, scale16, low, y);
+                    q4_pairs_f16(bits, perm(v[j + 1][0], v[j][0], part ? kHiHalves : kLoHalves), scale, scale16, low, y);
 #pragma unroll
                     for (int i = 0; i < (kDims < 4 ? kDims : 4); i++) x[4 * part + i][j / 2] = __builtin_bit_cast(uint32_t, y[i]);
                 }
@@ -234,63 +261,58 @@ struct Step<float, CT, HD> {
     static constexpr int kPositions = 16;
     static constexpr int kTiles = 1;
     static constexpr int kDims = HD / 16;
-    float q[HD / 4], k[HD / 4], v[4][kDims];
+    static constexpr bool kQ4 = std::is_same_v<CT, Quant4>;
+    static constexpr int kPerWord = kQ4 ? 8 : std::is_same_v<CT, half_t> ? 2 : 1;
+    static constexpr int kKWords = HD / 4 / kPerWord, kVWords = kQ4 ? 1 : kDims / kPerWord;
+    struct Queries {
+        float q[HD / 4];
+    };
+    // as the cache holds them, so that a load need not have arrived before the next one is issued
+    uint32_t k[kKWords], kp, v[4][kVWords], vp[4];
 
     template <typename QT>
-    __device__ void load_q(const QT *row, int h) {
+    __device__ static void load_q(Queries &to, const QT *row, int h) {
 #pragma unroll
-        for (int i = 0; i < HD / 4; i++) q[i] = (float)row[h * (HD / 4) + i];
+        for (int i = 0; i < HD / 4; i++) to.q[i] = (float)row[h * (HD / 4) + i];
     }
-    template <int kN>
-    __device__ static void load_values(float (&dst)[kN], const PlaneRef &p, size_t at) {
-        if constexpr (std::is_same_v<CT, Quant4>) {
-            const uint32_t pair = p.pairs[at / 32];
-            const float s = q4_scale(pair), l = q4_lowest(pair);
-            uint32_t w = 0;
+    __device__ void load(buffer_t ck, buffer_t ckp, buffer_t cv, buffer_t cvp, int lane) {
+        constexpr int kBits = kElementBits<CT>;
+        const int m = lane & 15, h = lane >> 4;
+        load_words(k, ck, (m * HD + h * (HD / 4)) * kBits / 8);
+        if constexpr (kQ4) kp = __builtin_amdgcn_raw_buffer_load_b32(ckp, (m * HD + h * (HD / 4)) / 32 * 4, 0, 0);
 #pragma unroll
-            for (int i = 0; i < kN; i++) {
-                if (i % 8 == 0)
-                    w = kN >= 8   ? reinterpret_cast<const uint32_t *>(p.data)[(at + i) / 8]
-                        : kN == 4 ? (uint32_t)reinterpret_cast<const uint16_t *>(p.data)[at / 4]
-                                  : (uint32_t)reinterpret_cast<const uint8_t *>(p.data)[at / 2];
-                dst[i] = fmaf((float)((w >> (4 * (i % 8))) & 15u), s, l);
-            }
-        } else {
-            const CT *src = reinterpret_cast<const CT *>(p.data) + at;
-            constexpr int kPer = 16 / sizeof(CT) < kN ? 16 / sizeof(CT) : kN;
-            typedef __attribute__((ext_vector_type(kPer))) CT vec_t;
-#pragma unroll
-            for (int i = 0; i < kN; i += kPer) {
-                const vec_t x = *reinterpret_cast<const vec_t *>(src + i);
-#pragma unroll
-                for (int j = 0; j < kPer; j++) dst[i + j] = (float)x[j];
+        for (int i = 0; i < 4; i++) {
+            if constexpr (kQ4) {
+                v[i][0] = load_codes<kDims>(cv, (4 * h * HD + m * kDims) / 2 + i * HD / 2);
+                vp[i] = __builtin_amdgcn_raw_buffer_load_b32(cvp, (4 * h * HD + m * kDims) / 32 * 4 + i * HD / 8, 0, 0);
+            } else {
+                load_words(v[i], cv, (4 * h * HD + m * kDims) * (kBits / 8) + i * HD * (kBits / 8));
             }
         }
     }
-    template <typename F>
-    __device__ void load(const PlaneRef &ck, const PlaneRef &cv, int lane, F row_of) {
-        const int m = lane & 15, h = lane >> 4;
-        load_values(k, ck, (size_t)row_of(m) * HD + h * (HD / 4));
-#pragma unroll
-        for (int i = 0; i < 4; i++) load_values(v[i], cv, (size_t)row_of(4 * h + i) * HD + m * kDims);
+    template <int kWords>
+    __device__ static float value(const uint32_t (&w)[kWords], uint32_t pair, int i) {
+        if constexpr (kQ4) return fmaf((float)((w[i / 8] >> (4 * (i % 8))) & 15u), q4_scale(pair), q4_lowest(pair));
+        else if constexpr (kPerWord == 2) return (float)__builtin_bit_cast(half2_t, w[i / 2])[i % 2];
+        else return __builtin_bit_cast(float, w[i]);
     }
-    __device__ void scores(float4_t (&s)[kTiles]) const {
+    __device__ void scores(const Queries &of, const Q4Bits &bits, float4_t (&s)[kTiles]) const {
         s[0] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < HD / 4; i++) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i], q[i], s[0], 0, 0, 0);
+        for (int i = 0; i < HD / 4; i++) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(value(k, kp, i), of.q[i], s[0], 0, 0, 0);
     }
-    __device__ void values(const float4_t (&w)[kTiles], float4_t (&o)[kDims]) const {
+    __device__ void values(const float4_t (&w)[kTiles], const Q4Bits &bits, float4_t (&o)[kDims]) const {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int e = 0; e < kDims; e++) o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][e], w[0][i], o[e], 0, 0, 0);
+            for (int e = 0; e < kDims; e++) o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(value(v[i], vp[i], e), w[0][i], o[e], 0, 0, 0);
     }
     __device__ bool odd_values() const {
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int e = 0; e < kDims; e++) odd |= !(fabsf(v[i][e]) <= 3.402823466e38f);
+            for (int e = 0; e < kDims; e++) odd |= !(fabsf(value(v[i], vp[i], e)) <= 3.402823466e38f);
         return odd;
     }
 };
@@ -308,7 +330,6 @@ __device__ __forceinline__ float plane_load1(const PlaneRef &p, size_t at) {
 struct AttnRowsParams {
     AttnWindowParams a;
     float *ws;
-    unsigned *tickets;
     int pieces, piece_steps;
 };
 
@@ -338,7 +359,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
     // (bitwise on purpose: with short circuits the compiler made branches of this and lost the masking of a step's first position)
     auto sees = [&](int at, int t_last) { return (bool)((int)(at <= min(my_p, t_last)) & ((int)(at >= my_low) | (int)(at < p.sinks))); };
 
-    Span span = span_of<kStep>(p0, p1, p.window, p.sinks);
+    Span span = span_of<kStep>(p0, p1, p.window, p.sinks, p.max_seq_len);
     if (p1 < 0) span.steps = 0;
     const int n_pieces = (span.steps + pp.piece_steps - 1) / pp.piece_steps;
     if (piece >= max(1, n_pieces)) return;
@@ -350,45 +371,69 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
 
     const size_t plane = (size_t)unit * p.max_seq_len;
     const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
-    const int ring = p.max_seq_len - p.sinks;
-    St st;
-    st.load_q(reinterpret_cast<const QT *>(p.q) + ((size_t)(b * p.n + my_i) * p.n_heads + g * group + (my_r - my_i * group)) * HD, h);
+    typename St::Queries queries;
+    St::load_q(queries, reinterpret_cast<const QT *>(p.q) + ((size_t)(b * p.n + my_i) * p.n_heads + g * group + (my_r - my_i * group)) * HD, h);
 
-    const int s_end = min(span.steps, (piece + 1) * pp.piece_steps);
-    for (int s = piece * pp.piece_steps + wave; s < s_end; s += kAwWaves) {
-        const bool front = s < span.first_steps;
-        const int t0 = front ? s * kStep : span.low + (s - span.first_steps) * kStep;
-        const int t_last = front ? span.first_end - 1 : span.last;
-        const int base = cache_row(t0, p.max_seq_len, p.sinks);
-        // positions past the end read the last one's row
-        auto row_of = [&](int j) {
-            int r = base + min(j, t_last - t0);
-            if (r >= p.max_seq_len) r -= ring;
-            return plane + r;
-        };
-        st.load(p.cache_k, p.cache_v, lane, row_of);
+    struct Place {
+        int t0, last, row; // positions t0 .. min(last, t0 + kStep - 1), row of the first one
+        bool front;
+    };
+    auto place_of = [&](int s) {
+        if (s < span.steps0) return Place{s * kStep, span.first_end - 1, s * kStep, true};
+        if (s < span.steps1) return Place{span.low + (s - span.steps0) * kStep, span.turn - 1, span.row + (s - span.steps0) * kStep, false};
+        return Place{span.turn + (s - span.steps1) * kStep, span.last, p.sinks + (s - span.steps1) * kStep, false};
+    };
+    const Q4Bits bits;
+    auto load = [&](St &st, int s) {
+        constexpr int kBits = kElementBits<CT>, kRow = HD * kBits / 8, kPairRow = HD / 8;
+        const Place at = place_of(s);
+        const int rows_here = min(kStep, at.last - at.t0 + 1);
+        const size_t row = plane + at.row;
+        if constexpr (kBits == 4) {
+            st.load(buffer_of(p.cache_k.data, row * kRow, rows_here * kRow), buffer_of(p.cache_k.pairs, row * kPairRow, rows_here * kPairRow),
+                    buffer_of(p.cache_v.data, row * kRow, rows_here * kRow), buffer_of(p.cache_v.pairs, row * kPairRow, rows_here * kPairRow), lane);
+        } else {
+            const buffer_t k = buffer_of(p.cache_k.data, row * kRow, rows_here * kRow), v = buffer_of(p.cache_v.data, row * kRow, rows_here * kRow);
+            st.load(k, k, v, v, lane);
+        }
+    };
+    // every row sees the whole step?
+    auto whole_step = [&](const Place &at) {
+        return at.t0 + kStep - 1 <= min(at.last, p0) && start + r0 / group >= 0 && (at.front || p.window == 0 || at.t0 > p1 - p.window);
+    };
+    bool skipped = false;
+    auto consume = [&](const St &st, int s, auto slow) {
+        const Place here = place_of(s);
+        const int t0 = here.t0;
+        const bool whole = whole_step(here);
+        if (!whole && __any(st.odd_values()) != decltype(slow)::value) { // (see below)
+            skipped = true;
+            return;
+        }
         float4_t w[kTiles];
-        st.scores(w);
-        // every row sees the whole step?
-        const bool whole = t0 + kStep - 1 <= min(t_last, p0) && start + r0 / group >= 0 && (front || p.window == 0 || t0 > p1 - p.window);
+        st.scores(queries, bits, w);
         if (!whole) {
 #pragma unroll
             for (int t = 0; t < kTiles; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int at = t0 + 16 * t + 4 * h + i;
-                    w[t][i] = sees(at, t_last) ? w[t][i] : -INFINITY;
-                }
+                for (int i = 0; i < 4; i++) w[t][i] = sees(t0 + 16 * t + 4 * h + i, here.last) ? w[t][i] : -INFINITY;
         }
         float top = -INFINITY;
 #pragma unroll
         for (int t = 0; t < kTiles; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) top = fmaxf(top, w[t][i]);
+        // The reference point of the exponentials follows the maximum only when some row's has grown by more than 2^8 (any point gives the same
+        // softmax): weights stay below 2^8, and rescaling leaves the common path.
         const float m_new = fmaxf(m_run, col_max(top));
-        const float mc = m_new > -INFINITY ? m_new * c2 : 0.0f;
-        const float alpha = __builtin_amdgcn_exp2f(fmaf(m_run, c2, -mc)); // nothing seen so far: exp2(-inf) = 0
-        m_run = m_new;
+        if (__any((m_new - m_run) * c2 > 8.0f)) { // the first maximum: infinity
+            const float alpha = m_run > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 0.0f;
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int e = 0; e < kDims; e++) o[e] *= alpha;
+        }
+        const float mc = m_run > -INFINITY ? m_run * c2 : 0.0f;
         float sum = 0.0f;
 #pragma unroll
         for (int t = 0; t < kTiles; t++)
@@ -397,21 +442,20 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
                 w[t][i] = __builtin_amdgcn_exp2f(fmaf(w[t][i], c2, -mc));
                 sum += w[t][i];
             }
-        l_run = fmaf(l_run, alpha, sum);
-#pragma unroll
-        for (int e = 0; e < kDims; e++) o[e] *= alpha;
-        if (!whole && __any(st.odd_values())) {
-            // a value that is not finite and that some row may not see: its weight 0 would still make a NaN of it in the product
+        l_run += sum;
+        if constexpr (!decltype(slow)::value) {
+            st.values(w, bits, o);
+        } else {
 #pragma unroll
             for (int t = 0; t < kTiles; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
 #pragma unroll 1
                     for (int hh = 0; hh < 4; hh++) {
-                        const int j = 16 * t + 4 * hh + i, at = t0 + j;
+                        const int j = 16 * t + 4 * hh + i;
                         const float wt = __shfl(w[t][i], hh * 16 + m, kWave);
-                        const bool seen = sees(at, t_last);
-                        const size_t from = (size_t)row_of(j) * HD + 4 * h * kDims;
+                        const bool seen = sees(t0 + j, here.last);
+                        const size_t from = (plane + here.row + j) * HD + 4 * h * kDims;
 #pragma unroll
                         for (int x = 0; x < 4; x++)
 #pragma unroll
@@ -419,8 +463,34 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
                                 if (seen) o[e][x] = fmaf(wt, plane_load1<CT>(p.cache_v, from + x * kDims + e), o[e][x]);
                     }
                 }
-        } else {
-            st.values(w, o);
+        }
+    };
+    // two sets of operands: a step's are on their way while the one before is worked on
+    const int s_end = min(span.steps, (piece + 1) * pp.piece_steps), s_first = piece * pp.piece_steps + wave;
+    {
+        St even, odd;
+        int s = s_first;
+        if (s < s_end) load(even, s);
+        while (s < s_end) {
+            if (s + kAwWaves < s_end) load(odd, s + kAwWaves);
+            __builtin_amdgcn_sched_barrier(0);
+            consume(even, s, std::false_type{});
+            s += kAwWaves;
+            if (s >= s_end) break;
+            if (s + kAwWaves < s_end) load(even, s + kAwWaves);
+            __builtin_amdgcn_sched_barrier(0);
+            consume(odd, s, std::false_type{});
+            s += kAwWaves;
+        }
+    }
+    if (skipped) {
+        // Steps that hold a value that is not finite and that some row may not see: in the product its weight 0 would make a NaN of it.
+        // Such steps were left out above; here every row adds up what it sees, position by position.
+        for (int s = s_first; s < s_end; s += kAwWaves) {
+            if (whole_step(place_of(s))) continue;
+            St st;
+            load(st, s);
+            consume(st, s, std::true_type{});
         }
     }
 
@@ -462,50 +532,77 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
         }
         return;
     }
-    // ---- join the pieces
-    __shared__ int is_last;
-    const size_t slot = (size_t)unit * gridDim.y + tile;
-    float *ws = pp.ws + slot * pp.pieces * (kAwRows * (HD + 2));
-    auto put = [](float *dst, float v) { __hip_atomic_store(dst, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-    auto get = [](const float *src) { return __hip_atomic_load(src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-    float *own = ws + (size_t)piece * (kAwRows * (HD + 2)) + jr * (HD + 2);
+    // ---- leave the piece's (m, sum) and O for attn_join_kernel: of every row first the pairs of all pieces, then the sums
     if (mine) {
+        const size_t slot = ((size_t)unit * gridDim.y + tile) * kAwRows + jr;
+        float *ws = pp.ws + slot * pp.pieces * (HD + 2);
         if (jd == 0) {
-            put(own, M);
-            put(own + 1, L);
+            ws[2 * piece] = M;
+            ws[2 * piece + 1] = L;
         }
 #pragma unroll
-        for (int i = 0; i < kPer; i++) put(own + 2 + jd + i, O[i]);
+        for (int i = 0; i < kPer; i++) ws[2 * pp.pieces + piece * HD + jd + i] = O[i];
     }
-    // Device-scope stores go through this part's L2s and device-scope loads miss them, so a store that has been acknowledged is seen by
-    // the workgroup that draws the last ticket (a property of gfx950; rlh_init refuses every other part).
-    asm volatile("" ::: "memory");
-    wait_vmcnt<0>();
-    asm volatile("" ::: "memory");
+}
+
+// Joins the pieces of one row: weights exp(m_s - M) of all pieces at once (a lane each), then the sums, wavefront w taking the pieces w, w + 4, ... A launch of
+// its own: joining by the last workgroup to arrive took 5.7 us behind pieces of 1000 positions and 11 us behind 32 pieces of 2000 (device-scope
+// stores, ticket and loads, one after the other), this takes about 3.
+constexpr int kAjThreads = 256;
+
+template <typename AC, typename QT, int HD>
+__global__ __launch_bounds__(kAjThreads) void attn_join_kernel(AttnRowsParams pp) {
+    constexpr int kStep = std::is_same_v<AC, float> ? 16 : 32, kWaves = kAjThreads / kWave, kLanes = HD / 2, kPerWave = kWave / kLanes > 0 ? kWave / kLanes : 1;
+    __shared__ float part[kWaves * kPerWave][HD];
+    const AttnWindowParams &p = pp.a;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    const int unit = blockIdx.y, r = blockIdx.x;
+    const int b = unit / p.n_kv, g = unit - b * p.n_kv, group = p.n_heads / p.n_kv, rows = p.n * group;
+    const int tile = r / kAwRows, r0 = tile * kAwRows, r1 = min(rows, r0 + kAwRows) - 1, start = p.start[b];
+    const Span span = span_of<kStep>(max(0, start + r0 / group), start + r1 / group, p.window, p.sinks, p.max_seq_len);
+    const int n_pieces = start + r1 / group < 0 ? 0 : (span.steps + pp.piece_steps - 1) / pp.piece_steps;
+    if (n_pieces <= 1) return; // the row is finished
+    const int tiles = (rows + kAwRows - 1) / kAwRows;
+    const float *ws = pp.ws + (((size_t)unit * tiles + tile) * kAwRows + (r - r0)) * pp.pieces * (HD + 2);
+    const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
+    // the first sums are on their way before their weights are known
+    const int sub = lane / kLanes, d = (lane % kLanes) * 2, s_first = wave * kPerWave + sub;
+    constexpr int kBatch = 4;
+    float2 x[kBatch];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) x[u] = *reinterpret_cast<const float2 *>(ws + 2 * pp.pieces + (size_t)min(s0 + u * kWaves * kPerWave, n_pieces - 1) * HD + d);
+    };
+    fetch(s_first);
+    float m = -INFINITY, l = 0.0f;
+    if (lane < n_pieces) {
+        m = ws[2 * lane];
+        l = ws[2 * lane + 1];
+    }
+    const float M = wave_max(m);
+    const float f = m > -INFINITY ? __builtin_amdgcn_exp2f((m - M) * c2) : 0.0f;
+    const float L = wave_sum(m > -INFINITY ? l * f : l); // (nothing seen: 0; only NaN: NaN)
+    float2 o = make_float2(0.0f, 0.0f);
+    for (int s0 = s_first; s0 - sub < n_pieces; s0 += kWaves * kPerWave * kBatch) {
+        if (s0 != s_first) fetch(s0);
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {
+            const int s = s0 + u * kWaves * kPerWave;
+            const float fs = __shfl(f, min(s, kWave - 1), kWave);
+            if (s < n_pieces && fs > 0.0f) {
+                o.x = fmaf(x[u].x, fs, o.x);
+                o.y = fmaf(x[u].y, fs, o.y);
+            }
+        }
+    }
+    *reinterpret_cast<float2 *>(&part[wave * kPerWave + sub][d]) = o;
     __syncthreads();
-    if (tid == 0) {
-        const unsigned before = __hip_atomic_fetch_add(pp.tickets + slot, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        is_last = before == (unsigned)(n_pieces - 1);
-        if (is_last) __hip_atomic_store(pp.tickets + slot, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // ready for the next launch
-    }
-    __syncthreads();
-    if (!is_last || !mine) return;
-    const float *from = ws + jr * (HD + 2);
-    M = -INFINITY;
-    L = 0.0f;
-    for (int s = 0; s < n_pieces; s++) M = fmaxf(M, get(from + (size_t)s * (kAwRows * (HD + 2))));
+    if (tid >= HD) return;
+    float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPer; i++) O[i] = 0.0f;
-    for (int s = 0; s < n_pieces; s++) {
-        const float *x = from + (size_t)s * (kAwRows * (HD + 2));
-        const float ms = get(x), ls = get(x + 1);
-        const float f = ms > -INFINITY ? __builtin_amdgcn_exp2f((ms - M) * c2) : 0.0f;
-        L += ms > -INFINITY ? ls * f : ls;
-#pragma unroll
-        for (int i = 0; i < kPer; i++) O[i] = fmaf(f > 0.0f ? get(x + 2 + jd + i) : 0.0f, f, O[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kPer; i++) out[i] = (QT)(L == 0.0f ? 0.0f : O[i] / L);
+    for (int w = 0; w < kWaves * kPerWave; w++) sum += part[w][tid];
+    const int i = r / group;
+    reinterpret_cast<QT *>(p.out)[((size_t)(b * p.n + i) * p.n_heads + g * group + (r - i * group)) * HD + tid] = (QT)(L == 0.0f ? 0.0f : sum / L);
 }
 
 template <typename AC, typename QT, typename CT, int HD>
@@ -513,6 +610,7 @@ static hipError_t launch_rows(const AttnRowsParams &p, hipStream_t s) {
     const int rows = p.a.n * (p.a.n_heads / p.a.n_kv);
     const dim3 grid((unsigned)p.pieces, (unsigned)((rows + kAwRows - 1) / kAwRows), (unsigned)(p.a.n_seqs * p.a.n_kv));
     hipLaunchKernelGGL((attn_rows_kernel<AC, QT, CT, HD>), grid, dim3(kAwThreads), 0, s, p);
+    if (p.pieces > 1) hipLaunchKernelGGL((attn_join_kernel<AC, QT, HD>), dim3((unsigned)rows, grid.z), dim3(kAjThreads), 0, s, p);
     return hipGetLastError();
 }
 template <typename AC, typename QT, typename CT>
@@ -540,28 +638,28 @@ static void cut_rows(const AttnWindowParams &p, int compute_units, int *pieces, 
         if (last < 0) continue;
         int64_t count = (last + step) / step;
         if (p.window > 0) count = std::min(count, (p.window - 1 + apart + step) / step) + (p.sinks + step - 1) / step;
+        if (last >= p.max_seq_len) count++; // the ring's end cuts a step in two
         steps = std::max(steps, count);
     }
-    const int64_t want = std::max<int64_t>(1, 2 * compute_units / units);
-    const int64_t n = std::min<int64_t>({want, (steps + kAwWaves - 1) / kAwWaves, 64});
+    // About one workgroup per compute unit, with a step for each wavefront at least.  Two steps per wavefront are not cut: joining costs a launch, about 3 us
+    // (32 heads, f16: 384 positions 7.4 us against 8.7 in two pieces, 512: 8.8 / 9.3, 768: 9.7 cut against 10.5, 1024: 9.7 / 12.0).
+    const int64_t want = std::max<int64_t>(1, compute_units / units);
+    const int64_t n = steps <= 2 * kAwWaves ? 1 : std::min<int64_t>({want, (steps + kAwWaves - 1) / kAwWaves, kAwMaxPieces});
     *piece_steps = (int)((steps + n - 1) / n);
     *pieces = (int)((steps + *piece_steps - 1) / *piece_steps);
 }
 
-void attn_window_work(const AttnWindowParams &p, int compute_units, size_t *floats, size_t *tickets) {
+size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units) {
     int pieces, piece_steps;
     cut_rows(p, compute_units, &pieces, &piece_steps);
     const int rows = p.n * (p.n_heads / p.n_kv);
-    const size_t slots = (size_t)((rows + kAwRows - 1) / kAwRows) * p.n_seqs * p.n_kv;
-    *tickets = pieces > 1 ? slots : 0;
-    *floats = pieces > 1 ? slots * pieces * kAwRows * (p.head_dim + 2) : 0;
+    return pieces > 1 ? (size_t)((rows + kAwRows - 1) / kAwRows) * kAwRows * p.n_seqs * p.n_kv * pieces * (p.head_dim + 2) : 0;
 }
 
-hipError_t launch_attn_window(const AttnWindowParams &a, int compute_units, float *ws, unsigned *tickets, hipStream_t s) {
+hipError_t launch_attn_window(const AttnWindowParams &a, int compute_units, float *ws, hipStream_t s) {
     AttnRowsParams p;
     p.a = a;
     p.ws = ws;
-    p.tickets = tickets;
     cut_rows(a, compute_units, &p.pieces, &p.piece_steps);
     if ((int64_t)a.n_seqs * a.n_kv > 65535 || (int64_t)a.n * (a.n_heads / a.n_kv) > 65535 * kAwRows) return hipErrorInvalidValue;
     switch (a.cache * 2 + a.f16) {

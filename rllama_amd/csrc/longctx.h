@@ -35,9 +35,8 @@ struct AttnWindowParams {
     int window, sinks;     // window 0: everything up to the row's own position
     int32_t start[kLongMaxSeqs];
 };
-// work memory: floats for partial results and arrival counters (which start at zero and are left at zero)
-void attn_window_work(const AttnWindowParams &p, int compute_units, size_t *floats, size_t *tickets);
-hipError_t launch_attn_window(const AttnWindowParams &p, int compute_units, float *ws, unsigned *tickets, hipStream_t s);
+size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units); // partial results of texts that are cut
+hipError_t launch_attn_window(const AttnWindowParams &p, int compute_units, float *ws, hipStream_t s);
 
 // elements between f16, f32 and 4 bits; count a multiple of 32 where one side has 4 bits
 hipError_t launch_plane_convert(const PlaneRef &dst, int dst_type, const PlaneRef &src, int src_type, size_t count, hipStream_t s);

@@ -1,0 +1,348 @@
+// attn_tiles.hip -- rlh_attn_window for many rows: f16 arithmetic, tiles of keys staged in LDS.
+//
+// Workgroup = kWaves wavefronts of 32 rows each, all on one key and value head (row r = row r / group of the sequence, head r % group of the
+// group); the keys they look at pass by in tiles of 64, K and V [64 x hd] as f16 in two LDS stages: the next tile is on its way while this one is
+// used, one barrier per tile.  f16 caches go from memory straight into LDS; of 4-bit caches a thread takes whole groups of 32 codes, converts
+// them in registers and writes 64 bytes, so a code is converted once per workgroup and not once per wavefront.
+//
+// Both products run transposed through v_mfma_f32_32x32x16_f16, so that a row is a lane pair's column of both results:
+//   S^T [key x row] = K . q^T,   O^T [dim x row] += V^T . W
+// Register v of lane l holds row 8 (v / 4) + 4 (l / 32) + v % 4 of a result, column l % 32.  The weights a lane has just formed are the second product's
+// operand when its inner index runs over the keys in that order: slot i of half h in 16-key slab s is key 16 s + 8 (i / 4) + 4 h + i % 4, i.e.
+// two runs of four keys.  ds_read_b64_tr_b16 delivers exactly such a run: of a 4 x 16 block (16 lanes, lane i addressing 4 columns of row i / 4) lane i
+// receives column i's four rows.  V therefore stays in LDS as the cache has it, one key per row.
+//
+// LDS places.  Rows of K: the 16-byte pieces of row r are permuted by r, so that eight consecutive rows' pieces of one column lie in different banks.  Rows of V:
+// 64-byte blocks are permuted by r so that the four rows of a transposing read do.
+#include "kernels.h"
+#include "attn_window_device.h"
+
+#include <algorithm>
+
+namespace rlh {
+
+typedef __attribute__((ext_vector_type(16))) float float16_t;
+typedef __attribute__((ext_vector_type(4))) _Float16 half4_t;
+typedef __attribute__((ext_vector_type(4))) short short4_t;
+
+constexpr int kAtKeys = 64;
+
+template <typename CT, int HD, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowParams p) {
+    constexpr bool kQ4 = std::is_same_v<CT, Quant4>;
+    constexpr int kRows = 32 * kWaves;
+    constexpr int kKS = HD / 16;                 // MFMA steps over the head dimension
+    constexpr int kDT = HD / 32;                 // 32-dim tiles of O^T
+    constexpr int kPieces = HD / 8;              // 16-byte pieces per row
+    constexpr int kRowBytes = HD * 2;
+    constexpr int kTileBytes = kAtKeys * kRowBytes;
+    constexpr int kStageBytes = 2 * kTileBytes;
+    constexpr int kOutRow = HD + 8;              // padded row of the output tile, halves
+    constexpr int kLdsBytes = 2 * kStageBytes > kRows * kOutRow * 2 ? 2 * kStageBytes : kRows * kOutRow * 2;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    // late rows see more keys and start first; a unit's workgroups are a multiple of its number apart, on one XCD where the units are a multiple of eight
+    const int unit = blockIdx.x;
+    const int b = unit / p.n_kv, g = unit - b * p.n_kv;
+    const int group = p.n_heads / p.n_kv, rows = p.n * group, start = p.start[b];
+    const int r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * kRows, r1 = min(rows, r0 + kRows) - 1;
+    const int p0 = max(0, start + r0 / group), p1 = start + r1 / group;
+    // this wavefront's rows, and this lane's
+    const int w0 = r0 + wave * 32, w1 = min(r1, w0 + 31);
+    const int wp0 = start + w0 / group, wp1 = w1 < w0 ? -1 : start + w1 / group;
+    const int my_r = min(w0 + col, r1), my_i = my_r / group;
+    const int my_p = w0 + col <= r1 ? start + my_i : -1;
+    const int my_low = p.window > 0 ? my_p - p.window + 1 : 0;
+    const half_t *q_row = reinterpret_cast<const half_t *>(p.q) + ((size_t)(b * p.n + my_i) * p.n_heads + g * group + (my_r - my_i * group)) * HD;
+
+    // q as the second operand: lane supplies dims 16 ks + 8 half .. + 7, in the order of the converted codes where the cache has 4 bits
+    half8_t q[kKS];
+#pragma unroll
+    for (int ks = 0; ks < kKS; ks++) {
+        const half8_t x = *reinterpret_cast<const half8_t *>(q_row + ks * 16 + half * 8);
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[ks][i] = x[kQ4 ? (i >> 1) + 4 * (i & 1) : i];
+    }
+    float16_t o[kDT];
+#pragma unroll
+    for (int d = 0; d < kDT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f;
+
+    Span span = span_of<kAtKeys>(p0, p1, p.window, p.sinks, p.max_seq_len);
+    if (p1 < 0) span.steps = 0;
+    const size_t plane = (size_t)unit * p.max_seq_len;
+    const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
+    const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
+
+    struct Place {
+        int t0, last, row;
+        bool front;
+    };
+    auto place_of = [&](int s) {
+        if (s < span.steps0) return Place{s * kAtKeys, span.first_end - 1, s * kAtKeys, true};
+        if (s < span.steps1) return Place{span.low + (s - span.steps0) * kAtKeys, span.turn - 1, span.row + (s - span.steps0) * kAtKeys, false};
+        return Place{span.turn + (s - span.steps1) * kAtKeys, span.last, p.sinks + (s - span.steps1) * kAtKeys, false};
+    };
+    auto k_swz = [](int row) { return kPieces >= 16 ? row & 15 : (row / (16 / kPieces)) & (kPieces - 1); };
+    auto v_swz = [](int row) { return HD == 128 ? (row & 3) * 4 : HD == 64 ? ((row >> 1) & 1) * 4 : 0; }; // in pieces
+
+    // ---- staging
+    constexpr int kIssues = kTileBytes / (kWaves * 1024) > 0 ? kTileBytes / (kWaves * 1024) : 1; // f16: wavefront-wide 1 KiB loads per tile of K (and of V)
+    constexpr int kGroups = 2 * kAtKeys * HD / 32, kItems = kGroups / (64 * kWaves) > 0 ? kGroups / (64 * kWaves) : 1; // 4 bits: groups per thread and tile
+    uint32_t codes[kQ4 ? kItems : 1][4], pairs[kQ4 ? kItems : 1];
+    auto fetch = [&](int s, unsigned stage) { // tile s: f16 on its way to LDS, codes on their way to registers
+        const Place at = place_of(s);
+        const int here = min(kAtKeys, at.last - at.t0 + 1);
+        const size_t row = plane + at.row;
+        if constexpr (kQ4) {
+            const buffer_t k = buffer_of(p.cache_k.data, row * (HD / 2), here * (HD / 2)), kp = buffer_of(p.cache_k.pairs, row * (HD / 8), here * (HD / 8));
+            const buffer_t v = buffer_of(p.cache_v.data, row * (HD / 2), here * (HD / 2)), vp = buffer_of(p.cache_v.pairs, row * (HD / 8), here * (HD / 8));
+#pragma unroll
+            for (int i = 0; i < kItems; i++) {
+                const int item = i * 64 * kWaves + tid, at_group = item % (kGroups / 2); // row at_group / (HD / 32), group at_group % (HD / 32)
+                const bool is_v = __builtin_amdgcn_readfirstlane(item / (kGroups / 2)) & 1;
+                const auto x = is_v ? __builtin_amdgcn_raw_buffer_load_b128(v, at_group * 16, 0, 0) : __builtin_amdgcn_raw_buffer_load_b128(k, at_group * 16, 0, 0);
+#pragma unroll
+                for (int w = 0; w < 4; w++) codes[i][w] = x[w];
+                pairs[i] = is_v ? __builtin_amdgcn_raw_buffer_load_b32(vp, at_group * 4, 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(kp, at_group * 4, 0, 0);
+            }
+        } else {
+            const half_t *k = reinterpret_cast<const half_t *>(p.cache_k.data) + row * HD, *v = reinterpret_cast<const half_t *>(p.cache_v.data) + row * HD;
+#pragma unroll
+            for (int i = 0; i < kIssues; i++) {
+                const int L = (i * kWaves + wave) * 64 + lane, r = L / kPieces, c = L % kPieces;
+                const unsigned from = (unsigned)min(r, here - 1) * kRowBytes; // keys past the last one are masked below
+                const unsigned to = lds_base + stage * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u;
+                dma16_base(k, from + ((c ^ k_swz(r)) << 4), to);
+                dma16_base(v, from + ((c ^ v_swz(r)) << 4), to + kTileBytes);
+            }
+        }
+    };
+    const Q4Bits bits;
+    auto place = [&](unsigned stage) { // 4 bits: the fetched codes as f16 into LDS
+        if constexpr (kQ4) {
+#pragma unroll
+            for (int i = 0; i < kItems; i++) {
+                const int item = i * 64 * kWaves + tid;
+                if (kGroups < 64 * kWaves && item >= kGroups) break;
+                const int at_group = item % (kGroups / 2), r = at_group / (HD / 32), c0 = at_group % (HD / 32) * 4;
+                const bool is_v = item >= kGroups / 2;
+                const half2_t pair = __builtin_bit_cast(half2_t, pairs[i]), scale = {pair[0], pair[0]}, low = {pair[1], pair[1]};
+                unsigned char *to = lds + stage * kStageBytes + (is_v ? kTileBytes : 0) + r * kRowBytes;
+                const int swz = is_v ? v_swz(r) : k_swz(r);
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    half2_t x[4];
+                    q4_pairs_f16(bits, codes[i][w], scale, low, x);
+                    uint4_t y;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) y[j] = __builtin_bit_cast(uint32_t, x[j]);
+                    *reinterpret_cast<uint4_t *>(to + (((c0 + w) ^ swz) << 4)) = y;
+                }
+            }
+        }
+    };
+
+    auto sees = [&](int at, int last) { return (bool)((int)(at <= min(my_p, last)) & ((int)(at >= my_low) | (int)(at < p.sinks))); };
+    // every row of this wavefront sees the whole tile / none sees any of it
+    auto whole_tile = [&](const Place &at) { return w0 + 31 <= r1 && wp0 >= 0 && at.t0 + kAtKeys - 1 <= min(at.last, wp0) && (at.front || p.window == 0 || at.t0 > wp1 - p.window); };
+    auto unseen_tile = [&](const Place &at) {
+        const int end = min(at.last, at.t0 + kAtKeys - 1);
+        return at.t0 > wp1 || (p.window > 0 && !at.front && end <= max(0, wp0) - p.window && at.t0 >= p.sinks);
+    };
+    bool skipped = false;
+
+    // One tile; `stage` is a compile-time constant at both call sites, so that every LDS address is the lane's base plus an immediate.
+    auto tile_step = [&](int s, auto stage) {
+        wait_vmcnt<0>(); // this wavefront's part of the tile has landed
+        __syncthreads(); // ... and everybody's; everybody is done with the tile before, whose stage is filled next
+        const bool more = s + 1 < span.steps;
+        if (more) fetch(s + 1, 1 - decltype(stage)::value);
+        const Place at = place_of(s);
+        const unsigned char *lds_k = lds + decltype(stage)::value * kStageBytes, *lds_v = lds_k + kTileBytes;
+        if (!unseen_tile(at)) {
+            const bool whole = whole_tile(at);
+            bool odd = false;
+            if (!whole) { // is every value of V finite?
+#pragma unroll
+                for (int i = 0; i < kTileBytes / 1024; i++) {
+                    const uint4_t x = *reinterpret_cast<const uint4_t *>(lds_v + i * 1024 + lane * 16);
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        odd |= ((x[w] & 0x7c000000u) == 0x7c000000u);
+                        odd |= ((x[w] & 0x7c00u) == 0x7c00u);
+                    }
+                }
+                odd = __any(odd);
+            }
+            if (odd) {
+                skipped = true;
+            } else {
+                float16_t w[2];
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+#pragma unroll
+                    for (int v = 0; v < 16; v++) w[t][v] = 0.0f;
+                    const int row = t * 32 + col;
+                    const unsigned char *from = lds_k + row * kRowBytes;
+#pragma unroll
+                    for (int ks = 0; ks < kKS; ks++)
+                        w[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t *>(from + (((ks * 2 + half) ^ k_swz(row)) << 4)), q[ks], w[t], 0, 0, 0);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int v = 0; v < 16; v++) w[t][v] = sees(at.t0 + t * 32 + (v >> 2) * 8 + half * 4 + (v & 3), at.last) ? w[t][v] : -INFINITY;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) top = fmaxf(top, w[t][v]);
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                // the reference point follows the maximum when some row's has grown by more than 2^8: weights stay below 2^8
+                const float m_new = fmaxf(m_run, top);
+                if (__any((m_new - m_run) * c2 > 8.0f)) {
+                    const float alpha = m_run > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 0.0f;
+                    m_run = m_new;
+                    l_run *= alpha;
+#pragma unroll
+                    for (int d = 0; d < kDT; d++)
+#pragma unroll
+                        for (int v = 0; v < 16; v++) o[d][v] *= alpha;
+                }
+                const float mc = m_run > -INFINITY ? m_run * c2 : 0.0f;
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) {
+                        w[t][v] = __builtin_amdgcn_exp2f(fmaf(w[t][v], c2, -mc));
+                        sum += w[t][v];
+                    }
+                l_run += sum;
+                // O^T += V^T . W, 16 keys at a time
+#pragma unroll
+                for (int sl = 0; sl < 4; sl++) {
+                    half8_t wh;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) wh[i] = (half_t)w[sl / 2][(sl % 2) * 8 + i];
+                    const int row = sl * 16 + half * 4 + ((lane & 15) >> 2); // of the first run of four keys; the second one is 8 further
+#pragma unroll
+                    for (int d = 0; d < kDT; d++) {
+                        const int piece = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                        const unsigned char *from = lds_v + row * kRowBytes + ((piece ^ v_swz(row)) << 4) + (lane & 1) * 8;
+                        typedef __attribute__((address_space(3))) short4_t *lds4;
+                        const half4_t a0 = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__attribute__((address_space(3))) void *)from));
+                        const half4_t a1 = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__attribute__((address_space(3))) void *)(from + 8 * kRowBytes)));
+                        const half8_t a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wh, o[d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if (kQ4 && more) place(1 - decltype(stage)::value);
+    };
+    if (span.steps > 0) {
+        fetch(0, 0);
+        if constexpr (kQ4) place(0);
+        for (int s = 0; s < span.steps; s += 2) {
+            tile_step(s, std::integral_constant<int, 0>{});
+            if (s + 1 < span.steps) tile_step(s + 1, std::integral_constant<int, 1>{});
+        }
+    }
+
+    if (__any(skipped)) {
+        // Tiles that hold a value of V that is not finite and that some row of the wavefront may not see (weight 0 would make a NaN of it in the product)
+        // were left out above.  Here every row adds up what it sees, key by key in f32.
+        for (int s = 0; s < span.steps; s++) {
+            const Place at = place_of(s);
+            if (unseen_tile(at) || whole_tile(at)) continue;
+            const int here = min(kAtKeys, at.last - at.t0 + 1);
+            bool odd = false;
+            for (int i = lane; i < here * HD; i += 64) odd |= !(fabsf(plane_load1<CT, true>(p.cache_v, (plane + at.row) * HD + i)) < INFINITY);
+            if (!__any(odd)) continue;
+#pragma unroll 1
+            for (int j = 0; j < here; j++) {
+                const size_t from = (plane + at.row + j) * HD;
+                float dot = 0.0f;
+#pragma unroll 1
+                for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d++) dot = fmaf((float)q_row[d], plane_load1<CT, true>(p.cache_k, from + d), dot);
+                dot += __shfl_xor(dot, 32, 64);
+                const bool seen = sees(at.t0 + j, at.last);
+                const float m_new = seen ? fmaxf(m_run, dot) : m_run;
+                const float alpha = m_new > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 1.0f;
+                const float wt = seen ? __builtin_amdgcn_exp2f((dot - (m_new > -INFINITY ? m_new : 0.0f)) * c2) : 0.0f;
+                m_run = m_new;
+                l_run = fmaf(l_run, alpha, half == 0 ? wt : 0.0f);
+#pragma unroll
+                for (int d = 0; d < kDT; d++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) {
+                        const int dim8 = (v >> 2) * 8, in8 = half * 4 + (v & 3); // place in O^T
+                        const float x = plane_load1<CT, true>(p.cache_v, from + d * 32 + dim8 + (kQ4 ? (in8 >> 1) + 4 * (in8 & 1) : in8));
+                        o[d][v] = seen ? fmaf(wt, x, o[d][v] * alpha) : o[d][v];
+                    }
+            }
+        }
+    }
+
+    // ---- normalise, round to f16, turn O^T into rows through LDS and store 16-byte pieces
+    __syncthreads(); // everybody is done with the tiles
+    const float l = l_run + __shfl_xor(l_run, 32, 64);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    half_t *ot = reinterpret_cast<half_t *>(lds) + wave * (32 * kOutRow);
+#pragma unroll
+    for (int d = 0; d < kDT; d++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            half4_t y;
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = (half_t)(l == 0.0f ? 0.0f : o[d][x * 4 + i] * inv);
+            half_t *to = ot + col * kOutRow + d * 32 + x * 8;
+            if constexpr (kQ4) { // places 4 half + i of eight hold dims (place / 2) + 4 (place % 2)
+                *reinterpret_cast<half2_t *>(to + 2 * half) = half2_t{y[0], y[2]};
+                *reinterpret_cast<half2_t *>(to + 2 * half + 4) = half2_t{y[1], y[3]};
+            } else {
+                *reinterpret_cast<half4_t *>(to + 4 * half) = y;
+            }
+        }
+    // (a wavefront reads back only what it wrote)
+    half_t *out = reinterpret_cast<half_t *>(p.out);
+#pragma unroll
+    for (int i = 0; i < 32 * kPieces / 64; i++) {
+        const int at = i * 64 + lane, r = w0 + at / kPieces, c = at % kPieces;
+        if (r > r1) continue;
+        const int ri = r / group;
+        *reinterpret_cast<half8_t *>(out + ((size_t)(b * p.n + ri) * p.n_heads + g * group + (r - ri * group)) * HD + c * 8) =
+            *reinterpret_cast<const half8_t *>(ot + (at / kPieces) * kOutRow + c * 8);
+    }
+}
+
+bool attn_tiles_takes(const AttnWindowParams &p) { return p.f16 && p.cache != kPlaneF32 && p.n * (p.n_heads / p.n_kv) > 64; }
+
+template <typename CT, int kWaves>
+static hipError_t launch_tiles(const AttnWindowParams &a, hipStream_t s) {
+    const int64_t rows = (int64_t)a.n * (a.n_heads / a.n_kv);
+    const dim3 grid((unsigned)(a.n_seqs * a.n_kv), (unsigned)((rows + 32 * kWaves - 1) / (32 * kWaves))), block(64 * kWaves);
+    switch (a.head_dim) {
+    case 32: hipLaunchKernelGGL((attn_tiles_kernel<CT, 32, kWaves>), grid, block, 0, s, a); break;
+    case 64: hipLaunchKernelGGL((attn_tiles_kernel<CT, 64, kWaves>), grid, block, 0, s, a); break;
+    case 128: hipLaunchKernelGGL((attn_tiles_kernel<CT, 128, kWaves>), grid, block, 0, s, a); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_attn_tiles(const AttnWindowParams &a, hipStream_t s) {
+    if ((int64_t)a.n * (a.n_heads / a.n_kv) > (int64_t)65535 * 128) return hipErrorInvalidValue;
+    if (a.cache == kPlaneQ4) return launch_tiles<Quant4, 4>(a, s);
+    return launch_tiles<half_t, 4>(a, s);
+}
+
+} // namespace rlh

@@ -20,7 +20,7 @@
 //
 // A text is cut into pieces when there are few rows: every workgroup leaves its (m, sum, O) in work memory and a second launch joins them.
 #include "kernels.h"
-#include "longctx.h"
+#include "attn_window_device.h"
 
 #include <algorithm>
 
@@ -31,29 +31,6 @@ constexpr int kAwThreads = kAwWaves * kWave;
 constexpr int kAwRows = 16; // rows per workgroup
 constexpr int kAwMaxPieces = 64;
 
-// What one workgroup's rows look at, in steps of kStep positions that lie side by side in the cache: the first tokens that stay visible,
-// the window up to the end of the ring, the rest of the window from the ring's beginning.
-struct Span {
-    int first_end;  // positions 0 .. first_end - 1 are looked at through `sinks`
-    int low, last;  // and low .. last
-    int row, turn;  // row of position low; the first position behind the ring's end (last + 1 if none is)
-    int steps0, steps1, steps;
-};
-template <int kStep>
-__device__ inline Span span_of(int p0, int p1, int window, int sinks, int max_seq_len) { // positions of the first and the last row that is no padding
-    Span s;
-    s.low = window > 0 ? max(0, p0 - window + 1) : 0;
-    s.last = p1;
-    s.first_end = min(sinks, s.low);
-    s.row = cache_row(s.low, max_seq_len, sinks);
-    const int room = max_seq_len - s.row; // (all of low .. last fit the ring, so they pass its end once at most)
-    s.turn = s.last - s.low < room ? s.last + 1 : s.low + room;
-    s.steps0 = (s.first_end + kStep - 1) / kStep;
-    s.steps1 = s.steps0 + (s.turn - s.low + kStep - 1) / kStep;
-    s.steps = s.steps1 + (s.last + 1 - s.turn + kStep - 1) / kStep;
-    return s;
-}
-
 __device__ __forceinline__ float col_max(float v) { // over the four lanes of a column
     v = fmaxf(v, __shfl_xor(v, 16, kWave));
     return fmaxf(v, __shfl_xor(v, 32, kWave));
@@ -63,38 +40,9 @@ __device__ __forceinline__ float col_sum(float v) {
     return v + __shfl_xor(v, 32, kWave);
 }
 
-// Masks and exponent bits of the conversion below, kept in registers: masking and setting the exponent are one instruction then, which takes
-// no literals and one scalar register at most.
-struct Q4Bits {
-    uint32_t even = 0x000f000fu, odd = 0x00f000f0u, exponent = 0x64006400u;
-    __device__ Q4Bits() {
-        asm("" : "+s"(even));
-        asm("" : "+s"(odd));
-        asm("" : "+v"(exponent));
-    }
-};
-// eight codes of a word as f16 numbers lowest + code * scale: pairs (0, 4), (1, 5), (2, 6), (3, 7).  1024 + c is the f16 number with c in its
-// last bits (0x6400 | c); 1024 + 16 c likewise, which saves half of the shifts.  The difference to 1024 is exact, the multiply-add rounds once.
-__device__ __forceinline__ void q4_pairs_f16(const Q4Bits &bits, uint32_t w, half2_t scale, half2_t scale16, half2_t low, half2_t (&out)[4]) {
-    const half2_t k1024 = {(half_t)1024.0f, (half_t)1024.0f};
-#pragma unroll
-    for (int s = 0; s < 2; s++) {
-        const uint32_t x = w >> (8 * s);
-        const half2_t a = __builtin_bit_cast(half2_t, (x & bits.even) | bits.exponent) - k1024;
-        const half2_t b = __builtin_bit_cast(half2_t, (x & bits.odd) | bits.exponent) - k1024;
-        out[2 * s] = __builtin_elementwise_fma(a, scale, low);
-        out[2 * s + 1] = __builtin_elementwise_fma(b, scale16, low);
-    }
-}
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
 constexpr uint32_t kLoHalves = 0x05040100u, kHiHalves = 0x07060302u; // of (first, second): perm(second, first, .)
 
-// Loads through a buffer descriptor of the step's rows: offsets per lane that never change, one scalar base per step, and rows past the step's
-// last one read as zeros by the hardware's bounds check, whatever memory holds there.
-typedef __amdgpu_buffer_rsrc_t buffer_t;
-__device__ __forceinline__ buffer_t buffer_of(const void *data, size_t offset, int bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(reinterpret_cast<const char *>(data)) + offset, 0, bytes, 0x00027000);
-}
 template <int kWords>
 __device__ __forceinline__ void load_words(uint32_t (&dst)[kWords], buffer_t src, int offset) {
     if constexpr (kWords % 4 == 0) {
@@ -178,18 +126,17 @@ struct Step<half_t, CT, HD> {
 #pragma unroll
         for (int t = 0; t < kTiles; t++) {
             s[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            half2_t scale, scale16, low;
+            half2_t scale, low;
             if constexpr (kQ4) {
                 scale = __builtin_bit_cast(half2_t, perm(kp[t], kp[t], kLoHalves));
                 low = __builtin_bit_cast(half2_t, perm(kp[t], kp[t], kHiHalves));
-                scale16 = scale * half2_t{(half_t)0.0625f, (half_t)0.0625f};
             }
 #pragma unroll
             for (int c = 0; c < kKs; c++) {
                 half8_t a;
                 if constexpr (kQ4) {
                     half2_t x[4];
-                    q4_pairs_f16(bits, k[t][c], scale, scale16, low, x);
+                    q4_pairs_f16(bits, k[t][c], scale, low, x);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         a[2 * i] = x[i][0];
@@ -217,11 +164,10 @@ struct Step<half_t, CT, HD> {
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const half2_t scale = __builtin_bit_cast(half2_t, perm(vp[j + 1], vp[j], kLoHalves)), low = __builtin_bit_cast(half2_t, perm(vp[j + 1], vp[j], kHiHalves));
-                const half2_t scale16 = scale * half2_t{(half_t)0.0625f, (half_t)0.0625f};
 #pragma unroll
                 for (int part = 0; part < (kDims + 3) / 4; part++) {
                     half2_t y[4];
-                    q4_pairs_f16(bits, perm(v[j + 1][0], v[j][0], part ? kHiHalves : kLoHalves), scale, scale16, low, y);
+                    q4_pairs_f16(bits, perm(v[j + 1][0], v[j][0], part ? kHiHalves : kLoHalves), scale, low, y);
 #pragma unroll
                     for (int i = 0; i < (kDims < 4 ? kDims : 4); i++) x[4 * part + i][j / 2] = __builtin_bit_cast(uint32_t, y[i]);
                 }
@@ -245,7 +191,7 @@ struct Step<half_t, CT, HD> {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             if constexpr (kQ4) {
-                odd |= ((vp[j] & 0x7c000000u) == 0x7c000000u) || ((vp[j] & 0x7c00u) == 0x7c00u);
+                odd |= !q4_finite_f16(vp[j]);
             } else {
 #pragma unroll
                 for (int w = 0; w < kDims / 2; w++) odd |= ((v[j][w] & 0x7c000000u) == 0x7c000000u) || ((v[j][w] & 0x7c00u) == 0x7c00u);
@@ -316,16 +262,6 @@ struct Step<float, CT, HD> {
         return odd;
     }
 };
-
-template <typename T>
-__device__ __forceinline__ float plane_load1(const PlaneRef &p, size_t at) {
-    if constexpr (std::is_same_v<T, Quant4>) {
-        const uint32_t pair = p.pairs[at / 32], c = (reinterpret_cast<const uint8_t *>(p.data)[at / 2] >> (4 * (at & 1))) & 15u;
-        return fmaf((float)c, q4_scale(pair), q4_lowest(pair));
-    } else {
-        return (float)reinterpret_cast<const T *>(p.data)[at];
-    }
-}
 
 struct AttnRowsParams {
     AttnWindowParams a;
@@ -460,7 +396,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
                         for (int x = 0; x < 4; x++)
 #pragma unroll
                             for (int e = 0; e < kDims; e++)
-                                if (seen) o[e][x] = fmaf(wt, plane_load1<CT>(p.cache_v, from + x * kDims + e), o[e][x]);
+                                if (seen) o[e][x] = fmaf(wt, plane_load1<CT, std::is_same_v<AC, half_t>>(p.cache_v, from + x * kDims + e), o[e][x]);
                     }
                 }
         }
@@ -650,6 +586,7 @@ static void cut_rows(const AttnWindowParams &p, int compute_units, int *pieces, 
 }
 
 size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units) {
+    if (attn_tiles_takes(p)) return 0;
     int pieces, piece_steps;
     cut_rows(p, compute_units, &pieces, &piece_steps);
     const int rows = p.n * (p.n_heads / p.n_kv);
@@ -657,6 +594,7 @@ size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units) {
 }
 
 hipError_t launch_attn_window(const AttnWindowParams &a, int compute_units, float *ws, hipStream_t s) {
+    if (attn_tiles_takes(a)) return launch_attn_tiles(a, s);
     AttnRowsParams p;
     p.a = a;
     p.ws = ws;

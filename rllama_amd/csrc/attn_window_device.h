@@ -1,0 +1,80 @@
+// attn_window_device.h -- what the two kernels of rlh_attn_window share: the span of positions a workgroup looks at, loads through buffer
+// descriptors, and the conversion of 4-bit codes to f16.
+#pragma once
+
+#include "longctx.h"
+
+namespace rlh {
+
+// What one workgroup's rows look at, in steps of kStep positions that lie side by side in the cache: the first tokens that stay visible,
+// the window up to the end of the ring, the rest of the window from the ring's beginning.
+struct Span {
+    int first_end;  // positions 0 .. first_end - 1 are looked at through `sinks`
+    int low, last;  // and low .. last
+    int row, turn;  // row of position low; the first position behind the ring's end (last + 1 if none is)
+    int steps0, steps1, steps;
+};
+template <int kStep>
+__device__ inline Span span_of(int p0, int p1, int window, int sinks, int max_seq_len) { // positions of the first and the last row that is no padding
+    Span s;
+    s.low = window > 0 ? max(0, p0 - window + 1) : 0;
+    s.last = p1;
+    s.first_end = min(sinks, s.low);
+    s.row = cache_row(s.low, max_seq_len, sinks);
+    const int room = max_seq_len - s.row; // (all of low .. last fit the ring, so they pass its end once at most)
+    s.turn = s.last - s.low < room ? s.last + 1 : s.low + room;
+    s.steps0 = (s.first_end + kStep - 1) / kStep;
+    s.steps1 = s.steps0 + (s.turn - s.low + kStep - 1) / kStep;
+    s.steps = s.steps1 + (s.last + 1 - s.turn + kStep - 1) / kStep;
+    return s;
+}
+
+// Loads through a buffer descriptor of the step's rows: offsets per lane that never change, one scalar base per step, and rows past the step's
+// last one read as zeros by the hardware's bounds check, whatever memory holds there.
+typedef __amdgpu_buffer_rsrc_t buffer_t;
+__device__ __forceinline__ buffer_t buffer_of(const void *data, size_t offset, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(reinterpret_cast<const char *>(data)) + offset, 0, bytes, 0x00027000);
+}
+// Masks and exponent bits of the conversion below, kept in registers: masking and setting the exponent are one instruction then, which takes
+// no literals and one scalar register at most.
+struct Q4Bits {
+    uint32_t even = 0x000f000fu, odd = 0x00f000f0u, exp_even = 0x64006400u, exp_odd = 0x54005400u;
+    __device__ Q4Bits() {
+        asm("" : "+s"(even));
+        asm("" : "+s"(odd));
+        asm("" : "+v"(exp_even));
+        asm("" : "+v"(exp_odd));
+    }
+};
+// eight codes of a word as f16 numbers lowest + code * scale: pairs (0, 4), (1, 5), (2, 6), (3, 7).  1024 + c is the f16 number with c in its
+// last four bits (0x6400 | c), 64 + c the one with c four bits further up (0x5400 | 16 c), which saves half of the shifts.  The differences to
+// 1024 and 64 are exact, the multiply-add rounds once.
+__device__ __forceinline__ void q4_pairs_f16(const Q4Bits &bits, uint32_t w, half2_t scale, half2_t low, half2_t (&out)[4]) {
+    const half2_t k1024 = {(half_t)1024.0f, (half_t)1024.0f}, k64 = {(half_t)64.0f, (half_t)64.0f};
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+        const uint32_t x = w >> (8 * s);
+        out[2 * s] = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (x & bits.even) | bits.exp_even) - k1024, scale, low);
+        out[2 * s + 1] = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (x & bits.odd) | bits.exp_odd) - k64, scale, low);
+    }
+}
+// whether the values of a group are all finite as f16 numbers
+__device__ __forceinline__ bool q4_finite_f16(uint32_t pair) {
+    const half2_t x = __builtin_bit_cast(half2_t, pair);
+    const half_t top = __builtin_fmaf16((half_t)15.0f, x[0], x[1]);
+    return (int)(__builtin_fabsf16(x[1]) < (half_t)INFINITY) & (int)(__builtin_fabsf16(top) < (half_t)INFINITY);
+}
+
+// One element; f16 arithmetic: with the rounding of q4_pairs_f16.
+template <typename T, bool kF16>
+__device__ __forceinline__ float plane_load1(const PlaneRef &p, size_t at) {
+    if constexpr (std::is_same_v<T, Quant4>) {
+        const uint32_t pair = p.pairs[at / 32], c = (reinterpret_cast<const uint8_t *>(p.data)[at / 2] >> (4 * (at & 1))) & 15u;
+        if constexpr (kF16) return (float)__builtin_fmaf16((half_t)(float)c, __builtin_bit_cast(half2_t, pair)[0], __builtin_bit_cast(half2_t, pair)[1]);
+        else return fmaf((float)c, q4_scale(pair), q4_lowest(pair));
+    } else {
+        return (float)reinterpret_cast<const T *>(p.data)[at];
+    }
+}
+
+} // namespace rlh

@@ -28,7 +28,7 @@ typedef __attribute__((ext_vector_type(4))) short short4_t;
 constexpr int kAtKeys = 64;
 
 template <typename CT, int HD, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowParams p) {
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParams pp) {
     constexpr bool kQ4 = std::is_same_v<CT, Quant4>;
     constexpr int kRows = 32 * kWaves;
     constexpr int kKS = HD / 16;                 // MFMA steps over the head dimension
@@ -41,6 +41,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowPa
     constexpr int kLdsBytes = 2 * kStageBytes > kRows * kOutRow * 2 ? 2 * kStageBytes : kRows * kOutRow * 2;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
 
+    const AttnWindowParams &p = pp.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
     // late rows see more keys and start first; a unit's workgroups are a multiple of its number apart, on one XCD where the units are a multiple of eight
@@ -74,6 +75,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowPa
 
     Span span = span_of<kAtKeys>(p0, p1, p.window, p.sinks, p.max_seq_len);
     if (p1 < 0) span.steps = 0;
+    const int n_pieces = (span.steps + pp.piece_steps - 1) / pp.piece_steps, piece = blockIdx.z;
+    if (piece >= max(1, n_pieces)) return;
+    const int s_first = piece * pp.piece_steps, s_end = min(span.steps, s_first + pp.piece_steps);
     const size_t plane = (size_t)unit * p.max_seq_len;
     const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
     const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
@@ -148,8 +152,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowPa
     };
 
     auto sees = [&](int at, int last) { return (bool)((int)(at <= min(my_p, last)) & ((int)(at >= my_low) | (int)(at < p.sinks))); };
-    // every row of this wavefront sees the whole tile / none sees any of it
-    auto whole_tile = [&](const Place &at) { return w0 + 31 <= r1 && wp0 >= 0 && at.t0 + kAtKeys - 1 <= min(at.last, wp0) && (at.front || p.window == 0 || at.t0 > wp1 - p.window); };
+    // every row of this wavefront that is no padding sees the whole tile / none sees any of it
+    auto whole_tile = [&](const Place &at) { return at.t0 + kAtKeys - 1 <= min(at.last, max(0, wp0)) && (at.front || p.window == 0 || at.t0 > wp1 - p.window); };
     auto unseen_tile = [&](const Place &at) {
         const int end = min(at.last, at.t0 + kAtKeys - 1);
         return at.t0 > wp1 || (p.window > 0 && !at.front && end <= max(0, wp0) - p.window && at.t0 >= p.sinks);
@@ -160,7 +164,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowPa
     auto tile_step = [&](int s, auto stage) {
         wait_vmcnt<0>(); // this wavefront's part of the tile has landed
         __syncthreads(); // ... and everybody's; everybody is done with the tile before, whose stage is filled next
-        const bool more = s + 1 < span.steps;
+        const bool more = s + 1 < s_end;
         if (more) fetch(s + 1, 1 - decltype(stage)::value);
         const Place at = place_of(s);
         const unsigned char *lds_k = lds + decltype(stage)::value * kStageBytes, *lds_v = lds_k + kTileBytes;
@@ -248,19 +252,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowPa
         }
         if (kQ4 && more) place(1 - decltype(stage)::value);
     };
-    if (span.steps > 0) {
-        fetch(0, 0);
+    if (s_first < s_end) {
+        fetch(s_first, 0);
         if constexpr (kQ4) place(0);
-        for (int s = 0; s < span.steps; s += 2) {
+        for (int s = s_first; s < s_end; s += 2) {
             tile_step(s, std::integral_constant<int, 0>{});
-            if (s + 1 < span.steps) tile_step(s + 1, std::integral_constant<int, 1>{});
+            if (s + 1 < s_end) tile_step(s + 1, std::integral_constant<int, 1>{});
         }
     }
 
     if (__any(skipped)) {
         // Tiles that hold a value of V that is not finite and that some row of the wavefront may not see (weight 0 would make a NaN of it in the product)
         // were left out above.  Here every row adds up what it sees, key by key in f32.
-        for (int s = 0; s < span.steps; s++) {
+        for (int s = s_first; s < s_end; s++) {
             const Place at = place_of(s);
             if (unseen_tile(at) || whole_tile(at)) continue;
             const int here = min(kAtKeys, at.last - at.t0 + 1);
@@ -292,9 +296,32 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowPa
         }
     }
 
+    const float l = my_p < 0 ? 0.0f : l_run + __shfl_xor(l_run, 32, 64); // (padding: 0)
+    if (n_pieces > 1) { // ---- leave (m, sum) and O of the piece for attn_join_kernel
+        if (w0 + col > r1) return;
+        float *ws = pp.ws + ((size_t)unit * rows + w0 + col) * pp.pieces * (HD + 2);
+        if (half == 0) {
+            ws[2 * piece] = m_run;
+            ws[2 * piece + 1] = l;
+        }
+        ws += 2 * pp.pieces + (size_t)piece * HD;
+#pragma unroll
+        for (int d = 0; d < kDT; d++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                float *to = ws + d * 32 + x * 8;
+                if constexpr (kQ4) { // places 4 half + i of eight hold dims (place / 2) + 4 (place % 2)
+                    *reinterpret_cast<float2 *>(to + 2 * half) = make_float2(o[d][x * 4], o[d][x * 4 + 2]);
+                    *reinterpret_cast<float2 *>(to + 2 * half + 4) = make_float2(o[d][x * 4 + 1], o[d][x * 4 + 3]);
+                } else {
+                    *reinterpret_cast<float2 *>(to + 4 * half) = make_float2(o[d][x * 4], o[d][x * 4 + 1]);
+                    *reinterpret_cast<float2 *>(to + 4 * half + 2) = make_float2(o[d][x * 4 + 2], o[d][x * 4 + 3]);
+                }
+            }
+        return;
+    }
     // ---- normalise, round to f16, turn O^T into rows through LDS and store 16-byte pieces
     __syncthreads(); // everybody is done with the tiles
-    const float l = l_run + __shfl_xor(l_run, 32, 64);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     half_t *ot = reinterpret_cast<half_t *>(lds) + wave * (32 * kOutRow);
 #pragma unroll
@@ -305,7 +332,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowPa
 #pragma unroll
             for (int i = 0; i < 4; i++) y[i] = (half_t)(l == 0.0f ? 0.0f : o[d][x * 4 + i] * inv);
             half_t *to = ot + col * kOutRow + d * 32 + x * 8;
-            if constexpr (kQ4) { // places 4 half + i of eight hold dims (place / 2) + 4 (place % 2)
+            if constexpr (kQ4) { // (as above)
                 *reinterpret_cast<half2_t *>(to + 2 * half) = half2_t{y[0], y[2]};
                 *reinterpret_cast<half2_t *>(to + 2 * half + 4) = half2_t{y[1], y[3]};
             } else {
@@ -326,23 +353,70 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnWindowPa
 
 bool attn_tiles_takes(const AttnWindowParams &p) { return p.f16 && p.cache != kPlaneF32 && p.n * (p.n_heads / p.n_kv) > 64; }
 
-template <typename CT, int kWaves>
-static hipError_t launch_tiles(const AttnWindowParams &a, hipStream_t s) {
-    const int64_t rows = (int64_t)a.n * (a.n_heads / a.n_kv);
-    const dim3 grid((unsigned)(a.n_seqs * a.n_kv), (unsigned)((rows + 32 * kWaves - 1) / (32 * kWaves))), block(64 * kWaves);
-    switch (a.head_dim) {
-    case 32: hipLaunchKernelGGL((attn_tiles_kernel<CT, 32, kWaves>), grid, block, 0, s, a); break;
-    case 64: hipLaunchKernelGGL((attn_tiles_kernel<CT, 64, kWaves>), grid, block, 0, s, a); break;
-    case 128: hipLaunchKernelGGL((attn_tiles_kernel<CT, 128, kWaves>), grid, block, 0, s, a); break;
+constexpr int kAtWaves = 4;
+constexpr int kAtRows = 32 * kAtWaves;
+
+// How the texts are cut.  A workgroup alone on its compute unit takes 1.4 us per tile of 128 rows and 64 keys of 128 dims, two of them 2.3 us (together less per
+// tile); joining costs 4 us and writing and reading the partial results, p * 2 (hd + 2) floats per row and head at about 4.5 bytes per ps.  The number of pieces with the
+// least sum is taken: 400 rows behind 8000 positions, 32 heads on 8 key heads: 4 pieces, 92 us; 1024 rows from the text's beginning: 1 piece.
+static void cut_tiles(const AttnWindowParams &p, int compute_units, int *pieces, int *piece_steps) {
+    const int group = p.n_heads / p.n_kv;
+    const int64_t rows = (int64_t)p.n * group, units = (rows + kAtRows - 1) / kAtRows * p.n_seqs * p.n_kv;
+    const int64_t apart = std::min<int64_t>(p.n - 1, (kAtRows - 2) / group + 1); // of a workgroup's rows
+    int64_t steps = 1;                                                           // no workgroup has more
+    for (int b = 0; b < p.n_seqs; b++) {
+        const int64_t last = (int64_t)p.start[b] + p.n - 1;
+        if (last < 0) continue;
+        int64_t count = (last + kAtKeys) / kAtKeys;
+        if (p.window > 0) count = std::min(count, (p.window - 1 + apart + kAtKeys) / kAtKeys) + (p.sinks + kAtKeys - 1) / kAtKeys;
+        if (last >= p.max_seq_len) count++; // the ring's end cuts a tile in two
+        steps = std::max(steps, count);
+    }
+    const double tile_us = 1.4 * p.head_dim / 128, shared_us = 2.3 * p.head_dim / 128, piece_us = (double)p.n * p.n_heads * p.n_seqs * (p.head_dim + 2) * 8 / 4.5e6;
+    int64_t n = 1;
+    double best = steps * (units > compute_units ? shared_us : tile_us);
+    for (int64_t c = 2; c <= kMaxPieces && c <= steps && c * units <= 2 * compute_units; c++) {
+        const double us = (double)((steps + c - 1) / c) * (c * units > compute_units ? shared_us : tile_us) + 4.0 + c * piece_us;
+        if (us < best) {
+            best = us;
+            n = c;
+        }
+    }
+    *piece_steps = (int)((steps + n - 1) / n);
+    *pieces = (int)((steps + *piece_steps - 1) / *piece_steps);
+}
+
+size_t attn_tiles_work_floats(const AttnWindowParams &p, int compute_units) {
+    int pieces, piece_steps;
+    cut_tiles(p, compute_units, &pieces, &piece_steps);
+    return pieces > 1 ? (size_t)p.n * p.n_heads * p.n_seqs * pieces * (p.head_dim + 2) : 0;
+}
+
+template <typename CT, int HD>
+static void launch_tiles(const AttnCutParams &p, hipStream_t s) {
+    const int rows = p.a.n * (p.a.n_heads / p.a.n_kv);
+    const unsigned units = (unsigned)(p.a.n_seqs * p.a.n_kv);
+    const dim3 grid(units, (unsigned)((rows + kAtRows - 1) / kAtRows), (unsigned)p.pieces);
+    hipLaunchKernelGGL((attn_tiles_kernel<CT, HD, kAtWaves>), grid, dim3(64 * kAtWaves), 0, s, p);
+    if (p.pieces > 1) launch_attn_join<half_t, HD, kAtRows, kAtKeys>(p, s);
+}
+
+hipError_t launch_attn_tiles(const AttnWindowParams &a, int compute_units, float *ws, hipStream_t s) {
+    if ((int64_t)a.n * (a.n_heads / a.n_kv) > (int64_t)65535 * kAtRows || (int64_t)a.n_seqs * a.n_kv > 65535) return hipErrorInvalidValue;
+    AttnCutParams p;
+    p.a = a;
+    p.ws = ws;
+    cut_tiles(a, compute_units, &p.pieces, &p.piece_steps);
+    switch (a.head_dim * 2 + (a.cache == kPlaneQ4)) {
+    case 64: launch_tiles<half_t, 32>(p, s); break;
+    case 65: launch_tiles<Quant4, 32>(p, s); break;
+    case 128: launch_tiles<half_t, 64>(p, s); break;
+    case 129: launch_tiles<Quant4, 64>(p, s); break;
+    case 256: launch_tiles<half_t, 128>(p, s); break;
+    case 257: launch_tiles<Quant4, 128>(p, s); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
-}
-
-hipError_t launch_attn_tiles(const AttnWindowParams &a, hipStream_t s) {
-    if ((int64_t)a.n * (a.n_heads / a.n_kv) > (int64_t)65535 * 128) return hipErrorInvalidValue;
-    if (a.cache == kPlaneQ4) return launch_tiles<Quant4, 4>(a, s);
-    return launch_tiles<half_t, 4>(a, s);
 }
 
 } // namespace rlh

@@ -29,7 +29,6 @@ namespace rlh {
 constexpr int kAwWaves = 8;
 constexpr int kAwThreads = kAwWaves * kWave;
 constexpr int kAwRows = 16; // rows per workgroup
-constexpr int kAwMaxPieces = 64;
 
 __device__ __forceinline__ float col_max(float v) { // over the four lanes of a column
     v = fmaxf(v, __shfl_xor(v, 16, kWave));
@@ -263,14 +262,8 @@ struct Step<float, CT, HD> {
     }
 };
 
-struct AttnRowsParams {
-    AttnWindowParams a;
-    float *ws;
-    int pieces, piece_steps;
-};
-
 template <typename AC, typename QT, typename CT, int HD>
-__global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp) {
+__global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp) {
     typedef Step<AC, CT, HD> St;
     constexpr int kDims = St::kDims, kTiles = St::kTiles, kStep = St::kPositions;
     constexpr int kPad = HD + 4;
@@ -333,9 +326,9 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
             st.load(k, k, v, v, lane);
         }
     };
-    // every row sees the whole step?
+    // every row that is no padding sees the whole step?
     auto whole_step = [&](const Place &at) {
-        return at.t0 + kStep - 1 <= min(at.last, p0) && start + r0 / group >= 0 && (at.front || p.window == 0 || at.t0 > p1 - p.window);
+        return at.t0 + kStep - 1 <= min(at.last, p0) && (at.front || p.window == 0 || at.t0 > p1 - p.window);
     };
     bool skipped = false;
     auto consume = [&](const St &st, int s, auto slow) {
@@ -460,6 +453,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
         for (int i = 0; i < kPer; i++) O[i] = fmaf(so[w][jr][jd + i], f, O[i]);
     }
     const int jri = (r0 + jr) / group;
+    if (start + jri < 0) L = 0.0f; // padding
     QT *out = reinterpret_cast<QT *>(p.out) + ((size_t)(b * p.n + jri) * p.n_heads + g * group + (r0 + jr - jri * group)) * HD + jd;
     if (n_pieces <= 1) {
         if (mine) {
@@ -470,8 +464,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
     }
     // ---- leave the piece's (m, sum) and O for attn_join_kernel: of every row first the pairs of all pieces, then the sums
     if (mine) {
-        const size_t slot = ((size_t)unit * gridDim.y + tile) * kAwRows + jr;
-        float *ws = pp.ws + slot * pp.pieces * (HD + 2);
+        float *ws = pp.ws + ((size_t)unit * rows + r0 + jr) * pp.pieces * (HD + 2);
         if (jd == 0) {
             ws[2 * piece] = M;
             ws[2 * piece + 1] = L;
@@ -481,76 +474,16 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnRowsParams pp
     }
 }
 
-// Joins the pieces of one row: weights exp(m_s - M) of all pieces at once (a lane each), then the sums, wavefront w taking the pieces w, w + 4, ... A launch of
-// its own: joining by the last workgroup to arrive took 5.7 us behind pieces of 1000 positions and 11 us behind 32 pieces of 2000 (device-scope
-// stores, ticket and loads, one after the other), this takes about 3.
-constexpr int kAjThreads = 256;
-
-template <typename AC, typename QT, int HD>
-__global__ __launch_bounds__(kAjThreads) void attn_join_kernel(AttnRowsParams pp) {
-    constexpr int kStep = std::is_same_v<AC, float> ? 16 : 32, kWaves = kAjThreads / kWave, kLanes = HD / 2, kPerWave = kWave / kLanes > 0 ? kWave / kLanes : 1;
-    __shared__ float part[kWaves * kPerWave][HD];
-    const AttnWindowParams &p = pp.a;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const int unit = blockIdx.y, r = blockIdx.x;
-    const int b = unit / p.n_kv, g = unit - b * p.n_kv, group = p.n_heads / p.n_kv, rows = p.n * group;
-    const int tile = r / kAwRows, r0 = tile * kAwRows, r1 = min(rows, r0 + kAwRows) - 1, start = p.start[b];
-    const Span span = span_of<kStep>(max(0, start + r0 / group), start + r1 / group, p.window, p.sinks, p.max_seq_len);
-    const int n_pieces = start + r1 / group < 0 ? 0 : (span.steps + pp.piece_steps - 1) / pp.piece_steps;
-    if (n_pieces <= 1) return; // the row is finished
-    const int tiles = (rows + kAwRows - 1) / kAwRows;
-    const float *ws = pp.ws + (((size_t)unit * tiles + tile) * kAwRows + (r - r0)) * pp.pieces * (HD + 2);
-    const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
-    // the first sums are on their way before their weights are known
-    const int sub = lane / kLanes, d = (lane % kLanes) * 2, s_first = wave * kPerWave + sub;
-    constexpr int kBatch = 4;
-    float2 x[kBatch];
-    auto fetch = [&](int s0) {
-#pragma unroll
-        for (int u = 0; u < kBatch; u++) x[u] = *reinterpret_cast<const float2 *>(ws + 2 * pp.pieces + (size_t)min(s0 + u * kWaves * kPerWave, n_pieces - 1) * HD + d);
-    };
-    fetch(s_first);
-    float m = -INFINITY, l = 0.0f;
-    if (lane < n_pieces) {
-        m = ws[2 * lane];
-        l = ws[2 * lane + 1];
-    }
-    const float M = wave_max(m);
-    const float f = m > -INFINITY ? __builtin_amdgcn_exp2f((m - M) * c2) : 0.0f;
-    const float L = wave_sum(m > -INFINITY ? l * f : l); // (nothing seen: 0; only NaN: NaN)
-    float2 o = make_float2(0.0f, 0.0f);
-    for (int s0 = s_first; s0 - sub < n_pieces; s0 += kWaves * kPerWave * kBatch) {
-        if (s0 != s_first) fetch(s0);
-#pragma unroll
-        for (int u = 0; u < kBatch; u++) {
-            const int s = s0 + u * kWaves * kPerWave;
-            const float fs = __shfl(f, min(s, kWave - 1), kWave);
-            if (s < n_pieces && fs > 0.0f) {
-                o.x = fmaf(x[u].x, fs, o.x);
-                o.y = fmaf(x[u].y, fs, o.y);
-            }
-        }
-    }
-    *reinterpret_cast<float2 *>(&part[wave * kPerWave + sub][d]) = o;
-    __syncthreads();
-    if (tid >= HD) return;
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves * kPerWave; w++) sum += part[w][tid];
-    const int i = r / group;
-    reinterpret_cast<QT *>(p.out)[((size_t)(b * p.n + i) * p.n_heads + g * group + (r - i * group)) * HD + tid] = (QT)(L == 0.0f ? 0.0f : sum / L);
-}
-
 template <typename AC, typename QT, typename CT, int HD>
-static hipError_t launch_rows(const AttnRowsParams &p, hipStream_t s) {
+static hipError_t launch_rows(const AttnCutParams &p, hipStream_t s) {
     const int rows = p.a.n * (p.a.n_heads / p.a.n_kv);
     const dim3 grid((unsigned)p.pieces, (unsigned)((rows + kAwRows - 1) / kAwRows), (unsigned)(p.a.n_seqs * p.a.n_kv));
     hipLaunchKernelGGL((attn_rows_kernel<AC, QT, CT, HD>), grid, dim3(kAwThreads), 0, s, p);
-    if (p.pieces > 1) hipLaunchKernelGGL((attn_join_kernel<AC, QT, HD>), dim3((unsigned)rows, grid.z), dim3(kAjThreads), 0, s, p);
+    if (p.pieces > 1) launch_attn_join<QT, HD, kAwRows, Step<AC, CT, HD>::kPositions>(p, s);
     return hipGetLastError();
 }
 template <typename AC, typename QT, typename CT>
-static hipError_t launch_rows_hd(const AttnRowsParams &p, hipStream_t s) {
+static hipError_t launch_rows_hd(const AttnCutParams &p, hipStream_t s) {
     switch (p.a.head_dim) {
     case 32: return launch_rows<AC, QT, CT, 32>(p, s);
     case 64: return launch_rows<AC, QT, CT, 64>(p, s);
@@ -580,22 +513,21 @@ static void cut_rows(const AttnWindowParams &p, int compute_units, int *pieces, 
     // About one workgroup per compute unit, with a step for each wavefront at least.  Two steps per wavefront are not cut: joining costs a launch, about 3 us
     // (32 heads, f16: 384 positions 7.4 us against 8.7 in two pieces, 512: 8.8 / 9.3, 768: 9.7 cut against 10.5, 1024: 9.7 / 12.0).
     const int64_t want = std::max<int64_t>(1, compute_units / units);
-    const int64_t n = steps <= 2 * kAwWaves ? 1 : std::min<int64_t>({want, (steps + kAwWaves - 1) / kAwWaves, kAwMaxPieces});
+    const int64_t n = steps <= 2 * kAwWaves ? 1 : std::min<int64_t>({want, (steps + kAwWaves - 1) / kAwWaves, kMaxPieces});
     *piece_steps = (int)((steps + n - 1) / n);
     *pieces = (int)((steps + *piece_steps - 1) / *piece_steps);
 }
 
 size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units) {
-    if (attn_tiles_takes(p)) return 0;
+    if (attn_tiles_takes(p)) return attn_tiles_work_floats(p, compute_units);
     int pieces, piece_steps;
     cut_rows(p, compute_units, &pieces, &piece_steps);
-    const int rows = p.n * (p.n_heads / p.n_kv);
-    return pieces > 1 ? (size_t)((rows + kAwRows - 1) / kAwRows) * kAwRows * p.n_seqs * p.n_kv * pieces * (p.head_dim + 2) : 0;
+    return pieces > 1 ? (size_t)p.n * p.n_heads * p.n_seqs * pieces * (p.head_dim + 2) : 0;
 }
 
 hipError_t launch_attn_window(const AttnWindowParams &a, int compute_units, float *ws, hipStream_t s) {
-    if (attn_tiles_takes(a)) return launch_attn_tiles(a, s);
-    AttnRowsParams p;
+    if (attn_tiles_takes(a)) return launch_attn_tiles(a, compute_units, ws, s);
+    AttnCutParams p;
     p.a = a;
     p.ws = ws;
     cut_rows(a, compute_units, &p.pieces, &p.piece_steps);

@@ -77,4 +77,89 @@ __device__ __forceinline__ float plane_load1(const PlaneRef &p, size_t at) {
     }
 }
 
+// A text that is cut: work memory, for every row first the pairs (m, sum) of its pieces and then the sums O of each, and how it is cut.
+struct AttnCutParams {
+    AttnWindowParams a;
+    float *ws;
+    int pieces, piece_steps; // pieces of `piece_steps` steps, at most `pieces` of them
+};
+constexpr int kMaxPieces = 64;
+
+// Joins the pieces of rows: weights exp(m_s - M) of all pieces of a row at once (a lane each), then the sums, added up in the same order whatever
+// arrives when.  kShare wavefronts take a row: four where there are few rows, one where there are many (a workgroup for each of 32768 rows took 40 us).
+// A launch of its own: joining by the last workgroup to arrive took 5.7 us behind pieces of 1000 positions and 11 us behind 32 pieces of 2000
+// (device-scope stores, ticket and loads, one after the other), this takes about 3.
+constexpr int kAjWaves = 4;
+
+template <typename QT, int HD, int kTileRows, int kStep, int kShare>
+__global__ __launch_bounds__(kAjWaves *kWave) void attn_join_kernel(AttnCutParams pp) {
+    constexpr int kLanes = HD / 2, kSub = kWave / kLanes; // lanes per piece, pieces side by side in a wavefront
+    constexpr int kParts = kShare * kSub;
+    __shared__ float part[kAjWaves * kSub][HD];
+    const AttnWindowParams &p = pp.a;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int group = p.n_heads / p.n_kv, rows = p.n * group;
+    const int unit = blockIdx.y, b = unit / p.n_kv, g = unit - b * p.n_kv, start = p.start[b];
+    const int r = blockIdx.x * (kAjWaves / kShare) + wave / kShare; // (with four wavefronts per row all of them leave together below)
+    int n_pieces = 0;
+    if (r < rows) {
+        const int r0 = r / kTileRows * kTileRows, r1 = min(rows, r0 + kTileRows) - 1;
+        const Span span = span_of<kStep>(max(0, start + r0 / group), start + r1 / group, p.window, p.sinks, p.max_seq_len);
+        n_pieces = start + r1 / group < 0 ? 0 : (span.steps + pp.piece_steps - 1) / pp.piece_steps;
+    }
+    if (n_pieces <= 1) { // the row is finished
+        if constexpr (kShare == 1) __syncthreads();
+        return;
+    }
+    const float *ws = pp.ws + ((size_t)unit * rows + r) * pp.pieces * (HD + 2);
+    const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
+    // the first sums are on their way before their weights are known
+    const int sub = lane / kLanes, d = (lane % kLanes) * 2, s_first = (wave % kShare) * kSub + sub;
+    constexpr int kBatch = 4;
+    float2 x[kBatch];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) x[u] = *reinterpret_cast<const float2 *>(ws + 2 * pp.pieces + (size_t)min(s0 + u * kParts, n_pieces - 1) * HD + d);
+    };
+    fetch(s_first);
+    float m = -INFINITY, l = 0.0f;
+    if (lane < n_pieces) {
+        m = ws[2 * lane];
+        l = ws[2 * lane + 1];
+    }
+    const float M = wave_max(m);
+    const float f = m > -INFINITY ? __builtin_amdgcn_exp2f((m - M) * c2) : 0.0f;
+    const float L = wave_sum(m > -INFINITY ? l * f : l); // (nothing seen: 0; only NaN: NaN)
+    float2 o = make_float2(0.0f, 0.0f);
+    for (int s0 = s_first; s0 - sub < n_pieces; s0 += kParts * kBatch) {
+        if (s0 != s_first) fetch(s0);
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {
+            const int s = s0 + u * kParts;
+            const float fs = __shfl(f, min(s, kWave - 1), kWave);
+            if (s < n_pieces && fs > 0.0f) {
+                o.x = fmaf(x[u].x, fs, o.x);
+                o.y = fmaf(x[u].y, fs, o.y);
+            }
+        }
+    }
+    *reinterpret_cast<float2 *>(&part[wave * kSub + sub][d]) = o;
+    __syncthreads();
+    const int i = r / group;
+    QT *out = reinterpret_cast<QT *>(p.out) + ((size_t)(b * p.n + i) * p.n_heads + g * group + (r - i * group)) * HD;
+    for (int e = kShare == 1 ? lane : (int)threadIdx.x; e < HD; e += kShare * kWave) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kParts; w++) sum += part[wave / kShare * kParts + w][e];
+        out[e] = (QT)(L == 0.0f ? 0.0f : sum / L);
+    }
+}
+
+template <typename QT, int HD, int kTileRows, int kStep>
+inline void launch_attn_join(const AttnCutParams &p, hipStream_t s) {
+    const unsigned rows = (unsigned)(p.a.n * (p.a.n_heads / p.a.n_kv)), units = (unsigned)(p.a.n_seqs * p.a.n_kv);
+    if ((int64_t)rows * units <= 1024) hipLaunchKernelGGL((attn_join_kernel<QT, HD, kTileRows, kStep, kAjWaves>), dim3(rows, units), dim3(kAjWaves * kWave), 0, s, p);
+    else hipLaunchKernelGGL((attn_join_kernel<QT, HD, kTileRows, kStep, 1>), dim3((rows + kAjWaves - 1) / kAjWaves, units), dim3(kAjWaves * kWave), 0, s, p);
+}
+
 } // namespace rlh

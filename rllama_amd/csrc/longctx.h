@@ -36,9 +36,10 @@ struct AttnWindowParams {
     int32_t start[kLongMaxSeqs];
 };
 size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units); // partial results of texts that are cut
-// the form for many rows (attn_tiles.hip): which calls it takes, and its launch
+// the form for many rows (attn_tiles.hip): which calls it takes, its work memory and its launch
 bool attn_tiles_takes(const AttnWindowParams &p);
-hipError_t launch_attn_tiles(const AttnWindowParams &p, hipStream_t s);
+size_t attn_tiles_work_floats(const AttnWindowParams &p, int compute_units);
+hipError_t launch_attn_tiles(const AttnWindowParams &p, int compute_units, float *ws, hipStream_t s);
 hipError_t launch_attn_window(const AttnWindowParams &p, int compute_units, float *ws, hipStream_t s);
 
 // elements between f16, f32 and 4 bits; count a multiple of 32 where one side has 4 bits

@@ -18,70 +18,78 @@ constexpr int kAppendThreads = 256;
 
 template <typename IN, typename CT, int HD>
 __global__ __launch_bounds__(kAppendThreads) void qkv_append_kernel(QkvAppendParams p) {
-    constexpr int kLanes = HD / 8;
-    const int slots = p.n_heads + 2 * p.n_kv;
-    const int64_t unit = ((int64_t)blockIdx.x * kAppendThreads + threadIdx.x) / kLanes;
-    const int dl = threadIdx.x % kLanes;
-    const int64_t rows = (int64_t)p.n * p.n_seqs;
-    if (unit >= rows * slots) return; // (the lanes of a head leave together)
-    const int row = (int)(unit / slots), slot = (int)(unit - (int64_t)row * slots);
-    const int b = row / p.n, pos = p.start[b] + (row - b * p.n);
-    const size_t q_index = (size_t)row * p.n_heads * HD + (size_t)slot * HD + dl * 8;
+    constexpr int kLanes = HD / 8, kUnits = kAppendThreads / kLanes;
+    const int row = blockIdx.x, b = row / p.n, pos = p.start[b] + (row - b * p.n);
+    const int dl = threadIdx.x % kLanes, slots = p.n_heads + 2 * p.n_kv;
+    const int first = blockIdx.y * kUnits + threadIdx.x / kLanes, stride = gridDim.y * kUnits;
+    const size_t q_row = (size_t)row * p.n_heads * HD + dl * 8;
     if (pos < 0) { // padding: zero queries, nothing in the cache
-        if (slot < p.n_heads) {
-            const float zero[8] = {};
-            plane_store8<IN>(p.q, q_index, zero);
-        }
+        const float zero[8] = {};
+        for (int slot = first; slot < p.n_heads; slot += stride) plane_store8<IN>(p.q, q_row + (size_t)slot * HD, zero);
         return;
     }
-    float v[8];
-    plane_load8<IN>(p.qkv, (size_t)unit * HD + dl * 8, v);
-    const int kind = slot < p.n_heads ? 0 : slot < p.n_heads + p.n_kv ? 1 : 2; // query, key, value
-    if (kind < 2) {
-        const float *norm = kind == 0 ? p.q_norm : p.k_norm;
-        if (norm) {
-            float sq = 0.0f;
+    // the row's angles and the norms' weights, once for all heads that this thread takes
+    const float2 *turn = reinterpret_cast<const float2 *>(p.freqs) + (size_t)pos * (HD / 2) + (p.halves ? dl % (kLanes / 2) * 8 : dl * 4);
+    const bool second = dl >= kLanes / 2;
+    float2 angle[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) sq = fmaf(v[i], v[i], sq);
-            const float r = 1.0f / sqrtf(group_sum<kLanes>(sq) / (float)HD + p.eps);
+    for (int i = 0; i < 8; i++) angle[i] = i < 4 || p.halves ? turn[i] : make_float2(0.0f, 0.0f);
+    float qw[8], kw[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = v[i] * r * norm[dl * 8 + i];
-        }
-        const float2 *turn = reinterpret_cast<const float2 *>(p.freqs) + (size_t)pos * (HD / 2);
-        if (p.halves) {
-            const bool second = dl >= kLanes / 2;
-            const float2 *f = turn + (dl % (kLanes / 2)) * 8;
+    for (int i = 0; i < 8; i++) {
+        qw[i] = p.q_norm ? p.q_norm[dl * 8 + i] : 1.0f;
+        kw[i] = p.k_norm ? p.k_norm[dl * 8 + i] : 1.0f;
+    }
+    const size_t cache_at = (size_t)cache_row(pos, p.max_seq_len, p.sinks) * HD + dl * 8;
+    for (int slot = first; slot < slots; slot += stride) { // (the lanes of a head stay together)
+        float v[8];
+        plane_load8<IN>(p.qkv, ((size_t)row * slots + slot) * HD + dl * 8, v);
+        const int kind = slot < p.n_heads ? 0 : slot < p.n_heads + p.n_kv ? 1 : 2; // query, key, value
+        if (kind < 2) {
+            if (kind == 0 ? p.q_norm != nullptr : p.k_norm != nullptr) {
+                float sq = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float other = __shfl_xor(v[i], kLanes / 2, kLanes);
-                float re, im;
-                rope_pair(second ? other : v[i], second ? v[i] : other, f[i], re, im);
-                v[i] = second ? im : re;
+                for (int i = 0; i < 8; i++) sq = fmaf(v[i], v[i], sq);
+                const float r = 1.0f / sqrtf(group_sum<kLanes>(sq) / (float)HD + p.eps);
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = v[i] * r * (kind == 0 ? qw[i] : kw[i]);
             }
-        } else {
+            if (p.halves) {
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) rope_pair(v[i], v[i + 1], turn[dl * 4 + i / 2], v[i], v[i + 1]);
+                for (int i = 0; i < 8; i++) {
+                    const float other = __shfl_xor(v[i], kLanes / 2, kLanes);
+                    float re, im;
+                    rope_pair(second ? other : v[i], second ? v[i] : other, angle[i], re, im);
+                    v[i] = second ? im : re;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) rope_pair(v[i], v[i + 1], angle[i / 2], v[i], v[i + 1]);
+            }
+        }
+        if (kind == 0) {
+            plane_store8<IN>(p.q, q_row + (size_t)slot * HD, v);
+        } else {
+            const int g = slot - p.n_heads - (kind == 2 ? p.n_kv : 0);
+            plane_store8<CT>(kind == 1 ? p.cache_k : p.cache_v, (size_t)(b * p.n_kv + g) * p.max_seq_len * HD + cache_at, v);
         }
     }
-    if (kind == 0) {
-        plane_store8<IN>(p.q, q_index, v);
-        return;
-    }
-    const int g = slot - p.n_heads - (kind == 2 ? p.n_kv : 0);
-    const size_t at = ((size_t)(b * p.n_kv + g) * p.max_seq_len + cache_row(pos, p.max_seq_len, p.sinks)) * HD + dl * 8;
-    plane_store8<CT>(kind == 1 ? p.cache_k : p.cache_v, at, v);
+}
+
+template <typename IN, typename CT, int HD>
+static void launch_append(const QkvAppendParams &p, hipStream_t s) {
+    const int units = kAppendThreads * 8 / HD, slots = p.n_heads + 2 * p.n_kv, rows = p.n * p.n_seqs;
+    // Few rows: a workgroup for every `units` heads of a row, so that nothing waits.  Many rows: one per row, so that angles and weights are read once.
+    const int blocks = rows < 512 ? (slots + units - 1) / units : 1;
+    hipLaunchKernelGGL((qkv_append_kernel<IN, CT, HD>), dim3((unsigned)rows, (unsigned)blocks), dim3(kAppendThreads), 0, s, p);
 }
 
 template <typename IN, typename CT>
 static hipError_t launch_append_t(const QkvAppendParams &p, hipStream_t s) {
-    const int64_t threads = (int64_t)p.n * p.n_seqs * (p.n_heads + 2 * p.n_kv) * (p.head_dim / 8);
-    const int64_t blocks = (threads + kAppendThreads - 1) / kAppendThreads;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks), block(kAppendThreads);
     switch (p.head_dim) {
-    case 32: hipLaunchKernelGGL((qkv_append_kernel<IN, CT, 32>), grid, block, 0, s, p); break;
-    case 64: hipLaunchKernelGGL((qkv_append_kernel<IN, CT, 64>), grid, block, 0, s, p); break;
-    case 128: hipLaunchKernelGGL((qkv_append_kernel<IN, CT, 128>), grid, block, 0, s, p); break;
+    case 32: launch_append<IN, CT, 32>(p, s); break;
+    case 64: launch_append<IN, CT, 64>(p, s); break;
+    case 128: launch_append<IN, CT, 128>(p, s); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -26,6 +26,11 @@ __host__ __device__ inline int cache_row(int t, int max_seq_len, int sinks) { re
 __device__ __forceinline__ float q4_scale(uint32_t pair) { return (float)__builtin_bit_cast(half2_t, pair)[0]; }
 __device__ __forceinline__ float q4_lowest(uint32_t pair) { return (float)__builtin_bit_cast(half2_t, pair)[1]; }
 
+template <int kCtrl>
+__device__ __forceinline__ float quad_perm(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, false));
+}
+
 // Pair and codes of a group of 32 values held by four neighbouring lanes, eight consecutive ones each: the lane's codes; every lane
 // of the four gets the pair.
 __device__ __forceinline__ uint32_t q4_encode8(const float (&v)[8], uint32_t &pair) {
@@ -36,10 +41,10 @@ __device__ __forceinline__ uint32_t q4_encode8(const float (&v)[8], uint32_t &pa
         mx = fmaxf(mx, v[i]);
         odd += v[i] - v[i];
     }
-    mn = fminf(mn, __shfl_xor(mn, 1, 4));
-    mn = fminf(mn, __shfl_xor(mn, 2, 4));
-    mx = fmaxf(mx, __shfl_xor(mx, 1, 4));
-    mx = fmaxf(mx, __shfl_xor(mx, 2, 4));
+    mn = fminf(mn, quad_perm<kDppQuadPerm1032>(mn));
+    mn = fminf(mn, quad_perm<kDppQuadPerm2301>(mn));
+    mx = fmaxf(mx, quad_perm<kDppQuadPerm1032>(mx));
+    mx = fmaxf(mx, quad_perm<kDppQuadPerm2301>(mx));
     odd = group_sum<4>(odd);
     half_t low = to_f16(mn + 0.0f); // (zeros of either kind are positive: which of two zeros fminf gives is open)
     half_t scale = to_f16((mx - (float)low + 0.0f) / 15.0f);
@@ -52,8 +57,22 @@ __device__ __forceinline__ uint32_t q4_encode8(const float (&v)[8], uint32_t &pa
     pair = (uint32_t)__builtin_bit_cast(uint16_t, scale) | ((uint32_t)__builtin_bit_cast(uint16_t, low) << 16);
     const float s = (float)scale, l = (float)low;
     if (s > 0.0f) {
+        // (v - l) / s rounded to a whole number, by the reciprocal: within 2^-20 of the quotient up to 16, so only next to a tie is the quotient itself needed
+        const float inv = 1.0f / s;
+        bool tie = false;
+        float c[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) codes |= (uint32_t)fminf(fmaxf(rintf((v[i] - l) / s), 0.0f), 15.0f) << (4 * i);
+        for (int i = 0; i < 8; i++) {
+            const float t = (v[i] - l) * inv;
+            c[i] = rintf(t);
+            tie |= fabsf(fabsf(t - c[i]) - 0.5f) < 1e-5f;
+        }
+        if (tie) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) c[i] = rintf((v[i] - l) / s);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) codes |= (uint32_t)fminf(fmaxf(c[i], 0.0f), 15.0f) << (4 * i);
     }
     return codes;
 }

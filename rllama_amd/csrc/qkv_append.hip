@@ -16,62 +16,100 @@ namespace rlh {
 
 constexpr int kAppendThreads = 256;
 
-template <typename IN, typename CT, int HD>
+// eight floats at a 16-byte aligned address
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+    const float4_t a = *reinterpret_cast<const float4_t *>(p), b = *reinterpret_cast<const float4_t *>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        v[i] = a[i];
+        v[i + 4] = b[i];
+    }
+}
+
+// the value of lane i ^ kLanes / 2 of a head's kLanes lanes
+template <int kLanes>
+__device__ __forceinline__ float other_half(float v) {
+    const int x = __builtin_bit_cast(int, v);
+    if constexpr (kLanes == 16) return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, 0x128 /* row_ror:8 */, 0xf, 0xf, false));
+    else if constexpr (kLanes == 8) return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(x, 0x101f /* xor 4 */));
+    else return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, kDppQuadPerm2301, 0xf, 0xf, false));
+}
+
+// kTake: heads per thread, all of them loaded before the first is worked on.
+template <typename IN, typename CT, int HD, int kTake>
 __global__ __launch_bounds__(kAppendThreads) void qkv_append_kernel(QkvAppendParams p) {
     constexpr int kLanes = HD / 8, kUnits = kAppendThreads / kLanes;
     const int row = blockIdx.x, b = row / p.n, pos = p.start[b] + (row - b * p.n);
     const int dl = threadIdx.x % kLanes, slots = p.n_heads + 2 * p.n_kv;
-    const int first = blockIdx.y * kUnits + threadIdx.x / kLanes, stride = gridDim.y * kUnits;
+    const int first = blockIdx.y * (kUnits * kTake) + threadIdx.x / kLanes;
     const size_t q_row = (size_t)row * p.n_heads * HD + dl * 8;
     if (pos < 0) { // padding: zero queries, nothing in the cache
         const float zero[8] = {};
-        for (int slot = first; slot < p.n_heads; slot += stride) plane_store8<IN>(p.q, q_row + (size_t)slot * HD, zero);
+#pragma unroll
+        for (int u = 0; u < kTake; u++)
+            if (first + u * kUnits < p.n_heads) plane_store8<IN>(p.q, q_row + (size_t)(first + u * kUnits) * HD, zero);
         return;
     }
-    // the row's angles and the norms' weights, once for all heads that this thread takes
-    const float2 *turn = reinterpret_cast<const float2 *>(p.freqs) + (size_t)pos * (HD / 2) + (p.halves ? dl % (kLanes / 2) * 8 : dl * 4);
-    const bool second = dl >= kLanes / 2;
-    float2 angle[8];
+    float v[kTake][8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) angle[i] = i < 4 || p.halves ? turn[i] : make_float2(0.0f, 0.0f);
-    float qw[8], kw[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        qw[i] = p.q_norm ? p.q_norm[dl * 8 + i] : 1.0f;
-        kw[i] = p.k_norm ? p.k_norm[dl * 8 + i] : 1.0f;
+    for (int u = 0; u < kTake; u++) {
+        const int slot = min(first + u * kUnits, slots - 1); // (past the last head: read along, not stored)
+        plane_load8<IN>(p.qkv, ((size_t)row * slots + slot) * HD + dl * 8, v[u]);
     }
+    // the row's angles and the norms' weights, once for all heads that this thread takes
+    const float *turn = p.freqs + (size_t)pos * HD;
+    float angle[16], qw[8], kw[8];
+    const bool second = dl >= kLanes / 2;
+    if (p.halves) {
+        float lo[8], hi[8];
+        load8(turn + dl % (kLanes / 2) * 16, lo);
+        load8(turn + dl % (kLanes / 2) * 16 + 8, hi);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            angle[i] = lo[i];
+            angle[i + 8] = hi[i];
+        }
+    } else {
+        float lo[8];
+        load8(turn + dl * 8, lo);
+#pragma unroll
+        for (int i = 0; i < 8; i++) angle[i] = lo[i], angle[i + 8] = 0.0f;
+    }
+    if (p.q_norm) load8(p.q_norm + dl * 8, qw);
+    if (p.k_norm) load8(p.k_norm + dl * 8, kw);
     const size_t cache_at = (size_t)cache_row(pos, p.max_seq_len, p.sinks) * HD + dl * 8;
-    for (int slot = first; slot < slots; slot += stride) { // (the lanes of a head stay together)
-        float v[8];
-        plane_load8<IN>(p.qkv, ((size_t)row * slots + slot) * HD + dl * 8, v);
+#pragma unroll
+    for (int u = 0; u < kTake; u++) {
+        const int slot = first + u * kUnits; // (the lanes of a head stay together)
+        if (slot >= slots) break;
         const int kind = slot < p.n_heads ? 0 : slot < p.n_heads + p.n_kv ? 1 : 2; // query, key, value
         if (kind < 2) {
             if (kind == 0 ? p.q_norm != nullptr : p.k_norm != nullptr) {
                 float sq = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) sq = fmaf(v[i], v[i], sq);
+                for (int i = 0; i < 8; i++) sq = fmaf(v[u][i], v[u][i], sq);
                 const float r = 1.0f / sqrtf(group_sum<kLanes>(sq) / (float)HD + p.eps);
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = v[i] * r * (kind == 0 ? qw[i] : kw[i]);
+                for (int i = 0; i < 8; i++) v[u][i] = v[u][i] * r * (kind == 0 ? qw[i] : kw[i]);
             }
             if (p.halves) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float other = __shfl_xor(v[i], kLanes / 2, kLanes);
+                    const float other = other_half<kLanes>(v[u][i]);
                     float re, im;
-                    rope_pair(second ? other : v[i], second ? v[i] : other, angle[i], re, im);
-                    v[i] = second ? im : re;
+                    rope_pair(second ? other : v[u][i], second ? v[u][i] : other, make_float2(angle[2 * i], angle[2 * i + 1]), re, im);
+                    v[u][i] = second ? im : re;
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) rope_pair(v[i], v[i + 1], angle[i / 2], v[i], v[i + 1]);
+                for (int i = 0; i < 8; i += 2) rope_pair(v[u][i], v[u][i + 1], make_float2(angle[i], angle[i + 1]), v[u][i], v[u][i + 1]);
             }
         }
         if (kind == 0) {
-            plane_store8<IN>(p.q, q_row + (size_t)slot * HD, v);
+            plane_store8<IN>(p.q, q_row + (size_t)slot * HD, v[u]);
         } else {
             const int g = slot - p.n_heads - (kind == 2 ? p.n_kv : 0);
-            plane_store8<CT>(kind == 1 ? p.cache_k : p.cache_v, (size_t)(b * p.n_kv + g) * p.max_seq_len * HD + cache_at, v);
+            plane_store8<CT>(kind == 1 ? p.cache_k : p.cache_v, (size_t)(b * p.n_kv + g) * p.max_seq_len * HD + cache_at, v[u]);
         }
     }
 }
@@ -79,9 +117,11 @@ __global__ __launch_bounds__(kAppendThreads) void qkv_append_kernel(QkvAppendPar
 template <typename IN, typename CT, int HD>
 static void launch_append(const QkvAppendParams &p, hipStream_t s) {
     const int units = kAppendThreads * 8 / HD, slots = p.n_heads + 2 * p.n_kv, rows = p.n * p.n_seqs;
-    // Few rows: a workgroup for every `units` heads of a row, so that nothing waits.  Many rows: one per row, so that angles and weights are read once.
-    const int blocks = rows < 512 ? (slots + units - 1) / units : 1;
-    hipLaunchKernelGGL((qkv_append_kernel<IN, CT, HD>), dim3((unsigned)rows, (unsigned)blocks), dim3(kAppendThreads), 0, s, p);
+    // Few rows: a head per thread group, so that nothing waits.  Many rows: several, so that angles and weights are read once for them.
+    const int take = rows < 512 ? 1 : 3;
+    const dim3 grid((unsigned)rows, (unsigned)((slots + units * take - 1) / (units * take)));
+    if (take == 1) hipLaunchKernelGGL((qkv_append_kernel<IN, CT, HD, 1>), grid, dim3(kAppendThreads), 0, s, p);
+    else hipLaunchKernelGGL((qkv_append_kernel<IN, CT, HD, 3>), grid, dim3(kAppendThreads), 0, s, p);
 }
 
 template <typename IN, typename CT>

@@ -44,11 +44,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParam
     const AttnWindowParams &p = pp.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
-    // late rows see more keys and start first; a unit's workgroups are a multiple of its number apart, on one XCD where the units are a multiple of eight
+    // a unit's workgroups are a multiple of the number of units apart: on one XCD where that is a multiple of eight
     const int unit = blockIdx.x;
     const int b = unit / p.n_kv, g = unit - b * p.n_kv;
     const int group = p.n_heads / p.n_kv, rows = p.n * group, start = p.start[b];
-    const int r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * kRows, r1 = min(rows, r0 + kRows) - 1;
+    const int r0 = ((int)blockIdx.y < pp.descend ? (int)gridDim.y - 1 - (int)blockIdx.y : (int)blockIdx.y - pp.descend) * kRows, r1 = min(rows, r0 + kRows) - 1;
     const int p0 = max(0, start + r0 / group), p1 = start + r1 / group;
     // this wavefront's rows, and this lane's
     const int w0 = r0 + wave * 32, w1 = min(r1, w0 + 31);
@@ -407,6 +407,10 @@ hipError_t launch_attn_tiles(const AttnWindowParams &a, int compute_units, float
     p.a = a;
     p.ws = ws;
     cut_tiles(a, compute_units, &p.pieces, &p.piece_steps);
+    // Late rows see more keys and start first.  Where every workgroup is resident from the start, two to a compute unit, the second ones come in rising order, so that a
+    // unit's two have about the same sum (2048 rows of 32 heads: 58.6 -> 45 us).
+    const int tiles = (int)(((int64_t)a.n * (a.n_heads / a.n_kv) + kAtRows - 1) / kAtRows), units = a.n_seqs * a.n_kv;
+    p.descend = p.pieces == 1 && tiles * units <= 2 * compute_units ? std::min(tiles, (compute_units + units - 1) / units) : tiles;
     switch (a.head_dim * 2 + (a.cache == kPlaneQ4)) {
     case 64: launch_tiles<half_t, 32>(p, s); break;
     case 65: launch_tiles<Quant4, 32>(p, s); break;

@@ -14,8 +14,9 @@
 // transposes them in registers with byte permutes, so cached rows go from memory into registers and nowhere else: no LDS, no barrier in
 // the loop.  Tile e of O^T is made of the dims hd / 16 * m + e (m = 0 .. 15).
 //
-// Two arithmetics.  16 bits: f16 operands, v_mfma_f32_16x16x32_f16; weights are rounded to f16, as are values of 4 bits (each half a
-// unit in the eleventh bit, and neither adds up over a text).  32 bits: everything in f32 through v_mfma_f32_16x16x4_f32; also taken where f16
+// Two arithmetics.  16 bits: f16 operands, v_mfma_f32_16x16x32_f16; the weights are rounded to f16 (half a unit in the eleventh bit each, which does not add up
+// over a text).  Values of 4 bits are not: a value is code * (upper part of the scale) + code * (rest) + lowest, two products that f16 holds exactly and a
+// term that is the same for 32 dims, and each goes through the matrix cores by itself.  32 bits: everything in f32 through v_mfma_f32_16x16x4_f32; also taken where f16
 // queries meet an f32 cache, whose values f16 may not hold.
 //
 // A text is cut into pieces when there are few rows: every workgroup leaves its (m, sum, O) in work memory and a second launch joins them.
@@ -78,6 +79,7 @@ struct Step;
 template <typename CT, int HD>
 struct Step<half_t, CT, HD> {
     static constexpr int kPositions = 32;
+    static constexpr bool kLowSums = std::is_same_v<CT, Quant4>;
     static constexpr int kTiles = 2;            // of 16 positions
     static constexpr int kKs = HD / 32;         // MFMAs per score tile
     static constexpr int kDims = HD / 16;       // neighbouring dims of V per lane = tiles of O^T
@@ -85,6 +87,10 @@ struct Step<half_t, CT, HD> {
     static constexpr int kBits = kElementBits<CT>;
     struct Queries {
         half8_t q[kKs];
+        half8_t sums; // 4 bits: the sum of the lane's dims of q in two f16 parts (the term of the lowest values)
+    };
+    struct Sums { // 4 bits: the lowest values' part of O^T, row m for all dims kDims * m + e
+        float4_t low;
     };
     uint32_t k[kTiles][kQ4 ? HD / 32 : HD / 8 /* words: a quarter of a row */];
     uint32_t kp[kTiles];
@@ -101,6 +107,15 @@ struct Step<half_t, CT, HD> {
                 const int d = kQ4 ? (i >> 1) + 4 * (i & 1) : i;
                 to.q[c][i] = (half_t)(float)row[h * (HD / 4) + 8 * c + d];
             }
+        }
+        if constexpr (kQ4) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 4; i++) sum += (float)row[h * (HD / 4) + i];
+#pragma unroll
+            for (int i = 0; i < 8; i++) to.sums[i] = (half_t)0.0f;
+            to.sums[0] = (half_t)sum;
+            to.sums[1] = (half_t)(sum - (float)to.sums[0]);
         }
     }
     __device__ void load(buffer_t ck, buffer_t ckp, buffer_t cv, buffer_t cvp, int lane) {
@@ -122,34 +137,49 @@ struct Step<half_t, CT, HD> {
         }
     }
     __device__ void scores(const Queries &of, const Q4Bits &bits, float4_t (&s)[kTiles]) const {
+        const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (kQ4) {
+            // codes times either part of the scale, exactly, and the lowest value times the sum of q over the lane's dims: four chains of products
+            static_assert(kTiles == 2, "two tiles");
+            const Q4Scale scale0(perm(kp[0], kp[0], kLoHalves)), scale1(perm(kp[1], kp[1], kLoHalves));
+            auto low_term = [&](uint32_t pair) {
+                half8_t a = {};
+                a[0] = a[1] = __builtin_bit_cast(half2_t, pair)[1];
+                return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, of.sums, zero, 0, 0, 0);
+            };
+            float4_t s0 = zero, s1 = zero, rest0 = low_term(kp[0]), rest1 = low_term(kp[1]);
+            auto add = [&](float4_t &s, float4_t &rest, const Q4Scale &scale, uint32_t word, const half8_t &q) {
+                half2_t x[4];
+                q4_codes_f16(bits, word, x);
+                uint4_t hi, lo;
 #pragma unroll
-        for (int t = 0; t < kTiles; t++) {
-            s[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            half2_t scale, low;
-            if constexpr (kQ4) {
-                scale = __builtin_bit_cast(half2_t, perm(kp[t], kp[t], kLoHalves));
-                low = __builtin_bit_cast(half2_t, perm(kp[t], kp[t], kHiHalves));
-            }
+                for (int i = 0; i < 4; i++) {
+                    hi[i] = __builtin_bit_cast(uint32_t, x[i] * scale.hi);
+                    lo[i] = __builtin_bit_cast(uint32_t, x[i] * scale.lo);
+                }
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, hi), q, s, 0, 0, 0);
+                rest = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, lo), q, rest, 0, 0, 0);
+            };
 #pragma unroll
             for (int c = 0; c < kKs; c++) {
-                half8_t a;
-                if constexpr (kQ4) {
-                    half2_t x[4];
-                    q4_pairs_f16(bits, k[t][c], scale, low, x);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        a[2 * i] = x[i][0];
-                        a[2 * i + 1] = x[i][1];
-                    }
-                } else {
-                    a = __builtin_bit_cast(half8_t, uint4_t{k[t][4 * c], k[t][4 * c + 1], k[t][4 * c + 2], k[t][4 * c + 3]});
-                }
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, of.q[c], s[t], 0, 0, 0);
+                add(s0, rest0, scale0, k[0][c], of.q[c]);
+                add(s1, rest1, scale1, k[1][c], of.q[c]);
             }
+            s[0] = s0 + rest0;
+            s[1] = s1 + rest1;
+        } else {
+#pragma unroll
+            for (int t = 0; t < kTiles; t++) s[t] = zero;
+#pragma unroll
+            for (int c = 0; c < kKs; c++)
+#pragma unroll
+                for (int t = 0; t < kTiles; t++)
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, uint4_t{k[t][4 * c], k[t][4 * c + 1], k[t][4 * c + 2], k[t][4 * c + 3]}), of.q[c],
+                                                                  s[t], 0, 0, 0);
         }
     }
     // w[t][i]: weights of positions 16 t + 4 h + i
-    __device__ void values(const float4_t (&w)[kTiles], const Q4Bits &bits, float4_t (&o)[kDims]) const {
+    __device__ void values(const float4_t (&w)[kTiles], const Q4Bits &bits, float4_t (&o)[kDims], Sums &sums) const {
         half8_t b;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -159,21 +189,32 @@ struct Step<half_t, CT, HD> {
         if constexpr (kQ4) {
             // positions two by two: the codes of dims 0 .. 3 of both in one word, those of dims 4 .. 7 in another, and each nibble of the pair
             // becomes a pair (first position, second position) of one dim
-            uint32_t x[kDims][4];
+            uint4_t low;
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const half2_t scale = __builtin_bit_cast(half2_t, perm(vp[j + 1], vp[j], kLoHalves)), low = __builtin_bit_cast(half2_t, perm(vp[j + 1], vp[j], kHiHalves));
+            for (int j = 0; j < 4; j++) low[j] = perm(vp[2 * j + 1], vp[2 * j], kHiHalves);
+            sums.low = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, low), b, sums.low, 0, 0, 0);
+            constexpr int kPart = kDims < 4 ? kDims : 4;
 #pragma unroll
-                for (int part = 0; part < (kDims + 3) / 4; part++) {
+            for (int part = 0; part < kDims / kPart; part++) {
+                uint4_t hi[kPart], lo[kPart];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const Q4Scale scale(perm(vp[2 * j + 1], vp[2 * j], kLoHalves));
                     half2_t y[4];
-                    q4_pairs_f16(bits, perm(v[j + 1][0], v[j][0], part ? kHiHalves : kLoHalves), scale, low, y);
+                    q4_codes_f16(bits, perm(v[2 * j + 1][0], v[2 * j][0], part ? kHiHalves : kLoHalves), y);
 #pragma unroll
-                    for (int i = 0; i < (kDims < 4 ? kDims : 4); i++) x[4 * part + i][j / 2] = __builtin_bit_cast(uint32_t, y[i]);
+                    for (int i = 0; i < kPart; i++) {
+                        hi[i][j] = __builtin_bit_cast(uint32_t, y[i] * scale.hi);
+                        lo[i][j] = __builtin_bit_cast(uint32_t, y[i] * scale.lo);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kPart; i++) {
+                    float4_t &to = o[part * kPart + i];
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, hi[i]), b, to, 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, lo[i]), b, to, 0, 0, 0);
                 }
             }
-#pragma unroll
-            for (int e = 0; e < kDims; e++)
-                o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, uint4_t{x[e][0], x[e][1], x[e][2], x[e][3]}), b, o[e], 0, 0, 0);
         } else {
 #pragma unroll
             for (int e = 0; e < kDims; e++) {
@@ -204,6 +245,7 @@ struct Step<half_t, CT, HD> {
 template <typename CT, int HD>
 struct Step<float, CT, HD> {
     static constexpr int kPositions = 16;
+    static constexpr bool kLowSums = false;
     static constexpr int kTiles = 1;
     static constexpr int kDims = HD / 16;
     static constexpr bool kQ4 = std::is_same_v<CT, Quant4>;
@@ -211,6 +253,9 @@ struct Step<float, CT, HD> {
     static constexpr int kKWords = HD / 4 / kPerWord, kVWords = kQ4 ? 1 : kDims / kPerWord;
     struct Queries {
         float q[HD / 4];
+    };
+    struct Sums {
+        float4_t low; // (of the f16 form)
     };
     // as the cache holds them, so that a load need not have arrived before the next one is issued
     uint32_t k[kKWords], kp, v[4][kVWords], vp[4];
@@ -246,7 +291,7 @@ struct Step<float, CT, HD> {
 #pragma unroll
         for (int i = 0; i < HD / 4; i++) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(value(k, kp, i), of.q[i], s[0], 0, 0, 0);
     }
-    __device__ void values(const float4_t (&w)[kTiles], const Q4Bits &bits, float4_t (&o)[kDims]) const {
+    __device__ void values(const float4_t (&w)[kTiles], const Q4Bits &bits, float4_t (&o)[kDims], Sums &sums) const {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -297,6 +342,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
     float4_t o[kDims];
 #pragma unroll
     for (int e = 0; e < kDims; e++) o[e] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    typename St::Sums sums{float4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 
     const size_t plane = (size_t)unit * p.max_seq_len;
     const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
@@ -361,6 +407,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
             l_run *= alpha;
 #pragma unroll
             for (int e = 0; e < kDims; e++) o[e] *= alpha;
+            if constexpr (St::kLowSums) sums.low *= alpha;
         }
         const float mc = m_run > -INFINITY ? m_run * c2 : 0.0f;
         float sum = 0.0f;
@@ -373,7 +420,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
             }
         l_run += sum;
         if constexpr (!decltype(slow)::value) {
-            st.values(w, bits, o);
+            st.values(w, bits, o, sums);
         } else {
 #pragma unroll
             for (int t = 0; t < kTiles; t++)
@@ -394,23 +441,13 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
                 }
         }
     };
-    // two sets of operands: a step's are on their way while the one before is worked on
+    // (The other wavefronts cover a step's wait for memory: a second set of operands, loaded ahead, gained nothing at any length and cost 2 to 8 % in f32 for
+    // its registers.)
     const int s_end = min(span.steps, (piece + 1) * pp.piece_steps), s_first = piece * pp.piece_steps + wave;
-    {
-        St even, odd;
-        int s = s_first;
-        if (s < s_end) load(even, s);
-        while (s < s_end) {
-            if (s + kAwWaves < s_end) load(odd, s + kAwWaves);
-            __builtin_amdgcn_sched_barrier(0);
-            consume(even, s, std::false_type{});
-            s += kAwWaves;
-            if (s >= s_end) break;
-            if (s + kAwWaves < s_end) load(even, s + kAwWaves);
-            __builtin_amdgcn_sched_barrier(0);
-            consume(odd, s, std::false_type{});
-            s += kAwWaves;
-        }
+    for (int s = s_first; s < s_end; s += kAwWaves) {
+        St st;
+        load(st, s);
+        consume(st, s, std::false_type{});
     }
     if (skipped) {
         // Steps that hold a value that is not finite and that some row may not see: in the product its weight 0 would make a NaN of it.
@@ -432,7 +469,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
 #pragma unroll
     for (int x = 0; x < 4; x++)
 #pragma unroll
-        for (int e = 0; e < kDims; e++) so[wave][m][(4 * h + x) * kDims + e] = o[e][x];
+        for (int e = 0; e < kDims; e++) so[wave][m][(4 * h + x) * kDims + e] = St::kLowSums ? o[e][x] + sums.low[x] : o[e][x];
     __syncthreads();
     // thread: row tid / 32, dims HD / 32 of it
     constexpr int kPer = HD / 32;

@@ -46,18 +46,28 @@ struct Q4Bits {
         asm("" : "+v"(exp_odd));
     }
 };
-// eight codes of a word as f16 numbers lowest + code * scale: pairs (0, 4), (1, 5), (2, 6), (3, 7).  1024 + c is the f16 number with c in its
-// last four bits (0x6400 | c), 64 + c the one with c four bits further up (0x5400 | 16 c), which saves half of the shifts.  The differences to
-// 1024 and 64 are exact, the multiply-add rounds once.
-__device__ __forceinline__ void q4_pairs_f16(const Q4Bits &bits, uint32_t w, half2_t scale, half2_t low, half2_t (&out)[4]) {
+// eight codes of a word as f16 numbers: pairs (0, 4), (1, 5), (2, 6), (3, 7).  1024 + c is the f16 number with c in its last four bits
+// (0x6400 | c), 64 + c the one with c four bits further up (0x5400 | 16 c), which saves half of the shifts.  The differences are exact.
+__device__ __forceinline__ void q4_codes_f16(const Q4Bits &bits, uint32_t w, half2_t (&out)[4]) {
     const half2_t k1024 = {(half_t)1024.0f, (half_t)1024.0f}, k64 = {(half_t)64.0f, (half_t)64.0f};
 #pragma unroll
     for (int s = 0; s < 2; s++) {
         const uint32_t x = w >> (8 * s);
-        out[2 * s] = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (x & bits.even) | bits.exp_even) - k1024, scale, low);
-        out[2 * s + 1] = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (x & bits.odd) | bits.exp_odd) - k64, scale, low);
+        out[2 * s] = __builtin_bit_cast(half2_t, (x & bits.even) | bits.exp_even) - k1024;
+        out[2 * s + 1] = __builtin_bit_cast(half2_t, (x & bits.odd) | bits.exp_odd) - k64;
     }
 }
+// the values, lowest + code * scale, each rounded once
+__device__ __forceinline__ void q4_pairs_f16(const Q4Bits &bits, uint32_t w, half2_t scale, half2_t low, half2_t (&out)[4]) {
+    q4_codes_f16(bits, w, out);
+#pragma unroll
+    for (int i = 0; i < 4; i++) out[i] = __builtin_elementwise_fma(out[i], scale, low);
+}
+// A scale as a sum of its upper seven bits and the rest: products of either part with a code have at most eleven bits, so f16 holds them exactly.
+struct Q4Scale {
+    half2_t hi, lo;
+    __device__ explicit Q4Scale(uint32_t scales) : hi(__builtin_bit_cast(half2_t, scales & 0xfff0fff0u)), lo(__builtin_bit_cast(half2_t, scales) - hi) {}
+};
 // whether the values of a group are all finite as f16 numbers
 __device__ __forceinline__ bool q4_finite_f16(uint32_t pair) {
     const half2_t x = __builtin_bit_cast(half2_t, pair);
@@ -82,6 +92,7 @@ struct AttnCutParams {
     AttnWindowParams a;
     float *ws;
     int pieces, piece_steps; // pieces of `piece_steps` steps, at most `pieces` of them
+    int descend;             // attn_tiles_kernel: so many tiles of rows are started from the last one downwards, the others from the first one upwards
 };
 constexpr int kMaxPieces = 64;
 

@@ -1,9 +1,13 @@
 // attn_tiles.hip -- rlh_attn_window for many rows: f16 arithmetic, tiles of keys staged in LDS.
 //
-// Workgroup = kWaves wavefronts of 32 rows each, all on one key and value head (row r = row r / group of the sequence, head r % group of the
-// group); the keys they look at pass by in tiles of 64, K and V [64 x hd] as f16 in two LDS stages: the next tile is on its way while this one is
-// used, one barrier per tile.  f16 caches go from memory straight into LDS; of 4-bit caches a thread takes whole groups of 32 codes, converts
-// them in registers and writes 64 bytes, so a code is converted once per workgroup and not once per wavefront.
+// Workgroup = four row groups of 32 rows on one key and value head (row r = row r / group of the sequence, head r % group of the group), a wavefront for each,
+// or two of them that share the keys.  The keys the rows look at pass by in tiles of 64 per wavefront, K and V as f16 in two LDS stages: the next tile is on
+// its way while this one is used, one barrier per tile.  f16 caches go from memory straight into LDS; of 4-bit caches a thread takes whole groups of 32
+// codes, converts them in registers and writes 64 bytes, so a code is converted once per workgroup and not once per wavefront.
+//
+// Tiles that every row of the wavefront sees whole, in the middle of a run of rows that lie side by side in the cache, go through a loop of their own with
+// nothing but running addresses between the products.  (2048 rows behind 2000 positions, 32 heads of 128 on 8: 133 us with the place of every tile and its
+// masks worked out anew, 119 so.)
 //
 // Both products run transposed through v_mfma_f32_32x32x16_f16, so that a row is a lane pair's column of both results:
 //   S^T [key x row] = K . q^T,   O^T [dim x row] += V^T . W
@@ -25,33 +29,47 @@ typedef __attribute__((ext_vector_type(16))) float float16_t;
 typedef __attribute__((ext_vector_type(4))) _Float16 half4_t;
 typedef __attribute__((ext_vector_type(4))) short short4_t;
 
-constexpr int kAtKeys = 64;
+// The value of lane i ^ 32.  (Written out: of the builtin's two results the compiler kept one where both operands are the same value.)
+__device__ __forceinline__ float other_half_lane(float v) {
+    float a = v, b = v; // afterwards lanes 32 .. 63 of a hold lanes 0 .. 31 of v, and lanes 0 .. 31 of b hold lanes 32 .. 63
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    return (threadIdx.x & 32) ? a : b;
+}
 
-template <typename CT, int HD, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParams pp) {
+constexpr int kAtGroups = 4; // of 32 rows
+constexpr int kAtRows = 32 * kAtGroups;
+
+// kShares: wavefronts per row group
+template <typename CT, int HD, int kShares>
+__global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(AttnCutParams pp) {
     constexpr bool kQ4 = std::is_same_v<CT, Quant4>;
-    constexpr int kRows = 32 * kWaves;
+    constexpr int kWaves = kAtGroups * kShares, kRows = kAtRows;
+    constexpr int kAtKeys = 64 * kShares;        // per tile
     constexpr int kKS = HD / 16;                 // MFMA steps over the head dimension
     constexpr int kDT = HD / 32;                 // 32-dim tiles of O^T
     constexpr int kPieces = HD / 8;              // 16-byte pieces per row
     constexpr int kRowBytes = HD * 2;
-    constexpr int kTileBytes = kAtKeys * kRowBytes;
+    constexpr int kTileBytes = kAtKeys * kRowBytes; // of K or of V
     constexpr int kStageBytes = 2 * kTileBytes;
     constexpr int kOutRow = HD + 8;              // padded row of the output tile, halves
-    constexpr int kLdsBytes = 2 * kStageBytes > kRows * kOutRow * 2 ? 2 * kStageBytes : kRows * kOutRow * 2;
+    constexpr int kJoinFloats = (HD / 2 + 2) * 64; // of one wavefront: O, m and sum
+    constexpr int kEndBytes = kShares > 1 ? kAtGroups * kJoinFloats * 4 : kAtGroups * 32 * kOutRow * 2;
+    constexpr int kLdsBytes = 2 * kStageBytes > kEndBytes ? 2 * kStageBytes : kEndBytes;
+    static_assert(32 * kOutRow * 2 <= kJoinFloats * 4, "a row group's output goes where its join was");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
 
     const AttnWindowParams &p = pp.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
-    // a unit's workgroups are a multiple of the number of units apart: on one XCD where that is a multiple of eight
+    const int rg = wave % kAtGroups, kh = wave / kAtGroups; // row group, half of the keys
+    // late rows see more keys and start first; a unit's workgroups are a multiple of the number of units apart, on one XCD where that is a multiple of eight
     const int unit = blockIdx.x;
     const int b = unit / p.n_kv, g = unit - b * p.n_kv;
     const int group = p.n_heads / p.n_kv, rows = p.n * group, start = p.start[b];
-    const int r0 = ((int)blockIdx.y < pp.descend ? (int)gridDim.y - 1 - (int)blockIdx.y : (int)blockIdx.y - pp.descend) * kRows, r1 = min(rows, r0 + kRows) - 1;
+    const int r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * kRows, r1 = min(rows, r0 + kRows) - 1;
     const int p0 = max(0, start + r0 / group), p1 = start + r1 / group;
     // this wavefront's rows, and this lane's
-    const int w0 = r0 + wave * 32, w1 = min(r1, w0 + 31);
+    const int w0 = r0 + rg * 32, w1 = min(r1, w0 + 31);
     const int wp0 = start + w0 / group, wp1 = w1 < w0 ? -1 : start + w1 / group;
     const int my_r = min(w0 + col, r1), my_i = my_r / group;
     const int my_p = w0 + col <= r1 ? start + my_i : -1;
@@ -75,9 +93,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParam
 
     Span span = span_of<kAtKeys>(p0, p1, p.window, p.sinks, p.max_seq_len);
     if (p1 < 0) span.steps = 0;
-    const int n_pieces = (span.steps + pp.piece_steps - 1) / pp.piece_steps, piece = blockIdx.z;
+    // (texts are cut into pieces with two wavefronts per row group only)
+    const int n_pieces = kShares > 1 ? (span.steps + pp.piece_steps - 1) / pp.piece_steps : 1, piece = kShares > 1 ? blockIdx.z : 0;
     if (piece >= max(1, n_pieces)) return;
-    const int s_first = piece * pp.piece_steps, s_end = min(span.steps, s_first + pp.piece_steps);
+    const int s_first = kShares > 1 ? piece * pp.piece_steps : 0, s_end = kShares > 1 ? min(span.steps, s_first + pp.piece_steps) : span.steps;
     const size_t plane = (size_t)unit * p.max_seq_len;
     const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
     const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
@@ -96,19 +115,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParam
 
     // ---- staging
     constexpr int kIssues = kTileBytes / (kWaves * 1024) > 0 ? kTileBytes / (kWaves * 1024) : 1; // f16: wavefront-wide 1 KiB loads per tile of K (and of V)
-    constexpr int kGroups = 2 * kAtKeys * HD / 32, kItems = kGroups / (64 * kWaves) > 0 ? kGroups / (64 * kWaves) : 1; // 4 bits: groups per thread and tile
+    constexpr int kIssueRows = kWaves * 64 / kPieces;        // rows from one to the next: a multiple of what the permutations repeat after
+    constexpr int kGroups = 2 * kAtKeys * HD / 32, kItems = kGroups / (64 * kWaves) > 0 ? kGroups / (64 * kWaves) : 1; // 4 bits: groups per tile, and per thread
+    static_assert(kTileBytes >= kWaves * 1024 || kIssues == 1, "a tile's shares");
+    const int my_row = (wave * 64 + lane) / kPieces, my_piece = lane % kPieces;
+    const unsigned k_from = (my_piece ^ k_swz(my_row)) << 4, v_from = (my_piece ^ v_swz(my_row)) << 4; // within the row
     uint32_t codes[kQ4 ? kItems : 1][4], pairs[kQ4 ? kItems : 1];
-    auto fetch = [&](int s, unsigned stage) { // tile s: f16 on its way to LDS, codes on their way to registers
-        const Place at = place_of(s);
-        const int here = min(kAtKeys, at.last - at.t0 + 1);
-        const size_t row = plane + at.row;
+    // `here` rows from plane row `row` on: f16 on their way to a stage, codes on their way to registers
+    auto fetch = [&](size_t row, int here, unsigned stage) __attribute__((always_inline)) {
         if constexpr (kQ4) {
             const buffer_t k = buffer_of(p.cache_k.data, row * (HD / 2), here * (HD / 2)), kp = buffer_of(p.cache_k.pairs, row * (HD / 8), here * (HD / 8));
             const buffer_t v = buffer_of(p.cache_v.data, row * (HD / 2), here * (HD / 2)), vp = buffer_of(p.cache_v.pairs, row * (HD / 8), here * (HD / 8));
 #pragma unroll
             for (int i = 0; i < kItems; i++) {
                 const int item = i * 64 * kWaves + tid, at_group = item % (kGroups / 2); // row at_group / (HD / 32), group at_group % (HD / 32)
-                const bool is_v = __builtin_amdgcn_readfirstlane(item / (kGroups / 2)) & 1;
+                const bool is_v = kItems > 1 ? i >= kItems / 2 : (__builtin_amdgcn_readfirstlane(item / (kGroups / 2)) & 1);
                 const auto x = is_v ? __builtin_amdgcn_raw_buffer_load_b128(v, at_group * 16, 0, 0) : __builtin_amdgcn_raw_buffer_load_b128(k, at_group * 16, 0, 0);
 #pragma unroll
                 for (int w = 0; w < 4; w++) codes[i][w] = x[w];
@@ -116,22 +137,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParam
             }
         } else {
             const half_t *k = reinterpret_cast<const half_t *>(p.cache_k.data) + row * HD, *v = reinterpret_cast<const half_t *>(p.cache_v.data) + row * HD;
+            if (kTileBytes < kWaves * 1024 && wave >= kTileBytes / 1024) return;
 #pragma unroll
             for (int i = 0; i < kIssues; i++) {
-                const int L = (i * kWaves + wave) * 64 + lane, r = L / kPieces, c = L % kPieces;
-                const unsigned from = (unsigned)min(r, here - 1) * kRowBytes; // keys past the last one are masked below
+                const unsigned from = (unsigned)min(my_row + i * kIssueRows, here - 1) * kRowBytes; // keys past the last one are masked below
                 const unsigned to = lds_base + stage * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u;
-                dma16_base(k, from + ((c ^ k_swz(r)) << 4), to);
-                dma16_base(v, from + ((c ^ v_swz(r)) << 4), to + kTileBytes);
+                dma16_base(k, from + k_from, to);
+                dma16_base(v, from + v_from, to + kTileBytes);
             }
         }
     };
     const Q4Bits bits;
-    auto place = [&](unsigned stage) { // 4 bits: the fetched codes as f16 into LDS
+    auto place = [&](unsigned stage) __attribute__((always_inline)) { // 4 bits: the fetched codes as f16 into LDS
         if constexpr (kQ4) {
+            int me = tid;
+            asm volatile("" : "+v"(me)); // the addresses are formed here, not kept in registers over the products
 #pragma unroll
             for (int i = 0; i < kItems; i++) {
-                const int item = i * 64 * kWaves + tid;
+                const int item = i * 64 * kWaves + me;
                 if (kGroups < 64 * kWaves && item >= kGroups) break;
                 const int at_group = item % (kGroups / 2), r = at_group / (HD / 32), c0 = at_group % (HD / 32) * 4;
                 const bool is_v = item >= kGroups / 2;
@@ -152,112 +175,160 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParam
     };
 
     auto sees = [&](int at, int last) { return (bool)((int)(at <= min(my_p, last)) & ((int)(at >= my_low) | (int)(at < p.sinks))); };
-    // every row of this wavefront that is no padding sees the whole tile / none sees any of it
-    auto whole_tile = [&](const Place &at) { return at.t0 + kAtKeys - 1 <= min(at.last, max(0, wp0)) && (at.front || p.window == 0 || at.t0 > wp1 - p.window); };
-    auto unseen_tile = [&](const Place &at) {
-        const int end = min(at.last, at.t0 + kAtKeys - 1);
-        return at.t0 > wp1 || (p.window > 0 && !at.front && end <= max(0, wp0) - p.window && at.t0 >= p.sinks);
+    // of this wavefront's half of a tile: every row that is no padding sees all of it / none sees any of it
+    auto whole_half = [&](const Place &at) {
+        const int t0 = at.t0 + kh * 64;
+        return t0 + 63 <= min(at.last, max(0, wp0)) && (at.front || p.window == 0 || t0 > wp1 - p.window);
+    };
+    auto unseen_half = [&](const Place &at) {
+        const int t0 = at.t0 + kh * 64, end = min(at.last, t0 + 63);
+        return t0 > min(wp1, at.last) || (p.window > 0 && !at.front && end <= max(0, wp0) - p.window && t0 >= p.sinks);
     };
     bool skipped = false;
 
-    // One tile; `stage` is a compile-time constant at both call sites, so that every LDS address is the lane's base plus an immediate.
-    auto tile_step = [&](int s, auto stage) {
-        wait_vmcnt<0>(); // this wavefront's part of the tile has landed
-        __syncthreads(); // ... and everybody's; everybody is done with the tile before, whose stage is filled next
-        const bool more = s + 1 < s_end;
-        if (more) fetch(s + 1, 1 - decltype(stage)::value);
-        const Place at = place_of(s);
-        const unsigned char *lds_k = lds + decltype(stage)::value * kStageBytes, *lds_v = lds_k + kTileBytes;
-        if (!unseen_tile(at)) {
-            const bool whole = whole_tile(at);
-            bool odd = false;
-            if (!whole) { // is every value of V finite?
+    // ---- one tile: both products and the softmax of this wavefront's 64 keys
+    const int v_row = half * 4 + ((lane & 15) >> 2);               // of the first run of four keys; the second one is 8 further
+    const int v_piece = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1); // + 4 d
+    auto work = [&](unsigned stage, int t0, int last, auto whole) __attribute__((always_inline)) {
+        const unsigned char *lds_k = lds + stage * kStageBytes + kh * (64 * kRowBytes), *lds_v = lds_k + kTileBytes;
+        // S^T: the two 32-key products side by side, K three steps ahead of them
+        float16_t w[2];
 #pragma unroll
-                for (int i = 0; i < kTileBytes / 1024; i++) {
-                    const uint4_t x = *reinterpret_cast<const uint4_t *>(lds_v + i * 1024 + lane * 16);
+        for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        odd |= ((x[w] & 0x7c000000u) == 0x7c000000u);
-                        odd |= ((x[w] & 0x7c00u) == 0x7c00u);
-                    }
-                }
-                odd = __any(odd);
+            for (int v = 0; v < 16; v++) w[t][v] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < kKS; ks++)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+                w[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t *>(lds_k + (t * 32 + col) * kRowBytes + (((ks * 2 + half) ^ k_swz(col)) << 4)), q[ks],
+                                                              w[t], 0, 0, 0);
+        constexpr int kLead = 4;
+        __builtin_amdgcn_sched_group_barrier(0x100, kLead, 0); // LDS reads
+#pragma unroll
+        for (int i = 0; i < (2 * kKS - kLead) / 2; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); // MFMAs
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, kLead, 0);
+        if constexpr (!decltype(whole)::value) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) w[t][v] = sees(t0 + t * 32 + (v >> 2) * 8 + half * 4 + (v & 3), last) ? w[t][v] : -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) top = fmaxf(top, w[t][v]);
+        top = fmaxf(top, other_half_lane(top));
+        // the reference point follows the maximum when some row's has grown by more than 2^8: weights stay below 2^8
+        const float m_new = fmaxf(m_run, top);
+        if (__any((m_new - m_run) * c2 > 8.0f)) {
+            const float alpha = m_run > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 0.0f;
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int d = 0; d < kDT; d++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) o[d][v] *= alpha;
+        }
+        const float mc = m_run > -INFINITY ? m_run * c2 : 0.0f;
+        // O^T += V^T . W, 16 keys at a time: the next 16 keys' weights are formed and their V read between the products of these
+        auto weights = [&](int sl) {
+            half8_t h;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(w[sl / 2][(sl % 2) * 8 + i], c2, -mc));
+                sum += e;
+                h[i] = (half_t)e;
             }
-            if (odd) {
-                skipped = true;
-            } else {
-                float16_t w[2];
+            l_run += sum;
+            return h;
+        };
+        auto read_v = [&](int sl, int d) {
+            const unsigned char *from = lds_v + (sl * 16 + v_row) * kRowBytes + (((d * 4 + v_piece) ^ v_swz(v_row)) << 4) + (lane & 1) * 8;
+            typedef __attribute__((address_space(3))) short4_t *lds4;
+            const half4_t a0 = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__attribute__((address_space(3))) void *)from));
+            const half4_t a1 = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__attribute__((address_space(3))) void *)(from + 8 * kRowBytes)));
+            return __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        half8_t v_frag[kDT];
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
+        for (int d = 0; d < kDT; d++) v_frag[d] = read_v(0, d);
+        half8_t wh = weights(0);
 #pragma unroll
-                    for (int v = 0; v < 16; v++) w[t][v] = 0.0f;
-                    const int row = t * 32 + col;
-                    const unsigned char *from = lds_k + row * kRowBytes;
+        for (int sl = 0; sl < 4; sl++) {
 #pragma unroll
-                    for (int ks = 0; ks < kKS; ks++)
-                        w[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t *>(from + (((ks * 2 + half) ^ k_swz(row)) << 4)), q[ks], w[t], 0, 0, 0);
-                }
-                if (!whole) {
+            for (int d = 0; d < kDT; d++) {
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag[d], wh, o[d], 0, 0, 0);
+                if (sl < 3) v_frag[d] = read_v(sl + 1, d);
+            }
+            if (sl < 3) wh = weights(sl + 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * kDT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, 32, 0); // the first weights
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
+        for (int sl = 0; sl < 3; sl++) {
 #pragma unroll
-                        for (int v = 0; v < 16; v++) w[t][v] = sees(at.t0 + t * 32 + (v >> 2) * 8 + half * 4 + (v & 3), at.last) ? w[t][v] : -INFINITY;
-                }
-                float top = -INFINITY;
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int v = 0; v < 16; v++) top = fmaxf(top, w[t][v]);
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                // the reference point follows the maximum when some row's has grown by more than 2^8: weights stay below 2^8
-                const float m_new = fmaxf(m_run, top);
-                if (__any((m_new - m_run) * c2 > 8.0f)) {
-                    const float alpha = m_run > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 0.0f;
-                    m_run = m_new;
-                    l_run *= alpha;
-#pragma unroll
-                    for (int d = 0; d < kDT; d++)
-#pragma unroll
-                        for (int v = 0; v < 16; v++) o[d][v] *= alpha;
-                }
-                const float mc = m_run > -INFINITY ? m_run * c2 : 0.0f;
-                float sum = 0.0f;
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int v = 0; v < 16; v++) {
-                        w[t][v] = __builtin_amdgcn_exp2f(fmaf(w[t][v], c2, -mc));
-                        sum += w[t][v];
-                    }
-                l_run += sum;
-                // O^T += V^T . W, 16 keys at a time
-#pragma unroll
-                for (int sl = 0; sl < 4; sl++) {
-                    half8_t wh;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) wh[i] = (half_t)w[sl / 2][(sl % 2) * 8 + i];
-                    const int row = sl * 16 + half * 4 + ((lane & 15) >> 2); // of the first run of four keys; the second one is 8 further
-#pragma unroll
-                    for (int d = 0; d < kDT; d++) {
-                        const int piece = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-                        const unsigned char *from = lds_v + row * kRowBytes + ((piece ^ v_swz(row)) << 4) + (lane & 1) * 8;
-                        typedef __attribute__((address_space(3))) short4_t *lds4;
-                        const half4_t a0 = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__attribute__((address_space(3))) void *)from));
-                        const half4_t a1 = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__attribute__((address_space(3))) void *)(from + 8 * kRowBytes)));
-                        const half8_t a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wh, o[d], 0, 0, 0);
-                    }
-                }
+            for (int d = 0; d < kDT; d++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x402, 32 / kDT, 0);
             }
         }
-        if (kQ4 && more) place(1 - decltype(stage)::value);
+        __builtin_amdgcn_sched_group_barrier(0x008, kDT, 0);
     };
+
     if (s_first < s_end) {
-        fetch(s_first, 0);
-        if constexpr (kQ4) place(0);
-        for (int s = s_first; s < s_end; s += 2) {
-            tile_step(s, std::integral_constant<int, 0>{});
-            if (s + 1 < s_end) tile_step(s + 1, std::integral_constant<int, 1>{});
+        Place at = place_of(s_first);
+        fetch(plane + at.row, min(kAtKeys, at.last - at.t0 + 1), 0);
+        place(0);
+        unsigned stage = 0;
+        for (int s = s_first; s < s_end; s++) {
+            // tiles from here on that every row sees whole and that a whole tile follows (wavefronts may count differently: both loops stage and wait alike)
+            const int seen = min(at.last, max(0, wp0)) - kh * 64 - 63 - at.t0, follow = at.last + 1 - at.t0;
+            int run = whole_half(at) ? min(min(seen / kAtKeys + 1, follow / kAtKeys - 1), s_end - 1 - s) : 0;
+            if (run > 0) {
+                s += run;
+                at.t0 += run * kAtKeys;
+                at.row += run * kAtKeys;
+                size_t row = plane + at.row - (size_t)(run - 1) * kAtKeys;
+                do {
+                    wait_vmcnt<0>();
+                    __syncthreads();
+                    fetch(row, kAtKeys, 1 - stage);
+                    __builtin_amdgcn_sched_barrier(0);
+                    work(stage, 0, 0, std::true_type{});
+                    __builtin_amdgcn_sched_barrier(0);
+                    stage = 1 - stage;
+                    place(stage);
+                    row += kAtKeys;
+                } while (--run > 0);
+            }
+            wait_vmcnt<0>(); // this wavefront's part of the tile has landed
+            __syncthreads(); // ... and everybody's; everybody is done with the tile before, whose stage is filled next
+            Place next = {at.t0 + kAtKeys, at.last, at.row + kAtKeys, at.front};
+            if (next.t0 > next.last) next = place_of(s + 1);
+            if (s + 1 < s_end) fetch(plane + next.row, min(kAtKeys, next.last - next.t0 + 1), 1 - stage);
+            if (!unseen_half(at)) { // is every value of V finite?
+                const unsigned char *v = lds + stage * kStageBytes + kTileBytes + kh * (64 * kRowBytes);
+                bool odd = false;
+#pragma unroll 2
+                for (int i = 0; i < 64 * kRowBytes / 1024; i++) {
+                    const uint4_t x = *reinterpret_cast<const uint4_t *>(v + i * 1024 + lane * 16);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) odd |= ((x[j] & 0x7c000000u) == 0x7c000000u) | ((x[j] & 0x7c00u) == 0x7c00u);
+                }
+                if (__any(odd) && !whole_half(at)) skipped = true;
+                else work(stage, at.t0 + kh * 64, at.last, std::false_type{});
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            stage = 1 - stage;
+            if (s + 1 < s_end) place(stage);
+            at = next;
         }
     }
 
@@ -266,19 +337,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParam
         // were left out above.  Here every row adds up what it sees, key by key in f32.
         for (int s = s_first; s < s_end; s++) {
             const Place at = place_of(s);
-            if (unseen_tile(at) || whole_tile(at)) continue;
-            const int here = min(kAtKeys, at.last - at.t0 + 1);
+            if (unseen_half(at) || whole_half(at)) continue;
+            const int t0 = at.t0 + kh * 64, here = min(64, at.last - t0 + 1);
+            const size_t row = plane + at.row + kh * 64;
             bool odd = false;
-            for (int i = lane; i < here * HD; i += 64) odd |= !(fabsf(plane_load1<CT, true>(p.cache_v, (plane + at.row) * HD + i)) < INFINITY);
+            for (int i = lane; i < here * HD; i += 64) odd |= !(fabsf(plane_load1<CT, true>(p.cache_v, row * HD + i)) < INFINITY);
             if (!__any(odd)) continue;
 #pragma unroll 1
             for (int j = 0; j < here; j++) {
-                const size_t from = (plane + at.row + j) * HD;
+                const size_t from = (row + j) * HD;
                 float dot = 0.0f;
 #pragma unroll 1
                 for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d++) dot = fmaf((float)q_row[d], plane_load1<CT, true>(p.cache_k, from + d), dot);
                 dot += __shfl_xor(dot, 32, 64);
-                const bool seen = sees(at.t0 + j, at.last);
+                const bool seen = sees(t0 + j, at.last);
                 const float m_new = seen ? fmaxf(m_run, dot) : m_run;
                 const float alpha = m_new > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 1.0f;
                 const float wt = seen ? __builtin_amdgcn_exp2f((dot - (m_new > -INFINITY ? m_new : 0.0f)) * c2) : 0.0f;
@@ -296,8 +368,33 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParam
         }
     }
 
+    __syncthreads(); // everybody is done with the tiles
+    if constexpr (kShares > 1) { // the second half of the keys hands its (O, m, sum) to the first
+        float *join = reinterpret_cast<float *>(lds) + rg * kJoinFloats + lane;
+        if (kh == 1) {
+#pragma unroll
+            for (int d = 0; d < kDT; d++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) join[(d * 16 + v) * 64] = o[d][v];
+            join[(kDT * 16) * 64] = m_run;
+            join[(kDT * 16 + 1) * 64] = l_run;
+        }
+        __syncthreads();
+        if (kh == 1) return;
+        const float m1 = join[(kDT * 16) * 64], l1 = join[(kDT * 16 + 1) * 64], m = fmaxf(m_run, m1);
+        const float a0 = m_run > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m) * c2) : 0.0f, a1 = m1 > -INFINITY ? __builtin_amdgcn_exp2f((m1 - m) * c2) : 0.0f;
+        l_run = (m_run > -INFINITY ? l_run * a0 : l_run) + (m1 > -INFINITY ? l1 * a1 : l1); // (nothing seen: 0; only NaN: NaN)
+        m_run = m;
+#pragma unroll
+        for (int d = 0; d < kDT; d++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const float x = join[(d * 16 + v) * 64];
+                o[d][v] = (a0 > 0.0f ? o[d][v] * a0 : 0.0f) + (a1 > 0.0f ? x * a1 : 0.0f);
+            }
+    }
     const float l = my_p < 0 ? 0.0f : l_run + __shfl_xor(l_run, 32, 64); // (padding: 0)
-    if (n_pieces > 1) { // ---- leave (m, sum) and O of the piece for attn_join_kernel
+    if (kShares > 1 && n_pieces > 1) { // ---- leave (m, sum) and O of the piece for attn_join_kernel
         if (w0 + col > r1) return;
         float *ws = pp.ws + ((size_t)unit * rows + w0 + col) * pp.pieces * (HD + 2);
         if (half == 0) {
@@ -321,9 +418,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParam
         return;
     }
     // ---- normalise, round to f16, turn O^T into rows through LDS and store 16-byte pieces
-    __syncthreads(); // everybody is done with the tiles
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    half_t *ot = reinterpret_cast<half_t *>(lds) + wave * (32 * kOutRow);
+    half_t *ot = reinterpret_cast<half_t *>(lds + rg * (kShares > 1 ? kJoinFloats * 4 : 32 * kOutRow * 2));
 #pragma unroll
     for (int d = 0; d < kDT; d++)
 #pragma unroll
@@ -353,71 +449,85 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_tiles_kernel(AttnCutParam
 
 bool attn_tiles_takes(const AttnWindowParams &p) { return p.f16 && p.cache != kPlaneF32 && p.n * (p.n_heads / p.n_kv) > 64; }
 
-constexpr int kAtWaves = 4;
-constexpr int kAtRows = 32 * kAtWaves;
-
-// How the texts are cut.  A workgroup alone on its compute unit takes 1.4 us per tile of 128 rows and 64 keys of 128 dims, two of them 2.3 us (together less per
-// tile); joining costs 4 us and writing and reading the partial results, p * 2 (hd + 2) floats per row and head at about 4.5 bytes per ps.  The number of pieces with the
-// least sum is taken: 400 rows behind 8000 positions, 32 heads on 8 key heads: 4 pieces, 92 us; 1024 rows from the text's beginning: 1 piece.
-static void cut_tiles(const AttnWindowParams &p, int compute_units, int *pieces, int *piece_steps) {
+// How the work is split: wavefronts per row group, and pieces of each text, of `piece_steps` tiles.
+//
+// A workgroup with two wavefronts per row group has a compute unit to itself; of those with one there are two on a compute unit.  Two are taken where the
+// workgroups would otherwise leave wavefronts idle: fewer of them than compute units, or at most two each while the first rows of a text see little of it
+// and their workgroups end early.  (1 / 2 wavefronts, 32 heads of 128: 1024 rows from position 0, 256 workgroups, 29.4 / 24.4 us; 1500, 384, 42.0 / 35.8;
+// 2048, 512, 57.2 / 52.2; over 4 bits 35.4 / 28.5, 50.1 / 40.2 and 66.4 / 59.3.  40 heads, 1700 rows, 560: 51.2 / 59.2; 2048, 640: 61.4 / 72.1.  1500 rows
+// that all see 1024 positions, 376: 54.3 / 68.4.)
+//
+// Pieces (with two wavefronts per row group): a compute unit takes 2.3 us per tile of 128 rows and 128 keys of 128 dims; joining costs 4 us and writing and
+// reading the partial results, p * 2 (hd + 2) floats per row and head at about 4.5 bytes per ps.  The number of pieces with the least sum is taken.
+struct TilesCut {
+    int shares, pieces, piece_steps;
+};
+constexpr int kCutKeys = 128;
+static TilesCut cut_tiles(const AttnWindowParams &p, int compute_units) {
     const int group = p.n_heads / p.n_kv;
     const int64_t rows = (int64_t)p.n * group, units = (rows + kAtRows - 1) / kAtRows * p.n_seqs * p.n_kv;
     const int64_t apart = std::min<int64_t>(p.n - 1, (kAtRows - 2) / group + 1); // of a workgroup's rows
     int64_t steps = 1;                                                           // no workgroup has more
+    bool uneven = false;
     for (int b = 0; b < p.n_seqs; b++) {
         const int64_t last = (int64_t)p.start[b] + p.n - 1;
         if (last < 0) continue;
-        int64_t count = (last + kAtKeys) / kAtKeys;
-        if (p.window > 0) count = std::min(count, (p.window - 1 + apart + kAtKeys) / kAtKeys) + (p.sinks + kAtKeys - 1) / kAtKeys;
+        int64_t count = (last + kCutKeys) / kCutKeys;
+        if (p.window > 0) count = std::min(count, (p.window - 1 + apart + kCutKeys) / kCutKeys) + (p.sinks + kCutKeys - 1) / kCutKeys;
         if (last >= p.max_seq_len) count++; // the ring's end cuts a tile in two
         steps = std::max(steps, count);
+        uneven |= (p.window == 0 || p.window > last) && p.start[b] < p.n;
     }
-    const double tile_us = 1.4 * p.head_dim / 128, shared_us = 2.3 * p.head_dim / 128, piece_us = (double)p.n * p.n_heads * p.n_seqs * (p.head_dim + 2) * 8 / 4.5e6;
+    const double tile_us = 2.3 * p.head_dim / 128, piece_us = (double)p.n * p.n_heads * p.n_seqs * (p.head_dim + 2) * 8 / 4.5e6;
     int64_t n = 1;
-    double best = steps * (units > compute_units ? shared_us : tile_us);
+    double best = steps * tile_us * std::max(1.0, (double)units / compute_units);
     for (int64_t c = 2; c <= kMaxPieces && c <= steps && c * units <= 2 * compute_units; c++) {
-        const double us = (double)((steps + c - 1) / c) * (c * units > compute_units ? shared_us : tile_us) + 4.0 + c * piece_us;
+        const double us = (double)((steps + c - 1) / c) * tile_us * std::max(1.0, (double)(c * units) / compute_units) + 4.0 + c * piece_us;
         if (us < best) {
             best = us;
             n = c;
         }
     }
-    *piece_steps = (int)((steps + n - 1) / n);
-    *pieces = (int)((steps + *piece_steps - 1) / *piece_steps);
+    TilesCut cut;
+    cut.piece_steps = (int)((steps + n - 1) / n);
+    cut.pieces = (int)((steps + cut.piece_steps - 1) / cut.piece_steps);
+    cut.shares = cut.pieces > 1 || units <= (uneven ? 2 : 1) * compute_units ? 2 : 1;
+    return cut;
 }
 
 size_t attn_tiles_work_floats(const AttnWindowParams &p, int compute_units) {
-    int pieces, piece_steps;
-    cut_tiles(p, compute_units, &pieces, &piece_steps);
+    const int pieces = cut_tiles(p, compute_units).pieces;
     return pieces > 1 ? (size_t)p.n * p.n_heads * p.n_seqs * pieces * (p.head_dim + 2) : 0;
 }
 
 template <typename CT, int HD>
-static void launch_tiles(const AttnCutParams &p, hipStream_t s) {
+static void launch_tiles(const AttnCutParams &p, int shares, hipStream_t s) {
     const int rows = p.a.n * (p.a.n_heads / p.a.n_kv);
     const unsigned units = (unsigned)(p.a.n_seqs * p.a.n_kv);
     const dim3 grid(units, (unsigned)((rows + kAtRows - 1) / kAtRows), (unsigned)p.pieces);
-    hipLaunchKernelGGL((attn_tiles_kernel<CT, HD, kAtWaves>), grid, dim3(64 * kAtWaves), 0, s, p);
-    if (p.pieces > 1) launch_attn_join<half_t, HD, kAtRows, kAtKeys>(p, s);
+    if (shares == 1) {
+        hipLaunchKernelGGL((attn_tiles_kernel<CT, HD, 1>), grid, dim3(64 * kAtGroups), 0, s, p);
+        return;
+    }
+    hipLaunchKernelGGL((attn_tiles_kernel<CT, HD, 2>), grid, dim3(128 * kAtGroups), 0, s, p);
+    if (p.pieces > 1) launch_attn_join<half_t, HD, kAtRows, kCutKeys>(p, s);
 }
 
 hipError_t launch_attn_tiles(const AttnWindowParams &a, int compute_units, float *ws, hipStream_t s) {
     if ((int64_t)a.n * (a.n_heads / a.n_kv) > (int64_t)65535 * kAtRows || (int64_t)a.n_seqs * a.n_kv > 65535) return hipErrorInvalidValue;
+    const TilesCut cut = cut_tiles(a, compute_units);
     AttnCutParams p;
     p.a = a;
     p.ws = ws;
-    cut_tiles(a, compute_units, &p.pieces, &p.piece_steps);
-    // Late rows see more keys and start first.  Where every workgroup is resident from the start, two to a compute unit, the second ones come in rising order, so that a
-    // unit's two have about the same sum (2048 rows of 32 heads: 58.6 -> 45 us).
-    const int tiles = (int)(((int64_t)a.n * (a.n_heads / a.n_kv) + kAtRows - 1) / kAtRows), units = a.n_seqs * a.n_kv;
-    p.descend = p.pieces == 1 && tiles * units <= 2 * compute_units ? std::min(tiles, (compute_units + units - 1) / units) : tiles;
+    p.pieces = cut.pieces;
+    p.piece_steps = cut.piece_steps;
     switch (a.head_dim * 2 + (a.cache == kPlaneQ4)) {
-    case 64: launch_tiles<half_t, 32>(p, s); break;
-    case 65: launch_tiles<Quant4, 32>(p, s); break;
-    case 128: launch_tiles<half_t, 64>(p, s); break;
-    case 129: launch_tiles<Quant4, 64>(p, s); break;
-    case 256: launch_tiles<half_t, 128>(p, s); break;
-    case 257: launch_tiles<Quant4, 128>(p, s); break;
+    case 64: launch_tiles<half_t, 32>(p, cut.shares, s); break;
+    case 65: launch_tiles<Quant4, 32>(p, cut.shares, s); break;
+    case 128: launch_tiles<half_t, 64>(p, cut.shares, s); break;
+    case 129: launch_tiles<Quant4, 64>(p, cut.shares, s); break;
+    case 256: launch_tiles<half_t, 128>(p, cut.shares, s); break;
+    case 257: launch_tiles<Quant4, 128>(p, cut.shares, s); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

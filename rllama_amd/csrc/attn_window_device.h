@@ -92,7 +92,6 @@ struct AttnCutParams {
     AttnWindowParams a;
     float *ws;
     int pieces, piece_steps; // pieces of `piece_steps` steps, at most `pieces` of them
-    int descend;             // attn_tiles_kernel: so many tiles of rows are started from the last one downwards, the others from the first one upwards
 };
 constexpr int kMaxPieces = 64;
 

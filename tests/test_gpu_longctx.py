@@ -251,6 +251,15 @@ ATTEND = [
     (128, 2, 1, 90, 300, 130, 4, [250, 7777]),
     (32, 2, 2, 1, 50, 49, 0, [99]),
 ]
+MANY_ROWS = [  # (two forms of the product: up to 256 workgroups, with uneven work up to 512, and above)
+    (128, 20, 20, 260, 300, 0, 0, [0, 5, 40, -7, 0, 0, 0, 0, 0]),
+    (64, 60, 20, 130, 330, 70, 3, [190, 200, -129, 3]),
+    (32, 30, 30, 129, 200, 60, 5, [0, 180, 400, 31, 64, 71, 1000, 70, 69, 68]),
+    (128, 24, 24, 129, 450, 200, 70, [300, 5000, 321, 440, 449, 448]),
+    (128, 24, 24, 150, 700, 0, 0, [500, 550, 63, 64, 150, 300]),
+    (64, 24, 24, 150, 700, 0, 0, [500, 550, 63, 64, 150, 300]),
+    (32, 16, 16, 400, 400, 0, 0, [0, 0, 0]),
+]
 TYPES = [("f16", "f16"), ("f16", "q4"), ("f32", "f32"), ("f32", "q4"), ("f32", "f16"), ("f16", "f32")]
 
 
@@ -267,6 +276,12 @@ def _attend_case(hd, H, G, n, S, window, sinks, starts, seed=0, poison=True):
             K[b, :, ~keep] = np.nan
             V[b, :, ~keep] = np.nan
     return q, K, V
+
+
+@pytest.mark.parametrize("hd,H,G,n,S,window,sinks,starts", MANY_ROWS)
+@pytest.mark.parametrize("cache", ["f16", "q4"])
+def test_attention_of_many_rows(ctx, hd, H, G, n, S, window, sinks, starts, cache):
+    test_attention(ctx, hd, H, G, n, S, window, sinks, starts, "f16", cache)
 
 
 @pytest.mark.parametrize("hd,H,G,n,S,window,sinks,starts", ATTEND)
@@ -350,6 +365,26 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them(ctx):
         got = Tensor.from_numpy(ctx, q).attn_window(upload(ctx, K, kind), upload(ctx, V, kind), H, H, S, [0]).to_numpy()
         assert np.isnan(got[20:, 5]).all()
         assert np.isfinite(got[:20]).all() and np.isfinite(np.delete(got, 5, 1)).all()
+
+
+@pytest.mark.parametrize("n,start,H,B", [(40, 90, 1, 1), (90, 0, 2, 1), (300, 100, 2, 1), (130, 260, 30, 10)])
+@pytest.mark.parametrize("cache", ["f16", "q4"])
+def test_an_infinite_value_reaches_all_that_see_it_and_no_others(ctx, cache, n, start, H, B):
+    hd, S = 32, start + n
+    rng = np.random.default_rng(n)
+    q = rng.standard_normal((B, n, H, hd))
+    K, V = rng.standard_normal((B, H, S, hd)), rng.standard_normal((B, H, S, hd))
+    at = min(70, S - 1)
+    V[:, 0, at, 5] = np.inf  # (of 4 bits its whole group is NaN)
+    got = Tensor.from_numpy(ctx, q.reshape(B * n, H * hd).astype(f16)).attn_window(upload(ctx, K.reshape(-1, hd), cache), upload(ctx, V.reshape(-1, hd), cache), H, H, S, [start] * B)
+    got = got.to_numpy().reshape(B, n, H, hd)
+    first = max(0, at - start)
+    hit = got[:, first:, 0]
+    if cache == "f16":
+        assert (hit[..., 5] == np.inf).all() and np.isfinite(np.delete(hit, 5, -1)).all()
+    else:
+        assert np.isnan(hit).all()
+    assert np.isfinite(got[:, :first]).all() and np.isfinite(got[:, :, 1:]).all()
 
 
 @pytest.mark.parametrize("n", [1, 33])

@@ -290,16 +290,18 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
         for (int s = s_first; s < s_end; s++) {
             // tiles from here on that every row sees whole and that a whole tile follows (wavefronts may count differently: both loops stage and wait alike)
             const int seen = min(at.last, max(0, wp0)) - kh * 64 - 63 - at.t0, follow = at.last + 1 - at.t0;
-            int run = whole_half(at) ? min(min(seen / kAtKeys + 1, follow / kAtKeys - 1), s_end - 1 - s) : 0;
+            int run = whole_half(at) ? min(min(seen / kAtKeys + 1, (kQ4 ? (follow + kAtKeys - 1) / kAtKeys : follow / kAtKeys) - 1), s_end - 1 - s) : 0;
             if (run > 0) {
                 s += run;
                 at.t0 += run * kAtKeys;
                 at.row += run * kAtKeys;
                 size_t row = plane + at.row - (size_t)(run - 1) * kAtKeys;
+                int left = follow - kAtKeys;
                 do {
                     wait_vmcnt<0>();
                     __syncthreads();
-                    fetch(row, kAtKeys, 1 - stage);
+                    fetch(row, kQ4 ? min(kAtKeys, left) : kAtKeys, 1 - stage);
+                    left -= kAtKeys;
                     __builtin_amdgcn_sched_barrier(0);
                     work(stage, 0, 0, std::true_type{});
                     __builtin_amdgcn_sched_barrier(0);

@@ -44,6 +44,8 @@ class OpenCL {
     OpenCL(const OpenCL &) = delete;
     OpenCL &operator=(const OpenCL &) = delete;
     void flush() { check(rlh_sync(ctx_)); } // src/tensor_opencl_support.rs:130
+    void wait_stream(void *stream) { check(rlh_wait_stream(ctx_, stream)); }       // later work here waits for what is queued there by now
+    void release_stream(void *stream) { check(rlh_release_stream(ctx_, stream)); } // later work there waits for what is queued here by now
     rlh_ctx *raw() const { return ctx_; }
 
   private:
@@ -207,7 +209,7 @@ class TokenSampler {
     rlh_sampler_params p_;
 };
 
-// Device tensor with the op set of OpenCLTensor (src/tensor_opencl_support.rs:215-405)
+// Device tensor with the op set of OpenCLTensor (src/tensor_opencl_support.rs:215-405), and ops of this library
 class Tensor {
   public:
     // to_gpu_inplace (src/tensor.rs:2127-2147): host data [rows x cols], row stride cols_capacity elements
@@ -249,6 +251,52 @@ class Tensor {
     Tensor matrix_mul_transposed(const Tensor &other) const { // src/tensor.rs:999-1025
         Tensor out = zeros(cl_, rows_, other.rows_, dtype_);
         check(rlh_matrix_mul_inplace_transposed(out.h_, h_, other.h_));
+        return out;
+    }
+
+    // ---- long contexts and drafted tokens (no reference counterpart)
+    // Over device memory that the caller owns and keeps; nothing is copied.
+    static Tensor from_device(const std::shared_ptr<OpenCL> &cl, void *device_memory, int64_t rows, int64_t cols, TensorDType dtype) {
+        rlh_tensor *t = nullptr;
+        check(rlh_tensor_wrap(cl->raw(), device_memory, (int)rows, (int)cols, (int)dtype, &t));
+        return Tensor(cl, t, rows, cols, dtype);
+    }
+    Tensor convert(TensorDType dtype) const {
+        Tensor out = zeros(cl_, rows_, cols_, dtype);
+        check(rlh_convert(out.h_, h_));
+        return out;
+    }
+    // f32 [positions x head_dim]: the angles qkv_append takes
+    static Tensor rope_table(const std::shared_ptr<OpenCL> &cl, int64_t positions, int64_t head_dim, double theta = 10000.0) {
+        Tensor out = zeros(cl, positions, head_dim, TensorDType::Float32);
+        check(rlh_rope_table(out.h_, theta));
+        return out;
+    }
+    // this = qkv: norms per head, rotation, keys and values into the planes; the queries are returned
+    Tensor qkv_append(Tensor &cache_k, Tensor &cache_v, const Tensor &freqs, int n_heads, int n_kv_heads, int max_seq_len, const std::vector<int32_t> &start_pos,
+                      const Tensor *q_norm = nullptr, const Tensor *k_norm = nullptr, double eps = 1e-6, bool halves = false, int sinks = 0) const {
+        Tensor q = zeros(cl_, rows_, (int64_t)n_heads * cache_k.cols_, dtype_);
+        check(rlh_qkv_append(q.h_, h_, q_norm ? q_norm->h_ : nullptr, k_norm ? k_norm->h_ : nullptr, eps, freqs.h_, halves ? 1 : 0, cache_k.h_, cache_v.h_, n_heads,
+                             n_kv_heads, max_seq_len, sinks, start_pos.data(), (int)start_pos.size()));
+        return q;
+    }
+    // this = q after qkv_append; window 0 = the whole text
+    Tensor attn_window(const Tensor &cache_k, const Tensor &cache_v, int n_heads, int n_kv_heads, int max_seq_len, const std::vector<int32_t> &start_pos, int window = 0,
+                       int sinks = 0) const {
+        Tensor out = zeros(cl_, rows_, cols_, dtype_);
+        check(rlh_attn_window(out.h_, h_, cache_k.h_, cache_v.h_, n_heads, n_kv_heads, max_seq_len, start_pos.data(), (int)start_pos.size(), window, sinks));
+        return out;
+    }
+    // this = logits
+    Tensor softmax_rows(float temperature = 1.0f) const {
+        Tensor out = zeros(cl_, rows_, cols_, TensorDType::Float32);
+        check(rlh_softmax_rows(out.h_, h_, temperature));
+        return out;
+    }
+    // this = drafted ids i32 [sequences x k]: i32 [sequences x (k + 2)], accepted count, those, the drawn token, -1 after it
+    Tensor verify_draft(const Tensor &target, const Tensor *draft, const Tensor &uniforms) const {
+        Tensor out = zeros(cl_, rows_, cols_ + 2, TensorDType::Int32);
+        check(rlh_verify_draft(out.h_, target.h_, draft ? draft->h_ : nullptr, h_, uniforms.h_));
         return out;
     }
 

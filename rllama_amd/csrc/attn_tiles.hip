@@ -74,7 +74,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     const int wp0 = start + w0 / group, wp1 = w1 < w0 ? -1 : start + w1 / group;
     const int my_r = min(w0 + col, r1), my_i = my_r / group;
     const int my_p = w0 + col <= r1 ? start + my_i : -1;
-    const int my_low = p.window > 0 ? my_p - p.window + 1 : 0;
+    const int my_low = p.window > 0 ? max(0, my_p - p.window + 1) : 0;
     const half_t *q_row = reinterpret_cast<const half_t *>(p.q) + ((size_t)(b * p.n + my_i) * p.n_heads + g * group + (my_r - my_i * group)) * HD;
 
     // q as the second operand: lane supplies dims 16 ks + 8 half .. + 7, in the order of the converted codes where the cache has 4 bits
@@ -227,11 +227,16 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
 #pragma unroll
         for (int d = 0; d < kDT; d++) read_v(0, d);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!decltype(whole)::value) {
+        if constexpr (!decltype(whole)::value) { // a bit per key of the tile (what sees() says of each), and a select by it
+            auto ones = [](int n) { return n <= 0 ? 0ull : ~0ull >> (64 - min(n, 64)); };
+            const uint64_t seen = (ones(min(my_p, last) - t0 + 1) & (~ones(my_low - t0) | ones(p.sinks - t0))) >> (half * 4);
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) w[t][v] = sees(t0 + t * 32 + (v >> 2) * 8 + half * 4 + (v & 3), last) ? w[t][v] : -INFINITY;
+                for (int v = 0; v < 16; v++) {
+                    const uint32_t all = (uint32_t)((int32_t)((uint32_t)(seen >> (t * 32)) << (31 - (v >> 2) * 8 - (v & 3))) >> 31);
+                    w[t][v] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, (float)w[t][v]) & all) | (0xff800000u & ~all)); // else -infinity
+                }
         }
         float top = -INFINITY;
 #pragma unroll

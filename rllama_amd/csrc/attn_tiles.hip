@@ -151,13 +151,11 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     const Q4Bits bits;
     auto place = [&](unsigned stage) __attribute__((always_inline)) { // 4 bits: the fetched codes as f16 into LDS
         if constexpr (kQ4) {
-            int me = tid;
-            asm volatile("" : "+v"(me)); // the addresses are formed here, not kept in registers over the products
 #pragma unroll
             for (int i = 0; i < kItems; i++) {
-                const int item = i * 64 * kWaves + me;
+                const unsigned item = i * 64 * kWaves + (unsigned)tid;
                 if (kGroups < 64 * kWaves && item >= kGroups) break;
-                const int at_group = item % (kGroups / 2), r = at_group / (HD / 32), c0 = at_group % (HD / 32) * 4;
+                const unsigned at_group = item % (kGroups / 2), r = at_group / (HD / 32), c0 = at_group % (HD / 32) * 4;
                 const bool is_v = item >= kGroups / 2;
                 const half2_t pair = __builtin_bit_cast(half2_t, pairs[i]), scale = {pair[0], pair[0]}, low = {pair[1], pair[1]};
                 unsigned char *to = lds + stage * kStageBytes + (is_v ? kTileBytes : 0) + r * kRowBytes;

@@ -149,27 +149,25 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
         }
     };
     const Q4Bits bits;
-    auto place = [&](unsigned stage) __attribute__((always_inline)) { // 4 bits: the fetched codes as f16 into LDS
+    // 4 bits: word w of the fetched codes (eight of them) as f16 into a stage
+    auto place_word = [&](unsigned stage, int word) __attribute__((always_inline)) {
+        const int i = word / 4, w = word % 4;
+        const unsigned item = i * 64 * kWaves + (unsigned)tid;
+        if (kGroups < 64 * kWaves && item >= kGroups) return;
+        const unsigned at_group = item % (kGroups / 2), r = at_group / (HD / 32), c = at_group % (HD / 32) * 4 + w;
+        const bool is_v = item >= kGroups / 2;
+        const half2_t pair = __builtin_bit_cast(half2_t, pairs[i]), scale = {pair[0], pair[0]}, low = {pair[1], pair[1]};
+        half2_t x[4];
+        q4_pairs_f16(bits, codes[i][w], scale, low, x);
+        uint4_t y;
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] = __builtin_bit_cast(uint32_t, x[j]);
+        *reinterpret_cast<uint4_t *>(lds + stage * kStageBytes + (is_v ? kTileBytes : 0) + r * kRowBytes + ((c ^ (is_v ? v_swz(r) : k_swz(r))) << 4)) = y;
+    };
+    auto place = [&](unsigned stage) __attribute__((always_inline)) {
         if constexpr (kQ4) {
 #pragma unroll
-            for (int i = 0; i < kItems; i++) {
-                const unsigned item = i * 64 * kWaves + (unsigned)tid;
-                if (kGroups < 64 * kWaves && item >= kGroups) break;
-                const unsigned at_group = item % (kGroups / 2), r = at_group / (HD / 32), c0 = at_group % (HD / 32) * 4;
-                const bool is_v = item >= kGroups / 2;
-                const half2_t pair = __builtin_bit_cast(half2_t, pairs[i]), scale = {pair[0], pair[0]}, low = {pair[1], pair[1]};
-                unsigned char *to = lds + stage * kStageBytes + (is_v ? kTileBytes : 0) + r * kRowBytes;
-                const int swz = is_v ? v_swz(r) : k_swz(r);
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    half2_t x[4];
-                    q4_pairs_f16(bits, codes[i][w], scale, low, x);
-                    uint4_t y;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) y[j] = __builtin_bit_cast(uint32_t, x[j]);
-                    *reinterpret_cast<uint4_t *>(to + (((c0 + w) ^ swz) << 4)) = y;
-                }
-            }
+            for (int word = 0; word < 4 * kItems; word++) place_word(stage, word);
         }
     };
 
@@ -188,7 +186,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     // ---- one tile: both products and the softmax of this wavefront's 64 keys
     const int v_row = half * 4 + ((lane & 15) >> 2);               // of the first run of four keys; the second one is 8 further
     const int v_piece = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1); // + 4 d
-    auto work = [&](unsigned stage, int t0, int last, auto whole) __attribute__((always_inline)) {
+    auto work = [&](unsigned stage, int t0, int last, auto whole, auto fetch_more) __attribute__((always_inline)) {
         const unsigned char *lds_k = lds + stage * kStageBytes + kh * (64 * kRowBytes), *lds_v = lds_k + kTileBytes;
         // S^T: the two 32-key products side by side, K read two steps ahead of them.  (Barriers against reordering: left alone, every read ends up right in
         // front of its product, and its latency in between.)
@@ -211,9 +209,14 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
             if (ks + 2 < kKS) read_k(ks + 2);
 #pragma unroll
             for (int t = 0; t < 2; t++) w[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_frag[ks % 3][t], q[ks], w[t], 0, 0, 0);
+            if constexpr (kQ4) { // the next tile's codes are converted beside the products, which leave the vector ALU idle
+#pragma unroll
+                for (int word = ks * 4 * kItems / kKS; word < (ks + 1) * 4 * kItems / kKS; word++) place_word(1 - stage, word);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
+        fetch_more();
         half8_t v_frag[2][kDT];
         auto read_v = [&](int sl, int d) {
             const unsigned char *from = lds_v + (sl * 16 + v_row) * kRowBytes + (((d * 4 + v_piece) ^ v_swz(v_row)) << 4) + (lane & 1) * 8;
@@ -283,39 +286,51 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     };
 
     if (s_first < s_end) {
-        Place at = place_of(s_first);
-        fetch(plane + at.row, min(kAtKeys, at.last - at.t0 + 1), 0);
+        Place at = place_of(s_first), ahead = at; // `ahead`: the tile after the one fetched last
+        auto fetch_ahead = [&](int s) __attribute__((always_inline)) {
+            if (s >= s_end) return;
+            fetch(plane + ahead.row, min(kAtKeys, ahead.last - ahead.t0 + 1), (unsigned)(s - s_first) & 1);
+            ahead.t0 += kAtKeys;
+            ahead.row += kAtKeys;
+            if (ahead.t0 > ahead.last) ahead = place_of(s + 1);
+        };
+        fetch_ahead(s_first);
         place(0);
+        if constexpr (kQ4) fetch_ahead(s_first + 1);
         unsigned stage = 0;
         for (int s = s_first; s < s_end; s++) {
-            // tiles from here on that every row sees whole and that a whole tile follows (wavefronts may count differently: both loops stage and wait alike)
+            // tiles from here on that every row sees whole and that another tile (f16: a whole one) follows in the same run of rows (wavefronts may count
+            // differently: both loops stage and wait alike)
             const int seen = min(at.last, max(0, wp0)) - kh * 64 - 63 - at.t0, follow = at.last + 1 - at.t0;
             int run = whole_half(at) ? min(min(seen / kAtKeys + 1, (kQ4 ? (follow + kAtKeys - 1) / kAtKeys : follow / kAtKeys) - 1), s_end - 1 - s) : 0;
             if (run > 0) {
-                s += run;
+                const int end = s + run;
+                if constexpr (!kQ4) {
+                    ahead.t0 = at.t0 + (run + 1) * kAtKeys;
+                    ahead.row = at.row + (run + 1) * kAtKeys;
+                    if (ahead.t0 > ahead.last) ahead = place_of(end + 1);
+                }
+                size_t row = plane + at.row + kAtKeys;
                 at.t0 += run * kAtKeys;
                 at.row += run * kAtKeys;
-                size_t row = plane + at.row - (size_t)(run - 1) * kAtKeys;
-                int left = follow - kAtKeys;
                 do {
-                    wait_vmcnt<0>();
+                    if constexpr (!kQ4) wait_vmcnt<0>();
                     __syncthreads();
-                    fetch(row, kQ4 ? min(kAtKeys, left) : kAtKeys, 1 - stage);
-                    left -= kAtKeys;
-                    __builtin_amdgcn_sched_barrier(0);
-                    work(stage, 0, 0, std::true_type{});
+                    if constexpr (!kQ4) {
+                        fetch(row, kAtKeys, 1 - stage);
+                        row += kAtKeys;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    work(stage, 0, 0, std::true_type{}, [&]() __attribute__((always_inline)) { if constexpr (kQ4) fetch_ahead(s + 2); });
                     __builtin_amdgcn_sched_barrier(0);
                     stage = 1 - stage;
-                    place(stage);
-                    row += kAtKeys;
-                } while (--run > 0);
+                } while (++s < end);
             }
-            wait_vmcnt<0>(); // this wavefront's part of the tile has landed
-            __syncthreads(); // ... and everybody's; everybody is done with the tile before, whose stage is filled next
-            Place next = {at.t0 + kAtKeys, at.last, at.row + kAtKeys, at.front};
-            if (next.t0 > next.last) next = place_of(s + 1);
-            if (s + 1 < s_end) fetch(plane + next.row, min(kAtKeys, next.last - next.t0 + 1), 1 - stage);
-            if (!unseen_half(at)) { // is every value of V finite?
+            if constexpr (!kQ4) wait_vmcnt<0>(); // this wavefront's part of the tile has landed
+            __syncthreads();                     // ... and everybody's; everybody is done with the tile before, whose stage is filled next
+            if constexpr (!kQ4) fetch_ahead(s + 1);
+            bool use = !unseen_half(at);
+            if (use) { // is every value of V finite?
                 const unsigned char *v = lds + stage * kStageBytes + kTileBytes + kh * (64 * kRowBytes);
                 ushort2_t top = {0, 0};
 #pragma unroll 4
@@ -325,13 +340,22 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
                     for (int j = 0; j < 4; j++) top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, x[j] & 0x7fff7fffu));
                 }
                 const bool odd = (int)(top[0] >= 0x7c00) | (int)(top[1] >= 0x7c00);
-                if (__any(odd) && !whole_half(at)) skipped = true;
-                else work(stage, at.t0 + kh * 64, at.last, std::false_type{});
+                if (__any(odd) && !whole_half(at)) {
+                    skipped = true;
+                    use = false;
+                }
+            }
+            if (use) {
+                work(stage, at.t0 + kh * 64, at.last, std::false_type{}, [&]() __attribute__((always_inline)) { if constexpr (kQ4) fetch_ahead(s + 2); });
+            } else if constexpr (kQ4) {
+                place(1 - stage); // (behind the last tile: into a stage that is read no more)
+                fetch_ahead(s + 2);
             }
             __builtin_amdgcn_sched_barrier(0);
             stage = 1 - stage;
-            if (s + 1 < s_end) place(stage);
-            at = next;
+            at.t0 += kAtKeys;
+            at.row += kAtKeys;
+            if (at.t0 > at.last) at = place_of(s + 1);
         }
     }
 

@@ -188,27 +188,28 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     const int v_piece = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1); // + 4 d
     auto work = [&](unsigned stage, int t0, int last, auto whole, auto fetch_more) __attribute__((always_inline)) {
         const unsigned char *lds_k = lds + stage * kStageBytes + kh * (64 * kRowBytes), *lds_v = lds_k + kTileBytes;
-        // S^T: the two 32-key products side by side, K read two steps ahead of them.  (Barriers against reordering: left alone, every read ends up right in
+        // S^T: the two 32-key products side by side, K read three steps ahead of them.  (Barriers against reordering: left alone, every read ends up right in
         // front of its product, and its latency in between.)
         float16_t w[2];
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int v = 0; v < 16; v++) w[t][v] = 0.0f;
-        half8_t k_frag[3][2];
+        half8_t k_frag[4][2];
         auto read_k = [&](int ks) {
 #pragma unroll
-            for (int t = 0; t < 2; t++) k_frag[ks % 3][t] = *reinterpret_cast<const half8_t *>(lds_k + (t * 32 + col) * kRowBytes + (((ks * 2 + half) ^ k_swz(col)) << 4));
+            for (int t = 0; t < 2; t++) k_frag[ks % 4][t] = *reinterpret_cast<const half8_t *>(lds_k + (t * 32 + col) * kRowBytes + (((ks * 2 + half) ^ k_swz(col)) << 4));
         };
         __builtin_amdgcn_s_setprio(1); // a wavefront at its products before one at its softmax (1500 rows with a window: 53.4 -> 50.7 us)
         read_k(0);
         if (kKS > 1) read_k(1);
+        if (kKS > 2) read_k(2);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < kKS; ks++) {
-            if (ks + 2 < kKS) read_k(ks + 2);
+            if (ks + 3 < kKS) read_k(ks + 3);
 #pragma unroll
-            for (int t = 0; t < 2; t++) w[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_frag[ks % 3][t], q[ks], w[t], 0, 0, 0);
+            for (int t = 0; t < 2; t++) w[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_frag[ks % 4][t], q[ks], w[t], 0, 0, 0);
             if constexpr (kQ4) { // the next tile's codes are converted beside the products, which leave the vector ALU idle
 #pragma unroll
                 for (int word = ks * 4 * kItems / kKS; word < (ks + 1) * 4 * kItems / kKS; word++) place_word(1 - stage, word);

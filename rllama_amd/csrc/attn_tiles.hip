@@ -475,8 +475,6 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     }
 }
 
-bool attn_tiles_takes(const AttnWindowParams &p) { return p.f16 && p.cache != kPlaneF32 && p.n * (p.n_heads / p.n_kv) > 64; }
-
 // How the work is split: wavefronts per row group, and pieces of each text, of `piece_steps` tiles.
 //
 // A workgroup with two wavefronts per row group has a compute unit to itself; of those with one there are two on a compute unit.  Two are taken where the
@@ -487,8 +485,10 @@ bool attn_tiles_takes(const AttnWindowParams &p) { return p.f16 && p.cache != kP
 //
 // Pieces (with two wavefronts per row group): a compute unit takes 2.3 us per tile of 128 rows and 128 keys of 128 dims; joining costs 4 us and writing and
 // reading the partial results, p * 2 (hd + 2) floats per row and head at about 4.5 bytes per ps.  The number of pieces with the least sum is taken.
+// What a call takes is about that and 6.5 us.
 struct TilesCut {
     int shares, pieces, piece_steps;
+    double us;
 };
 constexpr int kCutKeys = 128;
 static TilesCut cut_tiles(const AttnWindowParams &p, int compute_units) {
@@ -517,11 +517,14 @@ static TilesCut cut_tiles(const AttnWindowParams &p, int compute_units) {
         }
     }
     TilesCut cut;
+    cut.us = 6.5 + best;
     cut.piece_steps = (int)((steps + n - 1) / n);
     cut.pieces = (int)((steps + cut.piece_steps - 1) / cut.piece_steps);
     cut.shares = cut.pieces > 1 || units <= (uneven ? 2 : 1) * compute_units ? 2 : 1;
     return cut;
 }
+
+double attn_tiles_us(const AttnWindowParams &p, int compute_units) { return cut_tiles(p, compute_units).us; }
 
 size_t attn_tiles_work_floats(const AttnWindowParams &p, int compute_units) {
     const int pieces = cut_tiles(p, compute_units).pieces;

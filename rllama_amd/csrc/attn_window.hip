@@ -532,42 +532,64 @@ static hipError_t launch_rows_hd(const AttnCutParams &p, hipStream_t s) {
 // f32 arithmetic is needed for f32 queries and where an f32 cache may hold what f16 cannot
 static bool f16_arithmetic(const AttnWindowParams &p) { return p.f16 && p.cache != kPlaneF32; }
 
-// How the texts are cut: pieces of `piece_steps` steps, at most `pieces` of them.
-static void cut_rows(const AttnWindowParams &p, int compute_units, int *pieces, int *piece_steps) {
+// How the texts are cut: pieces of `piece_steps` steps, at most `pieces` of them; and about what the call takes.
+struct RowsCut {
+    int pieces, piece_steps;
+    double us;
+};
+static RowsCut cut_rows(const AttnWindowParams &p, int compute_units) {
     const int group = p.n_heads / p.n_kv, rows = p.n * group, step = f16_arithmetic(p) ? 32 : 16;
-    const int64_t units = (int64_t)((rows + kAwRows - 1) / kAwRows) * p.n_seqs * p.n_kv;
+    const int64_t tiles = (rows + kAwRows - 1) / kAwRows, units = tiles * p.n_seqs * p.n_kv;
     // no tile has more steps than this: its rows' positions are at most `apart` from each other
     const int64_t apart = std::min<int64_t>(p.n - 1, (kAwRows - 2) / group + 1);
     int64_t steps = 1;
+    double keys = 0.0; // that an average tile looks at, summed over the sequences
     for (int b = 0; b < p.n_seqs; b++) {
         const int64_t last = (int64_t)p.start[b] + p.n - 1;
         if (last < 0) continue;
         int64_t count = (last + step) / step;
-        if (p.window > 0) count = std::min(count, (p.window - 1 + apart + step) / step) + (p.sinks + step - 1) / step;
+        double mean = 0.5 * (double)(std::max(0, p.start[b]) + last + 1);
+        if (p.window > 0) {
+            count = std::min(count, (p.window - 1 + apart + step) / step) + (p.sinks + step - 1) / step;
+            mean = std::min(mean, (double)p.window + apart + p.sinks);
+        }
         if (last >= p.max_seq_len) count++; // the ring's end cuts a step in two
         steps = std::max(steps, count);
+        keys += mean;
     }
     // About one workgroup per compute unit, with a step for each wavefront at least.  Two steps per wavefront are not cut: joining costs a launch, about 3 us
     // (32 heads, f16: 384 positions 7.4 us against 8.7 in two pieces, 512: 8.8 / 9.3, 768: 9.7 cut against 10.5, 1024: 9.7 / 12.0).
     const int64_t want = std::max<int64_t>(1, compute_units / units);
     const int64_t n = steps <= 2 * kAwWaves ? 1 : std::min<int64_t>({want, (steps + kAwWaves - 1) / kAwWaves, kMaxPieces});
-    *piece_steps = (int)((steps + n - 1) / n);
-    *pieces = (int)((steps + *piece_steps - 1) / *piece_steps);
+    RowsCut cut;
+    cut.piece_steps = (int)((steps + n - 1) / n);
+    cut.pieces = (int)((steps + cut.piece_steps - 1) / cut.piece_steps);
+    cut.us = 5.0 + (cut.pieces > 1 ? 3.5 : 0.0) + units * 0.01 + tiles * p.n_kv * keys * p.head_dim / 128 * 30e-6 + (double)cut.piece_steps * step * p.head_dim / 128 * 4e-3;
+    return cut;
+}
+
+// The tiles of attn_tiles.hip take 128 rows at once, this kernel 16: it reads K and V once per 16 rows, but has more workgroups, no second rounding of 4-bit values
+// and more wavefronts per key.  Both sides' estimates were fitted to 180 measured shapes (17 .. 2400 rows per key and value head, 0 .. 8000 positions, f16 and 4 bits);
+// going by them costs 1 to 2 % over always taking the faster one, a fixed limit of 64 rows 11 to 13 %.  (us, this / tiles, 32 heads of 128: 128 rows from position 0
+// 7.1 / 8.8, behind 500 14.9 / 20.0, behind 2000 41 / 21.7; 64 rows behind 4000 44 / 22.)
+static bool tiles_take(const AttnWindowParams &p, int compute_units) {
+    return f16_arithmetic(p) && p.n * (int64_t)(p.n_heads / p.n_kv) > kAwRows && attn_tiles_us(p, compute_units) < cut_rows(p, compute_units).us;
 }
 
 size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units) {
-    if (attn_tiles_takes(p)) return attn_tiles_work_floats(p, compute_units);
-    int pieces, piece_steps;
-    cut_rows(p, compute_units, &pieces, &piece_steps);
+    if (tiles_take(p, compute_units)) return attn_tiles_work_floats(p, compute_units);
+    const int pieces = cut_rows(p, compute_units).pieces;
     return pieces > 1 ? (size_t)p.n * p.n_heads * p.n_seqs * pieces * (p.head_dim + 2) : 0;
 }
 
 hipError_t launch_attn_window(const AttnWindowParams &a, int compute_units, float *ws, hipStream_t s) {
-    if (attn_tiles_takes(a)) return launch_attn_tiles(a, compute_units, ws, s);
+    if (tiles_take(a, compute_units)) return launch_attn_tiles(a, compute_units, ws, s);
     AttnCutParams p;
     p.a = a;
     p.ws = ws;
-    cut_rows(a, compute_units, &p.pieces, &p.piece_steps);
+    const RowsCut cut = cut_rows(a, compute_units);
+    p.pieces = cut.pieces;
+    p.piece_steps = cut.piece_steps;
     if ((int64_t)a.n_seqs * a.n_kv > 65535 || (int64_t)a.n * (a.n_heads / a.n_kv) > 65535 * kAwRows) return hipErrorInvalidValue;
     switch (a.cache * 2 + a.f16) {
     case kPlaneF16 * 2: return launch_rows_hd<float, float, half_t>(p, s);

@@ -37,7 +37,7 @@ struct AttnWindowParams {
 };
 size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units); // partial results of texts that are cut
 // the form for many rows (attn_tiles.hip): which calls it takes, its work memory and its launch
-bool attn_tiles_takes(const AttnWindowParams &p);
+double attn_tiles_us(const AttnWindowParams &p, int compute_units); // about what a call takes
 size_t attn_tiles_work_floats(const AttnWindowParams &p, int compute_units);
 hipError_t launch_attn_tiles(const AttnWindowParams &p, int compute_units, float *ws, hipStream_t s);
 hipError_t launch_attn_window(const AttnWindowParams &p, int compute_units, float *ws, hipStream_t s);

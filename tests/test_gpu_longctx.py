@@ -259,6 +259,12 @@ MANY_ROWS = [  # (two forms of the product: up to 256 workgroups, with uneven wo
     (128, 24, 24, 150, 700, 0, 0, [500, 550, 63, 64, 150, 300]),
     (64, 24, 24, 150, 700, 0, 0, [500, 550, 63, 64, 150, 300]),
     (32, 16, 16, 400, 400, 0, 0, [0, 0, 0]),
+    (128, 8, 2, 40, 16100, 0, 0, [16000]),         # few of them behind long texts: cut into pieces
+    (64, 4, 2, 90, 30100, 0, 0, [30010, -20]),
+    (32, 4, 2, 100, 25200, 25000, 7, [30190]),
+    (128, 40, 10, 140, 500, 97, 3, [0, 100, 333, 20]),
+    (32, 40, 20, 300, 700, 5, 40, [333, 0]),
+    (64, 36, 12, 150, 900, 64, 4, [600, 88, 3]),
 ]
 TYPES = [("f16", "f16"), ("f16", "q4"), ("f32", "f32"), ("f32", "q4"), ("f32", "f16"), ("f16", "f32")]
 
@@ -367,7 +373,7 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them(ctx):
         assert np.isfinite(got[:20]).all() and np.isfinite(np.delete(got, 5, 1)).all()
 
 
-@pytest.mark.parametrize("n,start,H,B", [(40, 90, 1, 1), (90, 0, 2, 1), (300, 100, 2, 1), (130, 260, 30, 10)])
+@pytest.mark.parametrize("n,start,H,B", [(40, 90, 1, 1), (90, 0, 2, 1), (300, 100, 2, 1), (130, 60, 20, 10), (130, 260, 30, 10)])
 @pytest.mark.parametrize("cache", ["f16", "q4"])
 def test_an_infinite_value_reaches_all_that_see_it_and_no_others(ctx, cache, n, start, H, B):
     hd, S = 32, start + n

@@ -20,6 +20,10 @@
 // queries meet an f32 cache, whose values f16 may not hold.
 //
 // A text is cut into pieces when there are few rows: every workgroup leaves its (m, sum, O) in work memory and a second launch joins them.
+//
+// Measured: 16 texts, one row each over a window of 1024 and 4, 32 heads on 8 of 128: 63 MB in 13.3 us, 4.8 TB/s, and 3.9 us of join.  5 rows in f32 behind 2107
+// positions of 32 heads: 69 MB in 15.4 us, 4.5 TB/s.  Both are bound by memory.  One row behind 65700 positions in 4 bits, 64 heads on 8: 84 MB in 24.3 us,
+// 3.5 TB/s: bound by the vector ALU, which takes codes apart.  One row behind 383 positions, 6.3 MB: 7.7 us, a chain of latencies.
 #include "kernels.h"
 #include "attn_window_device.h"
 

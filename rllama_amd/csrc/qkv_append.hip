@@ -7,6 +7,8 @@
 // Bound by memory: every element is read once and written once, about 20 operations each.  hd / 8 lanes hold one head's vector,
 // 8 consecutive elements per lane: 16-byte accesses, the sum of squares is one exchange over at most 16 lanes, and a 4-bit group is four
 // neighbouring lanes, so quantising needs no memory of its own.
+//
+// Measured: 1500 rows of 32 heads on 8 of 128 into 4 bits, 42 MB: 13.4 us, 3.1 TB/s (a copy of as many bytes: 8.7).  One row of 32 heads: 2.7 us, a launch.
 #include "kernels.h"
 #include "longctx.h"
 

@@ -561,10 +561,11 @@ static RowsCut cut_rows(const AttnWindowParams &p, int compute_units) {
         steps = std::max(steps, count);
         keys += mean;
     }
-    // About one workgroup per compute unit, with a step for each wavefront at least.  Two steps per wavefront are not cut: joining costs a launch, about 3 us
-    // (32 heads, f16: 384 positions 7.4 us against 8.7 in two pieces, 512: 8.8 / 9.3, 768: 9.7 cut against 10.5, 1024: 9.7 / 12.0).
+    // About one workgroup per compute unit, with a step for each wavefront at least.  Up to two and a half steps per wavefront are not cut, nor up to four where there
+    // would be two pieces: joining costs a launch, about 3 us (f16, us, whole / cut; 32 heads, one text: 384 positions 7.4 / 8.7 in two pieces, 600: 9.3 / 9.5, 768:
+    // 10.5 / 9.7, 1024: 12.0 / 9.7; 16 texts of 8 key and value heads, in two pieces: 600: 9.6 / 11.3, 1000: 13.5 / 13.7).
     const int64_t want = std::max<int64_t>(1, compute_units / units);
-    const int64_t n = steps <= 2 * kAwWaves ? 1 : std::min<int64_t>({want, (steps + kAwWaves - 1) / kAwWaves, kMaxPieces});
+    const int64_t n = 2 * steps <= (want == 2 ? 8 : 5) * kAwWaves ? 1 : std::min<int64_t>({want, (steps + kAwWaves - 1) / kAwWaves, kMaxPieces});
     RowsCut cut;
     cut.piece_steps = (int)((steps + n - 1) / n);
     cut.pieces = (int)((steps + cut.piece_steps - 1) / cut.piece_steps);

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     constexpr int kIssues = kTileBytes / (kWaves * 1024) > 0 ? kTileBytes / (kWaves * 1024) : 1; // f16: wavefront-wide 1 KiB loads per tile of K (and of V)
     constexpr int kIssueRows = kWaves * 64 / kPieces;        // rows from one to the next: a multiple of what the permutations repeat after
     constexpr int kGroups = 2 * kAtKeys * HD / 32, kItems = kGroups / (64 * kWaves) > 0 ? kGroups / (64 * kWaves) : 1; // 4 bits: groups per tile, and per thread
-    static_assert(kTileBytes >= kWaves * 1024 || kIssues == 1, "a tile's shares");
+    static_assert((kTileBytes >= kWaves * 1024 || kIssues == 1) && 2 * kIssues == kKS, "a tile's shares, one load beside each step of the first product");
     const int my_row = (wave * 64 + lane) / kPieces, my_piece = lane % kPieces;
     const unsigned k_from = (my_piece ^ k_swz(my_row)) << 4, v_from = (my_piece ^ v_swz(my_row)) << 4; // within the row
     uint32_t codes[kQ4 ? kItems : 1][4], pairs[kQ4 ? kItems : 1];
@@ -194,6 +194,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     // ---- one tile: both products and the softmax of this wavefront's 64 keys
     const int v_row = half * 4 + ((lane & 15) >> 2);               // of the first run of four keys; the second one is 8 further
     const int v_piece = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1); // + 4 d
+    // fetch_more(ks): f16: called beside every step of the first product (all loads at once hold a wavefront up for 400 cycles); 4 bits: once behind it
     auto work = [&](unsigned stage, int t0, int last, auto whole, auto fetch_more) __attribute__((always_inline)) {
         const unsigned char *lds_k = lds + stage * kStageBytes + kh * (64 * kRowBytes), *lds_v = lds_k + kTileBytes;
         // S^T: the two 32-key products side by side, K read three steps ahead of them.  (Barriers against reordering: left alone, every read ends up right in
@@ -218,6 +219,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
             if (ks + 3 < kKS) read_k(ks + 3);
 #pragma unroll
             for (int t = 0; t < 2; t++) w[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_frag[ks % 4][t], q[ks], w[t], 0, 0, 0);
+            if constexpr (!kQ4) fetch_more(ks);
             if constexpr (kQ4) { // the next tile's codes are converted beside the products, which leave the vector ALU idle
 #pragma unroll
                 for (int word = ks * 4 * kItems / kKS; word < (ks + 1) * 4 * kItems / kKS; word++) place_word(1 - stage, word);
@@ -225,7 +227,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
-        fetch_more();
+        if constexpr (kQ4) fetch_more(0);
         half8_t v_frag[2][kDT];
         auto read_v = [&](int sl, int d) {
             const unsigned char *from = lds_v + (sl * 16 + v_row) * kRowBytes + (((d * 4 + v_piece) ^ v_swz(v_row)) << 4) + (lane & 1) * 8;
@@ -325,12 +327,16 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
                 do {
                     if constexpr (!kQ4) wait_vmcnt<0>();
                     __syncthreads();
-                    if constexpr (!kQ4) {
-                        fetch(row, kAtKeys, 1 - stage);
-                        row += kAtKeys;
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                    work(stage, 0, 0, std::true_type{}, [&]() __attribute__((always_inline)) { if constexpr (kQ4) fetch_ahead(s + 2); });
+                    work(stage, 0, 0, std::true_type{}, [&](int ks) __attribute__((always_inline)) {
+                        if constexpr (kQ4) fetch_ahead(s + 2);
+                        else if (kTileBytes >= kWaves * 1024 || wave < kTileBytes / 1024) {
+                            const half_t *from = reinterpret_cast<const half_t *>(ks < kIssues ? p.cache_k.data : p.cache_v.data) + row * HD;
+                            const int i = ks % kIssues;
+                            dma16_base(from, (unsigned)(my_row + i * kIssueRows) * kRowBytes + (ks < kIssues ? k_from : v_from),
+                                       lds_base + (1 - stage) * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u + (ks < kIssues ? 0 : kTileBytes));
+                        }
+                    });
+                    row += kAtKeys;
                     __builtin_amdgcn_sched_barrier(0);
                     stage = 1 - stage;
                 } while (++s < end);
@@ -355,7 +361,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
                 }
             }
             if (use) {
-                work(stage, at.t0 + kh * 64, at.last, std::false_type{}, [&]() __attribute__((always_inline)) { if constexpr (kQ4) fetch_ahead(s + 2); });
+                work(stage, at.t0 + kh * 64, at.last, std::false_type{}, [&](int) __attribute__((always_inline)) { if constexpr (kQ4) fetch_ahead(s + 2); });
             } else if constexpr (kQ4) {
                 place(1 - stage); // (behind the last tile: into a stage that is read no more)
                 fetch_ahead(s + 2);

@@ -493,9 +493,9 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
 //
 // A workgroup with two wavefronts per row group has a compute unit to itself; of those with one there are two on a compute unit.  Two are taken where the
 // workgroups would otherwise leave wavefronts idle: fewer of them than compute units, or at most two each while the first rows of a text see little of it
-// and their workgroups end early.  (1 / 2 wavefronts, 32 heads of 128: 1024 rows from position 0, 256 workgroups, 29.4 / 24.4 us; 1500, 384, 42.0 / 35.8;
-// 2048, 512, 57.2 / 52.2; over 4 bits 35.4 / 28.5, 50.1 / 40.2 and 66.4 / 59.3.  40 heads, 1700 rows, 560: 51.2 / 59.2; 2048, 640: 61.4 / 72.1.  1500 rows
-// that all see 1024 positions, 376: 54.3 / 68.4.)
+// and their workgroups end early.  (1 / 2 wavefronts, us, 32 heads of 128: 1024 rows from position 0, 256 workgroups, 23.1 / 21.8; 1500, 384, 36.1 / 32.4;
+// 2048, 512, 51.4 / 48.3; over 4 bits 27.9 / 25.8, 43.1 / 37.1 and 59.3 / 55.8.  40 heads, 1700 rows, 560: 46.4 / 53.3; 2048, 640: 56.8 / 64.1.  1500 rows
+// that all see 1024 positions, 376: 42.3 / 54.2.)
 //
 // Pieces (with two wavefronts per row group): a compute unit takes 2.3 us per tile of 128 rows and 128 keys of 128 dims; joining costs 4 us and writing and
 // reading the partial results, p * 2 (hd + 2) floats per row and head at about 4.5 bytes per ps.  The number of pieces with the least sum is taken.

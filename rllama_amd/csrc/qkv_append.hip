@@ -60,16 +60,18 @@ __global__ __launch_bounds__(kAppendThreads) void qkv_append_kernel(QkvAppendPar
     }
     // the row's angles and the norms' weights, once for all heads that this thread takes
     const float *turn = p.freqs + (size_t)pos * HD;
-    float angle[16], qw[8], kw[8];
+    float angle[16], qw[8], kw[8]; // neighbouring pairs: (cos, sin) four times; halves: eight cosines, and sines with the sign that this lane's part takes
     const bool second = dl >= kLanes / 2;
     if (p.halves) {
         float lo[8], hi[8];
         load8(turn + dl % (kLanes / 2) * 16, lo);
         load8(turn + dl % (kLanes / 2) * 16 + 8, hi);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            angle[i] = lo[i];
-            angle[i + 8] = hi[i];
+        for (int i = 0; i < 4; i++) {
+            angle[i] = lo[2 * i];
+            angle[i + 4] = hi[2 * i];
+            angle[i + 8] = second ? lo[2 * i + 1] : -lo[2 * i + 1];
+            angle[i + 12] = second ? hi[2 * i + 1] : -hi[2 * i + 1];
         }
     } else {
         float lo[8];
@@ -90,17 +92,17 @@ __global__ __launch_bounds__(kAppendThreads) void qkv_append_kernel(QkvAppendPar
                 float sq = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) sq = fmaf(v[u][i], v[u][i], sq);
-                const float r = 1.0f / sqrtf(group_sum<kLanes>(sq) / (float)HD + p.eps);
+                const float r = rsqrtf(group_sum<kLanes>(sq) / (float)HD + p.eps);
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[u][i] = v[u][i] * r * (kind == 0 ? qw[i] : kw[i]);
             }
             if (p.halves) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
+#pragma clang fp contract(off) // as rope_pair: products and their sum rounded one by one
                     const float other = other_half<kLanes>(v[u][i]);
-                    float re, im;
-                    rope_pair(second ? other : v[u][i], second ? v[u][i] : other, make_float2(angle[2 * i], angle[2 * i + 1]), re, im);
-                    v[u][i] = second ? im : re;
+                    const float own = v[u][i] * angle[i], turned = other * angle[i + 8];
+                    v[u][i] = own + turned;
                 }
             } else {
 #pragma unroll

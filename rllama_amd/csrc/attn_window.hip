@@ -15,8 +15,8 @@
 // the loop.  Tile e of O^T is made of the dims hd / 16 * m + e (m = 0 .. 15).
 //
 // Two arithmetics.  16 bits: f16 operands, v_mfma_f32_16x16x32_f16; the weights are rounded to f16 (half a unit in the eleventh bit each, which does not add up
-// over a text).  Values of 4 bits are not: a value is code * (upper part of the scale) + code * (rest) + lowest, two products that f16 holds exactly and a
-// term that is the same for 32 dims, and each goes through the matrix cores by itself.  32 bits: everything in f32 through v_mfma_f32_16x16x4_f32; also taken where f16
+// over a text).  Values of 4 bits are not: a value is 16 * code * (upper part of the scale / 16) + code * (rest) + lowest, two products that f16 holds exactly
+// for every scale and a term that is the same for 32 dims, and each goes through the matrix cores by itself.  32 bits: everything in f32 through v_mfma_f32_16x16x4_f32; also taken where f16
 // queries meet an f32 cache, whose values f16 may not hold.
 //
 // A text is cut into pieces when there are few rows: every workgroup leaves its (m, sum, O) in work memory and a second launch joins them.
@@ -93,7 +93,7 @@ struct Step<half_t, CT, HD> {
         half8_t q[kKs];
         half8_t sums; // 4 bits: the sum of the lane's dims of q in two f16 parts (the term of the lowest values)
     };
-    struct Sums { // 4 bits: the lowest values' part of O^T, row m for all dims kDims * m + e
+    struct Sums { // 4 bits: the lowest values' part of O^T, row m for all dims kDims * m + e; O^T itself is then kept divided by 16
         float4_t low;
     };
     uint32_t k[kTiles][kQ4 ? HD / 32 : HD / 8 /* words: a quarter of a row */];
@@ -158,7 +158,7 @@ struct Step<half_t, CT, HD> {
                 uint4_t hi, lo;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    hi[i] = __builtin_bit_cast(uint32_t, x[i] * scale.hi);
+                    hi[i] = __builtin_bit_cast(uint32_t, x[i] * scale.hi16);
                     lo[i] = __builtin_bit_cast(uint32_t, x[i] * scale.lo);
                 }
                 s = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, hi), q, s, 0, 0, 0);
@@ -169,8 +169,11 @@ struct Step<half_t, CT, HD> {
                 add(s0, rest0, scale0, k[0][c], of.q[c]);
                 add(s1, rest1, scale1, k[1][c], of.q[c]);
             }
-            s[0] = s0 + rest0;
-            s[1] = s1 + rest1;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[0][i] = fmaf(16.0f, s0[i], rest0[i]);
+                s[1][i] = fmaf(16.0f, s1[i], rest1[i]);
+            }
         } else {
 #pragma unroll
             for (int t = 0; t < kTiles; t++) s[t] = zero;
@@ -193,6 +196,9 @@ struct Step<half_t, CT, HD> {
         if constexpr (kQ4) {
             // positions two by two: the codes of dims 0 .. 3 of both in one word, those of dims 4 .. 7 in another, and each nibble of the pair
             // becomes a pair (first position, second position) of one dim
+            half8_t b16; // for the rest of the scales (of a sixteenth of a weight f16 keeps enough bits for a part of at most 2^-7 of the value)
+#pragma unroll
+            for (int i = 0; i < 8; i++) b16[i] = b[i] * (half_t)0.0625f;
             uint4_t low;
 #pragma unroll
             for (int j = 0; j < 4; j++) low[j] = perm(vp[2 * j + 1], vp[2 * j], kHiHalves);
@@ -208,7 +214,7 @@ struct Step<half_t, CT, HD> {
                     q4_codes_f16(bits, perm(v[2 * j + 1][0], v[2 * j][0], part ? kHiHalves : kLoHalves), y);
 #pragma unroll
                     for (int i = 0; i < kPart; i++) {
-                        hi[i][j] = __builtin_bit_cast(uint32_t, y[i] * scale.hi);
+                        hi[i][j] = __builtin_bit_cast(uint32_t, y[i] * scale.hi16);
                         lo[i][j] = __builtin_bit_cast(uint32_t, y[i] * scale.lo);
                     }
                 }
@@ -216,7 +222,7 @@ struct Step<half_t, CT, HD> {
                 for (int i = 0; i < kPart; i++) {
                     float4_t &to = o[part * kPart + i];
                     to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, hi[i]), b, to, 0, 0, 0);
-                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, lo[i]), b, to, 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, lo[i]), b16, to, 0, 0, 0);
                 }
             }
         } else {
@@ -235,7 +241,7 @@ struct Step<half_t, CT, HD> {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             if constexpr (kQ4) {
-                odd |= !q4_finite_f16(vp[j]);
+                odd |= !q4_finite(vp[j]);
             } else {
 #pragma unroll
                 for (int w = 0; w < kDims / 2; w++) odd |= ((v[j][w] & 0x7c000000u) == 0x7c000000u) || ((v[j][w] & 0x7c00u) == 0x7c00u);
@@ -433,14 +439,14 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
 #pragma unroll 1
                     for (int hh = 0; hh < 4; hh++) {
                         const int j = 16 * t + 4 * hh + i;
-                        const float wt = __shfl(w[t][i], hh * 16 + m, kWave);
+                        const float wt = __shfl(w[t][i], hh * 16 + m, kWave) * (St::kLowSums ? 0.0625f : 1.0f);
                         const bool seen = sees(t0 + j, here.last);
                         const size_t from = (plane + here.row + j) * HD + 4 * h * kDims;
 #pragma unroll
                         for (int x = 0; x < 4; x++)
 #pragma unroll
                             for (int e = 0; e < kDims; e++)
-                                if (seen) o[e][x] = fmaf(wt, plane_load1<CT, std::is_same_v<AC, half_t>>(p.cache_v, from + x * kDims + e), o[e][x]);
+                                if (seen) o[e][x] = fmaf(wt, plane_load1<CT, false>(p.cache_v, from + x * kDims + e), o[e][x]);
                     }
                 }
         }
@@ -473,7 +479,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
 #pragma unroll
     for (int x = 0; x < 4; x++)
 #pragma unroll
-        for (int e = 0; e < kDims; e++) so[wave][m][(4 * h + x) * kDims + e] = St::kLowSums ? o[e][x] + sums.low[x] : o[e][x];
+        for (int e = 0; e < kDims; e++) so[wave][m][(4 * h + x) * kDims + e] = St::kLowSums ? fmaf(16.0f, o[e][x], sums.low[x]) : o[e][x];
     __syncthreads();
     // thread: row tid / 32, dims HD / 32 of it
     constexpr int kPer = HD / 32;

@@ -64,16 +64,17 @@ __device__ __forceinline__ void q4_pairs_f16(const Q4Bits &bits, uint32_t w, hal
     for (int i = 0; i < 4; i++) out[i] = __builtin_elementwise_fma(out[i], scale, low);
 }
 // A scale as a sum of its upper seven bits and the rest: products of either part with a code have at most eleven bits, so f16 holds them exactly.
+// The upper part comes divided by 16: f16 holds that too (its last bit is 16 units of the scale's), and 15 codes of it for every scale there is.
 struct Q4Scale {
-    half2_t hi, lo;
-    __device__ explicit Q4Scale(uint32_t scales) : hi(__builtin_bit_cast(half2_t, scales & 0xfff0fff0u)), lo(__builtin_bit_cast(half2_t, scales) - hi) {}
+    half2_t hi16, lo;
+    __device__ explicit Q4Scale(uint32_t scales) {
+        const half2_t hi = __builtin_bit_cast(half2_t, scales & 0xfff0fff0u);
+        hi16 = hi * half2_t{(half_t)0.0625f, (half_t)0.0625f};
+        lo = __builtin_bit_cast(half2_t, scales) - hi;
+    }
 };
-// whether the values of a group are all finite as f16 numbers
-__device__ __forceinline__ bool q4_finite_f16(uint32_t pair) {
-    const half2_t x = __builtin_bit_cast(half2_t, pair);
-    const half_t top = __builtin_fmaf16((half_t)15.0f, x[0], x[1]);
-    return (int)(__builtin_fabsf16(x[1]) < (half_t)INFINITY) & (int)(__builtin_fabsf16(top) < (half_t)INFINITY);
-}
+// whether scale and lowest value of a group are finite
+__device__ __forceinline__ bool q4_finite(uint32_t pair) { return (int)((pair & 0x7c000000u) != 0x7c000000u) & (int)((pair & 0x7c00u) != 0x7c00u); }
 
 // One element; f16 arithmetic: with the rounding of q4_pairs_f16.
 template <typename T, bool kF16>

@@ -1,0 +1,43 @@
+"""The long-context operators at the edges of what their numbers and sizes allow, against their definitions in 64 bits."""
+import numpy as np
+import pytest
+
+from rllama_amd import Tensor, TensorDType
+from test_gpu_longctx import EPS16, NUMPY, attention_reference, f16, f32, f64, upload, values
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(ctx, q, K, V, cache, starts, window=0, sinks=0):
+    """q [B, n, H, hd] f16, K and V [B, G, S, hd] -> (what the call gives, the definition's values, the bound of f32 arithmetic, what the planes hold)."""
+    B, n, H, hd = q.shape
+    G, S = K.shape[1:3]
+    ck, cv = upload(ctx, K.reshape(-1, hd), cache), upload(ctx, V.reshape(-1, hd), cache)
+    K, V = (values(t).reshape(B, G, S, hd) for t in (ck, cv))
+    want, bound, _ = attention_reference(q.astype(f64), K, V, H, G, hd, starts, n, S, window, sinks)
+    got = Tensor.from_numpy(ctx, q.reshape(B * n, H * hd)).attn_window(ck, cv, H, G, S, starts, window=window, sinks=sinks)
+    return got.to_numpy().astype(f64).reshape(want.shape), want, bound, K, V
+
+
+# -- groups of 4 bits that span more than f16 does -----------------------------------------------------------------------------
+
+FEW = [(128, 4, 2, 1, 300), (64, 16, 1, 1, 90), (32, 6, 6, 3, 40), (128, 4, 1, 4, 2500)]  # hd, heads, kv heads, rows, positions
+
+
+@pytest.mark.parametrize("hd,H,G,n,S", FEW)
+def test_few_rows_over_wide_groups(ctx, hd, H, G, n, S):
+    """Groups from -40000 to 40000, seen and not seen: 15 steps of their scale are more than f16 holds, every value is less."""
+    rng = np.random.default_rng(hd + n)
+    start = S - n - 5
+    q = (rng.standard_normal((1, n, H, hd)) * 2e-4).astype(f16)
+    K, V = rng.standard_normal((1, G, S, hd)), rng.standard_normal((1, G, S, hd))
+    for x, at in ((K, (3, start, S - 1)), (V, (5, start, S - 2))):
+        x[0, :, at, :32] = np.linspace(-40000, 40000, 32)
+    got, want, bound, K, V = attend(ctx, q, K, V, "q4", [start])
+    # the weights' and the result's rounding to f16
+    assert (np.abs(got - want) <= bound + 2 * EPS16 * 40000).all()
+    # ... and where nobody sees a wide group, of what is seen
+    V[..., :] = np.clip(V, -8, 8)
+    V[0, :, S - 2, :32] = np.linspace(-40000, 40000, 32)
+    got, want, bound, _, V = attend(ctx, q, K, V, "q4", [start])
+    assert (np.abs(got - want) <= bound + 2 * EPS16 * np.abs(V[0, :, :start + n]).max()).all()

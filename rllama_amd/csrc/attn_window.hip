@@ -92,6 +92,7 @@ struct Step<half_t, CT, HD> {
     struct Queries {
         half8_t q[kKs];
         half8_t sums; // 4 bits: the sum of the lane's dims of q in two f16 parts (the term of the lowest values)
+        float up = 1.0f; // what the row's scores are to be multiplied by
     };
     struct Sums { // 4 bits: the lowest values' part of O^T, row m for all dims kDims * m + e; O^T itself is then kept divided by 16
         float4_t low;
@@ -116,6 +117,12 @@ struct Step<half_t, CT, HD> {
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < HD / 4; i++) sum += (float)row[h * (HD / 4) + i];
+            if (col_max(fabsf(sum)) > 65504.0f) { // f16 holds each of the dims but not their sum: the whole row by 2^-6, which is made up for later
+                to.up = 64.0f;
+                sum *= 0.015625f;
+#pragma unroll
+                for (int c = 0; c < kKs; c++) to.q[c] *= (half_t)0.015625f;
+            }
 #pragma unroll
             for (int i = 0; i < 8; i++) to.sums[i] = (half_t)0.0f;
             to.sums[0] = (half_t)sum;
@@ -263,6 +270,7 @@ struct Step<float, CT, HD> {
     static constexpr int kKWords = HD / 4 / kPerWord, kVWords = kQ4 ? 1 : kDims / kPerWord;
     struct Queries {
         float q[HD / 4];
+        static constexpr float up = 1.0f;
     };
     struct Sums {
         float4_t low; // (of the f16 form)
@@ -355,9 +363,9 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
     typename St::Sums sums{float4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 
     const size_t plane = (size_t)unit * p.max_seq_len;
-    const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
     typename St::Queries queries;
     St::load_q(queries, reinterpret_cast<const QT *>(p.q) + ((size_t)(b * p.n + my_i) * p.n_heads + g * group + (my_r - my_i * group)) * HD, h);
+    const float c2_all = 1.44269504088896340736f / sqrtf((float)HD), c2 = c2_all * queries.up; // (the second one is the row's own)
 
     struct Place {
         int t0, last, row; // positions t0 .. min(last, t0 + kStep - 1), row of the first one
@@ -473,7 +481,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
     // ---- join the wavefronts
     l_run = col_sum(l_run);
     if (h == 0) {
-        sm[wave][m] = m_run;
+        sm[wave][m] = m_run * queries.up;
         sl[wave][m] = l_run;
     }
 #pragma unroll
@@ -494,7 +502,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
             L += sl[w][jr];
             continue;
         }
-        const float f = __builtin_amdgcn_exp2f((sm[w][jr] - M) * c2);
+        const float f = __builtin_amdgcn_exp2f((sm[w][jr] - M) * c2_all);
         L = fmaf(sl[w][jr], f, L);
 #pragma unroll
         for (int i = 0; i < kPer; i++) O[i] = fmaf(so[w][jr][jd + i], f, O[i]);

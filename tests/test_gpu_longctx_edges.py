@@ -41,3 +41,14 @@ def test_few_rows_over_wide_groups(ctx, hd, H, G, n, S):
     V[0, :, S - 2, :32] = np.linspace(-40000, 40000, 32)
     got, want, bound, _, V = attend(ctx, q, K, V, "q4", [start])
     assert (np.abs(got - want) <= bound + 2 * EPS16 * np.abs(V[0, :, :start + n]).max()).all()
+
+
+@pytest.mark.parametrize("hd,H,G,n,S", FEW)
+def test_few_rows_of_large_queries_over_4_bits(ctx, hd, H, G, n, S):
+    """The sum of a quarter of a query is more than f16 holds."""
+    rng = np.random.default_rng(hd + n)
+    big = 65504 / (hd // 4) * 2
+    q = (rng.uniform(0.8, 1.2, (1, n, H, hd)) * np.where(rng.random((1, n, H, 1)) < 0.7, big, 1.5)).astype(f16)
+    K, V = rng.standard_normal((1, G, S, hd)) * 2 / (big * np.sqrt(hd)), rng.standard_normal((1, G, S, hd))
+    got, want, bound, _, V = attend(ctx, q, K, V, "q4", [S - n])
+    assert (np.abs(got - want) <= bound + 2 * EPS16 * np.abs(V).max()).all()

@@ -337,8 +337,9 @@ int  rlh_qkv_append(rlh_tensor *q, const rlh_tensor *qkv, const rlh_tensor *q_no
 /* Attention of the rows over the planes, which hold the rows' own positions already: the row at position p sees the positions
  * t <= p with t < sinks or t > p - window (window 0: all of them), out = softmax(q K^T / sqrt(head_dim)) V.  q and out
  * [n_seqs * n x n_heads head_dim], both f16 or both f32.  f32 rows, or an f32 cache: f32 arithmetic throughout.  Otherwise f16 operands with
- * f32 sums: the softmax's weights are rounded to f16 in front of the second product, and values of 4 bits are rounded to f16 (half a unit,
- * 2^-12 of the value) where many rows share a key and value head; up to 16 rows always read them exactly.  Rows and keys outside what
+ * f32 sums: the softmax's weights are rounded to f16 in front of the second product, and values of 4 bits are rounded to f16 (half a unit in
+ * the eleventh bit, up to 2^-11 of the value) where many rows share a key and value head; up to 16 rows always read them exactly.  Values
+ * of 4 bits beyond what f16 holds are read exactly in both; with many rows such a call takes some 300 times as long.  Rows and keys outside what
  * is seen may hold anything, NaN included.  Positions beyond max_seq_len need window > 0 and sinks + window + n - 1 <= max_seq_len.
  * The first call of a size allocates work memory that stays with the context (partial results of a sequence that is cut). */
 int  rlh_attn_window(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *cache_k, const rlh_tensor *cache_v, int n_heads, int n_kv_heads,

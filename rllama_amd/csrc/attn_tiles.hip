@@ -6,7 +6,7 @@
 // codes, converts them in registers and writes 64 bytes, so a code is converted once per workgroup and not once per wavefront.
 //
 // Rounded to f16: the softmax's weights, as operands of the second product, and 4-bit values when they are converted (lowest + code * scale, one rounding of at most
-// 2^-12 of the value, where the codes themselves are off by 1/30 of a group's range).  Random values, a window of 1024: the result is off by 4.6e-4 of its size, 2.6e-4
+// 2^-11 of the value, where the codes themselves are off by 1/30 of a group's range).  Random values, a window of 1024: the result is off by 4.6e-4 of its size, 2.6e-4
 // with an f16 cache, 2.1e-4 with nothing but the result rounded.  Exact values would take two products for each of these.
 //
 // Tiles that every row of the wavefront sees whole, in the middle of a run of rows that lie side by side in the cache, go through a loop of their own with
@@ -66,6 +66,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     constexpr int kLdsBytes = 2 * kStageBytes > kEndBytes ? 2 * kStageBytes : kEndBytes;
     static_assert(32 * kOutRow * 2 <= kJoinFloats * 4, "a row group's output goes where its join was");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
+    __shared__ int sh_wide; // 4 bits: some group of the tiles holds a value that is infinity in f16
 
     const AttnWindowParams &p = pp.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -157,6 +158,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
         }
     };
     const Q4Bits bits;
+    bool wide = false;
     // 4 bits: word w of the fetched codes (eight of them) as f16 into a stage
     auto place_word = [&](unsigned stage, int word) __attribute__((always_inline)) {
         const int i = word / 4, w = word % 4;
@@ -165,6 +167,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
         const unsigned at_group = item % (kGroups / 2), r = at_group / (HD / 32), c = at_group % (HD / 32) * 4 + w;
         const bool is_v = item >= kGroups / 2;
         const half2_t pair = __builtin_bit_cast(half2_t, pairs[i]), scale = {pair[0], pair[0]}, low = {pair[1], pair[1]};
+        if (w == 0) wide |= __builtin_fabsf16(__builtin_fmaf16((half_t)15.0f, pair[0], pair[1])) == (half_t)INFINITY;
         half2_t x[4];
         q4_pairs_f16(bits, codes[i][w], scale, low, x);
         uint4_t y;
@@ -296,6 +299,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
         l_run += sum[0] + sum[1];
     };
 
+    if (kQ4 && tid == 0) sh_wide = 0;
     if (s_first < s_end) {
         Place at = place_of(s_first), ahead = at; // `ahead`: the tile after the one fetched last
         auto fetch_ahead = [&](int s) __attribute__((always_inline)) {
@@ -374,23 +378,40 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
         }
     }
 
-    if (__any(skipped)) {
+    bool anew = false; // every tile again
+    if constexpr (kQ4) {
+        if (wide) sh_wide = 1; // (0 since before the barriers of the loop, without which there is no tile)
+        __syncthreads();
+        anew = sh_wide != 0;
+    }
+    if (anew) {
+        m_run = -INFINITY;
+        l_run = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDT; d++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
+    }
+    if (anew || __any(skipped)) {
         // Tiles that hold a value of V that is not finite and that some row of the wavefront may not see (weight 0 would make a NaN of it in the product)
-        // were left out above.  Here every row adds up what it sees, key by key in f32.
+        // were left out above.  Here every row adds up what it sees, key by key in f32.  So it does with all tiles where 4 bits stand for values that f16
+        // does not hold (a group from -65504 to 65504 reads as 65536 at its upper end): 1500 rows of 32 heads on 8 then take 14.6 ms instead of 48 us.
         for (int s = s_first; s < s_end; s++) {
             const Place at = place_of(s);
-            if (unseen_half(at) || whole_half(at)) continue;
+            if (unseen_half(at) || (!anew && whole_half(at))) continue;
             const int t0 = at.t0 + kh * 64, here = min(64, at.last - t0 + 1);
             const size_t row = plane + at.row + kh * 64;
-            bool odd = false;
-            for (int i = lane; i < here * HD; i += 64) odd |= !(fabsf(plane_load1<CT, true>(p.cache_v, row * HD + i)) < INFINITY);
-            if (!__any(odd)) continue;
+            if (!anew) {
+                bool odd = false;
+                for (int i = lane; i < here * HD; i += 64) odd |= !(fabsf(plane_load1<CT>(p.cache_v, row * HD + i)) < INFINITY);
+                if (!__any(odd)) continue;
+            }
 #pragma unroll 1
             for (int j = 0; j < here; j++) {
                 const size_t from = (row + j) * HD;
                 float dot = 0.0f;
 #pragma unroll 1
-                for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d++) dot = fmaf((float)q_row[d], plane_load1<CT, true>(p.cache_k, from + d), dot);
+                for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d++) dot = fmaf((float)q_row[d], plane_load1<CT>(p.cache_k, from + d), dot);
                 dot += __shfl_xor(dot, 32, 64);
                 const bool seen = sees(t0 + j, at.last);
                 const float m_new = seen ? fmaxf(m_run, dot) : m_run;
@@ -403,7 +424,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
 #pragma unroll
                     for (int v = 0; v < 16; v++) {
                         const int dim8 = (v >> 2) * 8, in8 = half * 4 + (v & 3); // place in O^T
-                        const float x = plane_load1<CT, true>(p.cache_v, from + d * 32 + dim8 + (kQ4 ? (in8 >> 1) + 4 * (in8 & 1) : in8));
+                        const float x = plane_load1<CT>(p.cache_v, from + d * 32 + dim8 + (kQ4 ? (in8 >> 1) + 4 * (in8 & 1) : in8));
                         o[d][v] = seen ? fmaf(wt, x, o[d][v] * alpha) : o[d][v];
                     }
             }

@@ -454,7 +454,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
                         for (int x = 0; x < 4; x++)
 #pragma unroll
                             for (int e = 0; e < kDims; e++)
-                                if (seen) o[e][x] = fmaf(wt, plane_load1<CT, false>(p.cache_v, from + x * kDims + e), o[e][x]);
+                                if (seen) o[e][x] = fmaf(wt, plane_load1<CT>(p.cache_v, from + x * kDims + e), o[e][x]);
                     }
                 }
         }

@@ -76,13 +76,12 @@ struct Q4Scale {
 // whether scale and lowest value of a group are finite
 __device__ __forceinline__ bool q4_finite(uint32_t pair) { return (int)((pair & 0x7c000000u) != 0x7c000000u) & (int)((pair & 0x7c00u) != 0x7c00u); }
 
-// One element; f16 arithmetic: with the rounding of q4_pairs_f16.
-template <typename T, bool kF16>
+// One element
+template <typename T>
 __device__ __forceinline__ float plane_load1(const PlaneRef &p, size_t at) {
     if constexpr (std::is_same_v<T, Quant4>) {
         const uint32_t pair = p.pairs[at / 32], c = (reinterpret_cast<const uint8_t *>(p.data)[at / 2] >> (4 * (at & 1))) & 15u;
-        if constexpr (kF16) return (float)__builtin_fmaf16((half_t)(float)c, __builtin_bit_cast(half2_t, pair)[0], __builtin_bit_cast(half2_t, pair)[1]);
-        else return fmaf((float)c, q4_scale(pair), q4_lowest(pair));
+        return fmaf((float)c, q4_scale(pair), q4_lowest(pair));
     } else {
         return (float)reinterpret_cast<const T *>(p.data)[at];
     }

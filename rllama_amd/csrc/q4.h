@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t q4_encode8(const float (&v)[8], uint32_t &pa
     pair = (uint32_t)__builtin_bit_cast(uint16_t, scale) | ((uint32_t)__builtin_bit_cast(uint16_t, low) << 16);
     const float s = (float)scale, l = (float)low;
     if (s > 0.0f) {
-        // (v - l) / s rounded to a whole number, by the reciprocal: within 2^-20 of the quotient up to 16, so only next to a tie is the quotient itself needed
+        // (v - l) / s rounded to a whole number, by the reciprocal: within 2^-19 of the quotient up to 16 (two roundings), so only next to a tie is the quotient itself needed
         const float inv = 1.0f / s;
         bool tie = false;
         float c[8];

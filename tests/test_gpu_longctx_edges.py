@@ -52,3 +52,22 @@ def test_few_rows_of_large_queries_over_4_bits(ctx, hd, H, G, n, S):
     K, V = rng.standard_normal((1, G, S, hd)) * 2 / (big * np.sqrt(hd)), rng.standard_normal((1, G, S, hd))
     got, want, bound, _, V = attend(ctx, q, K, V, "q4", [S - n])
     assert (np.abs(got - want) <= bound + 2 * EPS16 * np.abs(V).max()).all()
+
+
+# -- values of 4 bits that f16 does not hold ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("hd,H,G,n,S,top", [(128, 32, 8, 600, 620, 65504), (64, 4, 1, 200, 9205, 65504), (32, 40, 40, 500, 600, 65504), (128, 2, 2, 150, 300, 65504),
+                                            (128, 4, 2, 1, 300, 65504), (64, 36, 12, 600, 700, 3e5), (128, 8, 2, 200, 2000, 3e5), (64, 8, 2, 3, 500, 3e5)])
+def test_values_of_4_bits_beyond_f16(ctx, hd, H, G, n, S, top):
+    """Groups from -65504 up: the highest value reads as 65536 or more, whose place in f16 is infinity."""
+    rng = np.random.default_rng(hd + n)
+    start = S - n - 5
+    q = (rng.standard_normal((1, n, H, hd)) * 1e-4).astype(f16)
+    K, V = rng.standard_normal((1, G, S, hd)), rng.standard_normal((1, G, S, hd))
+    for x, at in ((K, (3, start + n // 2, S - 1)), (V, (5, start + n // 3, S - 2))):
+        x[0, :, at, :32] = np.linspace(-65504, top, 32)
+    got, want, bound, K, V = attend(ctx, q, K, V, "q4", [start])
+    assert max(K.max(), V.max()) > 65520
+    over = np.abs(want) > 65520  # (results of few positions among values of 300000)
+    assert (got[over] == np.copysign(np.inf, want[over])).all() and np.isfinite(got[~over]).all()
+    assert (np.abs(got - want) <= bound + 2 * EPS16 * np.abs(V).max())[~over].all()

@@ -71,3 +71,19 @@ def test_values_of_4_bits_beyond_f16(ctx, hd, H, G, n, S, top):
     over = np.abs(want) > 65520  # (results of few positions among values of 300000)
     assert (got[over] == np.copysign(np.inf, want[over])).all() and np.isfinite(got[~over]).all()
     assert (np.abs(got - want) <= bound + 2 * EPS16 * np.abs(V).max())[~over].all()
+
+
+# -- 4 bits and few rows: nothing but the weights and the result is rounded ----------------------------------------------------------
+
+@pytest.mark.parametrize("hd,H,G,n,S,window,sinks", [(128, 4, 2, 1, 1000, 0, 0), (128, 32, 4, 2, 700, 0, 0), (64, 8, 1, 2, 5000, 0, 0), (32, 3, 3, 16, 333, 0, 0),
+                                                     (128, 8, 8, 5, 3000, 300, 4)])
+def test_up_to_16_rows_read_4_bits_exactly(ctx, hd, H, G, n, S, window, sinks):
+    rng = np.random.default_rng(hd + n)
+    q = (rng.standard_normal((1, n, H, hd)) * 1.5).astype(f16)
+    # keys far from zero and large queries: rounding a key's values to f16 would move the scores by more than the rest of the call does
+    q, K, V = q * f16(4), rng.standard_normal((1, G, S, hd)) + 8.0, rng.standard_normal((1, G, S, hd))
+    got, want, bound, _, V = attend(ctx, q, K, V, "q4", [S - n], window, sinks)
+    error = np.abs(got - want)
+    assert (error <= bound + 2 * EPS16 * np.abs(V).max()).all()
+    # on average: the result's rounding, and the weights', which fall on V independently of each other
+    assert error.mean() <= EPS16 * (np.abs(want).mean() + np.sqrt((V * V).mean()))

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
 #pragma unroll
             for (int v = 0; v < 16; v++) top = fmaxf(top, w[t][v]);
         top = fmaxf(top, other_half_lane(top));
-        // the reference point follows the maximum when some row's has grown by more than 2^8: weights stay below 2^8
+        // the reference point follows the maximum when some row's has grown by more than 2^8: weights stay below 2^8 times what they are carried by
         const float m_new = fmaxf(m_run, top);
         if (__any((m_new - m_run) * c2 > 8.0f)) {
             const float alpha = m_run > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 0.0f;
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
 #pragma unroll
                 for (int v = 0; v < 16; v++) o[d][v] *= alpha;
         }
-        const float mc = m_run > -INFINITY ? m_run * c2 : 0.0f;
+        const float mc = (m_run > -INFINITY ? m_run * c2 : 0.0f) - kWeightLift;
         // O^T += V^T . W, 16 keys at a time: between the products of one step the weights of the next are formed and its V is read
         half8_t h[2];
         float sum[2] = {0.0f, 0.0f};
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
                 const bool seen = sees(t0 + j, at.last);
                 const float m_new = seen ? fmaxf(m_run, dot) : m_run;
                 const float alpha = m_new > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 1.0f;
-                const float wt = seen ? __builtin_amdgcn_exp2f((dot - (m_new > -INFINITY ? m_new : 0.0f)) * c2) : 0.0f;
+                const float wt = seen ? __builtin_amdgcn_exp2f(fmaf(dot - (m_new > -INFINITY ? m_new : 0.0f), c2, kWeightLift)) : 0.0f;
                 m_run = m_new;
                 l_run = fmaf(l_run, alpha, half == 0 ? wt : 0.0f);
 #pragma unroll

@@ -14,8 +14,8 @@
 // transposes them in registers with byte permutes, so cached rows go from memory into registers and nowhere else: no LDS, no barrier in
 // the loop.  Tile e of O^T is made of the dims hd / 16 * m + e (m = 0 .. 15).
 //
-// Two arithmetics.  16 bits: f16 operands, v_mfma_f32_16x16x32_f16; the weights are rounded to f16 (half a unit in the eleventh bit each, which does not add up
-// over a text).  Values of 4 bits are not: a value is 16 * code * (upper part of the scale / 16) + code * (rest) + lowest, two products that f16 holds exactly
+// Two arithmetics.  16 bits: f16 operands, v_mfma_f32_16x16x32_f16; the weights are rounded to f16 (half a unit in the eleventh bit each, also far below the largest: kWeightLift;
+// they do not add up over a text).  Values of 4 bits are not: a value is 16 * code * (upper part of the scale / 16) + code * (rest) + lowest, two products that f16 holds exactly
 // for every scale and a term that is the same for 32 dims, and each goes through the matrix cores by itself.  32 bits: everything in f32 through v_mfma_f32_16x16x4_f32; also taken where f16
 // queries meet an f32 cache, whose values f16 may not hold.
 //
@@ -85,6 +85,7 @@ struct Step<half_t, CT, HD> {
     static constexpr int kPositions = 32;
     static constexpr bool kLowSums = std::is_same_v<CT, Quant4>;
     static constexpr int kTiles = 2;            // of 16 positions
+    static constexpr float kLift = kWeightLift;
     static constexpr int kKs = HD / 32;         // MFMAs per score tile
     static constexpr int kDims = HD / 16;       // neighbouring dims of V per lane = tiles of O^T
     static constexpr bool kQ4 = std::is_same_v<CT, Quant4>;
@@ -264,6 +265,7 @@ struct Step<float, CT, HD> {
     static constexpr int kPositions = 16;
     static constexpr bool kLowSums = false;
     static constexpr int kTiles = 1;
+    static constexpr float kLift = 0.0f; // (weights stay in f32)
     static constexpr int kDims = HD / 16;
     static constexpr bool kQ4 = std::is_same_v<CT, Quant4>;
     static constexpr int kPerWord = kQ4 ? 8 : std::is_same_v<CT, half_t> ? 2 : 1;
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
 #pragma unroll
             for (int i = 0; i < 4; i++) top = fmaxf(top, w[t][i]);
         // The reference point of the exponentials follows the maximum only when some row's has grown by more than 2^8 (any point gives the same
-        // softmax): weights stay below 2^8, and rescaling leaves the common path.
+        // softmax): weights stay below 2^8 times what they are carried by, and rescaling leaves the common path.
         const float m_new = fmaxf(m_run, col_max(top));
         if (__any((m_new - m_run) * c2 > 8.0f)) { // the first maximum: infinity
             const float alpha = m_run > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 0.0f;
@@ -427,7 +429,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
             for (int e = 0; e < kDims; e++) o[e] *= alpha;
             if constexpr (St::kLowSums) sums.low *= alpha;
         }
-        const float mc = m_run > -INFINITY ? m_run * c2 : 0.0f;
+        const float mc = (m_run > -INFINITY ? m_run * c2 : 0.0f) - St::kLift;
         float sum = 0.0f;
 #pragma unroll
         for (int t = 0; t < kTiles; t++)

@@ -87,3 +87,31 @@ def test_up_to_16_rows_read_4_bits_exactly(ctx, hd, H, G, n, S, window, sinks):
     assert (error <= bound + 2 * EPS16 * np.abs(V).max()).all()
     # on average: the result's rounding, and the weights', which fall on V independently of each other
     assert error.mean() <= EPS16 * (np.abs(want).mean() + np.sqrt((V * V).mean()))
+
+
+# -- a first token that takes most of the weight -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("hd,H,G,n,T", [(128, 4, 2, 1, 20000), (64, 8, 1, 2, 65700), (128, 8, 2, 60, 12000), (64, 4, 1, 200, 9000), (128, 32, 8, 130, 6000)])
+@pytest.mark.parametrize("cache", ["f16", "q4"])
+@pytest.mark.parametrize("share", [0.1, 0.02, 0.002])
+def test_what_a_dominating_first_token_leaves(ctx, hd, H, G, n, T, cache, share):
+    """All but `share` of the weight is on position 0, the rest on thousands of others alike."""
+    rng = np.random.default_rng(T)
+    S = T + n
+    K, V = np.zeros((1, G, S, hd)), np.zeros((1, G, S, hd))
+    q = np.zeros((1, n, H, hd))
+    q[..., 0] = 8.0
+    # keys and values that 4 bits and f16 both hold: fifteen steps of a scale of few bits, sixteenths
+    K[:, :, 0, 0] = 15 * np.rint(np.log((1 - share) / share * T) * np.sqrt(hd) / 8.0 / 15 * 32) / 32
+    steps = rng.integers(0, 16, hd)
+    steps[0::32], steps[1::32] = 0, 15
+    V[:, :, 1:] = 0.5 + steps / 16
+    ck, cv = upload(ctx, K.reshape(-1, hd), cache), upload(ctx, V.reshape(-1, hd), cache)
+    K, V = (values(t).reshape(1, G, S, hd) for t in (ck, cv))
+    got = Tensor.from_numpy(ctx, q.reshape(n, -1).astype(f16)).attn_window(ck, cv, H, G, S, [T]).to_numpy().astype(f64).reshape(n, H, hd)
+    first = np.exp(8.0 * K[0, :, 0, 0] / np.sqrt(hd))  # [G]; the others' weights are 1
+    rest = T + np.arange(n)
+    want = (rest[:, None] / (first + rest[:, None]))[..., None] * V[0, None, :, 1]
+    want = np.repeat(want, H // G, 1)
+    # weights and result are rounded to f16, relative to themselves; sums in f32
+    assert (np.abs(got / want - 1) <= 2 * EPS16 + (4 * np.sqrt(S) + 200) * 2.0 ** -24).all()

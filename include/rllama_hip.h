@@ -312,7 +312,7 @@ int  rlh_argmax_greedy(const rlh_tensor *logits, float temperature, int32_t *tok
  * first `sinks`: row sinks + (t - sinks) % (max_seq_len - sinks).  Both calls below take the same `sinks`.
  * ---------------------------------------------------------------------------------------------- */
 /* A tensor over device memory that the caller owns (another library's, on this device; 16-byte aligned): nothing is copied, and
- * rlh_tensor_free frees only the handle, when the context's queued work is done.  The memory has to outlive the handle.  Work that the
+ * rlh_tensor_free frees only the handle, when the queued work that uses it is done, other contexts' too.  The memory has to outlive the handle.  Work that the
  * caller queued on a stream of its own is not seen: order it with the two calls below. */
 int  rlh_tensor_wrap(rlh_ctx *ctx, void *device_memory, int rows, int cols, int dtype, rlh_tensor **out);
 /* The context's later work waits for what is queued on `stream` (a hipStream_t; NULL = the default stream) by now ... */

@@ -89,8 +89,9 @@ extern "C" void rlh_tensor_free(rlh_tensor *t) {
     if (!t) return;
     CtxLock lock(t->ctx);
     TensorPool &pool = t->ctx->pool;
-    if (t->wrapped) {
-        (void)hipStreamSynchronize(t->ctx->stream); // the memory is the caller's again
+    if (t->wrapped) { // the memory is the caller's again
+        if (t->lent.load(std::memory_order_relaxed)) (void)hipDeviceSynchronize(); // (another context's work may read it yet)
+        else (void)hipStreamSynchronize(t->ctx->stream);
     } else if (t->p && TensorPool::keeps(t->capacity) && !t->lent.load(std::memory_order_relaxed)) {
         if (!pool.room(t->capacity)) {
             (void)hipStreamSynchronize(t->ctx->stream);

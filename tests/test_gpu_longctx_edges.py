@@ -1,8 +1,11 @@
 """The long-context operators at the edges of what their numbers and sizes allow, against their definitions in 64 bits."""
+import ctypes
+
 import numpy as np
 import pytest
 
-from rllama_amd import Tensor, TensorDType
+import rllama_amd
+from rllama_amd import Context, Tensor, TensorDType
 from test_gpu_longctx import EPS16, NUMPY, attention_reference, f16, f32, f64, upload, values
 
 pytestmark = pytest.mark.gpu
@@ -115,3 +118,37 @@ def test_what_a_dominating_first_token_leaves(ctx, hd, H, G, n, T, cache, share)
     want = np.repeat(want, H // G, 1)
     # weights and result are rounded to f16, relative to themselves; sums in f32
     assert (np.abs(got / want - 1) <= 2 * EPS16 + (4 * np.sqrt(S) + 200) * 2.0 ** -24).all()
+
+
+# -- memory of another owner -----------------------------------------------------------------------------------------------------------------
+
+def hip_runtime():
+    """The HIP runtime that the library has loaded."""
+    with open("/proc/self/maps") as f:
+        return ctypes.CDLL(next(line.split()[-1] for line in f if "libamdhip64" in line))
+
+
+def test_freeing_a_wrapped_tensor_waits_for_other_contexts(ctx):
+    """The owner may use the memory again: what another context had queued on it is done."""
+    other, hip = Context(0), hip_runtime()
+    x = np.arange(64 * 96, dtype=f32).reshape(64, 96)
+    memory = ctypes.c_void_p()
+    put = lambda a: hip.hipMemcpy(memory, a.ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(a.nbytes), 1)  # noqa: E731
+    assert hip.hipMalloc(ctypes.byref(memory), ctypes.c_size_t(x.nbytes)) == 0
+    try:
+        assert put(x) == 0
+        wrapped = Tensor.from_device(ctx, memory.value, 64, 96, TensorDType.Float32)
+        a, b, c = (Tensor.zeros(other, 8192, 8192, TensorDType.Float16) for _ in range(3))
+        got = Tensor.zeros(other, 64, 96, TensorDType.Float32)
+        other.sync()
+        for _ in range(60):  # keeps the other context's stream busy for some 50 ms
+            rllama_amd._lib.check(ctx._lib.rlh_matrix_mul_inplace_transposed(c._h, a._h, b._h))
+        rllama_amd._lib.check(ctx._lib.rlh_copy_inplace(got._h, wrapped._h))
+        wrapped.free()
+        assert put(np.zeros_like(x)) == 0
+        assert np.array_equal(got.to_numpy(), x)
+        for t in (a, b, c, got):
+            t.free()
+    finally:
+        other.close()
+        assert hip.hipFree(memory) == 0

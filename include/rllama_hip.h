@@ -301,7 +301,7 @@ int  rlh_argmax_greedy(const rlh_tensor *logits, float temperature, int32_t *tok
 /* ------------------------------------------------------------------------------------------------
  * Long contexts and drafted tokens (no reference counterpart): the attention block over caches of 16, 32 or 4 bits with grouped
  * heads, several sequences and a sliding window, and the choice of tokens from rows of logits.  All work is queued on the
- * context's stream; no call here waits for it, and none allocates device memory except where it says so.
+ * context's stream; no call here waits for it or allocates device memory except where it says so.
  *
  * Rows and positions.  A call takes n rows of each of n_seqs sequences (1..256): row b * n + i of its tensors is sequence b's
  * row at position start_pos[b] + i.  A negative position is padding (rows on the left of a short prompt, an idle slot of a batch):
@@ -341,7 +341,8 @@ int  rlh_qkv_append(rlh_tensor *q, const rlh_tensor *qkv, const rlh_tensor *q_no
  * the eleventh bit, up to 2^-11 of the value) where many rows share a key and value head; up to 16 rows always read them exactly.  Values
  * of 4 bits beyond what f16 holds are read exactly in both; with many rows such a call takes some 300 times as long.  Rows and keys outside what
  * is seen may hold anything, NaN included.  Positions beyond max_seq_len need window > 0 and sinks + window + n - 1 <= max_seq_len.
- * The first call of a size allocates work memory that stays with the context (partial results of a sequence that is cut). */
+ * Partial results of sequences that are cut go to work memory that stays with the context, 34 MB at most.  A call that needs more than every
+ * one before it waits for the context's queued work and allocates it: of a text that gets longer one call or two, when it is first cut. */
 int  rlh_attn_window(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *cache_k, const rlh_tensor *cache_v, int n_heads, int n_kv_heads,
                      int max_seq_len, const int32_t *start_pos, int n_seqs, int window, int sinks);
 /* Probabilities of rows of logits: probs f32 [n x vocab] = softmax(logits / temperature), logits f16 or f32.  temperature 0: 1 at the

@@ -523,6 +523,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
 // What a call takes is about that and 6.5 us.
 struct TilesCut {
     int shares, pieces, piece_steps;
+    int most; // pieces of a text of any length
     double us;
 };
 constexpr int kCutKeys = 128;
@@ -553,6 +554,7 @@ static TilesCut cut_tiles(const AttnWindowParams &p, int compute_units) {
     }
     TilesCut cut;
     cut.us = 6.5 + best;
+    cut.most = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxPieces, 2 * compute_units / units));
     cut.piece_steps = (int)((steps + n - 1) / n);
     cut.pieces = (int)((steps + cut.piece_steps - 1) / cut.piece_steps);
     cut.shares = cut.pieces > 1 || units <= (uneven ? 2 : 1) * compute_units ? 2 : 1;
@@ -562,8 +564,8 @@ static TilesCut cut_tiles(const AttnWindowParams &p, int compute_units) {
 double attn_tiles_us(const AttnWindowParams &p, int compute_units) { return cut_tiles(p, compute_units).us; }
 
 size_t attn_tiles_work_floats(const AttnWindowParams &p, int compute_units) {
-    const int pieces = cut_tiles(p, compute_units).pieces;
-    return pieces > 1 ? (size_t)p.n * p.n_heads * p.n_seqs * pieces * (p.head_dim + 2) : 0;
+    const TilesCut cut = cut_tiles(p, compute_units);
+    return cut.pieces > 1 ? (size_t)p.n * p.n_heads * p.n_seqs * cut.most * (p.head_dim + 2) : 0;
 }
 
 template <typename CT, int HD>

@@ -555,6 +555,7 @@ static bool f16_arithmetic(const AttnWindowParams &p) { return p.f16 && p.cache 
 // How the texts are cut: pieces of `piece_steps` steps, at most `pieces` of them; and about what the call takes.
 struct RowsCut {
     int pieces, piece_steps;
+    int most; // pieces of a text of any length
     double us;
 };
 static RowsCut cut_rows(const AttnWindowParams &p, int compute_units) {
@@ -583,6 +584,7 @@ static RowsCut cut_rows(const AttnWindowParams &p, int compute_units) {
     const int64_t want = std::max<int64_t>(1, compute_units / units);
     const int64_t n = 2 * steps <= (want == 2 ? 8 : 5) * kAwWaves ? 1 : std::min<int64_t>({want, (steps + kAwWaves - 1) / kAwWaves, kMaxPieces});
     RowsCut cut;
+    cut.most = (int)std::min<int64_t>(want, kMaxPieces);
     cut.piece_steps = (int)((steps + n - 1) / n);
     cut.pieces = (int)((steps + cut.piece_steps - 1) / cut.piece_steps);
     cut.us = 5.0 + (cut.pieces > 1 ? 3.5 : 0.0) + units * 0.01 + tiles * p.n_kv * keys * p.head_dim / 128 * 30e-6 + (double)cut.piece_steps * step * p.head_dim / 128 * 4e-3;
@@ -599,8 +601,8 @@ static bool tiles_take(const AttnWindowParams &p, int compute_units) {
 
 size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units) {
     if (tiles_take(p, compute_units)) return attn_tiles_work_floats(p, compute_units);
-    const int pieces = cut_rows(p, compute_units).pieces;
-    return pieces > 1 ? (size_t)p.n * p.n_heads * p.n_seqs * pieces * (p.head_dim + 2) : 0;
+    const RowsCut cut = cut_rows(p, compute_units);
+    return cut.pieces > 1 ? (size_t)p.n * p.n_heads * p.n_seqs * cut.most * (p.head_dim + 2) : 0;
 }
 
 hipError_t launch_attn_window(const AttnWindowParams &a, int compute_units, float *ws, hipStream_t s) {

@@ -35,7 +35,8 @@ struct AttnWindowParams {
     int window, sinks;     // window 0: everything up to the row's own position
     int32_t start[kLongMaxSeqs];
 };
-size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units); // partial results of texts that are cut
+// work memory for partial results where this call cuts its texts: enough for as many pieces as texts of any length are cut into, at most 512 workgroups' rows (34 MB)
+size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units);
 // the form for many rows (attn_tiles.hip): which calls it takes, its work memory and its launch
 double attn_tiles_us(const AttnWindowParams &p, int compute_units); // about what a call takes
 size_t attn_tiles_work_floats(const AttnWindowParams &p, int compute_units);

@@ -152,3 +152,29 @@ def test_freeing_a_wrapped_tensor_waits_for_other_contexts(ctx):
     finally:
         other.close()
         assert hip.hipFree(memory) == 0
+
+
+# -- work memory ------------------------------------------------------------------------------------------------------------------
+
+def test_work_memory_does_not_grow_with_the_text(ctx):
+    """A text that gets longer is cut into more pieces; memory for all of them is there from the first cut on."""
+    hip = hip_runtime()
+
+    def used():
+        free, total = ctypes.c_size_t(), ctypes.c_size_t()
+        assert hip.hipMemGetInfo(ctypes.byref(free), ctypes.byref(total)) == 0
+        return total.value - free.value
+
+    c = Context(0)
+    try:
+        hd, H, G, n, S = 128, 32, 8, 32, 40000
+        ck, cv = (Tensor.zeros(c, G * S, hd, TensorDType.Float16) for _ in range(2))
+        q, out = (Tensor.zeros(c, n, H * hd, TensorDType.Float16) for _ in range(2))
+        held = []
+        for start in (4000, 8000, 16000, 24000, 39000):
+            q.attn_window(ck, cv, H, G, S, [start], out=out)
+            c.sync()
+            held.append(used())
+        assert len(set(held)) == 1, held
+    finally:
+        c.close()

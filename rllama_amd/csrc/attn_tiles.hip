@@ -124,10 +124,10 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
     auto v_swz = [](int row) { return HD == 128 ? (row & 3) * 4 : HD == 64 ? ((row >> 1) & 1) * 4 : 0; }; // in pieces
 
     // ---- staging
-    constexpr int kIssues = kTileBytes / (kWaves * 1024) > 0 ? kTileBytes / (kWaves * 1024) : 1; // f16: wavefront-wide 1 KiB loads per tile of K (and of V)
+    constexpr int kIssues = kTileBytes / (kWaves * 1024);    // f16: wavefront-wide 1 KiB loads per tile of K (and of V)
     constexpr int kIssueRows = kWaves * 64 / kPieces;        // rows from one to the next: a multiple of what the permutations repeat after
     constexpr int kGroups = 2 * kAtKeys * HD / 32, kItems = kGroups / (64 * kWaves) > 0 ? kGroups / (64 * kWaves) : 1; // 4 bits: groups per tile, and per thread
-    static_assert((kTileBytes >= kWaves * 1024 || kIssues == 1) && 2 * kIssues == kKS, "a tile's shares, one load beside each step of the first product");
+    static_assert(kTileBytes == kIssues * kWaves * 1024 && 2 * kIssues == kKS, "whole loads of every wavefront, one beside each step of the first product");
     const int my_row = (wave * 64 + lane) / kPieces, my_piece = lane % kPieces;
     const unsigned k_from = (my_piece ^ k_swz(my_row)) << 4, v_from = (my_piece ^ v_swz(my_row)) << 4; // within the row
     uint32_t codes[kQ4 ? kItems : 1][4], pairs[kQ4 ? kItems : 1];
@@ -147,7 +147,6 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
             }
         } else {
             const half_t *k = reinterpret_cast<const half_t *>(p.cache_k.data) + row * HD, *v = reinterpret_cast<const half_t *>(p.cache_v.data) + row * HD;
-            if (kTileBytes < kWaves * 1024 && wave >= kTileBytes / 1024) return;
 #pragma unroll
             for (int i = 0; i < kIssues; i++) {
                 const unsigned from = (unsigned)min(my_row + i * kIssueRows, here - 1) * kRowBytes; // keys past the last one are masked below
@@ -333,7 +332,7 @@ __global__ __launch_bounds__(64 * kAtGroups *kShares, 2) void attn_tiles_kernel(
                     __syncthreads();
                     work(stage, 0, 0, std::true_type{}, [&](int ks) __attribute__((always_inline)) {
                         if constexpr (kQ4) fetch_ahead(s + 2);
-                        else if (kTileBytes >= kWaves * 1024 || wave < kTileBytes / 1024) {
+                        else {
                             const half_t *from = reinterpret_cast<const half_t *>(ks < kIssues ? p.cache_k.data : p.cache_v.data) + row * HD;
                             const int i = ks % kIssues;
                             dma16_base(from, (unsigned)(my_row + i * kIssueRows) * kRowBytes + (ks < kIssues ? k_from : v_from),

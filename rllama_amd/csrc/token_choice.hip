@@ -15,7 +15,7 @@ typedef half_t half4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 __device__ __forceinline__ float4_t load4(const T *x, int i, int n, float fill) {
     float4_t v;
-    if (i + 4 <= n) {
+    if (i <= n - 4) { // (i + 4 may pass 32 bits)
         if constexpr (sizeof(T) == 2) {
             const half4_any h = *reinterpret_cast<const half4_any *>(x + i);
 #pragma unroll
@@ -32,7 +32,7 @@ __device__ __forceinline__ float4_t load4(const T *x, int i, int n, float fill) 
     return v;
 }
 __device__ __forceinline__ void store4(float *y, int i, int n, float4_t v) {
-    if (i + 4 <= n) {
+    if (i <= n - 4) { // (i + 4 may pass 32 bits)
         float4_any f;
 #pragma unroll
         for (int j = 0; j < 4; j++) f[j] = v[j];
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(kVdThreads) void verify_draft_kernel(VerifyParams p
     const float *prow = p.target + ((size_t)b * (k + 1) + count) * V;
     const float *qrow = sh_sub && p.draft ? p.draft + ((size_t)b * k + count) * V : nullptr;
     const int certain = sh_sub && !p.draft ? ids[count] : -1; // a draft without probabilities: all of it on the token itself
-    const int per_wave = ((V + kVdWaves - 1) / kVdWaves + 255) / 256; // in groups of 256
+    const int per_wave = (int)((((int64_t)V + kVdWaves - 1) / kVdWaves + 255) / 256); // in groups of 256
     const int chunk = (per_wave + kVdChunks - 1) / kVdChunks * 256, chunks = (per_wave * 256 + chunk - 1) / chunk;
     const int64_t lo = (int64_t)wave * chunks * chunk; // (may lie past the row)
     const float mf = fminf(fmaxf(u[k] * 16777216.0f, 0.0f), 16777215.0f); // (NaN: 0)

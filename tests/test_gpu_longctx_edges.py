@@ -178,3 +178,50 @@ def test_work_memory_does_not_grow_with_the_text(ctx):
         assert len(set(held)) == 1, held
     finally:
         c.close()
+
+
+# -- rows of nearly 2^31 entries --------------------------------------------------------------------------------------------------------------
+
+def test_the_longest_rows(ctx):
+    """2^31 - 1 entries: the places of the last ones plus four are more than 32 bits hold.  What lies behind a row must not count."""
+    hip, V = hip_runtime(), 2 ** 31 - 1
+    memory = [ctypes.c_void_p() for _ in range(2)]
+
+    def fill(m, value, count):
+        bits = int(np.array(value, f32).view(np.int32))
+        assert hip.hipMemsetD32(m, ctypes.c_int(bits), ctypes.c_size_t(count)) == 0 and hip.hipDeviceSynchronize() == 0
+
+    def put(m, at, a):
+        a = np.array(a, f32)
+        assert hip.hipMemcpy(ctypes.c_void_p(m.value + 4 * at), a.ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(a.nbytes), 1) == 0
+
+    def get(m, at, count):
+        a = np.empty(count, f32)
+        assert hip.hipMemcpy(a.ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(m.value + 4 * at), ctypes.c_size_t(a.nbytes), 2) == 0
+        return a
+
+    try:
+        for m, count in zip(memory, (2 * V + 2, V + 1)):
+            assert hip.hipMalloc(ctypes.byref(m), ctypes.c_size_t(4 * count)) == 0
+        x, p = (Tensor.from_device(ctx, m.value, 1, V, TensorDType.Float32) for m in memory)
+        fill(memory[0], -np.inf, V)
+        put(memory[0], V - 3, [0.0, 0.0, np.log(2.0), np.nan])  # the last three, and one behind them
+        put(memory[1], V - 4, [9.0] * 5)
+        for temperature, want in ((1.0, [0, 0.25, 0.25, 0.5, 9]), (0.0, [0, 0, 0, 1, 9])):
+            x.softmax_rows(temperature, out=p)
+            ctx.sync()
+            assert np.allclose(get(memory[1], V - 4, 5), want, rtol=1e-5)
+        x.free()
+        # a drafted last token that is accepted, and a second row of which only the last entry is possible
+        fill(memory[0], 0.0, 2 * V)
+        put(memory[0], V - 1, [1.0])
+        put(memory[0], 2 * V - 1, [0.5, 1.0])
+        target = Tensor.from_device(ctx, memory[0].value, 2, V, TensorDType.Float32)
+        drafted = Tensor.from_numpy(ctx, np.array([[V - 1]], np.int32))
+        for u in (0.0, 0.9):
+            out = drafted.verify_draft(target, None, Tensor.from_numpy(ctx, np.array([[0.5, u]], f32)))
+            assert out.to_numpy().tolist() == [[1, V - 1, V - 1]]
+    finally:
+        ctx.sync()
+        for m in memory:
+            hip.hipFree(m)

@@ -304,7 +304,7 @@ int  rlh_argmax_greedy(const rlh_tensor *logits, float temperature, int32_t *tok
  * context's stream; no call here waits for it or allocates device memory except where it says so.
  *
  * Rows and positions.  A call takes n rows of each of n_seqs sequences (1..256): row b * n + i of its tensors is sequence b's
- * row at position start_pos[b] + i.  A negative position is padding (rows on the left of a short prompt, an idle slot of a batch):
+ * row at position start_pos[b] + i, below 2^31 - 256.  A negative position is padding (rows on the left of a short prompt, an idle slot of a batch):
  * it is neither written nor looked at, and its rows of the results are zeros.
  * Cache planes are two tensors [n_seqs * n_kv_heads * max_seq_len x head_dim] of one dtype (f16, f32 or Q4), head_dim 32, 64 or
  * 128; row (b * n_kv_heads + g) * max_seq_len + r.  Query head h reads key and value head h / (n_heads / n_kv_heads).

@@ -88,7 +88,7 @@ static int plan_rows(const char *who, const rlh_tensor *ck, const rlh_tensor *cv
     plan->n = rows / n_seqs;
     for (int b = 0; b < n_seqs; b++) {
         const int64_t end = (int64_t)start_pos[b] + plan->n;
-        if (end > INT32_MAX) return fail(RLH_ERR_INVALID, "%s: sequence %d: position %lld", who, b, (long long)end);
+        if (end > kLongMaxPosition) return fail(RLH_ERR_INVALID, "%s: sequence %d: position %lld", who, b, (long long)end);
         if (end > max_seq_len) plan->wraps = true;
     }
     return RLH_OK;

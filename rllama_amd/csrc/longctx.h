@@ -6,6 +6,7 @@
 namespace rlh {
 
 constexpr int kLongMaxSeqs = 256; // positions travel as kernel arguments: 1 KiB of the 4 KiB a launch may carry
+constexpr int64_t kLongMaxPosition = INT32_MAX - 255; // the kernels add up to a tile of positions to one in 32 bits
 
 enum PlaneType { kPlaneF16 = 0, kPlaneF32 = 1, kPlaneQ4 = 2 };
 

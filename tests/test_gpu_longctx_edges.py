@@ -6,7 +6,7 @@ import pytest
 
 import rllama_amd
 from rllama_amd import Context, Tensor, TensorDType
-from test_gpu_longctx import EPS16, NUMPY, attention_reference, f16, f32, f64, upload, values
+from test_gpu_longctx import EPS16, INVALID, attention_reference, f16, f32, f64, refused, upload, values
 
 pytestmark = pytest.mark.gpu
 
@@ -225,3 +225,14 @@ def test_the_longest_rows(ctx):
         ctx.sync()
         for m in memory:
             hip.hipFree(m)
+
+
+# -- sizes that are refused ---------------------------------------------------------------------------------------------------------------------
+
+def test_positions_next_to_32_bits_are_refused(ctx):
+    z = lambda r, c, k=TensorDType.Float16: Tensor.zeros(ctx, r, c, k)  # noqa: E731
+    ck, cv, q, qkv, freqs = z(64, 64), z(64, 64), z(2, 64), z(2, 192), z(64, 64, TensorDType.Float32)
+    for at in (2 ** 31 - 257, 2 ** 31 - 200, 2 ** 31 - 2):
+        refused(INVALID, q.attn_window, ck, cv, 1, 1, 64, [at], window=16)
+        refused(INVALID, qkv.qkv_append, q, ck, cv, freqs, 1, 1, 64, [at])
+    q.attn_window(ck, cv, 1, 1, 64, [2 ** 31 - 258], window=16)

@@ -341,6 +341,7 @@ int  rlh_qkv_append(rlh_tensor *q, const rlh_tensor *qkv, const rlh_tensor *q_no
  * the eleventh bit, up to 2^-11 of the value) where many rows share a key and value head; up to 16 rows always read them exactly.  Values
  * of 4 bits beyond what f16 holds are read exactly in both; with many rows such a call takes some 300 times as long.  Rows and keys outside what
  * is seen may hold anything, NaN included.  Positions beyond max_seq_len need window > 0 and sinks + window + n - 1 <= max_seq_len.
+ * A call takes at least 1048560 rows n * n_heads / n_kv_heads of a sequence, and 65535 sequences * n_kv_heads; more are RLH_ERR_UNSUPPORTED.
  * Partial results of sequences that are cut go to work memory that stays with the context, 34 MB at most.  A call that needs more than every
  * one before it waits for the context's queued work and allocates it: of a text that gets longer one call or two, when it is first cut. */
 int  rlh_attn_window(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *cache_k, const rlh_tensor *cache_v, int n_heads, int n_kv_heads,

@@ -192,6 +192,8 @@ extern "C" int rlh_attn_window(rlh_tensor *out, const rlh_tensor *q, const rlh_t
     p.sinks = sinks;
     for (int b = 0; b < n_seqs; b++) p.start[b] = start_pos[b];
     const int cus = ctx->prop.multiProcessorCount;
+    const int64_t rows = (int64_t)p.n * (n_heads / n_kv_heads), most = attn_window_most_rows(p, cus);
+    if (rows > most) return fail(RLH_ERR_UNSUPPORTED, "rlh_attn_window: %lld rows on one key and value head, %lld at once (65535 sequences and key heads)", (long long)rows, (long long)most);
     HIP_TRY(window_work_reserve(ctx, attn_window_work_floats(p, cus)));
     HIP_TRY(launch_attn_window(p, cus, ctx->ops.window_ws, ctx->stream));
     return RLH_OK;

@@ -560,6 +560,8 @@ static TilesCut cut_tiles(const AttnWindowParams &p, int compute_units) {
     return cut;
 }
 
+int attn_tiles_rows() { return kAtRows; }
+
 double attn_tiles_us(const AttnWindowParams &p, int compute_units) { return cut_tiles(p, compute_units).us; }
 
 size_t attn_tiles_work_floats(const AttnWindowParams &p, int compute_units) {
@@ -581,7 +583,6 @@ static void launch_tiles(const AttnCutParams &p, int shares, hipStream_t s) {
 }
 
 hipError_t launch_attn_tiles(const AttnWindowParams &a, int compute_units, float *ws, hipStream_t s) {
-    if ((int64_t)a.n * (a.n_heads / a.n_kv) > (int64_t)65535 * kAtRows || (int64_t)a.n_seqs * a.n_kv > 65535) return hipErrorInvalidValue;
     const TilesCut cut = cut_tiles(a, compute_units);
     AttnCutParams p;
     p.a = a;

@@ -559,8 +559,8 @@ struct RowsCut {
     double us;
 };
 static RowsCut cut_rows(const AttnWindowParams &p, int compute_units) {
-    const int group = p.n_heads / p.n_kv, rows = p.n * group, step = f16_arithmetic(p) ? 32 : 16;
-    const int64_t tiles = (rows + kAwRows - 1) / kAwRows, units = tiles * p.n_seqs * p.n_kv;
+    const int group = p.n_heads / p.n_kv, step = f16_arithmetic(p) ? 32 : 16;
+    const int64_t rows = (int64_t)p.n * group, tiles = (rows + kAwRows - 1) / kAwRows, units = tiles * p.n_seqs * p.n_kv;
     // no tile has more steps than this: its rows' positions are at most `apart` from each other
     const int64_t apart = std::min<int64_t>(p.n - 1, (kAwRows - 2) / group + 1);
     int64_t steps = 1;
@@ -599,6 +599,11 @@ static bool tiles_take(const AttnWindowParams &p, int compute_units) {
     return f16_arithmetic(p) && p.n * (int64_t)(p.n_heads / p.n_kv) > kAwRows && attn_tiles_us(p, compute_units) < cut_rows(p, compute_units).us;
 }
 
+int64_t attn_window_most_rows(const AttnWindowParams &p, int compute_units) {
+    if ((int64_t)p.n_seqs * p.n_kv > 65535) return 0;
+    return 65535 * (int64_t)(tiles_take(p, compute_units) ? attn_tiles_rows() : kAwRows);
+}
+
 size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units) {
     if (tiles_take(p, compute_units)) return attn_tiles_work_floats(p, compute_units);
     const RowsCut cut = cut_rows(p, compute_units);
@@ -613,7 +618,6 @@ hipError_t launch_attn_window(const AttnWindowParams &a, int compute_units, floa
     const RowsCut cut = cut_rows(a, compute_units);
     p.pieces = cut.pieces;
     p.piece_steps = cut.piece_steps;
-    if ((int64_t)a.n_seqs * a.n_kv > 65535 || (int64_t)a.n * (a.n_heads / a.n_kv) > 65535 * kAwRows) return hipErrorInvalidValue;
     switch (a.cache * 2 + a.f16) {
     case kPlaneF16 * 2: return launch_rows_hd<float, float, half_t>(p, s);
     case kPlaneF16 * 2 + 1: return launch_rows_hd<half_t, half_t, half_t>(p, s);

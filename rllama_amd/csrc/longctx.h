@@ -36,9 +36,12 @@ struct AttnWindowParams {
     int window, sinks;     // window 0: everything up to the row's own position
     int32_t start[kLongMaxSeqs];
 };
+// rows of one key and value head (n * n_heads / n_kv) that a launch takes; 0: too many sequences and heads
+int64_t attn_window_most_rows(const AttnWindowParams &p, int compute_units);
 // work memory for partial results where this call cuts its texts: enough for as many pieces as texts of any length are cut into, at most 512 workgroups' rows (34 MB)
 size_t attn_window_work_floats(const AttnWindowParams &p, int compute_units);
 // the form for many rows (attn_tiles.hip): which calls it takes, its work memory and its launch
+int attn_tiles_rows(); // of a workgroup
 double attn_tiles_us(const AttnWindowParams &p, int compute_units); // about what a call takes
 size_t attn_tiles_work_floats(const AttnWindowParams &p, int compute_units);
 hipError_t launch_attn_tiles(const AttnWindowParams &p, int compute_units, float *ws, hipStream_t s);

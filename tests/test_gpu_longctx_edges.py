@@ -6,7 +6,7 @@ import pytest
 
 import rllama_amd
 from rllama_amd import Context, Tensor, TensorDType
-from test_gpu_longctx import EPS16, INVALID, attention_reference, f16, f32, f64, refused, upload, values
+from test_gpu_longctx import EPS16, INVALID, UNSUPPORTED, attention_reference, f16, f32, f64, refused, upload, values
 
 pytestmark = pytest.mark.gpu
 
@@ -236,3 +236,19 @@ def test_positions_next_to_32_bits_are_refused(ctx):
         refused(INVALID, q.attn_window, ck, cv, 1, 1, 64, [at], window=16)
         refused(INVALID, qkv.qkv_append, q, ck, cv, freqs, 1, 1, 64, [at])
     q.attn_window(ck, cv, 1, 1, 64, [2 ** 31 - 258], window=16)
+
+
+def test_more_rows_than_a_launch_takes_are_refused(ctx):
+    n, hd = 131070, 32
+    ck, cv = (Tensor.zeros(ctx, 64, hd, TensorDType.Float32) for _ in range(2))
+    for rows in (n, n + 1):
+        q, out = (Tensor.zeros(ctx, rows, 8 * hd, TensorDType.Float32) for _ in range(2))
+        if rows == n:
+            q.attn_window(ck, cv, 8, 1, 64, [64 - n], out=out)
+            assert (out.to_numpy() == 0).all()
+        else:
+            refused(UNSUPPORTED, q.attn_window, ck, cv, 8, 1, 64, [64 - rows], out=out)
+    B, G = 256, 256
+    plane = Tensor.zeros(ctx, B * G, hd, TensorDType.Float32)
+    q, out = (Tensor.zeros(ctx, B, G * hd, TensorDType.Float32) for _ in range(2))
+    refused(UNSUPPORTED, q.attn_window, plane, plane, G, G, 1, [0] * B, out=out)

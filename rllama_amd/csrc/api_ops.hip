@@ -8,6 +8,8 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <memory>
+#include <new>
 #include <vector>
 
 using namespace rlh;
@@ -375,16 +377,17 @@ extern "C" int rlh_ffn_gate(rlh_tensor *dst, const rlh_tensor *x, const rlh_tens
     return RLH_OK;
 }
 
-// (cos, sin) of compute_freqs_cis (transformer.rs:858-885) for positions first .. first + n - 1, as f32 like :836-837
-static std::vector<float2> rope_table(int head_dim, int first, int n, double theta = 10000.0) {
+// (cos, sin) of compute_freqs_cis (transformer.rs:858-885), as f32 like :836-837: pair j of a position
+static float2 rope_angle(int head_dim, int position, int j, double theta) {
+    const double freq = 1.0 / std::pow(theta, (double)j * 2.0 / (double)head_dim);
+    const double ang = freq * (double)position;
+    return make_float2((float)std::cos(ang), (float)std::sin(ang));
+}
+// ... of positions first .. first + n - 1
+static std::vector<float2> rope_table(int head_dim, int first, int n) {
     std::vector<float2> tab((size_t)n * (head_dim / 2));
-    for (int i = 0; i < n; i++) {
-        for (int j = 0; j < head_dim / 2; j++) {
-            const double freq = 1.0 / std::pow(theta, (double)j * 2.0 / (double)head_dim);
-            const double ang = freq * (double)(first + i);
-            tab[(size_t)i * (head_dim / 2) + j] = make_float2((float)std::cos(ang), (float)std::sin(ang));
-        }
-    }
+    for (int i = 0; i < n; i++)
+        for (int j = 0; j < head_dim / 2; j++) tab[(size_t)i * (head_dim / 2) + j] = rope_angle(head_dim, first + i, j, 10000.0);
     return tab;
 }
 
@@ -392,12 +395,15 @@ extern "C" int rlh_rope_table(rlh_tensor *freqs, double theta) {
     if (!freqs || freqs->dtype != RLH_F32 || freqs->cols % 2 != 0) return fail(RLH_ERR_INVALID, "rlh_rope_table: an f32 tensor [positions x head_dim], head_dim even, is needed");
     if (!(theta > 0.0) || std::isinf(theta)) return fail(RLH_ERR_INVALID, "rlh_rope_table: theta must be positive");
     CtxLock lock(freqs->ctx);
-    constexpr int kChunk = 4096; // positions formed and sent at a time
-    for (int first = 0; first < freqs->rows; first += kChunk) {
-        const int n = std::min(kChunk, freqs->rows - first);
-        const std::vector<float2> tab = rope_table(freqs->cols, first, n, theta);
-        HIP_TRY(hipMemcpyAsync((float *)freqs->p + (size_t)first * freqs->cols, tab.data(), tab.size() * sizeof(float2), hipMemcpyHostToDevice, freqs->ctx->stream));
-        HIP_TRY(hipStreamSynchronize(freqs->ctx->stream)); // the host table goes out of scope
+    constexpr size_t kChunk = (size_t)1 << 18; // pairs formed and sent at a time: 2 MiB, whatever the table's shape
+    const size_t pairs = freqs->count() / 2, per_row = (size_t)freqs->cols / 2;
+    const std::unique_ptr<float2[]> tab(new (std::nothrow) float2[std::min(kChunk, pairs)]);
+    if (!tab) return fail(RLH_ERR_OOM, "rlh_rope_table: out of host memory");
+    for (size_t first = 0; first < pairs; first += kChunk) {
+        const size_t n = std::min(kChunk, pairs - first);
+        for (size_t i = 0; i < n; i++) tab[i] = rope_angle(freqs->cols, (int)((first + i) / per_row), (int)((first + i) % per_row), theta);
+        HIP_TRY(hipMemcpyAsync((float2 *)freqs->p + first, tab.get(), n * sizeof(float2), hipMemcpyHostToDevice, freqs->ctx->stream));
+        HIP_TRY(hipStreamSynchronize(freqs->ctx->stream)); // the next ones go into the same memory
     }
     return RLH_OK;
 }

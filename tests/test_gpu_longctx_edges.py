@@ -1,5 +1,8 @@
 """The long-context operators at the edges of what their numbers and sizes allow, against their definitions in 64 bits."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -252,3 +255,31 @@ def test_more_rows_than_a_launch_takes_are_refused(ctx):
     plane = Tensor.zeros(ctx, B * G, hd, TensorDType.Float32)
     q, out = (Tensor.zeros(ctx, B, G * hd, TensorDType.Float32) for _ in range(2))
     refused(UNSUPPORTED, q.attn_window, plane, plane, G, G, 1, [0] * B, out=out)
+
+
+# -- host memory ---------------------------------------------------------------------------------------------------------------------------------
+
+WIDE_TABLE = """
+import resource
+import numpy as np
+from rllama_amd import Context, Tensor, TensorDType
+peak = lambda: resource.getrusage(resource.RUSAGE_SELF).ru_maxrss >> 10
+ctx = Context(0)
+Tensor.zeros(ctx, 3, 128, TensorDType.Float32).rope_table()
+t = Tensor.zeros(ctx, 4096, 16384, TensorDType.Float32)
+before = peak()
+t.rope_table(500.0)
+print("MiB more:", peak() - before)
+assert peak() - before < 32
+last = t.to_numpy()[-1]
+angle = 4095 * 500.0 ** (-np.arange(0, 16384, 2) / 16384)
+assert np.abs(last.reshape(-1, 2) - np.stack([np.cos(angle), np.sin(angle)], -1)).max() < 1e-7
+print("the same")
+"""
+
+
+def test_a_table_of_angles_takes_little_host_memory(ctx):
+    """256 MiB of them: formed and sent piece by piece (in a process of its own, for its peak)."""
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    r = subprocess.run([sys.executable, "-c", WIDE_TABLE], env=env, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "the same" in r.stdout, r.stdout + r.stderr

@@ -330,6 +330,16 @@ class Tensor:
         return Tensor(ctx, h, a.shape[0], a.shape[1], dt)
 
     @staticmethod
+    def from_q4(ctx: Context, buffer: np.ndarray, rows: int, cols: int) -> "Tensor":
+        """A 4-bit tensor from its buffer, as to_numpy() gives it: rows * cols / 32 * 20 bytes, the codes and then the pairs."""
+        a = np.ascontiguousarray(buffer)
+        if a.dtype != np.uint8 or a.size * 32 != rows * cols * 20:
+            raise ValueError(f"{rows} x {cols} values of 4 bits are {rows * cols // 32 * 20} bytes (uint8), not {a.size} of {a.dtype}")
+        h = C.c_void_p()
+        check(ctx._lib.rlh_tensor_upload(ctx._h, a.ctypes.data_as(C.c_void_p), rows, cols, cols, TensorDType.K4BitQuantization, C.byref(h)))
+        return Tensor(ctx, h, rows, cols, TensorDType.K4BitQuantization)
+
+    @staticmethod
     def zeros(ctx: Context, rows: int, cols: int, dtype: int) -> "Tensor":
         h = C.c_void_p()
         check(ctx._lib.rlh_tensor_alloc(ctx._h, rows, cols, dtype, C.byref(h)))
@@ -354,7 +364,7 @@ class Tensor:
 
     def to_numpy(self) -> np.ndarray:
         """to_cpu_inplace (src/tensor.rs:2150-2166): f16 tensors come back as float16 arrays, whole numbers as int32; of a 4-bit tensor the
-        buffer as bytes (convert() gives the values)."""
+        buffer as bytes (convert() gives the values, from_q4() the tensor again)."""
         if self._dtype in (TensorDType.K4BitQuantization, TensorDType.Int32):
             shape, kind = ((self._rows, self._cols), np.int32) if self._dtype == TensorDType.Int32 else (self._rows * self._cols // 32 * 20, np.uint8)
             out = np.empty(shape, dtype=kind)

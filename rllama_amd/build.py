@@ -71,19 +71,29 @@ def build(force: bool = False) -> str:
 
 
 HOST_BIN = os.path.join(HERE, "host", "rllama_generate")
+TENSORS_BIN = os.path.join(HERE, "host", "rllama_check_tensors")
+
+
+def _build_host(main: str, binary: str, force: bool) -> str:
+    src = os.path.join(HERE, "host", main)
+    hdrs = [os.path.join(HERE, "host", h) for h in ("rllama_hip.hpp", "model_files.hpp", "tokenizer.hpp", "file_tools.hpp")]
+    if not force and os.path.exists(binary) and all(os.path.getmtime(binary) >= os.path.getmtime(f) for f in (src, *hdrs, LIB)):
+        return binary
+    cmd = ["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", src, "-o", binary, "-L" + HERE, "-lrllama_hip", "-Wl,-rpath,$ORIGIN/..", "-ldl"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("host build failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+    return binary
 
 
 def build_host(force: bool = False) -> str:
     """Compiles the C++ host example (header-only mirror of the reference API + the token loop) against the library."""
-    src = os.path.join(HERE, "host", "generate_main.cpp")
-    hdrs = [os.path.join(HERE, "host", h) for h in ("rllama_hip.hpp", "model_files.hpp", "tokenizer.hpp", "file_tools.hpp")]
-    if not force and os.path.exists(HOST_BIN) and all(os.path.getmtime(HOST_BIN) >= os.path.getmtime(f) for f in (src, *hdrs, LIB)):
-        return HOST_BIN
-    cmd = ["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", src, "-o", HOST_BIN, "-L" + HERE, "-lrllama_hip", "-Wl,-rpath,$ORIGIN/.."]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("host build failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
-    return HOST_BIN
+    return _build_host("generate_main.cpp", HOST_BIN, force)
+
+
+def build_host_tensors(force: bool = False) -> str:
+    """The C++ mirror's tensor methods for long contexts and drafted tokens, as a program that runs one step of them."""
+    return _build_host("check_tensors_main.cpp", TENSORS_BIN, force)
 
 
 ASAN_BIN = os.path.join(HERE, "host", "rllama_check_files_asan")
@@ -110,3 +120,4 @@ if __name__ == "__main__":
     else:
         print(build(force="--force" in sys.argv))
         print(build_host(force="--force" in sys.argv))
+        print(build_host_tensors(force="--force" in sys.argv))

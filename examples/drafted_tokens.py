@@ -1,15 +1,18 @@
 """Several chats with long texts, a small model drafting and a large one verifying.
 
-    python examples/drafted_tokens.py [--chats 4] [--tokens 48] [--draft 4] [--window 96] [--cache q4|f16|f32] [--temperature 0.8]
+    python examples/drafted_tokens.py [--chats 4] [--tokens 48] [--draft 4] [--window 96] [--cache q4|f16|f32] [--arithmetic f32|f16]
+                                      [--temperature 0.8]
 
 Both models are LLaMA-shaped stacks with grouped heads, normalised queries and keys and random weights, written out op by op:
 
     rows -> rmsnorm -> wq|wk|wv -> qkv_append (norms, rotation, cache rows) -> attn_window -> wo, add -> rmsnorm -> silu(w1) * w3 -> w2, add
 
-The caches are rings: the first `sinks` positions stay, of the others the last `window` are seen, so a chat may run on for ever.  A round takes
+The caches are rings: the first `sinks` positions stay, of the others the last `window` are seen, so memory does not grow with a chat; it may run on as far
+as the table of angles goes (a row of head_dim numbers for every position).  A round takes
 `draft` tokens from the small model one by one, runs the large one over all of them at once (one pass over its weights) and keeps what
 verify_draft accepts plus the token it draws itself: the tokens are distributed as if the large model had drawn each of them, whatever the
-small one proposes.  Positions that were appended for refused tokens are simply written again by the next round.
+small one proposes.  Positions that were appended for refused tokens are simply written again by the next round; the rows they took in the ring are
+counted in its size (sinks + window + rows at once - 1), so that no position still seen is lost to them.
 """
 import argparse
 import os
@@ -25,13 +28,16 @@ CACHES = {"f16": TensorDType.Float16, "f32": TensorDType.Float32, "q4": TensorDT
 
 
 class Stack:
-    """A transformer of random weights in f32, with caches for `chats` texts."""
+    """A transformer of random weights, with caches for `chats` texts.  f32: everything in f32.  f16: weights and what goes between the products in f16, norms and
+    the residual stream in f32."""
 
-    def __init__(self, ctx, seed, layers, dim, n_heads, n_kv_heads, head_dim, ffn, vocab, positions, chats, window, sinks, rows_at_once, cache):
+    def __init__(self, ctx, seed, layers, dim, n_heads, n_kv_heads, head_dim, ffn, vocab, positions, chats, window, sinks, rows_at_once, cache, f16=False):
         rng = np.random.default_rng(seed)
+        self.dtype = TensorDType.Float16 if f16 else TensorDType.Float32
 
         def weights(rows, cols):
-            return Tensor.from_numpy(ctx, rng.standard_normal((rows, cols), np.float32) / np.float32(np.sqrt(cols)))
+            w = rng.standard_normal((rows, cols), np.float32) / np.float32(np.sqrt(cols))
+            return Tensor.from_numpy(ctx, w.astype(np.float16) if f16 else w)
 
         def ones(cols):
             return Tensor.from_numpy(ctx, np.ones((1, cols), np.float32))
@@ -47,18 +53,20 @@ class Stack:
         self.norm, self.output = ones(dim), weights(vocab, dim)
 
     def forward(self, tokens, start_pos):
-        """Logits f32 [chats * n x vocab] of tokens [chats x n], chat b's at positions start_pos[b] on (negative: padding)."""
-        rows = tokens.size
+        """Logits [chats * n x vocab] of tokens [chats x n], chat b's at positions start_pos[b] on (negative: padding)."""
+        rows, f16 = tokens.size, self.dtype == TensorDType.Float16
+        norm = lambda x, w: x.rmsnorm(w, 1e-6).convert(self.dtype) if f16 else x.rmsnorm(w, 1e-6)  # noqa: E731
+        add = lambda x, y: x.add(y.convert(TensorDType.Float32) if f16 else y)  # noqa: E731
         x = Tensor.from_numpy(self.ctx, self.embedding[np.maximum(tokens, 0).reshape(-1)])
         for w in self.layers:
-            qkv = x.rmsnorm(w["attention_norm"], 1e-6).matrix_mul_transposed(w["wqkv"])
-            q = Tensor.zeros(self.ctx, rows, self.n_heads * self.hd, TensorDType.Float32)
+            qkv = norm(x, w["attention_norm"]).matrix_mul_transposed(w["wqkv"])
+            q = Tensor.zeros(self.ctx, rows, self.n_heads * self.hd, self.dtype)
             qkv.qkv_append(q, w["k"], w["v"], self.freqs, self.n_heads, self.n_kv, self.ring, start_pos, q_norm=w["q_norm"], k_norm=w["k_norm"], sinks=self.sinks)
             seen = q.attn_window(w["k"], w["v"], self.n_heads, self.n_kv, self.ring, start_pos, window=self.window, sinks=self.sinks)
-            x = x.add(seen.matrix_mul_transposed(w["wo"]))
-            h = x.rmsnorm(w["ffn_norm"], 1e-6)
-            x = x.add(h.matrix_mul_transposed(w["w1"]).silu_mul(h.matrix_mul_transposed(w["w3"])).matrix_mul_transposed(w["w2"]))
-        return x.rmsnorm(self.norm, 1e-6).matrix_mul_transposed(self.output)
+            x = add(x, seen.matrix_mul_transposed(w["wo"]))
+            h = norm(x, w["ffn_norm"])
+            x = add(x, h.matrix_mul_transposed(w["w1"]).silu_mul(h.matrix_mul_transposed(w["w3"])).matrix_mul_transposed(w["w2"]))
+        return norm(x, self.norm).matrix_mul_transposed(self.output)
 
     def read(self, texts, rows_at_once):
         """The texts but for their last tokens into the caches, `rows_at_once` rows of each at a time, shorter texts padded on the left."""
@@ -102,10 +110,10 @@ def generate(ctx, large, small, texts, n_tokens, k, temperature, seed, rows_at_o
     return texts, rounds, accepted
 
 
-def models(ctx, chats, k, window, sinks, positions, rows_at_once, cache, vocab=512):
+def models(ctx, chats, k, window, sinks, positions, rows_at_once, cache, vocab=512, arithmetic="f32"):
     """A large model, and one that is its first layer with the same embedding and output: a draft that agrees now and then."""
     common = dict(dim=256, n_heads=8, n_kv_heads=2, head_dim=32, ffn=512, vocab=vocab, positions=positions, chats=chats, window=window, sinks=sinks,
-                  rows_at_once=max(k + 1, rows_at_once), cache=CACHES[cache])
+                  rows_at_once=max(k + 1, rows_at_once), cache=CACHES[cache], f16=arithmetic == "f16")
     large, small = Stack(ctx, 1, layers=3, **common), Stack(ctx, 1, layers=1, **common)
     small.output = large.output
     return large, small
@@ -118,13 +126,14 @@ def main():
     p.add_argument("--draft", type=int, default=4)
     p.add_argument("--window", type=int, default=96)
     p.add_argument("--cache", choices=sorted(CACHES), default="q4")
+    p.add_argument("--arithmetic", choices=["f32", "f16"], default="f32")
     p.add_argument("--temperature", type=float, default=0.8)
     a = p.parse_args()
     ctx, rows_at_once, sinks = Context(0), 32, 4
     rng = np.random.default_rng(0)
     texts = [rng.integers(0, 512, 20 + 37 * c).tolist() for c in range(a.chats)]
     positions = max(map(len, texts)) + a.tokens * (a.draft + 1) + a.draft + 1  # (a chat runs on until the slowest has its tokens)
-    large, small = models(ctx, a.chats, a.draft, a.window, sinks, positions, rows_at_once, a.cache)
+    large, small = models(ctx, a.chats, a.draft, a.window, sinks, positions, rows_at_once, a.cache, arithmetic=a.arithmetic)
     began = time.time()
     texts_out, rounds, accepted = generate(ctx, large, small, texts, a.tokens, a.draft, a.temperature, 1, rows_at_once)
     new = sum(len(t) for t in texts_out) - sum(len(t) for t in texts)

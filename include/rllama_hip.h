@@ -309,7 +309,8 @@ int  rlh_argmax_greedy(const rlh_tensor *logits, float temperature, int32_t *tok
  * Cache planes are two tensors [n_seqs * n_kv_heads * max_seq_len x head_dim] of one dtype (f16, f32 or Q4), head_dim 32, 64 or
  * 128; row (b * n_kv_heads + g) * max_seq_len + r.  Query head h reads key and value head h / (n_heads / n_kv_heads).
  * Position t is kept in row t while t < max_seq_len.  Later positions, which need a window, replace the oldest ones behind the
- * first `sinks`: row sinks + (t - sinks) % (max_seq_len - sinks).  Both calls below take the same `sinks`.
+ * first `sinks`: row sinks + (t - sinks) % (max_seq_len - sinks).  Both calls below take the same `sinks`.  Positions that are appended and then taken back
+ * (refused drafts) have replaced old ones all the same: max_seq_len - sinks has to hold the window and the most rows ever appended at once, less one.
  * ---------------------------------------------------------------------------------------------- */
 /* A tensor over device memory that the caller owns (another library's, on this device; 16-byte aligned): nothing is copied, and
  * rlh_tensor_free frees only the handle, when the queued work that uses it is done, other contexts' too.  The memory has to outlive the handle.  Work that the
@@ -320,8 +321,8 @@ int  rlh_wait_stream(rlh_ctx *ctx, void *stream);
 /* ... and later work on `stream` for what is queued on the context by now.  Neither makes the host wait. */
 int  rlh_release_stream(rlh_ctx *ctx, void *stream);
 /* dst = src between f16, f32 and Q4 tensors of one shape.  To Q4, per group of 32 columns: lowest = f16(min), scale =
- * f16((max - lowest) / 15), code = round((x - lowest) / scale), ties to even, within 0..15 (scale 0: code 0).  A group with a value
- * that is not finite, or whose lowest or scale f16 cannot hold, reads as NaN throughout. */
+ * f16((max - lowest) / 15), code = round((x - lowest) / scale), ties to even, within 0..15 (code 0 where the scale is not above 0, as in a
+ * group of one value).  A group with a value that is not finite, or whose lowest or scale f16 cannot hold, reads as NaN throughout. */
 int  rlh_convert(rlh_tensor *dst, const rlh_tensor *src);
 /* The angles of positions 0 .. rows - 1, freqs f32 [rows x head_dim]: pairs (cos, sin) of position * theta^(-2j / head_dim), formed in
  * 64 bits on the host and rounded (compute_freqs_cis, src/transformer.rs:858-885, with theta 10000).  Waits for the upload. */
@@ -330,7 +331,8 @@ int  rlh_rope_table(rlh_tensor *freqs, double theta);
  * queries, then keys, then values.  Queries and keys are normalised per head (x / sqrt(mean x^2 + eps) * weight; q_norm and k_norm
  * f32 [1 x head_dim], NULL = left out) and rotated by their position's row of freqs (f32, a row for every position; halves = 0: columns
  * 2j and 2j + 1 are a pair, as in the reference; 1: columns j and j + head_dim / 2); queries go to q [n_seqs * n x n_heads head_dim]
- * (dtype of qkv), keys and values into the planes.  Arithmetic in f32, one rounding to each result's type. */
+ * (dtype of qkv), keys and values into the planes.  Arithmetic in f32, one rounding to each result's type.  A call that reaches past
+ * max_seq_len takes max_seq_len - sinks rows of a sequence at most. */
 int  rlh_qkv_append(rlh_tensor *q, const rlh_tensor *qkv, const rlh_tensor *q_norm, const rlh_tensor *k_norm, double eps, const rlh_tensor *freqs,
                     int halves, rlh_tensor *cache_k, rlh_tensor *cache_v, int n_heads, int n_kv_heads, int max_seq_len, int sinks,
                     const int32_t *start_pos, int n_seqs);

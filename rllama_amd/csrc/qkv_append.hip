@@ -10,7 +10,7 @@
 //
 // Measured: 1500 rows of 32 heads on 8 of 128 into 4 bits, 33 MB: 11.8 us, 2.8 TB/s (a copy of as many bytes: 7.9).  All workgroups are on the part at once, so
 // their loads, their arithmetic and their stores come one after the other.  One row of 32 heads: 2.7 us, a launch.
-// Call after call: 11.0 us; into f16 9.4 (4.0 TB/s), 32 key and value heads into f16 14.6 (5.1 TB/s).  One or two heads per thread instead of three: 12.4, 11.7.
+// Call after call: 11.0 us; into f16 9.4 (4.0 TB/s), 32 key and value heads into f16 14.6 (5.1 TB/s).
 #include "kernels.h"
 #include "longctx.h"
 
@@ -123,8 +123,13 @@ __global__ __launch_bounds__(kAppendThreads) void qkv_append_kernel(QkvAppendPar
 template <typename IN, typename CT, int HD>
 static void launch_append(const QkvAppendParams &p, hipStream_t s) {
     const int units = kAppendThreads * 8 / HD, slots = p.n_heads + 2 * p.n_kv, rows = p.n * p.n_seqs;
-    // Few rows: a head per thread group, so that nothing waits.  Many rows: several, so that angles and weights are read once for them.
-    const int take = rows < 512 ? 1 : 3;
+    // Few workgroups: a head per thread group, so that nothing waits.  More than four per compute unit: three heads, so that angles and weights are read once for them.
+    // (1 / 2 / 3 / 4 heads, us a call, 4.2 of it the call; 32 heads on 8 of 128 into f16: 384 rows, 1152 workgroups of one head each, 4.6 / 4.3 / 4.7 / 4.6; 512, 5.2 /
+    // 4.7 / 4.7 / 4.7; 1500, 10.9 / 9.8 / 8.4 / 8.4.  32 heads on 32: 256 rows, 1536 workgroups, 5.1 / 4.9 / 5.2 / 5.1; 384, 6.8 / 5.7 / 5.5 / 6.0; 1500, 18.1 / 14.5 / 13.3 /
+    // 14.3.  16 of 64 on 16: 768, 1536 workgroups, 4.8 / 4.4 / 4.9 / 4.8; 1500, 7.9 / 6.0 / 6.1 / 6.3.  One workgroup holds all heads of a row, 8 of 32 on 2: 2500 rows 5.1 / 5.4
+    // / 5.6 / 5.8.)
+    const int groups = (slots + units - 1) / units;
+    const int take = groups > 1 && (int64_t)rows * groups > 1024 ? 3 : 1;
     const dim3 grid((unsigned)rows, (unsigned)((slots + units * take - 1) / (units * take)));
     if (take == 1) hipLaunchKernelGGL((qkv_append_kernel<IN, CT, HD, 1>), grid, dim3(kAppendThreads), 0, s, p);
     else hipLaunchKernelGGL((qkv_append_kernel<IN, CT, HD, 3>), grid, dim3(kAppendThreads), 0, s, p);

@@ -9,7 +9,7 @@ import pytest
 
 import rllama_amd
 from rllama_amd import Context, Tensor, TensorDType
-from test_gpu_longctx import EPS16, INVALID, UNSUPPORTED, attention_reference, f16, f32, f64, refused, upload, values
+from test_gpu_longctx import EPS16, INVALID, UNSUPPORTED, attention_reference, f16, f32, f64, refused, test_append as append_test, upload, values
 
 pytestmark = pytest.mark.gpu
 
@@ -283,3 +283,16 @@ def test_a_table_of_angles_takes_little_host_memory(ctx):
     env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     r = subprocess.run([sys.executable, "-c", WIDE_TABLE], env=env, capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and "the same" in r.stdout, r.stdout + r.stderr
+
+
+# -- appends of many rows: several heads per thread ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("hd,H,G,n,S,sinks,starts", [
+    (128, 34, 2, 400, 500, 0, [7]),              # 38 heads of 16 per workgroup and pass: the last pass is not full
+    (64, 16, 16, 180, 220, 0, [0, 11, -30, 40]),
+    (32, 40, 20, 300, 320, 4, [900, -5]),        # rings
+])
+@pytest.mark.parametrize("kind,cache", [("f16", "f16"), ("f16", "q4"), ("f32", "f32")])
+@pytest.mark.parametrize("halves,norms", [(False, True), (True, True), (True, False)])
+def test_append_of_many_rows(ctx, hd, H, G, n, S, sinks, starts, kind, cache, halves, norms):
+    append_test(ctx, hd, H, G, n, S, sinks, starts, kind, cache, halves, norms)

@@ -339,9 +339,9 @@ int  rlh_qkv_append(rlh_tensor *q, const rlh_tensor *qkv, const rlh_tensor *q_no
 /* Attention of the rows over the planes, which hold the rows' own positions already: the row at position p sees the positions
  * t <= p with t < sinks or t > p - window (window 0: all of them), out = softmax(q K^T / sqrt(head_dim)) V.  q and out
  * [n_seqs * n x n_heads head_dim], both f16 or both f32.  f32 rows, or an f32 cache: f32 arithmetic throughout.  Otherwise f16 operands with
- * f32 sums: the softmax's weights are rounded to f16 in front of the second product, and values of 4 bits are rounded to f16 (half a unit in
- * the eleventh bit, up to 2^-11 of the value) where many rows share a key and value head; up to 16 rows always read them exactly (with more, the form that is
- * estimated to be the faster one is taken, so whether they are rounded depends on the call's sizes).  Values of 4 bits beyond what f16 holds are read exactly in both; with many rows such a call takes some 300 times as long.  Rows and keys outside what
+ * f32 sums.  Up to 16 rows of a key and value head (n * n_heads / n_kv_heads) round nothing but the result.  With more, the form that is estimated to
+ * be the faster one is taken: that one, or one that rounds the softmax's weights and values of 4 bits to f16 in front of its products (half a
+ * unit in the eleventh bit, up to 2^-11 of each).  Values of 4 bits beyond what f16 holds are read exactly in both; with many rows such a call takes some 300 times as long.  Rows and keys outside what
  * is seen may hold anything, NaN included.  Positions beyond max_seq_len need window > 0 and sinks + window + n - 1 <= max_seq_len.
  * A call takes at least 1048560 rows n * n_heads / n_kv_heads of a sequence, and 65535 sequences * n_kv_heads; more are RLH_ERR_UNSUPPORTED.
  * Partial results of sequences that are cut go to work memory that stays with the context, 34 MB at most.  A call that needs more than every

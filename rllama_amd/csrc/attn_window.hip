@@ -14,10 +14,11 @@
 // transposes them in registers with byte permutes, so cached rows go from memory into registers and nowhere else: no LDS, no barrier in
 // the loop.  Tile e of O^T is made of the dims hd / 16 * m + e (m = 0 .. 15).
 //
-// Two arithmetics.  16 bits: f16 operands, v_mfma_f32_16x16x32_f16; the weights are rounded to f16 (half a unit in the eleventh bit each, also far below the largest: kWeightLift;
-// they do not add up over a text).  Values of 4 bits are not: a value is 16 * code * (upper part of the scale / 16) + code * (rest) + lowest, two products that f16 holds exactly
-// for every scale and a term that is the same for 32 dims, and each goes through the matrix cores by itself.  32 bits: everything in f32 through v_mfma_f32_16x16x4_f32; also taken where f16
-// queries meet an f32 cache, whose values f16 may not hold.
+// Two arithmetics.  16 bits: f16 operands, v_mfma_f32_16x16x32_f16, and nothing but the result is rounded to f16.  A weight is the sum of two f16 numbers, 22 bits, and takes
+// two products with V (one row behind 383 positions 7.3 -> 7.5 us, 16 texts with a window 16.2 -> 16.5, 65700 positions in 4 bits 27.4 -> 28.1; rounded to f16 the weights left
+// 1.6e-4 of the result's size).  A value of 4 bits is 16 * code * (upper part of the scale / 16) + code * (rest) + lowest, two products that f16 holds exactly for every
+// scale and a term that is the same for 32 dims, and each goes through the matrix cores by itself.  32 bits: everything in f32 through v_mfma_f32_16x16x4_f32; also
+// taken where f16 queries meet an f32 cache, whose values f16 may not hold.
 //
 // A text is cut into pieces when there are few rows: every workgroup leaves its (m, sum, O) in work memory and a second launch joins them.
 //
@@ -195,22 +196,24 @@ struct Step<half_t, CT, HD> {
     }
     // w[t][i]: weights of positions 16 t + 4 h + i
     __device__ void values(const float4_t (&w)[kTiles], const Q4Bits &bits, float4_t (&o)[kDims], Sums &sums) const {
-        half8_t b;
+        half8_t b, rest; // a weight is the sum of two f16 numbers
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            b[i] = (half_t)w[0][i];
-            b[i + 4] = (half_t)w[1][i];
+        for (int i = 0; i < 8; i++) {
+            const float x = w[i / 4][i % 4];
+            b[i] = (half_t)x;
+            rest[i] = (half_t)(x - (float)b[i]);
         }
         if constexpr (kQ4) {
             // positions two by two: the codes of dims 0 .. 3 of both in one word, those of dims 4 .. 7 in another, and each nibble of the pair
             // becomes a pair (first position, second position) of one dim
-            half8_t b16; // for the rest of the scales (of a sixteenth of a weight f16 keeps enough bits for a part of at most 2^-7 of the value)
+            half8_t b16; // for the rest of the scales: a part of at most 2^-7 of the value, for which the first number of a weight is enough
 #pragma unroll
             for (int i = 0; i < 8; i++) b16[i] = b[i] * (half_t)0.0625f;
             uint4_t low;
 #pragma unroll
             for (int j = 0; j < 4; j++) low[j] = perm(vp[2 * j + 1], vp[2 * j], kHiHalves);
             sums.low = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, low), b, sums.low, 0, 0, 0);
+            sums.low = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, low), rest, sums.low, 0, 0, 0);
             constexpr int kPart = kDims < 4 ? kDims : 4;
 #pragma unroll
             for (int part = 0; part < kDims / kPart; part++) {
@@ -230,6 +233,7 @@ struct Step<half_t, CT, HD> {
                 for (int i = 0; i < kPart; i++) {
                     float4_t &to = o[part * kPart + i];
                     to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, hi[i]), b, to, 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, hi[i]), rest, to, 0, 0, 0);
                     to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, lo[i]), b16, to, 0, 0, 0);
                 }
             }
@@ -240,6 +244,7 @@ struct Step<half_t, CT, HD> {
 #pragma unroll
                 for (int j = 0; j < 4; j++) a[j] = perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], e % 2 ? kHiHalves : kLoHalves);
                 o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), b, o[e], 0, 0, 0);
+                o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), rest, o[e], 0, 0, 0);
             }
         }
     }
@@ -396,13 +401,17 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
     auto whole_step = [&](const Place &at) {
         return at.t0 + kStep - 1 <= min(at.last, p0) && (at.front || p.window == 0 || at.t0 > p1 - p.window);
     };
-    bool skipped = false;
+    bool skipped = false, anew = false;
     auto consume = [&](const St &st, int s, auto slow) {
         const Place here = place_of(s);
         const int t0 = here.t0;
         const bool whole = whole_step(here);
-        if (!whole && __any(st.odd_values()) != decltype(slow)::value) { // (see below)
-            skipped = true;
+        if constexpr (!decltype(slow)::value) { // (see below)
+            if (!whole && __any(st.odd_values())) {
+                skipped = true;
+                return;
+            }
+        } else if (!anew && !__any(st.odd_values())) {
             return;
         }
         float4_t w[kTiles];
@@ -469,11 +478,27 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
         load(st, s);
         consume(st, s, std::false_type{});
     }
-    if (skipped) {
+    if constexpr (St::kLift != 0.0f) {
+        // An infinity that a row sees: the second number of its weight may be 0 or negative, and the sum of both products NaN.
+        float odd = 0.0f; // NaN if a sum is not finite
+#pragma unroll
+        for (int e = 0; e < kDims; e++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) odd = fmaf(o[e][x], 0.0f, odd);
+        anew = __any((int)(odd != 0.0f) & (int)(l_run < INFINITY));
+        if (anew) {
+            m_run = -INFINITY;
+            l_run = 0.0f;
+#pragma unroll
+            for (int e = 0; e < kDims; e++) o[e] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            sums.low = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    if (skipped || anew) {
         // Steps that hold a value that is not finite and that some row may not see: in the product its weight 0 would make a NaN of it.
-        // Such steps were left out above; here every row adds up what it sees, position by position.
+        // Such steps were left out above; here every row adds up what it sees, position by position.  So it does with all steps if some sum is not finite.
         for (int s = s_first; s < s_end; s += kAwWaves) {
-            if (whole_step(place_of(s))) continue;
+            if (!anew && whole_step(place_of(s))) continue;
             St st;
             load(st, s);
             consume(st, s, std::true_type{});

@@ -76,7 +76,7 @@ struct Q4Scale {
 // whether scale and lowest value of a group are finite
 __device__ __forceinline__ bool q4_finite(uint32_t pair) { return (int)((pair & 0x7c000000u) != 0x7c000000u) & (int)((pair & 0x7c00u) != 0x7c00u); }
 
-// Weights that are rounded to f16 are carried this power of two larger: the largest is 2^7, and 2^15 while the reference point lags.  Behind a first token that takes
+// Weights that go through the matrix cores in f16 are carried this power of two larger: the largest is 2^7, and 2^15 while the reference point lags.  Behind a first token that takes
 // most of the weight the others are small; below 2^-14 f16 has fewer than eleven bits and the sum in f32 would keep what the products lose (6000 positions with
 // 0.2 % of the weight: 7e-3 of the result).  So n weights lose n 2^-32 of the result at most to that.
 constexpr float kWeightLift = 7.0f;

@@ -95,6 +95,24 @@ def test_up_to_16_rows_read_4_bits_exactly(ctx, hd, H, G, n, S, window, sinks):
     assert error.mean() <= EPS16 * (np.abs(want).mean() + np.sqrt((V * V).mean()))
 
 
+@pytest.mark.parametrize("hd,H,G,n,T,window", [(128, 4, 4, 1, 1000, 0), (64, 2, 2, 1, 300, 0), (32, 8, 8, 1, 5000, 700), (128, 2, 2, 7, 900, 0)])
+@pytest.mark.parametrize("cache", ["f16", "q4"])
+def test_up_to_16_rows_round_only_their_result(ctx, hd, H, G, n, T, window, cache):
+    """Values whose weighted mean is next to zero for every row, so that the result's own rounding hides nothing."""
+    rng = np.random.default_rng(T + hd)
+    q = np.repeat((rng.standard_normal((1, 1, H, hd)) * 1.5).astype(f16), n, 1)
+    K, V = rng.standard_normal((1, G, T, hd)), rng.standard_normal((1, G, T, hd))
+    K[:, :, T - n + 1:] = K[:, :, T - n:T - n + 1]  # rows that look at nearly the same
+    V[:, :, T - n + 1:] = 0
+    _, want, _, _, V0 = attend(ctx, q, K, V, cache, [T - n], window)
+    got, want, bound, _, V = attend(ctx, q, K, V0 - want[:, 0, :, None], cache, [T - n], window)
+    error, size = np.abs(got - want), np.sqrt((V * V).mean())
+    assert (error <= bound + EPS16 * np.abs(want) + 2.0 ** -24).all()
+    # on average the scores are off by some roundings of f32, which the weights take on independently of each other; weights rounded to
+    # f16 would leave some 2^-15 of V
+    assert error.mean() <= EPS16 * np.abs(want).mean() + 2.0 ** -20 * size
+
+
 # -- a first token that takes most of the weight -----------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("hd,H,G,n,T", [(128, 4, 2, 1, 20000), (64, 8, 1, 2, 65700), (128, 8, 2, 60, 12000), (64, 4, 1, 200, 9000), (128, 32, 8, 130, 6000)])

@@ -341,8 +341,8 @@ int  rlh_qkv_append(rlh_tensor *q, const rlh_tensor *qkv, const rlh_tensor *q_no
  * [n_seqs * n x n_heads head_dim], both f16 or both f32.  f32 rows, or an f32 cache: f32 arithmetic throughout.  Otherwise f16 operands with
  * f32 sums.  Up to 16 rows of a key and value head (n * n_heads / n_kv_heads) round nothing but the result.  With more, the form that is estimated to
  * be the faster one is taken: that one, or one that rounds the softmax's weights and values of 4 bits to f16 in front of its products (half a
- * unit in the eleventh bit, up to 2^-11 of each).  Values of 4 bits beyond what f16 holds are read exactly in both; with many rows such a call takes some 300 times as long.  Rows and keys outside what
- * is seen may hold anything, NaN included.  Positions beyond max_seq_len need window > 0 and sinks + window + n - 1 <= max_seq_len.
+ * unit in the eleventh bit, up to 2^-11 of each; rlh_set_option ATTN_EXACT = 1 leaves it out).  Values of 4 bits beyond what f16 holds are read
+ * exactly there too, and take some 300 times as long.  Rows and keys outside what is seen may hold anything, NaN included.  Positions beyond max_seq_len need window > 0 and sinks + window + n - 1 <= max_seq_len.
  * A call takes at least 1048560 rows n * n_heads / n_kv_heads of a sequence, and 65535 sequences * n_kv_heads; more are RLH_ERR_UNSUPPORTED.
  * Partial results of sequences that are cut go to work memory that stays with the context, 34 MB at most.  A call that needs more than every
  * one before it waits for the context's queued work and allocates it: of a text that gets longer one call or two, when it is first cut. */

@@ -155,6 +155,7 @@ bool tunables_set(Tunables &t, const char *name, const char *value) {
     if (n == "ATTN_SINGLE_MAX") { t.attn_single_max = reset ? dflt.attn_single_max : v; return reset || v >= 0; }
     if (n == "ATTN_MERGE") { t.attn_merge_mode = reset ? dflt.attn_merge_mode : v; return reset || v == 0 || v == 2; }
     if (n == "ATTN_LDS") { t.attn_lds = reset ? 0 : (v != 0); return true; }
+    if (n == "ATTN_EXACT") { t.attn_exact = reset ? 0 : (v != 0); return true; }
     if (n == "PREFILL_ATTN") { t.prefill_attn_gemm = !reset && !strcmp(value, "gemm"); return reset || !strcmp(value, "gemm") || !strcmp(value, "fused"); }
     if (n == "PREFILL_ATTN_ORDER") { t.prefill_attn_order = reset ? dflt.prefill_attn_order : v; return reset || (v >= 0 && v <= 2); }
     if (n == "DECODE_GRAPH") { t.decode_graph = reset ? 0 : (v != 0); return true; }
@@ -174,7 +175,7 @@ bool tunables_set(Tunables &t, const char *name, const char *value) {
 }
 
 void tunables_from_env(Tunables &t) {
-    static const char *const names[] = {"GEMV_BURST", "ATTN_CHUNK", "ATTN_SINGLE_MAX", "ATTN_MERGE", "ATTN_LDS", "PREFILL_ATTN", "PREFILL_ATTN_ORDER",
+    static const char *const names[] = {"GEMV_BURST", "ATTN_CHUNK", "ATTN_SINGLE_MAX", "ATTN_MERGE", "ATTN_LDS", "ATTN_EXACT", "PREFILL_ATTN", "PREFILL_ATTN_ORDER",
                                         "DECODE_GRAPH", "DECODE_FOLD", "GEMM_TILE", "GEMM_SPLIT_K", "GEMM_SPLIT_HALF", "GEMM_DUAL", "GEMM_DUAL_CUT",
                                         "GEMM_ROPE", "FINISH_NORM", "GEMM_KGROUP", "GEMM_SKINNY", "GEMM_ROWS", "GEMM_SPLIT3"};
     for (const char *name : names) {

@@ -51,6 +51,7 @@ struct Tunables {
     int attn_single_max = 384;     // ATTN_SINGLE_MAX=N: longest sequence one workgroup per head handles alone
     int attn_merge_mode = 2;       // ATTN_MERGE=0: the pieces of a split sequence are combined by a second launch; 2: inside the kernel
     int attn_lds = 0;              // ATTN_LDS=1: cache rows staged through LDS (comparison form)
+    int attn_exact = 0;            // ATTN_EXACT=1: rlh_attn_window in f16 rounds nothing but its result, whatever the number of rows
     int prefill_attn_gemm = 0;     // PREFILL_ATTN=gemm: multi-token attention as two batched GEMMs around a softmax kernel
     int prefill_attn_order = 2;    // PREFILL_ATTN_ORDER=0/1/2: launch order of the query blocks of the one-kernel attention
     int decode_graph = 0;          // DECODE_GRAPH=1: greedy decode loops replay one captured HIP graph per token

@@ -190,6 +190,7 @@ extern "C" int rlh_attn_window(rlh_tensor *out, const rlh_tensor *q, const rlh_t
     p.n_seqs = n_seqs;
     p.window = window;
     p.sinks = sinks;
+    p.exact = ctx->tun.attn_exact;
     for (int b = 0; b < n_seqs; b++) p.start[b] = start_pos[b];
     const int cus = ctx->prop.multiProcessorCount;
     const int64_t rows = (int64_t)p.n * (n_heads / n_kv_heads), most = attn_window_most_rows(p, cus);

@@ -621,7 +621,7 @@ static RowsCut cut_rows(const AttnWindowParams &p, int compute_units) {
 // going by them costs 1 to 2 % over always taking the faster one, a fixed limit of 64 rows 11 to 13 %.  (us, this / tiles, 32 heads of 128: 128 rows from position 0
 // 7.1 / 8.8, behind 500 14.9 / 20.0, behind 2000 41 / 21.7; 64 rows behind 4000 44 / 22.)
 static bool tiles_take(const AttnWindowParams &p, int compute_units) {
-    return f16_arithmetic(p) && p.n * (int64_t)(p.n_heads / p.n_kv) > kAwRows && attn_tiles_us(p, compute_units) < cut_rows(p, compute_units).us;
+    return f16_arithmetic(p) && !p.exact && p.n * (int64_t)(p.n_heads / p.n_kv) > kAwRows && attn_tiles_us(p, compute_units) < cut_rows(p, compute_units).us;
 }
 
 int64_t attn_window_most_rows(const AttnWindowParams &p, int compute_units) {

@@ -34,6 +34,7 @@ struct AttnWindowParams {
     int n_heads, n_kv, head_dim, max_seq_len;
     int n, n_seqs;
     int window, sinks;     // window 0: everything up to the row's own position
+    int exact;             // only the form that rounds nothing but the result
     int32_t start[kLongMaxSeqs];
 };
 // rows of one key and value head (n * n_heads / n_kv) that a launch takes; 0: too many sequences and heads

@@ -113,6 +113,17 @@ def test_up_to_16_rows_round_only_their_result(ctx, hd, H, G, n, T, window, cach
     assert error.mean() <= EPS16 * np.abs(want).mean() + 2.0 ** -20 * size
 
 
+@pytest.mark.parametrize("hd,H,G,n,T", [(128, 16, 16, 200, 2000), (64, 20, 20, 200, 3000)])
+@pytest.mark.parametrize("cache", ["f16", "q4"])
+def test_many_rows_round_only_their_result_on_request(ctx, hd, H, G, n, T, cache):
+    """The same for calls that otherwise go to the form that rounds weights and values of 4 bits."""
+    ctx.set_option("ATTN_EXACT", "1")
+    try:
+        test_up_to_16_rows_round_only_their_result(ctx, hd, H, G, n, T, 0, cache)
+    finally:
+        ctx.set_option("ATTN_EXACT", None)
+
+
 # -- a first token that takes most of the weight -----------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("hd,H,G,n,T", [(128, 4, 2, 1, 20000), (64, 8, 1, 2, 65700), (128, 8, 2, 60, 12000), (64, 4, 1, 200, 9000), (128, 32, 8, 130, 6000)])

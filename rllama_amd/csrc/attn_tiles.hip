@@ -7,15 +7,16 @@
 //
 // Rounded to f16: the softmax's weights, as operands of the second product, and 4-bit values when they are converted (lowest + code * scale, one rounding of at most
 // 2^-11 of the value, where the codes themselves are off by 1/30 of a group's range).  Random values, a window of 1024: the result is off by 4.6e-4 of its size, 2.6e-4
-// with an f16 cache, 2.1e-4 with nothing but the result rounded.  Exact values would take two products for each of these.
+// with an f16 cache, 2.1e-4 with nothing but the result rounded, as in the form for few rows.  Weights as sums of two f16 numbers alone took 57 -> 78 us (2048 rows of 40
+// heads) and 51 -> 61 (1500 rows with a window over 4 bits, then 4.1e-4); values of 4 bits would take a second product each besides.
 //
 // Tiles that every row of the wavefront sees whole, in the middle of a run of rows that lie side by side in the cache, go through a loop of their own with
 // nothing but running addresses between the products.  (2048 rows behind 2000 positions, 32 heads of 128 on 8: 133 us with the place of every tile and its
 // masks worked out anew, 119 so.)
 //
-// Measured: 2048 rows from position 0, 40 heads of 128, 43 GFLOP: 57 us, 750 TFLOP/s; 2048 rows behind 2000 positions, 32 heads on 8, 101 GFLOP: 110 us, 920 (a large
-// library product reaches 1190).  The matrix cores are busy for a third of the first: texts from position 0 give workgroups of 2 to 32 tiles, so that on average
-// 1.3 wavefronts of two per SIMD are there, and a tile's softmax costs a wavefront as many cycles of vector ALU as its products take on the matrix cores.
+// Measured: 2048 rows from position 0, 40 heads of 128, 43 GFLOP: 56 us, 765 TFLOP/s; 2048 rows behind 2000 positions, 32 heads on 8, 101 GFLOP: 112 us, 900 (a large
+// library product reaches 1190).  The matrix cores are busy for 34 % of the first, the vector ALU for 38 %: texts from position 0 give workgroups of 2 to 32 tiles, so that on
+// average 1.3 wavefronts of two per SIMD are there, which wait for 23 % of their time.
 //
 // Both products run transposed through v_mfma_f32_32x32x16_f16, so that a row is a lane pair's column of both results:
 //   S^T [key x row] = K . q^T,   O^T [dim x row] += V^T . W

@@ -22,9 +22,10 @@
 //
 // A text is cut into pieces when there are few rows: every workgroup leaves its (m, sum, O) in work memory and a second launch joins them.
 //
-// Measured: 16 texts, one row each over a window of 1024 and 4, 32 heads on 8 of 128: 63 MB in 13.3 us, 4.8 TB/s, and 3.9 us of join.  5 rows in f32 behind 2107
-// positions of 32 heads: 69 MB in 15.4 us, 4.5 TB/s.  Both are bound by memory.  One row behind 65700 positions in 4 bits, 64 heads on 8: 84 MB in 24.3 us,
-// 3.5 TB/s: bound by the vector ALU, which takes codes apart.  One row behind 383 positions, 6.3 MB: 7.7 us, a chain of latencies.
+// Measured: 16 texts, one row each over a window of 1024 and 4, 32 heads on 8 of 128: 63 MB in 13.4 us, 4.7 TB/s, and 3.9 us of join.  5 rows in f32 behind 2107
+// positions of 32 heads: 69 MB in 15.0 us, 4.6 TB/s.  Both are bound by memory.  One row behind 65700 positions in 4 bits, 64 heads on 8: 84 MB in 25.8 us,
+// 3.3 TB/s: nothing is saturated (vector ALU 43 %, matrix cores 15 %); its 166 registers leave one workgroup to a compute unit, two wavefronts per SIMD, each of which waits for
+// the loads of a step 41 % of its time.  One row behind 383 positions, 6.3 MB: 7.6 us, a chain of latencies.
 #include "kernels.h"
 #include "attn_window_device.h"
 
@@ -470,8 +471,7 @@ __global__ __launch_bounds__(kAwThreads) void attn_rows_kernel(AttnCutParams pp)
                 }
         }
     };
-    // (The other wavefronts cover a step's wait for memory: a second set of operands, loaded ahead, gained nothing at any length and cost 2 to 8 % in f32 for
-    // its registers.)
+    // (A second set of operands, loaded ahead, gained nothing at any length and cost 2 to 8 % in f32 for its registers.)
     const int s_end = min(span.steps, (piece + 1) * pp.piece_steps), s_first = piece * pp.piece_steps + wave;
     for (int s = s_first; s < s_end; s += kAwWaves) {
         St st;
@@ -617,8 +617,8 @@ static RowsCut cut_rows(const AttnWindowParams &p, int compute_units) {
 }
 
 // The tiles of attn_tiles.hip take 128 rows at once, this kernel 16: it reads K and V once per 16 rows, but has more workgroups, no second rounding of 4-bit values
-// and more wavefronts per key.  Both sides' estimates were fitted to 180 measured shapes (17 .. 2400 rows per key and value head, 0 .. 8000 positions, f16 and 4 bits);
-// going by them costs 1 to 2 % over always taking the faster one, a fixed limit of 64 rows 11 to 13 %.  (us, this / tiles, 32 heads of 128: 128 rows from position 0
+// and more wavefronts per key.  Both sides' estimates were fitted to measured shapes (17 .. 2400 rows per key and value head, 0 .. 8000 positions, f16 and 4 bits);
+// over 262 of them going by the estimates costs 1.5 % over always taking the faster one, 60 % at worst, a fixed limit of 64 rows 11 to 13 %, 140 at worst.  (us, this / tiles, 32 heads of 128: 128 rows from position 0
 // 7.1 / 8.8, behind 500 14.9 / 20.0, behind 2000 41 / 21.7; 64 rows behind 4000 44 / 22.)
 static bool tiles_take(const AttnWindowParams &p, int compute_units) {
     return f16_arithmetic(p) && !p.exact && p.n * (int64_t)(p.n_heads / p.n_kv) > kAwRows && attn_tiles_us(p, compute_units) < cut_rows(p, compute_units).us;

@@ -8,9 +8,9 @@
 // 8 consecutive elements per lane: 16-byte accesses, the sum of squares is one exchange over at most 16 lanes, and a 4-bit group is four
 // neighbouring lanes, so quantising needs no memory of its own.
 //
-// Measured: 1500 rows of 32 heads on 8 of 128 into 4 bits, 33 MB: 11.8 us, 2.8 TB/s (a copy of as many bytes: 7.9).  All workgroups are on the part at once, so
+// Measured: 1500 rows of 32 heads on 8 of 128 into 4 bits, 33 MB: 11.8 to 12.7 us, 2.7 TB/s (a copy of as many bytes: 7.9).  All workgroups are on the part at once, so
 // their loads, their arithmetic and their stores come one after the other.  One row of 32 heads: 2.7 us, a launch.
-// Call after call: 11.0 us; into f16 9.4 (4.0 TB/s), 32 key and value heads into f16 14.6 (5.1 TB/s).
+// Call after call, the rows in the caches: 9.0 us; into f16 8.4, 32 key and value heads into f16 13.3.
 #include "kernels.h"
 #include "longctx.h"
 

@@ -9,9 +9,10 @@ typedef half_t half4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 // ---- softmax of rows ---------------------------------------------------------------------------------------------------------
 // p_i = exp((x_i - m) / T) / sum_j exp((x_j - m) / T), m the row's largest.  Bound by memory.  One workgroup per row; a row of up to 32768 elements is
-// read once and stays in registers (32 per thread) between the two reductions, a longer one is read a second time, from the caches.
+// read once and stays in registers (32 per thread) between the two reductions, a longer one is read three times: maximum, sum, result.
 // T = 0: 1 at the first of the largest.
-// Measured, rows of 32000: 320 in f16, 61 MB, 13.6 us, 4.5 TB/s; 5 in f32 5.9 us, two reductions over 1024 threads.
+// Measured, rows of 32000: 320 in f16, 61 MB, 13.0 us, 4.7 TB/s; 5 in f32 5.9 us, two reductions over 1024 threads.  Rows of 128256, f16: 320, 246 MB if each is
+// read and written once, 67 us, 3.7 TB/s.
 template <typename T>
 __device__ __forceinline__ float4_t load4(const T *x, int i, int n, float fill) {
     float4_t v;
@@ -146,8 +147,8 @@ hipError_t launch_softmax_rows(float *probs, const void *logits, int logits_f16,
 // is taken in whole numbers (2^-31 of a probability: one conversion per entry, 64-bit sums), so it is exact and the drawn token does
 // not depend on how the row is shared: every wavefront sums a contiguous piece of the row in chunks of 256 entries (four neighbouring ones per lane), keeps
 // the chunks' sums in LDS, and the wavefront whose piece holds the drawn place reads that one chunk again.
-// Bound by latency: three dependent trips to memory (the ids, their probabilities, the row).  Rows of 32000: one sequence of 4 drafted tokens 9.6 us, 64 of 7
-// 11.9 us (16 MB).
+// Bound by latency: three dependent trips to memory (the ids, their probabilities, the row).  Rows of 32000: one sequence of 4 drafted tokens 9.8 us, 64 of 7
+// 11.4 us (16 MB).
 constexpr int kVdThreads = 1024;
 constexpr int kVdWaves = kVdThreads / kWave;
 constexpr int kVdChunks = 64; // per wavefront at most; longer rows have larger chunks

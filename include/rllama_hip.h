@@ -45,8 +45,11 @@ typedef enum {
  * (token ids) are taken by the calls that say so; every other call refuses them with RLH_ERR_UNSUPPORTED.
  * A 4-bit tensor [rows x cols], cols a multiple of 32, is one buffer of rows * cols / 32 * 20 bytes: first the codes, row after row,
  * two to a byte (the even column in the low half), then for each row and each group of 32 columns a pair of f16 numbers (scale,
- * lowest).  A value is lowest + code * scale. */
-typedef enum { RLH_F16 = 0, RLH_F32 = 1, RLH_Q4 = 2, RLH_I32 = 3 } rlh_dtype;
+ * lowest).  A value is lowest + code * scale.
+ * RLH_F8 and RLH_F8_TILES are 8-bit floating point (e4m3: 448 at most, no infinities), also taken by the calls that say so: [rows x cols], cols a multiple
+ * of 16, is one buffer of the codes, rows * cols bytes, row after row, and then f32 scales.  A value is code * scale.  RLH_F8: a scale for every 128 columns of
+ * a row, [rows x ceil(cols / 128)]; RLH_F8_TILES: one for every tile of 128 rows and 128 columns, [ceil(rows / 128) x ceil(cols / 128)]. */
+typedef enum { RLH_F16 = 0, RLH_F32 = 1, RLH_Q4 = 2, RLH_I32 = 3, RLH_F8 = 5, RLH_F8_TILES = 6 } rlh_dtype;
 
 /* Weight names: src/transformer.rs:297-304, 405-412, 490-503, 595-614; src/embedding.rs:18 */
 typedef enum {
@@ -320,7 +323,7 @@ int  rlh_tensor_wrap(rlh_ctx *ctx, void *device_memory, int rows, int cols, int 
 int  rlh_wait_stream(rlh_ctx *ctx, void *stream);
 /* ... and later work on `stream` for what is queued on the context by now.  Neither makes the host wait. */
 int  rlh_release_stream(rlh_ctx *ctx, void *stream);
-/* dst = src between f16, f32 and Q4 tensors of one shape.  To Q4, per group of 32 columns: lowest = f16(min), scale =
+/* dst = src between f16, f32 and Q4 tensors of one shape, and between f16 or f32 and 8 bits (see below).  To Q4, per group of 32 columns: lowest = f16(min), scale =
  * f16((max - lowest) / 15), code = round((x - lowest) / scale), ties to even, within 0..15 (code 0 where the scale is not above 0, as in a
  * group of one value).  A group with a value that is not finite, or whose lowest or scale f16 cannot hold, reads as NaN throughout. */
 int  rlh_convert(rlh_tensor *dst, const rlh_tensor *src);
@@ -361,6 +364,36 @@ int  rlh_softmax_rows(rlh_tensor *probs, const rlh_tensor *logits, float tempera
  * running sum exceeds floor(sum * m / 2^24): the same whatever order the sums are formed in.  Where nothing is left of max(p - q, 0) the
  * weights are p's; where p has no positive entry either, the drawn token is -1. */
 int  rlh_verify_draft(rlh_tensor *out, const rlh_tensor *target, const rlh_tensor *draft, const rlh_tensor *drafted, const rlh_tensor *uniforms);
+
+/* ------------------------------------------------------------------------------------------------
+ * Many answers to one prompt (no reference counterpart): one step of a batch of texts that share a long prefix, with weights of 8 bits.  All work is queued on the
+ * context's stream; a call waits for nothing.  Work memory that a call needs beyond its operands stays with the context: a call that needs more than every one before it
+ * allocates it, and is refused with RLH_ERR_STATE while the stream is being captured (make one call of that size before).  Buffers that were outgrown are kept until the
+ * context ends, so a captured graph stays valid; graphs of one context share them and must not run side by side.
+ * ---------------------------------------------------------------------------------------------- */
+/* rlh_rope_table of positions first .. first + rows - 1: row 0 of the table that rlh_qkv_append takes for texts behind a prefix is position prefix_len. */
+int  rlh_rope_table_from(rlh_tensor *freqs, double theta, int first);
+/* Attention of n rows of each of n_seqs texts (1..256) that continue one prefix.  Row b * n + i is text b's row at position start_pos[b] + i, counted from the prefix's end: it
+ * sees the prefix_len positions of the prefix and the text's own positions up to its own; out = softmax(q K^T / sqrt(head_dim)) V over them.  A negative position is padding:
+ * its rows of the result are zeros.  Prefix planes: two tensors [n_kv_heads * prefix_rows x head_dim], row g * prefix_rows + t, prefix_rows >= prefix_len (no prefix: 0, and
+ * the planes may be NULL); cache planes: two tensors [n_seqs * n_kv_heads * max_seq_len x head_dim], row (b * n_kv_heads + g) * max_seq_len + t, which hold the rows' own positions
+ * already; all four of one dtype, f16, f32 or Q4; head_dim 32, 64 or 128.  Query head h reads key and value head h / (n_heads / n_kv_heads).  q and out
+ * [n_seqs * n x n_heads head_dim], both f16 or both f32.  f32 rows, or f32 planes: f32 arithmetic throughout; otherwise f16 operands with f32 sums.
+ * The prefix is read once for the rows of all texts and not once for each.  Rows and keys outside what is seen may hold anything, NaN included. */
+int  rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *prefix_k, const rlh_tensor *prefix_v, int prefix_len, const rlh_tensor *cache_k,
+                     const rlh_tensor *cache_v, int n_heads, int n_kv_heads, int max_seq_len, const int32_t *start_pos, int n_seqs);
+/* Log probabilities under softmax(logits / temperature), logits f16 or f32 [n x vocab]: logprobs f32 [n x m] those of tokens i32 [n x m] (a negative id, a place without
+ * a token: 0; an id past the vocabulary: -infinity); entropy f32 [n x 1], in nats; top_ids i32 and top_logprobs f32 [n x k], k up to 32, the k most probable ids of each
+ * row, the lowest first among equal ones.  logprobs and tokens, entropy, and top_ids and top_logprobs may each be NULL, but not all of them.  temperature: 1e-30 to 1e30.
+ * Logits of -infinity have probability 0.  A row of nothing else: -infinity, entropy 0, the first k ids.  A row with a NaN or +infinity: NaN, and ids of -1. */
+int  rlh_token_logprobs(rlh_tensor *logprobs, rlh_tensor *entropy, rlh_tensor *top_ids, rlh_tensor *top_logprobs, const rlh_tensor *logits, const rlh_tensor *tokens,
+                        float temperature);
+/* rlh_convert to 8 bits: per block, a = max(largest |x|, 448 * 2^-126), scale = a / 448, code = e4m3(x * (448 / a)), each step one f32 operation, the last one rounded to
+ * even and limited to 448.  A block with a value that is not finite reads as NaN throughout.  From 8 bits: code * scale in f32, rounded once more for f16.
+ *
+ * dst [n x m] = src [n x k] times weights[m x k]^T: weights RLH_F8_TILES; src RLH_F8, or f16 or f32, which is converted to RLH_F8 first; dst f16 or f32.
+ * Products and sums of a block of 128 in f32, each block's sum times both scales in f32. */
+int  rlh_matrix_mul_f8(rlh_tensor *dst, const rlh_tensor *src, const rlh_tensor *weights);
 
 /* ------------------------------------------------------------------------------------------------
  * Measurement aids (no reference counterpart; src/benches/benchmark.rs times the CPU/OpenCL ops with criterion).

@@ -26,11 +26,23 @@ TOK_EMB, WQ, WK, WV, WO, W1, W2, W3, ATTN_NORM, FFN_NORM, NORM, OUTPUT = range(1
 
 class TensorDType:
     """TensorDType of src/tensor.rs:50-54 (the reference names the 4-bit variant and leaves it unimplemented; here cache planes and
-    convert() take it), and whole numbers (token ids)."""
+    convert() take it), whole numbers (token ids), and 8-bit floating point with a scale for each 128 columns of a row (Float8) or each tile
+    of 128 x 128 (Float8Tiles: weights)."""
     Float16 = 0
     Float32 = 1
     K4BitQuantization = 2
     Int32 = 3
+    Float8 = 5
+    Float8Tiles = 6
+
+    @staticmethod
+    def buffer_bytes(dtype: int, rows: int, cols: int) -> int:
+        """Bytes of a tensor of 4 or 8 bits: its codes and then its scales."""
+        if dtype == TensorDType.K4BitQuantization:
+            return rows * cols // 32 * 20
+        if dtype not in (TensorDType.Float8, TensorDType.Float8Tiles):
+            raise ValueError(f"type {dtype} is not one of codes and scales")
+        return rows * cols + 4 * (rows if dtype == TensorDType.Float8 else -(-rows // 128)) * -(-cols // 128)
 
 
 def llama_ffn_hidden(dim: int, multiple_of: int = 256) -> int:
@@ -340,6 +352,19 @@ class Tensor:
         return Tensor(ctx, h, rows, cols, TensorDType.K4BitQuantization)
 
     @staticmethod
+    def from_f8(ctx: Context, codes: np.ndarray, scales: np.ndarray) -> "Tensor":
+        """A tensor of 8 bits from its e4m3 codes (uint8 [rows x cols]) and its scales (float32: [rows x ceil(cols / 128)], a scale for every 128 columns of a
+        row, or [ceil(rows / 128) x ceil(cols / 128)], one for every tile; a single row has the first)."""
+        c, s = np.ascontiguousarray(codes), np.ascontiguousarray(scales)
+        if c.dtype != np.uint8 or c.ndim != 2 or s.dtype != np.float32 or s.ndim != 2 or s.shape[1] != -(-c.shape[1] // 128) or s.shape[0] not in (c.shape[0], -(-c.shape[0] // 128)):
+            raise ValueError(f"codes {c.dtype} {c.shape} and scales {s.dtype} {s.shape} do not fit each other")
+        kind = TensorDType.Float8 if s.shape[0] == c.shape[0] else TensorDType.Float8Tiles
+        a = np.concatenate([c.reshape(-1), s.reshape(-1).view(np.uint8)])
+        h = C.c_void_p()
+        check(ctx._lib.rlh_tensor_upload(ctx._h, a.ctypes.data_as(C.c_void_p), c.shape[0], c.shape[1], c.shape[1], kind, C.byref(h)))
+        return Tensor(ctx, h, c.shape[0], c.shape[1], kind)
+
+    @staticmethod
     def zeros(ctx: Context, rows: int, cols: int, dtype: int) -> "Tensor":
         h = C.c_void_p()
         check(ctx._lib.rlh_tensor_alloc(ctx._h, rows, cols, dtype, C.byref(h)))
@@ -363,10 +388,10 @@ class Tensor:
         return self._dtype
 
     def to_numpy(self) -> np.ndarray:
-        """to_cpu_inplace (src/tensor.rs:2150-2166): f16 tensors come back as float16 arrays, whole numbers as int32; of a 4-bit tensor the
-        buffer as bytes (convert() gives the values, from_q4() the tensor again)."""
-        if self._dtype in (TensorDType.K4BitQuantization, TensorDType.Int32):
-            shape, kind = ((self._rows, self._cols), np.int32) if self._dtype == TensorDType.Int32 else (self._rows * self._cols // 32 * 20, np.uint8)
+        """to_cpu_inplace (src/tensor.rs:2150-2166): f16 tensors come back as float16 arrays, whole numbers as int32; of a tensor of 4 or 8 bits
+        the buffer as bytes (convert() gives the values, from_q4() and from_f8() the tensor again)."""
+        if self._dtype not in (TensorDType.Float16, TensorDType.Float32):
+            shape, kind = ((self._rows, self._cols), np.int32) if self._dtype == TensorDType.Int32 else (TensorDType.buffer_bytes(self._dtype, self._rows, self._cols), np.uint8)
             out = np.empty(shape, dtype=kind)
             check(self._lib.rlh_tensor_download(self._h, out.ctypes.data_as(C.c_void_p), self._cols, None))
             return out
@@ -461,7 +486,7 @@ class Tensor:
 
     # long contexts and drafted tokens
     def convert(self, dtype: Optional[int] = None, out: Optional["Tensor"] = None) -> "Tensor":
-        """The same values as f16, f32 or 4 bits."""
+        """The same values as f16, f32, 4 or 8 bits."""
         out = out or Tensor.zeros(self.ctx, self._rows, self._cols, dtype)
         check(self._lib.rlh_convert(out._h, self._h))
         return out
@@ -497,6 +522,41 @@ class Tensor:
         """self = drafted ids i32 [n_seqs x k]: i32 [n_seqs x (k + 2)] of how many are accepted, those, the token drawn behind them, -1 after it."""
         out = out or Tensor.zeros(self.ctx, self._rows, self._cols + 2, TensorDType.Int32)
         check(self._lib.rlh_verify_draft(out._h, target._h, draft._h if draft else None, self._h, uniforms._h))
+        return out
+
+    # many answers to one prompt
+    def rope_table_from(self, first: int, theta: float = 10000.0) -> "Tensor":
+        """self f32 [positions x head_dim] becomes the table of angles of positions first, first + 1, ...: for texts behind a prefix of `first` positions."""
+        check(self._lib.rlh_rope_table_from(self._h, theta, first))
+        return self
+
+    def attn_shared(self, prefix_k: Optional["Tensor"], prefix_v: Optional["Tensor"], prefix_len: int, cache_k: "Tensor", cache_v: "Tensor", n_heads: int, n_kv_heads: int,
+                    max_seq_len: int, start_pos: Sequence[int], out: Optional["Tensor"] = None) -> "Tensor":
+        """self = q [rows x n_heads head_dim] after qkv_append: attention of the rows of texts that continue one prefix over its planes
+        [n_kv_heads * prefix_rows x head_dim] and their own; start_pos counts from the prefix's end."""
+        out = out or self._like()
+        check(self._lib.rlh_attn_shared(out._h, self._h, prefix_k._h if prefix_k else None, prefix_v._h if prefix_v else None, prefix_len, cache_k._h, cache_v._h, n_heads,
+                                        n_kv_heads, max_seq_len, (C.c_int32 * len(start_pos))(*start_pos), len(start_pos)))
+        return out
+
+    def token_logprobs(self, tokens: Optional["Tensor"] = None, temperature: float = 1.0, top: int = 0, logprobs: Optional["Tensor"] = None, entropy: Optional["Tensor"] = None,
+                       top_ids: Optional["Tensor"] = None, top_logprobs: Optional["Tensor"] = None):
+        """self = logits [n x vocab]: (log probabilities of tokens i32 [n x m], entropy [n x 1], the `top` most probable ids and their log probabilities [n x top]);
+        None in the place of what is not asked for.  Results that are given are written to instead."""
+        make = lambda cols, kind: Tensor.zeros(self.ctx, self._rows, cols, kind)  # noqa: E731
+        logprobs = logprobs or (make(tokens._cols, TensorDType.Float32) if tokens else None)
+        entropy = entropy or make(1, TensorDType.Float32)
+        top_ids = top_ids or (make(top, TensorDType.Int32) if top else None)
+        top_logprobs = top_logprobs or (make(top_ids._cols, TensorDType.Float32) if top_ids else None)
+        handle = lambda t: t._h if t else None  # noqa: E731
+        check(self._lib.rlh_token_logprobs(handle(logprobs), entropy._h, handle(top_ids), handle(top_logprobs), self._h, handle(tokens), temperature))
+        return logprobs, entropy, top_ids, top_logprobs
+
+    def matrix_mul_f8(self, weights: "Tensor", dtype: Optional[int] = None, out: Optional["Tensor"] = None) -> "Tensor":
+        """self [n x k], f16, f32 or Float8, times weights[m x k]^T in Float8Tiles -> [n x m] of `dtype`, self's own type (of Float8: f16)."""
+        kind = dtype if dtype is not None else TensorDType.Float16 if self._dtype == TensorDType.Float8 else self._dtype
+        out = out or Tensor.zeros(self.ctx, self._rows, weights._rows, kind)
+        check(self._lib.rlh_matrix_mul_f8(out._h, self._h, weights._h))
         return out
 
     def argmax_greedy(self, temperature: float = 1.0) -> int:

@@ -104,6 +104,10 @@ SIGNATURES = {
     "rlh_attn_window": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _i32p, C.c_int, C.c_int, C.c_int]),
     "rlh_softmax_rows": (C.c_int, [_vp, _vp, C.c_float]),
     "rlh_verify_draft": (C.c_int, [_vp, _vp, _vp, _vp, _vp]),
+    "rlh_rope_table_from": (C.c_int, [_vp, C.c_double, C.c_int]),
+    "rlh_attn_shared": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _i32p, C.c_int]),
+    "rlh_token_logprobs": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_float]),
+    "rlh_matrix_mul_f8": (C.c_int, [_vp, _vp, _vp]),
     "rlh_model_time_kernel": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _fp, C.POINTER(C.c_uint64)]),
     "rlh_time_gemv": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _fp]),
     "rlh_probe_gemv_phases": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, _fp]),

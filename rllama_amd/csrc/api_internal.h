@@ -27,6 +27,16 @@ int set_error(int code, const char *msg);
         }                                                                                                      \
     } while (0)
 
+// Work memory that a graph may go on using after a later call has needed more: buffers that were too small are kept until the context ends (each is twice the one
+// before at least, so they hold no more than the last one).
+struct AnswerWork {
+    static constexpr int kMost = 24;
+    void *kept[kMost] = {};
+    int count = 0;
+    size_t bytes = 0; // of the last one
+    void *memory() const { return count > 0 ? kept[count - 1] : nullptr; }
+};
+
 // Work memory of the op-level entry points that need more than their operands (rlh_attn_decode, rlh_argmax_greedy):
 // allocated on first use, kept until rlh_shutdown.
 struct OpScratch {
@@ -39,6 +49,8 @@ struct OpScratch {
     size_t gemm_ws_bytes = 0;
     float *window_ws = nullptr;    // rlh_attn_window: partial results of sequences that are cut
     size_t window_ws_floats = 0;
+    AnswerWork shared_work;        // rlh_attn_shared: partial results
+    AnswerWork f8_work;            // rlh_matrix_mul_f8: src in 8 bits
 };
 constexpr int kOpMaxHeads = 1024;
 
@@ -63,6 +75,8 @@ namespace rlh {
 bool tunables_set(Tunables &t, const char *name, const char *value);
 void tunables_from_env(Tunables &t);
 } // namespace rlh
+
+inline bool known_dtype(int dtype) { return (dtype >= RLH_F16 && dtype <= RLH_I32) || dtype == RLH_F8 || dtype == RLH_F8_TILES; }
 
 constexpr size_t kStageBytes = (size_t)1 << 20;
 
@@ -95,9 +109,14 @@ struct rlh_tensor {
     // is freed, so the buffer is not handed out again but freed, which waits for the device
     mutable std::atomic<bool> lent{false};
     bool wrapped = false; // the memory is the caller's
-    size_t esize() const { return dtype == RLH_F16 ? 2 : 4; } // (not of RLH_Q4, which has no whole bytes per element)
+    size_t esize() const { return dtype == RLH_F16 ? 2 : 4; } // (not of 4 and 8 bits, whose buffers hold scales too)
     size_t count() const { return (size_t)rows * cols; }
-    size_t bytes() const { return dtype == RLH_Q4 ? count() / 32 * 20 : count() * esize(); }
+    size_t bytes() const {
+        if (is_eight()) return count() + ((size_t)rows + (dtype == RLH_F8 ? 0 : 127)) / (dtype == RLH_F8 ? 1 : 128) * (((size_t)cols + 127) / 128) * sizeof(float);
+        return dtype == RLH_Q4 ? count() / 32 * 20 : count() * esize();
+    }
+    bool is_eight() const { return dtype == RLH_F8 || dtype == RLH_F8_TILES; }
+    bool whole_buffer() const { return dtype == RLH_Q4 || is_eight(); } // travels as its whole buffer
     bool is_float() const { return dtype == RLH_F16 || dtype == RLH_F32; }
 };
 

@@ -1,8 +1,8 @@
 // api_longctx.hip -- entry points of the C ABI for long contexts and drafted tokens (include/rllama_hip.h): tensors over the caller's
 // memory, conversion to and from 4 bits, the append of a projection's rows to the caches, attention with a window, the
 // probabilities of rows of logits and the verification of drafted tokens.
-#include "api_internal.h"
-#include "longctx.h"
+#include "api_planes.h"
+#include "answers.h"
 
 #include <climits>
 #include <cmath>
@@ -10,17 +10,10 @@
 
 using namespace rlh;
 
-static PlaneRef plane_of(const rlh_tensor *t) {
-    PlaneRef r{t->p, nullptr};
-    if (t->dtype == RLH_Q4) r.pairs = reinterpret_cast<uint32_t *>(static_cast<char *>(t->p) + q4_pairs_offset(t->count()));
-    return r;
-}
-static int plane_type(const rlh_tensor *t) { return t->dtype == RLH_F16 ? kPlaneF16 : t->dtype == RLH_F32 ? kPlaneF32 : kPlaneQ4; }
-static bool shaped(const rlh_tensor *t, int64_t rows, int64_t cols) { return t->rows == rows && t->cols == cols; }
-
 extern "C" int rlh_tensor_wrap(rlh_ctx *ctx, void *device_memory, int rows, int cols, int dtype, rlh_tensor **out) {
-    if (!ctx || !out || !device_memory || rows <= 0 || cols <= 0 || dtype < RLH_F16 || dtype > RLH_I32) return fail(RLH_ERR_INVALID, "rlh_tensor_wrap: bad argument");
+    if (!ctx || !out || !device_memory || rows <= 0 || cols <= 0 || !known_dtype(dtype)) return fail(RLH_ERR_INVALID, "rlh_tensor_wrap: bad argument");
     if (dtype == RLH_Q4 && cols % kQ4Group != 0) return fail(RLH_ERR_INVALID, "rlh_tensor_wrap: %d columns of 4 bits: a multiple of %d is needed", cols, kQ4Group);
+    if (dtype >= RLH_F8 && cols % 16 != 0) return fail(RLH_ERR_INVALID, "rlh_tensor_wrap: %d columns of 8 bits: a multiple of 16 is needed", cols);
     if (reinterpret_cast<uintptr_t>(device_memory) % 16 != 0) return fail(RLH_ERR_INVALID, "rlh_tensor_wrap: the memory must be 16-byte aligned");
     *out = nullptr;
     rlh_tensor *t = new (std::nothrow) rlh_tensor();
@@ -60,10 +53,19 @@ extern "C" int rlh_release_stream(rlh_ctx *ctx, void *stream) {
 
 extern "C" int rlh_convert(rlh_tensor *dst, const rlh_tensor *src) {
     if (!dst || !src || dst->rows != src->rows || dst->cols != src->cols) return fail(RLH_ERR_INVALID, "rlh_convert: two tensors of one shape are needed");
-    if (dst->dtype == RLH_I32 || src->dtype == RLH_I32) return fail(RLH_ERR_UNSUPPORTED, "rlh_convert: f16, f32 and 4-bit tensors only");
+    if (dst->dtype == RLH_I32 || src->dtype == RLH_I32) return fail(RLH_ERR_UNSUPPORTED, "rlh_convert: f16, f32, 4-bit and 8-bit tensors only");
     if (dst->dtype == src->dtype) return rlh_copy_inplace(dst, src);
+    if ((dst->is_eight() && !src->is_float()) || (src->is_eight() && !dst->is_float())) return fail(RLH_ERR_UNSUPPORTED, "rlh_convert: 8 bits from and to f16 and f32 only");
     CtxLock lock(dst->ctx);
     lend(dst->ctx, {src});
+    if (dst->is_eight()) {
+        HIP_TRY(launch_f8_encode(eight_of(dst), src->p, src->dtype == RLH_F16, dst->rows, dst->cols, dst->ctx->stream));
+        return RLH_OK;
+    }
+    if (src->is_eight()) {
+        HIP_TRY(launch_f8_decode(dst->p, dst->dtype == RLH_F16, eight_of(src), dst->rows, dst->cols, dst->ctx->stream));
+        return RLH_OK;
+    }
     HIP_TRY(launch_plane_convert(plane_of(dst), plane_type(dst), plane_of(src), plane_type(src), dst->count(), dst->ctx->stream));
     return RLH_OK;
 }
@@ -78,7 +80,7 @@ static int plan_rows(const char *who, const rlh_tensor *ck, const rlh_tensor *cv
                      int rows, RowPlan *plan) {
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0) return fail(RLH_ERR_INVALID, "%s: %d heads do not share %d key and value heads evenly", who, n_heads, n_kv_heads);
     if (!start_pos || n_seqs < 1 || n_seqs > kLongMaxSeqs) return fail(RLH_ERR_INVALID, "%s: 1 to %d sequences with a position each", who, kLongMaxSeqs);
-    if (!ck || !cv || max_seq_len <= 0 || ck->dtype != cv->dtype || ck->dtype == RLH_I32 || ck->rows != cv->rows || ck->cols != cv->cols ||
+    if (!ck || !cv || max_seq_len <= 0 || ck->dtype != cv->dtype || !holds_plane(ck) || ck->rows != cv->rows || ck->cols != cv->cols ||
         (int64_t)ck->rows != (int64_t)n_seqs * n_kv_heads * max_seq_len) {
         return fail(RLH_ERR_INVALID, "%s: cache planes must be two [n_seqs * n_kv_heads * max_seq_len x head_dim] tensors of one dtype", who);
     }

@@ -18,8 +18,9 @@ using namespace rlh;
 // op level
 // ------------------------------------------------------------------------------------------------
 extern "C" int rlh_tensor_alloc(rlh_ctx *ctx, int rows, int cols, int dtype, rlh_tensor **out) {
-    if (!ctx || !out || rows <= 0 || cols <= 0 || dtype < RLH_F16 || dtype > RLH_I32) return fail(RLH_ERR_INVALID, "rlh_tensor_alloc: bad argument");
+    if (!ctx || !out || rows <= 0 || cols <= 0 || !known_dtype(dtype)) return fail(RLH_ERR_INVALID, "rlh_tensor_alloc: bad argument");
     if (dtype == RLH_Q4 && cols % 32 != 0) return fail(RLH_ERR_INVALID, "rlh_tensor_alloc: %d columns of 4 bits: a multiple of 32 is needed", cols);
+    if (dtype >= RLH_F8 && cols % 16 != 0) return fail(RLH_ERR_INVALID, "rlh_tensor_alloc: %d columns of 8 bits: a multiple of 16 is needed", cols);
     *out = nullptr;
     CtxLock lock(ctx);
     rlh_tensor *t = new rlh_tensor();
@@ -46,7 +47,7 @@ extern "C" int rlh_tensor_alloc(rlh_ctx *ctx, int rows, int cols, int dtype, rlh
 
 extern "C" int rlh_tensor_upload(rlh_ctx *ctx, const void *host, int rows, int cols, int cols_capacity, int dtype, rlh_tensor **out) {
     if (!host || cols_capacity < cols) return fail(RLH_ERR_INVALID, "rlh_tensor_upload: bad argument");
-    if (dtype == RLH_Q4 && cols_capacity != cols) return fail(RLH_ERR_UNSUPPORTED, "rlh_tensor_upload: a 4-bit tensor travels as its whole buffer (cols_capacity = cols)");
+    if ((dtype == RLH_Q4 || dtype >= RLH_F8) && cols_capacity != cols) return fail(RLH_ERR_UNSUPPORTED, "rlh_tensor_upload: a tensor of 4 or 8 bits travels as its whole buffer (cols_capacity = cols)");
     int rc = rlh_tensor_alloc(ctx, rows, cols, dtype, out);
     if (rc != RLH_OK) return rc;
     CtxLock lock(ctx);
@@ -67,7 +68,7 @@ extern "C" int rlh_tensor_upload(rlh_ctx *ctx, const void *host, int rows, int c
 
 extern "C" int rlh_tensor_download(rlh_tensor *t, void *host, int cols_capacity, rlh_event **ev) {
     if (!t || !host || cols_capacity < t->cols) return fail(RLH_ERR_INVALID, "rlh_tensor_download: bad argument");
-    if (t->dtype == RLH_Q4 && cols_capacity != t->cols) return fail(RLH_ERR_UNSUPPORTED, "rlh_tensor_download: a 4-bit tensor travels as its whole buffer (cols_capacity = cols)");
+    if (t->whole_buffer() && cols_capacity != t->cols) return fail(RLH_ERR_UNSUPPORTED, "rlh_tensor_download: a tensor of 4 or 8 bits travels as its whole buffer (cols_capacity = cols)");
     CtxLock lock(t->ctx);
     const size_t es = t->esize();
     if (t->cols == cols_capacity && !ev) { // (with an event the caller's memory is written after this call returns)
@@ -391,22 +392,26 @@ static std::vector<float2> rope_table(int head_dim, int first, int n) {
     return tab;
 }
 
-extern "C" int rlh_rope_table(rlh_tensor *freqs, double theta) {
-    if (!freqs || freqs->dtype != RLH_F32 || freqs->cols % 2 != 0) return fail(RLH_ERR_INVALID, "rlh_rope_table: an f32 tensor [positions x head_dim], head_dim even, is needed");
-    if (!(theta > 0.0) || std::isinf(theta)) return fail(RLH_ERR_INVALID, "rlh_rope_table: theta must be positive");
+static int fill_rope_table(const char *who, rlh_tensor *freqs, double theta, int from) {
+    if (!freqs || freqs->dtype != RLH_F32 || freqs->cols % 2 != 0) return fail(RLH_ERR_INVALID, "%s: an f32 tensor [positions x head_dim], head_dim even, is needed", who);
+    if (!(theta > 0.0) || std::isinf(theta)) return fail(RLH_ERR_INVALID, "%s: theta must be positive", who);
+    if (from < 0 || (int64_t)from + freqs->rows > (int64_t)INT32_MAX + 1) return fail(RLH_ERR_INVALID, "%s: %d positions from %d on", who, freqs->rows, from);
     CtxLock lock(freqs->ctx);
     constexpr size_t kChunk = (size_t)1 << 18; // pairs formed and sent at a time: 2 MiB, whatever the table's shape
     const size_t pairs = freqs->count() / 2, per_row = (size_t)freqs->cols / 2;
     const std::unique_ptr<float2[]> tab(new (std::nothrow) float2[std::min(kChunk, pairs)]);
-    if (!tab) return fail(RLH_ERR_OOM, "rlh_rope_table: out of host memory");
+    if (!tab) return fail(RLH_ERR_OOM, "%s: out of host memory", who);
     for (size_t first = 0; first < pairs; first += kChunk) {
         const size_t n = std::min(kChunk, pairs - first);
-        for (size_t i = 0; i < n; i++) tab[i] = rope_angle(freqs->cols, (int)((first + i) / per_row), (int)((first + i) % per_row), theta);
+        for (size_t i = 0; i < n; i++) tab[i] = rope_angle(freqs->cols, from + (int)((first + i) / per_row), (int)((first + i) % per_row), theta);
         HIP_TRY(hipMemcpyAsync((float2 *)freqs->p + first, tab.get(), n * sizeof(float2), hipMemcpyHostToDevice, freqs->ctx->stream));
         HIP_TRY(hipStreamSynchronize(freqs->ctx->stream)); // the next ones go into the same memory
     }
     return RLH_OK;
 }
+
+extern "C" int rlh_rope_table(rlh_tensor *freqs, double theta) { return fill_rope_table("rlh_rope_table", freqs, theta, 0); }
+extern "C" int rlh_rope_table_from(rlh_tensor *freqs, double theta, int first) { return fill_rope_table("rlh_rope_table_from", freqs, theta, first); }
 
 // Checks one layer's pair of cache planes [n_heads * max_seq_len x head_dim] and returns head_dim (0 on a mismatch).
 static int cache_planes_head_dim(const rlh_tensor *ck, const rlh_tensor *cv, int n_heads, int max_seq_len) {
@@ -532,6 +537,8 @@ hipError_t gemm_work_reserve(rlh_ctx *ctx, void **p, size_t *bytes, size_t need)
 void ops_release(rlh_ctx *ctx) {
     pool_release(ctx);
     OpScratch &o = ctx->ops;
+    for (AnswerWork *w : {&o.shared_work, &o.f8_work})
+        for (int i = 0; i < w->count; i++) (void)hipFree(w->kept[i]);
     void *all[] = {o.state, o.attn_ws, o.tickets, o.token, o.gemm_ws, o.window_ws};
     for (void *b : all)
         if (b) (void)hipFree(b);

@@ -81,17 +81,6 @@ __device__ __forceinline__ bool q4_finite(uint32_t pair) { return (int)((pair & 
 // 0.2 % of the weight: 7e-3 of the result).  So n weights lose n 2^-32 of the result at most to that.
 constexpr float kWeightLift = 7.0f;
 
-// One element
-template <typename T>
-__device__ __forceinline__ float plane_load1(const PlaneRef &p, size_t at) {
-    if constexpr (std::is_same_v<T, Quant4>) {
-        const uint32_t pair = p.pairs[at / 32], c = (reinterpret_cast<const uint8_t *>(p.data)[at / 2] >> (4 * (at & 1))) & 15u;
-        return fmaf((float)c, q4_scale(pair), q4_lowest(pair));
-    } else {
-        return (float)reinterpret_cast<const T *>(p.data)[at];
-    }
-}
-
 // A text that is cut: work memory, for every row first the pairs (m, sum) of its pieces and then the sums O of each, and how it is cut.
 struct AttnCutParams {
     AttnWindowParams a;

@@ -83,6 +83,17 @@ __device__ __forceinline__ void q4_decode8(uint32_t codes, uint32_t pair, float 
     for (int i = 0; i < 8; i++) v[i] = fmaf((float)((codes >> (4 * i)) & 15u), s, l);
 }
 
+// One element
+template <typename T>
+__device__ __forceinline__ float plane_load1(const PlaneRef &p, size_t at) {
+    if constexpr (std::is_same_v<T, Quant4>) {
+        const uint32_t pair = p.pairs[at / 32], c = (reinterpret_cast<const uint8_t *>(p.data)[at / 2] >> (4 * (at & 1))) & 15u;
+        return fmaf((float)c, q4_scale(pair), q4_lowest(pair));
+    } else {
+        return (float)reinterpret_cast<const T *>(p.data)[at];
+    }
+}
+
 // Eight consecutive elements, index a multiple of 8, of a plane or a tensor of type T as floats and back.  For 4 bits the four lanes of a group
 // store together.
 template <typename T>

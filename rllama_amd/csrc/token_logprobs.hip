@@ -1,0 +1,290 @@
+// token_logprobs.hip -- log probabilities of given tokens, the entropy of rows of logits and their most probable tokens.
+//
+// With z = (x - m) / T, m the row's largest, and s the sum of exp(z) over all entries but one that is the largest:
+//   log p(t) = z_t - log(1 + s),   entropy = log(1 + s) - (sum of z exp(z)) / (1 + s).
+// Leaving one largest entry out of the sum keeps what is small beside it: where a token is all but certain, its log probability and the entropy are as exact as
+// the others' weights are (a sum that holds the 1 loses everything below 2^-24 of it).
+//
+// One workgroup per row.  A row of up to 32768 entries is read once and stays in registers, 64 bytes (f16) or 128 of them per thread; a longer one is read
+// three times, the second and third time from the caches.
+//
+// The k most probable: the 64 groups of threads have a largest entry each, and the k-th largest of those bounds the k-th largest entry from below, since k groups hold an
+// entry that large.  What reaches the bound (about k ln(64 / (64 - k)) / (k / 64) of 32000 random entries) goes to a list in LDS, and an entry's place is the number
+// of those in front of it.  Lists that overflow: of rows with many entries equal to the bound (masks) those above it, and then the first equal ones in order of their ids;
+// where those above it are too many as well, one entry after the other.
+#include "kernels.h"
+#include "answers.h"
+
+namespace rlh {
+
+constexpr int kTlList = 256;
+constexpr int kTlGroups = 64;
+
+template <int kCtrl>
+__device__ __forceinline__ float dpp_max(float v) {
+    const int x = __builtin_bit_cast(int, v);
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(x, x, kCtrl, 0xf, 0xf, false)));
+}
+
+// Sixteen bytes of a row.  Rows of any length: only the element's own alignment.
+template <typename T>
+struct RowPiece {
+    static constexpr int kN = 16 / (int)sizeof(T);
+    typedef T any __attribute__((ext_vector_type(kN), aligned(sizeof(T))));
+    typedef T vec __attribute__((ext_vector_type(kN)));
+    vec v;
+    __device__ __forceinline__ void load(const T *x, int64_t i, int n) { // -infinity behind the row's end
+        if (i <= (int64_t)n - kN) {
+            v = *reinterpret_cast<const any *>(x + i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kN; j++) v[j] = i + j < n ? x[i + j] : (T)-INFINITY;
+        }
+    }
+    __device__ __forceinline__ float at(int j) const { return (float)v[j]; }
+};
+
+// larger values first, of equal ones the lower id; all keys differ
+__device__ __forceinline__ unsigned long long logit_key(float v, int id) {
+    const uint32_t w = __builtin_bit_cast(uint32_t, v + 0.0f); // (zeros of either kind are equal)
+    return ((unsigned long long)(w & 0x80000000u ? ~w : w | 0x80000000u) << 32) | (uint32_t)~(uint32_t)id;
+}
+__device__ __forceinline__ float key_logit(unsigned long long key) {
+    const uint32_t w = (uint32_t)(key >> 32);
+    return __builtin_bit_cast(float, w & 0x80000000u ? w & 0x7fffffffu : ~w);
+}
+
+// kKeep: pieces that a thread keeps; 0: rows of any length.  c2 = log2(e) / T.
+template <typename T, int kThreads, int kKeep>
+__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams p, float c2) {
+    typedef RowPiece<T> Piece;
+    constexpr int kN = Piece::kN, kStep = kThreads * kN, kWaves = kThreads / kWave, kLanes = kThreads / kTlGroups;
+    __shared__ float group_top[kTlGroups], sums[3][kWaves];
+    __shared__ float sh_bound;
+    __shared__ unsigned long long list[kTlList], sh_best;
+    __shared__ int sh_count, sh_ties[kWaves];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int row = blockIdx.x, vocab = p.vocab;
+    const T *x = reinterpret_cast<const T *>(p.logits) + (size_t)row * vocab;
+    Piece kept[kKeep > 0 ? kKeep : 1];
+    // f(piece, id of its first entry) over the thread's pieces
+    auto pieces = [&](auto f) __attribute__((always_inline)) {
+        if constexpr (kKeep > 0) {
+#pragma unroll
+            for (int k = 0; k < kKeep; k++) f(kept[k], (int64_t)(k * kStep + tid * kN));
+        } else {
+            for (int64_t i = (int64_t)tid * kN; i < vocab; i += kStep) {
+                Piece piece;
+                piece.load(x, i, vocab);
+                f(piece, i);
+            }
+        }
+    };
+    if constexpr (kKeep > 0) {
+#pragma unroll
+        for (int k = 0; k < kKeep; k++) kept[k].load(x, k * kStep + tid * kN, vocab);
+    }
+    // ---- the largest entry, of the thread, of its group and of the row
+    float mine = -INFINITY;
+    pieces([&](const Piece &piece, int64_t) {
+        typename Piece::vec t = piece.v;
+#pragma unroll
+        for (int n = kN / 2; n > 0; n /= 2)
+#pragma unroll
+            for (int j = 0; j < n; j++) t[j] = __builtin_elementwise_max(t[j], t[j + n]);
+        mine = fmaxf(mine, (float)t[0]);
+    });
+    {
+        float top = dpp_max<kDppQuadPerm2301>(dpp_max<kDppQuadPerm1032>(mine));
+        if constexpr (kLanes == 16) top = dpp_max<kDppRowMirror>(dpp_max<kDppRowHalfMirror>(top));
+        static_assert(kLanes == 16 || kLanes == 4, "1024 or 256 threads");
+        if (tid % kLanes == 0) group_top[tid / kLanes] = top;
+    }
+    if (tid == 0) sh_count = 0;
+    __syncthreads();
+    const float of_lane = group_top[lane], m = wave_max(of_lane), base = m > -INFINITY ? m : 0.0f;
+    if (p.top > 0 && wave == kWaves - 1) { // the k-th largest of the groups' entries
+        int above = 0;
+#pragma unroll 16
+        for (int g = 0; g < kTlGroups; g++) above += group_top[g] > of_lane;
+        const float bound = -wave_max(above < p.top ? -of_lane : -INFINITY);
+        if (lane == 0) sh_bound = bound;
+    }
+    // ---- the sums.  f16: z = x c2 - m c2 in one operation; m c2 was rounded, which shifts all z by the same `shift`.  f32: the difference first, since m c2 may not be
+    // representable.  (A bound keeps 0 * infinity out of the second sum.)
+    const float mc = sizeof(T) == 2 ? base * c2 : 0.0f, shift = sizeof(T) == 2 ? fmaf(base, c2, -mc) : 0.0f;
+    auto exponent = [&](float v) { return sizeof(T) == 2 ? fmaf(v, c2, -mc) : (v - base) * c2; };
+    float s = 0.0f, u = 0.0f, count = 0.0f;
+    if (mine < m || !(m > -INFINITY)) {
+        pieces([&](const Piece &piece, int64_t) {
+#pragma unroll
+            for (int j = 0; j < kN; j++) {
+                const float z = exponent(piece.at(j)), e = __builtin_amdgcn_exp2f(z);
+                s += e;
+                u = fmaf(e, fmaxf(z, -300.0f), u);
+            }
+        });
+    } else { // the thread holds a largest entry: one is left out
+        count = 1.0f;
+        pieces([&](const Piece &piece, int64_t) {
+#pragma unroll
+            for (int j = 0; j < kN; j++) {
+                const bool out = count > 0.0f && piece.at(j) == m;
+                const float z = exponent(piece.at(j)), e = out ? 0.0f : __builtin_amdgcn_exp2f(z);
+                if (out) count = 0.0f;
+                s += e;
+                u = fmaf(e, fmaxf(z, -300.0f), u);
+            }
+        });
+        count = 1.0f;
+    }
+    s = wave_sum(s);
+    u = wave_sum(u);
+    count = wave_sum(count);
+    if (lane == 0) {
+        sums[0][wave] = s;
+        sums[1][wave] = u;
+        sums[2][wave] = count;
+    }
+    __syncthreads();
+    s = u = count = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        s += sums[0][w];
+        u += sums[1][w];
+        count += sums[2][w];
+    }
+    const bool none = !(m > -INFINITY), odd = !(s < INFINITY) || m == INFINITY; // (a NaN is in the sum)
+    constexpr float kLn2 = 0.69314718055994530942f;
+    const float e_top = __builtin_amdgcn_exp2f(shift);
+    const float others = fmaf(fmaxf(count - 1.0f, 0.0f), e_top, s) / e_top; // (a thread each left out one of several that are the largest)
+    const float log_s = log1pf(others), u_top = (u - shift * s) / e_top;
+    auto logprob = [&](float v) { return odd ? NAN : none ? -INFINITY : fmaf(exponent(v) - shift, kLn2, -log_s); };
+    if (tid == 0 && p.entropy) p.entropy[row] = odd ? NAN : none ? 0.0f : log_s - kLn2 * u_top / (1.0f + others);
+    for (int i = tid; i < p.n_tokens; i += kThreads) {
+        const int id = p.tokens[(size_t)row * p.n_tokens + i];
+        p.logprobs[(size_t)row * p.n_tokens + i] = id < 0 ? 0.0f : id < vocab ? logprob((float)x[id]) : odd ? NAN : -INFINITY;
+    }
+    if (p.top == 0) return;
+    int32_t *ids = p.top_ids + (size_t)row * p.top;
+    float *logprobs = p.top_logprobs + (size_t)row * p.top;
+    if (odd) {
+        if (tid < p.top) {
+            ids[tid] = -1;
+            logprobs[tid] = NAN;
+        }
+        return;
+    }
+    // ---- the most probable
+    const float bound = sh_bound;
+    auto collect = [&](bool equal_ones) __attribute__((always_inline)) {
+        if (!(mine >= bound)) return;
+        pieces([&](const Piece &piece, int64_t i) {
+#pragma unroll
+            for (int j = 0; j < kN; j++) {
+                const float v = piece.at(j);
+                if ((equal_ones ? v >= bound : v > bound) && i + j < vocab) {
+                    const int at = atomicAdd(&sh_count, 1);
+                    if (at < kTlList) list[at] = logit_key(v, (int)(i + j));
+                }
+            }
+        });
+    };
+    collect(true);
+    __syncthreads();
+    int found = sh_count, wanted = p.top; // of the list
+    if (found > kTlList) {
+        __syncthreads();
+        if (tid == 0) sh_count = 0;
+        __syncthreads();
+        collect(false);
+        __syncthreads();
+        found = sh_count;
+        if (found > kTlList) { // one after the other
+            unsigned long long below = ~0ull;
+            for (int k = 0; k < p.top; k++) {
+                if (tid == 0) sh_best = 0;
+                __syncthreads();
+                unsigned long long best = 0;
+                pieces([&](const Piece &piece, int64_t i) {
+#pragma unroll
+                    for (int j = 0; j < kN; j++) {
+                        const unsigned long long key = logit_key(piece.at(j), (int)(i + j));
+                        if (key < below && key > best && i + j < vocab) best = key;
+                    }
+                });
+                if (best) atomicMax(&sh_best, best);
+                __syncthreads();
+                below = sh_best;
+                __syncthreads();
+                if (tid == 0) {
+                    ids[k] = (int)~(uint32_t)below;
+                    logprobs[k] = logprob(key_logit(below));
+                }
+            }
+            return;
+        }
+        wanted = min(p.top, found);
+        // the first ids of entries that equal the bound, a stretch of the row at a time
+        const float at_bound = logprob(bound);
+        int place = found;
+        for (int64_t from = 0; place < p.top && from < vocab; from += kStep) {
+            Piece piece;
+            piece.load(x, from + (int64_t)tid * kN, vocab);
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < kN; j++) n += piece.at(j) == bound && from + tid * kN + j < vocab;
+            int before = n; // of the wavefront's lanes up to this one
+#pragma unroll
+            for (int off = 1; off < kWave; off <<= 1) {
+                const int up = __shfl_up(before, off, kWave);
+                if (lane >= off) before += up;
+            }
+            if (lane == kWave - 1) sh_ties[wave] = before;
+            __syncthreads();
+            int at = place + before - n;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                if (w < wave) at += sh_ties[w];
+                place += sh_ties[w];
+            }
+            if (n > 0) {
+#pragma unroll
+                for (int j = 0; j < kN; j++)
+                    if (piece.at(j) == bound && from + tid * kN + j < vocab && at < p.top) {
+                        ids[at] = (int)(from + tid * kN + j);
+                        logprobs[at++] = at_bound;
+                    }
+            }
+            __syncthreads();
+        }
+    }
+    for (int i = tid; i < found; i += kThreads) {
+        const unsigned long long key = list[i];
+        int at = 0;
+        for (int j = 0; j < found; j++) at += list[j] > key;
+        if (at < wanted) {
+            ids[at] = (int)~(uint32_t)key;
+            logprobs[at] = logprob(key_logit(key));
+        }
+    }
+}
+
+template <typename T>
+static void launch_t(const LogprobsParams &p, hipStream_t s) {
+    constexpr int kN = RowPiece<T>::kN;
+    const float c2 = (float)(1.44269504088896340736 / (double)p.temperature);
+    const dim3 grid((unsigned)p.rows);
+    if (p.vocab <= 2048) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 8 / kN>), grid, dim3(256), 0, s, p, c2);
+    else if (p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 8 / kN>), grid, dim3(1024), 0, s, p, c2);
+    else if (p.vocab <= 32768) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 32 / kN>), grid, dim3(1024), 0, s, p, c2);
+    else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0>), grid, dim3(1024), 0, s, p, c2);
+}
+
+hipError_t launch_token_logprobs(const LogprobsParams &p, hipStream_t s) {
+    if (p.f16) launch_t<half_t>(p, s);
+    else launch_t<float>(p, s);
+    return hipGetLastError();
+}
+
+} // namespace rlh

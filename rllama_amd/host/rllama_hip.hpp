@@ -34,7 +34,7 @@ inline void check(int rc) {
     if (rc != RLH_OK) throw Error(rc, rlh_last_error());
 }
 
-enum class TensorDType { Float16 = RLH_F16, Float32 = RLH_F32, K4BitQuantization = RLH_Q4, Int32 = RLH_I32 }; // src/tensor.rs:50-54
+enum class TensorDType { Float16 = RLH_F16, Float32 = RLH_F32, K4BitQuantization = RLH_Q4, Int32 = RLH_I32, Float8 = RLH_F8, Float8Tiles = RLH_F8_TILES }; // src/tensor.rs:50-54
 
 // OpenCL::new(verbose, nth_device) (src/tensor_opencl_support.rs:86)
 class OpenCL {
@@ -300,6 +300,30 @@ class Tensor {
         return out;
     }
 
+    // ---- many answers to one prompt (no reference counterpart)
+    // the angles of positions first, first + 1, ...
+    static Tensor rope_table_from(const std::shared_ptr<OpenCL> &cl, int first, int64_t positions, int64_t head_dim, double theta = 10000.0) {
+        Tensor out = zeros(cl, positions, head_dim, TensorDType::Float32);
+        check(rlh_rope_table_from(out.h_, theta, first));
+        return out;
+    }
+    // this = q after qkv_append: rows of texts that continue one prefix; start_pos counts from the prefix's end
+    Tensor attn_shared(const Tensor &prefix_k, const Tensor &prefix_v, int prefix_len, const Tensor &cache_k, const Tensor &cache_v, int n_heads, int n_kv_heads, int max_seq_len,
+                       const std::vector<int32_t> &start_pos) const {
+        Tensor out = zeros(cl_, rows_, cols_, dtype_);
+        check(rlh_attn_shared(out.h_, h_, prefix_k.h_, prefix_v.h_, prefix_len, cache_k.h_, cache_v.h_, n_heads, n_kv_heads, max_seq_len, start_pos.data(), (int)start_pos.size()));
+        return out;
+    }
+    // this = logits: log probabilities of tokens i32 [rows x m], the entropy of each row, and its `top` most probable ids (top > 0)
+    struct Logprobs;
+    Logprobs token_logprobs(const Tensor &tokens, int top, float temperature = 1.0f) const;
+    // this [n x k], f16, f32 or Float8, times weights[m x k]^T in Float8Tiles
+    Tensor matrix_mul_f8(const Tensor &weights, TensorDType result = TensorDType::Float16) const {
+        Tensor out = zeros(cl_, rows_, weights.rows_, result);
+        check(rlh_matrix_mul_f8(out.h_, h_, weights.h_));
+        return out;
+    }
+
   private:
     Tensor(std::shared_ptr<OpenCL> cl, rlh_tensor *h, int64_t r, int64_t c, TensorDType d) : cl_(std::move(cl)), h_(h), rows_(r), cols_(c), dtype_(d) {}
     std::shared_ptr<OpenCL> cl_;
@@ -307,5 +331,15 @@ class Tensor {
     int64_t rows_ = 0, cols_ = 0;
     TensorDType dtype_ = TensorDType::Float16;
 };
+
+struct Tensor::Logprobs {
+    Tensor logprobs, entropy, top_ids, top_logprobs;
+};
+inline Tensor::Logprobs Tensor::token_logprobs(const Tensor &tokens, int top, float temperature) const {
+    Logprobs r{zeros(cl_, rows_, tokens.cols_, TensorDType::Float32), zeros(cl_, rows_, 1, TensorDType::Float32), zeros(cl_, rows_, top, TensorDType::Int32),
+               zeros(cl_, rows_, top, TensorDType::Float32)};
+    check(rlh_token_logprobs(r.logprobs.h_, r.entropy.h_, r.top_ids.h_, r.top_logprobs.h_, h_, tokens.h_, temperature));
+    return r;
+}
 
 } // namespace rllama

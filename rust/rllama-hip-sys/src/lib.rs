@@ -43,6 +43,8 @@ pub const RLH_F16: c_int = 0;
 pub const RLH_F32: c_int = 1;
 pub const RLH_Q4: c_int = 2;
 pub const RLH_I32: c_int = 3;
+pub const RLH_F8: c_int = 5;
+pub const RLH_F8_TILES: c_int = 6;
 
 // rlh_tensor_kind
 pub const RLH_TOK_EMB: c_int = 0;
@@ -145,6 +147,10 @@ extern "C" {
     pub fn rlh_attn_window(out: *mut rlh_tensor, q: *const rlh_tensor, cache_k: *const rlh_tensor, cache_v: *const rlh_tensor, n_heads: c_int, n_kv_heads: c_int, max_seq_len: c_int, start_pos: *const i32, n_seqs: c_int, window: c_int, sinks: c_int) -> c_int;
     pub fn rlh_softmax_rows(probs: *mut rlh_tensor, logits: *const rlh_tensor, temperature: c_float) -> c_int;
     pub fn rlh_verify_draft(out: *mut rlh_tensor, target: *const rlh_tensor, draft: *const rlh_tensor, drafted: *const rlh_tensor, uniforms: *const rlh_tensor) -> c_int;
+    pub fn rlh_rope_table_from(freqs: *mut rlh_tensor, theta: c_double, first: c_int) -> c_int;
+    pub fn rlh_attn_shared(out: *mut rlh_tensor, q: *const rlh_tensor, prefix_k: *const rlh_tensor, prefix_v: *const rlh_tensor, prefix_len: c_int, cache_k: *const rlh_tensor, cache_v: *const rlh_tensor, n_heads: c_int, n_kv_heads: c_int, max_seq_len: c_int, start_pos: *const i32, n_seqs: c_int) -> c_int;
+    pub fn rlh_token_logprobs(logprobs: *mut rlh_tensor, entropy: *mut rlh_tensor, top_ids: *mut rlh_tensor, top_logprobs: *mut rlh_tensor, logits: *const rlh_tensor, tokens: *const rlh_tensor, temperature: c_float) -> c_int;
+    pub fn rlh_matrix_mul_f8(dst: *mut rlh_tensor, src: *const rlh_tensor, weights: *const rlh_tensor) -> c_int;
     pub fn rlh_model_time_kernel(model: *mut rlh_model, caches: *mut rlh_caches, which: c_int, T: c_int, iters: c_int, us_per_launch: *mut c_float, bytes_per_launch: *mut u64) -> c_int;
     pub fn rlh_time_gemv(ctx: *mut rlh_ctx, rows: c_int, k: c_int, w_dtype: c_int, round_x: c_int, round_y: c_int, n_buffers: c_int, iters: c_int, us_per_launch: *mut c_float) -> c_int;
     pub fn rlh_probe_gemv_phases(ctx: *mut rlh_ctx, rows: c_int, k: c_int, n_buffers: c_int, launches: c_int, out_us: *mut c_float) -> c_int;

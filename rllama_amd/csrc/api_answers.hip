@@ -127,6 +127,7 @@ extern "C" int rlh_matrix_mul_f8(rlh_tensor *dst, const rlh_tensor *src, const r
     if (weights->dtype != RLH_F8_TILES) return fail(RLH_ERR_INVALID, "%s: weights must be 8 bits with a scale for each tile", who);
     if (!src->is_float() && src->dtype != RLH_F8) return fail(RLH_ERR_INVALID, "%s: src must be f16, f32 or 8 bits with a scale for each row's blocks", who);
     if (!dst->is_float() || src->cols != weights->cols || !shaped(dst, src->rows, weights->rows)) return fail(RLH_ERR_INVALID, "%s: src [n x k], weights [m x k] and dst [n x m], f16 or f32, are needed", who);
+    if (src->cols > (1 << 24)) return fail(RLH_ERR_UNSUPPORTED, "%s: rows of %d (%d at most)", who, src->cols, 1 << 24);
     if (dst->p == src->p || dst->p == weights->p) return fail(RLH_ERR_INVALID, "%s: dst must not share memory with the operands", who);
     rlh_ctx *ctx = dst->ctx;
     CtxLock lock(ctx);
@@ -137,17 +138,21 @@ extern "C" int rlh_matrix_mul_f8(rlh_tensor *dst, const rlh_tensor *src, const r
     p.y = dst->p;
     p.y_f16 = dst->dtype == RLH_F16;
     p.w = eight_of(weights);
+    const int cus = ctx->prop.multiProcessorCount;
+    // work memory: the sums of pieces of K, and src in 8 bits where the product does not convert it on the way
+    const bool on_the_way = src->dtype != RLH_F8 && matmul_f8_converts(p.m), before = src->dtype != RLH_F8 && !on_the_way;
+    const size_t sums = (matmul_f8_work_floats(p, cus) * sizeof(float) + 15) / 16 * 16, codes = src->count();
+    const int rc = work_reserve(who, ctx, ctx->ops.f8_work, sums + (before ? codes + (size_t)p.m * f8_blocks(p.k) * sizeof(float) : 0));
+    if (rc != RLH_OK) return rc;
+    char *work = static_cast<char *>(ctx->ops.f8_work.memory());
     if (src->dtype == RLH_F8) {
         p.x = eight_of(src);
-    } else {
-        const size_t codes = src->count();
-        const int rc = work_reserve(who, ctx, ctx->ops.f8_work, codes + (size_t)p.m * f8_blocks(p.k) * sizeof(float));
-        if (rc != RLH_OK) return rc;
-        uint8_t *at = static_cast<uint8_t *>(ctx->ops.f8_work.memory());
+    } else if (before) {
+        uint8_t *at = reinterpret_cast<uint8_t *>(work + sums);
         p.x = {at, reinterpret_cast<float *>(at + codes), 1};
     }
     lend(ctx, {src, weights});
-    if (src->dtype != RLH_F8) HIP_TRY(launch_f8_encode(p.x, src->p, src->dtype == RLH_F16, p.m, p.k, ctx->stream));
-    HIP_TRY(launch_matmul_f8(p, ctx->prop.multiProcessorCount, ctx->stream));
+    if (before) HIP_TRY(launch_f8_encode(p.x, src->p, src->dtype == RLH_F16, p.m, p.k, ctx->stream));
+    HIP_TRY(launch_matmul_f8(p, on_the_way ? src->p : nullptr, src->dtype == RLH_F16, cus, reinterpret_cast<float *>(work), ctx->stream));
     return RLH_OK;
 }

@@ -1,40 +1,434 @@
 // gemm_f8.hip -- products of 8-bit floating point with a scale for each block of 128:
 //   y[r, c] = sum_b sx[r, b] sw[c / 128, b] sum_{k in block b} x[r, k] w[c, k].
+//
+// A block's sum is formed by the matrix cores and added to y in f32 with both scales: weights are the first operand, so a lane holds four neighbouring columns of
+// one row, whose scale is the lane's own; the columns' scale is the same for a whole tile.
+//
+// Which matrix instruction.  v_mfma_f32_16x16x128_f8f6f4 takes 128 products at once, but adds them up eight at a time with the products aligned to the largest one's power
+// of two and cut off 2^-13 below it (measured; random operands: 1.5e-5 of the result, whatever the number of blocks), where f32 sums keep 1e-7.  f16 results are
+// rounded by 2.1e-4 of their size anyway.  So it is taken for f16 results of many rows, which the matrix cores bound.  Few rows are bound by memory, and f32 results
+// are to be as exact as f32 is: there the codes become f16 numbers (exactly: one conversion per pair) for v_mfma_f32_16x16x32_f16.
 #include "kernels.h"
 #include "answers.h"
 
+#include <algorithm>
+
 namespace rlh {
 
-// One thread per result.
-template <typename T>
-__global__ __launch_bounds__(256) void matmul_f8_kernel(MatmulF8Params p) {
-    const int c = blockIdx.x * 16 + threadIdx.x % 16;
-    const int64_t r = (int64_t)blockIdx.y * 16 + threadIdx.x / 16;
-    if (r >= p.m || c >= p.n) return;
-    const int across = f8_blocks(p.k);
-    float y = 0.0f;
-    for (int b = 0; b < across; b++) {
-        float part = 0.0f;
-        for (int k = b * kF8Block; k < min(p.k, (b + 1) * kF8Block); k += 16) {
-            const uint4_t x = *reinterpret_cast<const uint4_t *>(p.x.codes + (size_t)r * p.k + k), w = *reinterpret_cast<const uint4_t *>(p.w.codes + (size_t)c * p.k + k);
-            for (int i = 0; i < 4; i++) {
-                const half2_t x0 = f8_pair_f16<false>(x[i]), x1 = f8_pair_f16<true>(x[i]), w0 = f8_pair_f16<false>(w[i]), w1 = f8_pair_f16<true>(w[i]);
-                part = fmaf((float)x0[0], (float)w0[0], part);
-                part = fmaf((float)x0[1], (float)w0[1], part);
-                part = fmaf((float)x1[0], (float)w1[0], part);
-                part = fmaf((float)x1[1], (float)w1[1], part);
-            }
-        }
-        y = fmaf(part, p.x.scales[(size_t)r * across + b] * p.w.scales[(size_t)(c / kF8Block) * across + b], y);
-    }
-    reinterpret_cast<T *>(p.y)[(size_t)r * p.n + c] = (T)y;
+typedef __attribute__((ext_vector_type(8))) int int8_t_;
+typedef __amdgpu_buffer_rsrc_t buffer_t;
+
+__device__ __forceinline__ buffer_t f8_buffer(const void *data, size_t offset, size_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(reinterpret_cast<const char *>(data)) + offset, 0, (int)bytes, 0x00027000);
+}
+constexpr int kF8Outside = 0x7ffffff0; // an offset past every buffer: reads as zeros
+
+// sixteen codes as two operands of the f16 instruction
+__device__ __forceinline__ half8_t f8_half8(uint32_t a, uint32_t b) {
+    const half2_t x0 = f8_pair_f16<false>(a), x1 = f8_pair_f16<true>(a), x2 = f8_pair_f16<false>(b), x3 = f8_pair_f16<true>(b);
+    return half8_t{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
 }
 
-hipError_t launch_matmul_f8(const MatmulF8Params &p, int compute_units, hipStream_t s) {
-    const dim3 grid((unsigned)((p.n + 15) / 16), (unsigned)((p.m + 15) / 16));
-    if (p.y_f16) hipLaunchKernelGGL(matmul_f8_kernel<half_t>, grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL(matmul_f8_kernel<float>, grid, dim3(256), 0, s, p);
+template <typename Y>
+__device__ __forceinline__ void store_row4(Y *y, int n, int left, const float4_t &v, bool aligned) { // columns n .. n + 3, of which `left` are inside
+    if (aligned && left >= 4) {
+        if constexpr (sizeof(Y) == 2) {
+            typedef __attribute__((ext_vector_type(4))) _Float16 half4_t;
+            *reinterpret_cast<half4_t *>(y + n) = half4_t{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
+        } else {
+            *reinterpret_cast<float4_t *>(y + n) = v;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < left) y[n + i] = (Y)v[i];
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------------------------------------
+// A workgroup owns all rows (16 kMF of them at most) and 16 kNF columns; its wavefronts share the blocks of K, each reading its operands from memory into registers and
+// nowhere else, and add their sums up through LDS in their own order.
+enum F8Source { kF8Codes = 0, kF8FromF16 = 1, kF8FromF32 = 2 };
+struct RowsF8Params {
+    MatmulF8Params p;
+    const void *src; // f16 or f32 rows, converted on the way
+};
+constexpr int kRfWaves = 8;
+
+template <int kMF, int kNF, int kSource, typename Y>
+__global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8Params pp) {
+    const MatmulF8Params &p = pp.p;
+    constexpr int kScales = kF8Block % (16 * kNF) == 0 ? 1 : kNF; // of the workgroup's columns
+    constexpr int kXWords = kSource == kF8Codes ? 8 : kSource == kF8FromF16 ? 16 : 32;
+    __shared__ __attribute__((aligned(16))) float4_t red[kRfWaves][kMF * kNF][kWave];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int c = lane & 15, h = lane >> 4;
+    const int n0 = blockIdx.x * 16 * kNF, across = f8_blocks(p.k);
+    const int rows_w = min(p.n - n0, 16 * kNF);
+    constexpr int kXBytes = kSource == kF8Codes ? 1 : kSource == kF8FromF16 ? 2 : 4;
+    const buffer_t wb = f8_buffer(p.w.codes, (size_t)n0 * p.k, (size_t)rows_w * p.k);
+    const buffer_t xb = f8_buffer(kSource == kF8Codes ? (const void *)p.x.codes : pp.src, 0, (size_t)p.m * p.k * kXBytes);
+    const buffer_t sb = f8_buffer(p.x.scales, 0, (size_t)p.m * across * 4);
+    int w_at[kNF], x_at[kMF], s_at[kMF];
+#pragma unroll
+    for (int j = 0; j < kNF; j++) w_at[j] = min(j * 16 + c, rows_w - 1) * p.k + h * 32;
+#pragma unroll
+    for (int i = 0; i < kMF; i++) {
+        const int r = min(i * 16 + c, p.m - 1);
+        x_at[i] = (r * p.k + h * 32) * kXBytes;
+        s_at[i] = r * across * 4;
+    }
+    struct Block {
+        uint32_t w[kNF][8], x[kMF][kXWords];
+        float sx[kMF], sw[kScales];
+    };
+    auto load = [&](Block &k, int b) __attribute__((always_inline)) {
+        const int k0 = b * kF8Block;
+        const bool in0 = k0 + h * 32 < p.k, in1 = k0 + h * 32 + 16 < p.k;
+        auto take = [](uint32_t *to, buffer_t from, int at) {
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) to[i] = v[i];
+        };
+#pragma unroll
+        for (int j = 0; j < kNF; j++) {
+            take(k.w[j], wb, in0 ? w_at[j] + k0 : kF8Outside);
+            take(k.w[j] + 4, wb, in1 ? w_at[j] + k0 + 16 : kF8Outside);
+        }
+#pragma unroll
+        for (int i = 0; i < kMF; i++) {
+#pragma unroll
+            for (int q = 0; q < kXWords / 4; q++) take(k.x[i] + 4 * q, xb, (q < kXWords / 8 ? in0 : in1) ? x_at[i] + k0 * kXBytes + 16 * q : kF8Outside);
+            if constexpr (kSource == kF8Codes) k.sx[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sb, s_at[i] + b * 4, 0, 0));
+        }
+#pragma unroll
+        for (int t = 0; t < kScales; t++) k.sw[t] = p.w.scales[(size_t)(min(n0 + t * 16, p.n - 1) / kF8Block) * across + b];
+    };
+    float4_t acc[kMF][kNF];
+#pragma unroll
+    for (int i = 0; i < kMF; i++)
+#pragma unroll
+        for (int j = 0; j < kNF; j++) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    auto use = [&](Block &k) __attribute__((always_inline)) {
+        half8_t xs[kMF][4];
+#pragma unroll
+        for (int i = 0; i < kMF; i++) {
+            if constexpr (kSource == kF8Codes) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) xs[i][q] = f8_half8(k.x[i][2 * q], k.x[i][2 * q + 1]);
+            } else { // the block's largest value is that of the four lanes of a row; codes as rlh_convert forms them
+                float v[32], top = 0.0f, odd = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    v[e] = kSource == kF8FromF16 ? (float)__builtin_bit_cast(half2_t, k.x[i][e / 2 % kXWords])[e % 2] : __builtin_bit_cast(float, k.x[i][e % kXWords]);
+                    top = fmaxf(top, fabsf(v[e]));
+                    odd = fmaf(v[e], 0.0f, odd);
+                }
+#pragma unroll
+                for (int off = 16; off < 64; off <<= 1) {
+                    top = fmaxf(top, __shfl_xor(top, off, kWave));
+                    odd += __shfl_xor(odd, off, kWave);
+                }
+                const F8Scale by(top);
+                k.sx[i] = odd == 0.0f ? by.scale : NAN;
+                uint32_t codes[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    int x = f8_codes<false>(v[4 * e] * by.factor, v[4 * e + 1] * by.factor, 0);
+                    codes[e] = (uint32_t)f8_codes<true>(v[4 * e + 2] * by.factor, v[4 * e + 3] * by.factor, x);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; q++) xs[i][q] = f8_half8(codes[2 * q], codes[2 * q + 1]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kNF; j++) {
+            float4_t part[kMF];
+#pragma unroll
+            for (int i = 0; i < kMF; i++) part[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const half8_t w = f8_half8(k.w[j][2 * q], k.w[j][2 * q + 1]);
+#pragma unroll
+                for (int i = 0; i < kMF; i++) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, xs[i][q], part[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kMF; i++) {
+                const float by = k.sx[i] * k.sw[kScales > 1 ? j : 0];
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(part[i][e], by, acc[i][j][e]);
+            }
+        }
+    };
+    // Workgroups in step would ask for the same columns of all rows, which meet in few memory channels: each starts at another block.
+    const int rot = (int)(blockIdx.x * 5u % (unsigned)across);
+    auto block_of = [&](int t) {
+        const int b = t + rot;
+        return b < across ? b : b - across;
+    };
+    Block now, next;
+    if (wave < across) load(now, block_of(wave));
+    for (int t = wave; t < across; t += kRfWaves) {
+        if (t + kRfWaves < across) load(next, block_of(t + kRfWaves));
+        use(now);
+        now = next;
+    }
+#pragma unroll
+    for (int i = 0; i < kMF; i++)
+#pragma unroll
+        for (int j = 0; j < kNF; j++) red[wave][i * kNF + j][lane] = acc[i][j];
+    __syncthreads();
+    Y *y = reinterpret_cast<Y *>(p.y);
+    const bool aligned = p.n % 4 == 0;
+    for (int s = tid; s < kMF * kNF * kWave; s += kRfWaves * kWave) {
+        const int f = s / kWave, l = s % kWave, r = f / kNF * 16 + (l & 15), n = n0 + f % kNF * 16 + (l >> 4) * 4;
+        float4_t v = red[0][f][l];
+#pragma unroll
+        for (int w = 1; w < kRfWaves; w++) v += red[w][f][l];
+        if (r < p.m && n < p.n) store_row4(y + (size_t)r * p.n, n, p.n - n, v, aligned);
+    }
+}
+
+// ---- many rows -------------------------------------------------------------------------------------------------------------------------
+// A workgroup owns 16 kMT kWM rows and 16 kNT kWN columns; blocks of K pass by in LDS, two stages of 128 bytes of every row, the next one on its way while this one is
+// used.  Sixteen-byte pieces of a row are permuted by (row / 2) % 8: sixteen rows' pieces of one column lie in different banks, and every lane of a load names its own
+// address anyway.
+__device__ const uint4_t f8_zeros = {0u, 0u, 0u, 0u};
+
+struct TilesF8Params {
+    MatmulF8Params p;
+    float *parts;  // [pieces x m x n] sums of ranges of blocks, or null: y itself
+    int pieces;
+    int tiles_m, tiles_n;
+};
+
+template <int kWM, int kWN, int kMT, int kNT, bool kExact, typename Y>
+__global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(TilesF8Params pp) {
+    const MatmulF8Params &p = pp.p;
+    constexpr int kWaves = kWM * kWN, kBM = 16 * kMT * kWM, kBN = 16 * kNT * kWN;
+    constexpr int kStageBytes = (kBM + kBN) * kF8Block;
+    constexpr int kLoads = kStageBytes / 1024, kPerWave = (kLoads + kWaves - 1) / kWaves;
+    static_assert(128 % (16 * kNT) == 0, "a wavefront's columns share their scale");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kStageBytes];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int c = lane & 15, h = lane >> 4, wm = wave / kWN, wn = wave % kWN;
+    const int across = f8_blocks(p.k);
+    const int piece = blockIdx.y, b0 = (int)((int64_t)across * piece / pp.pieces), b1 = (int)((int64_t)across * (piece + 1) / pp.pieces);
+    const int tm = blockIdx.x % pp.tiles_m, tn = blockIdx.x / pp.tiles_m;
+    const int m0 = tm * kBM, n0 = tn * kBN;
+    const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
+
+    // staging: rows of x, then of w; a wavefront-wide load covers 8 rows
+    const uint8_t *from[kPerWave];
+    int piece_at[kPerWave]; // of the lane's sixteen bytes in a block
+#pragma unroll
+    for (int i = 0; i < kPerWave; i++) {
+        const int r = (i * kWaves + wave) * 8 + lane / 8; // row of the stage
+        const bool is_x = r < kBM;
+        const int row = is_x ? min(m0 + r, p.m - 1) : min(n0 + r - kBM, p.n - 1);
+        piece_at[i] = ((lane % 8) ^ ((r >> 1) & 7)) * 16;
+        from[i] = (is_x ? p.x.codes : p.w.codes) + (size_t)row * p.k + piece_at[i];
+    }
+    auto fetch = [&](int b, unsigned stage) __attribute__((always_inline)) {
+        const bool whole = (b + 1) * kF8Block <= p.k;
+#pragma unroll
+        for (int i = 0; i < kPerWave; i++) {
+            if (kLoads % kWaves != 0 && i * kWaves + wave >= kLoads) continue;
+            const uint8_t *at = from[i] + (size_t)b * kF8Block;
+            if (!whole && b * kF8Block + piece_at[i] >= p.k) at = reinterpret_cast<const uint8_t *>(&f8_zeros); // behind the last column
+            dma16(reinterpret_cast<const half_t *>(at), lds_base + stage * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
+        }
+    };
+    const float *sx[kMT];
+#pragma unroll
+    for (int i = 0; i < kMT; i++) sx[i] = p.x.scales + (size_t)min(m0 + (wm * kMT + i) * 16 + c, p.m - 1) * across;
+    const int nw = n0 + wn * kNT * 16; // the wavefront's first column
+    const float *sw = p.w.scales + (size_t)(min(nw, p.n - 1) / kF8Block) * across;
+
+    float4_t acc[kMT][kNT];
+#pragma unroll
+    for (int i = 0; i < kMT; i++)
+#pragma unroll
+        for (int j = 0; j < kNT; j++) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    auto frag = [&](unsigned stage, int row, uint32_t (&to)[8]) __attribute__((always_inline)) {
+        const unsigned char *at = lds + stage * kStageBytes + row * kF8Block;
+        const int swz = (row >> 1) & 7;
+        const uint4_t a = *reinterpret_cast<const uint4_t *>(at + (((2 * h) ^ swz) << 4)), b = *reinterpret_cast<const uint4_t *>(at + (((2 * h + 1) ^ swz) << 4));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            to[i] = a[i];
+            to[4 + i] = b[i];
+        }
+    };
+    float scale[kMT], ahead[kMT];
+    if (b0 < b1) {
+#pragma unroll
+        for (int i = 0; i < kMT; i++) ahead[i] = sx[i][b0] * sw[b0];
+        fetch(b0, 0);
+    }
+    unsigned stage = 0;
+    for (int b = b0; b < b1; b++) {
+        wait_vmcnt<0>();  // this wavefront's part of the block has landed
+        __syncthreads();  // ... and everybody's; everybody is done with the block before, whose stage is filled next
+#pragma unroll
+        for (int i = 0; i < kMT; i++) scale[i] = ahead[i];
+        if (b + 1 < b1) {
+#pragma unroll
+            for (int i = 0; i < kMT; i++) ahead[i] = sx[i][b + 1] * sw[b + 1];
+            fetch(b + 1, 1 - stage);
+        }
+        uint32_t x[kMT][8];
+#pragma unroll
+        for (int i = 0; i < kMT; i++) frag(stage, (wm * kMT + i) * 16 + c, x[i]);
+        if constexpr (kExact) {
+            half8_t xs[kMT][4];
+#pragma unroll
+            for (int i = 0; i < kMT; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) xs[i][q] = f8_half8(x[i][2 * q], x[i][2 * q + 1]);
+#pragma unroll
+            for (int j = 0; j < kNT; j++) {
+                uint32_t w[8];
+                frag(stage, kBM + (wn * kNT + j) * 16 + c, w);
+                float4_t part[kMT];
+#pragma unroll
+                for (int i = 0; i < kMT; i++) part[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const half8_t ws = f8_half8(w[2 * q], w[2 * q + 1]);
+#pragma unroll
+                    for (int i = 0; i < kMT; i++) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ws, xs[i][q], part[i], 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < kMT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(part[i][e], scale[i], acc[i][j][e]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kNT; j++) {
+                uint32_t w[8];
+                frag(stage, kBM + (wn * kNT + j) * 16 + c, w);
+                const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                float4_t part[kMT];
+#pragma unroll
+                for (int i = 0; i < kMT; i++)
+                    part[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(int8_t_, w), __builtin_bit_cast(int8_t_, x[i]), zero, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < kMT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(part[i][e], scale[i], acc[i][j][e]);
+            }
+        }
+        stage = 1 - stage;
+    }
+    const bool aligned = p.n % 4 == 0;
+#pragma unroll
+    for (int i = 0; i < kMT; i++) {
+        const int r = m0 + (wm * kMT + i) * 16 + c;
+        if (r >= p.m) continue;
+#pragma unroll
+        for (int j = 0; j < kNT; j++) {
+            const int n = nw + j * 16 + h * 4;
+            if (n >= p.n) continue;
+            if (pp.parts) store_row4(pp.parts + ((size_t)piece * p.m + r) * p.n, n, p.n - n, acc[i][j], aligned);
+            else store_row4(reinterpret_cast<Y *>(p.y) + (size_t)r * p.n, n, p.n - n, acc[i][j], aligned);
+        }
+    }
+}
+
+// adds up the pieces in their order
+template <typename Y>
+__global__ __launch_bounds__(256) void matmul_f8_join_kernel(Y *y, const float *parts, int pieces, size_t count) {
+    for (size_t i = (blockIdx.x * (size_t)256 + threadIdx.x) * 4; i < count; i += (size_t)gridDim.x * 1024) {
+        if (i + 4 <= count && count % 4 == 0) {
+            float4_t v = *reinterpret_cast<const float4_t *>(parts + i);
+            for (int s = 1; s < pieces; s++) v += *reinterpret_cast<const float4_t *>(parts + s * count + i);
+            store_row4(y + i, 0, 4, v, true);
+        } else {
+            for (size_t e = i; e < count && e < i + 4; e++) {
+                float v = parts[e];
+                for (int s = 1; s < pieces; s++) v += parts[s * count + e];
+                y[e] = (Y)v;
+            }
+        }
+    }
+}
+
+// ---- which kernel ----------------------------------------------------------------------------------------------------------------------
+constexpr int kFewRows = 64;
+constexpr int kFusedRows = 16; // up to which rows of f16 and f32 are converted on the way
+
+bool matmul_f8_converts(int m) { return m <= kFusedRows; }
+
+static int pieces_of(const MatmulF8Params &p, int tiles, int compute_units) {
+    const int across = f8_blocks(p.k);
+    return std::max(1, std::min({compute_units / tiles, across / 4, 8}));
+}
+
+struct TilesPlan {
+    int bm, bn, tiles_m, tiles_n, pieces;
+};
+static TilesPlan plan_tiles(const MatmulF8Params &p, int compute_units) {
+    TilesPlan t;
+    t.bm = t.bn = p.m > 128 && (int64_t)((p.m + 255) / 256) * ((p.n + 255) / 256) >= compute_units / 2 ? 256 : 128;
+    t.tiles_m = (p.m + t.bm - 1) / t.bm;
+    t.tiles_n = (p.n + t.bn - 1) / t.bn;
+    t.pieces = (int64_t)t.tiles_m * t.tiles_n >= compute_units ? 1 : pieces_of(p, t.tiles_m * t.tiles_n, compute_units);
+    return t;
+}
+
+size_t matmul_f8_work_floats(const MatmulF8Params &p, int compute_units) {
+    if (p.m <= kFewRows) return 0;
+    const TilesPlan t = plan_tiles(p, compute_units);
+    return t.pieces > 1 ? (size_t)t.pieces * p.m * p.n : 0;
+}
+
+template <int kMF, int kNF, typename Y>
+static void launch_rows(const RowsF8Params &p, int source, hipStream_t s) {
+    const dim3 grid((unsigned)((p.p.n + 16 * kNF - 1) / (16 * kNF))), block(kRfWaves * kWave);
+    if (source == kF8Codes) hipLaunchKernelGGL((matmul_f8_rows_kernel<kMF, kNF, kF8Codes, Y>), grid, block, 0, s, p);
+    else if constexpr (kMF == 1) {
+        if (source == kF8FromF16) hipLaunchKernelGGL((matmul_f8_rows_kernel<kMF, kNF, kF8FromF16, Y>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((matmul_f8_rows_kernel<kMF, kNF, kF8FromF32, Y>), grid, block, 0, s, p);
+    }
+}
+
+template <typename Y>
+static hipError_t launch_y(const MatmulF8Params &p, const void *src, int source, int compute_units, float *ws, hipStream_t s) {
+    if (p.m <= kFewRows) {
+        const RowsF8Params r{p, src};
+        const int tiles = (p.n + 15) / 16;
+        if (p.m <= 16) {
+            if (tiles <= 2 * compute_units) launch_rows<1, 1, Y>(r, source, s);
+            else if (tiles <= 4 * compute_units) launch_rows<1, 2, Y>(r, source, s);
+            else launch_rows<1, 4, Y>(r, source, s);
+        } else if (p.m <= 32) {
+            if (tiles <= compute_units) launch_rows<2, 1, Y>(r, kF8Codes, s);
+            else if (tiles <= 2 * compute_units) launch_rows<2, 2, Y>(r, kF8Codes, s);
+            else launch_rows<2, 4, Y>(r, kF8Codes, s);
+        } else {
+            if (tiles <= compute_units) launch_rows<4, 1, Y>(r, kF8Codes, s);
+            else if (tiles <= 2 * compute_units) launch_rows<4, 2, Y>(r, kF8Codes, s);
+            else launch_rows<4, 3, Y>(r, kF8Codes, s);
+        }
+        return hipGetLastError();
+    }
+    const TilesPlan t = plan_tiles(p, compute_units);
+    const TilesF8Params q{p, t.pieces > 1 ? ws : nullptr, t.pieces, t.tiles_m, t.tiles_n};
+    const dim3 grid((unsigned)(t.tiles_m * t.tiles_n), (unsigned)t.pieces);
+    if (t.bm == 256) hipLaunchKernelGGL((matmul_f8_tiles_kernel<4, 2, 4, 8, sizeof(Y) == 4, Y>), grid, dim3(512), 0, s, q);
+    else hipLaunchKernelGGL((matmul_f8_tiles_kernel<4, 2, 2, 4, sizeof(Y) == 4, Y>), grid, dim3(512), 0, s, q);
+    if (t.pieces > 1) {
+        const size_t count = (size_t)p.m * p.n;
+        hipLaunchKernelGGL(matmul_f8_join_kernel<Y>, dim3((unsigned)std::min<size_t>((count + 1023) / 1024, 8192)), dim3(256), 0, s, (Y *)p.y, ws, t.pieces, count);
+    }
     return hipGetLastError();
+}
+
+hipError_t launch_matmul_f8(const MatmulF8Params &p, const void *src, int src_f16, int compute_units, float *ws, hipStream_t s) {
+    const int source = !src ? kF8Codes : src_f16 ? kF8FromF16 : kF8FromF32;
+    return p.y_f16 ? launch_y<half_t>(p, src, source, compute_units, ws, s) : launch_y<float>(p, src, source, compute_units, ws, s);
 }
 
 } // namespace rlh

@@ -207,41 +207,62 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
     const MatmulF8Params &p = pp.p;
     constexpr int kWaves = kWM * kWN, kBM = 16 * kMT * kWM, kBN = 16 * kNT * kWN;
     constexpr int kStageBytes = (kBM + kBN) * kF8Block;
-    constexpr int kLoads = kStageBytes / 1024, kPerWave = (kLoads + kWaves - 1) / kWaves;
+    constexpr int kGroups = kStageBytes / 1024, kLoads = (kGroups + kWaves - 1) / kWaves; // of eight rows each, and of a wavefront
+    constexpr int kAhead = 2; // fragments of w read ahead
     static_assert(128 % (16 * kNT) == 0, "a wavefront's columns share their scale");
+    static_assert(kBM % 8 == 0, "a load is of x or of w");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kStageBytes];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, h = lane >> 4, wm = wave / kWN, wn = wave % kWN;
     const int across = f8_blocks(p.k);
     const int piece = blockIdx.y, b0 = (int)((int64_t)across * piece / pp.pieces), b1 = (int)((int64_t)across * (piece + 1) / pp.pieces);
-    const int tm = blockIdx.x % pp.tiles_m, tn = blockIdx.x / pp.tiles_m;
+    // Workgroups of one XCD, eight apart, take tiles that lie together: all rows of a stretch of columns, row tiles first.
+    const int tiles = pp.tiles_m * pp.tiles_n, xcd = blockIdx.x % 8;
+    const int tile = (int)((int64_t)tiles * xcd / 8) + (int)(blockIdx.x / 8);
+    if (tile >= (int)((int64_t)tiles * (xcd + 1) / 8)) return;
+    const int tm = tile % pp.tiles_m, tn = tile / pp.tiles_m;
     const int m0 = tm * kBM, n0 = tn * kBN;
     const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
 
-    // staging: rows of x, then of w; a wavefront-wide load covers 8 rows
-    const uint8_t *from[kPerWave];
-    int piece_at[kPerWave]; // of the lane's sixteen bytes in a block
+    // staging: rows of x, then of w; a wavefront-wide load covers eight rows, and their sixteen bytes per lane are wherever the permutation wants them
+    const uint8_t *const x0 = p.x.codes + (size_t)m0 * p.k, *const w0 = p.w.codes + (size_t)n0 * p.k;
+    uint32_t from[kLoads];
 #pragma unroll
-    for (int i = 0; i < kPerWave; i++) {
+    for (int i = 0; i < kLoads; i++) {
         const int r = (i * kWaves + wave) * 8 + lane / 8; // row of the stage
-        const bool is_x = r < kBM;
-        const int row = is_x ? min(m0 + r, p.m - 1) : min(n0 + r - kBM, p.n - 1);
-        piece_at[i] = ((lane % 8) ^ ((r >> 1) & 7)) * 16;
-        from[i] = (is_x ? p.x.codes : p.w.codes) + (size_t)row * p.k + piece_at[i];
+        const int row = r < kBM ? min(r, p.m - 1 - m0) : min(r - kBM, p.n - 1 - n0);
+        from[i] = (uint32_t)row * (uint32_t)p.k + (uint32_t)((lane % 8) ^ ((r >> 1) & 7)) * 16u; // (below 2^32: 256 rows of 2^24)
     }
-    auto fetch = [&](int b, unsigned stage) __attribute__((always_inline)) {
-        const bool whole = (b + 1) * kF8Block <= p.k;
+    auto fetch1 = [&](int b, unsigned stage, int i) __attribute__((always_inline)) {
+        if (kGroups % kWaves != 0 && i * kWaves + wave >= kGroups) return;
+        const uint8_t *base = ((i * kWaves + wave) * 8 < kBM ? x0 : w0) + (size_t)b * kF8Block;
+        dma16_base(reinterpret_cast<const half_t *>(base), from[i], lds_base + stage * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
+    };
+    auto fetch_short = [&](int b, unsigned stage) __attribute__((always_inline)) { // the last block of rows whose length is no multiple of 128: zeros behind it
+        int l = lane;
+        asm volatile("" : "+v"(l)); // (worked out here: kept in registers through the loop it cost more than 16 of them)
 #pragma unroll
-        for (int i = 0; i < kPerWave; i++) {
-            if (kLoads % kWaves != 0 && i * kWaves + wave >= kLoads) continue;
-            const uint8_t *at = from[i] + (size_t)b * kF8Block;
-            if (!whole && b * kF8Block + piece_at[i] >= p.k) at = reinterpret_cast<const uint8_t *>(&f8_zeros); // behind the last column
-            dma16(reinterpret_cast<const half_t *>(at), lds_base + stage * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
+        for (int i = 0; i < kLoads; i++) {
+            if (kGroups % kWaves != 0 && i * kWaves + wave >= kGroups) continue;
+            const int r = (i * kWaves + wave) * 8 + l / 8, at = ((l % 8) ^ ((r >> 1) & 7)) * 16;
+            const uint8_t *row = r < kBM ? x0 + (size_t)min(r, p.m - 1 - m0) * p.k : w0 + (size_t)min(r - kBM, p.n - 1 - n0) * p.k;
+            const uint8_t *from16 = b * kF8Block + at < p.k ? row + (size_t)b * kF8Block + at : reinterpret_cast<const uint8_t *>(&f8_zeros);
+            dma16(reinterpret_cast<const half_t *>(from16), lds_base + stage * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
         }
     };
-    const float *sx[kMT];
+    const int whole = p.k / kF8Block; // blocks
+    auto fetch = [&](int b, unsigned stage) __attribute__((always_inline)) {
+        if (b < whole) {
 #pragma unroll
-    for (int i = 0; i < kMT; i++) sx[i] = p.x.scales + (size_t)min(m0 + (wm * kMT + i) * 16 + c, p.m - 1) * across;
+            for (int i = 0; i < kLoads; i++) fetch1(b, stage, i);
+        } else {
+            fetch_short(b, stage);
+        }
+    };
+    const buffer_t sxb = f8_buffer(p.x.scales, (size_t)m0 * across * 4, (size_t)min(kBM, p.m - m0) * across * 4);
+    int sx_at[kMT];
+#pragma unroll
+    for (int i = 0; i < kMT; i++) sx_at[i] = min((wm * kMT + i) * 16 + c, p.m - 1 - m0) * across * 4;
     const int nw = n0 + wn * kNT * 16; // the wavefront's first column
     const float *sw = p.w.scales + (size_t)(min(nw, p.n - 1) / kF8Block) * across;
 
@@ -250,76 +271,99 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
     for (int i = 0; i < kMT; i++)
 #pragma unroll
         for (int j = 0; j < kNT; j++) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    auto frag = [&](unsigned stage, int row, uint32_t (&to)[8]) __attribute__((always_inline)) {
-        const unsigned char *at = lds + stage * kStageBytes + row * kF8Block;
-        const int swz = (row >> 1) & 7;
-        const uint4_t a = *reinterpret_cast<const uint4_t *>(at + (((2 * h) ^ swz) << 4)), b = *reinterpret_cast<const uint4_t *>(at + (((2 * h + 1) ^ swz) << 4));
+    // the lane's 32 bytes of row 16 f + c: two pieces, the same permutation for every f
+    const unsigned char *const frag_x = lds + (wm * kMT * 16 + c) * kF8Block, *const frag_w = lds + (kBM + wn * kNT * 16 + c) * kF8Block;
+    const int p0 = ((2 * h) ^ (c >> 1)) << 4, p1 = ((2 * h + 1) ^ (c >> 1)) << 4;
+    auto frag = [&](const unsigned char *at, unsigned stage, int f, uint32_t (&to)[8]) __attribute__((always_inline)) {
+        const uint4_t a = *reinterpret_cast<const uint4_t *>(at + stage * kStageBytes + f * (16 * kF8Block) + p0);
+        const uint4_t b = *reinterpret_cast<const uint4_t *>(at + stage * kStageBytes + f * (16 * kF8Block) + p1);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             to[i] = a[i];
             to[4 + i] = b[i];
         }
     };
-    float scale[kMT], ahead[kMT];
-    if (b0 < b1) {
+    float sx_next[kMT], sw_next = 0.0f;
+    auto fetch_scales = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kMT; i++) ahead[i] = sx[i][b0] * sw[b0];
+        for (int i = 0; i < kMT; i++) sx_next[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sxb, sx_at[i], b * 4, 0));
+        sw_next = sw[b];
+    };
+    if (b0 < b1) {
+        fetch_scales(b0);
         fetch(b0, 0);
     }
     unsigned stage = 0;
-    for (int b = b0; b < b1; b++) {
-        wait_vmcnt<0>();  // this wavefront's part of the block has landed
-        __syncthreads();  // ... and everybody's; everybody is done with the block before, whose stage is filled next
+    // One block.  more(i): a load of the block after it, called beside the products (all at once hold a wavefront up).
+    auto work = [&](auto more) __attribute__((always_inline)) {
+        float scale[kMT];
 #pragma unroll
-        for (int i = 0; i < kMT; i++) scale[i] = ahead[i];
-        if (b + 1 < b1) {
+        for (int i = 0; i < kMT; i++) scale[i] = sx_next[i] * sw_next;
+        uint32_t x[kMT][8], w[kAhead + 1][8];
 #pragma unroll
-            for (int i = 0; i < kMT; i++) ahead[i] = sx[i][b + 1] * sw[b + 1];
-            fetch(b + 1, 1 - stage);
-        }
-        uint32_t x[kMT][8];
+        for (int i = 0; i < kMT; i++) frag(frag_x, stage, i, x[i]);
 #pragma unroll
-        for (int i = 0; i < kMT; i++) frag(stage, (wm * kMT + i) * 16 + c, x[i]);
+        for (int j = 0; j < kAhead && j < kNT; j++) frag(frag_w, stage, j, w[j]);
+        half8_t xs[kExact ? kMT : 1][4];
         if constexpr (kExact) {
-            half8_t xs[kMT][4];
 #pragma unroll
             for (int i = 0; i < kMT; i++)
 #pragma unroll
                 for (int q = 0; q < 4; q++) xs[i][q] = f8_half8(x[i][2 * q], x[i][2 * q + 1]);
-#pragma unroll
-            for (int j = 0; j < kNT; j++) {
-                uint32_t w[8];
-                frag(stage, kBM + (wn * kNT + j) * 16 + c, w);
-                float4_t part[kMT];
-#pragma unroll
-                for (int i = 0; i < kMT; i++) part[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const half8_t ws = f8_half8(w[2 * q], w[2 * q + 1]);
-#pragma unroll
-                    for (int i = 0; i < kMT; i++) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ws, xs[i][q], part[i], 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < kMT; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(part[i][e], scale[i], acc[i][j][e]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kNT; j++) {
-                uint32_t w[8];
-                frag(stage, kBM + (wn * kNT + j) * 16 + c, w);
-                const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                float4_t part[kMT];
-#pragma unroll
-                for (int i = 0; i < kMT; i++)
-                    part[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(int8_t_, w), __builtin_bit_cast(int8_t_, x[i]), zero, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < kMT; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(part[i][e], scale[i], acc[i][j][e]);
-            }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        // a block's sum of one tile is scaled and added beside the products of the tiles after it
+        constexpr int kLag = 2;
+        float4_t part[kLag + 1];
+        auto add = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[t % kMT][t / kMT][e] = fmaf(part[t % (kLag + 1)][e], scale[t % kMT], acc[t % kMT][t / kMT][e]);
+        };
+        half8_t ws[4];
+#pragma unroll
+        for (int t = 0; t < kMT * kNT; t++) {
+            const int i = t % kMT, j = t / kMT;
+            const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (i == 0 && j + kAhead < kNT) frag(frag_w, stage, j + kAhead, w[(j + kAhead) % (kAhead + 1)]);
+            if constexpr (kExact) {
+                if (i == 0) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) ws[q] = f8_half8(w[j % (kAhead + 1)][2 * q], w[j % (kAhead + 1)][2 * q + 1]);
+                }
+                float4_t s = zero;
+#pragma unroll
+                for (int q = 0; q < 4; q++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ws[q], xs[i][q], s, 0, 0, 0);
+                part[t % (kLag + 1)] = s;
+            } else {
+                part[t % (kLag + 1)] =
+                    __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(int8_t_, w[j % (kAhead + 1)]), __builtin_bit_cast(int8_t_, x[i]), zero, 0, 0, 0, 0, 0, 0);
+            }
+            if (t >= kLag) add(t - kLag);
+            if (t * kLoads / (kMT * kNT) != (t + 1) * kLoads / (kMT * kNT)) more(t * kLoads / (kMT * kNT));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int t = kMT * kNT - kLag; t < kMT * kNT; t++) add(t);
+    };
+    // At the top this wavefront's part of the block has landed, and behind the barrier everybody's; everybody is done with the block before, whose stage is filled next.
+    int b = b0;
+    for (; b + 1 < min(b1, whole); b++) {
+        wait_vmcnt<0>();
+        __syncthreads();
+        work([&](int i) __attribute__((always_inline)) {
+            if (i == 0) fetch_scales(b + 1);
+            fetch1(b + 1, 1 - stage, i);
+        });
+        stage = 1 - stage;
+    }
+    for (; b < b1; b++) { // the last one, or two if the last one is short (branches between the products would pull them apart)
+        wait_vmcnt<0>();
+        __syncthreads();
+        const bool more = b + 1 < b1;
+        if (more) fetch_short(b + 1, 1 - stage);
+        work([&](int i) __attribute__((always_inline)) {
+            if (i == 0) fetch_scales(more ? b + 1 : b);
+        });
         stage = 1 - stage;
     }
     const bool aligned = p.n % 4 == 0;
@@ -371,7 +415,10 @@ struct TilesPlan {
 };
 static TilesPlan plan_tiles(const MatmulF8Params &p, int compute_units) {
     TilesPlan t;
-    t.bm = t.bn = p.m > 128 && (int64_t)((p.m + 255) / 256) * ((p.n + 255) / 256) >= compute_units / 2 ? 256 : 128;
+    const int wide = p.y_f16 ? 256 : 128; // of the larger tile: the f16 form needs more registers
+    const bool large = p.m > 128 && (int64_t)((p.m + 255) / 256) * ((p.n + wide - 1) / wide) >= compute_units / 2;
+    t.bm = large ? 256 : 128;
+    t.bn = large ? wide : 128;
     t.tiles_m = (p.m + t.bm - 1) / t.bm;
     t.tiles_n = (p.n + t.bn - 1) / t.bn;
     t.pieces = (int64_t)t.tiles_m * t.tiles_n >= compute_units ? 1 : pieces_of(p, t.tiles_m * t.tiles_n, compute_units);
@@ -416,8 +463,9 @@ static hipError_t launch_y(const MatmulF8Params &p, const void *src, int source,
     }
     const TilesPlan t = plan_tiles(p, compute_units);
     const TilesF8Params q{p, t.pieces > 1 ? ws : nullptr, t.pieces, t.tiles_m, t.tiles_n};
-    const dim3 grid((unsigned)(t.tiles_m * t.tiles_n), (unsigned)t.pieces);
-    if (t.bm == 256) hipLaunchKernelGGL((matmul_f8_tiles_kernel<4, 2, 4, 8, sizeof(Y) == 4, Y>), grid, dim3(512), 0, s, q);
+    const dim3 grid((unsigned)((t.tiles_m * t.tiles_n + 7) / 8 * 8), (unsigned)t.pieces);
+    constexpr bool kExact = sizeof(Y) == 4;
+    if (t.bm == 256) hipLaunchKernelGGL((matmul_f8_tiles_kernel<4, 2, 4, kExact ? 4 : 8, kExact, Y>), grid, dim3(512), 0, s, q);
     else hipLaunchKernelGGL((matmul_f8_tiles_kernel<4, 2, 2, 4, sizeof(Y) == 4, Y>), grid, dim3(512), 0, s, q);
     if (t.pieces > 1) {
         const size_t count = (size_t)p.m * p.n;

@@ -190,9 +190,14 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------------
-// A workgroup owns 16 kMT kWM rows and 16 kNT kWN columns; blocks of K pass by in LDS, two stages of 128 bytes of every row, the next one on its way while this one is
-// used.  Sixteen-byte pieces of a row are permuted by (row / 2) % 8: sixteen rows' pieces of one column lie in different banks, and every lane of a load names its own
-// address anyway.
+// A workgroup owns 16 kMT kWM rows and 16 kNT kWN columns; blocks of K pass by in two LDS stages of 128 bytes of every row.  A wavefront keeps its rows' operands of a
+// block and reads those of its columns two tiles ahead.  The one barrier of a block comes before its last two column tiles: by then everybody has read the whole stage, so
+// the loads of the block after the next go there, and the next block, on its way for as long as a block takes, has landed; its first operands are read
+// beside the last products, and the matrix cores do not wait between blocks.  (A barrier between blocks left them idle for 700 of 3300 cycles.)
+//
+// LDS places.  Sixteen-byte pieces of a row are permuted by (row / 2) % 8, and a lane's 32 bytes of K are pieces h and h + 4: the lanes that an LDS read serves at once (0 .. 3, 12 .. 15
+// and 20 .. 27, for instance) are then in 16 different places.  With pieces 2 h and 2 h + 1 they met two by two.
+// The rows' scales come through LDS as well, eight blocks at a time: a lane that reads its own from memory touches a line of its own.
 __device__ const uint4_t f8_zeros = {0u, 0u, 0u, 0u};
 
 struct TilesF8Params {
@@ -205,13 +210,21 @@ struct TilesF8Params {
 template <int kWM, int kWN, int kMT, int kNT, bool kExact, typename Y>
 __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(TilesF8Params pp) {
     const MatmulF8Params &p = pp.p;
-    constexpr int kWaves = kWM * kWN, kBM = 16 * kMT * kWM, kBN = 16 * kNT * kWN;
+    constexpr int kWaves = kWM * kWN, kThreads = kWaves * kWave, kBM = 16 * kMT * kWM, kBN = 16 * kNT * kWN, kTiles = kMT * kNT;
     constexpr int kStageBytes = (kBM + kBN) * kF8Block;
-    constexpr int kGroups = kStageBytes / 1024, kLoads = (kGroups + kWaves - 1) / kWaves; // of eight rows each, and of a wavefront
-    constexpr int kAhead = 2; // fragments of w read ahead
+    constexpr int kLoads = kStageBytes / 1024 / kWaves;         // of a wavefront, eight rows each
+    constexpr int kRing = 4, kAhead = 2;                        // operands of columns: places, and how far ahead they are read
+    constexpr int kMeet = (kNT - kAhead) * kMT;                 // the tile before which the barrier is
+    constexpr int kSpan = 8, kScales = (kBM * kSpan + kThreads - 1) / kThreads; // blocks whose scales are in LDS, and a thread's share of them
     static_assert(128 % (16 * kNT) == 0, "a wavefront's columns share their scale");
-    static_assert(kBM % 8 == 0, "a load is of x or of w");
+    constexpr int kLoadsX = kBM / 8 / kWaves;
+    static_assert(kBM % (8 * kWaves) == 0 && kBN % (8 * kWaves) == 0, "whole loads of every wavefront, of x and then of w");
+    static_assert(kNT % kRing == 0 && kNT >= kRing, "a block's first column has the same place as the one before it");
+    static_assert(kSpan % kScales == 0, "a thread's scales are of one row");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kStageBytes];
+    constexpr int kWT = (kBN + kF8Block - 1) / kF8Block; // tiles of weights' scales side by side
+    __shared__ float sx_lds[2][kSpan][kBM], sw_lds[2][kSpan][kWT];
+    static_assert(kThreads >= kSpan * kWT, "a thread for each");
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, h = lane >> 4, wm = wave / kWN, wn = wave % kWN;
     const int across = f8_blocks(p.k);
@@ -224,111 +237,111 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
     const int m0 = tm * kBM, n0 = tn * kBN;
     const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
 
-    // staging: rows of x, then of w; a wavefront-wide load covers eight rows, and their sixteen bytes per lane are wherever the permutation wants them
-    const uint8_t *const x0 = p.x.codes + (size_t)m0 * p.k, *const w0 = p.w.codes + (size_t)n0 * p.k;
+    // staging: rows of x, then of w; a wavefront-wide load covers eight rows, and the sixteen bytes of a lane are those that belong in its place
+    const uint8_t *x0 = p.x.codes + (size_t)m0 * p.k, *w0 = p.w.codes + (size_t)n0 * p.k;
+    asm volatile("" : "+s"(x0), "+s"(w0)); // (kept in scalar registers, which the loads take them from)
     uint32_t from[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
         const int r = (i * kWaves + wave) * 8 + lane / 8; // row of the stage
-        const int row = r < kBM ? min(r, p.m - 1 - m0) : min(r - kBM, p.n - 1 - n0);
+        const int row = i < kLoadsX ? min(r, p.m - 1 - m0) : min(r - kBM, p.n - 1 - n0);
         from[i] = (uint32_t)row * (uint32_t)p.k + (uint32_t)((lane % 8) ^ ((r >> 1) & 7)) * 16u; // (below 2^32: 256 rows of 2^24)
     }
-    auto fetch1 = [&](int b, unsigned stage, int i) __attribute__((always_inline)) {
-        if (kGroups % kWaves != 0 && i * kWaves + wave >= kGroups) return;
-        const uint8_t *base = ((i * kWaves + wave) * 8 < kBM ? x0 : w0) + (size_t)b * kF8Block;
-        dma16_base(reinterpret_cast<const half_t *>(base), from[i], lds_base + stage * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
+    auto fetch1 = [&](int b, int i) __attribute__((always_inline)) {
+        dma16_base(reinterpret_cast<const half_t *>((i < kLoadsX ? x0 : w0) + (size_t)b * kF8Block), from[i], lds_base + (unsigned)(b & 1) * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
     };
-    auto fetch_short = [&](int b, unsigned stage) __attribute__((always_inline)) { // the last block of rows whose length is no multiple of 128: zeros behind it
-        int l = lane;
+    const int whole = p.k / kF8Block; // blocks
+    auto fetch = [&](int b) __attribute__((always_inline)) {
+        if (b < whole) {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) fetch1(b, i);
+            return;
+        }
+        int l = lane; // the last block of rows whose length is no multiple of 128: zeros behind it
         asm volatile("" : "+v"(l)); // (worked out here: kept in registers through the loop it cost more than 16 of them)
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            if (kGroups % kWaves != 0 && i * kWaves + wave >= kGroups) continue;
             const int r = (i * kWaves + wave) * 8 + l / 8, at = ((l % 8) ^ ((r >> 1) & 7)) * 16;
-            const uint8_t *row = r < kBM ? x0 + (size_t)min(r, p.m - 1 - m0) * p.k : w0 + (size_t)min(r - kBM, p.n - 1 - n0) * p.k;
+            const uint8_t *row = i < kLoadsX ? x0 + (size_t)min(r, p.m - 1 - m0) * p.k : w0 + (size_t)min(r - kBM, p.n - 1 - n0) * p.k;
             const uint8_t *from16 = b * kF8Block + at < p.k ? row + (size_t)b * kF8Block + at : reinterpret_cast<const uint8_t *>(&f8_zeros);
-            dma16(reinterpret_cast<const half_t *>(from16), lds_base + stage * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
+            dma16(reinterpret_cast<const half_t *>(from16), lds_base + (unsigned)(b & 1) * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
         }
     };
-    const int whole = p.k / kF8Block; // blocks
-    auto fetch = [&](int b, unsigned stage) __attribute__((always_inline)) {
-        if (b < whole) {
+    // scales of blocks b0 + 8 span .. + 7: a thread has kScales neighbouring blocks of one row
+    const int s_row = tid / (kSpan / kScales), s_block = tid % (kSpan / kScales) * kScales;
+    const float *const s_from = p.x.scales + (size_t)min(m0 + s_row, p.m - 1) * across;
+    const float *const s_from_w = p.w.scales + (size_t)min(n0 / kF8Block + tid / kSpan % kWT, (p.n - 1) / kF8Block) * across;
+    float s_held[kScales], s_held_w;
+    auto take_scales = [&](int span) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < kLoads; i++) fetch1(b, stage, i);
-        } else {
-            fetch_short(b, stage);
-        }
+        for (int i = 0; i < kScales; i++) s_held[i] = s_from[min(b0 + span * kSpan + s_block + i, b1 - 1)];
+        s_held_w = s_from_w[min(b0 + span * kSpan + tid % kSpan, b1 - 1)];
     };
-    const buffer_t sxb = f8_buffer(p.x.scales, (size_t)m0 * across * 4, (size_t)min(kBM, p.m - m0) * across * 4);
-    int sx_at[kMT];
+    auto put_scales = [&](int span) __attribute__((always_inline)) {
+        if (tid < kSpan * kWT) sw_lds[span & 1][tid % kSpan][tid / kSpan] = s_held_w;
+        if (kThreads * kScales > kBM * kSpan && s_row >= kBM) return;
 #pragma unroll
-    for (int i = 0; i < kMT; i++) sx_at[i] = min((wm * kMT + i) * 16 + c, p.m - 1 - m0) * across * 4;
+        for (int i = 0; i < kScales; i++) sx_lds[span & 1][s_block + i][s_row] = s_held[i];
+    };
     const int nw = n0 + wn * kNT * 16; // the wavefront's first column
-    const float *sw = p.w.scales + (size_t)(min(nw, p.n - 1) / kF8Block) * across;
-
     float4_t acc[kMT][kNT];
 #pragma unroll
     for (int i = 0; i < kMT; i++)
 #pragma unroll
         for (int j = 0; j < kNT; j++) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    // the lane's 32 bytes of row 16 f + c: two pieces, the same permutation for every f
     const unsigned char *const frag_x = lds + (wm * kMT * 16 + c) * kF8Block, *const frag_w = lds + (kBM + wn * kNT * 16 + c) * kF8Block;
-    const int p0 = ((2 * h) ^ (c >> 1)) << 4, p1 = ((2 * h + 1) ^ (c >> 1)) << 4;
-    auto frag = [&](const unsigned char *at, unsigned stage, int f, uint32_t (&to)[8]) __attribute__((always_inline)) {
-        const uint4_t a = *reinterpret_cast<const uint4_t *>(at + stage * kStageBytes + f * (16 * kF8Block) + p0);
-        const uint4_t b = *reinterpret_cast<const uint4_t *>(at + stage * kStageBytes + f * (16 * kF8Block) + p1);
+    const int p0 = (h ^ (c >> 1)) << 4, p1 = ((h + 4) ^ (c >> 1)) << 4;
+    auto frag = [&](const unsigned char *at, int f, int b, uint32_t (&to)[8]) __attribute__((always_inline)) {
+        at += (b & 1) * kStageBytes + f * (16 * kF8Block);
+        const uint4_t lo = *reinterpret_cast<const uint4_t *>(at + p0), hi = *reinterpret_cast<const uint4_t *>(at + p1);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            to[i] = a[i];
-            to[4 + i] = b[i];
+            to[i] = lo[i];
+            to[4 + i] = hi[i];
         }
     };
-    float sx_next[kMT], sw_next = 0.0f;
-    auto fetch_scales = [&](int b) __attribute__((always_inline)) {
+    uint32_t x[kMT][8], w[kRing][8];
+    float scale[kMT], sx_next[kMT], sw_next;
+    auto read_scales = [&](int b) __attribute__((always_inline)) { // (behind the last block: of some block)
+        const int t = b - b0;
+        sw_next = sw_lds[(t / kSpan) & 1][t % kSpan][wn * kNT * 16 / kF8Block];
 #pragma unroll
-        for (int i = 0; i < kMT; i++) sx_next[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sxb, sx_at[i], b * 4, 0));
-        sw_next = sw[b];
+        for (int i = 0; i < kMT; i++) sx_next[i] = sx_lds[(t / kSpan) & 1][t % kSpan][(wm * kMT + i) * 16 + c];
     };
-    if (b0 < b1) {
-        fetch_scales(b0);
-        fetch(b0, 0);
-    }
-    unsigned stage = 0;
-    // One block.  more(i): a load of the block after it, called beside the products (all at once hold a wavefront up).
-    auto work = [&](auto more) __attribute__((always_inline)) {
-        float scale[kMT];
+    auto meet = [&]() __attribute__((always_inline)) { // loads and reads of this wavefront are done, and behind the barrier everybody's
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // One block, whose first operands are in registers.  more(i): a load of the block after the next.
+    auto work = [&](int b, auto more) __attribute__((always_inline)) {
+        constexpr int kLag = 2; // a block's sum of one tile is scaled and added beside the products of the tiles after it
+        float4_t part[kLag + 1];
+        auto add = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kMT; i++) scale[i] = sx_next[i] * sw_next;
-        uint32_t x[kMT][8], w[kAhead + 1][8];
-#pragma unroll
-        for (int i = 0; i < kMT; i++) frag(frag_x, stage, i, x[i]);
-#pragma unroll
-        for (int j = 0; j < kAhead && j < kNT; j++) frag(frag_w, stage, j, w[j]);
-        half8_t xs[kExact ? kMT : 1][4];
+            for (int e = 0; e < 4; e++) acc[t % kMT][t / kMT][e] = fmaf(part[t % (kLag + 1)][e], scale[t % kMT], acc[t % kMT][t / kMT][e]);
+        };
+        half8_t xs[kExact ? kMT : 1][4], ws[4];
         if constexpr (kExact) {
 #pragma unroll
             for (int i = 0; i < kMT; i++)
 #pragma unroll
                 for (int q = 0; q < 4; q++) xs[i][q] = f8_half8(x[i][2 * q], x[i][2 * q + 1]);
         }
+#pragma unroll
+        for (int i = 0; i < kMT; i++) scale[i] = sx_next[i] * sw_next;
         __builtin_amdgcn_sched_barrier(0);
-        // a block's sum of one tile is scaled and added beside the products of the tiles after it
-        constexpr int kLag = 2;
-        float4_t part[kLag + 1];
-        auto add = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[t % kMT][t / kMT][e] = fmaf(part[t % (kLag + 1)][e], scale[t % kMT], acc[t % kMT][t / kMT][e]);
-        };
-        half8_t ws[4];
-#pragma unroll
-        for (int t = 0; t < kMT * kNT; t++) {
+        for (int t = 0; t < kTiles; t++) {
             const int i = t % kMT, j = t / kMT;
             const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (i == 0 && j + kAhead < kNT) frag(frag_w, stage, j + kAhead, w[(j + kAhead) % (kAhead + 1)]);
+            if (t == kMeet) meet();
+            if (i == 0) frag(frag_w, (j + kAhead) % kNT, j + kAhead < kNT ? b : b + 1, w[(j + kAhead) % kRing]);
             if constexpr (kExact) {
                 if (i == 0) {
 #pragma unroll
-                    for (int q = 0; q < 4; q++) ws[q] = f8_half8(w[j % (kAhead + 1)][2 * q], w[j % (kAhead + 1)][2 * q + 1]);
+                    for (int q = 0; q < 4; q++) ws[q] = f8_half8(w[j % kRing][2 * q], w[j % kRing][2 * q + 1]);
                 }
                 float4_t s = zero;
 #pragma unroll
@@ -336,35 +349,49 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
                 part[t % (kLag + 1)] = s;
             } else {
                 part[t % (kLag + 1)] =
-                    __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(int8_t_, w[j % (kAhead + 1)]), __builtin_bit_cast(int8_t_, x[i]), zero, 0, 0, 0, 0, 0, 0);
+                    __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(int8_t_, w[j % kRing]), __builtin_bit_cast(int8_t_, x[i]), zero, 0, 0, 0, 0, 0, 0);
             }
+            __builtin_amdgcn_sched_barrier(0); // (the next product has to be on its way before the sums that wait for the one before)
             if (t >= kLag) add(t - kLag);
-            if (t * kLoads / (kMT * kNT) != (t + 1) * kLoads / (kMT * kNT)) more(t * kLoads / (kMT * kNT));
+            if (t >= kMeet) {
+                constexpr int kLeft = kTiles - kMeet;
+#pragma unroll
+                for (int l = (t - kMeet) * kLoads / kLeft; l < (t - kMeet + 1) * kLoads / kLeft; l++) more(l);
+                if (t == kMeet) read_scales(b + 1);
+            }
             __builtin_amdgcn_sched_barrier(0);
+            if (j == kNT - 1) {
+                frag(frag_x, i, b + 1, x[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
 #pragma unroll
-        for (int t = kMT * kNT - kLag; t < kMT * kNT; t++) add(t);
+        for (int t = kTiles - kLag; t < kTiles; t++) add(t);
     };
-    // At the top this wavefront's part of the block has landed, and behind the barrier everybody's; everybody is done with the block before, whose stage is filled next.
+    auto spans = [&](int b) __attribute__((always_inline)) {
+        const int t = b - b0;
+        if (t % kSpan == 0) take_scales(t / kSpan + 1);
+        if (t % kSpan == kSpan / 2) put_scales(t / kSpan + 1);
+    };
+    take_scales(0); // (a piece has one block at least)
+    put_scales(0);
+    fetch(b0);
+    meet();
+    if (b0 + 1 < min(b1, whole)) fetch(b0 + 1);
+    read_scales(b0);
+#pragma unroll
+    for (int i = 0; i < kMT; i++) frag(frag_x, i, b0, x[i]);
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) frag(frag_w, j, b0, w[j]);
     int b = b0;
-    for (; b + 1 < min(b1, whole); b++) {
-        wait_vmcnt<0>();
-        __syncthreads();
-        work([&](int i) __attribute__((always_inline)) {
-            if (i == 0) fetch_scales(b + 1);
-            fetch1(b + 1, 1 - stage, i);
-        });
-        stage = 1 - stage;
+    for (; b + 2 < min(b1, whole); b++) {
+        spans(b);
+        work(b, [&](int i) __attribute__((always_inline)) { fetch1(b + 2, i); });
     }
-    for (; b < b1; b++) { // the last one, or two if the last one is short (branches between the products would pull them apart)
-        wait_vmcnt<0>();
-        __syncthreads();
-        const bool more = b + 1 < b1;
-        if (more) fetch_short(b + 1, 1 - stage);
-        work([&](int i) __attribute__((always_inline)) {
-            if (i == 0) fetch_scales(more ? b + 1 : b);
-        });
-        stage = 1 - stage;
+    for (; b < b1; b++) { // the last two or three, without branches between the products, which would pull them apart
+        spans(b);
+        if (b + 1 < b1 && b + 1 == whole) fetch(b + 1);
+        work(b, [](int) {});
     }
     const bool aligned = p.n % 4 == 0;
 #pragma unroll

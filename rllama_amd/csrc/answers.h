@@ -19,6 +19,8 @@ struct AttnSharedParams {
     int n, n_seqs;
     int32_t start[kLongMaxSeqs];
 };
+size_t attn_shared_work_floats(const AttnSharedParams &p, int compute_units); // work memory of a call
+int64_t attn_shared_workgroups(const AttnSharedParams &p, int compute_units);
 hipError_t launch_attn_shared(const AttnSharedParams &p, int compute_units, float *ws, hipStream_t s);
 
 constexpr int kMaxTop = 32; // alternatives of a row

@@ -8,6 +8,24 @@
 
 using namespace rlh;
 
+// Work memory of calls that need more than their operands.  It grows by doubling, and a smaller one is kept until the context ends: a graph that captured a
+// call goes on using the one it was captured with.  While the stream is being captured nothing can be allocated: the call is refused.
+static int work_reserve(const char *who, rlh_ctx *ctx, AnswerWork &w, size_t bytes) {
+    if (bytes <= w.bytes) return RLH_OK;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(ctx->stream, &status));
+    if (status != hipStreamCaptureStatusNone) return fail(RLH_ERR_STATE, "%s: %zu bytes of work memory cannot be allocated while the stream is captured: make a call of this size before", who, bytes);
+    if (w.count == AnswerWork::kMost) return fail(RLH_ERR_OOM, "%s: work memory has grown too often", who);
+    size_t more = 1 << 20;
+    while (more < bytes) more *= 2;
+    void *p = nullptr;
+    const hipError_t e = device_alloc(ctx, &p, more);
+    if (e != hipSuccess) return fail(e == hipErrorOutOfMemory ? RLH_ERR_OOM : RLH_ERR_HIP, "%s: work memory of %zu bytes: %s", who, more, hipGetErrorString(e));
+    w.kept[w.count++] = p;
+    w.bytes = more;
+    return RLH_OK;
+}
+
 extern "C" int rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *prefix_k, const rlh_tensor *prefix_v, int prefix_len, const rlh_tensor *cache_k,
                                const rlh_tensor *cache_v, int n_heads, int n_kv_heads, int max_seq_len, const int32_t *start_pos, int n_seqs) {
     const char *who = "rlh_attn_shared";
@@ -57,7 +75,12 @@ extern "C" int rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_t
     p.n = n;
     p.n_seqs = n_seqs;
     for (int b = 0; b < n_seqs; b++) p.start[b] = start_pos[b];
-    HIP_TRY(launch_attn_shared(p, ctx->prop.multiProcessorCount, nullptr, ctx->stream));
+    const int cus = ctx->prop.multiProcessorCount;
+    const int64_t groups = attn_shared_workgroups(p, cus), rows = (int64_t)q->rows * (n_heads / n_kv_heads);
+    if (groups > INT32_MAX || n_kv_heads > 65535 || rows > INT32_MAX) return fail(RLH_ERR_UNSUPPORTED, "%s: %lld rows on each of %d key and value heads are more than a launch takes", who, (long long)rows, n_kv_heads);
+    const int rc = work_reserve(who, ctx, ctx->ops.shared_work, attn_shared_work_floats(p, cus) * sizeof(float));
+    if (rc != RLH_OK) return rc;
+    HIP_TRY(launch_attn_shared(p, cus, static_cast<float *>(ctx->ops.shared_work.memory()), ctx->stream));
     return RLH_OK;
 }
 
@@ -100,24 +123,6 @@ extern "C" int rlh_token_logprobs(rlh_tensor *logprobs, rlh_tensor *entropy, rlh
         p.top = top_ids->cols;
     }
     HIP_TRY(launch_token_logprobs(p, ctx->stream));
-    return RLH_OK;
-}
-
-// Work memory of calls that need more than their operands.  It grows by doubling, and a smaller one is kept until the context ends: a graph that captured a
-// call goes on using the one it was captured with.  While the stream is being captured nothing can be allocated: the call is refused.
-static int work_reserve(const char *who, rlh_ctx *ctx, AnswerWork &w, size_t bytes) {
-    if (bytes <= w.bytes) return RLH_OK;
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    HIP_TRY(hipStreamIsCapturing(ctx->stream, &status));
-    if (status != hipStreamCaptureStatusNone) return fail(RLH_ERR_STATE, "%s: %zu bytes of work memory cannot be allocated while the stream is captured: make a call of this size before", who, bytes);
-    if (w.count == AnswerWork::kMost) return fail(RLH_ERR_OOM, "%s: work memory has grown too often", who);
-    size_t more = 1 << 20;
-    while (more < bytes) more *= 2;
-    void *p = nullptr;
-    const hipError_t e = device_alloc(ctx, &p, more);
-    if (e != hipSuccess) return fail(e == hipErrorOutOfMemory ? RLH_ERR_OOM : RLH_ERR_HIP, "%s: work memory of %zu bytes: %s", who, more, hipGetErrorString(e));
-    w.kept[w.count++] = p;
-    w.bytes = more;
     return RLH_OK;
 }
 

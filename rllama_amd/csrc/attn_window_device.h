@@ -88,6 +88,18 @@ struct AttnCutParams {
     int pieces, piece_steps; // pieces of `piece_steps` steps, at most `pieces` of them
 };
 constexpr int kMaxPieces = 64;
+// How the kernels see a call of rlh_attn_window: its parameters, the position of a sequence's row i, and where a row's partial results go.  rlh_attn_shared has another one.
+struct WindowView {
+    static constexpr bool kPartial = false; // whether results are left for a join whatever the number of pieces
+    static constexpr int first_slot = 0;    // of the pieces' places in work memory
+    const AttnWindowParams &p;
+    float *ws;
+    int pieces, piece_steps;
+    __device__ explicit WindowView(const AttnCutParams &c) : p(c.a), ws(c.ws), pieces(c.pieces), piece_steps(c.piece_steps) {}
+    __device__ int start(int b) const { return p.start[b]; }
+    __device__ int position(int start, int i) const { return start + i; }
+    __device__ float *partials(int unit, int rows, int r, int hd) const { return ws + ((size_t)unit * rows + r) * pieces * (hd + 2); }
+};
 
 // Joins the pieces of rows: weights exp(m_s - M) of all pieces of a row at once (a lane each), then the sums, added up in the same order whatever
 // arrives when.  kShare wavefronts take a row: four where there are few rows, one where there are many (a workgroup for each of 32768 rows took 40 us).
@@ -95,27 +107,12 @@ constexpr int kMaxPieces = 64;
 // (device-scope stores, ticket and loads, one after the other), this takes about 3.
 constexpr int kAjWaves = 4;
 
-template <typename QT, int HD, int kTileRows, int kStep, int kShare>
-__global__ __launch_bounds__(kAjWaves *kWave) void attn_join_kernel(AttnCutParams pp) {
+// One row: `ws` holds the pairs (m, sum) of `slots` pieces and then their sums O; the first n_pieces count.  All threads of the workgroup take part.
+template <typename QT, int HD, int kShare>
+__device__ __forceinline__ void join_pieces(float (&part)[kAjWaves * (kWave / (HD / 2))][HD], const float *ws, int slots, int n_pieces, QT *out) {
     constexpr int kLanes = HD / 2, kSub = kWave / kLanes; // lanes per piece, pieces side by side in a wavefront
     constexpr int kParts = kShare * kSub;
-    __shared__ float part[kAjWaves * kSub][HD];
-    const AttnWindowParams &p = pp.a;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int group = p.n_heads / p.n_kv, rows = p.n * group;
-    const int unit = blockIdx.y, b = unit / p.n_kv, g = unit - b * p.n_kv, start = p.start[b];
-    const int r = blockIdx.x * (kAjWaves / kShare) + wave / kShare; // (with four wavefronts per row all of them leave together below)
-    int n_pieces = 0;
-    if (r < rows) {
-        const int r0 = r / kTileRows * kTileRows, r1 = min(rows, r0 + kTileRows) - 1;
-        const Span span = span_of<kStep>(max(0, start + r0 / group), start + r1 / group, p.window, p.sinks, p.max_seq_len);
-        n_pieces = start + r1 / group < 0 ? 0 : (span.steps + pp.piece_steps - 1) / pp.piece_steps;
-    }
-    if (n_pieces <= 1) { // the row is finished
-        if constexpr (kShare == 1) __syncthreads();
-        return;
-    }
-    const float *ws = pp.ws + ((size_t)unit * rows + r) * pp.pieces * (HD + 2);
     const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
     // the first sums are on their way before their weights are known
     const int sub = lane / kLanes, d = (lane % kLanes) * 2, s_first = (wave % kShare) * kSub + sub;
@@ -123,7 +120,7 @@ __global__ __launch_bounds__(kAjWaves *kWave) void attn_join_kernel(AttnCutParam
     float2 x[kBatch];
     auto fetch = [&](int s0) {
 #pragma unroll
-        for (int u = 0; u < kBatch; u++) x[u] = *reinterpret_cast<const float2 *>(ws + 2 * pp.pieces + (size_t)min(s0 + u * kParts, n_pieces - 1) * HD + d);
+        for (int u = 0; u < kBatch; u++) x[u] = *reinterpret_cast<const float2 *>(ws + 2 * slots + (size_t)min(s0 + u * kParts, n_pieces - 1) * HD + d);
     };
     fetch(s_first);
     float m = -INFINITY, l = 0.0f;
@@ -149,14 +146,35 @@ __global__ __launch_bounds__(kAjWaves *kWave) void attn_join_kernel(AttnCutParam
     }
     *reinterpret_cast<float2 *>(&part[wave * kSub + sub][d]) = o;
     __syncthreads();
-    const int i = r / group;
-    QT *out = reinterpret_cast<QT *>(p.out) + ((size_t)(b * p.n + i) * p.n_heads + g * group + (r - i * group)) * HD;
     for (int e = kShare == 1 ? lane : (int)threadIdx.x; e < HD; e += kShare * kWave) {
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kParts; w++) sum += part[wave / kShare * kParts + w][e];
         out[e] = (QT)(L == 0.0f ? 0.0f : sum / L);
     }
+}
+
+template <typename QT, int HD, int kTileRows, int kStep, int kShare>
+__global__ __launch_bounds__(kAjWaves *kWave) void attn_join_kernel(AttnCutParams pp) {
+    __shared__ float part[kAjWaves * (kWave / (HD / 2))][HD];
+    const AttnWindowParams &p = pp.a;
+    const int wave = threadIdx.x / kWave;
+    const int group = p.n_heads / p.n_kv, rows = p.n * group;
+    const int unit = blockIdx.y, b = unit / p.n_kv, g = unit - b * p.n_kv, start = p.start[b];
+    const int r = blockIdx.x * (kAjWaves / kShare) + wave / kShare; // (with four wavefronts per row all of them leave together below)
+    int n_pieces = 0;
+    if (r < rows) {
+        const int r0 = r / kTileRows * kTileRows, r1 = min(rows, r0 + kTileRows) - 1;
+        const Span span = span_of<kStep>(max(0, start + r0 / group), start + r1 / group, p.window, p.sinks, p.max_seq_len);
+        n_pieces = start + r1 / group < 0 ? 0 : (span.steps + pp.piece_steps - 1) / pp.piece_steps;
+    }
+    if (n_pieces <= 1) { // the row is finished
+        if constexpr (kShare == 1) __syncthreads();
+        return;
+    }
+    const int i = r / group;
+    join_pieces<QT, HD, kShare>(part, pp.ws + ((size_t)unit * rows + r) * pp.pieces * (HD + 2), pp.pieces, n_pieces,
+                                reinterpret_cast<QT *>(p.out) + ((size_t)(b * p.n + i) * p.n_heads + g * group + (r - i * group)) * HD);
 }
 
 template <typename QT, int HD, int kTileRows, int kStep>

@@ -49,7 +49,7 @@ struct MatmulF8Params {
     int y_f16;
     int m, n, k;
 };
-bool matmul_f8_converts(int m);                                          // whether a product of m rows converts f16 and f32 rows on the way
+bool matmul_f8_converts(int m, int k);                                   // whether a product of m rows converts f16 and f32 rows on the way
 size_t matmul_f8_work_floats(const MatmulF8Params &p, int compute_units); // sums of pieces of K
 // src: f16 or f32 rows that are converted on the way (p.x is not used then), or null
 hipError_t launch_matmul_f8(const MatmulF8Params &p, const void *src, int src_f16, int compute_units, float *ws, hipStream_t s);

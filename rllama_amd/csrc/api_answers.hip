@@ -145,7 +145,7 @@ extern "C" int rlh_matrix_mul_f8(rlh_tensor *dst, const rlh_tensor *src, const r
     p.w = eight_of(weights);
     const int cus = ctx->prop.multiProcessorCount;
     // work memory: the sums of pieces of K, and src in 8 bits where the product does not convert it on the way
-    const bool on_the_way = src->dtype != RLH_F8 && matmul_f8_converts(p.m), before = src->dtype != RLH_F8 && !on_the_way;
+    const bool on_the_way = src->dtype != RLH_F8 && matmul_f8_converts(p.m, p.k), before = src->dtype != RLH_F8 && !on_the_way;
     const size_t sums = (matmul_f8_work_floats(p, cus) * sizeof(float) + 15) / 16 * 16, codes = src->count();
     const int rc = work_reserve(who, ctx, ctx->ops.f8_work, sums + (before ? codes + (size_t)p.m * f8_blocks(p.k) * sizeof(float) : 0));
     if (rc != RLH_OK) return rc;

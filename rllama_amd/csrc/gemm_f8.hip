@@ -10,6 +10,7 @@
 // are to be as exact as f32 is: there the codes become f16 numbers (exactly: one conversion per pair) for v_mfma_f32_16x16x32_f16.
 #include "kernels.h"
 #include "answers.h"
+#include "q4.h"
 
 #include <algorithm>
 
@@ -48,26 +49,33 @@ __device__ __forceinline__ void store_row4(Y *y, int n, int left, const float4_t
 // ---- few rows --------------------------------------------------------------------------------------------------------------------------
 // A workgroup owns all rows (16 kMF of them at most) and 16 kNF columns; its wavefronts share the blocks of K, each reading its operands from memory into registers and
 // nowhere else, and add their sums up through LDS in their own order.
+//
+// Up to 16 rows of f16 or f32 are converted by the workgroup itself: a wavefront converts the blocks that it needs, sixteen lanes a row's block, while its first
+// weights are on their way, and keeps the codes in LDS.  (A launch of its own took 5 us; converted by the lanes that use them, sixteen times over for one row, 3 us.)
 enum F8Source { kF8Codes = 0, kF8FromF16 = 1, kF8FromF32 = 2 };
 struct RowsF8Params {
     MatmulF8Params p;
     const void *src; // f16 or f32 rows, converted on the way
 };
 constexpr int kRfWaves = 8;
+constexpr int kRfRow = kF8Block + 16; // of a block's codes in LDS: padded, so that rows lie in different banks
+constexpr int kRfLds = 96 * 1024;     // for converted rows
+static int rows_f8_share(int k) { return (f8_blocks(k) + kRfWaves - 1) / kRfWaves; } // blocks of a wavefront
+static size_t rows_f8_lds(int m, int k) { return (size_t)kRfWaves * rows_f8_share(k) * m * (kRfRow + 4); }
 
-template <int kMF, int kNF, int kSource, typename Y>
+// kExact: see above; kSource other than codes: kMF = 1.
+template <int kMF, int kNF, int kSource, bool kExact, typename Y>
 __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8Params pp) {
     const MatmulF8Params &p = pp.p;
     constexpr int kScales = kF8Block % (16 * kNF) == 0 ? 1 : kNF; // of the workgroup's columns
-    constexpr int kXWords = kSource == kF8Codes ? 8 : kSource == kF8FromF16 ? 16 : 32;
     __shared__ __attribute__((aligned(16))) float4_t red[kRfWaves][kMF * kNF][kWave];
+    extern __shared__ __attribute__((aligned(16))) unsigned char converted[]; // of each wavefront the codes [block][row][128], then the scales
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, h = lane >> 4;
     const int n0 = blockIdx.x * 16 * kNF, across = f8_blocks(p.k);
     const int rows_w = min(p.n - n0, 16 * kNF);
-    constexpr int kXBytes = kSource == kF8Codes ? 1 : kSource == kF8FromF16 ? 2 : 4;
     const buffer_t wb = f8_buffer(p.w.codes, (size_t)n0 * p.k, (size_t)rows_w * p.k);
-    const buffer_t xb = f8_buffer(kSource == kF8Codes ? (const void *)p.x.codes : pp.src, 0, (size_t)p.m * p.k * kXBytes);
+    const buffer_t xb = f8_buffer(p.x.codes, 0, (size_t)p.m * p.k);
     const buffer_t sb = f8_buffer(p.x.scales, 0, (size_t)p.m * across * 4);
     int w_at[kNF], x_at[kMF], s_at[kMF];
 #pragma unroll
@@ -75,82 +83,135 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
 #pragma unroll
     for (int i = 0; i < kMF; i++) {
         const int r = min(i * 16 + c, p.m - 1);
-        x_at[i] = (r * p.k + h * 32) * kXBytes;
+        x_at[i] = r * p.k + h * 32;
         s_at[i] = r * across * 4;
     }
     struct Block {
-        uint32_t w[kNF][8], x[kMF][kXWords];
+        uint32_t w[kNF][8], x[kMF][8];
         float sx[kMF], sw[kScales];
+    };
+    auto take = [](uint32_t *to, buffer_t from, int at) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; i++) to[i] = v[i];
     };
     auto load = [&](Block &k, int b) __attribute__((always_inline)) {
         const int k0 = b * kF8Block;
         const bool in0 = k0 + h * 32 < p.k, in1 = k0 + h * 32 + 16 < p.k;
-        auto take = [](uint32_t *to, buffer_t from, int at) {
-            const auto v = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; i++) to[i] = v[i];
-        };
 #pragma unroll
         for (int j = 0; j < kNF; j++) {
             take(k.w[j], wb, in0 ? w_at[j] + k0 : kF8Outside);
             take(k.w[j] + 4, wb, in1 ? w_at[j] + k0 + 16 : kF8Outside);
         }
+        if constexpr (kSource == kF8Codes) {
 #pragma unroll
-        for (int i = 0; i < kMF; i++) {
-#pragma unroll
-            for (int q = 0; q < kXWords / 4; q++) take(k.x[i] + 4 * q, xb, (q < kXWords / 8 ? in0 : in1) ? x_at[i] + k0 * kXBytes + 16 * q : kF8Outside);
-            if constexpr (kSource == kF8Codes) k.sx[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sb, s_at[i] + b * 4, 0, 0));
+            for (int i = 0; i < kMF; i++) {
+                take(k.x[i], xb, in0 ? x_at[i] + k0 : kF8Outside);
+                take(k.x[i] + 4, xb, in1 ? x_at[i] + k0 + 16 : kF8Outside);
+                k.sx[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sb, s_at[i] + b * 4, 0, 0));
+            }
         }
 #pragma unroll
         for (int t = 0; t < kScales; t++) k.sw[t] = p.w.scales[(size_t)(min(n0 + t * 16, p.n - 1) / kF8Block) * across + b];
     };
+    // Workgroups in step would ask for the same columns of all rows, which meet in few memory channels: each starts at another block.
+    const int rot = (int)(blockIdx.x * 5u % (unsigned)across);
+    auto block_of = [&](int t) {
+        const int b = t + rot;
+        return b < across ? b : b - across;
+    };
+    // converted rows: the wavefront's block t is its t / 8-th
+    const int share = (across + kRfWaves - 1) / kRfWaves;
+    unsigned char *const codes = converted + (size_t)wave * share * p.m * (kRfRow + 4);
+    float *const scales = reinterpret_cast<float *>(codes + (size_t)share * p.m * kRfRow);
+    Block now, next;
+    if constexpr (kSource == kF8Codes) {
+        if (wave < across) load(now, block_of(wave));
+    } else {
+        constexpr int kBytes = kSource == kF8FromF16 ? 2 : 4, kLoads = kBytes / 2, kBatch = 4;
+        const buffer_t src = f8_buffer(pp.src, 0, (size_t)p.m * p.k * kBytes);
+        const int mine = across > wave ? (across - wave + kRfWaves - 1) / kRfWaves : 0, items = mine * p.m; // (block, row), four at a time
+        for (int first = 0; first < items; first += 4 * kBatch) {
+            uint32_t raw[kBatch][4 * kLoads];
+#pragma unroll
+            for (int u = 0; u < kBatch; u++) {
+                const int item = first + u * 4 + h, t = item / p.m, r = item - t * p.m, k0 = block_of(min(wave + t * kRfWaves, across - 1)) * kF8Block + c * 8;
+                const int at = item < items && k0 < p.k ? (r * p.k + k0) * kBytes : kF8Outside;
+#pragma unroll
+                for (int l = 0; l < kLoads; l++) take(raw[u] + 4 * l, src, at == kF8Outside ? at : at + 16 * l);
+            }
+            if (first == 0) load(now, block_of(wave));
+#pragma unroll
+            for (int u = 0; u < kBatch; u++) {
+                const int item = first + u * 4 + h;
+                float v[8], top = 0.0f, odd = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    v[e] = kSource == kF8FromF16 ? (float)__builtin_bit_cast(half2_t, raw[u][e / 2])[e % 2] : __builtin_bit_cast(float, raw[u][e % (4 * kLoads)]);
+                    top = fmaxf(top, fabsf(v[e]));
+                    odd = fmaf(v[e], 0.0f, odd);
+                }
+                top = fmaxf(top, quad_perm<kDppQuadPerm1032>(top)); // over the sixteen lanes of the block
+                top = fmaxf(top, quad_perm<kDppQuadPerm2301>(top));
+                top = fmaxf(top, quad_perm<kDppRowHalfMirror>(top));
+                top = fmaxf(top, quad_perm<kDppRowMirror>(top));
+                odd = group_sum<16>(odd);
+                const F8Scale by(top);
+                typedef __attribute__((ext_vector_type(2))) uint32_t uint2_t;
+                uint2_t w;
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int lo = f8_codes<false>(v[4 * e] * by.factor, v[4 * e + 1] * by.factor, 0);
+                    w[e] = (uint32_t)f8_codes<true>(v[4 * e + 2] * by.factor, v[4 * e + 3] * by.factor, lo);
+                }
+                if (item < items) {
+                    *reinterpret_cast<uint2_t *>(codes + (size_t)item * kRfRow + c * 8) = w;
+                    if (c == 0) scales[item] = odd == 0.0f ? by.scale : NAN;
+                }
+            }
+        }
+        // (a wavefront reads back only what it wrote)
+    }
     float4_t acc[kMF][kNF];
 #pragma unroll
     for (int i = 0; i < kMF; i++)
 #pragma unroll
         for (int j = 0; j < kNF; j++) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    auto use = [&](Block &k) __attribute__((always_inline)) {
-        half8_t xs[kMF][4];
+    auto use = [&](Block &k, int t) __attribute__((always_inline)) {
+        if constexpr (kSource != kF8Codes) {
+            const int item = t / kRfWaves * p.m + min(c, p.m - 1);
+            const uint4_t lo = *reinterpret_cast<const uint4_t *>(codes + (size_t)item * kRfRow + h * 32), hi = *reinterpret_cast<const uint4_t *>(codes + (size_t)item * kRfRow + h * 32 + 16);
 #pragma unroll
-        for (int i = 0; i < kMF; i++) {
-            if constexpr (kSource == kF8Codes) {
+            for (int i = 0; i < 4; i++) {
+                k.x[0][i] = lo[i];
+                k.x[0][4 + i] = hi[i];
+            }
+            k.sx[0] = scales[item];
+        }
+        half8_t xs[kExact ? kMF : 1][4];
+        if constexpr (kExact) {
+#pragma unroll
+            for (int i = 0; i < kMF; i++)
 #pragma unroll
                 for (int q = 0; q < 4; q++) xs[i][q] = f8_half8(k.x[i][2 * q], k.x[i][2 * q + 1]);
-            } else { // the block's largest value is that of the four lanes of a row; codes as rlh_convert forms them
-                float v[32], top = 0.0f, odd = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 32; e++) {
-                    v[e] = kSource == kF8FromF16 ? (float)__builtin_bit_cast(half2_t, k.x[i][e / 2 % kXWords])[e % 2] : __builtin_bit_cast(float, k.x[i][e % kXWords]);
-                    top = fmaxf(top, fabsf(v[e]));
-                    odd = fmaf(v[e], 0.0f, odd);
-                }
-#pragma unroll
-                for (int off = 16; off < 64; off <<= 1) {
-                    top = fmaxf(top, __shfl_xor(top, off, kWave));
-                    odd += __shfl_xor(odd, off, kWave);
-                }
-                const F8Scale by(top);
-                k.sx[i] = odd == 0.0f ? by.scale : NAN;
-                uint32_t codes[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    int x = f8_codes<false>(v[4 * e] * by.factor, v[4 * e + 1] * by.factor, 0);
-                    codes[e] = (uint32_t)f8_codes<true>(v[4 * e + 2] * by.factor, v[4 * e + 3] * by.factor, x);
-                }
-#pragma unroll
-                for (int q = 0; q < 4; q++) xs[i][q] = f8_half8(codes[2 * q], codes[2 * q + 1]);
-            }
         }
 #pragma unroll
         for (int j = 0; j < kNF; j++) {
+            const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
             float4_t part[kMF];
+            if constexpr (kExact) {
 #pragma unroll
-            for (int i = 0; i < kMF; i++) part[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int i = 0; i < kMF; i++) part[i] = zero;
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const half8_t w = f8_half8(k.w[j][2 * q], k.w[j][2 * q + 1]);
+                for (int q = 0; q < 4; q++) {
+                    const half8_t w = f8_half8(k.w[j][2 * q], k.w[j][2 * q + 1]);
 #pragma unroll
-                for (int i = 0; i < kMF; i++) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, xs[i][q], part[i], 0, 0, 0);
+                    for (int i = 0; i < kMF; i++) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, xs[i][q], part[i], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kMF; i++)
+                    part[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(int8_t_, k.w[j]), __builtin_bit_cast(int8_t_, k.x[i]), zero, 0, 0, 0, 0, 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < kMF; i++) {
@@ -160,17 +221,9 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
             }
         }
     };
-    // Workgroups in step would ask for the same columns of all rows, which meet in few memory channels: each starts at another block.
-    const int rot = (int)(blockIdx.x * 5u % (unsigned)across);
-    auto block_of = [&](int t) {
-        const int b = t + rot;
-        return b < across ? b : b - across;
-    };
-    Block now, next;
-    if (wave < across) load(now, block_of(wave));
     for (int t = wave; t < across; t += kRfWaves) {
         if (t + kRfWaves < across) load(next, block_of(t + kRfWaves));
-        use(now);
+        use(now, t);
         now = next;
     }
 #pragma unroll
@@ -215,7 +268,7 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
     constexpr int kLoads = kStageBytes / 1024 / kWaves;         // of a wavefront, eight rows each
     constexpr int kRing = 4, kAhead = 2;                        // operands of columns: places, and how far ahead they are read
     constexpr int kMeet = (kNT - kAhead) * kMT;                 // the tile before which the barrier is
-    constexpr int kSpan = 8, kScales = (kBM * kSpan + kThreads - 1) / kThreads; // blocks whose scales are in LDS, and a thread's share of them
+    constexpr int kSpan = 8, kShare = (kBM * kSpan + kThreads - 1) / kThreads, kScales = kShare <= 2 ? kShare : kShare <= 4 ? 4 : 8; // blocks whose scales are in LDS, and a thread's share of them
     static_assert(128 % (16 * kNT) == 0, "a wavefront's columns share their scale");
     constexpr int kLoadsX = kBM / 8 / kWaves;
     static_assert(kBM % (8 * kWaves) == 0 && kBN % (8 * kWaves) == 0, "whole loads of every wavefront, of x and then of w");
@@ -428,9 +481,8 @@ __global__ __launch_bounds__(256) void matmul_f8_join_kernel(Y *y, const float *
 
 // ---- which kernel ----------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 64;
-constexpr int kFusedRows = 16; // up to which rows of f16 and f32 are converted on the way
 
-bool matmul_f8_converts(int m) { return m <= kFusedRows; }
+bool matmul_f8_converts(int m, int k) { return m <= 16 && rows_f8_lds(m, k) <= kRfLds; }
 
 static int pieces_of(const MatmulF8Params &p, int tiles, int compute_units) {
     const int across = f8_blocks(p.k);
@@ -443,8 +495,8 @@ struct TilesPlan {
 static TilesPlan plan_tiles(const MatmulF8Params &p, int compute_units) {
     TilesPlan t;
     const int wide = p.y_f16 ? 256 : 128; // of the larger tile: the f16 form needs more registers
-    const bool large = p.m > 128 && (int64_t)((p.m + 255) / 256) * ((p.n + wide - 1) / wide) >= compute_units / 2;
-    t.bm = large ? 256 : 128;
+    const bool large = p.m > 160 && (int64_t)((p.m + 255) / 256) * ((p.n + wide - 1) / wide) >= compute_units / 2;
+    t.bm = large ? 256 : p.m > 128 && p.m <= 160 ? 160 : 128;
     t.bn = large ? wide : 128;
     t.tiles_m = (p.m + t.bm - 1) / t.bm;
     t.tiles_n = (p.n + t.bn - 1) / t.bn;
@@ -458,14 +510,30 @@ size_t matmul_f8_work_floats(const MatmulF8Params &p, int compute_units) {
     return t.pieces > 1 ? (size_t)t.pieces * p.m * p.n : 0;
 }
 
+// f16 results of up to 16 rows are exact sums too: the products are not what bounds them.
 template <int kMF, int kNF, typename Y>
-static void launch_rows(const RowsF8Params &p, int source, hipStream_t s) {
+static hipError_t launch_rows(const RowsF8Params &p, int source, hipStream_t s) {
+    constexpr bool kExact = kMF == 1 || sizeof(Y) == 4;
     const dim3 grid((unsigned)((p.p.n + 16 * kNF - 1) / (16 * kNF))), block(kRfWaves * kWave);
-    if (source == kF8Codes) hipLaunchKernelGGL((matmul_f8_rows_kernel<kMF, kNF, kF8Codes, Y>), grid, block, 0, s, p);
+    if (source == kF8Codes) hipLaunchKernelGGL((matmul_f8_rows_kernel<kMF, kNF, kF8Codes, kExact, Y>), grid, block, 0, s, p);
     else if constexpr (kMF == 1) {
-        if (source == kF8FromF16) hipLaunchKernelGGL((matmul_f8_rows_kernel<kMF, kNF, kF8FromF16, Y>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((matmul_f8_rows_kernel<kMF, kNF, kF8FromF32, Y>), grid, block, 0, s, p);
+        const unsigned lds = (unsigned)rows_f8_lds(p.p.m, p.p.k);
+        const auto kernel = source == kF8FromF16 ? matmul_f8_rows_kernel<kMF, kNF, kF8FromF16, kExact, Y> : matmul_f8_rows_kernel<kMF, kNF, kF8FromF32, kExact, Y>;
+        if (lds > 24 * 1024) { // with the sums more than the 64 KiB that a kernel may have unasked
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kRfLds);
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL(kernel, grid, block, lds, s, p);
     }
+    return hipGetLastError();
+}
+
+template <int kMF, typename Y>
+static hipError_t launch_few(const RowsF8Params &p, int source, int nf, hipStream_t s) {
+    constexpr int kMost = kMF == 4 ? 3 : 4;
+    if (nf <= 1) return launch_rows<kMF, 1, Y>(p, source, s);
+    if (nf == 2) return launch_rows<kMF, 2, Y>(p, source, s);
+    return launch_rows<kMF, kMost, Y>(p, source, s);
 }
 
 template <typename Y>
@@ -473,26 +541,16 @@ static hipError_t launch_y(const MatmulF8Params &p, const void *src, int source,
     if (p.m <= kFewRows) {
         const RowsF8Params r{p, src};
         const int tiles = (p.n + 15) / 16;
-        if (p.m <= 16) {
-            if (tiles <= 2 * compute_units) launch_rows<1, 1, Y>(r, source, s);
-            else if (tiles <= 4 * compute_units) launch_rows<1, 2, Y>(r, source, s);
-            else launch_rows<1, 4, Y>(r, source, s);
-        } else if (p.m <= 32) {
-            if (tiles <= compute_units) launch_rows<2, 1, Y>(r, kF8Codes, s);
-            else if (tiles <= 2 * compute_units) launch_rows<2, 2, Y>(r, kF8Codes, s);
-            else launch_rows<2, 4, Y>(r, kF8Codes, s);
-        } else {
-            if (tiles <= compute_units) launch_rows<4, 1, Y>(r, kF8Codes, s);
-            else if (tiles <= 2 * compute_units) launch_rows<4, 2, Y>(r, kF8Codes, s);
-            else launch_rows<4, 3, Y>(r, kF8Codes, s);
-        }
-        return hipGetLastError();
+        if (p.m <= 16) return launch_few<1, Y>(r, source, (tiles + 2 * compute_units - 1) / (2 * compute_units), s);
+        if (p.m <= 32) return launch_few<2, Y>(r, kF8Codes, (tiles + compute_units - 1) / compute_units, s);
+        return launch_few<4, Y>(r, kF8Codes, (tiles + compute_units - 1) / compute_units, s);
     }
     const TilesPlan t = plan_tiles(p, compute_units);
     const TilesF8Params q{p, t.pieces > 1 ? ws : nullptr, t.pieces, t.tiles_m, t.tiles_n};
     const dim3 grid((unsigned)((t.tiles_m * t.tiles_n + 7) / 8 * 8), (unsigned)t.pieces);
     constexpr bool kExact = sizeof(Y) == 4;
     if (t.bm == 256) hipLaunchKernelGGL((matmul_f8_tiles_kernel<4, 2, 4, kExact ? 4 : 8, kExact, Y>), grid, dim3(512), 0, s, q);
+    else if (t.bm == 160) hipLaunchKernelGGL((matmul_f8_tiles_kernel<2, 2, 5, 4, kExact, Y>), grid, dim3(256), 0, s, q);
     else hipLaunchKernelGGL((matmul_f8_tiles_kernel<4, 2, 2, 4, sizeof(Y) == 4, Y>), grid, dim3(512), 0, s, q);
     if (t.pieces > 1) {
         const size_t count = (size_t)p.m * p.n;

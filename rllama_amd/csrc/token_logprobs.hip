@@ -20,10 +20,15 @@ namespace rlh {
 constexpr int kTlList = 256;
 constexpr int kTlGroups = 64;
 
-template <int kCtrl>
-__device__ __forceinline__ float dpp_max(float v) {
+template <int kCtrl, int kRowMask = 0xf>
+__device__ __forceinline__ float dpp_max(float v) { // (lanes whose row is masked out keep v)
     const int x = __builtin_bit_cast(int, v);
-    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(x, x, kCtrl, 0xf, 0xf, false)));
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(x, x, kCtrl, kRowMask, 0xf, false)));
+}
+__device__ __forceinline__ float wave_top(float v) { // the wavefront's largest, in all lanes
+    v = dpp_max<kDppRowMirror>(dpp_max<kDppRowHalfMirror>(dpp_max<kDppQuadPerm2301>(dpp_max<kDppQuadPerm1032>(v))));
+    v = dpp_max<kDppRowBcast31, 0xc>(dpp_max<kDppRowBcast15, 0xa>(v));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // Sixteen bytes of a row.  Rows of any length: only the element's own alignment.
@@ -42,6 +47,13 @@ struct RowPiece {
         }
     }
     __device__ __forceinline__ float at(int j) const { return (float)v[j]; }
+    // Keeps the sixteen bytes as they are from one pass over the pieces to the next (converted once for all passes they took four times the registers, and half of the
+    // workgroups fit a compute unit).
+    __device__ __forceinline__ void hold() {
+        uint4_t w = __builtin_bit_cast(uint4_t, v);
+        asm volatile("" : "+v"(w));
+        v = __builtin_bit_cast(vec, w);
+    }
 };
 
 // larger values first, of equal ones the lower id; all keys differ
@@ -54,15 +66,15 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
     return __builtin_bit_cast(float, w & 0x80000000u ? w & 0x7fffffffu : ~w);
 }
 
-// kKeep: pieces that a thread keeps; 0: rows of any length.  c2 = log2(e) / T.
-template <typename T, int kThreads, int kKeep>
-__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams p, float c2) {
+// kKeep: pieces that a thread keeps; 0: rows of any length.  kMany: of more rows than compute units, two to a compute unit.  c2 = log2(e) / T.
+template <typename T, int kThreads, int kKeep, bool kMany>
+__global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void token_logprobs_kernel(LogprobsParams p, float c2) {
     typedef RowPiece<T> Piece;
     constexpr int kN = Piece::kN, kStep = kThreads * kN, kWaves = kThreads / kWave, kLanes = kThreads / kTlGroups;
-    __shared__ float group_top[kTlGroups], sums[3][kWaves];
-    __shared__ float sh_bound;
+    __shared__ __attribute__((aligned(16))) float group_top[kTlGroups];
+    __shared__ float group_low[kTlGroups], sums[3][kWaves];
     __shared__ unsigned long long list[kTlList], sh_best;
-    __shared__ int sh_count, sh_ties[kWaves];
+    __shared__ int sh_count, sh_holders, holders[kThreads], sh_ties[kWaves];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int row = blockIdx.x, vocab = p.vocab;
     const T *x = reinterpret_cast<const T *>(p.logits) + (size_t)row * vocab;
@@ -71,7 +83,11 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams
     auto pieces = [&](auto f) __attribute__((always_inline)) {
         if constexpr (kKeep > 0) {
 #pragma unroll
-            for (int k = 0; k < kKeep; k++) f(kept[k], (int64_t)(k * kStep + tid * kN));
+            for (int k = 0; k < kKeep; k++) {
+                if (kMany) kept[k].hold();
+                f(kept[k], k * kStep + tid * kN);
+                if (kMany) __builtin_amdgcn_sched_barrier(0); // (one after the other, or each piece takes registers of its own for what is worked out)
+            }
         } else {
             for (int64_t i = (int64_t)tid * kN; i < vocab; i += kStep) {
                 Piece piece;
@@ -80,13 +96,22 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams
             }
         }
     };
+    // the same, from memory again
+    auto reread = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll 1
+        for (int64_t i = (int64_t)tid * kN; i < vocab; i += kStep) {
+            Piece piece;
+            piece.load(x, i, vocab);
+            f(piece, i);
+        }
+    };
     if constexpr (kKeep > 0) {
 #pragma unroll
         for (int k = 0; k < kKeep; k++) kept[k].load(x, k * kStep + tid * kN, vocab);
     }
     // ---- the largest entry, of the thread, of its group and of the row
     float mine = -INFINITY;
-    pieces([&](const Piece &piece, int64_t) {
+    pieces([&](const Piece &piece, auto) {
         typename Piece::vec t = piece.v;
 #pragma unroll
         for (int n = kN / 2; n > 0; n /= 2)
@@ -100,15 +125,21 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams
         static_assert(kLanes == 16 || kLanes == 4, "1024 or 256 threads");
         if (tid % kLanes == 0) group_top[tid / kLanes] = top;
     }
-    if (tid == 0) sh_count = 0;
+    if (tid < kTlList) list[tid] = 0;
+    if (tid == 0) sh_count = sh_holders = 0;
     __syncthreads();
-    const float of_lane = group_top[lane], m = wave_max(of_lane), base = m > -INFINITY ? m : 0.0f;
-    if (p.top > 0 && wave == kWaves - 1) { // the k-th largest of the groups' entries
-        int above = 0;
-#pragma unroll 16
-        for (int g = 0; g < kTlGroups; g++) above += group_top[g] > of_lane;
-        const float bound = -wave_max(above < p.top ? -of_lane : -INFINITY);
-        if (lane == 0) sh_bound = bound;
+    const float m = wave_top(group_top[lane]), base = m > -INFINITY ? m : 0.0f;
+    if (p.top > 0) { // the groups whose entry is among the k largest: a group's threads compare its own with a few others each
+        const float own = group_top[tid / kLanes];
+        float above = 0.0f;
+#pragma unroll
+        for (int g = 0; g < kTlGroups / kLanes; g += 4) {
+            const float4_t other = *reinterpret_cast<const float4_t *>(&group_top[tid % kLanes * (kTlGroups / kLanes) + g]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) above += other[j] > own ? 1.0f : 0.0f;
+        }
+        above = group_sum<kLanes>(above);
+        if (tid % kLanes == 0) group_low[tid / kLanes] = above < (float)p.top ? -own : -INFINITY;
     }
     // ---- the sums.  f16: z = x c2 - m c2 in one operation; m c2 was rounded, which shifts all z by the same `shift`.  f32: the difference first, since m c2 may not be
     // representable.  (A bound keeps 0 * infinity out of the second sum.)
@@ -116,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams
     auto exponent = [&](float v) { return sizeof(T) == 2 ? fmaf(v, c2, -mc) : (v - base) * c2; };
     float s = 0.0f, u = 0.0f, count = 0.0f;
     if (mine < m || !(m > -INFINITY)) {
-        pieces([&](const Piece &piece, int64_t) {
+        pieces([&](const Piece &piece, auto) {
 #pragma unroll
             for (int j = 0; j < kN; j++) {
                 const float z = exponent(piece.at(j)), e = __builtin_amdgcn_exp2f(z);
@@ -126,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams
         });
     } else { // the thread holds a largest entry: one is left out
         count = 1.0f;
-        pieces([&](const Piece &piece, int64_t) {
+        pieces([&](const Piece &piece, auto) {
 #pragma unroll
             for (int j = 0; j < kN; j++) {
                 const bool out = count > 0.0f && piece.at(j) == m;
@@ -176,19 +207,25 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams
         return;
     }
     // ---- the most probable
-    const float bound = sh_bound;
+    const float bound = -wave_top(group_low[lane]); // the least of theirs
+    // Threads that hold such an entry note themselves; their entries are then shared out, one to a thread, and read again.  (Each looking through its own
+    // took 4 us: nearly every wavefront has one of them.)
+    if (mine >= bound) holders[atomicAdd(&sh_holders, 1)] = tid;
+    __syncthreads();
+    typedef std::conditional_t<(kKeep > 0), int, int64_t> index_t;
+    const index_t each = kKeep > 0 ? kKeep * kN : (int)(((int64_t)vocab + kStep - 1) / kStep) * kN;
     auto collect = [&](bool equal_ones) __attribute__((always_inline)) {
-        if (!(mine >= bound)) return;
-        pieces([&](const Piece &piece, int64_t i) {
-#pragma unroll
-            for (int j = 0; j < kN; j++) {
-                const float v = piece.at(j);
-                if ((equal_ones ? v >= bound : v > bound) && i + j < vocab) {
-                    const int at = atomicAdd(&sh_count, 1);
-                    if (at < kTlList) list[at] = logit_key(v, (int)(i + j));
-                }
+        const index_t all = (index_t)sh_holders * each;
+        for (index_t e = tid; e < all; e += kThreads) {
+            const int h = (int)(e / each), j = (int)(e - (index_t)h * each);
+            const index_t id = (index_t)(j / kN) * kStep + holders[h] * kN + j % kN;
+            if (id >= vocab) continue;
+            const float v = (float)x[id];
+            if (equal_ones ? v >= bound : v > bound) {
+                const int at = atomicAdd(&sh_count, 1);
+                if (at < kTlList) list[at] = logit_key(v, (int)id);
             }
-        });
+        }
     };
     collect(true);
     __syncthreads();
@@ -206,7 +243,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams
                 if (tid == 0) sh_best = 0;
                 __syncthreads();
                 unsigned long long best = 0;
-                pieces([&](const Piece &piece, int64_t i) {
+                reread([&](const Piece &piece, int64_t i) {
 #pragma unroll
                     for (int j = 0; j < kN; j++) {
                         const unsigned long long key = logit_key(piece.at(j), (int)(i + j));
@@ -262,7 +299,9 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams
     for (int i = tid; i < found; i += kThreads) {
         const unsigned long long key = list[i];
         int at = 0;
-        for (int j = 0; j < found; j++) at += list[j] > key;
+        for (int j = 0; j < found; j += 8) // (places behind the last one are 0)
+#pragma unroll
+            for (int u = 0; u < 8; u++) at += list[j + u] > key;
         if (at < wanted) {
             ids[at] = (int)~(uint32_t)key;
             logprobs[at] = logprob(key_logit(key));
@@ -270,20 +309,20 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobsParams
     }
 }
 
-template <typename T>
+template <typename T, bool kMany>
 static void launch_t(const LogprobsParams &p, hipStream_t s) {
     constexpr int kN = RowPiece<T>::kN;
     const float c2 = (float)(1.44269504088896340736 / (double)p.temperature);
     const dim3 grid((unsigned)p.rows);
-    if (p.vocab <= 2048) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 8 / kN>), grid, dim3(256), 0, s, p, c2);
-    else if (p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 8 / kN>), grid, dim3(1024), 0, s, p, c2);
-    else if (p.vocab <= 32768) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 32 / kN>), grid, dim3(1024), 0, s, p, c2);
-    else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0>), grid, dim3(1024), 0, s, p, c2);
+    if (p.vocab <= 2048) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 8 / kN, kMany>), grid, dim3(256), 0, s, p, c2);
+    else if (p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 8 / kN, kMany>), grid, dim3(1024), 0, s, p, c2);
+    else if (p.vocab <= 32768) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 32 / kN, kMany>), grid, dim3(1024), 0, s, p, c2);
+    else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0, kMany>), grid, dim3(1024), 0, s, p, c2);
 }
 
 hipError_t launch_token_logprobs(const LogprobsParams &p, hipStream_t s) {
-    if (p.f16) launch_t<half_t>(p, s);
-    else launch_t<float>(p, s);
+    if (p.f16) p.rows > 256 ? launch_t<half_t, true>(p, s) : launch_t<half_t, false>(p, s);
+    else p.rows > 256 ? launch_t<float, true>(p, s) : launch_t<float, false>(p, s);
     return hipGetLastError();
 }
 

@@ -140,6 +140,11 @@ __device__ __forceinline__ void dma16_base(const half_t *base, unsigned byte_off
     asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(byte_off), "s"(base), "s"(dst) : "memory");
 }
 
+// Four bytes per lane: lane l's land at LDS byte address dst + 4 l.
+__device__ __forceinline__ void dma4_base(const float *base, unsigned byte_off, unsigned dst) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" : : "v"(byte_off), "s"(base), "s"(dst) : "memory");
+}
+
 // f(integral_constant<int, 0>), f(integral_constant<int, 1>), ...: a loop whose index is a compile-time constant in every
 // iteration (register arrays indexed by it stay in registers)
 template <typename F, int... I>

@@ -6,7 +6,7 @@
 //
 // Which matrix instruction.  v_mfma_f32_16x16x128_f8f6f4 takes 128 products at once, but adds them up eight at a time with the products aligned to the largest one's power
 // of two and cut off 2^-13 below it (measured; random operands: 1.5e-5 of the result, whatever the number of blocks), where f32 sums keep 1e-7.  f16 results are
-// rounded by 2.1e-4 of their size anyway.  So it is taken for f16 results of many rows, which the matrix cores bound.  Few rows are bound by memory, and f32 results
+// rounded by 2.1e-4 of their size anyway.  So it is taken for f16 results of more than 16 rows.  Fewer are bound by memory, and f32 results
 // are to be as exact as f32 is: there the codes become f16 numbers (exactly: one conversion per pair) for v_mfma_f32_16x16x32_f16.
 #include "kernels.h"
 #include "answers.h"
@@ -47,10 +47,10 @@ __device__ __forceinline__ void store_row4(Y *y, int n, int left, const float4_t
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------------------------
-// A workgroup owns all rows (16 kMF of them at most) and 16 kNF columns; its wavefronts share the blocks of K, each reading its operands from memory into registers and
+// Up to 16 rows.  A workgroup owns all of them and 16 kNF columns; its wavefronts share the blocks of K, each reading its operands from memory into registers and
 // nowhere else, and add their sums up through LDS in their own order.
 //
-// Up to 16 rows of f16 or f32 are converted by the workgroup itself: a wavefront converts the blocks that it needs, sixteen lanes a row's block, while its first
+// A few rows of f16 or f32 are converted by the workgroup itself: a wavefront converts the blocks that it needs, sixteen lanes a row's block, while its first
 // weights are on their way, and keeps the codes in LDS.  (A launch of its own took 5 us; converted by the lanes that use them, sixteen times over for one row, 3 us.)
 enum F8Source { kF8Codes = 0, kF8FromF16 = 1, kF8FromF32 = 2 };
 struct RowsF8Params {
@@ -63,12 +63,11 @@ constexpr int kRfLds = 96 * 1024;     // for converted rows
 static int rows_f8_share(int k) { return (f8_blocks(k) + kRfWaves - 1) / kRfWaves; } // blocks of a wavefront
 static size_t rows_f8_lds(int m, int k) { return (size_t)kRfWaves * rows_f8_share(k) * m * (kRfRow + 4); }
 
-// kExact: see above; kSource other than codes: kMF = 1.
-template <int kMF, int kNF, int kSource, bool kExact, typename Y>
+template <int kNF, int kSource, typename Y>
 __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8Params pp) {
     const MatmulF8Params &p = pp.p;
     constexpr int kScales = kF8Block % (16 * kNF) == 0 ? 1 : kNF; // of the workgroup's columns
-    __shared__ __attribute__((aligned(16))) float4_t red[kRfWaves][kMF * kNF][kWave];
+    __shared__ __attribute__((aligned(16))) float4_t red[kRfWaves][kNF][kWave];
     extern __shared__ __attribute__((aligned(16))) unsigned char converted[]; // of each wavefront the codes [block][row][128], then the scales
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, h = lane >> 4;
@@ -77,18 +76,13 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
     const buffer_t wb = f8_buffer(p.w.codes, (size_t)n0 * p.k, (size_t)rows_w * p.k);
     const buffer_t xb = f8_buffer(p.x.codes, 0, (size_t)p.m * p.k);
     const buffer_t sb = f8_buffer(p.x.scales, 0, (size_t)p.m * across * 4);
-    int w_at[kNF], x_at[kMF], s_at[kMF];
+    int w_at[kNF];
 #pragma unroll
-    for (int j = 0; j < kNF; j++) w_at[j] = min(j * 16 + c, rows_w - 1) * p.k + h * 32;
-#pragma unroll
-    for (int i = 0; i < kMF; i++) {
-        const int r = min(i * 16 + c, p.m - 1);
-        x_at[i] = r * p.k + h * 32;
-        s_at[i] = r * across * 4;
-    }
+    for (int j = 0; j < kNF; j++) w_at[j] = min(j * 16 + c, rows_w - 1) * p.k + h * 16;
+    const int my_row = min(c, p.m - 1), x_at = my_row * p.k + h * 16, s_at = my_row * across * 4;
     struct Block {
-        uint32_t w[kNF][8], x[kMF][8];
-        float sx[kMF], sw[kScales];
+        uint32_t w[kNF][8], x[8];
+        float sx, sw[kScales];
     };
     auto take = [](uint32_t *to, buffer_t from, int at) {
         const auto v = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
@@ -97,19 +91,17 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
     };
     auto load = [&](Block &k, int b) __attribute__((always_inline)) {
         const int k0 = b * kF8Block;
-        const bool in0 = k0 + h * 32 < p.k, in1 = k0 + h * 32 + 16 < p.k;
+        // a lane's 32 bytes of a block are pieces h and h + 4: each load takes whole halves of lines
+        const bool in0 = k0 + h * 16 < p.k, in1 = k0 + h * 16 + 64 < p.k;
 #pragma unroll
         for (int j = 0; j < kNF; j++) {
             take(k.w[j], wb, in0 ? w_at[j] + k0 : kF8Outside);
-            take(k.w[j] + 4, wb, in1 ? w_at[j] + k0 + 16 : kF8Outside);
+            take(k.w[j] + 4, wb, in1 ? w_at[j] + k0 + 64 : kF8Outside);
         }
         if constexpr (kSource == kF8Codes) {
-#pragma unroll
-            for (int i = 0; i < kMF; i++) {
-                take(k.x[i], xb, in0 ? x_at[i] + k0 : kF8Outside);
-                take(k.x[i] + 4, xb, in1 ? x_at[i] + k0 + 16 : kF8Outside);
-                k.sx[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sb, s_at[i] + b * 4, 0, 0));
-            }
+            take(k.x, xb, in0 ? x_at + k0 : kF8Outside);
+            take(k.x + 4, xb, in1 ? x_at + k0 + 64 : kF8Outside);
+            k.sx = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sb, s_at + b * 4, 0, 0));
         }
 #pragma unroll
         for (int t = 0; t < kScales; t++) k.sw[t] = p.w.scales[(size_t)(min(n0 + t * 16, p.n - 1) / kF8Block) * across + b];
@@ -172,53 +164,31 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
         }
         // (a wavefront reads back only what it wrote)
     }
-    float4_t acc[kMF][kNF];
+    float4_t acc[kNF];
 #pragma unroll
-    for (int i = 0; i < kMF; i++)
-#pragma unroll
-        for (int j = 0; j < kNF; j++) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < kNF; j++) acc[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     auto use = [&](Block &k, int t) __attribute__((always_inline)) {
         if constexpr (kSource != kF8Codes) {
-            const int item = t / kRfWaves * p.m + min(c, p.m - 1);
-            const uint4_t lo = *reinterpret_cast<const uint4_t *>(codes + (size_t)item * kRfRow + h * 32), hi = *reinterpret_cast<const uint4_t *>(codes + (size_t)item * kRfRow + h * 32 + 16);
+            const int item = t / kRfWaves * p.m + my_row;
+            const uint4_t lo = *reinterpret_cast<const uint4_t *>(codes + (size_t)item * kRfRow + h * 16), hi = *reinterpret_cast<const uint4_t *>(codes + (size_t)item * kRfRow + h * 16 + 64);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                k.x[0][i] = lo[i];
-                k.x[0][4 + i] = hi[i];
+                k.x[i] = lo[i];
+                k.x[4 + i] = hi[i];
             }
-            k.sx[0] = scales[item];
+            k.sx = scales[item];
         }
-        half8_t xs[kExact ? kMF : 1][4];
-        if constexpr (kExact) {
+        half8_t xs[4];
 #pragma unroll
-            for (int i = 0; i < kMF; i++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) xs[i][q] = f8_half8(k.x[i][2 * q], k.x[i][2 * q + 1]);
-        }
+        for (int q = 0; q < 4; q++) xs[q] = f8_half8(k.x[2 * q], k.x[2 * q + 1]);
 #pragma unroll
         for (int j = 0; j < kNF; j++) {
-            const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-            float4_t part[kMF];
-            if constexpr (kExact) {
+            float4_t part = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < kMF; i++) part[i] = zero;
+            for (int q = 0; q < 4; q++) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(f8_half8(k.w[j][2 * q], k.w[j][2 * q + 1]), xs[q], part, 0, 0, 0);
+            const float by = k.sx * k.sw[kScales > 1 ? j : 0];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const half8_t w = f8_half8(k.w[j][2 * q], k.w[j][2 * q + 1]);
-#pragma unroll
-                    for (int i = 0; i < kMF; i++) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, xs[i][q], part[i], 0, 0, 0);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kMF; i++)
-                    part[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(int8_t_, k.w[j]), __builtin_bit_cast(int8_t_, k.x[i]), zero, 0, 0, 0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < kMF; i++) {
-                const float by = k.sx[i] * k.sw[kScales > 1 ? j : 0];
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(part[i][e], by, acc[i][j][e]);
-            }
+            for (int e = 0; e < 4; e++) acc[j][e] = fmaf(part[e], by, acc[j][e]);
         }
     };
     for (int t = wave; t < across; t += kRfWaves) {
@@ -227,14 +197,12 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
         now = next;
     }
 #pragma unroll
-    for (int i = 0; i < kMF; i++)
-#pragma unroll
-        for (int j = 0; j < kNF; j++) red[wave][i * kNF + j][lane] = acc[i][j];
+    for (int j = 0; j < kNF; j++) red[wave][j][lane] = acc[j];
     __syncthreads();
     Y *y = reinterpret_cast<Y *>(p.y);
     const bool aligned = p.n % 4 == 0;
-    for (int s = tid; s < kMF * kNF * kWave; s += kRfWaves * kWave) {
-        const int f = s / kWave, l = s % kWave, r = f / kNF * 16 + (l & 15), n = n0 + f % kNF * 16 + (l >> 4) * 4;
+    for (int s = tid; s < kNF * kWave; s += kRfWaves * kWave) {
+        const int f = s / kWave, l = s % kWave, r = l & 15, n = n0 + f * 16 + (l >> 4) * 4;
         float4_t v = red[0][f][l];
 #pragma unroll
         for (int w = 1; w < kRfWaves; w++) v += red[w][f][l];
@@ -243,14 +211,16 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------------
-// A workgroup owns 16 kMT kWM rows and 16 kNT kWN columns; blocks of K pass by in two LDS stages of 128 bytes of every row.  A wavefront keeps its rows' operands of a
+// A workgroup owns 16 kMT kWM rows and 16 kNT kWN columns; blocks of K pass by in kStages LDS stages of 128 bytes of every row.  A wavefront keeps its rows' operands of a
 // block and reads those of its columns two tiles ahead.  The one barrier of a block comes before its last two column tiles: by then everybody has read the whole stage, so
-// the loads of the block after the next go there, and the next block, on its way for as long as a block takes, has landed; its first operands are read
-// beside the last products, and the matrix cores do not wait between blocks.  (A barrier between blocks left them idle for 700 of 3300 cycles.)
+// the loads of the block kStages further on go there, and the next block, on its way for kStages - 1 blocks, has landed; its first operands are read
+// beside the last products, and the matrix cores do not wait between blocks.  (A barrier between blocks left them idle for 700 of 3300 cycles.)  Behind the last block
+// the last one is loaded again, so that every block waits for the same number of loads and has no branches, which would pull the products apart.
 //
 // LDS places.  Sixteen-byte pieces of a row are permuted by (row / 2) % 8, and a lane's 32 bytes of K are pieces h and h + 4: the lanes that an LDS read serves at once (0 .. 3, 12 .. 15
 // and 20 .. 27, for instance) are then in 16 different places.  With pieces 2 h and 2 h + 1 they met two by two.
-// The rows' scales come through LDS as well, eight blocks at a time: a lane that reads its own from memory touches a line of its own.
+// The rows' scales come through LDS as well: a lane that reads its own from memory touches a line of its own.  With many stages by a load of four bytes per row beside each
+// block's; with two, in large tiles, eight blocks at a time through registers (2048 x 13824 x 5120: 169 us with a load per block, 151 so).
 __device__ const uint4_t f8_zeros = {0u, 0u, 0u, 0u};
 
 struct TilesF8Params {
@@ -260,24 +230,27 @@ struct TilesF8Params {
     int tiles_m, tiles_n;
 };
 
-template <int kWM, int kWN, int kMT, int kNT, bool kExact, typename Y>
-__global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(TilesF8Params pp) {
+template <int kWM, int kWN, int kMT, int kNT, int kStages, bool kExact, typename Y>
+__global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN / 4) void matmul_f8_tiles_kernel(TilesF8Params pp) {
     const MatmulF8Params &p = pp.p;
-    constexpr int kWaves = kWM * kWN, kThreads = kWaves * kWave, kBM = 16 * kMT * kWM, kBN = 16 * kNT * kWN, kTiles = kMT * kNT;
+    constexpr int kWaves = kWM * kWN, kBM = 16 * kMT * kWM, kBN = 16 * kNT * kWN, kTiles = kMT * kNT;
     constexpr int kStageBytes = (kBM + kBN) * kF8Block;
     constexpr int kLoads = kStageBytes / 1024 / kWaves;         // of a wavefront, eight rows each
     constexpr int kRing = 4, kAhead = 2;                        // operands of columns: places, and how far ahead they are read
     constexpr int kMeet = (kNT - kAhead) * kMT;                 // the tile before which the barrier is
-    constexpr int kSpan = 8, kShare = (kBM * kSpan + kThreads - 1) / kThreads, kScales = kShare <= 2 ? kShare : kShare <= 4 ? 4 : 8; // blocks whose scales are in LDS, and a thread's share of them
+    constexpr int kChunks = (kBM + 63) / 64;                    // of rows whose scales a wavefront-wide load takes; one more is the columns'
+    constexpr int kWT = (kBN + kF8Block - 1) / kF8Block;        // tiles of weights' scales side by side
     static_assert(128 % (16 * kNT) == 0, "a wavefront's columns share their scale");
     constexpr int kLoadsX = kBM / 8 / kWaves;
     static_assert(kBM % (8 * kWaves) == 0 && kBN % (8 * kWaves) == 0, "whole loads of every wavefront, of x and then of w");
     static_assert(kNT % kRing == 0 && kNT >= kRing, "a block's first column has the same place as the one before it");
-    static_assert(kSpan % kScales == 0, "a thread's scales are of one row");
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kStageBytes];
-    constexpr int kWT = (kBN + kF8Block - 1) / kF8Block; // tiles of weights' scales side by side
-    __shared__ float sx_lds[2][kSpan][kBM], sw_lds[2][kSpan][kWT];
-    static_assert(kThreads >= kSpan * kWT, "a thread for each");
+    static_assert(kChunks + 1 <= kWaves, "a wavefront for each chunk of scales");
+    constexpr bool kSpans = kStages == 2;                       // scales of kSpan blocks at a time
+    constexpr int kSpan = 8, kScales = kBM * kSpan / (kWaves * kWave), kExtra = kSpans ? 0 : 1; // a thread's share of them; loads of scales beside a block's
+    static_assert(!kSpans || (kBM * kSpan % (kWaves * kWave) == 0 && kSpan % kScales == 0), "a thread's scales are of one row");
+    static_assert((kStages - 1) * (kLoads + kExtra) < 64, "loads that are counted");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[kStages * kStageBytes];
+    __shared__ __attribute__((aligned(256))) float scales_lds[kSpans ? 2 * kSpan : kStages][kChunks + 1][64];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, h = lane >> 4, wm = wave / kWN, wn = wave % kWN;
     const int across = f8_blocks(p.k);
@@ -300,41 +273,51 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
         const int row = i < kLoadsX ? min(r, p.m - 1 - m0) : min(r - kBM, p.n - 1 - n0);
         from[i] = (uint32_t)row * (uint32_t)p.k + (uint32_t)((lane % 8) ^ ((r >> 1) & 7)) * 16u; // (below 2^32: 256 rows of 2^24)
     }
-    auto fetch1 = [&](int b, int i) __attribute__((always_inline)) {
-        dma16_base(reinterpret_cast<const half_t *>((i < kLoadsX ? x0 : w0) + (size_t)b * kF8Block), from[i], lds_base + (unsigned)(b & 1) * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
+    // a wavefront's load of scales: rows 64 chunk + lane, or the columns' tiles
+    const int chunk = wave < kChunks ? wave : wave % (kChunks + 1);
+    const float *s0 = chunk < kChunks ? p.x.scales + (size_t)m0 * across : p.w.scales + (size_t)(n0 / kF8Block) * across;
+    asm volatile("" : "+s"(s0));
+    const uint32_t s_from = (uint32_t)(chunk < kChunks ? min(chunk * 64 + lane, p.m - 1 - m0) : min(min(lane, kWT - 1), (p.n - 1) / kF8Block - n0 / kF8Block)) * (uint32_t)across * 4u;
+    const unsigned s_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)scales_lds + (unsigned)chunk * 256u;
+    // spans: a thread has kScales neighbouring blocks of one row, the first ones one of a column tile
+    const int sp_row = kSpans ? tid / (kSpan / kScales) : 0, sp_block = kSpans ? tid % (kSpan / kScales) * kScales : 0;
+    const float *const sp_from = p.x.scales + (size_t)min(m0 + sp_row, p.m - 1) * across, *const sp_from_w = p.w.scales + (size_t)min(n0 / kF8Block + tid / kSpan % kWT, (p.n - 1) / kF8Block) * across;
+    float sp_held[kSpans ? kScales : 1], sp_held_w = 0.0f;
+    // The blocks in their order: one behind the last whole block of a row goes first.  Load i of the t-th block; kLoads is that of the scales.
+    const int whole = p.k / kF8Block, count = b1 - b0, short_first = b1 > whole ? 1 : 0;
+    auto block_at = [&](int t) { return t < short_first ? whole : b0 + t - short_first; };
+    auto fetch1 = [&](int b, int t, int i) __attribute__((always_inline)) {
+        const unsigned stage = (unsigned)t % kStages;
+        if (i < kLoads) dma16_base(reinterpret_cast<const half_t *>((i < kLoadsX ? x0 : w0) + (size_t)b * kF8Block), from[i < kLoads ? i : 0], lds_base + stage * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
+        else dma4_base(s0 + b, s_from, s_base + stage * (unsigned)((kChunks + 1) * 256));
     };
-    const int whole = p.k / kF8Block; // blocks
-    auto fetch = [&](int b) __attribute__((always_inline)) {
+    auto take_span = [&](int span) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kScales; i++) sp_held[i] = sp_from[block_at(min(span * kSpan + sp_block + i, count - 1))];
+        sp_held_w = sp_from_w[block_at(min(span * kSpan + tid % kSpan, count - 1))];
+    };
+    auto put_span = [&](int span) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kScales; i++) scales_lds[(span & 1) * kSpan + sp_block + i][0][sp_row] = sp_held[i];
+        if (tid < kSpan * kWT) scales_lds[(span & 1) * kSpan + tid % kSpan][kChunks][tid / kSpan] = sp_held_w;
+    };
+    auto fetch = [&](int t) __attribute__((always_inline)) { // the t-th block, or the last one again
+        const int b = block_at(min(t, count - 1));
         if (b < whole) {
 #pragma unroll
-            for (int i = 0; i < kLoads; i++) fetch1(b, i);
+            for (int i = 0; i < kLoads + kExtra; i++) fetch1(b, t, i);
             return;
         }
-        int l = lane; // the last block of rows whose length is no multiple of 128: zeros behind it
+        int l = lane; // columns b * 128 .. of rows whose length is no multiple of 128: zeros behind them
         asm volatile("" : "+v"(l)); // (worked out here: kept in registers through the loop it cost more than 16 of them)
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
             const int r = (i * kWaves + wave) * 8 + l / 8, at = ((l % 8) ^ ((r >> 1) & 7)) * 16;
             const uint8_t *row = i < kLoadsX ? x0 + (size_t)min(r, p.m - 1 - m0) * p.k : w0 + (size_t)min(r - kBM, p.n - 1 - n0) * p.k;
             const uint8_t *from16 = b * kF8Block + at < p.k ? row + (size_t)b * kF8Block + at : reinterpret_cast<const uint8_t *>(&f8_zeros);
-            dma16(reinterpret_cast<const half_t *>(from16), lds_base + (unsigned)(b & 1) * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
+            dma16(reinterpret_cast<const half_t *>(from16), lds_base + ((unsigned)t % kStages) * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u);
         }
-    };
-    // scales of blocks b0 + 8 span .. + 7: a thread has kScales neighbouring blocks of one row
-    const int s_row = tid / (kSpan / kScales), s_block = tid % (kSpan / kScales) * kScales;
-    const float *const s_from = p.x.scales + (size_t)min(m0 + s_row, p.m - 1) * across;
-    const float *const s_from_w = p.w.scales + (size_t)min(n0 / kF8Block + tid / kSpan % kWT, (p.n - 1) / kF8Block) * across;
-    float s_held[kScales], s_held_w;
-    auto take_scales = [&](int span) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < kScales; i++) s_held[i] = s_from[min(b0 + span * kSpan + s_block + i, b1 - 1)];
-        s_held_w = s_from_w[min(b0 + span * kSpan + tid % kSpan, b1 - 1)];
-    };
-    auto put_scales = [&](int span) __attribute__((always_inline)) {
-        if (tid < kSpan * kWT) sw_lds[span & 1][tid % kSpan][tid / kSpan] = s_held_w;
-        if (kThreads * kScales > kBM * kSpan && s_row >= kBM) return;
-#pragma unroll
-        for (int i = 0; i < kScales; i++) sx_lds[span & 1][s_block + i][s_row] = s_held[i];
+        if (!kSpans) fetch1(b, t, kLoads);
     };
     const int nw = n0 + wn * kNT * 16; // the wavefront's first column
     float4_t acc[kMT][kNT];
@@ -344,8 +327,8 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
         for (int j = 0; j < kNT; j++) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     const unsigned char *const frag_x = lds + (wm * kMT * 16 + c) * kF8Block, *const frag_w = lds + (kBM + wn * kNT * 16 + c) * kF8Block;
     const int p0 = (h ^ (c >> 1)) << 4, p1 = ((h + 4) ^ (c >> 1)) << 4;
-    auto frag = [&](const unsigned char *at, int f, int b, uint32_t (&to)[8]) __attribute__((always_inline)) {
-        at += (b & 1) * kStageBytes + f * (16 * kF8Block);
+    auto frag = [&](const unsigned char *at, int f, int t, uint32_t (&to)[8]) __attribute__((always_inline)) {
+        at += ((unsigned)t % kStages) * kStageBytes + f * (16 * kF8Block);
         const uint4_t lo = *reinterpret_cast<const uint4_t *>(at + p0), hi = *reinterpret_cast<const uint4_t *>(at + p1);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -355,19 +338,21 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
     };
     uint32_t x[kMT][8], w[kRing][8];
     float scale[kMT], sx_next[kMT], sw_next;
-    auto read_scales = [&](int b) __attribute__((always_inline)) { // (behind the last block: of some block)
-        const int t = b - b0;
-        sw_next = sw_lds[(t / kSpan) & 1][t % kSpan][wn * kNT * 16 / kF8Block];
+    auto read_scales = [&](int t) __attribute__((always_inline)) {
+        const float *at = scales_lds[(unsigned)t % (kSpans ? 2 * kSpan : kStages)][0];
+        sw_next = at[kChunks * 64 + wn * kNT * 16 / kF8Block];
 #pragma unroll
-        for (int i = 0; i < kMT; i++) sx_next[i] = sx_lds[(t / kSpan) & 1][t % kSpan][(wm * kMT + i) * 16 + c];
+        for (int i = 0; i < kMT; i++) sx_next[i] = at[(wm * kMT + i) * 16 + c];
     };
-    auto meet = [&]() __attribute__((always_inline)) { // loads and reads of this wavefront are done, and behind the barrier everybody's
+    auto meet = [&](auto left) __attribute__((always_inline)) { // all but `left` loads, and the reads, of this wavefront are done, and behind the barrier everybody's
         __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        wait_vmcnt<decltype(left)::value>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
-    // One block, whose first operands are in registers.  more(i): a load of the block after the next.
+    constexpr std::integral_constant<int, (kStages - 2) * (kLoads + kExtra)> kOnTheWay{};
+    // The b-th block, whose first operands are in registers.  more(i): a load of the block kStages further on.
     auto work = [&](int b, auto more) __attribute__((always_inline)) {
         constexpr int kLag = 2; // a block's sum of one tile is scaled and added beside the products of the tiles after it
         float4_t part[kLag + 1];
@@ -389,7 +374,7 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
         for (int t = 0; t < kTiles; t++) {
             const int i = t % kMT, j = t / kMT;
             const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (t == kMeet) meet();
+            if (t == kMeet) meet(kOnTheWay);
             if (i == 0) frag(frag_w, (j + kAhead) % kNT, j + kAhead < kNT ? b : b + 1, w[(j + kAhead) % kRing]);
             if constexpr (kExact) {
                 if (i == 0) {
@@ -409,7 +394,7 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
             if (t >= kMeet) {
                 constexpr int kLeft = kTiles - kMeet;
 #pragma unroll
-                for (int l = (t - kMeet) * kLoads / kLeft; l < (t - kMeet + 1) * kLoads / kLeft; l++) more(l);
+                for (int l = (t - kMeet) * (kLoads + kExtra) / kLeft; l < (t - kMeet + 1) * (kLoads + kExtra) / kLeft; l++) more(l);
                 if (t == kMeet) read_scales(b + 1);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -421,31 +406,32 @@ __global__ __launch_bounds__(kWM *kWN *kWave, 2) void matmul_f8_tiles_kernel(Til
 #pragma unroll
         for (int t = kTiles - kLag; t < kTiles; t++) add(t);
     };
-    auto spans = [&](int b) __attribute__((always_inline)) {
-        const int t = b - b0;
-        if (t % kSpan == 0) take_scales(t / kSpan + 1);
-        if (t % kSpan == kSpan / 2) put_scales(t / kSpan + 1);
-    };
-    take_scales(0); // (a piece has one block at least)
-    put_scales(0);
-    fetch(b0);
-    meet();
-    if (b0 + 1 < min(b1, whole)) fetch(b0 + 1);
-    read_scales(b0);
-#pragma unroll
-    for (int i = 0; i < kMT; i++) frag(frag_x, i, b0, x[i]);
-#pragma unroll
-    for (int j = 0; j < kAhead; j++) frag(frag_w, j, b0, w[j]);
-    int b = b0;
-    for (; b + 2 < min(b1, whole); b++) {
-        spans(b);
-        work(b, [&](int i) __attribute__((always_inline)) { fetch1(b + 2, i); });
+    if constexpr (kSpans) {
+        take_span(0);
+        put_span(0);
     }
-    for (; b < b1; b++) { // the last two or three, without branches between the products, which would pull them apart
-        spans(b);
-        if (b + 1 < b1 && b + 1 == whole) fetch(b + 1);
-        work(b, [](int) {});
+#pragma unroll
+    for (int t = 0; t < kStages; t++) fetch(t); // (a piece has one block at least)
+    meet(std::integral_constant<int, (kStages - 1) * (kLoads + kExtra)>{});
+    read_scales(0);
+#pragma unroll
+    for (int i = 0; i < kMT; i++) frag(frag_x, i, 0, x[i]);
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) frag(frag_w, j, 0, w[j]);
+    if (count == 1) { // no whole block may be left to be loaded again: zeros then
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) from[i] = 0;
+        x0 = w0 = reinterpret_cast<const uint8_t *>(&f8_zeros);
     }
+    for (int t = 0; t < count; t++) {
+        if constexpr (kSpans) {
+            if (t % kSpan == 0) take_span(t / kSpan + 1);
+            if (t % kSpan == kSpan / 2) put_span(t / kSpan + 1);
+        }
+        const int b = count > 1 ? block_at(min(t + kStages, count - 1)) : 0; // (a whole one)
+        work(t, [&](int i) __attribute__((always_inline)) { fetch1(b, t + kStages, i); });
+    }
+    wait_vmcnt<0>(); // nothing is on its way to LDS when the workgroup ends
     const bool aligned = p.n % 4 == 0;
 #pragma unroll
     for (int i = 0; i < kMT; i++) {
@@ -480,28 +466,42 @@ __global__ __launch_bounds__(256) void matmul_f8_join_kernel(Y *y, const float *
 }
 
 // ---- which kernel ----------------------------------------------------------------------------------------------------------------------
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 16;
+constexpr int kConvertRows = 8; // up to which rows of f16 and f32 are converted on the way (8 rows of 4096 columns 8.4 us either way, 4 6.3 / 7.7, 16 of 32000 35.7 / 31)
 
-bool matmul_f8_converts(int m, int k) { return m <= 16 && rows_f8_lds(m, k) <= kRfLds; }
+bool matmul_f8_converts(int m, int k) { return m <= kConvertRows && rows_f8_lds(m, k) <= kRfLds; }
 
-static int pieces_of(const MatmulF8Params &p, int tiles, int compute_units) {
-    const int across = f8_blocks(p.k);
-    return std::max(1, std::min({compute_units / tiles, across / 4, 8}));
-}
-
+// Tiles, and pieces of K.  A call takes about 5 us, tb for every block of K in every round of workgroups over the compute units, and where K is cut 3 us more and the sums' way to memory
+// and back, 8 bytes per sum and piece at 4.5 bytes per ps.  (tb of f16 and of f32 results, measured in products of 32 to 2048 rows.  Of the smallest tile two workgroups
+// fit a compute unit, which take 1.7 times as long as one.)  The least sum is taken: 64 rows of 11008 x 4096 in two pieces 15.2 us (one 18.7, three 18.7), 131 of 4096 x 11008 in
+// eight pieces of 160 rows 22.7 us (four of 128 23.8, five of 64 23.9), 1024 of 11008 x 4096 in large tiles 56 us (small ones 76), 1024 of 4096 x 4096 in small ones 27 (52).
 struct TilesPlan {
     int bm, bn, tiles_m, tiles_n, pieces;
 };
 static TilesPlan plan_tiles(const MatmulF8Params &p, int compute_units) {
-    TilesPlan t;
-    const int wide = p.y_f16 ? 256 : 128; // of the larger tile: the f16 form needs more registers
-    const bool large = p.m > 160 && (int64_t)((p.m + 255) / 256) * ((p.n + wide - 1) / wide) >= compute_units / 2;
-    t.bm = large ? 256 : p.m > 128 && p.m <= 160 ? 160 : 128;
-    t.bn = large ? wide : 128;
-    t.tiles_m = (p.m + t.bm - 1) / t.bm;
-    t.tiles_n = (p.n + t.bn - 1) / t.bn;
-    t.pieces = (int64_t)t.tiles_m * t.tiles_n >= compute_units ? 1 : pieces_of(p, t.tiles_m * t.tiles_n, compute_units);
-    return t;
+    struct Kind {
+        int bm, bn;
+        double tb;
+    };
+    const bool f16 = p.y_f16 != 0;
+    const Kind kinds[] = {{64, 128, f16 ? 0.43 : 0.73}, {128, 128, f16 ? 0.68 : 1.15}, {160, 128, f16 ? 0.66 : 1.2}, {256, f16 ? 256 : 128, f16 ? 1.6 : 1.76}};
+    const int across = f8_blocks(p.k);
+    TilesPlan best{};
+    double least = 0.0;
+    for (const Kind &kind : kinds) {
+        TilesPlan t{kind.bm, kind.bn, (p.m + kind.bm - 1) / kind.bm, (int)(((int64_t)p.n + kind.bn - 1) / kind.bn), 1};
+        const int64_t tiles = (int64_t)t.tiles_m * t.tiles_n;
+        for (t.pieces = 1; t.pieces <= 16 && t.pieces * 2 <= std::max(2, across); t.pieces++) {
+            const int64_t rounds = (tiles * t.pieces + compute_units - 1) / compute_units;
+            const double load = kind.bm == 64 && rounds > 1 ? 0.85 * (double)rounds : (double)rounds;
+            const double us = load * ((across + t.pieces - 1) / t.pieces) * kind.tb + (t.pieces > 1 ? 3.0 + (double)t.pieces * p.m * p.n * 8 / 4.5e6 : 0.0);
+            if (best.bm == 0 || us < least) {
+                least = us;
+                best = t;
+            }
+        }
+    }
+    return best;
 }
 
 size_t matmul_f8_work_floats(const MatmulF8Params &p, int compute_units) {
@@ -510,48 +510,46 @@ size_t matmul_f8_work_floats(const MatmulF8Params &p, int compute_units) {
     return t.pieces > 1 ? (size_t)t.pieces * p.m * p.n : 0;
 }
 
-// f16 results of up to 16 rows are exact sums too: the products are not what bounds them.
-template <int kMF, int kNF, typename Y>
+template <int kNF, typename Y>
 static hipError_t launch_rows(const RowsF8Params &p, int source, hipStream_t s) {
-    constexpr bool kExact = kMF == 1 || sizeof(Y) == 4;
     const dim3 grid((unsigned)((p.p.n + 16 * kNF - 1) / (16 * kNF))), block(kRfWaves * kWave);
-    if (source == kF8Codes) hipLaunchKernelGGL((matmul_f8_rows_kernel<kMF, kNF, kF8Codes, kExact, Y>), grid, block, 0, s, p);
-    else if constexpr (kMF == 1) {
-        const unsigned lds = (unsigned)rows_f8_lds(p.p.m, p.p.k);
-        const auto kernel = source == kF8FromF16 ? matmul_f8_rows_kernel<kMF, kNF, kF8FromF16, kExact, Y> : matmul_f8_rows_kernel<kMF, kNF, kF8FromF32, kExact, Y>;
-        if (lds > 24 * 1024) { // with the sums more than the 64 KiB that a kernel may have unasked
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kRfLds);
-            if (e != hipSuccess) return e;
-        }
-        hipLaunchKernelGGL(kernel, grid, block, lds, s, p);
+    if (source == kF8Codes) {
+        hipLaunchKernelGGL((matmul_f8_rows_kernel<kNF, kF8Codes, Y>), grid, block, 0, s, p);
+        return hipGetLastError();
     }
+    const unsigned lds = (unsigned)rows_f8_lds(p.p.m, p.p.k);
+    const auto kernel = source == kF8FromF16 ? matmul_f8_rows_kernel<kNF, kF8FromF16, Y> : matmul_f8_rows_kernel<kNF, kF8FromF32, Y>;
+    if (lds > 24 * 1024) { // with the sums more than the 64 KiB that a kernel may have unasked
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kRfLds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(kernel, grid, block, lds, s, p);
     return hipGetLastError();
 }
 
-template <int kMF, typename Y>
-static hipError_t launch_few(const RowsF8Params &p, int source, int nf, hipStream_t s) {
-    constexpr int kMost = kMF == 4 ? 3 : 4;
-    if (nf <= 1) return launch_rows<kMF, 1, Y>(p, source, s);
-    if (nf == 2) return launch_rows<kMF, 2, Y>(p, source, s);
-    return launch_rows<kMF, kMost, Y>(p, source, s);
+template <int kWM, int kWN, int kMT, int kNT, int kStages, typename Y>
+static void launch_tiles(const TilesF8Params &q, hipStream_t s) {
+    const dim3 grid((unsigned)((q.tiles_m * q.tiles_n + 7) / 8 * 8), (unsigned)q.pieces);
+    hipLaunchKernelGGL((matmul_f8_tiles_kernel<kWM, kWN, kMT, kNT, kStages, sizeof(Y) == 4, Y>), grid, dim3(kWM * kWN * kWave), 0, s, q);
 }
 
 template <typename Y>
 static hipError_t launch_y(const MatmulF8Params &p, const void *src, int source, int compute_units, float *ws, hipStream_t s) {
     if (p.m <= kFewRows) {
+        // Columns of a workgroup: as few as give every compute unit the same share of them.  Its rows have to come in as well, so the share counts 16 kNF columns and m rows in every
+        // round (us, 16 / 32 / 64 columns: one row of 4096 5.5 / 6.5 / 10.1, of 11008 9.6 / 11.2 / 10.2, of 32000 25.2 / 24.0 / 24.2; 16 rows of 32000 39 / 30.4 / 26.8).
         const RowsF8Params r{p, src};
-        const int tiles = (p.n + 15) / 16;
-        if (p.m <= 16) return launch_few<1, Y>(r, source, (tiles + 2 * compute_units - 1) / (2 * compute_units), s);
-        if (p.m <= 32) return launch_few<2, Y>(r, kF8Codes, (tiles + compute_units - 1) / compute_units, s);
-        return launch_few<4, Y>(r, kF8Codes, (tiles + compute_units - 1) / compute_units, s);
+        const int64_t tiles = ((int64_t)p.n + 15) / 16;
+        auto share = [&](int nf) { return (tiles + (int64_t)nf * compute_units - 1) / ((int64_t)nf * compute_units) * (16 * nf + p.m); };
+        if (share(1) <= share(2) && share(1) <= share(4)) return launch_rows<1, Y>(r, source, s);
+        return share(2) <= share(4) ? launch_rows<2, Y>(r, source, s) : launch_rows<4, Y>(r, source, s);
     }
     const TilesPlan t = plan_tiles(p, compute_units);
     const TilesF8Params q{p, t.pieces > 1 ? ws : nullptr, t.pieces, t.tiles_m, t.tiles_n};
-    const dim3 grid((unsigned)((t.tiles_m * t.tiles_n + 7) / 8 * 8), (unsigned)t.pieces);
-    constexpr bool kExact = sizeof(Y) == 4;
-    if (t.bm == 256) hipLaunchKernelGGL((matmul_f8_tiles_kernel<4, 2, 4, kExact ? 4 : 8, kExact, Y>), grid, dim3(512), 0, s, q);
-    else if (t.bm == 160) hipLaunchKernelGGL((matmul_f8_tiles_kernel<2, 2, 5, 4, kExact, Y>), grid, dim3(256), 0, s, q);
-    else hipLaunchKernelGGL((matmul_f8_tiles_kernel<4, 2, 2, 4, sizeof(Y) == 4, Y>), grid, dim3(512), 0, s, q);
+    if (t.bm == 64) launch_tiles<2, 2, 2, 4, 3, Y>(q, s);
+    else if (t.bm == 128) launch_tiles<4, 2, 2, 4, 4, Y>(q, s);
+    else if (t.bm == 160) launch_tiles<2, 2, 5, 4, 4, Y>(q, s);
+    else launch_tiles<4, 2, 4, sizeof(Y) == 4 ? 4 : 8, 2, Y>(q, s);
     if (t.pieces > 1) {
         const size_t count = (size_t)p.m * p.n;
         hipLaunchKernelGGL(matmul_f8_join_kernel<Y>, dim3((unsigned)std::min<size_t>((count + 1023) / 1024, 8192)), dim3(256), 0, s, (Y *)p.y, ws, t.pieces, count);

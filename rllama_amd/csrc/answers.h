@@ -19,9 +19,23 @@ struct AttnSharedParams {
     int n, n_seqs;
     int32_t start[kLongMaxSeqs];
 };
-size_t attn_shared_work_floats(const AttnSharedParams &p, int compute_units); // work memory of a call
-int64_t attn_shared_workgroups(const AttnSharedParams &p, int compute_units);
-hipError_t launch_attn_shared(const AttnSharedParams &p, int compute_units, float *ws, hipStream_t s);
+// How a call is cut: the prefix, where it goes through tiles, and the rest.
+struct SharedPart {
+    int blocks;     // of rows, of a unit
+    int units;      // n_kv; of texts in tiles: n_seqs * n_kv
+    int pieces, piece_steps;
+    int first_slot; // of its pieces' places in work memory
+    int tiles;      // whether 128 rows at a time
+};
+struct SharedPlan {
+    SharedPart part[2];
+    int slots;   // places for pieces
+    bool joined; // by a second launch
+    size_t work_floats;
+    int64_t workgroups;
+};
+SharedPlan plan_attn_shared(const AttnSharedParams &p, int compute_units);
+hipError_t launch_attn_shared(const AttnSharedParams &p, const SharedPlan &plan, float *ws, hipStream_t s);
 
 constexpr int kMaxTop = 32; // alternatives of a row
 struct LogprobsParams {

@@ -75,12 +75,12 @@ extern "C" int rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_t
     p.n = n;
     p.n_seqs = n_seqs;
     for (int b = 0; b < n_seqs; b++) p.start[b] = start_pos[b];
-    const int cus = ctx->prop.multiProcessorCount;
-    const int64_t groups = attn_shared_workgroups(p, cus), rows = (int64_t)q->rows * (n_heads / n_kv_heads);
-    if (groups > INT32_MAX || n_kv_heads > 65535 || rows > INT32_MAX) return fail(RLH_ERR_UNSUPPORTED, "%s: %lld rows on each of %d key and value heads are more than a launch takes", who, (long long)rows, n_kv_heads);
-    const int rc = work_reserve(who, ctx, ctx->ops.shared_work, attn_shared_work_floats(p, cus) * sizeof(float));
+    const SharedPlan plan = plan_attn_shared(p, ctx->prop.multiProcessorCount);
+    const int64_t rows = (int64_t)q->rows * (n_heads / n_kv_heads);
+    if (plan.workgroups > INT32_MAX || n_kv_heads > 65535 || rows > INT32_MAX) return fail(RLH_ERR_UNSUPPORTED, "%s: %lld rows on each of %d key and value heads are more than a launch takes", who, (long long)rows, n_kv_heads);
+    const int rc = work_reserve(who, ctx, ctx->ops.shared_work, plan.work_floats * sizeof(float));
     if (rc != RLH_OK) return rc;
-    HIP_TRY(launch_attn_shared(p, cus, static_cast<float *>(ctx->ops.shared_work.memory()), ctx->stream));
+    HIP_TRY(launch_attn_shared(p, plan, static_cast<float *>(ctx->ops.shared_work.memory()), ctx->stream));
     return RLH_OK;
 }
 

@@ -314,7 +314,8 @@ struct RowsShared {
 };
 
 // Rows tile * 16 .. of unit b * n_kv + g, piece `piece` of their positions.  View: the call's parameters, and where the two callers differ: the position of a row, and where
-// partial results go (see attn_window_device.h).
+// partial results go (see attn_window_device.h).  View::kTexts: the unit is a key and value head, its rows are those of all texts, and the steps are the shared prefix's and
+// then those of every text's own positions, which that text's rows see.
 template <typename AC, typename QT, typename CT, int HD, typename View>
 __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared, int unit, int tile, int piece) {
     typedef Step<AC, CT, HD> St;
@@ -324,23 +325,31 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
     auto &so = shared.o;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int m = lane & 15, h = lane >> 4;
-    const int b = unit / p.n_kv, g = unit - b * p.n_kv;
+    const int b = View::kTexts ? 0 : unit / p.n_kv, g = unit - b * p.n_kv;
     const int group = p.n_heads / p.n_kv, rows = p.n * group;
-    const int start = v.start(b);
+    const int start = View::kTexts ? 0 : v.start(b);
     const int r0 = tile * kAwRows, r1 = min(rows, r0 + kAwRows) - 1;
-    const int p0 = max(0, v.position(start, r0 / group)), p1 = v.position(start, r1 / group);
+    const int p0 = max(0, v.position(start, r0 / group)), p1 = v.position(start, r1 / group); // (kTexts: not used)
 
     // the rows' places in q and out: row r is row r / group of the sequence, head g * group + r % group
     const int my_r = min(r0 + m, r1);
     const int my_i = my_r / group;
     const int my_p = r0 + m <= r1 ? v.position(start, my_i) : -1;
+    const int my_text = View::kTexts && r0 + m <= r1 ? v.text(my_i) : -1;
 
     const int my_low = p.window > 0 ? my_p - p.window + 1 : 0;
     // (bitwise on purpose: with short circuits the compiler made branches of this and lost the masking of a step's first position)
-    auto sees = [&](int at, int t_last) { return (bool)((int)(at <= min(my_p, t_last)) & ((int)(at >= my_low) | (int)(at < p.sinks))); };
+    auto sees_window = [&](int at, int t_last) { return (bool)((int)(at <= min(my_p, t_last)) & ((int)(at >= my_low) | (int)(at < p.sinks))); };
 
-    Span span = span_of<kStep>(p0, p1, p.window, p.sinks, p.max_seq_len);
-    if (p1 < 0) span.steps = 0;
+    auto span = [&] {
+        if constexpr (View::kTexts) {
+            return v.template walk<kStep>(r0, r1, lane);
+        } else {
+            Span s = span_of<kStep>(p0, p1, p.window, p.sinks, p.max_seq_len);
+            if (p1 < 0) s.steps = 0;
+            return s;
+        }
+    }();
     const int n_pieces = (span.steps + v.piece_steps - 1) / v.piece_steps;
     if (piece >= max(1, n_pieces)) return;
 
@@ -358,29 +367,46 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
     struct Place {
         int t0, last, row; // positions t0 .. min(last, t0 + kStep - 1), row of the first one
         bool front;
+        int text = -1;     // kTexts: whose positions they are; the prefix's: -1
     };
     auto place_of = [&](int s) {
-        if (s < span.steps0) return Place{s * kStep, span.first_end - 1, s * kStep, true};
-        if (s < span.steps1) return Place{span.low + (s - span.steps0) * kStep, span.turn - 1, span.row + (s - span.steps0) * kStep, false};
-        return Place{span.turn + (s - span.steps1) * kStep, span.last, p.sinks + (s - span.steps1) * kStep, false};
+        if constexpr (View::kTexts) {
+            const auto at = span.at(s);
+            return Place{at.t0, at.last, at.t0, false, at.text};
+        } else {
+            if (s < span.steps0) return Place{s * kStep, span.first_end - 1, s * kStep, true};
+            if (s < span.steps1) return Place{span.low + (s - span.steps0) * kStep, span.turn - 1, span.row + (s - span.steps0) * kStep, false};
+            return Place{span.turn + (s - span.steps1) * kStep, span.last, p.sinks + (s - span.steps1) * kStep, false};
+        }
+    };
+    auto planes_of = [&](const Place &at) { // K, V and the place's first row in them
+        if constexpr (View::kTexts) return v.planes(at.text, g, at.row);
+        else return PlaneRows{p.cache_k, p.cache_v, plane + at.row};
     };
     const Q4Bits bits;
     auto load = [&](St &st, int s) {
         constexpr int kBits = kElementBits<CT>, kRow = HD * kBits / 8, kPairRow = HD / 8;
         const Place at = place_of(s);
         const int rows_here = min(kStep, at.last - at.t0 + 1);
-        const size_t row = plane + at.row;
+        const PlaneRows from = planes_of(at);
+        const size_t row = from.row;
         if constexpr (kBits == 4) {
-            st.load(buffer_of(p.cache_k.data, row * kRow, rows_here * kRow), buffer_of(p.cache_k.pairs, row * kPairRow, rows_here * kPairRow),
-                    buffer_of(p.cache_v.data, row * kRow, rows_here * kRow), buffer_of(p.cache_v.pairs, row * kPairRow, rows_here * kPairRow), lane);
+            st.load(buffer_of(from.k.data, row * kRow, rows_here * kRow), buffer_of(from.k.pairs, row * kPairRow, rows_here * kPairRow),
+                    buffer_of(from.v.data, row * kRow, rows_here * kRow), buffer_of(from.v.pairs, row * kPairRow, rows_here * kPairRow), lane);
         } else {
-            const buffer_t k = buffer_of(p.cache_k.data, row * kRow, rows_here * kRow), v = buffer_of(p.cache_v.data, row * kRow, rows_here * kRow);
+            const buffer_t k = buffer_of(from.k.data, row * kRow, rows_here * kRow), v = buffer_of(from.v.data, row * kRow, rows_here * kRow);
             st.load(k, k, v, v, lane);
         }
     };
     // every row that is no padding sees the whole step?
     auto whole_step = [&](const Place &at) {
-        return at.t0 + kStep - 1 <= min(at.last, p0) && (at.front || p.window == 0 || at.t0 > p1 - p.window);
+        if constexpr (View::kTexts) return at.text < 0 && at.t0 + kStep - 1 <= at.last;
+        else return at.t0 + kStep - 1 <= min(at.last, p0) && (at.front || p.window == 0 || at.t0 > p1 - p.window);
+    };
+    // whether this lane's row sees position `at` of a place
+    auto sees = [&](int at, const Place &here) {
+        if constexpr (View::kTexts) return (bool)((int)(at <= here.last) & ((int)(here.text < 0) | ((int)(here.text == my_text) & (int)(at <= my_p))));
+        else return sees_window(at, here.last);
     };
     bool skipped = false, anew = false;
     auto consume = [&](const St &st, int s, auto slow) {
@@ -401,7 +427,7 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
 #pragma unroll
             for (int t = 0; t < kTiles; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) w[t][i] = sees(t0 + 16 * t + 4 * h + i, here.last) ? w[t][i] : -INFINITY;
+                for (int i = 0; i < 4; i++) w[t][i] = sees(t0 + 16 * t + 4 * h + i, here) ? w[t][i] : -INFINITY;
         }
         float top = -INFINITY;
 #pragma unroll
@@ -432,6 +458,7 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
         if constexpr (!decltype(slow)::value) {
             st.values(w, bits, o, sums);
         } else {
+            const PlaneRows from_rows = planes_of(here);
 #pragma unroll
             for (int t = 0; t < kTiles; t++)
 #pragma unroll
@@ -440,13 +467,13 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
                     for (int hh = 0; hh < 4; hh++) {
                         const int j = 16 * t + 4 * hh + i;
                         const float wt = __shfl(w[t][i], hh * 16 + m, kWave) * (St::kLowSums ? 0.0625f : 1.0f);
-                        const bool seen = sees(t0 + j, here.last);
-                        const size_t from = (plane + here.row + j) * HD + 4 * h * kDims;
+                        const bool seen = sees(t0 + j, here);
+                        const size_t from = (from_rows.row + j) * HD + 4 * h * kDims;
 #pragma unroll
                         for (int x = 0; x < 4; x++)
 #pragma unroll
                             for (int e = 0; e < kDims; e++)
-                                if (seen) o[e][x] = fmaf(wt, plane_load1<CT>(p.cache_v, from + x * kDims + e), o[e][x]);
+                                if (seen) o[e][x] = fmaf(wt, plane_load1<CT>(from_rows.v, from + x * kDims + e), o[e][x]);
                     }
                 }
         }
@@ -514,10 +541,10 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
 #pragma unroll
         for (int i = 0; i < kPer; i++) O[i] = fmaf(so[w][jr][jd + i], f, O[i]);
     }
-    const int jri = (r0 + jr) / group;
+    const int jri = min(r0 + jr, r1) / group;
     if (v.position(start, jri) < 0) L = 0.0f; // padding
     QT *out = reinterpret_cast<QT *>(p.out) + ((size_t)(b * p.n + jri) * p.n_heads + g * group + (r0 + jr - jri * group)) * HD + jd;
-    if (!View::kPartial && n_pieces <= 1) {
+    if (!v.partial() && n_pieces <= 1) {
         if (mine) {
 #pragma unroll
             for (int i = 0; i < kPer; i++) out[i] = (QT)(L == 0.0f ? 0.0f : O[i] / L);
@@ -528,12 +555,14 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
     if (mine) {
         float *ws = v.partials(unit, rows, r0 + jr, HD);
         const int slot = v.first_slot + piece;
-        if (jd == 0) {
-            ws[2 * slot] = M;
-            ws[2 * slot + 1] = L;
-        }
+        if (jd == 0) *reinterpret_cast<float2 *>(ws + 2 * slot) = make_float2(M, L);
+        ws += 2 * v.pieces + slot * HD + jd;
+        if constexpr (kPer == 1) {
+            ws[0] = O[0];
+        } else {
 #pragma unroll
-        for (int i = 0; i < kPer; i++) ws[2 * v.pieces + slot * HD + jd + i] = O[i];
+            for (int i = 0; i < kPer; i += 2) *reinterpret_cast<float2 *>(ws + i) = make_float2(O[i], O[i + 1]);
+        }
     }
 }
 

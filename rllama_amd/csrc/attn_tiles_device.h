@@ -456,7 +456,7 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
             }
     }
     const float l = my_p < 0 ? 0.0f : l_run + __shfl_xor(l_run, 32, 64); // (padding: 0)
-    if (kShares > 1 && (View::kPartial || n_pieces > 1)) { // ---- leave (m, sum) and O of the piece for the join
+    if (kShares > 1 && (v.partial() || n_pieces > 1)) { // ---- leave (m, sum) and O of the piece for the join
         if (w0 + col > r1) return;
         float *ws = v.partials(unit, rows, w0 + col, HD);
         const int slot = v.first_slot + piece;

@@ -90,15 +90,22 @@ struct AttnCutParams {
 constexpr int kMaxPieces = 64;
 // How the kernels see a call of rlh_attn_window: its parameters, the position of a sequence's row i, and where a row's partial results go.  rlh_attn_shared has another one.
 struct WindowView {
-    static constexpr bool kPartial = false; // whether results are left for a join whatever the number of pieces
-    static constexpr int first_slot = 0;    // of the pieces' places in work memory
+    static constexpr bool kTexts = false; // see attn_rows_device.h
+    static constexpr int first_slot = 0;  // of the pieces' places in work memory
     const AttnWindowParams &p;
     float *ws;
     int pieces, piece_steps;
     __device__ explicit WindowView(const AttnCutParams &c) : p(c.a), ws(c.ws), pieces(c.pieces), piece_steps(c.piece_steps) {}
     __device__ int start(int b) const { return p.start[b]; }
     __device__ int position(int start, int i) const { return start + i; }
+    __device__ constexpr bool partial() const { return false; } // whether results are left for a join whatever the number of pieces
+    __device__ int text(int) const { return 0; }
     __device__ float *partials(int unit, int rows, int r, int hd) const { return ws + ((size_t)unit * rows + r) * pieces * (hd + 2); }
+};
+// Rows of K and V planes from `row` on.
+struct PlaneRows {
+    PlaneRef k, v;
+    size_t row;
 };
 
 // Joins the pieces of rows: weights exp(m_s - M) of all pieces of a row at once (a lane each), then the sums, added up in the same order whatever

@@ -388,8 +388,8 @@ int  rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *pre
  * Logits of -infinity have probability 0.  A row of nothing else: -infinity, entropy 0, the first k ids.  A row with a NaN or +infinity: NaN, and ids of -1. */
 int  rlh_token_logprobs(rlh_tensor *logprobs, rlh_tensor *entropy, rlh_tensor *top_ids, rlh_tensor *top_logprobs, const rlh_tensor *logits, const rlh_tensor *tokens,
                         float temperature);
-/* rlh_convert to 8 bits: per block, a = max(largest |x|, 448 * 2^-126), scale = a / 448, code = e4m3(x * (448 / a)), each step one f32 operation, the last one rounded to
- * even and limited to 448.  A block with a value that is not finite reads as NaN throughout.  From 8 bits: code * scale in f32, rounded once more for f16.
+/* rlh_convert to 8 bits: per block, a = max(largest |x|, 448 * 2^-126), scale = a / 448, code = e4m3(x * (448 * (1 / a))), each step one f32 operation, the last one
+ * rounded to even and limited to 448.  A block with a value that is not finite reads as NaN throughout.  From 8 bits: code * scale in f32, rounded once more for f16.
  *
  * dst [n x m] = src [n x k] times weights[m x k]^T: weights RLH_F8_TILES; src RLH_F8, or f16 or f32, which is converted to RLH_F8 first; dst f16 or f32.
  * Products and sums of a block of 128 in f32, each block's sum times both scales in f32. */

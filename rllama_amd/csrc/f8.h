@@ -21,13 +21,13 @@ struct EightRef {
 __host__ __device__ inline int f8_blocks(int cols) { return (cols + kF8Block - 1) / kF8Block; }
 
 // Scale and factor of a block whose largest value is `top` (finite): value = code * scale, code = e4m3(value * factor).  The bound keeps both normal numbers; below it
-// a block is all but zero.
+// a block is all but zero.  (The factor is a reciprocal and a product, two roundings, as array libraries divide a number by an array: codes made there and here are the same.)
 struct F8Scale {
     float scale, factor;
     __device__ explicit F8Scale(float top) {
         const float a = fmaxf(top, kF8Largest * 1.1754943508222875e-38f);
         scale = a / kF8Largest;
-        factor = kF8Largest / a;
+        factor = kF8Largest * (1.0f / a);
     }
 };
 // codes of two values, in the low or the high half of `word`; the conversion rounds ties to even, and codes above the largest one would read as NaN

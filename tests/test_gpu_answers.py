@@ -46,7 +46,7 @@ def encode(x, tile):
                 continue
             a = max(np.abs(v).max(), TINY)
             scales[i, j] = a / f32(448)
-            codes[at] = e4m3(np.clip(v * (f32(448) / a), f32(-448), f32(448)))
+            codes[at] = e4m3(np.clip(v * (f32(448) * (f32(1) / a)), f32(-448), f32(448)))
     return codes, scales
 
 

@@ -233,6 +233,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void
     if (found > kTlList) {
         __syncthreads();
         if (tid == 0) sh_count = 0;
+        if (tid < kTlList) list[tid] = 0;
         __syncthreads();
         collect(false);
         __syncthreads();

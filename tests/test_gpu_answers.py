@@ -451,6 +451,26 @@ def test_logprobs_of_special_rows(ctx, vocab, kind):
     assert np.array_equal(g[2][8][2:], [i for i in range(31) if i != 3])
 
 
+@pytest.mark.parametrize("vocab", [600, 5000, 32000, 40000])
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("larger", [3, 27, 101, 203, 255, 256, 257, 450])
+def test_logprobs_of_larger_ones_side_by_side(ctx, vocab, kind, larger):
+    """The larger entries lie together, at the front, in the middle and at the end, and all others are equal: what bounds the most probable ones from below is met by all."""
+    rng = np.random.default_rng(larger)
+    x = np.zeros((12, vocab), NUMPY[kind])
+    for r in range(12):
+        at = [0, (vocab - larger) // 2 + r, vocab - larger][r % 3]
+        x[r, at:at + larger] = rng.permutation(larger) / 64 + 0.5
+        if r >= 6:
+            x[r, x[r] == 0] = -np.inf
+    g = [t.to_numpy() for t in Tensor.from_numpy(ctx, x).token_logprobs(None, 0.9, 32)[2:]]
+    ids = first_of_the_largest(x, 32)
+    assert np.array_equal(g[0], ids)
+    want = np.take_along_axis(logprobs_reference(x, 0.9)[0], ids, 1)
+    with np.errstate(invalid="ignore"):
+        assert ((g[1] == want) | (np.abs(g[1] - want) <= EPS32 * (8 + 2 * np.sqrt(vocab) + 6 * np.abs(want) + 6 * np.log(vocab)))).all()
+
+
 # -- refusals ---------------------------------------------------------------------------------------------------------------------------
 
 def test_refusals_of_the_attention(ctx):

@@ -10,10 +10,13 @@
 //
 // The k most probable: the 64 groups of threads have a largest entry each, and the k-th largest of those bounds the k-th largest entry from below, since k groups hold an
 // entry that large.  What reaches the bound (about k ln(64 / (64 - k)) / (k / 64) of 32000 random entries) goes to a list in LDS, and an entry's place is the number
-// of those in front of it.  Lists that overflow: of rows with many entries equal to the bound (masks) those above it, and then the first equal ones in order of their ids;
-// where those above it are too many as well, one entry after the other.
+// of those in front of it.  Lists that overflow: of rows with many entries equal to the bound (masks) those above it, and then the first equal ones in order of their ids.
+// Where those above it are too many as well (they lie side by side, in fewer than k groups), the k-th largest of the threads' own entries is a closer bound, and
+// where that is not enough, one entry after the other.
 #include "kernels.h"
 #include "answers.h"
+
+#include <type_traits>
 
 namespace rlh {
 
@@ -31,10 +34,9 @@ __device__ __forceinline__ float wave_top(float v) { // the wavefront's largest,
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// Sixteen bytes of a row.  Rows of any length: only the element's own alignment.
-template <typename T>
+// kN entries of a row, sixteen bytes at most.  Rows of any length: only the element's own alignment.
+template <typename T, int kN>
 struct RowPiece {
-    static constexpr int kN = 16 / (int)sizeof(T);
     typedef T any __attribute__((ext_vector_type(kN), aligned(sizeof(T))));
     typedef T vec __attribute__((ext_vector_type(kN)));
     vec v;
@@ -47,10 +49,11 @@ struct RowPiece {
         }
     }
     __device__ __forceinline__ float at(int j) const { return (float)v[j]; }
-    // Keeps the sixteen bytes as they are from one pass over the pieces to the next (converted once for all passes they took four times the registers, and half of the
+    // Keeps the bytes as they are from one pass over the pieces to the next (converted once for all passes they took four times the registers, and half of the
     // workgroups fit a compute unit).
     __device__ __forceinline__ void hold() {
-        uint4_t w = __builtin_bit_cast(uint4_t, v);
+        typedef std::conditional_t<sizeof(v) == 4, uint32_t, std::conditional_t<sizeof(v) == 8, unsigned long long, uint4_t>> words;
+        words w = __builtin_bit_cast(words, v);
         asm volatile("" : "+v"(w));
         v = __builtin_bit_cast(vec, w);
     }
@@ -66,11 +69,11 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
     return __builtin_bit_cast(float, w & 0x80000000u ? w & 0x7fffffffu : ~w);
 }
 
-// kKeep: pieces that a thread keeps; 0: rows of any length.  kMany: of more rows than compute units, two to a compute unit.  c2 = log2(e) / T.
-template <typename T, int kThreads, int kKeep, bool kMany>
+// kKeep: pieces of kN entries that a thread keeps; 0: rows of any length.  kMany: of more rows than compute units, two to a compute unit.  c2 = log2(e) / T.
+template <typename T, int kThreads, int kN, int kKeep, bool kMany>
 __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void token_logprobs_kernel(LogprobsParams p, float c2) {
-    typedef RowPiece<T> Piece;
-    constexpr int kN = Piece::kN, kStep = kThreads * kN, kWaves = kThreads / kWave, kLanes = kThreads / kTlGroups;
+    typedef RowPiece<T, kN> Piece;
+    constexpr int kStep = kThreads * kN, kWaves = kThreads / kWave, kLanes = kThreads / kTlGroups;
     __shared__ __attribute__((aligned(16))) float group_top[kTlGroups];
     __shared__ float group_low[kTlGroups], sums[3][kWaves];
     __shared__ unsigned long long list[kTlList], sh_best;
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void
         return;
     }
     // ---- the most probable
-    const float bound = -wave_top(group_low[lane]); // the least of theirs
+    float bound = -wave_top(group_low[lane]); // the least of theirs
     // Threads that hold such an entry note themselves; their entries are then shared out, one to a thread, and read again.  (Each looking through its own
     // took 4 us: nearly every wavefront has one of them.)
     if (mine >= bound) holders[atomicAdd(&sh_holders, 1)] = tid;
@@ -227,17 +230,52 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void
             }
         }
     };
-    collect(true);
-    __syncthreads();
-    int found = sh_count, wanted = p.top; // of the list
-    if (found > kTlList) {
+    auto count_of = [&](bool equal_ones) __attribute__((always_inline)) {
+        collect(equal_ones);
+        __syncthreads();
+        return sh_count;
+    };
+    auto again = [&] { // the list is empty
         __syncthreads();
         if (tid == 0) sh_count = 0;
         if (tid < kTlList) list[tid] = 0;
         __syncthreads();
-        collect(false);
-        __syncthreads();
-        found = sh_count;
+    };
+    int found = count_of(true), wanted = p.top; // of the list
+    if (found > kTlList) {
+        again();
+        found = count_of(false);
+        bool equal_ones = true; // are left to be added
+        if (found > kTlList) {
+            again();
+            // the k-th largest of the threads' own (32 of 1000 entries side by side, all others masked, in 32000: 300 us one after the other, 33 so)
+            if (tid == 0) sh_holders = 0;
+            __syncthreads();
+            if (mine > bound) holders[atomicAdd(&sh_holders, 1)] = __builtin_bit_cast(int, mine);
+            __syncthreads();
+            int n = sh_holders, above = 0;
+            for (int i = 0; i < n; i++) above += __builtin_bit_cast(float, holders[i]) > mine;
+            const float low = wave_top(mine > bound && above < p.top ? -mine : -INFINITY);
+            if (lane == 0) sums[0][wave] = low;
+            __syncthreads();
+            float least = sums[0][0];
+#pragma unroll
+            for (int w = 1; w < kWaves; w++) least = fmaxf(least, sums[0][w]);
+            if (n >= p.top) {
+                bound = -least;
+                if (tid == 0) sh_holders = 0;
+                __syncthreads();
+                if (mine >= bound) holders[atomicAdd(&sh_holders, 1)] = tid;
+                __syncthreads();
+                found = count_of(true);
+                equal_ones = false;
+                if (found > kTlList) {
+                    again();
+                    found = count_of(false);
+                    equal_ones = true;
+                }
+            }
+        }
         if (found > kTlList) { // one after the other
             unsigned long long below = ~0ull;
             for (int k = 0; k < p.top; k++) {
@@ -262,10 +300,10 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void
             }
             return;
         }
-        wanted = min(p.top, found);
+        if (equal_ones) wanted = min(p.top, found);
         // the first ids of entries that equal the bound, a stretch of the row at a time
         const float at_bound = logprob(bound);
-        int place = found;
+        int place = equal_ones ? found : p.top;
         for (int64_t from = 0; place < p.top && from < vocab; from += kStep) {
             Piece piece;
             piece.load(x, from + (int64_t)tid * kN, vocab);
@@ -312,13 +350,15 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void
 
 template <typename T, bool kMany>
 static void launch_t(const LogprobsParams &p, hipStream_t s) {
-    constexpr int kN = RowPiece<T>::kN;
+    constexpr int kN = 16 / (int)sizeof(T);
     const float c2 = (float)(1.44269504088896340736 / (double)p.temperature);
     const dim3 grid((unsigned)p.rows);
-    if (p.vocab <= 2048) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 8 / kN, kMany>), grid, dim3(256), 0, s, p, c2);
-    else if (p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 8 / kN, kMany>), grid, dim3(1024), 0, s, p, c2);
-    else if (p.vocab <= 32768) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 32 / kN, kMany>), grid, dim3(1024), 0, s, p, c2);
-    else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0, kMany>), grid, dim3(1024), 0, s, p, c2);
+    // Narrow pieces in short rows, so that 33 groups at least hold entries: 20 or 32 alternatives of 500 entries, or of 2100 in f16, took 85 to 150 us in pieces of sixteen
+    // bytes, whose few groups give no bound, and take less than 20 so, as those of other lengths do.
+    if (p.vocab <= 2048) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 2, 4, kMany>), grid, dim3(256), 0, s, p, c2);
+    else if (p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 4, 2, kMany>), grid, dim3(1024), 0, s, p, c2);
+    else if (p.vocab <= 32768) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, kN, 32 / kN, kMany>), grid, dim3(1024), 0, s, p, c2);
+    else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, kN, 0, kMany>), grid, dim3(1024), 0, s, p, c2);
 }
 
 hipError_t launch_token_logprobs(const LogprobsParams &p, hipStream_t s) {

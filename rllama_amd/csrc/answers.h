@@ -19,13 +19,12 @@ struct AttnSharedParams {
     int n, n_seqs;
     int32_t start[kLongMaxSeqs];
 };
-// How a call is cut: the prefix, where it goes through tiles, and the rest.
+// How a call is cut: what goes through tiles, and what 16 rows at a time.  One of them has the prefix, one the texts' own positions.
 struct SharedPart {
-    int blocks;     // of rows, of a unit
-    int units;      // n_kv; of texts in tiles: n_seqs * n_kv
+    int prefix, texts;
+    int blocks; // of rows, of a key and value head
     int pieces, piece_steps;
     int first_slot; // of its pieces' places in work memory
-    int tiles;      // whether 128 rows at a time
 };
 struct SharedPlan {
     SharedPart part[2];

@@ -359,7 +359,6 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
     for (int e = 0; e < kDims; e++) o[e] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     typename St::Sums sums{float4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 
-    const size_t plane = (size_t)unit * p.max_seq_len;
     typename St::Queries queries;
     St::load_q(queries, reinterpret_cast<const QT *>(p.q) + ((size_t)(b * p.n + my_i) * p.n_heads + g * group + (my_r - my_i * group)) * HD, h);
     const float c2_all = 1.44269504088896340736f / sqrtf((float)HD), c2 = c2_all * queries.up; // (the second one is the row's own)
@@ -379,10 +378,7 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
             return Place{span.turn + (s - span.steps1) * kStep, span.last, p.sinks + (s - span.steps1) * kStep, false};
         }
     };
-    auto planes_of = [&](const Place &at) { // K, V and the place's first row in them
-        if constexpr (View::kTexts) return v.planes(at.text, g, at.row);
-        else return PlaneRows{p.cache_k, p.cache_v, plane + at.row};
-    };
+    auto planes_of = [&](const Place &at) { return v.planes(unit, at.text, at.row); };
     const Q4Bits bits;
     auto load = [&](St &st, int s) {
         constexpr int kBits = kElementBits<CT>, kRow = HD * kBits / 8, kPairRow = HD / 8;

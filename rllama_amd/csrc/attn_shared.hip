@@ -5,10 +5,11 @@
 // Sums over parts of the positions, each with a reference point m of its own, join into one: so the prefix is read once for the rows of all texts that share a key and value
 // head, instead of once per text.
 //
-// Few rows per key and value head, or f32 arithmetic: 16 rows at a time, whatever texts they are of, from memory into registers (attn_rows_device.h).  A tile's steps are the prefix's and
-// then every one of its texts', masked for the rows of the others; they are cut into pieces, and where there is only one the result is final.
-// Many: the prefix through tiles of keys in LDS for 128 rows (attn_tiles_device.h, f16 arithmetic), and the texts' own positions beside it in the same launch: 16 rows at a time as above, or,
-// where a text alone has many rows, in tiles as well.  Pieces leave (m, sum, O) of their rows in work memory, and a second launch joins them.
+// A workgroup takes rows of one key and value head, whatever texts they are of; its steps are the prefix's and then every one of its texts', masked for the rows of the others.  They
+// are cut into pieces; where there is only one the result is final, and pieces leave (m, sum, O) of their rows in work memory, which a second launch joins.
+//   Few rows per key and value head, or f32 arithmetic: 16 rows at a time, from memory into registers (attn_rows_device.h).
+//   Many rows of each text: 128 at a time, through tiles of keys in LDS (attn_tiles_device.h, f16 arithmetic).
+//   Many rows, but few of each text: the prefix in tiles; 128 rows would be of too many texts for the texts' own positions, which go 16 rows at a time beside them in the same launch.
 #include "kernels.h"
 #include "answers.h"
 #include "attn_rows_device.h"
@@ -22,10 +23,11 @@ struct SharedKernelParams {
     AttnSharedParams a;
     float *ws; // for every row of every key and value head the pairs (m, sum) of all its pieces, then the sums O of each
     int slots; // places for pieces
-    SharedPart part[2]; // the prefix in tiles (none where everything goes 16 rows at a time); the rest
+    SharedPart part[2]; // in tiles; 16 rows at a time
 };
 
-// The steps of a tile of 16 rows: the prefix's, and every text's own.
+constexpr int kMaxTexts = 16; // of a workgroup
+// The steps of a workgroup: the prefix's, and every one of its texts' own.
 template <int kStep>
 struct TextsWalk {
     int steps, prefix_steps, prefix_last;
@@ -45,112 +47,110 @@ struct PartParams {
     static constexpr int window = 0, sinks = 0;
     const void *q;
     void *out;
-    PlaneRef cache_k, cache_v;
     int n_heads, n_kv, max_seq_len, n;
 };
+// Rows of all texts, row i is row i % n of text i / n.
 struct SharedView {
     PartParams p;
     const AttnSharedParams &a;
-    int own; // 0: the prefix in tiles, 1: the rest
-    int prefix_len; // of the rest
     float *ws;
     int pieces, piece_steps, first_slot;
+    __device__ SharedView(const SharedKernelParams &c, int part)
+        : p{c.a.q, c.a.out, c.a.n_heads, c.a.n_kv, c.a.prefix_rows, c.a.n * c.a.n_seqs}, a(c.a), ws(c.ws), pieces(c.slots), piece_steps(c.part[part].piece_steps),
+          first_slot(c.part[part].first_slot) {}
+    __device__ float *partials(int g, int rows, int r, int hd) const { return ws + ((size_t)g * rows + r) * pieces * (hd + 2); }
+};
+// The prefix alone: all rows are at its last position.
+struct PrefixView : SharedView {
+    static constexpr bool kTexts = false;
     bool apart; // results are left for a join whatever the number of pieces
-    // rows of one text of the unit (texts in tiles), or of all (the prefix, and 16 rows at a time)
-    __device__ SharedView(const SharedKernelParams &c, int part, bool one_text)
-        : p{c.a.q, c.a.out, part ? c.a.cache_k : c.a.prefix_k, part ? c.a.cache_v : c.a.prefix_v, c.a.n_heads, c.a.n_kv, part ? c.a.max_seq_len : c.a.prefix_rows,
-            one_text ? c.a.n : c.a.n * c.a.n_seqs},
-          a(c.a), own(part), prefix_len(c.part[0].pieces > 0 ? 0 : c.a.prefix_len), ws(c.ws), pieces(c.slots), piece_steps(c.part[part].piece_steps), first_slot(c.part[part].first_slot),
-          apart(c.part[0].pieces > 0 || c.part[1].tiles) {}
+    __device__ explicit PrefixView(const SharedKernelParams &c) : SharedView(c, 0), apart(c.part[1].pieces > 0) {}
     __device__ bool partial() const { return apart; }
-    __device__ float *partials(int unit, int rows, int r, int hd) const { // a row's place among those of all texts
-        const int b = unit / a.n_kv, g = unit - b * a.n_kv;
-        return ws + ((size_t)g * (a.n_seqs * a.n * (a.n_heads / a.n_kv)) + (size_t)b * rows + r) * pieces * (hd + 2);
-    }
+    __device__ int start(int) const { return a.prefix_len - 1; }
+    __device__ int position(int start, int) const { return start; }
+    __device__ int text(int) const { return 0; }
+    __device__ PlaneRows planes(int g, int, int row) const { return {a.prefix_k, a.prefix_v, (size_t)g * a.prefix_rows + row}; }
 };
-// tiles: all rows of the prefix's part are at its last position
-struct TilesView : SharedView {
-    __device__ TilesView(const SharedKernelParams &c, int part) : SharedView(c, part, part == 1) {}
-    __device__ int start(int b) const { return own ? a.start[b] : a.prefix_len - 1; }
-    __device__ int position(int start, int i) const { return own ? start + i : start; }
-};
-// 16 rows of all texts at a time: row i is row i % n of text i / n
+// The texts' own positions, kPrefix: behind the prefix.
+template <bool kPrefix>
 struct TextsView : SharedView {
     static constexpr bool kTexts = true;
-    __device__ explicit TextsView(const SharedKernelParams &c) : SharedView(c, 1, false) {}
+    __device__ TextsView(const SharedKernelParams &c, int part) : SharedView(c, part) {}
+    __device__ constexpr bool partial() const { return !kPrefix; }
     __device__ int start(int) const { return 0; }
     __device__ int text(int i) const { return i / a.n; }
     __device__ int position(int, int i) const { return a.start[i / a.n] + i % a.n; }
-    __device__ PlaneRows planes(int text, int g, int row) const {
-        if (text < 0) return {a.prefix_k, a.prefix_v, (size_t)g * a.prefix_rows + row};
+    __device__ PlaneRows planes(int g, int text, int row) const {
+        if (kPrefix && text < 0) return {a.prefix_k, a.prefix_v, (size_t)g * a.prefix_rows + row};
         return {a.cache_k, a.cache_v, ((size_t)text * a.n_kv + g) * a.max_seq_len + row};
     }
     template <int kStep>
     __device__ TextsWalk<kStep> walk(int r0, int r1, int lane) const {
         const int group = a.n_heads / a.n_kv, rows = a.n * group;
         TextsWalk<kStep> w;
-        w.prefix_last = prefix_len - 1;
-        w.prefix_steps = (prefix_len + kStep - 1) / kStep;
+        w.prefix_last = a.prefix_len - 1;
+        w.prefix_steps = kPrefix ? (a.prefix_len + kStep - 1) / kStep : 0;
         w.first_text = r0 / rows;
-        const int text = w.first_text + lane; // (16 of them at most)
+        const int text = w.first_text + lane; // (16 of them at most: 16 rows, or 128 of more than 32 for each)
         w.last = text <= r1 / rows ? a.start[min(text, a.n_seqs - 1)] + (min(r1, (text + 1) * rows - 1) - text * rows) / group : -1;
         const int mine = w.last < 0 ? 0 : w.last / kStep + 1;
         int sum = mine;
 #pragma unroll
-        for (int off = 1; off < kAwRows; off <<= 1) {
+        for (int off = 1; off < kMaxTexts; off <<= 1) {
             const int up = __shfl_up(sum, off, kWave);
             if (lane >= off) sum += up;
         }
-        w.first = lane < kAwRows ? w.prefix_steps + sum - mine : INT32_MAX;
-        w.steps = w.prefix_steps + __builtin_amdgcn_readlane(sum, kAwRows - 1);
+        w.first = lane < kMaxTexts ? w.prefix_steps + sum - mine : INT32_MAX;
+        w.steps = w.prefix_steps + __builtin_amdgcn_readlane(sum, kMaxTexts - 1);
         return w;
     }
 };
 
-// kTiles: whether some part takes 128 rows at a time (LDS for it leaves room for one workgroup per compute unit).
-template <typename AC, typename QT, typename CT, int HD, bool kTiles>
-__global__ __launch_bounds__(kAwThreads, kTiles ? 2 : 1) void attn_shared_kernel(SharedKernelParams c) {
-    constexpr int kTilesBytes = kTiles ? TilesShared<HD, 2>::kBytes : 0, kRowsBytes = (int)sizeof(RowsShared<HD>);
+// kForm: what goes through tiles.  (LDS for them leaves room for one workgroup per compute unit.)
+enum SharedForm { kNoTiles, kPrefixTiles, kAllTiles };
+template <typename AC, typename QT, typename CT, int HD, int kForm>
+__global__ __launch_bounds__(kAwThreads, kForm == kNoTiles ? 1 : 2) void attn_shared_kernel(SharedKernelParams c) {
+    constexpr int kTilesBytes = kForm == kNoTiles ? 0 : TilesShared<HD, 2>::kBytes, kRowsBytes = kForm == kAllTiles ? 0 : (int)sizeof(RowsShared<HD>);
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kTilesBytes > kRowsBytes ? kTilesBytes : kRowsBytes];
     __shared__ int wide;
-    // the prefix's tiles first; those of one stretch of keys are a multiple of the number of units apart, on one XCD where that is a multiple of eight
+    // tiles first; those of one stretch of keys are a multiple of the number of heads apart, on one XCD where that is a multiple of eight
     int at = blockIdx.x;
-    const int first = c.part[0].units * c.part[0].blocks * c.part[0].pieces, own = at >= first ? 1 : 0;
+    const int first = kForm == kNoTiles ? 0 : c.a.n_kv * c.part[0].blocks * c.part[0].pieces, own = kForm == kNoTiles || (kForm == kPrefixTiles && at >= first) ? 1 : 0;
     if (own) at -= first;
-    const SharedPart &part = c.part[own];
-    const int unit = at % part.units, rest = at / part.units, block = rest % part.blocks, piece = rest / part.blocks;
-    if constexpr (kTiles) {
-        if (part.tiles) {
-            attn_tiles<CT, HD, 2>(TilesView(c, own), lds, wide, unit, block, piece);
-            return;
-        }
+    const int blocks = c.part[own].blocks, g = at % c.a.n_kv, rest = at / c.a.n_kv, block = rest % blocks, piece = rest / blocks;
+    if constexpr (kForm == kNoTiles) {
+        attn_rows<AC, QT, CT, HD>(TextsView<true>(c, 1), *reinterpret_cast<RowsShared<HD> *>(lds), g, block, piece);
+    } else if constexpr (kForm == kAllTiles) {
+        attn_tiles<CT, HD, 2>(TextsView<true>(c, 0), lds, wide, g, block, piece);
+    } else {
+        if (own) attn_rows<AC, QT, CT, HD>(TextsView<false>(c, 1), *reinterpret_cast<RowsShared<HD> *>(lds), g, block, piece);
+        else attn_tiles<CT, HD, 2>(PrefixView(c), lds, wide, g, block, piece);
     }
-    attn_rows<AC, QT, CT, HD>(TextsView(c), *reinterpret_cast<RowsShared<HD> *>(lds), unit, block, piece);
 }
 
+constexpr int kSharedTile = 128; // positions of a step in tiles
 // Where row r of a key and value head's is, and how many pieces it has.
 struct JoinRow {
     int n_pieces;
-    bool padding;
+    bool padding, finished;
     size_t out;
     __device__ JoinRow(const SharedKernelParams &c, int g, int r, int hd, int step) { // step: positions, of 16 rows at a time
         const AttnSharedParams &a = c.a;
         const int group = a.n_heads / a.n_kv, rows = a.n * group, b = r / rows, own = r - b * rows, i = own / group, start = a.start[b];
         padding = start + i < 0;
         out = ((size_t)(b * a.n + i) * a.n_heads + g * group + (own - i * group)) * hd;
-        int steps; // of the rows that were taken together
-        if (c.part[1].tiles) {
-            const int last = start + (min(rows, (own / kAtRows + 1) * kAtRows) - 1) / group;
-            steps = last < 0 ? 0 : last / 128 + 1;
-        } else {
-            const int r0 = r / kAwRows * kAwRows, r1 = min(a.n_seqs * rows, r0 + kAwRows) - 1;
-            steps = c.part[0].pieces > 0 ? 0 : (a.prefix_len + step - 1) / step;
-            for (int t = r0 / rows; t <= r1 / rows; t++) {
-                const int last = a.start[t] + (min(r1, (t + 1) * rows - 1) - t * rows) / group;
-                steps += last < 0 ? 0 : last / step + 1;
-            }
+        const bool in_tiles = c.part[0].texts;
+        const SharedPart &part = c.part[in_tiles ? 0 : 1];
+        const int together = in_tiles ? kAtRows : kAwRows, r0 = r / together * together, r1 = min(a.n_seqs * rows, r0 + together) - 1;
+        if (in_tiles) step = kSharedTile;
+        int steps = part.prefix ? (a.prefix_len + step - 1) / step : 0;
+        for (int t = r0 / rows; t <= r1 / rows; t++) {
+            const int last = a.start[t] + (min(r1, (t + 1) * rows - 1) - t * rows) / group;
+            steps += last < 0 ? 0 : last / step + 1;
         }
-        n_pieces = c.part[0].pieces + (steps + c.part[1].piece_steps - 1) / c.part[1].piece_steps;
+        n_pieces = (steps + part.piece_steps - 1) / part.piece_steps;
+        finished = n_pieces <= 1 && part.prefix;
+        if (!part.prefix) n_pieces += c.part[0].pieces;
     }
 };
 
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kAjWaves *kWave) void attn_shared_join_kernel(Share
     const int g = blockIdx.y, r = blockIdx.x, all = gridDim.x;
     const JoinRow row(c, g, r, HD, kRowsStep);
     QT *out = reinterpret_cast<QT *>(c.a.out) + row.out;
-    if (c.part[0].pieces == 0 && !c.part[1].tiles && row.n_pieces <= 1) return; // the row is finished
+    if (row.finished) return;
     if (row.padding) {
         if ((int)threadIdx.x < HD) out[threadIdx.x] = (QT)0.0f;
         return;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256) void attn_shared_join_rows_kernel(SharedKernel
     const int g = blockIdx.y, r = blockIdx.x * kRows + (int)threadIdx.x / kLanes, d = ((int)threadIdx.x % kLanes) * 4;
     if (r >= all) return;
     const JoinRow row(c, g, r, HD, kRowsStep);
-    if (c.part[0].pieces == 0 && !c.part[1].tiles && row.n_pieces <= 1) return; // the row is finished
+    if (row.finished) return;
     const float *ws = c.ws + ((size_t)g * all + r) * c.slots * (HD + 2);
     const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
     float M = -INFINITY, L = 0.0f;
@@ -252,102 +252,94 @@ SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
     const int64_t rows = (int64_t)a.n * group, all = rows * a.n_seqs;
     const bool f16 = f16_arithmetic(a), q4 = a.cache == kPlaneQ4;
     const double scale = a.head_dim / 128.0;
-    const double rows_fixed = 3.0, rows_step = (q4 ? 1.6 : 1.2) * scale, tiles_fixed = 7.0, tiles_step = (q4 ? 2.6 : 1.9) * scale;
-    const int step = f16 ? 32 : 16;
-    SharedPart &prefix = c.part[0], &own = c.part[1];
-    prefix.tiles = f16 && all > 2 * kAwRows;
-    own.tiles = f16 && rows > 2 * kAwRows;
-    // steps of the longest, and of all
-    int longest = 0, prefix_steps = 0;
-    int64_t total = 0;
-    if (own.tiles) {
-        own.units = a.n_kv * a.n_seqs;
-        own.blocks = (int)((rows + kAtRows - 1) / kAtRows);
-        for (int b = 0; b < a.n_seqs; b++) {
-            const int steps = (std::max(0, a.start[b] + a.n) + 127) / 128;
-            longest = std::max(longest, steps);
-            total += (int64_t)steps * own.blocks;
-        }
-    } else {
-        own.units = a.n_kv;
-        own.blocks = (int)((all + kAwRows - 1) / kAwRows);
-        const int first = prefix.tiles ? 0 : (a.prefix_len + step - 1) / step;
-        for (int t = 0; t < own.blocks; t++) {
-            const int64_t r0 = (int64_t)t * kAwRows, r1 = std::min(all, r0 + kAwRows) - 1;
+    const double fixed[2] = {7.0, 3.0}, per_step[2] = {(q4 ? 2.6 : 1.9) * scale, (q4 ? 1.6 : 1.2) * scale};
+    const int step[2] = {kSharedTile, f16 ? 32 : 16}, together[2] = {kAtRows, kAwRows};
+    // which parts there are, and what they have
+    const bool texts_tiles = f16 && rows > 2 * kAwRows, tiles = texts_tiles || (f16 && all > 2 * kAwRows && a.prefix_len > 0);
+    c.part[0].prefix = tiles;
+    c.part[0].texts = texts_tiles;
+    c.part[1].prefix = !tiles;
+    c.part[1].texts = !texts_tiles;
+    int longest[2] = {0, 0}; // steps of a workgroup
+    double mean[2] = {0.0, 0.0};
+    for (int k = 0; k < 2; k++) {
+        SharedPart &p = c.part[k];
+        if (!p.prefix && !p.texts) continue;
+        p.blocks = (int)((all + together[k] - 1) / together[k]);
+        const int first = p.prefix ? (a.prefix_len + step[k] - 1) / step[k] : 0;
+        longest[k] = first;
+        mean[k] = first;
+        for (int t = 0; p.texts && t < p.blocks; t++) {
+            const int64_t r0 = (int64_t)t * together[k], r1 = std::min(all, r0 + together[k]) - 1;
             int steps = first;
-            for (int64_t b = r0 / rows; b <= r1 / rows; b++) steps += (std::max(0, a.start[b] + a.n) + step - 1) / step;
-            longest = std::max(longest, steps);
-            total += steps;
+            for (int64_t b = r0 / rows; b <= r1 / rows; b++) {
+                const int64_t last = a.start[b] + (std::min(r1, (b + 1) * rows - 1) - b * rows) / group;
+                steps += last < 0 ? 0 : (int)(last / step[k]) + 1;
+            }
+            longest[k] = std::max(longest[k], steps);
+            mean[k] += (double)(steps - first) / p.blocks;
         }
     }
-    if (prefix.tiles) {
-        prefix.units = a.n_kv;
-        prefix.blocks = (int)((all + kAtRows - 1) / kAtRows);
-        prefix_steps = (a.prefix_len + 127) / 128;
-    }
-    const bool tiles = prefix_steps > 0 || own.tiles;
     const int places = compute_units * (a.head_dim == 128 || tiles ? 1 : 2); // (registers, and LDS of tiles)
-    const double mean = longest > 0 ? (double)total / own.blocks / (own.tiles ? a.n_seqs : 1) : 0.0;
-    const int most_own = std::min(own.tiles ? 16 : kMaxPieces * 3 / 4, (longest + (own.tiles ? 0 : kAwWaves - 1)) / (own.tiles ? 1 : kAwWaves));
-    double least = 0.0;
+    const int most[2] = {std::min(kMaxPieces / 2, longest[0]), std::min(kMaxPieces / 2, (longest[1] + kAwWaves - 1) / kAwWaves)};
+    double least = -1.0;
     int pieces[2] = {0, 0};
-    for (int n0 = prefix_steps > 0 ? 1 : 0; n0 <= std::min(kMaxPieces / 2, prefix_steps); n0 += 1 + n0 / 4) {
-        for (int n1 = longest > 0 ? 1 : 0; n1 <= std::min(most_own, kMaxPieces - n0); n1 += 1 + n1 / 4) {
-            const double part = n1 > 0 ? std::min((double)((longest + n1 - 1) / n1), mean) : 0.0; // steps of an average workgroup
-            const double us[2] = {tiles_fixed + (n0 > 0 ? (prefix_steps + n0 - 1) / n0 : 0) * tiles_step,
-                                  own.tiles ? tiles_fixed + part * tiles_step : rows_fixed + (double)(((int64_t)part + kAwWaves - 1) / kAwWaves) * rows_step};
-            const int64_t count[2] = {(int64_t)prefix.units * prefix.blocks * n0, (int64_t)own.units * own.blocks * n1};
-            const bool join = n0 > 0 || own.tiles || n1 > 1;
+    for (int n0 = std::min(1, most[0]); n0 <= most[0]; n0 += 1 + n0 / 4) {
+        for (int n1 = std::min(1, most[1]); n1 <= most[1]; n1 += 1 + n1 / 4) {
+            const int n[2] = {n0, n1};
+            double us[2];
+            int64_t count[2];
+            for (int k = 0; k < 2; k++) { // of an average workgroup
+                const double part = n[k] > 0 ? std::min((double)((longest[k] + n[k] - 1) / n[k]), mean[k]) : 0.0;
+                us[k] = fixed[k] + (k ? (double)(((int64_t)part + kAwWaves - 1) / kAwWaves) : part) * per_step[k];
+                count[k] = (int64_t)a.n_kv * c.part[k].blocks * n[k];
+            }
+            const bool join = n0 + n1 > 1;
             const double end = makespan(places, count, us) + (join ? 3.0 + (double)all * a.n_kv * (n0 + n1) * (a.head_dim + 2) * 8 / 4.5e6 : 0.0);
-            if ((pieces[0] == 0 && pieces[1] == 0) || end < least) {
+            if (least < 0.0 || end < least) {
                 least = end;
                 pieces[0] = n0;
                 pieces[1] = n1;
             }
-            if (longest == 0) break;
+            if (most[1] == 0) break;
         }
-        if (prefix_steps == 0) break;
+        if (most[0] == 0) break;
     }
-    const int steps[2] = {prefix_steps, longest};
     for (int k = 0; k < 2; k++) {
         SharedPart &p = c.part[k];
-        p.piece_steps = pieces[k] > 0 ? (steps[k] + pieces[k] - 1) / pieces[k] : 1;
-        p.pieces = steps[k] > 0 ? (steps[k] + p.piece_steps - 1) / p.piece_steps : 0;
+        p.piece_steps = pieces[k] > 0 ? (longest[k] + pieces[k] - 1) / pieces[k] : 1;
+        if (k && pieces[k] > 1) p.piece_steps = (p.piece_steps + kAwWaves - 1) / kAwWaves * kAwWaves; // (a step for every wavefront: eight texts' drafts in f32 22.7 -> 21.2 us)
+        p.pieces = (longest[k] + p.piece_steps - 1) / p.piece_steps;
+        if (p.prefix && p.texts) p.pieces = std::max(1, p.pieces); // (nothing but padding: zeros)
         p.first_slot = k ? c.part[0].pieces : 0;
+        c.slots += p.pieces;
+        c.workgroups += (int64_t)a.n_kv * p.blocks * p.pieces;
     }
-    if (prefix.pieces == 0 && !own.tiles) own.pieces = std::max(1, own.pieces); // (nothing but padding: zeros)
-    c.joined = prefix.pieces > 0 || own.tiles || own.pieces > 1;
-    c.slots = std::max(1, prefix.pieces + own.pieces);
+    c.joined = c.slots > 1;
     c.work_floats = c.joined ? (size_t)all * a.n_kv * c.slots * (a.head_dim + 2) : 0;
-    for (const SharedPart &p : c.part) c.workgroups += (int64_t)p.units * p.blocks * p.pieces;
     return c;
 }
 
 template <typename AC, typename QT, typename CT, int HD>
-static void launch_shared(const SharedKernelParams &c, bool joined, hipStream_t s) {
-    int64_t n = 0;
-    for (const SharedPart &p : c.part) n += (int64_t)p.units * p.blocks * p.pieces;
-    if (n > 0) { // (texts in tiles, and nothing but padding: the join's zeros)
-        const dim3 grid((unsigned)n), block(kAwThreads);
-        bool tiles = false;
-        if constexpr (std::is_same_v<AC, half_t>) {
-            tiles = (c.part[0].tiles && c.part[0].pieces > 0) || (c.part[1].tiles && c.part[1].pieces > 0);
-            if (tiles) hipLaunchKernelGGL((attn_shared_kernel<AC, QT, CT, HD, true>), grid, block, 0, s, c);
-        }
-        if (!tiles) hipLaunchKernelGGL((attn_shared_kernel<AC, QT, CT, HD, false>), grid, block, 0, s, c);
+static void launch_shared(const SharedKernelParams &c, const SharedPlan &plan, hipStream_t s) {
+    const dim3 grid((unsigned)plan.workgroups), block(kAwThreads);
+    if constexpr (std::is_same_v<AC, half_t>) {
+        if (c.part[0].texts) hipLaunchKernelGGL((attn_shared_kernel<AC, QT, CT, HD, kAllTiles>), grid, block, 0, s, c);
+        else if (c.part[0].prefix) hipLaunchKernelGGL((attn_shared_kernel<AC, QT, CT, HD, kPrefixTiles>), grid, block, 0, s, c);
     }
-    if (!joined) return;
+    if (!c.part[0].prefix) hipLaunchKernelGGL((attn_shared_kernel<AC, QT, CT, HD, kNoTiles>), grid, block, 0, s, c);
+    if (!plan.joined) return;
     const unsigned rows = (unsigned)(c.a.n * c.a.n_seqs * (c.a.n_heads / c.a.n_kv)), per = 256 / (HD / 4);
     constexpr int kStep = Step<AC, CT, HD>::kPositions;
     if ((int64_t)rows * c.a.n_kv <= 1024) hipLaunchKernelGGL((attn_shared_join_kernel<QT, HD, kStep>), dim3(rows, (unsigned)c.a.n_kv), dim3(kAjWaves * kWave), 0, s, c);
     else hipLaunchKernelGGL((attn_shared_join_rows_kernel<QT, HD, kStep>), dim3((rows + per - 1) / per, (unsigned)c.a.n_kv), dim3(256), 0, s, c, (int)rows);
 }
 template <typename AC, typename QT, typename CT>
-static hipError_t launch_hd(const SharedKernelParams &c, bool joined, hipStream_t s) {
+static hipError_t launch_hd(const SharedKernelParams &c, const SharedPlan &plan, hipStream_t s) {
     switch (c.a.head_dim) {
-    case 32: launch_shared<AC, QT, CT, 32>(c, joined, s); break;
-    case 64: launch_shared<AC, QT, CT, 64>(c, joined, s); break;
-    case 128: launch_shared<AC, QT, CT, 128>(c, joined, s); break;
+    case 32: launch_shared<AC, QT, CT, 32>(c, plan, s); break;
+    case 64: launch_shared<AC, QT, CT, 64>(c, plan, s); break;
+    case 128: launch_shared<AC, QT, CT, 128>(c, plan, s); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
@@ -356,12 +348,12 @@ static hipError_t launch_hd(const SharedKernelParams &c, bool joined, hipStream_
 hipError_t launch_attn_shared(const AttnSharedParams &a, const SharedPlan &plan, float *ws, hipStream_t s) {
     SharedKernelParams c{a, ws, plan.slots, {plan.part[0], plan.part[1]}};
     switch (a.cache * 2 + a.f16) {
-    case kPlaneF16 * 2: return launch_hd<float, float, half_t>(c, plan.joined, s);
-    case kPlaneF16 * 2 + 1: return launch_hd<half_t, half_t, half_t>(c, plan.joined, s);
-    case kPlaneF32 * 2: return launch_hd<float, float, float>(c, plan.joined, s);
-    case kPlaneF32 * 2 + 1: return launch_hd<float, half_t, float>(c, plan.joined, s);
-    case kPlaneQ4 * 2: return launch_hd<float, float, Quant4>(c, plan.joined, s);
-    case kPlaneQ4 * 2 + 1: return launch_hd<half_t, half_t, Quant4>(c, plan.joined, s);
+    case kPlaneF16 * 2: return launch_hd<float, float, half_t>(c, plan, s);
+    case kPlaneF16 * 2 + 1: return launch_hd<half_t, half_t, half_t>(c, plan, s);
+    case kPlaneF32 * 2: return launch_hd<float, float, float>(c, plan, s);
+    case kPlaneF32 * 2 + 1: return launch_hd<float, half_t, float>(c, plan, s);
+    case kPlaneQ4 * 2: return launch_hd<float, float, Quant4>(c, plan, s);
+    case kPlaneQ4 * 2 + 1: return launch_hd<half_t, half_t, Quant4>(c, plan, s);
     default: return hipErrorInvalidValue;
     }
 }

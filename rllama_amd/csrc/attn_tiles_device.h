@@ -56,7 +56,8 @@ struct TilesShared {
     static constexpr int kBytes = 4 * kTileBytes > kEndBytes ? 4 * kTileBytes : kEndBytes;
 };
 
-// Row block `block` (128 rows) of unit b * n_kv + g, piece `piece` of their positions.  View: see attn_window_device.h.
+// Row block `block` (128 rows) of unit b * n_kv + g, piece `piece` of their positions.  View: see attn_window_device.h; View::kTexts: the unit is a key and value head, its
+// rows are those of all texts, and the tiles are the shared prefix's and then those of every text's own positions, which that text's rows see.
 template <typename CT, int HD, int kShares, typename View>
 __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, int &sh_wide, int unit, int block, int piece) {
     constexpr bool kQ4 = std::is_same_v<CT, Quant4>;
@@ -74,16 +75,17 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int rg = wave % kAtGroups, kh = wave / kAtGroups; // row group, half of the keys
-    const int b = unit / p.n_kv, g = unit - b * p.n_kv;
+    const int b = View::kTexts ? 0 : unit / p.n_kv, g = unit - b * p.n_kv;
     const int group = p.n_heads / p.n_kv, rows = p.n * group, start = v.start(b);
     const int r0 = block * kRows, r1 = min(rows, r0 + kRows) - 1;
-    const int p0 = max(0, v.position(start, r0 / group)), p1 = v.position(start, r1 / group);
+    const int p0 = max(0, v.position(start, r0 / group)), p1 = v.position(start, r1 / group); // (kTexts: these and the next two are not used)
     // this wavefront's rows, and this lane's
     const int w0 = r0 + rg * 32, w1 = min(r1, w0 + 31);
-    const int wp0 = v.position(start, w0 / group), wp1 = w1 < w0 ? -1 : v.position(start, w1 / group);
+    const int wp0 = v.position(start, View::kTexts ? 0 : w0 / group), wp1 = w1 < w0 ? -1 : v.position(start, w1 / group);
     const int my_r = min(w0 + col, r1), my_i = my_r / group;
     const int my_p = w0 + col <= r1 ? v.position(start, my_i) : -1;
     const int my_low = p.window > 0 ? max(0, my_p - p.window + 1) : 0;
+    const int my_text = w0 + col <= r1 ? v.text(my_i) : -1, first_text = v.text(min(w0, r1) / group), last_text = v.text(w1 / group); // this lane's, this wavefront's
     const half_t *q_row = reinterpret_cast<const half_t *>(p.q) + ((size_t)(b * p.n + my_i) * p.n_heads + g * group + (my_r - my_i * group)) * HD;
 
     // q as the second operand: lane supplies dims 16 ks + 8 half .. + 7, in the order of the converted codes where the cache has 4 bits
@@ -101,25 +103,38 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
         for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
     float m_run = -INFINITY, l_run = 0.0f;
 
-    Span span = span_of<kAtKeys>(p0, p1, p.window, p.sinks, p.max_seq_len);
-    if (p1 < 0) span.steps = 0;
+    auto span = [&] {
+        if constexpr (View::kTexts) {
+            return v.template walk<kAtKeys>(r0, r1, lane);
+        } else {
+            Span s = span_of<kAtKeys>(p0, p1, p.window, p.sinks, p.max_seq_len);
+            if (p1 < 0) s.steps = 0;
+            return s;
+        }
+    }();
     // (texts are cut into pieces with two wavefronts per row group only)
     const int n_pieces = kShares > 1 ? (span.steps + v.piece_steps - 1) / v.piece_steps : 1;
     if (piece >= max(1, n_pieces)) return;
     const int s_first = kShares > 1 ? piece * v.piece_steps : 0, s_end = kShares > 1 ? min(span.steps, s_first + v.piece_steps) : span.steps;
-    const size_t plane = (size_t)unit * p.max_seq_len;
     const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
     const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
 
     struct Place {
         int t0, last, row;
         bool front;
+        int text = -1; // kTexts: whose positions they are; the prefix's: -1
     };
     auto place_of = [&](int s) {
-        if (s < span.steps0) return Place{s * kAtKeys, span.first_end - 1, s * kAtKeys, true};
-        if (s < span.steps1) return Place{span.low + (s - span.steps0) * kAtKeys, span.turn - 1, span.row + (s - span.steps0) * kAtKeys, false};
-        return Place{span.turn + (s - span.steps1) * kAtKeys, span.last, p.sinks + (s - span.steps1) * kAtKeys, false};
+        if constexpr (View::kTexts) {
+            const auto at = span.at(s);
+            return Place{at.t0, at.last, at.t0, false, at.text};
+        } else {
+            if (s < span.steps0) return Place{s * kAtKeys, span.first_end - 1, s * kAtKeys, true};
+            if (s < span.steps1) return Place{span.low + (s - span.steps0) * kAtKeys, span.turn - 1, span.row + (s - span.steps0) * kAtKeys, false};
+            return Place{span.turn + (s - span.steps1) * kAtKeys, span.last, p.sinks + (s - span.steps1) * kAtKeys, false};
+        }
     };
+    auto planes_of = [&](const Place &at) { return v.planes(unit, at.text, at.row); };
     auto k_swz = [](int row) { return kPieces >= 16 ? row & 15 : (row / (16 / kPieces)) & (kPieces - 1); };
     auto v_swz = [](int row) { return HD == 128 ? (row & 3) * 4 : HD == 64 ? ((row >> 1) & 1) * 4 : 0; }; // in pieces
 
@@ -131,11 +146,12 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
     const int my_row = (wave * 64 + lane) / kPieces, my_piece = lane % kPieces;
     const unsigned k_from = (my_piece ^ k_swz(my_row)) << 4, v_from = (my_piece ^ v_swz(my_row)) << 4; // within the row
     uint32_t codes[kQ4 ? kItems : 1][4], pairs[kQ4 ? kItems : 1];
-    // `here` rows from plane row `row` on: f16 on their way to a stage, codes on their way to registers
-    auto fetch = [&](size_t row, int here, unsigned stage) __attribute__((always_inline)) {
+    // `here` rows: f16 on their way to a stage, codes on their way to registers
+    auto fetch = [&](const PlaneRows &planes, int here, unsigned stage) __attribute__((always_inline)) {
+        const size_t row = planes.row;
         if constexpr (kQ4) {
-            const buffer_t k = buffer_of(p.cache_k.data, row * (HD / 2), here * (HD / 2)), kp = buffer_of(p.cache_k.pairs, row * (HD / 8), here * (HD / 8));
-            const buffer_t v = buffer_of(p.cache_v.data, row * (HD / 2), here * (HD / 2)), vp = buffer_of(p.cache_v.pairs, row * (HD / 8), here * (HD / 8));
+            const buffer_t k = buffer_of(planes.k.data, row * (HD / 2), here * (HD / 2)), kp = buffer_of(planes.k.pairs, row * (HD / 8), here * (HD / 8));
+            const buffer_t v = buffer_of(planes.v.data, row * (HD / 2), here * (HD / 2)), vp = buffer_of(planes.v.pairs, row * (HD / 8), here * (HD / 8));
 #pragma unroll
             for (int i = 0; i < kItems; i++) {
                 const int item = i * 64 * kWaves + tid, at_group = item % (kGroups / 2); // row at_group / (HD / 32), group at_group % (HD / 32)
@@ -146,7 +162,7 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
                 pairs[i] = is_v ? __builtin_amdgcn_raw_buffer_load_b32(vp, at_group * 4, 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(kp, at_group * 4, 0, 0);
             }
         } else {
-            const half_t *k = reinterpret_cast<const half_t *>(p.cache_k.data) + row * HD, *v = reinterpret_cast<const half_t *>(p.cache_v.data) + row * HD;
+            const half_t *k = reinterpret_cast<const half_t *>(planes.k.data) + row * HD, *v = reinterpret_cast<const half_t *>(planes.v.data) + row * HD;
 #pragma unroll
             for (int i = 0; i < kIssues; i++) {
                 const unsigned from = (unsigned)min(my_row + i * kIssueRows, here - 1) * kRowBytes; // keys past the last one are masked below
@@ -181,14 +197,24 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
         }
     };
 
-    auto sees = [&](int at, int last) { return (bool)((int)(at <= min(my_p, last)) & ((int)(at >= my_low) | (int)(at < p.sinks))); };
+    // the last position of a place that this lane's row may see
+    auto limit_of = [&](const Place &at) {
+        if constexpr (View::kTexts) return at.text < 0 ? at.last : at.text == my_text ? min(my_p, at.last) : -1;
+        else return min(my_p, at.last);
+    };
+    auto sees = [&](int at, int limit) { return (bool)((int)(at <= limit) & ((int)(at >= my_low) | (int)(at < p.sinks))); };
+    auto whole_to = [&](const Place &at) { // up to which every row of the wavefront sees a place
+        if constexpr (View::kTexts) return at.text < 0 ? at.last : -1;
+        else return min(at.last, max(0, wp0));
+    };
     // of this wavefront's half of a tile: every row that is no padding sees all of it / none sees any of it
     auto whole_half = [&](const Place &at) {
         const int t0 = at.t0 + kh * 64;
-        return t0 + 63 <= min(at.last, max(0, wp0)) && (at.front || p.window == 0 || t0 > wp1 - p.window);
+        return t0 + 63 <= whole_to(at) && (at.front || p.window == 0 || t0 > wp1 - p.window);
     };
     auto unseen_half = [&](const Place &at) {
         const int t0 = at.t0 + kh * 64, end = min(at.last, t0 + 63);
+        if constexpr (View::kTexts) return t0 > at.last || (at.text >= 0 && (at.text < first_text || at.text > last_text));
         return t0 > min(wp1, at.last) || (p.window > 0 && !at.front && end <= max(0, wp0) - p.window && t0 >= p.sinks);
     };
     bool skipped = false;
@@ -197,7 +223,7 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
     const int v_row = half * 4 + ((lane & 15) >> 2);               // of the first run of four keys; the second one is 8 further
     const int v_piece = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1); // + 4 d
     // fetch_more(ks): f16: called beside every step of the first product (all loads at once hold a wavefront up for 400 cycles); 4 bits: once behind it
-    auto work = [&](unsigned stage, int t0, int last, auto whole, auto fetch_more) __attribute__((always_inline)) {
+    auto work = [&](unsigned stage, int t0, int limit, auto whole, auto fetch_more) __attribute__((always_inline)) {
         const unsigned char *lds_k = lds + stage * kStageBytes + kh * (64 * kRowBytes), *lds_v = lds_k + kTileBytes;
         // S^T: the two 32-key products side by side, K read three steps ahead of them.  (Barriers against reordering: left alone, every read ends up right in
         // front of its product, and its latency in between.)
@@ -243,7 +269,7 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (!decltype(whole)::value) { // a bit per key of the tile (what sees() says of each), and a select by it
             auto ones = [](int n) { return n <= 0 ? 0ull : ~0ull >> (64 - min(n, 64)); };
-            const uint64_t seen = (ones(min(my_p, last) - t0 + 1) & (~ones(my_low - t0) | ones(p.sinks - t0))) >> (half * 4);
+            const uint64_t seen = (ones(limit - t0 + 1) & (~ones(my_low - t0) | ones(p.sinks - t0))) >> (half * 4);
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -303,7 +329,7 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
         Place at = place_of(s_first), ahead = at; // `ahead`: the tile after the one fetched last
         auto fetch_ahead = [&](int s) __attribute__((always_inline)) {
             if (s >= s_end) return;
-            fetch(plane + ahead.row, min(kAtKeys, ahead.last - ahead.t0 + 1), (unsigned)(s - s_first) & 1);
+            fetch(planes_of(ahead), min(kAtKeys, ahead.last - ahead.t0 + 1), (unsigned)(s - s_first) & 1);
             ahead.t0 += kAtKeys;
             ahead.row += kAtKeys;
             if (ahead.t0 > ahead.last) ahead = place_of(s + 1);
@@ -315,7 +341,7 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
         for (int s = s_first; s < s_end; s++) {
             // tiles from here on that every row sees whole and that another tile (f16: a whole one) follows in the same run of rows (wavefronts may count
             // differently: both loops stage and wait alike)
-            const int seen = min(at.last, max(0, wp0)) - kh * 64 - 63 - at.t0, follow = at.last + 1 - at.t0;
+            const int seen = whole_to(at) - kh * 64 - 63 - at.t0, follow = at.last + 1 - at.t0;
             int run = whole_half(at) ? min(min(seen / kAtKeys + 1, (kQ4 ? (follow + kAtKeys - 1) / kAtKeys : follow / kAtKeys) - 1), s_end - 1 - s) : 0;
             if (run > 0) {
                 const int end = s + run;
@@ -324,7 +350,8 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
                     ahead.row = at.row + (run + 1) * kAtKeys;
                     if (ahead.t0 > ahead.last) ahead = place_of(end + 1);
                 }
-                size_t row = plane + at.row + kAtKeys;
+                const PlaneRows planes = planes_of(at);
+                size_t row = planes.row + kAtKeys;
                 at.t0 += run * kAtKeys;
                 at.row += run * kAtKeys;
                 do {
@@ -333,7 +360,7 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
                     work(stage, 0, 0, std::true_type{}, [&](int ks) __attribute__((always_inline)) {
                         if constexpr (kQ4) fetch_ahead(s + 2);
                         else {
-                            const half_t *from = reinterpret_cast<const half_t *>(ks < kIssues ? p.cache_k.data : p.cache_v.data) + row * HD;
+                            const half_t *from = reinterpret_cast<const half_t *>(ks < kIssues ? planes.k.data : planes.v.data) + row * HD;
                             const int i = ks % kIssues;
                             dma16_base(from, (unsigned)(my_row + i * kIssueRows) * kRowBytes + (ks < kIssues ? k_from : v_from),
                                        lds_base + (1 - stage) * kStageBytes + (unsigned)(i * kWaves + wave) * 1024u + (ks < kIssues ? 0 : kTileBytes));
@@ -364,7 +391,7 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
                 }
             }
             if (use) {
-                work(stage, at.t0 + kh * 64, at.last, std::false_type{}, [&](int) __attribute__((always_inline)) { if constexpr (kQ4) fetch_ahead(s + 2); });
+                work(stage, at.t0 + kh * 64, limit_of(at), std::false_type{}, [&](int) __attribute__((always_inline)) { if constexpr (kQ4) fetch_ahead(s + 2); });
             } else if constexpr (kQ4) {
                 place(1 - stage); // (behind the last tile: into a stage that is read no more)
                 fetch_ahead(s + 2);
@@ -398,11 +425,12 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
         for (int s = s_first; s < s_end; s++) {
             const Place at = place_of(s);
             if (unseen_half(at) || (!anew && whole_half(at))) continue;
-            const int t0 = at.t0 + kh * 64, here = min(64, at.last - t0 + 1);
-            const size_t row = plane + at.row + kh * 64;
+            const int t0 = at.t0 + kh * 64, here = min(64, at.last - t0 + 1), limit = limit_of(at);
+            const PlaneRows planes = planes_of(at);
+            const size_t row = planes.row + kh * 64;
             if (!anew) {
                 bool odd = false;
-                for (int i = lane; i < here * HD; i += 64) odd |= !(fabsf(plane_load1<CT>(p.cache_v, row * HD + i)) < INFINITY);
+                for (int i = lane; i < here * HD; i += 64) odd |= !(fabsf(plane_load1<CT>(planes.v, row * HD + i)) < INFINITY);
                 if (!__any(odd)) continue;
             }
 #pragma unroll 1
@@ -410,9 +438,9 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
                 const size_t from = (row + j) * HD;
                 float dot = 0.0f;
 #pragma unroll 1
-                for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d++) dot = fmaf((float)q_row[d], plane_load1<CT>(p.cache_k, from + d), dot);
+                for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d++) dot = fmaf((float)q_row[d], plane_load1<CT>(planes.k, from + d), dot);
                 dot += __shfl_xor(dot, 32, 64);
-                const bool seen = sees(t0 + j, at.last);
+                const bool seen = sees(t0 + j, limit);
                 const float m_new = seen ? fmaxf(m_run, dot) : m_run;
                 const float alpha = m_new > -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * c2) : 1.0f;
                 const float wt = seen ? __builtin_amdgcn_exp2f(fmaf(dot - (m_new > -INFINITY ? m_new : 0.0f), c2, kWeightLift)) : 0.0f;
@@ -423,7 +451,7 @@ __device__ __forceinline__ void attn_tiles(const View &v, unsigned char *lds, in
 #pragma unroll
                     for (int v = 0; v < 16; v++) {
                         const int dim8 = (v >> 2) * 8, in8 = half * 4 + (v & 3); // place in O^T
-                        const float x = plane_load1<CT>(p.cache_v, from + d * 32 + dim8 + (kQ4 ? (in8 >> 1) + 4 * (in8 & 1) : in8));
+                        const float x = plane_load1<CT>(planes.v, from + d * 32 + dim8 + (kQ4 ? (in8 >> 1) + 4 * (in8 & 1) : in8));
                         o[d][v] = seen ? fmaf(wt, x, o[d][v] * alpha) : o[d][v];
                     }
             }

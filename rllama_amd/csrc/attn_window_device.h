@@ -88,6 +88,11 @@ struct AttnCutParams {
     int pieces, piece_steps; // pieces of `piece_steps` steps, at most `pieces` of them
 };
 constexpr int kMaxPieces = 64;
+// Rows of K and V planes from `row` on.
+struct PlaneRows {
+    PlaneRef k, v;
+    size_t row;
+};
 // How the kernels see a call of rlh_attn_window: its parameters, the position of a sequence's row i, and where a row's partial results go.  rlh_attn_shared has another one.
 struct WindowView {
     static constexpr bool kTexts = false; // see attn_rows_device.h
@@ -100,12 +105,8 @@ struct WindowView {
     __device__ int position(int start, int i) const { return start + i; }
     __device__ constexpr bool partial() const { return false; } // whether results are left for a join whatever the number of pieces
     __device__ int text(int) const { return 0; }
+    __device__ PlaneRows planes(int unit, int, int row) const { return {p.cache_k, p.cache_v, (size_t)unit * p.max_seq_len + row}; }
     __device__ float *partials(int unit, int rows, int r, int hd) const { return ws + ((size_t)unit * rows + r) * pieces * (hd + 2); }
-};
-// Rows of K and V planes from `row` on.
-struct PlaneRows {
-    PlaneRef k, v;
-    size_t row;
 };
 
 // Joins the pieces of rows: weights exp(m_s - M) of all pieces of a row at once (a lane each), then the sums, added up in the same order whatever

@@ -1,5 +1,7 @@
 """The operators for many answers to one prompt against their definitions in 64 bits: tensors and products of 8 bits, attention behind a shared prefix, log
 probabilities of tokens; their special rows (padding, NaN in what nobody sees, masks, ties), their refusals, and a step of them together."""
+import warnings
+
 import numpy as np
 import pytest
 
@@ -186,6 +188,9 @@ SHARED = [
     (128, 16, 2, 1, 30, 30, 3000, [2990, 1, 1500]),          # own texts much longer than the prefix
     (128, 5, 1, 60, 2107, 2107, 64, [0] * 6),
     (64, 1, 1, 1, 64, 64, 64, [63] * 256),
+    (64, 6, 2, 11, 200, 210, 150, [130, 0, -3, 64, 7, -11, 100, 139, 1, 55]),  # up to five texts in a block of 128 rows
+    (128, 4, 1, 10, 0, 0, 300, [290, 0, 100, -5, 17, 200]),
+    (128, 10, 2, 61, 700, 700, 61, [0] * 6),
 ]
 
 
@@ -252,6 +257,15 @@ def test_attention_behind_a_shared_prefix(ctx, hd, H, G, n, P, rows, S, starts, 
     assert np.array_equal(Q.attn_shared(*args).to_numpy(), out)
 
 
+@pytest.mark.parametrize("kind,cache", TYPES)
+@pytest.mark.parametrize("hd,n,P,starts", [(32, 40, 256, [-40, -40, -99]), (32, 2, 256, [-2, -9]), (64, 1, 0, [-2] * 40), (128, 50, 0, [-50]), (128, 1, 500, [-1] * 40), (64, 1, 0, [-1])])
+def test_nothing_but_padding(ctx, kind, cache, hd, n, P, starts):
+    with np.errstate(all="ignore"), warnings.catch_warnings():
+        warnings.simplefilter("ignore")  # (no position is seen, and all of them are NaN)
+        out = shared_case(ctx, hd, 4, 4, n, P, P, 40, starts, kind, cache)[0]
+    assert (out == 0).all()
+
+
 @pytest.mark.parametrize("P", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 511, 513, 1023, 1025, 3000])
 @pytest.mark.parametrize("kind,cache,B", [("f16", "f16", 1), ("f16", "f16", 20), ("f16", "q4", 5), ("f32", "f32", 3)])
 def test_prefixes_of_every_length(ctx, P, kind, cache, B):
@@ -260,7 +274,7 @@ def test_prefixes_of_every_length(ctx, P, kind, cache, B):
 
 
 @pytest.mark.parametrize("kind", ["f16", "f32"])
-@pytest.mark.parametrize("n,B", [(1, 3), (1, 40), (20, 5)])
+@pytest.mark.parametrize("n,B", [(1, 3), (1, 40), (20, 5), (70, 4)])
 def test_scores_far_apart(ctx, kind, n, B):
     """Scores of several hundred, rising and falling along prefix and text: the running maximum moves all the time, weights underflow, and one of the two parts may hold all of it."""
     rng = np.random.default_rng(9)
@@ -286,7 +300,7 @@ def test_scores_far_apart(ctx, kind, n, B):
 
 
 @pytest.mark.parametrize("kind,cache", [("f16", "f16"), ("f16", "q4"), ("f32", "f32"), ("f32", "q4")])
-@pytest.mark.parametrize("B,n,group", [(3, 1, 2), (30, 1, 4), (4, 20, 1), (12, 7, 3)])
+@pytest.mark.parametrize("B,n,group", [(3, 1, 2), (30, 1, 4), (4, 20, 1), (12, 7, 3), (5, 20, 2), (3, 34, 4)])
 @pytest.mark.parametrize("value", [np.nan, np.inf])
 def test_values_that_are_not_finite_reach_the_rows_that_see_them(ctx, kind, cache, B, n, group, value):
     G, hd, P, S = 2, 32, 150, 64

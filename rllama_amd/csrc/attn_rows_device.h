@@ -512,7 +512,7 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
     l_run = col_sum(l_run);
     if (h == 0) {
         sm[wave][m] = m_run * queries.up;
-        sl[wave][m] = l_run;
+        sl[wave][m] = my_p < 0 ? 0.0f : l_run; // (padding: 0)
     }
 #pragma unroll
     for (int x = 0; x < 4; x++)
@@ -538,7 +538,6 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
         for (int i = 0; i < kPer; i++) O[i] = fmaf(so[w][jr][jd + i], f, O[i]);
     }
     const int jri = min(r0 + jr, r1) / group;
-    if (v.position(start, jri) < 0) L = 0.0f; // padding
     QT *out = reinterpret_cast<QT *>(p.out) + ((size_t)(b * p.n + jri) * p.n_heads + g * group + (r0 + jr - jri * group)) * HD + jd;
     if (!v.partial() && n_pieces <= 1) {
         if (mine) {

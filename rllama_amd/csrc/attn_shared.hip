@@ -26,7 +26,7 @@ struct SharedKernelParams {
     SharedPart part[2]; // in tiles; 16 rows at a time
 };
 
-constexpr int kMaxTexts = 16; // of a workgroup
+constexpr int kMaxTexts = 16; // of a workgroup; a row of lanes
 // The steps of a workgroup: the prefix's, and every one of its texts' own.
 template <int kStep>
 struct TextsWalk {
@@ -94,12 +94,11 @@ struct TextsView : SharedView {
         const int text = w.first_text + lane; // (16 of them at most: 16 rows, or 128 of more than 32 for each)
         w.last = text <= r1 / rows ? a.start[min(text, a.n_seqs - 1)] + (min(r1, (text + 1) * rows - 1) - text * rows) / group : -1;
         const int mine = w.last < 0 ? 0 : w.last / kStep + 1;
-        int sum = mine;
-#pragma unroll
-        for (int off = 1; off < kMaxTexts; off <<= 1) {
-            const int up = __shfl_up(sum, off, kWave);
-            if (lane >= off) sum += up;
-        }
+        int sum = mine; // of the lanes up to this one
+        sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xf, 0xf, true); // (row_shr: from so many lanes below)
+        sum += __builtin_amdgcn_update_dpp(0, sum, 0x112, 0xf, 0xf, true);
+        sum += __builtin_amdgcn_update_dpp(0, sum, 0x114, 0xf, 0xf, true);
+        sum += __builtin_amdgcn_update_dpp(0, sum, 0x118, 0xf, 0xf, true);
         w.first = lane < kMaxTexts ? w.prefix_steps + sum - mine : INT32_MAX;
         w.steps = w.prefix_steps + __builtin_amdgcn_readlane(sum, kMaxTexts - 1);
         return w;

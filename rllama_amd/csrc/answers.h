@@ -23,12 +23,14 @@ struct AttnSharedParams {
 struct SharedPart {
     int prefix, texts;
     int blocks; // of rows, of a key and value head
-    int pieces, piece_steps;
+    int whole;  // of them the first ones, which are not cut
+    int pieces, piece_steps; // of the others
     int first_slot; // of its pieces' places in work memory
 };
 struct SharedPlan {
     SharedPart part[2];
     int slots;   // places for pieces
+    int cut;     // the first row of a head that is cut
     bool joined; // by a second launch
     size_t work_floats;
     int64_t workgroups;

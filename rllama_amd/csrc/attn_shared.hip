@@ -21,8 +21,9 @@ namespace rlh {
 
 struct SharedKernelParams {
     AttnSharedParams a;
-    float *ws; // for every row of every key and value head the pairs (m, sum) of all its pieces, then the sums O of each
+    float *ws; // for every row, from `cut` on, of every key and value head the pairs (m, sum) of all its pieces, then the sums O of each
     int slots; // places for pieces
+    int cut;
     SharedPart part[2]; // in tiles; 16 rows at a time
 };
 
@@ -54,17 +55,17 @@ struct SharedView {
     PartParams p;
     const AttnSharedParams &a;
     float *ws;
-    int pieces, piece_steps, first_slot;
-    __device__ SharedView(const SharedKernelParams &c, int part)
-        : p{c.a.q, c.a.out, c.a.n_heads, c.a.n_kv, c.a.prefix_rows, c.a.n * c.a.n_seqs}, a(c.a), ws(c.ws), pieces(c.slots), piece_steps(c.part[part].piece_steps),
-          first_slot(c.part[part].first_slot) {}
-    __device__ float *partials(int g, int rows, int r, int hd) const { return ws + ((size_t)g * rows + r) * pieces * (hd + 2); }
+    int pieces, piece_steps, first_slot, cut;
+    __device__ SharedView(const SharedKernelParams &c, int part, bool whole)
+        : p{c.a.q, c.a.out, c.a.n_heads, c.a.n_kv, c.a.prefix_rows, c.a.n * c.a.n_seqs}, a(c.a), ws(c.ws), pieces(c.slots), piece_steps(whole ? 1 << 30 : c.part[part].piece_steps),
+          first_slot(c.part[part].first_slot), cut(c.cut) {}
+    __device__ float *partials(int g, int rows, int r, int hd) const { return ws + ((size_t)g * (rows - cut) + r - cut) * pieces * (hd + 2); }
 };
 // The prefix alone: all rows are at its last position.
 struct PrefixView : SharedView {
     static constexpr bool kTexts = false;
     bool apart; // results are left for a join whatever the number of pieces
-    __device__ explicit PrefixView(const SharedKernelParams &c) : SharedView(c, 0), apart(c.part[1].pieces > 0) {}
+    __device__ explicit PrefixView(const SharedKernelParams &c) : SharedView(c, 0, false), apart(c.part[1].pieces > 0) {}
     __device__ bool partial() const { return apart; }
     __device__ int start(int) const { return a.prefix_len - 1; }
     __device__ int position(int start, int) const { return start; }
@@ -75,7 +76,7 @@ struct PrefixView : SharedView {
 template <bool kPrefix>
 struct TextsView : SharedView {
     static constexpr bool kTexts = true;
-    __device__ TextsView(const SharedKernelParams &c, int part) : SharedView(c, part) {}
+    __device__ TextsView(const SharedKernelParams &c, int part, bool whole) : SharedView(c, part, whole) {}
     __device__ constexpr bool partial() const { return !kPrefix; }
     __device__ int start(int) const { return 0; }
     __device__ int text(int i) const { return i / a.n; }
@@ -116,13 +117,16 @@ __global__ __launch_bounds__(kAwThreads, kForm == kNoTiles ? 1 : 2) void attn_sh
     int at = blockIdx.x;
     const int first = kForm == kNoTiles ? 0 : c.a.n_kv * c.part[0].blocks * c.part[0].pieces, own = kForm == kNoTiles || (kForm == kPrefixTiles && at >= first) ? 1 : 0;
     if (own) at -= first;
-    const int blocks = c.part[own].blocks, g = at % c.a.n_kv, rest = at / c.a.n_kv, block = rest % blocks, piece = rest / blocks;
+    // blocks that are not cut, and then the pieces of the others
+    const int g = at % c.a.n_kv, rest = at / c.a.n_kv, uncut = c.part[own].whole, cut = c.part[own].blocks - uncut;
+    const bool whole = rest < uncut;
+    const int block = whole ? rest : uncut + (rest - uncut) % cut, piece = whole ? 0 : (rest - uncut) / cut;
     if constexpr (kForm == kNoTiles) {
-        attn_rows<AC, QT, CT, HD>(TextsView<true>(c, 1), *reinterpret_cast<RowsShared<HD> *>(lds), g, block, piece);
+        attn_rows<AC, QT, CT, HD>(TextsView<true>(c, 1, whole), *reinterpret_cast<RowsShared<HD> *>(lds), g, block, piece);
     } else if constexpr (kForm == kAllTiles) {
-        attn_tiles<CT, HD, 2>(TextsView<true>(c, 0), lds, wide, g, block, piece);
+        attn_tiles<CT, HD, 2>(TextsView<true>(c, 0, whole), lds, wide, g, block, piece);
     } else {
-        if (own) attn_rows<AC, QT, CT, HD>(TextsView<false>(c, 1), *reinterpret_cast<RowsShared<HD> *>(lds), g, block, piece);
+        if (own) attn_rows<AC, QT, CT, HD>(TextsView<false>(c, 1, false), *reinterpret_cast<RowsShared<HD> *>(lds), g, block, piece);
         else attn_tiles<CT, HD, 2>(PrefixView(c), lds, wide, g, block, piece);
     }
 }
@@ -153,11 +157,11 @@ struct JoinRow {
     }
 };
 
-// Row r of key and value head g joins its pieces of the prefix and of its text: a workgroup for a row, where there are few.
+// The rows that were cut join their pieces: a workgroup for a row, where there are few.
 template <typename QT, int HD, int kRowsStep>
 __global__ __launch_bounds__(kAjWaves *kWave) void attn_shared_join_kernel(SharedKernelParams c) {
     __shared__ float part[kAjWaves * (kWave / (HD / 2))][HD];
-    const int g = blockIdx.y, r = blockIdx.x, all = gridDim.x;
+    const int g = blockIdx.y, r = c.cut + blockIdx.x, all = gridDim.x;
     const JoinRow row(c, g, r, HD, kRowsStep);
     QT *out = reinterpret_cast<QT *>(c.a.out) + row.out;
     if (row.finished) return;
@@ -165,7 +169,7 @@ __global__ __launch_bounds__(kAjWaves *kWave) void attn_shared_join_kernel(Share
         if ((int)threadIdx.x < HD) out[threadIdx.x] = (QT)0.0f;
         return;
     }
-    join_pieces<QT, HD, kAjWaves>(part, c.ws + ((size_t)g * all + r) * c.slots * (HD + 2), c.slots, row.n_pieces, out);
+    join_pieces<QT, HD, kAjWaves>(part, c.ws + ((size_t)g * all + blockIdx.x) * c.slots * (HD + 2), c.slots, row.n_pieces, out);
 }
 
 // ... HD / 4 lanes for a row, where there are many: every lane works out the pieces' weights for itself, eight pieces at a time with a running reference point, and adds up four
@@ -173,11 +177,11 @@ __global__ __launch_bounds__(kAjWaves *kWave) void attn_shared_join_kernel(Share
 template <typename QT, int HD, int kRowsStep>
 __global__ __launch_bounds__(256) void attn_shared_join_rows_kernel(SharedKernelParams c, int all) {
     constexpr int kLanes = HD / 4, kRows = 256 / kLanes, kBatch = 4;
-    const int g = blockIdx.y, r = blockIdx.x * kRows + (int)threadIdx.x / kLanes, d = ((int)threadIdx.x % kLanes) * 4;
-    if (r >= all) return;
+    const int g = blockIdx.y, at = blockIdx.x * kRows + (int)threadIdx.x / kLanes, r = c.cut + at, d = ((int)threadIdx.x % kLanes) * 4;
+    if (at >= all) return;
     const JoinRow row(c, g, r, HD, kRowsStep);
     if (row.finished) return;
-    const float *ws = c.ws + ((size_t)g * all + r) * c.slots * (HD + 2);
+    const float *ws = c.ws + ((size_t)g * all + at) * c.slots * (HD + 2);
     const float c2 = 1.44269504088896340736f / sqrtf((float)HD);
     float M = -INFINITY, L = 0.0f;
     float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -281,28 +285,46 @@ SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
     }
     const int places = compute_units * (a.head_dim == 128 || tiles ? 1 : 2); // (registers, and LDS of tiles)
     const int most[2] = {std::min(kMaxPieces / 2, longest[0]), std::min(kMaxPieces / 2, (longest[1] + kAwWaves - 1) / kAwWaves)};
+    auto time_of = [&](int k, int n) { // a workgroup of average length, cut into n
+        const double part = n > 0 ? std::min((double)((longest[k] + n - 1) / n), mean[k]) : 0.0;
+        return fixed[k] + (k ? (double)(((int64_t)part + kAwWaves - 1) / kAwWaves) : part) * per_step[k];
+    };
+    auto join_time = [&](int64_t rows, int n) { return 3.0 + (double)rows * a.n_kv * n * (a.head_dim + 2) * 8 / 4.5e6; };
     double least = -1.0;
     int pieces[2] = {0, 0};
-    for (int n0 = std::min(1, most[0]); n0 <= most[0]; n0 += 1 + n0 / 4) {
-        for (int n1 = std::min(1, most[1]); n1 <= most[1]; n1 += 1 + n1 / 4) {
-            const int n[2] = {n0, n1};
-            double us[2];
-            int64_t count[2];
-            for (int k = 0; k < 2; k++) { // of an average workgroup
-                const double part = n[k] > 0 ? std::min((double)((longest[k] + n[k] - 1) / n[k]), mean[k]) : 0.0;
-                us[k] = fixed[k] + (k ? (double)(((int64_t)part + kAwWaves - 1) / kAwWaves) : part) * per_step[k];
-                count[k] = (int64_t)a.n_kv * c.part[k].blocks * n[k];
+    if (c.part[0].texts || c.part[1].prefix) { // one part
+        const int k = c.part[0].texts ? 0 : 1;
+        SharedPart &p = c.part[k];
+        // Cut all blocks, or what is left behind as many whole ones as there is room for at a time (questions of 61 tokens: 616 blocks for 256 places: 85 -> 78 us)
+        const int rounds = (int)((int64_t)a.n_kv * p.blocks / places * places / a.n_kv), whole[2] = {0, rounds < p.blocks ? rounds : 0};
+        for (int n = std::min(1, most[k]); n <= most[k]; n += 1 + n / 4) {
+            for (int w = 0; w < (whole[1] > 0 && n > 1 ? 2 : 1); w++) {
+                const int64_t count[2] = {(int64_t)a.n_kv * whole[w], (int64_t)a.n_kv * (p.blocks - whole[w]) * n};
+                const double us[2] = {time_of(k, 1), time_of(k, n)};
+                const double end = makespan(places, count, us) + (n > 1 ? join_time(all - (int64_t)whole[w] * together[k], n) : 0.0);
+                if (least < 0.0 || end < least) {
+                    least = end;
+                    pieces[k] = n;
+                    p.whole = whole[w];
+                }
             }
-            const bool join = n0 + n1 > 1;
-            const double end = makespan(places, count, us) + (join ? 3.0 + (double)all * a.n_kv * (n0 + n1) * (a.head_dim + 2) * 8 / 4.5e6 : 0.0);
-            if (least < 0.0 || end < least) {
-                least = end;
-                pieces[0] = n0;
-                pieces[1] = n1;
-            }
-            if (most[1] == 0) break;
+            if (most[k] == 0) break;
         }
-        if (most[0] == 0) break;
+        if (pieces[k] > 1) c.cut = p.whole * together[k];
+    } else {
+        for (int n0 = 1; n0 <= most[0]; n0 += 1 + n0 / 4) {
+            for (int n1 = std::min(1, most[1]); n1 <= most[1]; n1 += 1 + n1 / 4) {
+                const int64_t count[2] = {(int64_t)a.n_kv * c.part[0].blocks * n0, (int64_t)a.n_kv * c.part[1].blocks * n1};
+                const double us[2] = {time_of(0, n0), time_of(1, n1)};
+                const double end = makespan(places, count, us) + (n0 + n1 > 1 ? join_time(all, n0 + n1) : 0.0);
+                if (least < 0.0 || end < least) {
+                    least = end;
+                    pieces[0] = n0;
+                    pieces[1] = n1;
+                }
+                if (most[1] == 0) break;
+            }
+        }
     }
     for (int k = 0; k < 2; k++) {
         SharedPart &p = c.part[k];
@@ -312,10 +334,10 @@ SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
         if (p.prefix && p.texts) p.pieces = std::max(1, p.pieces); // (nothing but padding: zeros)
         p.first_slot = k ? c.part[0].pieces : 0;
         c.slots += p.pieces;
-        c.workgroups += (int64_t)a.n_kv * p.blocks * p.pieces;
+        c.workgroups += (int64_t)a.n_kv * (p.whole + (p.blocks - p.whole) * (int64_t)p.pieces);
     }
     c.joined = c.slots > 1;
-    c.work_floats = c.joined ? (size_t)all * a.n_kv * c.slots * (a.head_dim + 2) : 0;
+    c.work_floats = c.joined ? (size_t)(all - c.cut) * a.n_kv * c.slots * (a.head_dim + 2) : 0;
     return c;
 }
 
@@ -328,7 +350,7 @@ static void launch_shared(const SharedKernelParams &c, const SharedPlan &plan, h
     }
     if (!c.part[0].prefix) hipLaunchKernelGGL((attn_shared_kernel<AC, QT, CT, HD, kNoTiles>), grid, block, 0, s, c);
     if (!plan.joined) return;
-    const unsigned rows = (unsigned)(c.a.n * c.a.n_seqs * (c.a.n_heads / c.a.n_kv)), per = 256 / (HD / 4);
+    const unsigned rows = (unsigned)(c.a.n * c.a.n_seqs * (c.a.n_heads / c.a.n_kv) - c.cut), per = 256 / (HD / 4);
     constexpr int kStep = Step<AC, CT, HD>::kPositions;
     if ((int64_t)rows * c.a.n_kv <= 1024) hipLaunchKernelGGL((attn_shared_join_kernel<QT, HD, kStep>), dim3(rows, (unsigned)c.a.n_kv), dim3(kAjWaves * kWave), 0, s, c);
     else hipLaunchKernelGGL((attn_shared_join_rows_kernel<QT, HD, kStep>), dim3((rows + per - 1) / per, (unsigned)c.a.n_kv), dim3(256), 0, s, c, (int)rows);
@@ -345,7 +367,7 @@ static hipError_t launch_hd(const SharedKernelParams &c, const SharedPlan &plan,
 }
 
 hipError_t launch_attn_shared(const AttnSharedParams &a, const SharedPlan &plan, float *ws, hipStream_t s) {
-    SharedKernelParams c{a, ws, plan.slots, {plan.part[0], plan.part[1]}};
+    SharedKernelParams c{a, ws, plan.slots, plan.cut, {plan.part[0], plan.part[1]}};
     switch (a.cache * 2 + a.f16) {
     case kPlaneF16 * 2: return launch_hd<float, float, half_t>(c, plan, s);
     case kPlaneF16 * 2 + 1: return launch_hd<half_t, half_t, half_t>(c, plan, s);

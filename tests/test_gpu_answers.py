@@ -363,6 +363,25 @@ def test_the_same_as_attention_over_whole_texts(ctx):
     assert np.abs(shared.astype(f64) - apart).max() <= 2 * EPS16 * np.abs(PV.astype(f64)).max()
 
 
+@pytest.mark.parametrize("kind,cache", [("f16", "f16"), ("f16", "q4"), ("f32", "f32")])
+def test_a_large_batch_is_its_texts(ctx, kind, cache):
+    """More blocks of rows than there is room for at a time, of which the last ones are cut: the same as every text by itself, which is cut into pieces.  Both are within
+    the bound of the results of each other."""
+    H, hd, n, B, P, S = 32, 64, 66, 20, 3000, 70
+    rng = np.random.default_rng(20)
+    pk, pv = (upload(ctx, rng.standard_normal((H * P, hd)), cache) for _ in range(2))
+    own = [rng.standard_normal((B, H * S, hd)) for _ in range(2)]
+    starts = [b % 7 - 3 for b in range(B)]
+    q = rng.standard_normal((B, n, H * hd)).astype(NUMPY[kind])
+    got = Tensor.from_numpy(ctx, q.reshape(B * n, -1)).attn_shared(pk, pv, P, *(upload(ctx, x.reshape(-1, hd), cache) for x in own), H, H, S, starts).to_numpy().reshape(B, n, -1).astype(f64)
+    for b in range(B):
+        alone = Tensor.from_numpy(ctx, q[b]).attn_shared(pk, pv, P, *(upload(ctx, x[b], cache) for x in own), H, H, S, starts[b:b + 1]).to_numpy().astype(f64)
+        size = max(np.abs(x).max() for x in own + [values(pv)])
+        scores = np.abs(q[b].astype(f64)).max() * hd ** 0.5 * size  # (no score is larger)
+        bound = size * (8 * np.sqrt(hd) * EPS32 * scores + (4 * np.sqrt(P + S) + 16) * EPS32) + (2 * EPS16 * size if kind == "f16" else 0)
+        assert (np.abs(got[b] - alone) <= 2 * bound).all()
+
+
 # -- log probabilities --------------------------------------------------------------------------------------------------------------------
 
 def logprobs_reference(x, temperature):

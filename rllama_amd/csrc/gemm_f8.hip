@@ -230,8 +230,10 @@ struct TilesF8Params {
     int tiles_m, tiles_n;
 };
 
+// (Two wavefronts to a SIMD where LDS, 80 KB of it, leaves room for two workgroups: 256 registers, and the products' results are where the vector ALU reads them.  With more the
+// compiler moves each through another register: 64 x 11008 x 4096 19.3 us, 18.4 so.)
 template <int kWM, int kWN, int kMT, int kNT, int kStages, bool kExact, typename Y>
-__global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN / 4) void matmul_f8_tiles_kernel(TilesF8Params pp) {
+__global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN == 8 || kStages * (kMT * kWM + kNT * kWN) * 16 <= 640 ? 2 : 1) void matmul_f8_tiles_kernel(TilesF8Params pp) {
     const MatmulF8Params &p = pp.p;
     constexpr int kWaves = kWM * kWN, kBM = 16 * kMT * kWM, kBN = 16 * kNT * kWN, kTiles = kMT * kNT;
     constexpr int kStageBytes = (kBM + kBN) * kF8Block;
@@ -243,7 +245,7 @@ __global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN / 4) void matmul_f8_tile
     static_assert(128 % (16 * kNT) == 0, "a wavefront's columns share their scale");
     constexpr int kLoadsX = kBM / 8 / kWaves;
     static_assert(kBM % (8 * kWaves) == 0 && kBN % (8 * kWaves) == 0, "whole loads of every wavefront, of x and then of w");
-    static_assert(kNT % kRing == 0 && kNT >= kRing, "a block's first column has the same place as the one before it");
+    static_assert(kNT % kRing == 0 && kNT >= kRing && kRing % 2 == 0, "a block's first column has the same place as the one before it");
     static_assert(kChunks + 1 <= kWaves, "a wavefront for each chunk of scales");
     constexpr bool kSpans = kStages == 2;                       // scales of kSpan blocks at a time
     constexpr int kSpan = 8, kScales = kBM * kSpan / (kWaves * kWave), kExtra = kSpans ? 0 : 1; // a thread's share of them; loads of scales beside a block's
@@ -352,21 +354,21 @@ __global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN / 4) void matmul_f8_tile
         __builtin_amdgcn_sched_barrier(0);
     };
     constexpr std::integral_constant<int, (kStages - 2) * (kLoads + kExtra)> kOnTheWay{};
+    // kExact: operands as f16 numbers, converted between the products that come before the ones that take them first: a row's beside the first column, a column's a part
+    // beside each tile of the column before it.  The four products of a tile wait for each other, and a wavefront issues in order: so everything else stands between them.
+    // (All rows' conversions in front of a block's first product, a column's in front of its own, sums behind a tile's four products: 131 x 4096 x 11008 33 us, 31 so; 64 x 11008 x 4096 19.8, 18.4.)
+    half8_t xs[kExact ? kMT : 1][4], ws[kExact ? 2 : 1][4];
+    auto row_f16 = [&](int i, int q) __attribute__((always_inline)) { xs[i][q] = f8_half8(x[i][2 * q], x[i][2 * q + 1]); };
+    auto column_f16 = [&](int j, int q) __attribute__((always_inline)) { ws[j % 2][q] = f8_half8(w[j % kRing][2 * q], w[j % kRing][2 * q + 1]); };
     // The b-th block, whose first operands are in registers.  more(i): a load of the block kStages further on.
     auto work = [&](int b, auto more) __attribute__((always_inline)) {
         constexpr int kLag = 2; // a block's sum of one tile is scaled and added beside the products of the tiles after it
         float4_t part[kLag + 1];
+        auto add1 = [&](int t, int e) __attribute__((always_inline)) { acc[t % kMT][t / kMT][e] = fmaf(part[t % (kLag + 1)][e], scale[t % kMT], acc[t % kMT][t / kMT][e]); };
         auto add = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[t % kMT][t / kMT][e] = fmaf(part[t % (kLag + 1)][e], scale[t % kMT], acc[t % kMT][t / kMT][e]);
+            for (int e = 0; e < 4; e++) add1(t, e);
         };
-        half8_t xs[kExact ? kMT : 1][4], ws[4];
-        if constexpr (kExact) {
-#pragma unroll
-            for (int i = 0; i < kMT; i++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) xs[i][q] = f8_half8(x[i][2 * q], x[i][2 * q + 1]);
-        }
 #pragma unroll
         for (int i = 0; i < kMT; i++) scale[i] = sx_next[i] * sw_next;
         __builtin_amdgcn_sched_barrier(0);
@@ -377,20 +379,24 @@ __global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN / 4) void matmul_f8_tile
             if (t == kMeet) meet(kOnTheWay);
             if (i == 0) frag(frag_w, (j + kAhead) % kNT, j + kAhead < kNT ? b : b + 1, w[(j + kAhead) % kRing]);
             if constexpr (kExact) {
-                if (i == 0) {
-#pragma unroll
-                    for (int q = 0; q < 4; q++) ws[q] = f8_half8(w[j % kRing][2 * q], w[j % kRing][2 * q + 1]);
-                }
                 float4_t s = zero;
 #pragma unroll
-                for (int q = 0; q < 4; q++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ws[q], xs[i][q], s, 0, 0, 0);
+                for (int q = 0; q < 4; q++) {
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ws[j % 2][q], xs[i][q], s, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (t >= kLag) add1(t - kLag, q);
+                    if (j == 0 && i + 1 < kMT) row_f16(i + 1, q);
+                    if ((i * 4 + q) % kMT == 0) column_f16(j + 1, (i * 4 + q) / kMT);
+                    if (t == kTiles - 1) row_f16(0, q); // (the next block's)
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 part[t % (kLag + 1)] = s;
             } else {
                 part[t % (kLag + 1)] =
                     __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(int8_t_, w[j % kRing]), __builtin_bit_cast(int8_t_, x[i]), zero, 0, 0, 0, 0, 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0); // (the next product has to be on its way before the sums that wait for the one before)
-            if (t >= kLag) add(t - kLag);
+            if (!kExact && t >= kLag) add(t - kLag);
             if (t >= kMeet) {
                 constexpr int kLeft = kTiles - kMeet;
 #pragma unroll
@@ -418,6 +424,13 @@ __global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN / 4) void matmul_f8_tile
     for (int i = 0; i < kMT; i++) frag(frag_x, i, 0, x[i]);
 #pragma unroll
     for (int j = 0; j < kAhead; j++) frag(frag_w, j, 0, w[j]);
+    if constexpr (kExact) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            row_f16(0, q);
+            column_f16(0, q);
+        }
+    }
     if (count == 1) { // no whole block may be left to be loaded again: zeros then
 #pragma unroll
         for (int i = 0; i < kLoads; i++) from[i] = 0;
@@ -484,7 +497,7 @@ static TilesPlan plan_tiles(const MatmulF8Params &p, int compute_units) {
         double tb;
     };
     const bool f16 = p.y_f16 != 0;
-    const Kind kinds[] = {{64, 128, f16 ? 0.43 : 0.73}, {128, 128, f16 ? 0.68 : 1.15}, {160, 128, f16 ? 0.66 : 1.2}, {256, f16 ? 256 : 128, f16 ? 1.6 : 1.76}};
+    const Kind kinds[] = {{64, 128, f16 ? 0.43 : 0.68}, {128, 128, f16 ? 0.68 : 1.15}, {160, 128, f16 ? 0.66 : 1.2}, {256, f16 ? 256 : 128, f16 ? 1.6 : 1.76}};
     const int across = f8_blocks(p.k);
     TilesPlan best{};
     double least = 0.0;

@@ -100,6 +100,10 @@ extern "C" int rlh_token_logprobs(rlh_tensor *logprobs, rlh_tensor *entropy, rlh
     if (top_ids && top_ids->cols > logits->cols) return fail(RLH_ERR_INVALID, "%s: %d alternatives of %d entries", who, top_ids->cols, logits->cols);
     if (top_ids && top_ids->cols > kMaxTop) return fail(RLH_ERR_UNSUPPORTED, "%s: %d alternatives (%d at most)", who, top_ids->cols, kMaxTop);
     if (!(temperature >= 1e-30f && temperature <= 1e30f)) return fail(RLH_ERR_INVALID, "%s: temperature %g (1e-30 to 1e30)", who, (double)temperature);
+    const rlh_tensor *const all[] = {logprobs, entropy, top_ids, top_logprobs, logits, tokens};
+    for (int i = 0; i < 4; i++)
+        for (int j = i + 1; j < 6; j++)
+            if (all[i] && all[j] && all[i]->p == all[j]->p) return fail(RLH_ERR_INVALID, "%s: results must not share memory with each other or the operands", who);
     rlh_ctx *ctx = (logprobs ? logprobs : entropy ? entropy : top_ids)->ctx;
     CtxLock lock(ctx);
     lend(ctx, {logits});

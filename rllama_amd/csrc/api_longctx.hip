@@ -56,6 +56,7 @@ extern "C" int rlh_convert(rlh_tensor *dst, const rlh_tensor *src) {
     if (dst->dtype == RLH_I32 || src->dtype == RLH_I32) return fail(RLH_ERR_UNSUPPORTED, "rlh_convert: f16, f32, 4-bit and 8-bit tensors only");
     if (dst->dtype == src->dtype) return rlh_copy_inplace(dst, src);
     if ((dst->is_eight() && !src->is_float()) || (src->is_eight() && !dst->is_float())) return fail(RLH_ERR_UNSUPPORTED, "rlh_convert: 8 bits from and to f16 and f32 only");
+    if ((dst->is_eight() || src->is_eight()) && dst->p == src->p) return fail(RLH_ERR_INVALID, "rlh_convert: tensors of 8 bits must not share memory with the other one");
     CtxLock lock(dst->ctx);
     lend(dst->ctx, {src});
     if (dst->is_eight()) {

@@ -72,6 +72,7 @@ def build(force: bool = False) -> str:
 
 HOST_BIN = os.path.join(HERE, "host", "rllama_generate")
 TENSORS_BIN = os.path.join(HERE, "host", "rllama_check_tensors")
+ANSWERS_BIN = os.path.join(HERE, "host", "rllama_check_answers")
 
 
 def _build_host(main: str, binary: str, force: bool) -> str:
@@ -94,6 +95,11 @@ def build_host(force: bool = False) -> str:
 def build_host_tensors(force: bool = False) -> str:
     """The C++ mirror's tensor methods for long contexts and drafted tokens, as a program that runs one step of them."""
     return _build_host("check_tensors_main.cpp", TENSORS_BIN, force)
+
+
+def build_host_answers(force: bool = False) -> str:
+    """The same of those for many answers to one prompt."""
+    return _build_host("check_answers_main.cpp", ANSWERS_BIN, force)
 
 
 ASAN_BIN = os.path.join(HERE, "host", "rllama_check_files_asan")
@@ -121,3 +127,4 @@ if __name__ == "__main__":
         print(build(force="--force" in sys.argv))
         print(build_host(force="--force" in sys.argv))
         print(build_host_tensors(force="--force" in sys.argv))
+        print(build_host_answers(force="--force" in sys.argv))

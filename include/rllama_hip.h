@@ -369,7 +369,8 @@ int  rlh_verify_draft(rlh_tensor *out, const rlh_tensor *target, const rlh_tenso
  * Many answers to one prompt (no reference counterpart): one step of a batch of texts that share a long prefix, with weights of 8 bits.  All work is queued on the
  * context's stream; a call waits for nothing.  Work memory that a call needs beyond its operands stays with the context: a call that needs more than every one before it
  * allocates it, and is refused with RLH_ERR_STATE while the stream is being captured (make one call of that size before).  Buffers that were outgrown are kept until the
- * context ends, so a captured graph stays valid; graphs of one context share them and must not run side by side.
+ * context ends, so a captured graph stays valid; graphs of one context share them and must not run side by side, nor beside other work of the context.  What a call takes from
+ * host memory (positions, lengths) is read while it is queued: a replayed graph has those it was captured with.
  * ---------------------------------------------------------------------------------------------- */
 /* rlh_rope_table of positions first .. first + rows - 1: row 0 of the table that rlh_qkv_append takes for texts behind a prefix is position prefix_len. */
 int  rlh_rope_table_from(rlh_tensor *freqs, double theta, int first);
@@ -378,21 +379,24 @@ int  rlh_rope_table_from(rlh_tensor *freqs, double theta, int first);
  * its rows of the result are zeros.  Prefix planes: two tensors [n_kv_heads * prefix_rows x head_dim], row g * prefix_rows + t, prefix_rows >= prefix_len (no prefix: 0, and
  * the planes may be NULL); cache planes: two tensors [n_seqs * n_kv_heads * max_seq_len x head_dim], row (b * n_kv_heads + g) * max_seq_len + t, which hold the rows' own positions
  * already; all four of one dtype, f16, f32 or Q4; head_dim 32, 64 or 128.  Query head h reads key and value head h / (n_heads / n_kv_heads).  q and out
- * [n_seqs * n x n_heads head_dim], both f16 or both f32.  f32 rows, or f32 planes: f32 arithmetic throughout; otherwise f16 operands with f32 sums.
- * The prefix is read once for the rows of all texts and not once for each.  Rows and keys outside what is seen may hold anything, NaN included. */
+ * [n_seqs * n x n_heads head_dim], both f16 or both f32.  f32 rows, or f32 planes: f32 arithmetic throughout; otherwise f16 operands with f32 sums,
+ * where more than 32 rows of a key and value head (n n_heads / n_kv_heads n_seqs) round the softmax's weights and 4-bit values to f16 (ATTN_EXACT: they do not).  The prefix is
+ * read once for the rows of all texts and not once for each.  Rows and keys outside what is seen may hold anything, NaN included. */
 int  rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *prefix_k, const rlh_tensor *prefix_v, int prefix_len, const rlh_tensor *cache_k,
                      const rlh_tensor *cache_v, int n_heads, int n_kv_heads, int max_seq_len, const int32_t *start_pos, int n_seqs);
 /* Log probabilities under softmax(logits / temperature), logits f16 or f32 [n x vocab]: logprobs f32 [n x m] those of tokens i32 [n x m] (a negative id, a place without
  * a token: 0; an id past the vocabulary: -infinity); entropy f32 [n x 1], in nats; top_ids i32 and top_logprobs f32 [n x k], k up to 32, the k most probable ids of each
  * row, the lowest first among equal ones.  logprobs and tokens, entropy, and top_ids and top_logprobs may each be NULL, but not all of them.  temperature: 1e-30 to 1e30.
- * Logits of -infinity have probability 0.  A row of nothing else: -infinity, entropy 0, the first k ids.  A row with a NaN or +infinity: NaN, and ids of -1. */
+ * Results must not share memory.  Logits of -infinity have probability 0.  A row of nothing else: -infinity, entropy 0, the first k ids.  A row with a NaN or +infinity: NaN, and ids of -1. */
 int  rlh_token_logprobs(rlh_tensor *logprobs, rlh_tensor *entropy, rlh_tensor *top_ids, rlh_tensor *top_logprobs, const rlh_tensor *logits, const rlh_tensor *tokens,
                         float temperature);
 /* rlh_convert to 8 bits: per block, a = max(largest |x|, 448 * 2^-126), scale = a / 448, code = e4m3(x * (448 * (1 / a))), each step one f32 operation, the last one
  * rounded to even and limited to 448.  A block with a value that is not finite reads as NaN throughout.  From 8 bits: code * scale in f32, rounded once more for f16.
  *
  * dst [n x m] = src [n x k] times weights[m x k]^T: weights RLH_F8_TILES; src RLH_F8, or f16 or f32, which is converted to RLH_F8 first; dst f16 or f32.
- * Products and sums of a block of 128 in f32, each block's sum times both scales in f32. */
+ * The sum of a block of 128 products, then that times both scales, added up in f32.  f32 results, and up to 16 rows: every sum is one of f32.  f16 results of more rows: the 8-bit
+ * matrix instruction, which adds products up eight at a time and cuts off what is 2^-13 and less of the largest one's power of two (random operands: off by 1.5e-5 of the
+ * result, a fourteenth of its rounding to f16).  k up to 2^24. */
 int  rlh_matrix_mul_f8(rlh_tensor *dst, const rlh_tensor *src, const rlh_tensor *weights);
 
 /* ------------------------------------------------------------------------------------------------

@@ -7,7 +7,7 @@
 //
 // A workgroup takes rows of one key and value head, whatever texts they are of; its steps are the prefix's and then every one of its texts', masked for the rows of the others.  They
 // are cut into pieces; where there is only one the result is final, and pieces leave (m, sum, O) of their rows in work memory, which a second launch joins.
-//   Few rows per key and value head, or f32 arithmetic: 16 rows at a time, from memory into registers (attn_rows_device.h).
+//   Few rows per key and value head, f32 arithmetic, or where nothing may be rounded but the result: 16 rows at a time, from memory into registers (attn_rows_device.h).
 //   Many rows of each text: 128 at a time, through tiles of keys in LDS (attn_tiles_device.h, f16 arithmetic).
 //   Many rows, but few of each text: the prefix in tiles; 128 rows would be of too many texts for the texts' own positions, which go 16 rows at a time beside them in the same launch.
 #include "kernels.h"
@@ -258,7 +258,7 @@ SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
     const double fixed[2] = {7.0, 3.0}, per_step[2] = {(q4 ? 2.6 : 1.9) * scale, (q4 ? 1.6 : 1.2) * scale};
     const int step[2] = {kSharedTile, f16 ? 32 : 16}, together[2] = {kAtRows, kAwRows};
     // which parts there are, and what they have
-    const bool texts_tiles = f16 && rows > 2 * kAwRows, tiles = texts_tiles || (f16 && all > 2 * kAwRows && a.prefix_len > 0);
+    const bool rounds = f16 && !a.exact, texts_tiles = rounds && rows > 2 * kAwRows, tiles = texts_tiles || (rounds && all > 2 * kAwRows && a.prefix_len > 0);
     c.part[0].prefix = tiles;
     c.part[0].texts = texts_tiles;
     c.part[1].prefix = !tiles;

@@ -306,6 +306,27 @@ def test_products_longer_than_32_bits(ctx, m, n, k, result):
             memory.free()
 
 
+# -- nothing rounded but the result ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cache", ["f16", "q4"])
+@pytest.mark.parametrize("H,G,n,B,P", [(8, 2, 1, 4, 300), (8, 2, 1, 40, 900), (4, 2, 50, 3, 700)])
+def test_only_the_result_is_rounded_on_request(ctx, cache, H, G, n, B, P):
+    """Values around zero, so that the result's own rounding hides nothing, in the forms for few rows, for a batch of single rows and for many rows of each text."""
+    hd, S = 64, 80
+    rng = np.random.default_rng(P)
+    q = rng.standard_normal((B, n, H, hd)).astype(f16)
+    planes = [upload(ctx, rng.standard_normal((rows, hd)), cache) for rows in (G * P, G * P, B * G * S, B * G * S)]
+    starts = [(5 * b) % (S - n) for b in range(B)]
+    wide = [values(t).reshape(-1, P, hd) if i < 2 else values(t).reshape(B, G, S, hd) for i, t in enumerate(planes)]
+    want, bound = shared_reference(q.astype(f64), *wide, starts)
+    ctx.set_option("ATTN_EXACT", "1")
+    try:
+        got = Tensor.from_numpy(ctx, q.reshape(B * n, -1)).attn_shared(*planes[:2], P, *planes[2:], H, G, S, starts).to_numpy().astype(f64).reshape(want.shape)
+    finally:
+        ctx.set_option("ATTN_EXACT", None)
+    assert (np.abs(got - want) <= bound + EPS16 * np.abs(want) + 2.0 ** -24).all()
+
+
 # -- operands that share memory -----------------------------------------------------------------------------------------------------------
 
 def test_results_that_share_memory_are_refused(ctx):

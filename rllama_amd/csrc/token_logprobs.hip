@@ -5,7 +5,7 @@
 // Leaving one largest entry out of the sum keeps what is small beside it: where a token is all but certain, its log probability and the entropy are as exact as
 // the others' weights are (a sum that holds the 1 loses everything below 2^-24 of it).
 //
-// One workgroup per row.  A row of up to 32768 entries is read once and stays in registers, 64 bytes (f16) or 128 of them per thread; a longer one is read
+// One workgroup per row, of 256 to 1024 threads.  A row of up to 32768 entries is read once and stays in registers, up to 128 bytes per thread; a longer one is read
 // three times, the second and third time from the caches.
 //
 // The k most probable: the 64 groups of threads have a largest entry each, and the k-th largest of those bounds the k-th largest entry from below, since k groups hold an
@@ -22,6 +22,7 @@ namespace rlh {
 
 constexpr int kTlList = 256;
 constexpr int kTlGroups = 64;
+constexpr int kTlCrowd = 700; // rows from which on small workgroups gain
 
 template <int kCtrl, int kRowMask = 0xf>
 __device__ __forceinline__ float dpp_max(float v) { // (lanes whose row is masked out keep v)
@@ -71,7 +72,7 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
 
 // kKeep: pieces of kN entries that a thread keeps; 0: rows of any length.  kMany: of more rows than compute units, two to a compute unit.  c2 = log2(e) / T.
 template <typename T, int kThreads, int kN, int kKeep, bool kMany>
-__global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void token_logprobs_kernel(LogprobsParams p, float c2) {
+__global__ __launch_bounds__(kThreads, kMany && kN > 2 ? 8 : 4) void token_logprobs_kernel(LogprobsParams p, float c2) {
     typedef RowPiece<T, kN> Piece;
     constexpr int kStep = kThreads * kN, kWaves = kThreads / kWave, kLanes = kThreads / kTlGroups;
     __shared__ __attribute__((aligned(16))) float group_top[kTlGroups];
@@ -87,6 +88,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void
         if constexpr (kKeep > 0) {
 #pragma unroll
             for (int k = 0; k < kKeep; k++) {
+                if (k * kStep >= vocab) break; // (behind the row: one row of 10000 7.6 -> 6.4 us)
                 if (kMany) kept[k].hold();
                 f(kept[k], k * kStep + tid * kN);
                 if (kMany) __builtin_amdgcn_sched_barrier(0); // (one after the other, or each piece takes registers of its own for what is worked out)
@@ -112,6 +114,9 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void
 #pragma unroll
         for (int k = 0; k < kKeep; k++) kept[k].load(x, k * kStep + tid * kN, vocab);
     }
+    // the first of the tokens asked for, on their way beside the row
+    const int token = tid < p.n_tokens ? p.tokens[(size_t)row * p.n_tokens + tid] : -1;
+    const float token_logit = token >= 0 && token < vocab ? (float)x[token] : 0.0f;
     // ---- the largest entry, of the thread, of its group and of the row
     float mine = -INFINITY;
     pieces([&](const Piece &piece, auto) {
@@ -124,8 +129,9 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void
     });
     {
         float top = dpp_max<kDppQuadPerm2301>(dpp_max<kDppQuadPerm1032>(mine));
-        if constexpr (kLanes == 16) top = dpp_max<kDppRowMirror>(dpp_max<kDppRowHalfMirror>(top));
-        static_assert(kLanes == 16 || kLanes == 4, "1024 or 256 threads");
+        if constexpr (kLanes >= 8) top = dpp_max<kDppRowHalfMirror>(top);
+        if constexpr (kLanes >= 16) top = dpp_max<kDppRowMirror>(top);
+        static_assert(kLanes == 16 || kLanes == 8 || kLanes == 4, "1024, 512 or 256 threads");
         if (tid % kLanes == 0) group_top[tid / kLanes] = top;
     }
     if (tid < kTlList) list[tid] = 0;
@@ -196,8 +202,8 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 4 : kMany ? 8 : 4) void
     auto logprob = [&](float v) { return odd ? NAN : none ? -INFINITY : fmaf(exponent(v) - shift, kLn2, -log_s); };
     if (tid == 0 && p.entropy) p.entropy[row] = odd ? NAN : none ? 0.0f : log_s - kLn2 * u_top / (1.0f + others);
     for (int i = tid; i < p.n_tokens; i += kThreads) {
-        const int id = p.tokens[(size_t)row * p.n_tokens + i];
-        p.logprobs[(size_t)row * p.n_tokens + i] = id < 0 ? 0.0f : id < vocab ? logprob((float)x[id]) : odd ? NAN : -INFINITY;
+        const int id = i == tid ? token : p.tokens[(size_t)row * p.n_tokens + i];
+        p.logprobs[(size_t)row * p.n_tokens + i] = id < 0 ? 0.0f : id < vocab ? logprob(i == tid ? token_logit : (float)x[id]) : odd ? NAN : -INFINITY;
     }
     if (p.top == 0) return;
     int32_t *ids = p.top_ids + (size_t)row * p.top;
@@ -355,7 +361,14 @@ static void launch_t(const LogprobsParams &p, hipStream_t s) {
     const dim3 grid((unsigned)p.rows);
     // Narrow pieces in short rows, so that 33 groups at least hold entries: 20 or 32 alternatives of 500 entries, or of 2100 in f16, took 85 to 150 us in pieces of sixteen
     // bytes, whose few groups give no bound, and take less than 20 so, as those of other lengths do.
+    // A row's time is mostly that of its steps one after the other, whatever its length: many rows go to workgroups as small as their registers allow, up to eight of which
+    // share a compute unit (f16, five alternatives: 2048 rows of 32000 41 -> 37 us, of 10000 38.5 -> 21, of 6000 24 -> 15; 800 rows 22.1 / 22.3, 20.9 / 12.7, 13 / 8.6;
+    // 400 rows of 32000 13.6 -> 14.1).
+    const bool crowd = p.rows > kTlCrowd;
     if (p.vocab <= 2048) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 2, 4, kMany>), grid, dim3(256), 0, s, p, c2);
+    else if (crowd && p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, kN, 32 / kN, true>), grid, dim3(256), 0, s, p, c2);
+    else if (crowd && p.vocab <= 16384) hipLaunchKernelGGL((token_logprobs_kernel<T, kN == 8 ? 256 : 512, kN, 8, true>), grid, dim3(kN == 8 ? 256 : 512), 0, s, p, c2);
+    else if (crowd && p.vocab <= 32768 && kN == 8) hipLaunchKernelGGL((token_logprobs_kernel<T, 512, kN, 8, true>), grid, dim3(512), 0, s, p, c2);
     else if (p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 4, 2, kMany>), grid, dim3(1024), 0, s, p, c2);
     else if (p.vocab <= 32768) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, kN, 32 / kN, kMany>), grid, dim3(1024), 0, s, p, c2);
     else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, kN, 0, kMany>), grid, dim3(1024), 0, s, p, c2);

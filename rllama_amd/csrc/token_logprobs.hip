@@ -8,6 +8,9 @@
 // One workgroup per row, of 256 to 1024 threads.  A row of up to 32768 entries is read once and stays in registers, up to 128 bytes per thread; a longer one is read
 // three times, the second and third time from the caches.
 //
+// Measured: 16 rows of 32000 in f32 with five alternatives 7.8 us, the latency of a row on one compute unit; 2048 rows in f16 with twenty 41 us, 3.2 TB/s: the vector ALU is busy for 61 %
+// (an exponential, two sums and a maximum for each entry).
+//
 // The k most probable: the 64 groups of threads have a largest entry each, and the k-th largest of those bounds the k-th largest entry from below, since k groups hold an
 // entry that large.  What reaches the bound (about k ln(64 / (64 - k)) / (k / 64) of 32000 random entries) goes to a list in LDS, and an entry's place is the number
 // of those in front of it.  Lists that overflow: of rows with many entries equal to the bound (masks) those above it, and then the first equal ones in order of their ids.

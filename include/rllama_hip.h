@@ -381,7 +381,8 @@ int  rlh_rope_table_from(rlh_tensor *freqs, double theta, int first);
  * already; all four of one dtype, f16, f32 or Q4; head_dim 32, 64 or 128.  Query head h reads key and value head h / (n_heads / n_kv_heads).  q and out
  * [n_seqs * n x n_heads head_dim], both f16 or both f32.  f32 rows, or f32 planes: f32 arithmetic throughout; otherwise f16 operands with f32 sums,
  * where more than 32 rows of a key and value head (n n_heads / n_kv_heads n_seqs) round the softmax's weights and 4-bit values to f16 (ATTN_EXACT: they do not).  The prefix is
- * read once for the rows of all texts and not once for each.  Rows and keys outside what is seen may hold anything, NaN included. */
+ * read once for the rows of all texts and not once for each.  Rows and keys outside what is seen may hold anything, NaN included.  prefix_len and max_seq_len: 2^31 - 257 at
+ * most. */
 int  rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *prefix_k, const rlh_tensor *prefix_v, int prefix_len, const rlh_tensor *cache_k,
                      const rlh_tensor *cache_v, int n_heads, int n_kv_heads, int max_seq_len, const int32_t *start_pos, int n_seqs);
 /* Log probabilities under softmax(logits / temperature), logits f16 or f32 [n x vocab]: logprobs f32 [n x m] those of tokens i32 [n x m] (a negative id, a place without
@@ -396,7 +397,7 @@ int  rlh_token_logprobs(rlh_tensor *logprobs, rlh_tensor *entropy, rlh_tensor *t
  * dst [n x m] = src [n x k] times weights[m x k]^T: weights RLH_F8_TILES; src RLH_F8, or f16 or f32, which is converted to RLH_F8 first; dst f16 or f32.
  * The sum of a block of 128 products, then that times both scales, added up in f32.  f32 results, and up to 16 rows: every sum is one of f32.  f16 results of more rows: the 8-bit
  * matrix instruction, which adds products up eight at a time and cuts off what is 2^-13 and less of the largest one's power of two (random operands: off by 1.5e-5 of the
- * result, a fourteenth of its rounding to f16).  k up to 2^24. */
+ * result, a fourteenth of its rounding to f16).  k up to 2^24, n and m up to 2^26. */
 int  rlh_matrix_mul_f8(rlh_tensor *dst, const rlh_tensor *src, const rlh_tensor *weights);
 
 /* ------------------------------------------------------------------------------------------------

@@ -32,6 +32,8 @@ extern "C" int rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_t
     if (!out || !q || !cache_k || !cache_v) return fail(RLH_ERR_INVALID, "%s: NULL argument", who);
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0) return fail(RLH_ERR_INVALID, "%s: %d heads do not share %d key and value heads evenly", who, n_heads, n_kv_heads);
     if (!start_pos || n_seqs < 1 || n_seqs > kLongMaxSeqs) return fail(RLH_ERR_INVALID, "%s: 1 to %d sequences with a position each", who, kLongMaxSeqs);
+    constexpr int kFar = INT32_MAX - 256; // (the kernels add up to a tile to a position)
+    if (max_seq_len > kFar || prefix_len > kFar) return fail(RLH_ERR_UNSUPPORTED, "%s: planes of %d and %d positions (%d at most)", who, prefix_len, max_seq_len, kFar);
     if (max_seq_len <= 0 || !holds_plane(cache_k) || cache_v->dtype != cache_k->dtype || cache_v->cols != cache_k->cols || (int64_t)n_seqs * n_kv_heads * max_seq_len != cache_k->rows ||
         cache_v->rows != cache_k->rows) {
         return fail(RLH_ERR_INVALID, "%s: cache planes must be two [n_seqs * n_kv_heads * max_seq_len x head_dim] tensors of one dtype", who);
@@ -78,7 +80,7 @@ extern "C" int rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_t
     for (int b = 0; b < n_seqs; b++) p.start[b] = start_pos[b];
     const SharedPlan plan = plan_attn_shared(p, ctx->prop.multiProcessorCount);
     const int64_t rows = (int64_t)q->rows * (n_heads / n_kv_heads);
-    if (plan.workgroups > INT32_MAX || n_kv_heads > 65535 || rows > INT32_MAX) return fail(RLH_ERR_UNSUPPORTED, "%s: %lld rows on each of %d key and value heads are more than a launch takes", who, (long long)rows, n_kv_heads);
+    if (plan.workgroups >= 1 << 23 || n_kv_heads > 65535 || rows > INT32_MAX) return fail(RLH_ERR_UNSUPPORTED, "%s: %lld rows on each of %d key and value heads are more than a launch takes", who, (long long)rows, n_kv_heads);
     const int rc = work_reserve(who, ctx, ctx->ops.shared_work, plan.work_floats * sizeof(float));
     if (rc != RLH_OK) return rc;
     HIP_TRY(launch_attn_shared(p, plan, static_cast<float *>(ctx->ops.shared_work.memory()), ctx->stream));
@@ -138,6 +140,7 @@ extern "C" int rlh_matrix_mul_f8(rlh_tensor *dst, const rlh_tensor *src, const r
     if (!src->is_float() && src->dtype != RLH_F8) return fail(RLH_ERR_INVALID, "%s: src must be f16, f32 or 8 bits with a scale for each row's blocks", who);
     if (!dst->is_float() || src->cols != weights->cols || !shaped(dst, src->rows, weights->rows)) return fail(RLH_ERR_INVALID, "%s: src [n x k], weights [m x k] and dst [n x m], f16 or f32, are needed", who);
     if (src->cols > (1 << 24)) return fail(RLH_ERR_UNSUPPORTED, "%s: rows of %d (%d at most)", who, src->cols, 1 << 24);
+    if (src->rows > (1 << 26) || weights->rows > (1 << 26)) return fail(RLH_ERR_UNSUPPORTED, "%s: %d rows and %d columns (%d at most of each)", who, src->rows, weights->rows, 1 << 26);
     if (dst->p == src->p || dst->p == weights->p) return fail(RLH_ERR_INVALID, "%s: dst must not share memory with the operands", who);
     rlh_ctx *ctx = dst->ctx;
     CtxLock lock(ctx);

@@ -100,8 +100,13 @@ template <typename T>
 static void launch_encode(const EightRef &dst, const T *src, int rows, int cols, hipStream_t s) {
     const int across = f8_blocks(cols);
     if (dst.rows == 1) {
-        const int64_t blocks = (int64_t)rows * across;
-        hipLaunchKernelGGL((f8_encode_kernel<T, 1>), dim3((unsigned)((blocks + 31) / 32)), dim3(256), 0, s, dst, src, rows, cols, across, blocks);
+        const int64_t step = std::max<int64_t>(1, (1 << 28) / across); // rows of a launch, which takes less than 2^32 threads
+        for (int64_t r0 = 0; r0 < rows; r0 += step) {
+            const int part = (int)std::min<int64_t>(step, rows - r0);
+            const int64_t blocks = (int64_t)part * across;
+            hipLaunchKernelGGL((f8_encode_kernel<T, 1>), dim3((unsigned)((blocks + 31) / 32)), dim3(256), 0, s, EightRef{dst.codes + (size_t)r0 * cols, dst.scales + (size_t)r0 * across, 1},
+                               src + (size_t)r0 * cols, part, cols, across, blocks);
+        }
     } else {
         const int64_t blocks = (int64_t)f8_blocks(rows) * across;
         hipLaunchKernelGGL((f8_encode_kernel<T, kF8Block>), dim3((unsigned)blocks), dim3(256), 0, s, dst, src, rows, cols, across, blocks);

@@ -19,6 +19,7 @@
 #include "kernels.h"
 #include "answers.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace rlh {
@@ -377,9 +378,24 @@ static void launch_t(const LogprobsParams &p, hipStream_t s) {
     else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, kN, 0, kMany>), grid, dim3(1024), 0, s, p, c2);
 }
 
-hipError_t launch_token_logprobs(const LogprobsParams &p, hipStream_t s) {
-    if (p.f16) p.rows > 256 ? launch_t<half_t, true>(p, s) : launch_t<half_t, false>(p, s);
-    else p.rows > 256 ? launch_t<float, true>(p, s) : launch_t<float, false>(p, s);
+hipError_t launch_token_logprobs(const LogprobsParams &all, hipStream_t s) {
+    constexpr int kRows = 1 << 21; // of a launch, which takes less than 2^32 threads
+    for (int64_t r0 = 0; r0 < all.rows; r0 += kRows) {
+        LogprobsParams p = all;
+        p.rows = (int)std::min<int64_t>(kRows, all.rows - r0);
+        p.logits = static_cast<const char *>(all.logits) + (size_t)r0 * all.vocab * (all.f16 ? 2 : 4);
+        if (all.tokens) {
+            p.tokens = all.tokens + (size_t)r0 * all.n_tokens;
+            p.logprobs = all.logprobs + (size_t)r0 * all.n_tokens;
+        }
+        if (all.entropy) p.entropy = all.entropy + r0;
+        if (all.top > 0) {
+            p.top_ids = all.top_ids + (size_t)r0 * all.top;
+            p.top_logprobs = all.top_logprobs + (size_t)r0 * all.top;
+        }
+        if (p.f16) p.rows > 256 ? launch_t<half_t, true>(p, s) : launch_t<half_t, false>(p, s);
+        else p.rows > 256 ? launch_t<float, true>(p, s) : launch_t<float, false>(p, s);
+    }
     return hipGetLastError();
 }
 

@@ -12,7 +12,7 @@ import pytest
 import rllama_amd
 from rllama_amd import Context, Tensor, TensorDType
 from test_gpu_answers import F8, TILES, decode, encode, first_of_the_largest, logprobs_reference, shared_reference, stands_for
-from test_gpu_longctx import EPS16, EPS32, INVALID, STATE, f16, f32, f64, refused, upload, values
+from test_gpu_longctx import EPS16, EPS32, INVALID, STATE, UNSUPPORTED, f16, f32, f64, refused, upload, values
 from test_gpu_longctx_edges import hip_runtime
 
 pytestmark = pytest.mark.gpu
@@ -304,6 +304,38 @@ def test_products_longer_than_32_bits(ctx, m, n, k, result):
     finally:
         for memory in (X, W, Y):
             memory.free()
+
+
+def test_more_rows_than_a_launch_takes(ctx):
+    """Log probabilities of 17 million short rows; attention of more rows than one launch's workgroups have is refused, as are planes whose positions come near 32 bits."""
+    rows, vocab = 17_000_000, 16
+    rng = np.random.default_rng(9)
+    m = Memory(ctx, rows * vocab * 2)
+    try:
+        known = [0, 2 ** 21 - 1, 2 ** 21, 2 ** 24, rows - 1]
+        x = rng.standard_normal((len(known), vocab)).astype(f16)
+        for r, at in enumerate(known):
+            m.put(x[r], at * vocab * 2)
+        logits = m.tensor(rows, vocab, TensorDType.Float16)
+        got = logits.token_logprobs(Tensor.from_numpy(ctx, np.full((rows, 1), 3, np.int32)), 1.0, 2)
+        want, entropy = logprobs_reference(x, 1.0)
+        assert np.abs(got[0].to_numpy()[known, 0] - want[:, 3]).max() < 1e-5 and np.abs(got[1].to_numpy()[known] - entropy).max() < 1e-4
+        assert np.array_equal(got[2].to_numpy()[known], first_of_the_largest(x, 2))
+        logits.free()
+    finally:
+        m.free()
+    n = 2 ** 27 + 16
+    q, out, plane = Memory(ctx, n * 128), Memory(ctx, n * 128), Tensor.zeros(ctx, 64, 32, TensorDType.Float32)
+    try:
+        Q, Out = q.tensor(n, 32, TensorDType.Float32), out.tensor(n, 32, TensorDType.Float32)
+        refused(UNSUPPORTED, Q.attn_shared, None, None, 0, plane, plane, 1, 1, 64, [64 - n], out=Out)
+        Q.free(), Out.free()
+    finally:
+        q.free()
+        out.free()
+    small = Tensor.zeros(ctx, 1, 32, TensorDType.Float32)
+    refused(UNSUPPORTED, small.attn_shared, None, None, 0, plane, plane, 1, 1, 2 ** 31 - 256, [0])
+    refused(UNSUPPORTED, small.attn_shared, plane, plane, 2 ** 31 - 256, plane, plane, 1, 1, 64, [0])
 
 
 # -- nothing rounded but the result ---------------------------------------------------------------------------------------------------------

@@ -33,15 +33,13 @@ __device__ __forceinline__ half8_t f8_half8(uint32_t a, uint32_t b) {
     return half8_t{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
 }
 
+// Columns n .. n + 3 of a row, of which `left` are inside.  (Rows of any length: the element's alignment is enough for one store.  One by one where rows are no multiple of four
+// columns: 1064 x 4959 x 496 23.1 us, 18.7 so; 865 x 333 x 10304 in f32 39 and 32.)
 template <typename Y>
-__device__ __forceinline__ void store_row4(Y *y, int n, int left, const float4_t &v, bool aligned) { // columns n .. n + 3, of which `left` are inside
-    if (aligned && left >= 4) {
-        if constexpr (sizeof(Y) == 2) {
-            typedef __attribute__((ext_vector_type(4))) _Float16 half4_t;
-            *reinterpret_cast<half4_t *>(y + n) = half4_t{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
-        } else {
-            *reinterpret_cast<float4_t *>(y + n) = v;
-        }
+__device__ __forceinline__ void store_row4(Y *y, int n, int left, const float4_t &v) {
+    typedef Y any __attribute__((ext_vector_type(4), aligned(sizeof(Y))));
+    if (left >= 4) {
+        *reinterpret_cast<any *>(y + n) = any{(Y)v[0], (Y)v[1], (Y)v[2], (Y)v[3]};
         return;
     }
 #pragma unroll
@@ -203,13 +201,12 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
     for (int j = 0; j < kNF; j++) red[wave][j][lane] = acc[j];
     __syncthreads();
     Y *y = reinterpret_cast<Y *>(p.y);
-    const bool aligned = p.n % 4 == 0;
     for (int s = tid; s < kNF * kWave; s += kRfWaves * kWave) {
         const int f = s / kWave, l = s % kWave, r = l & 15, n = n0 + f * 16 + (l >> 4) * 4;
         float4_t v = red[0][f][l];
 #pragma unroll
         for (int w = 1; w < kRfWaves; w++) v += red[w][f][l];
-        if (r < p.m && n < p.n) store_row4(y + (size_t)r * p.n, n, p.n - n, v, aligned);
+        if (r < p.m && n < p.n) store_row4(y + (size_t)r * p.n, n, p.n - n, v);
     }
 }
 
@@ -448,7 +445,6 @@ __global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN == 8 || kStages * (kMT *
         work(t, [&](int i) __attribute__((always_inline)) { fetch1(b, t + kStages, i); });
     }
     wait_vmcnt<0>(); // nothing is on its way to LDS when the workgroup ends
-    const bool aligned = p.n % 4 == 0;
 #pragma unroll
     for (int i = 0; i < kMT; i++) {
         const int r = m0 + (wm * kMT + i) * 16 + c;
@@ -457,8 +453,8 @@ __global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN == 8 || kStages * (kMT *
         for (int j = 0; j < kNT; j++) {
             const int n = nw + j * 16 + h * 4;
             if (n >= p.n) continue;
-            if (pp.parts) store_row4(pp.parts + ((size_t)piece * p.m + r) * p.n, n, p.n - n, acc[i][j], aligned);
-            else store_row4(reinterpret_cast<Y *>(p.y) + (size_t)r * p.n, n, p.n - n, acc[i][j], aligned);
+            if (pp.parts) store_row4(pp.parts + ((size_t)piece * p.m + r) * p.n, n, p.n - n, acc[i][j]);
+            else store_row4(reinterpret_cast<Y *>(p.y) + (size_t)r * p.n, n, p.n - n, acc[i][j]);
         }
     }
 }
@@ -467,10 +463,11 @@ __global__ __launch_bounds__(kWM *kWN *kWave, kWM * kWN == 8 || kStages * (kMT *
 template <typename Y>
 __global__ __launch_bounds__(256) void matmul_f8_join_kernel(Y *y, const float *parts, int pieces, size_t count) {
     for (size_t i = (blockIdx.x * (size_t)256 + threadIdx.x) * 4; i < count; i += (size_t)gridDim.x * 1024) {
-        if (i + 4 <= count && count % 4 == 0) {
-            float4_t v = *reinterpret_cast<const float4_t *>(parts + i);
-            for (int s = 1; s < pieces; s++) v += *reinterpret_cast<const float4_t *>(parts + s * count + i);
-            store_row4(y + i, 0, 4, v, true);
+        typedef float any __attribute__((ext_vector_type(4), aligned(4)));
+        if (i + 4 <= count) {
+            float4_t v = *reinterpret_cast<const any *>(parts + i);
+            for (int s = 1; s < pieces; s++) v += *reinterpret_cast<const any *>(parts + s * count + i);
+            store_row4(y + i, 0, 4, v);
         } else {
             for (size_t e = i; e < count && e < i + 4; e++) {
                 float v = parts[e];

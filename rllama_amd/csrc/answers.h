@@ -12,6 +12,7 @@ struct AttnSharedParams {
     void *out;
     int f16;                    // type of q and out
     int exact;                  // nothing is rounded but the result
+    int form;                   // 0: what takes less time, 1: 16 rows at a time, 2: tiles
     PlaneRef prefix_k, prefix_v; // [n_kv * prefix_rows x head_dim], of which prefix_len rows of each head are seen by every row
     PlaneRef cache_k, cache_v;  // [n_seqs * n_kv * max_seq_len x head_dim]
     int cache;                  // PlaneType of all four

@@ -62,6 +62,7 @@ extern "C" int rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_t
     p.out = out->p;
     p.f16 = q->dtype == RLH_F16;
     p.exact = ctx->tun.attn_exact;
+    p.form = ctx->tun.attn_shared_form;
     if (prefix_k) {
         p.prefix_k = plane_of(prefix_k);
         p.prefix_v = plane_of(prefix_v);

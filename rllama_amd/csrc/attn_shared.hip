@@ -7,9 +7,9 @@
 //
 // A workgroup takes rows of one key and value head, whatever texts they are of; its steps are the prefix's and then every one of its texts', masked for the rows of the others.  They
 // are cut into pieces; where there is only one the result is final, and pieces leave (m, sum, O) of their rows in work memory, which a second launch joins.
-//   Few rows per key and value head, f32 arithmetic, or where nothing may be rounded but the result: 16 rows at a time, from memory into registers (attn_rows_device.h).
-//   Many rows of each text: 128 at a time, through tiles of keys in LDS (attn_tiles_device.h, f16 arithmetic).
-//   Many rows, but few of each text: the prefix in tiles; 128 rows would be of too many texts for the texts' own positions, which go 16 rows at a time beside them in the same launch.
+//   Few rows or few positions, f32 arithmetic, or where nothing may be rounded but the result: 16 rows at a time, from memory into registers (attn_rows_device.h).
+//   Many rows of each text and many positions: 128 rows at a time, through tiles of keys in LDS (attn_tiles_device.h, f16 arithmetic).
+//   Many rows and positions, but few rows of each text: the prefix in tiles; 128 rows would be of too many texts for the texts' own positions, which go 16 rows at a time beside them in the same launch.
 //
 // Measured (heads of 128): a row each of 4 texts behind 383 positions, 32 heads: 9.8 us, the latency of one workgroup per head; of 64 texts behind 6001, 32 heads on 8: 26 us, 60 MB; of
 // 16 texts behind 65700, 64 heads on 8, 4 bits: 58 us, 590 TFLOP/s, conversions beside the products; 3 rows of 8 texts behind 1031, 32 heads in f32: 20 us, 2.3 TB/s of memory;
@@ -250,19 +250,19 @@ static double makespan(int places, const int64_t (&count)[2], const double (&us)
     return std::max(end, first);
 }
 
-// How a call is cut.  A workgroup of 16 rows takes `rows_fixed` and, with 128 dims, `rows_step` for every step (32 positions, 16 in f32) of its busiest wavefront; one of 128 rows
-// `tiles_fixed` and `tiles_step` for every 128 positions; partial results go to memory and back, and a launch joins them.  The numbers of pieces with the least sum are taken.
+// How a call is cut, with or without tiles, and how long that takes.  A workgroup of 16 rows takes `fixed` and `per_step` for every step (32 positions, 16 in f32) of its busiest wavefront;
+// one of 128 rows the same for every 128 positions; partial results go to memory and back, and a launch joins them.  The numbers of pieces with the least sum are taken.
 // The tiles' workgroups start first, the others fill what is left.
-SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
-    SharedPlan c{};
+static double plan_form(const AttnSharedParams &a, int compute_units, bool tiles, SharedPlan &c) {
+    c = SharedPlan{};
     const int group = a.n_heads / a.n_kv;
     const int64_t rows = (int64_t)a.n * group, all = rows * a.n_seqs;
     const bool f16 = f16_arithmetic(a), q4 = a.cache == kPlaneQ4;
-    const double scale = a.head_dim / 128.0;
-    const double fixed[2] = {7.0, 3.0}, per_step[2] = {(q4 ? 2.6 : 1.9) * scale, (q4 ? 1.6 : 1.2) * scale};
+    const double size = a.head_dim / 128.0;
+    const double launch = tiles ? 0.0 : 2.0, fixed[2] = {7.0, tiles ? 3.0 : 2.0}, per_step[2] = {(q4 ? 2.6 : 1.9) * size, tiles ? (q4 ? 1.6 : 1.2) * size : (q4 ? 1.15 : 1.0) * (0.6 + 1.4 * size)};
     const int step[2] = {kSharedTile, f16 ? 32 : 16}, together[2] = {kAtRows, kAwRows};
     // which parts there are, and what they have
-    const bool rounds = f16 && !a.exact, texts_tiles = rounds && rows > 2 * kAwRows, tiles = texts_tiles || (rounds && all > 2 * kAwRows && a.prefix_len > 0);
+    const bool texts_tiles = tiles && (rows > 2 * kAwRows || a.prefix_len == 0);
     c.part[0].prefix = tiles;
     c.part[0].texts = texts_tiles;
     c.part[1].prefix = !tiles;
@@ -287,7 +287,7 @@ SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
             mean[k] += (double)(steps - first) / p.blocks;
         }
     }
-    const int places = compute_units * (a.head_dim == 128 || tiles ? 1 : 2); // (registers, and LDS of tiles)
+    const int places = compute_units; // (two small workgroups on a compute unit take turns)
     const int most[2] = {std::min(kMaxPieces / 2, longest[0]), std::min(kMaxPieces / 2, (longest[1] + kAwWaves - 1) / kAwWaves)};
     auto time_of = [&](int k, int n) { // a workgroup of average length, cut into n
         const double part = n > 0 ? std::min((double)((longest[k] + n - 1) / n), mean[k]) : 0.0;
@@ -342,7 +342,16 @@ SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
     }
     c.joined = c.slots > 1;
     c.work_floats = c.joined ? (size_t)(all - c.cut) * a.n_kv * c.slots * (a.head_dim + 2) : 0;
-    return c;
+    return least + launch;
+}
+SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
+    const int64_t rows = (int64_t)a.n * (a.n_heads / a.n_kv), all = rows * a.n_seqs;
+    SharedPlan c, d;
+    const double us = plan_form(a, compute_units, false, c);
+    // Tiles take 128 rows of one head, of up to 16 texts where these go through tiles as well.  The estimates take the slower form by 0.5 % on average over 60 calls of all sizes, 16 % at
+    // worst; tiles for all of more than 32 rows took up to 2.5 times as long (245 rows of 16 heads behind 120 positions 20 us, 8; 1722 rows of 4 heads behind 8316 are 49 in tiles and 151).
+    if (a.form == 1 || !f16_arithmetic(a) || a.exact || all <= 2 * kAwRows || (a.prefix_len == 0 && rows < kAtRows / (kMaxTexts - 1) + 1)) return c;
+    return plan_form(a, compute_units, true, d) < us || a.form == 2 ? d : c;
 }
 
 template <typename AC, typename QT, typename CT, int HD>

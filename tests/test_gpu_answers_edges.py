@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 
 import rllama_amd
+import test_gpu_answers as base
 from rllama_amd import Context, Tensor, TensorDType
 from test_gpu_answers import F8, TILES, decode, encode, first_of_the_largest, logprobs_reference, shared_reference, stands_for
 from test_gpu_longctx import EPS16, EPS32, INVALID, STATE, UNSUPPORTED, f16, f32, f64, refused, upload, values
@@ -103,6 +104,7 @@ def test_work_memory_is_not_allocated_while_captured():
     """Calls that need work memory are refused while the stream is captured, nothing is recorded of them, and they run afterwards."""
     ctx = Context(0)
     hip = hip_runtime()
+    ctx.set_option("ATTN_SHARED_FORM", "2")  # (with partial results)
     step = Step(ctx, 3, B=70)
     step.next_input()
     ctx.sync()
@@ -304,6 +306,45 @@ def test_products_longer_than_32_bits(ctx, m, n, k, result):
     finally:
         for memory in (X, W, Y):
             memory.free()
+
+
+# -- the form that the estimate does not choose ---------------------------------------------------------------------------------------------
+
+@pytest.fixture(params=["1", "2"])
+def form(ctx, request):
+    ctx.set_option("ATTN_SHARED_FORM", request.param)
+    yield ctx
+    ctx.set_option("ATTN_SHARED_FORM", None)
+
+
+@pytest.mark.parametrize("case", base.SHARED)
+@pytest.mark.parametrize("kind,cache", [("f16", "f16"), ("f16", "q4")])
+def test_both_forms(form, case, kind, cache):
+    base.test_attention_behind_a_shared_prefix(form, *case, kind, cache)
+
+
+@pytest.mark.parametrize("P", [1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 191, 255, 256, 257, 383, 511, 513, 1025, 3000])
+@pytest.mark.parametrize("cache,B", [("f16", 20), ("q4", 20), ("f16", 70)])
+def test_both_forms_of_prefixes_of_every_length(form, P, cache, B):
+    base.test_prefixes_of_every_length(form, P, "f16", cache, B)
+
+
+@pytest.mark.parametrize("n,B", [(1, 40), (20, 5), (70, 4)])
+def test_both_forms_of_scores_far_apart(form, n, B):
+    base.test_scores_far_apart(form, "f16", n, B)
+
+
+@pytest.mark.parametrize("cache", ["f16", "q4"])
+@pytest.mark.parametrize("B,n,group", [(30, 1, 4), (4, 20, 1), (12, 7, 3), (5, 20, 2), (3, 34, 4)])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_both_forms_of_values_that_are_not_finite(form, cache, B, n, group, value):
+    base.test_values_that_are_not_finite_reach_the_rows_that_see_them(form, "f16", cache, B, n, group, value)
+
+
+@pytest.mark.parametrize("cache", ["f16", "q4"])
+@pytest.mark.parametrize("hd,n,P,starts", [(32, 40, 256, [-40, -40, -99]), (64, 1, 0, [-2] * 40), (128, 50, 0, [-50]), (128, 1, 500, [-1] * 40)])
+def test_both_forms_of_nothing_but_padding(form, cache, hd, n, P, starts):
+    base.test_nothing_but_padding(form, "f16", cache, hd, n, P, starts)
 
 
 def test_more_rows_than_a_launch_takes(ctx):

@@ -287,7 +287,7 @@ static double plan_form(const AttnSharedParams &a, int compute_units, bool tiles
             mean[k] += (double)(steps - first) / p.blocks;
         }
     }
-    const int places = compute_units; // (two small workgroups on a compute unit take turns)
+    const int places = compute_units; // (small workgroups that share one take turns)
     const int most[2] = {std::min(kMaxPieces / 2, longest[0]), std::min(kMaxPieces / 2, (longest[1] + kAwWaves - 1) / kAwWaves)};
     auto time_of = [&](int k, int n) { // a workgroup of average length, cut into n
         const double part = n > 0 ? std::min((double)((longest[k] + n - 1) / n), mean[k]) : 0.0;
@@ -348,7 +348,7 @@ SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
     const int64_t rows = (int64_t)a.n * (a.n_heads / a.n_kv), all = rows * a.n_seqs;
     SharedPlan c, d;
     const double us = plan_form(a, compute_units, false, c);
-    // Tiles take 128 rows of one head, of up to 16 texts where these go through tiles as well.  The estimates take the slower form by 0.5 % on average over 60 calls of all sizes, 16 % at
+    // Tiles take 128 rows of one head, of up to 16 texts where these go through tiles as well.  The estimates cost 1.2 % over the faster form on average over 160 calls of all sizes, 32 % at
     // worst; tiles for all of more than 32 rows took up to 2.5 times as long (245 rows of 16 heads behind 120 positions 20 us, 8; 1722 rows of 4 heads behind 8316 are 49 in tiles and 151).
     if (a.form == 1 || !f16_arithmetic(a) || a.exact || all <= 2 * kAwRows || (a.prefix_len == 0 && rows < kAtRows / (kMaxTexts - 1) + 1)) return c;
     return plan_form(a, compute_units, true, d) < us || a.form == 2 ? d : c;

@@ -50,7 +50,7 @@ struct OpScratch {
     float *window_ws = nullptr;    // rlh_attn_window: partial results of sequences that are cut
     size_t window_ws_floats = 0;
     AnswerWork shared_work;        // rlh_attn_shared: partial results
-    AnswerWork f8_work;            // rlh_matrix_mul_f8: src in 8 bits
+    AnswerWork f8_work;            // rlh_matrix_mul_f8: sums of pieces of K, src in 8 bits
 };
 constexpr int kOpMaxHeads = 1024;
 

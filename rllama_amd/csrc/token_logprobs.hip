@@ -74,9 +74,9 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
     return __builtin_bit_cast(float, w & 0x80000000u ? w & 0x7fffffffu : ~w);
 }
 
-// kKeep: pieces of kN entries that a thread keeps; 0: rows of any length.  kMany: of more rows than compute units, two to a compute unit.  c2 = log2(e) / T.
+// kKeep: pieces of kN entries that a thread keeps; 0: rows of any length.  kMany: of more rows than compute units, two to a compute unit.  c2 = log2(e) / T, inverse = 1 / T.
 template <typename T, int kThreads, int kN, int kKeep, bool kMany>
-__global__ __launch_bounds__(kThreads, kMany && kN > 2 ? 8 : 4) void token_logprobs_kernel(LogprobsParams p, float c2) {
+__global__ __launch_bounds__(kThreads, kMany && kN > 2 ? 8 : 4) void token_logprobs_kernel(LogprobsParams p, float c2, float inverse) {
     typedef RowPiece<T, kN> Piece;
     constexpr int kStep = kThreads * kN, kWaves = kThreads / kWave, kLanes = kThreads / kTlGroups;
     __shared__ __attribute__((aligned(16))) float group_top[kTlGroups];
@@ -154,10 +154,14 @@ __global__ __launch_bounds__(kThreads, kMany && kN > 2 ? 8 : 4) void token_logpr
         above = group_sum<kLanes>(above);
         if (tid % kLanes == 0) group_low[tid / kLanes] = above < (float)p.top ? -own : -INFINITY;
     }
-    // ---- the sums.  f16: z = x c2 - m c2 in one operation; m c2 was rounded, which shifts all z by the same `shift`.  f32: the difference first, since m c2 may not be
-    // representable.  (A bound keeps 0 * infinity out of the second sum.)
-    const float mc = sizeof(T) == 2 ? base * c2 : 0.0f, shift = sizeof(T) == 2 ? fmaf(base, c2, -mc) : 0.0f;
-    auto exponent = [&](float v) { return sizeof(T) == 2 ? fmaf(v, c2, -mc) : (v - base) * c2; };
+    // ---- the sums.  f16: z = x c2 - m c2 in one operation; m c2 was rounded, which shifts all z by the same `shift`, half a unit of m c2.  f32: the difference first, since
+    // m c2 may not be representable.  (A bound keeps 0 * infinity out of the second sum.)
+    // f16 with |m c2| from 2^24 on (a low temperature), where that unit grows without bound: numbers of 11 bits that differ from m differ by 2^-11 of it at least, so their z
+    // are below -2^12 and their weights 0 whatever c2 is.  A power of two in its place, m c2 between 2^23 and 2^24, gives the same sums with no shift.
+    const bool far = sizeof(T) == 2 && fabsf(base) * c2 >= 16777216.0f;
+    const float by = far ? ldexpf(1.0f, 24 - __builtin_amdgcn_frexp_expf(base)) : c2;
+    const float mc = sizeof(T) == 2 ? base * by : 0.0f, shift = sizeof(T) == 2 ? fmaf(base, by, -mc) : 0.0f;
+    auto exponent = [&](float v) { return sizeof(T) == 2 ? fmaf(v, by, -mc) : (v - base) * c2; };
     float s = 0.0f, u = 0.0f, count = 0.0f;
     if (mine < m || !(m > -INFINITY)) {
         pieces([&](const Piece &piece, auto) {
@@ -203,7 +207,7 @@ __global__ __launch_bounds__(kThreads, kMany && kN > 2 ? 8 : 4) void token_logpr
     const float e_top = __builtin_amdgcn_exp2f(shift);
     const float others = fmaf(fmaxf(count - 1.0f, 0.0f), e_top, s) / e_top; // (a thread each left out one of several that are the largest)
     const float log_s = log1pf(others), u_top = (u - shift * s) / e_top;
-    auto logprob = [&](float v) { return odd ? NAN : none ? -INFINITY : fmaf(exponent(v) - shift, kLn2, -log_s); };
+    auto logprob = [&](float v) { return odd ? NAN : none ? -INFINITY : fmaf(v - base, inverse, -log_s); };
     if (tid == 0 && p.entropy) p.entropy[row] = odd ? NAN : none ? 0.0f : log_s - kLn2 * u_top / (1.0f + others);
     for (int i = tid; i < p.n_tokens; i += kThreads) {
         const int id = i == tid ? token : p.tokens[(size_t)row * p.n_tokens + i];
@@ -348,6 +352,7 @@ __global__ __launch_bounds__(kThreads, kMany && kN > 2 ? 8 : 4) void token_logpr
     for (int i = tid; i < found; i += kThreads) {
         const unsigned long long key = list[i];
         int at = 0;
+#pragma unroll 1 // (32 places at a time took twice the registers of all that came before, and spilled)
         for (int j = 0; j < found; j += 8) // (places behind the last one are 0)
 #pragma unroll
             for (int u = 0; u < 8; u++) at += list[j + u] > key;
@@ -361,7 +366,7 @@ __global__ __launch_bounds__(kThreads, kMany && kN > 2 ? 8 : 4) void token_logpr
 template <typename T, bool kMany>
 static void launch_t(const LogprobsParams &p, hipStream_t s) {
     constexpr int kN = 16 / (int)sizeof(T);
-    const float c2 = (float)(1.44269504088896340736 / (double)p.temperature);
+    const float c2 = (float)(1.44269504088896340736 / (double)p.temperature), inverse = (float)(1.0 / (double)p.temperature);
     const dim3 grid((unsigned)p.rows);
     // Narrow pieces in short rows, so that 33 groups at least hold entries: 20 or 32 alternatives of 500 entries, or of 2100 in f16, took 85 to 150 us in pieces of sixteen
     // bytes, whose few groups give no bound, and take less than 20 so, as those of other lengths do.
@@ -369,13 +374,13 @@ static void launch_t(const LogprobsParams &p, hipStream_t s) {
     // share a compute unit (f16, five alternatives: 2048 rows of 32000 41 -> 37 us, of 10000 38.5 -> 21, of 6000 24 -> 15; 800 rows 22.1 / 22.3, 20.9 / 12.7, 13 / 8.6;
     // 400 rows of 32000 13.6 -> 14.1).
     const bool crowd = p.rows > kTlCrowd;
-    if (p.vocab <= 2048) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 2, 4, kMany>), grid, dim3(256), 0, s, p, c2);
-    else if (crowd && p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, kN, 32 / kN, true>), grid, dim3(256), 0, s, p, c2);
-    else if (crowd && p.vocab <= 16384) hipLaunchKernelGGL((token_logprobs_kernel<T, kN == 8 ? 256 : 512, kN, 8, true>), grid, dim3(kN == 8 ? 256 : 512), 0, s, p, c2);
-    else if (crowd && p.vocab <= 32768 && kN == 8) hipLaunchKernelGGL((token_logprobs_kernel<T, 512, kN, 8, true>), grid, dim3(512), 0, s, p, c2);
-    else if (p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 4, 2, kMany>), grid, dim3(1024), 0, s, p, c2);
-    else if (p.vocab <= 32768) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, kN, 32 / kN, kMany>), grid, dim3(1024), 0, s, p, c2);
-    else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, kN, 0, kMany>), grid, dim3(1024), 0, s, p, c2);
+    if (p.vocab <= 2048) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 2, 4, kMany>), grid, dim3(256), 0, s, p, c2, inverse);
+    else if (crowd && p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, kN, 32 / kN, true>), grid, dim3(256), 0, s, p, c2, inverse);
+    else if (crowd && p.vocab <= 16384) hipLaunchKernelGGL((token_logprobs_kernel<T, kN == 8 ? 256 : 512, kN, 8, true>), grid, dim3(kN == 8 ? 256 : 512), 0, s, p, c2, inverse);
+    else if (crowd && p.vocab <= 32768 && kN == 8) hipLaunchKernelGGL((token_logprobs_kernel<T, 512, kN, 8, true>), grid, dim3(512), 0, s, p, c2, inverse);
+    else if (p.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 4, 2, kMany>), grid, dim3(1024), 0, s, p, c2, inverse);
+    else if (p.vocab <= 32768) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, kN, 32 / kN, kMany>), grid, dim3(1024), 0, s, p, c2, inverse);
+    else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, kN, 0, kMany>), grid, dim3(1024), 0, s, p, c2, inverse);
 }
 
 hipError_t launch_token_logprobs(const LogprobsParams &all, hipStream_t s) {

@@ -1,0 +1,58 @@
+"""The operators for many answers to one prompt at the ends of what their calls accept: temperatures and logits at the types' limits, batches of nothing but padding,
+rows of padding that hold anything."""
+import numpy as np
+import pytest
+
+from rllama_amd import Tensor
+from test_gpu_answers import first_of_the_largest, logprobs_reference
+from test_gpu_longctx import EPS32, NUMPY, f16, f32, f64
+
+pytestmark = pytest.mark.gpu
+
+
+# -- log probabilities --------------------------------------------------------------------------------------------------------------------
+
+def check_logprobs(ctx, x, temperature, top=5):
+    """All results of rows x against 64 bits.  An exponent is the difference of two logits (exact or rounded once) times 1 / temperature (rounded once); the weights' sum,
+    all of them positive, and its logarithm add the rest, as in test_logprobs."""
+    rows, vocab = x.shape
+    top = min(top, vocab)
+    ids = first_of_the_largest(x, vocab)
+    tokens = np.ascontiguousarray(ids[:, [0, min(1, vocab - 1), vocab // 2, vocab - 1]])
+    got = [t.to_numpy().astype(f64) for t in Tensor.from_numpy(ctx, x).token_logprobs(Tensor.from_numpy(ctx, tokens), temperature, top)]
+    with np.errstate(over="ignore", invalid="ignore"):
+        want, entropy = logprobs_reference(x, temperature)
+        for g, w in ((got[0], np.take_along_axis(want, tokens, 1)), (got[3], np.take_along_axis(want, ids[:, :top], 1))):
+            tol = EPS32 * (8 + 2 * np.sqrt(vocab) + 6 * np.abs(w) + 6 * np.log(vocab))
+            assert not np.isnan(g).any()
+            lost = w.astype(f32) == -np.inf  # (past what 32 bits hold)
+            assert ((g == -np.inf) & lost | ~lost & (np.abs(g - w) <= tol)).all()
+    assert (np.abs(got[1] - entropy) <= EPS32 * (16 + 2 * np.sqrt(vocab)) * (np.abs(entropy) + np.log(vocab) * (vocab > 1) * 8)).all()
+    assert np.array_equal(got[2], ids[:, :top])
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-12, 1e-9, 3e-9, 1e-8, 1e-7, 1e-6, 4e-5, 1e-3, 0.05, 1e3, 1e30])
+@pytest.mark.parametrize("vocab", [33, 1000, 6000, 10000, 32000, 40000])
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+def test_logprobs_at_every_temperature(ctx, vocab, kind, temperature):
+    """Rows whose largest entry is small, large, negative, the type's largest and smallest number and 0, alone and shared by several."""
+    rng = np.random.default_rng(vocab)
+    info = np.finfo(NUMPY[kind])
+    x = np.concatenate([rng.standard_normal((3, vocab)) * 3, rng.standard_normal((3, vocab)) * 30, rng.standard_normal((2, vocab)) - 700, np.zeros((6, vocab))]).astype(NUMPY[kind])
+    x[8:] = -np.abs(rng.standard_normal((6, vocab))) * 5
+    x[8, 7], x[9, 9], x[10, 11], x[11, 3], x[12, 5] = info.max, info.max, info.tiny, info.smallest_subnormal if kind == "f16" else info.tiny, 0.0
+    x[13] = info.min / 2
+    for r, copies in ((1, 2), (4, 30), (7, 3), (9, 2), (10, 7), (12, 4)):  # ties
+        x[r, rng.choice(vocab, copies, replace=False)] = x[r].max()
+    check_logprobs(ctx, x, temperature)
+
+
+@pytest.mark.parametrize("rows", [900])
+@pytest.mark.parametrize("vocab", [6000, 10000, 32000])
+def test_logprobs_of_many_rows_at_low_temperatures(ctx, rows, vocab):
+    """The kernels for many rows."""
+    rng = np.random.default_rng(vocab)
+    x = (rng.standard_normal((rows, vocab)) * 4).astype(f16)
+    x[::3, 17] = x[::3].max(1)
+    for temperature in (1e-9, 1e-30):
+        check_logprobs(ctx, x, temperature)

@@ -155,13 +155,14 @@ __global__ __launch_bounds__(kThreads, kMany && kN > 2 ? 8 : 4) void token_logpr
         if (tid % kLanes == 0) group_low[tid / kLanes] = above < (float)p.top ? -own : -INFINITY;
     }
     // ---- the sums.  f16: z = x c2 - m c2 in one operation; m c2 was rounded, which shifts all z by the same `shift`, half a unit of m c2.  f32: the difference first, since
-    // m c2 may not be representable.  (A bound keeps 0 * infinity out of the second sum.)
+    // m c2 may not be representable, and half of it, since the difference of two numbers may not be either.  (A bound keeps 0 * infinity out of the second sum.)
     // f16 with |m c2| from 2^24 on (a low temperature), where that unit grows without bound: numbers of 11 bits that differ from m differ by 2^-11 of it at least, so their z
     // are below -2^12 and their weights 0 whatever c2 is.  A power of two in its place, m c2 between 2^23 and 2^24, gives the same sums with no shift.
     const bool far = sizeof(T) == 2 && fabsf(base) * c2 >= 16777216.0f;
     const float by = far ? ldexpf(1.0f, 24 - __builtin_amdgcn_frexp_expf(base)) : c2;
     const float mc = sizeof(T) == 2 ? base * by : 0.0f, shift = sizeof(T) == 2 ? fmaf(base, by, -mc) : 0.0f;
-    auto exponent = [&](float v) { return sizeof(T) == 2 ? fmaf(v, by, -mc) : (v - base) * c2; };
+    const float half_base = 0.5f * base, c2_twice = 2.0f * c2, inverse_twice = 2.0f * inverse;
+    auto exponent = [&](float v) { return sizeof(T) == 2 ? fmaf(v, by, -mc) : fmaf(v, 0.5f, -half_base) * c2_twice; };
     float s = 0.0f, u = 0.0f, count = 0.0f;
     if (mine < m || !(m > -INFINITY)) {
         pieces([&](const Piece &piece, auto) {
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(kThreads, kMany && kN > 2 ? 8 : 4) void token_logpr
     const float e_top = __builtin_amdgcn_exp2f(shift);
     const float others = fmaf(fmaxf(count - 1.0f, 0.0f), e_top, s) / e_top; // (a thread each left out one of several that are the largest)
     const float log_s = log1pf(others), u_top = (u - shift * s) / e_top;
-    auto logprob = [&](float v) { return odd ? NAN : none ? -INFINITY : fmaf(v - base, inverse, -log_s); };
+    auto logprob = [&](float v) { return odd ? NAN : none ? -INFINITY : fmaf(fmaf(v, 0.5f, -half_base), inverse_twice, -log_s); };
     if (tid == 0 && p.entropy) p.entropy[row] = odd ? NAN : none ? 0.0f : log_s - kLn2 * u_top / (1.0f + others);
     for (int i = tid; i < p.n_tokens; i += kThreads) {
         const int id = i == tid ? token : p.tokens[(size_t)row * p.n_tokens + i];

@@ -56,3 +56,18 @@ def test_logprobs_of_many_rows_at_low_temperatures(ctx, rows, vocab):
     x[::3, 17] = x[::3].max(1)
     for temperature in (1e-9, 1e-30):
         check_logprobs(ctx, x, temperature)
+
+
+@pytest.mark.parametrize("vocab", [33, 6000, 32000, 40000])
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+def test_logprobs_of_logits_from_end_to_end(ctx, vocab, kind):
+    """The type's largest and lowest number in one row: their difference is past what 32 bits hold, its quotient by a high temperature is not."""
+    info = np.finfo(NUMPY[kind])
+    x = np.zeros((5, vocab), NUMPY[kind])
+    x[0, ::2], x[0, 1::2] = info.max, info.min
+    x[1, 4:], x[1, 3] = info.min, info.max
+    x[2, :], x[2, 30] = info.min, info.max
+    x[3, :] = np.linspace(-1, 1, vocab) * f64(info.max)
+    x[4, 1] = info.min
+    for temperature in (1.0, 1e30, 2.5e29, 1e-30):
+        check_logprobs(ctx, x, temperature)

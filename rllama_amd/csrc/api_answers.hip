@@ -78,7 +78,12 @@ extern "C" int rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_t
     p.max_seq_len = max_seq_len;
     p.n = n;
     p.n_seqs = n_seqs;
-    for (int b = 0; b < n_seqs; b++) p.start[b] = start_pos[b];
+    bool idle = true; // nothing but padding: zeros, and no position is seen
+    for (int b = 0; b < n_seqs; b++) {
+        p.start[b] = start_pos[b];
+        if ((int64_t)start_pos[b] + n > 0) idle = false;
+    }
+    if (idle) p.prefix_len = 0;
     const SharedPlan plan = plan_attn_shared(p, ctx->prop.multiProcessorCount);
     const int64_t rows = (int64_t)q->rows * (n_heads / n_kv_heads);
     if (plan.workgroups >= 1 << 23 || n_kv_heads > 65535 || rows > INT32_MAX) return fail(RLH_ERR_UNSUPPORTED, "%s: %lld rows on each of %d key and value heads are more than a launch takes", who, (long long)rows, n_kv_heads);

@@ -65,12 +65,12 @@ struct SharedView {
           first_slot(c.part[part].first_slot), cut(c.cut) {}
     __device__ float *partials(int g, int rows, int r, int hd) const { return ws + ((size_t)g * (rows - cut) + r - cut) * pieces * (hd + 2); }
 };
-// The prefix alone: all rows are at its last position.
+// The prefix alone: all rows are at its last position, padding too, and a join tells these apart.  (There is always one: of a call that sees a prefix some row has a position
+// of its own, so the texts' part has a piece.)
 struct PrefixView : SharedView {
     static constexpr bool kTexts = false;
-    bool apart; // results are left for a join whatever the number of pieces
-    __device__ explicit PrefixView(const SharedKernelParams &c) : SharedView(c, 0, false), apart(c.part[1].pieces > 0) {}
-    __device__ bool partial() const { return apart; }
+    __device__ explicit PrefixView(const SharedKernelParams &c) : SharedView(c, 0, false) {}
+    __device__ constexpr bool partial() const { return true; }
     __device__ int start(int) const { return a.prefix_len - 1; }
     __device__ int position(int start, int) const { return start; }
     __device__ int text(int) const { return 0; }

@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 
 from rllama_amd import Tensor
-from test_gpu_answers import first_of_the_largest, logprobs_reference
-from test_gpu_longctx import EPS32, NUMPY, f16, f32, f64
+from test_gpu_answers import first_of_the_largest, logprobs_reference, shared_case
+from test_gpu_longctx import EPS32, NUMPY, f16, f32, f64, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,41 @@ def test_logprobs_of_logits_from_end_to_end(ctx, vocab, kind):
     x[4, 1] = info.min
     for temperature in (1.0, 1e30, 2.5e29, 1e-30):
         check_logprobs(ctx, x, temperature)
+
+
+# -- attention: padding -------------------------------------------------------------------------------------------------------------------
+
+IDLE = [
+    # hd, heads, kv heads, rows of a text, prefix, texts
+    (128, 32, 32, 20, 2000, 64), (128, 32, 8, 4, 300, 128), (64, 64, 8, 1, 1000, 128), (128, 40, 40, 16, 1000, 33), (128, 4, 4, 1, 100, 40), (32, 8, 1, 3, 128, 30), (128, 2, 2, 40, 17, 2),
+]
+
+
+@pytest.fixture(params=[None, "1", "2"])
+def form(ctx, request):
+    """The form that the estimate chooses, and either of the two."""
+    ctx.set_option("ATTN_SHARED_FORM", request.param)
+    yield ctx
+    ctx.set_option("ATTN_SHARED_FORM", None)
+
+
+@pytest.mark.parametrize("hd,H,G,n,P,B", IDLE)
+@pytest.mark.parametrize("cache", ["f16", "q4"])
+def test_an_idle_batch_behind_a_prefix(form, hd, H, G, n, P, B, cache):
+    """Every text is padding: zeros, whatever the prefix's length and the number of rows."""
+    rng = np.random.default_rng(P)
+    pk, pv = (upload(form, rng.standard_normal((G * P, hd)), cache) for _ in range(2))
+    own = upload(form, np.full((B * G * n, hd), np.nan), cache)
+    q = Tensor.from_numpy(form, rng.standard_normal((B * n, H * hd)).astype(f16))
+    for starts in ([-n] * B, [-n - b for b in range(B)]):
+        out = Tensor.from_numpy(form, np.full((B * n, H * hd), np.nan, f16))
+        q.attn_shared(pk, pv, P, own, own, H, G, n, starts, out=out)
+        assert (out.to_numpy() == 0).all()
+
+
+@pytest.mark.parametrize("hd,H,G,n,P,B", IDLE[4:])
+def test_one_text_of_an_idle_batch(form, hd, H, G, n, P, B):
+    starts = [-n] * (B - 1) + [1 - n]
+    out, want, bound, _, _ = shared_case(form, hd, H, G, n, P, P, 40, starts, "f16", "f16")
+    got = out.astype(f64).reshape(want.shape)
+    assert (np.abs(got - want) <= bound).all() and (got[:-1] == 0).all() and (got[-1, -1] != 0).all()

@@ -511,8 +511,8 @@ __device__ __forceinline__ void attn_rows(const View &v, RowsShared<HD> &shared,
     // ---- join the wavefronts
     l_run = col_sum(l_run);
     if (h == 0) {
-        sm[wave][m] = m_run * queries.up;
-        sl[wave][m] = my_p < 0 ? 0.0f : l_run; // (padding: 0)
+        sm[wave][m] = View::kTexts && my_p < 0 ? -INFINITY : m_run * queries.up; // (padding sees nothing, whatever its query's scores on a shared prefix are)
+        sl[wave][m] = my_p < 0 ? 0.0f : l_run;
     }
 #pragma unroll
     for (int x = 0; x < 4; x++)

@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 
 from rllama_amd import Tensor
-from test_gpu_answers import first_of_the_largest, logprobs_reference, shared_case
-from test_gpu_longctx import EPS32, NUMPY, f16, f32, f64, upload
+from test_gpu_answers import first_of_the_largest, logprobs_reference, shared_case, shared_reference
+from test_gpu_longctx import EPS16, EPS32, NUMPY, TYPES, f16, f32, f64, upload, values
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,32 @@ def test_one_text_of_an_idle_batch(form, hd, H, G, n, P, B):
     out, want, bound, _, _ = shared_case(form, hd, H, G, n, P, P, 40, starts, "f16", "f16")
     got = out.astype(f64).reshape(want.shape)
     assert (np.abs(got - want) <= bound).all() and (got[:-1] == 0).all() and (got[-1, -1] != 0).all()
+
+
+@pytest.mark.parametrize("kind,cache", TYPES)
+@pytest.mark.parametrize("hd,H,G,n,P,B", [(64, 4, 2, 1, 150, 5), (128, 8, 2, 3, 40, 9), (32, 6, 2, 1, 3000, 4), (64, 4, 4, 30, 700, 5), (128, 16, 2, 1, 900, 40), (64, 2, 1, 70, 60, 3), (128, 4, 1, 12, 0, 6)])
+def test_padding_rows_hold_anything(form, hd, H, G, n, P, B, kind, cache):
+    """Queries of padding rows are infinite, NaN, or the type's largest number, which overflows with any key: their results are zeros, and the other rows do not notice."""
+    rng = np.random.default_rng(P + n)
+    S = 90
+    info = np.finfo(NUMPY[kind])
+    starts = [0 if b % 3 == 0 else -n if b % 3 == 1 else -(n // 2) for b in range(B)]  # whole, idle, and padding in front
+    q = rng.standard_normal((B, n, H, hd)).astype(NUMPY[kind])
+    for b, start in enumerate(starts):
+        for i in range(min(n, -start)):
+            q[b, i, :, ::[1, hd][b % 2]] = [np.inf, -np.inf, np.nan, info.max, info.min][(b + i) % 5]  # (all dims, or the first alone: scores that are infinite, or not numbers)
+            q[b, i, :, 1::2] *= [1, -1][i % 2]
+    planes = [upload(form, rng.standard_normal((rows, hd)), cache) for rows in (G * max(P, 1), G * max(P, 1), B * G * S, B * G * S)]
+    wide = [values(t).reshape(G, -1, hd)[:, :P] if i < 2 else values(t).reshape(B, G, S, hd) for i, t in enumerate(planes)]
+    clean = q.astype(f64)
+    for b, start in enumerate(starts):
+        clean[b, :max(0, min(n, -start))] = 0
+    want, bound = shared_reference(clean, *wide, starts)
+    if kind == "f16":  # the result is rounded to f16; the weights may be
+        bound = bound + 2 * EPS16 * max(np.abs(x).max() for x in (wide[1], wide[3]) if x.size)
+    out = Tensor.from_numpy(form, np.full((B * n, H * hd), np.nan, NUMPY[kind]))
+    Tensor.from_numpy(form, q.reshape(B * n, -1)).attn_shared(*planes[:2], P, *planes[2:], H, G, S, starts, out=out)
+    got = out.to_numpy().astype(f64).reshape(want.shape)
+    for b, start in enumerate(starts):
+        assert (got[b, :max(0, min(n, -start))] == 0).all()
+    assert (np.abs(got - want) <= bound).all()

@@ -18,7 +18,7 @@ OBJ = os.path.join(HERE, "_obj")
 LIB = os.path.join(HERE, "librllama_hip.so")
 
 SOURCES = ["gemv.hip", "attention.hip", "gemm.hip", "gemm_dma.hip", "gemm_kgroup.hip", "gemm_split3.hip", "gemm_skinny.hip", "gemm_rows.hip", "gemm_rows_fused.hip", "gemm_rows_f32.hip", "attn_prefill.hip", "prefill.hip", "prefill_f32.hip", "misc.hip", "sampler.hip", "qkv_append.hip", "attn_window.hip", "attn_tiles.hip", "token_choice.hip", "attn_shared.hip", "token_logprobs.hip", "f8_convert.hip", "gemm_f8.hip", "api.hip", "api_ops.hip", "api_longctx.hip", "api_answers.hip"]
-HEADERS = ["kernels.h", "device_utils.h", "gemv_device.h", "gemm_epilogue.h", "gemm_rows_device.h", "split3_plan.h", "tensor_pool.h", "q4.h", "longctx.h", "attn_window_device.h", "attn_rows_device.h", "attn_tiles_device.h", "f8.h", "answers.h", "api_planes.h", "synth.h", "api_internal.h", os.path.join("..", "..", "include", "rllama_hip.h")]  # relative to csrc/
+HEADERS = ["kernels.h", "device_utils.h", "gemv_device.h", "gemm_epilogue.h", "gemm_rows_device.h", "split3_plan.h", "tensor_pool.h", "q4.h", "longctx.h", "attn_window_device.h", "attn_rows_device.h", "attn_tiles_device.h", "f8.h", "f8_layout.h", "answers.h", "api_planes.h", "synth.h", "api_internal.h", os.path.join("..", "..", "include", "rllama_hip.h")]  # relative to csrc/
 
 HIPCC = os.environ.get("HIPCC") or shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 FLAGS = [

@@ -6,10 +6,10 @@
 #pragma once
 
 #include "device_utils.h"
+#include "f8_layout.h"
 
 namespace rlh {
 
-constexpr int kF8Block = 128;
 constexpr float kF8Largest = 448.0f; // of e4m3
 
 struct EightRef {
@@ -17,8 +17,6 @@ struct EightRef {
     float *scales;
     int rows; // that share a scale: 1 or 128
 };
-
-__host__ __device__ inline int f8_blocks(int cols) { return (cols + kF8Block - 1) / kF8Block; }
 
 // Scale and factor of a block whose largest value is `top` (finite): value = code * scale, code = e4m3(value * factor).  The bound keeps both normal numbers; below it
 // a block is all but zero.  (The factor is a reciprocal and a product, two roundings, as array libraries divide a number by an array: codes made there and here are the same.)

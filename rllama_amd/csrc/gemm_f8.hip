@@ -58,11 +58,7 @@ struct RowsF8Params {
     MatmulF8Params p;
     const void *src; // f16 or f32 rows, converted on the way
 };
-constexpr int kRfWaves = 8;
-constexpr int kRfRow = kF8Block + 16; // of a block's codes in LDS: padded, so that rows lie in different banks
-constexpr int kRfLds = 96 * 1024;     // for converted rows
-static int rows_f8_share(int k) { return (f8_blocks(k) + kRfWaves - 1) / kRfWaves; } // blocks of a wavefront
-static size_t rows_f8_lds(int m, int k) { return (size_t)kRfWaves * rows_f8_share(k) * m * (kRfRow + 4); }
+constexpr int kRfLds = 96 * 1024; // for converted rows
 
 template <int kNF, int kSource, typename Y>
 __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8Params pp) {
@@ -114,8 +110,8 @@ __global__ __launch_bounds__(kRfWaves *kWave) void matmul_f8_rows_kernel(RowsF8P
         return b < across ? b : b - across;
     };
     // converted rows: the wavefront's block t is its t / 8-th
-    const int share = (across + kRfWaves - 1) / kRfWaves;
-    unsigned char *const codes = converted + (size_t)wave * share * p.m * (kRfRow + 4);
+    const int share = rows_f8_share(p.k);
+    unsigned char *const codes = converted + wave * rows_f8_region(p.m, p.k);
     float *const scales = reinterpret_cast<float *>(codes + (size_t)share * p.m * kRfRow);
     Block now, next;
     if constexpr (kSource == kF8Codes) {

@@ -58,11 +58,12 @@ struct PartParams {
 struct SharedView {
     PartParams p;
     const AttnSharedParams &a;
-    float *ws;
-    int pieces, piece_steps, first_slot, cut;
+    float *const &ws; // (references, as in WindowView)
+    const int &pieces, &first_slot, &cut;
+    int piece_steps;
     __device__ SharedView(const SharedKernelParams &c, int part, bool whole)
-        : p{c.a.q, c.a.out, c.a.n_heads, c.a.n_kv, c.a.prefix_rows, c.a.n * c.a.n_seqs}, a(c.a), ws(c.ws), pieces(c.slots), piece_steps(whole ? 1 << 30 : c.part[part].piece_steps),
-          first_slot(c.part[part].first_slot), cut(c.cut) {}
+        : p{c.a.q, c.a.out, c.a.n_heads, c.a.n_kv, c.a.prefix_rows, c.a.n * c.a.n_seqs}, a(c.a), ws(c.ws), pieces(c.slots), first_slot(c.part[part].first_slot), cut(c.cut),
+          piece_steps(whole ? 1 << 30 : c.part[part].piece_steps) {}
     __device__ float *partials(int g, int rows, int r, int hd) const { return ws + ((size_t)g * (rows - cut) + r - cut) * pieces * (hd + 2); }
 };
 // The prefix alone: all rows are at its last position, padding too, and a join tells these apart.  (There is always one: of a call that sees a prefix some row has a position
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(kAjWaves *kWave) void attn_shared_join_kernel(Share
         if ((int)threadIdx.x < HD) out[threadIdx.x] = (QT)0.0f;
         return;
     }
-    join_pieces<QT, HD, kAjWaves>(part, c.ws + ((size_t)g * all + blockIdx.x) * c.slots * (HD + 2), c.slots, row.n_pieces, out);
+    join_pieces<QT, HD, kAjWaves>(part, c.ws + ((size_t)g * all + blockIdx.x) * c.slots * (HD + 2), c.slots, row.n_pieces, [&] { return out; });
 }
 
 // ... HD / 4 lanes for a row, where there are many: every lane works out the pieces' weights for itself, eight pieces at a time with a running reference point, and adds up four

@@ -98,8 +98,8 @@ struct WindowView {
     static constexpr bool kTexts = false; // see attn_rows_device.h
     static constexpr int first_slot = 0;  // of the pieces' places in work memory
     const AttnWindowParams &p;
-    float *ws;
-    int pieces, piece_steps;
+    float *const &ws; // (references, to what a kernel reads from its arguments where it needs it: with copies, which lived through the loops, f16 heads of 64 took 93 registers instead of
+    const int &pieces, &piece_steps; // 80, and two workgroups fitted a compute unit instead of three)
     __device__ explicit WindowView(const AttnCutParams &c) : p(c.a), ws(c.ws), pieces(c.pieces), piece_steps(c.piece_steps) {}
     __device__ int start(int b) const { return p.start[b]; }
     __device__ int position(int start, int i) const { return start + i; }
@@ -115,9 +115,10 @@ struct WindowView {
 // (device-scope stores, ticket and loads, one after the other), this takes about 3.
 constexpr int kAjWaves = 4;
 
-// One row: `ws` holds the pairs (m, sum) of `slots` pieces and then their sums O; the first n_pieces count.  All threads of the workgroup take part.
-template <typename QT, int HD, int kShare>
-__device__ __forceinline__ void join_pieces(float (&part)[kAjWaves * (kWave / (HD / 2))][HD], const float *ws, int slots, int n_pieces, QT *out) {
+// One row: `ws` holds the pairs (m, sum) of `slots` pieces and then their sums O; the first n_pieces count.  All threads of the workgroup take part.  out(): where the row's
+// result goes, worked out behind the sums, which the loads have to be on their way for first.
+template <typename QT, int HD, int kShare, typename Out>
+__device__ __forceinline__ void join_pieces(float (&part)[kAjWaves * (kWave / (HD / 2))][HD], const float *ws, int slots, int n_pieces, Out out) {
     constexpr int kLanes = HD / 2, kSub = kWave / kLanes; // lanes per piece, pieces side by side in a wavefront
     constexpr int kParts = kShare * kSub;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -154,11 +155,12 @@ __device__ __forceinline__ void join_pieces(float (&part)[kAjWaves * (kWave / (H
     }
     *reinterpret_cast<float2 *>(&part[wave * kSub + sub][d]) = o;
     __syncthreads();
+    QT *const to = out();
     for (int e = kShare == 1 ? lane : (int)threadIdx.x; e < HD; e += kShare * kWave) {
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kParts; w++) sum += part[wave / kShare * kParts + w][e];
-        out[e] = (QT)(L == 0.0f ? 0.0f : sum / L);
+        to[e] = (QT)(L == 0.0f ? 0.0f : sum / L);
     }
 }
 
@@ -180,9 +182,10 @@ __global__ __launch_bounds__(kAjWaves *kWave) void attn_join_kernel(AttnCutParam
         if constexpr (kShare == 1) __syncthreads();
         return;
     }
-    const int i = r / group;
-    join_pieces<QT, HD, kShare>(part, pp.ws + ((size_t)unit * rows + r) * pp.pieces * (HD + 2), pp.pieces, n_pieces,
-                                reinterpret_cast<QT *>(p.out) + ((size_t)(b * p.n + i) * p.n_heads + g * group + (r - i * group)) * HD);
+    join_pieces<QT, HD, kShare>(part, pp.ws + ((size_t)unit * rows + r) * pp.pieces * (HD + 2), pp.pieces, n_pieces, [&] {
+        const int i = r / group;
+        return reinterpret_cast<QT *>(p.out) + ((size_t)(b * p.n + i) * p.n_heads + g * group + (r - i * group)) * HD;
+    });
 }
 
 template <typename QT, int HD, int kTileRows, int kStep>

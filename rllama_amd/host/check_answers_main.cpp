@@ -1,11 +1,13 @@
 // check_answers_main.cpp -- the tensor methods of rllama_hip.hpp for many answers to one prompt as a program: reads one step's inputs from a file, runs it through the
 // C++ mirror and writes what comes out (tests/test_gpu_answers_mirror.py compares with the same calls from Python).
 //
-//   rllama_check_answers IN OUT
+//   rllama_check_answers IN OUT [PARTS]
 //
 // IN: nine int32 (heads, key and value heads, head size, texts, prefix, cache rows of a text, vocabulary, tokens of a row, alternatives), then f32: the prompt's rows of the
 // projection [prefix x (heads + 2 kv) hd], rows of the step [texts x heads hd], weights of the projection and of the output head; i32: positions of the texts, tokens.
 // OUT: attention f32, the head's weights as their 8-bit buffer, logits f32, log probabilities, entropies, ids and log probabilities of the alternatives.
+// PARTS: the same calls with what may be left out: attention without a prefix f32; log probabilities and entropies without alternatives; entropies, ids and log probabilities of the
+// alternatives without tokens.
 #include "rllama_hip.hpp"
 
 #include <cstdio>
@@ -22,7 +24,7 @@ static void put(std::ofstream &to, const Tensor &t, size_t bytes) {
     to.write(host.data(), (std::streamsize)bytes);
 }
 
-static int run(const char *in_path, const char *out_path) {
+static int run(const char *in_path, const char *out_path, const char *parts_path) {
     std::ifstream in(in_path, std::ios::binary);
     const std::vector<char> data((std::istreambuf_iterator<char>(in)), std::istreambuf_iterator<char>());
     int32_t n[9];
@@ -64,16 +66,30 @@ static int run(const char *in_path, const char *out_path) {
     put(to, p.top_ids, (size_t)texts * top * 4);
     put(to, p.top_logprobs, (size_t)texts * top * 4);
     to.flush();
-    return to ? 0 : 1;
+    if (!to) return 1;
+    if (!parts_path) return 0;
+
+    const Tensor alone = q.attn_shared(cache_k, cache_v, heads, kv, cache_rows, starts);
+    const Tensor::Logprobs given = logits.token_logprobs(tokens), best = logits.token_logprobs(top, 0.7f);
+    if (!given.top_ids.empty() || !given.top_logprobs.empty() || !best.logprobs.empty()) throw std::runtime_error("results that were not asked for");
+    std::ofstream parts(parts_path, std::ios::binary);
+    put(parts, alone, (size_t)texts * dim * 4);
+    put(parts, given.logprobs, (size_t)texts * m * 4);
+    put(parts, given.entropy, (size_t)texts * 4);
+    put(parts, best.entropy, (size_t)texts * 4);
+    put(parts, best.top_ids, (size_t)texts * top * 4);
+    put(parts, best.top_logprobs, (size_t)texts * top * 4);
+    parts.flush();
+    return parts ? 0 : 1;
 }
 
 int main(int argc, char **argv) {
-    if (argc != 3) {
-        std::fprintf(stderr, "usage: rllama_check_answers IN OUT\n");
+    if (argc != 3 && argc != 4) {
+        std::fprintf(stderr, "usage: rllama_check_answers IN OUT [PARTS]\n");
         return 2;
     }
     try {
-        return run(argv[1], argv[2]);
+        return run(argv[1], argv[2], argc > 3 ? argv[3] : nullptr);
     } catch (const std::exception &e) {
         std::fprintf(stderr, "%s\n", e.what());
         return 1;

@@ -229,6 +229,7 @@ class Tensor {
     int64_t rows() const { return rows_; }
     int64_t cols() const { return cols_; }
     TensorDType dtype() const { return dtype_; }
+    bool empty() const { return h_ == nullptr; } // (moved from, or a result that was not asked for)
 
     void to_cpu(void *host, int64_t cols_capacity) const { check(rlh_tensor_download(h_, host, (int)cols_capacity, nullptr)); }
     Tensor transpose() const {
@@ -314,9 +315,16 @@ class Tensor {
         check(rlh_attn_shared(out.h_, h_, prefix_k.h_, prefix_v.h_, prefix_len, cache_k.h_, cache_v.h_, n_heads, n_kv_heads, max_seq_len, start_pos.data(), (int)start_pos.size()));
         return out;
     }
-    // this = logits: log probabilities of tokens i32 [rows x m], the entropy of each row, and its `top` most probable ids (top > 0)
+    // ... without a prefix
+    Tensor attn_shared(const Tensor &cache_k, const Tensor &cache_v, int n_heads, int n_kv_heads, int max_seq_len, const std::vector<int32_t> &start_pos) const {
+        Tensor out = zeros(cl_, rows_, cols_, dtype_);
+        check(rlh_attn_shared(out.h_, h_, nullptr, nullptr, 0, cache_k.h_, cache_v.h_, n_heads, n_kv_heads, max_seq_len, start_pos.data(), (int)start_pos.size()));
+        return out;
+    }
+    // this = logits: log probabilities of tokens i32 [rows x m], the entropy of each row, and its `top` most probable ids; what is not asked for (no tokens, top = 0) is empty
     struct Logprobs;
-    Logprobs token_logprobs(const Tensor &tokens, int top, float temperature = 1.0f) const;
+    Logprobs token_logprobs(const Tensor &tokens, int top = 0, float temperature = 1.0f) const;
+    Logprobs token_logprobs(int top, float temperature = 1.0f) const;
     // this [n x k], f16, f32 or Float8, times weights[m x k]^T in Float8Tiles
     Tensor matrix_mul_f8(const Tensor &weights, TensorDType result = TensorDType::Float16) const {
         Tensor out = zeros(cl_, rows_, weights.rows_, result);
@@ -325,6 +333,8 @@ class Tensor {
     }
 
   private:
+    Tensor() = default;
+    Logprobs token_logprobs(const Tensor *tokens, int top, float temperature) const;
     Tensor(std::shared_ptr<OpenCL> cl, rlh_tensor *h, int64_t r, int64_t c, TensorDType d) : cl_(std::move(cl)), h_(h), rows_(r), cols_(c), dtype_(d) {}
     std::shared_ptr<OpenCL> cl_;
     rlh_tensor *h_ = nullptr;
@@ -335,11 +345,14 @@ class Tensor {
 struct Tensor::Logprobs {
     Tensor logprobs, entropy, top_ids, top_logprobs;
 };
-inline Tensor::Logprobs Tensor::token_logprobs(const Tensor &tokens, int top, float temperature) const {
-    Logprobs r{zeros(cl_, rows_, tokens.cols_, TensorDType::Float32), zeros(cl_, rows_, 1, TensorDType::Float32), zeros(cl_, rows_, top, TensorDType::Int32),
-               zeros(cl_, rows_, top, TensorDType::Float32)};
-    check(rlh_token_logprobs(r.logprobs.h_, r.entropy.h_, r.top_ids.h_, r.top_logprobs.h_, h_, tokens.h_, temperature));
+inline Tensor::Logprobs Tensor::token_logprobs(const Tensor *tokens, int top, float temperature) const {
+    auto make = [&](bool asked, int64_t cols, TensorDType dtype) { return asked ? zeros(cl_, rows_, cols, dtype) : Tensor(); };
+    Logprobs r{make(tokens, tokens ? tokens->cols_ : 0, TensorDType::Float32), make(true, 1, TensorDType::Float32), make(top != 0, top, TensorDType::Int32),
+               make(top != 0, top, TensorDType::Float32)};
+    check(rlh_token_logprobs(r.logprobs.h_, r.entropy.h_, r.top_ids.h_, r.top_logprobs.h_, h_, tokens ? tokens->h_ : nullptr, temperature));
     return r;
 }
+inline Tensor::Logprobs Tensor::token_logprobs(const Tensor &tokens, int top, float temperature) const { return token_logprobs(&tokens, top, temperature); }
+inline Tensor::Logprobs Tensor::token_logprobs(int top, float temperature) const { return token_logprobs(nullptr, top, temperature); }
 
 } // namespace rllama

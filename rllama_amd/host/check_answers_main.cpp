@@ -7,7 +7,7 @@
 // projection [prefix x (heads + 2 kv) hd], rows of the step [texts x heads hd], weights of the projection and of the output head; i32: positions of the texts, tokens.
 // OUT: attention f32, the head's weights as their 8-bit buffer, logits f32, log probabilities, entropies, ids and log probabilities of the alternatives.
 // PARTS: the same calls with what may be left out: attention without a prefix f32; log probabilities and entropies without alternatives; entropies, ids and log probabilities of the
-// alternatives without tokens.
+// alternatives without tokens; attention times the head's weights in the rows' own type, f32, and from 8 bits, f16.
 #include "rllama_hip.hpp"
 
 #include <cstdio>
@@ -72,6 +72,8 @@ static int run(const char *in_path, const char *out_path, const char *parts_path
     const Tensor alone = q.attn_shared(cache_k, cache_v, heads, kv, cache_rows, starts);
     const Tensor::Logprobs given = logits.token_logprobs(tokens), best = logits.token_logprobs(top, 0.7f);
     if (!given.top_ids.empty() || !given.top_logprobs.empty() || !best.logprobs.empty()) throw std::runtime_error("results that were not asked for");
+    const Tensor whole = out.matrix_mul_f8(w_head), narrow = out.convert(TensorDType::Float8).matrix_mul_f8(w_head);
+    if (whole.dtype() != TensorDType::Float32 || narrow.dtype() != TensorDType::Float16) throw std::runtime_error("results of another type");
     std::ofstream parts(parts_path, std::ios::binary);
     put(parts, alone, (size_t)texts * dim * 4);
     put(parts, given.logprobs, (size_t)texts * m * 4);
@@ -79,6 +81,8 @@ static int run(const char *in_path, const char *out_path, const char *parts_path
     put(parts, best.entropy, (size_t)texts * 4);
     put(parts, best.top_ids, (size_t)texts * top * 4);
     put(parts, best.top_logprobs, (size_t)texts * top * 4);
+    put(parts, whole, (size_t)texts * vocab * 4);
+    put(parts, narrow, (size_t)texts * vocab * 2);
     parts.flush();
     return parts ? 0 : 1;
 }

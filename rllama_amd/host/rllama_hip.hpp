@@ -325,8 +325,9 @@ class Tensor {
     struct Logprobs;
     Logprobs token_logprobs(const Tensor &tokens, int top = 0, float temperature = 1.0f) const;
     Logprobs token_logprobs(int top, float temperature = 1.0f) const;
-    // this [n x k], f16, f32 or Float8, times weights[m x k]^T in Float8Tiles
-    Tensor matrix_mul_f8(const Tensor &weights, TensorDType result = TensorDType::Float16) const {
+    // this [n x k], f16, f32 or Float8, times weights[m x k]^T in Float8Tiles -> [n x m] of this tensor's own type (of Float8: f16), or of the one that is given
+    Tensor matrix_mul_f8(const Tensor &weights) const { return matrix_mul_f8(weights, dtype_ == TensorDType::Float8 ? TensorDType::Float16 : dtype_); }
+    Tensor matrix_mul_f8(const Tensor &weights, TensorDType result) const {
         Tensor out = zeros(cl_, rows_, weights.rows_, result);
         check(rlh_matrix_mul_f8(out.h_, h_, weights.h_));
         return out;

@@ -32,5 +32,5 @@ def test_calls_with_parts_left_out(ctx, tmp_path, B):
     logits = out.convert(TensorDType.Float8).matrix_mul_f8(w_head, TensorDType.Float32)
     given, best = logits.token_logprobs(Tensor.from_numpy(ctx, tokens)), logits.token_logprobs(None, 0.7, top)
     assert given[2] is None and given[3] is None and best[0] is None
-    want = [q.attn_shared(None, None, 0, ck, cv, H, G, S, starts), *given[:2], *best[1:]]
+    want = [q.attn_shared(None, None, 0, ck, cv, H, G, S, starts), *given[:2], *best[1:], out.matrix_mul_f8(w_head), out.convert(TensorDType.Float8).matrix_mul_f8(w_head)]
     assert rest.read_bytes() == b"".join(t.to_numpy().tobytes() for t in want)

@@ -539,17 +539,17 @@ class Tensor:
                                         n_kv_heads, max_seq_len, (C.c_int32 * len(start_pos))(*start_pos), len(start_pos)))
         return out
 
-    def token_logprobs(self, tokens: Optional["Tensor"] = None, temperature: float = 1.0, top: int = 0, logprobs: Optional["Tensor"] = None, entropy: Optional["Tensor"] = None,
+    def token_logprobs(self, tokens: Optional["Tensor"] = None, temperature: float = 1.0, top: int = 0, logprobs: Optional["Tensor"] = None, entropy: "Tensor | bool | None" = None,
                        top_ids: Optional["Tensor"] = None, top_logprobs: Optional["Tensor"] = None):
         """self = logits [n x vocab]: (log probabilities of tokens i32 [n x m], entropy [n x 1], the `top` most probable ids and their log probabilities [n x top]);
-        None in the place of what is not asked for.  Results that are given are written to instead."""
+        None in the place of what is not asked for (no tokens, top = 0, entropy = False).  Results that are given are written to instead."""
         make = lambda cols, kind: Tensor.zeros(self.ctx, self._rows, cols, kind)  # noqa: E731
         logprobs = logprobs or (make(tokens._cols, TensorDType.Float32) if tokens else None)
-        entropy = entropy or make(1, TensorDType.Float32)
+        entropy = None if entropy is False else entropy if isinstance(entropy, Tensor) else make(1, TensorDType.Float32)
         top_ids = top_ids or (make(top, TensorDType.Int32) if top else None)
         top_logprobs = top_logprobs or (make(top_ids._cols, TensorDType.Float32) if top_ids else None)
         handle = lambda t: t._h if t else None  # noqa: E731
-        check(self._lib.rlh_token_logprobs(handle(logprobs), entropy._h, handle(top_ids), handle(top_logprobs), self._h, handle(tokens), temperature))
+        check(self._lib.rlh_token_logprobs(handle(logprobs), handle(entropy), handle(top_ids), handle(top_logprobs), self._h, handle(tokens), temperature))
         return logprobs, entropy, top_ids, top_logprobs
 
     def matrix_mul_f8(self, weights: "Tensor", dtype: Optional[int] = None, out: Optional["Tensor"] = None) -> "Tensor":

@@ -5,7 +5,7 @@ import pytest
 
 from rllama_amd import Tensor
 from test_gpu_answers import first_of_the_largest, logprobs_reference, shared_case, shared_reference
-from test_gpu_longctx import EPS16, EPS32, NUMPY, TYPES, f16, f32, f64, upload, values
+from test_gpu_longctx import EPS16, EPS32, INVALID, NUMPY, TYPES, f16, f32, f64, refused, upload, values
 
 pytestmark = pytest.mark.gpu
 
@@ -71,6 +71,17 @@ def test_logprobs_of_logits_from_end_to_end(ctx, vocab, kind):
     x[4, 1] = info.min
     for temperature in (1.0, 1e30, 2.5e29, 1e-30):
         check_logprobs(ctx, x, temperature)
+
+
+def test_the_entropy_may_be_left_out(ctx):
+    """entropy=False: None, and the library is not asked for it; a call that asks for nothing is refused."""
+    logits, tokens = Tensor.from_numpy(ctx, np.eye(3, 50, dtype=f32)), Tensor.from_numpy(ctx, np.array([[0], [1], [2]], np.int32))
+    whole = logits.token_logprobs(tokens, 0.5, 2)
+    part = logits.token_logprobs(tokens, 0.5, 2, entropy=False)
+    assert part[1] is None and whole[1].to_numpy().shape == (3, 1)
+    assert all(np.array_equal(a.to_numpy(), b.to_numpy()) for a, b in zip(whole, part) if b is not None)
+    assert logits.token_logprobs(entropy=whole[1])[1] is whole[1]
+    refused(INVALID, logits.token_logprobs, entropy=False)
 
 
 # -- attention: padding -------------------------------------------------------------------------------------------------------------------

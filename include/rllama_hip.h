@@ -396,8 +396,10 @@ int  rlh_token_logprobs(rlh_tensor *logprobs, rlh_tensor *entropy, rlh_tensor *t
  *
  * dst [n x m] = src [n x k] times weights[m x k]^T: weights RLH_F8_TILES; src RLH_F8, or f16 or f32, which is converted to RLH_F8 first; dst f16 or f32.
  * The sum of a block of 128 products, then that times both scales, added up in f32.  f32 results, and up to 16 rows: every sum is one of f32.  f16 results of more rows: the 8-bit
- * matrix instruction, which adds products up eight at a time and cuts off what is 2^-13 and less of the largest one's power of two (random operands: off by 1.5e-5 of the
- * result, a fourteenth of its rounding to f16).  k up to 2^24, n and m up to 2^26. */
+ * matrix instruction, which adds products up eight at a time and cuts off what is 2^-13 and less of the largest one's power of two.  That is off by 1.4e-5 of the results' size for
+ * operands of one size (a fifteenth of the rounding to f16), by 2e-5 to 6e-5 where columns are powers of ten apart (standard deviations of their logarithms from 0.7 to 4); a result that
+ * cancels has up to 1e-4 of its products' magnitudes (4096 columns; 7 * 2^-13 at most) on top of its rounding.  rlh_set_option GEMM_F8_EXACT = 1: those are sums of f32 too (2048 rows
+ * of 13824 x 5120 147 -> 288 us, 64 of 11008 x 4096 16.8 -> 21.3).  k up to 2^24, n and m up to 2^26. */
 int  rlh_matrix_mul_f8(rlh_tensor *dst, const rlh_tensor *src, const rlh_tensor *weights);
 
 /* ------------------------------------------------------------------------------------------------

@@ -64,6 +64,7 @@ struct MatmulF8Params {
     EightRef x, w; // [m x k] a scale for every row and block, [n x k] a scale for every tile
     void *y;       // [m x n]
     int y_f16;
+    int exact; // f16 results of many rows are summed up in f32 as well
     int m, n, k;
 };
 bool matmul_f8_converts(int m, int k);                                   // whether a product of m rows converts f16 and f32 rows on the way

@@ -156,6 +156,7 @@ bool tunables_set(Tunables &t, const char *name, const char *value) {
     if (n == "ATTN_MERGE") { t.attn_merge_mode = reset ? dflt.attn_merge_mode : v; return reset || v == 0 || v == 2; }
     if (n == "ATTN_LDS") { t.attn_lds = reset ? 0 : (v != 0); return true; }
     if (n == "ATTN_EXACT") { t.attn_exact = reset ? 0 : (v != 0); return true; }
+    if (n == "GEMM_F8_EXACT") { t.gemm_f8_exact = reset ? 0 : (v != 0); return true; }
     if (n == "ATTN_SHARED_FORM") { t.attn_shared_form = reset ? 0 : v; return reset || (v >= 0 && v <= 2); }
     if (n == "PREFILL_ATTN") { t.prefill_attn_gemm = !reset && !strcmp(value, "gemm"); return reset || !strcmp(value, "gemm") || !strcmp(value, "fused"); }
     if (n == "PREFILL_ATTN_ORDER") { t.prefill_attn_order = reset ? dflt.prefill_attn_order : v; return reset || (v >= 0 && v <= 2); }
@@ -176,7 +177,7 @@ bool tunables_set(Tunables &t, const char *name, const char *value) {
 }
 
 void tunables_from_env(Tunables &t) {
-    static const char *const names[] = {"GEMV_BURST", "ATTN_CHUNK", "ATTN_SINGLE_MAX", "ATTN_MERGE", "ATTN_LDS", "ATTN_EXACT", "ATTN_SHARED_FORM", "PREFILL_ATTN", "PREFILL_ATTN_ORDER",
+    static const char *const names[] = {"GEMV_BURST", "ATTN_CHUNK", "ATTN_SINGLE_MAX", "ATTN_MERGE", "ATTN_LDS", "ATTN_EXACT", "ATTN_SHARED_FORM", "GEMM_F8_EXACT", "PREFILL_ATTN", "PREFILL_ATTN_ORDER",
                                         "DECODE_GRAPH", "DECODE_FOLD", "GEMM_TILE", "GEMM_SPLIT_K", "GEMM_SPLIT_HALF", "GEMM_DUAL", "GEMM_DUAL_CUT",
                                         "GEMM_ROPE", "FINISH_NORM", "GEMM_KGROUP", "GEMM_SKINNY", "GEMM_ROWS", "GEMM_SPLIT3"};
     for (const char *name : names) {

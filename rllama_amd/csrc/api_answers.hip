@@ -156,6 +156,7 @@ extern "C" int rlh_matrix_mul_f8(rlh_tensor *dst, const rlh_tensor *src, const r
     p.k = src->cols;
     p.y = dst->p;
     p.y_f16 = dst->dtype == RLH_F16;
+    p.exact = ctx->tun.gemm_f8_exact;
     p.w = eight_of(weights);
     const int cus = ctx->prop.multiProcessorCount;
     // work memory: the sums of pieces of K, and src in 8 bits where the product does not convert it on the way

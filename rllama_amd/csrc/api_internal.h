@@ -64,6 +64,7 @@ struct Tunables {
     int attn_merge_mode = 2;       // ATTN_MERGE=0: the pieces of a split sequence are combined by a second launch; 2: inside the kernel
     int attn_lds = 0;              // ATTN_LDS=1: cache rows staged through LDS (comparison form)
     int attn_exact = 0;            // ATTN_EXACT=1: rlh_attn_window and rlh_attn_shared in f16 round nothing but their result, whatever the number of rows
+    int gemm_f8_exact = 0;         // GEMM_F8_EXACT=1: rlh_matrix_mul_f8 sums up in f32 whatever the results' type and the number of rows
     int attn_shared_form = 0;      // ATTN_SHARED_FORM=1/2: rlh_attn_shared takes 16 rows at a time, or tiles wherever it can; 0: what an estimate of the time says
     int prefill_attn_gemm = 0;     // PREFILL_ATTN=gemm: multi-token attention as two batched GEMMs around a softmax kernel
     int prefill_attn_order = 2;    // PREFILL_ATTN_ORDER=0/1/2: launch order of the query blocks of the one-kernel attention

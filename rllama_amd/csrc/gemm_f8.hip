@@ -5,9 +5,9 @@
 // one row, whose scale is the lane's own; the columns' scale is the same for a whole tile.
 //
 // Which matrix instruction.  v_mfma_f32_16x16x128_f8f6f4 takes 128 products at once, but adds them up eight at a time with the products aligned to the largest one's power
-// of two and cut off 2^-13 below it (measured; random operands: 1.5e-5 of the result, whatever the number of blocks), where f32 sums keep 1e-7.  f16 results are
-// rounded by 2.1e-4 of their size anyway.  So it is taken for f16 results of more than 16 rows.  Fewer are bound by memory, and f32 results
-// are to be as exact as f32 is: there the codes become f16 numbers (exactly: one conversion per pair) for v_mfma_f32_16x16x32_f16.
+// of two and cut off 2^-13 below it (measured: 1.4e-5 of the results' size for operands of one size, whatever the number of blocks, up to 6e-5 where columns are powers of ten apart),
+// where f32 sums keep 1e-7.  f16 results are rounded by 2.1e-4 of their size anyway.  So it is taken for f16 results of more than 16 rows (GEMM_F8_EXACT: not there either).  Fewer
+// are bound by memory, and f32 results are to be as exact as f32 is: there the codes become f16 numbers (exactly: one conversion per pair) for v_mfma_f32_16x16x32_f16.
 //
 // Measured, with the conversion of f16 or f32 rows: 1 row of 4096 x 4096 5.4 us; 16 rows of 32000 x 4096, f32 results, 29.8 us, the weights at 5.5 TB/s in 24 of it; 64 rows of 11008 x 4096
 // 16.3 us; 131 rows of 4096 x 11008, f32 results, 30 us; 2048 rows of 13824 x 5120 from 8 bits 152 us, 1.9 PFLOP/s (a library product with one scale for all: 116 us).
@@ -480,8 +480,11 @@ constexpr int kConvertRows = 8; // up to which rows of f16 and f32 are converted
 
 bool matmul_f8_converts(int m, int k) { return m <= kConvertRows && rows_f8_lds(m, k) <= kRfLds; }
 
+// by the f16 instruction, of more rows than a few
+static bool exact_products(const MatmulF8Params &p) { return !p.y_f16 || p.exact; }
+
 // Tiles, and pieces of K.  A call takes about 5 us, tb for every block of K in every round of workgroups over the compute units, and where K is cut 3 us more and the sums' way to memory
-// and back, 8 bytes per sum and piece at 4.5 bytes per ps.  (tb of f16 and of f32 results, measured in products of 32 to 2048 rows.  Of the smallest tile two workgroups
+// and back, 8 bytes per sum and piece at 4.5 bytes per ps.  (tb of the 8-bit instruction and of the f16 one, measured in products of 32 to 2048 rows.  Of the smallest tile two workgroups
 // fit a compute unit, which take 1.7 times as long as one.)  The least sum is taken: 64 rows of 11008 x 4096 in two pieces 15.2 us (one 18.7, three 18.7), 131 of 4096 x 11008 in
 // eight pieces of 160 rows 22.7 us (four of 128 23.8, five of 64 23.9), 1024 of 11008 x 4096 in large tiles 56 us (small ones 76), 1024 of 4096 x 4096 in small ones 27 (52).
 struct TilesPlan {
@@ -492,8 +495,8 @@ static TilesPlan plan_tiles(const MatmulF8Params &p, int compute_units) {
         int bm, bn;
         double tb;
     };
-    const bool f16 = p.y_f16 != 0;
-    const Kind kinds[] = {{64, 128, f16 ? 0.43 : 0.68}, {128, 128, f16 ? 0.68 : 1.15}, {160, 128, f16 ? 0.66 : 1.2}, {256, f16 ? 256 : 128, f16 ? 1.6 : 1.76}};
+    const bool quick = !exact_products(p);
+    const Kind kinds[] = {{64, 128, quick ? 0.43 : 0.68}, {128, 128, quick ? 0.68 : 1.15}, {160, 128, quick ? 0.66 : 1.2}, {256, quick ? 256 : 128, quick ? 1.6 : 1.76}};
     const int across = f8_blocks(p.k);
     TilesPlan best{};
     double least = 0.0;
@@ -536,10 +539,18 @@ static hipError_t launch_rows(const RowsF8Params &p, int source, hipStream_t s) 
     return hipGetLastError();
 }
 
-template <int kWM, int kWN, int kMT, int kNT, int kStages, typename Y>
+template <int kWM, int kWN, int kMT, int kNT, int kStages, bool kExact, typename Y>
 static void launch_tiles(const TilesF8Params &q, hipStream_t s) {
     const dim3 grid((unsigned)((q.tiles_m * q.tiles_n + 7) / 8 * 8), (unsigned)q.pieces);
-    hipLaunchKernelGGL((matmul_f8_tiles_kernel<kWM, kWN, kMT, kNT, kStages, sizeof(Y) == 4, Y>), grid, dim3(kWM * kWN * kWave), 0, s, q);
+    hipLaunchKernelGGL((matmul_f8_tiles_kernel<kWM, kWN, kMT, kNT, kStages, kExact, Y>), grid, dim3(kWM * kWN * kWave), 0, s, q);
+}
+
+template <bool kExact, typename Y>
+static void launch_plan(const TilesPlan &t, const TilesF8Params &q, hipStream_t s) {
+    if (t.bm == 64) launch_tiles<2, 2, 2, 4, 3, kExact, Y>(q, s);
+    else if (t.bm == 128) launch_tiles<4, 2, 2, 4, 4, kExact, Y>(q, s);
+    else if (t.bm == 160) launch_tiles<2, 2, 5, 4, 4, kExact, Y>(q, s);
+    else launch_tiles<4, 2, 4, kExact ? 4 : 8, 2, kExact, Y>(q, s);
 }
 
 template <typename Y>
@@ -555,10 +566,12 @@ static hipError_t launch_y(const MatmulF8Params &p, const void *src, int source,
     }
     const TilesPlan t = plan_tiles(p, compute_units);
     const TilesF8Params q{p, t.pieces > 1 ? ws : nullptr, t.pieces, t.tiles_m, t.tiles_n};
-    if (t.bm == 64) launch_tiles<2, 2, 2, 4, 3, Y>(q, s);
-    else if (t.bm == 128) launch_tiles<4, 2, 2, 4, 4, Y>(q, s);
-    else if (t.bm == 160) launch_tiles<2, 2, 5, 4, 4, Y>(q, s);
-    else launch_tiles<4, 2, 4, sizeof(Y) == 4 ? 4 : 8, 2, Y>(q, s);
+    if constexpr (sizeof(Y) == 2) {
+        if (exact_products(p)) launch_plan<true, Y>(t, q, s);
+        else launch_plan<false, Y>(t, q, s);
+    } else {
+        launch_plan<true, Y>(t, q, s);
+    }
     if (t.pieces > 1) {
         const size_t count = (size_t)p.m * p.n;
         hipLaunchKernelGGL(matmul_f8_join_kernel<Y>, dim3((unsigned)std::min<size_t>((count + 1023) / 1024, 8192)), dim3(256), 0, s, (Y *)p.y, ws, t.pieces, count);

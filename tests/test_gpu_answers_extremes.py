@@ -3,6 +3,7 @@ rows of padding that hold anything."""
 import numpy as np
 import pytest
 
+import test_gpu_answers as base
 from rllama_amd import Tensor
 from test_gpu_answers import first_of_the_largest, logprobs_reference, shared_case, shared_reference
 from test_gpu_longctx import EPS16, EPS32, INVALID, NUMPY, TYPES, f16, f32, f64, refused, upload, values
@@ -149,3 +150,29 @@ def test_padding_rows_hold_anything(form, hd, H, G, n, P, B, kind, cache):
     for b, start in enumerate(starts):
         assert (got[b, :max(0, min(n, -start))] == 0).all()
     assert (np.abs(got - want) <= bound).all()
+
+
+# -- products -----------------------------------------------------------------------------------------------------------------------------
+
+@pytest.fixture
+def exact(ctx):
+    ctx.set_option("GEMM_F8_EXACT", "1")
+    yield ctx
+    ctx.set_option("GEMM_F8_EXACT", None)
+
+
+@pytest.mark.parametrize("m,n,k", base.PRODUCTS)
+@pytest.mark.parametrize("source,spread", [("f16", 1.0), ("f8", 1.0), ("f8", 3.0)])
+def test_f16_results_summed_up_in_f32_on_request(exact, m, n, k, source, spread):
+    """Columns of x a few powers of ten apart, whose products the 8-bit instruction cuts off beside the largest ones: the bound is that of sums in f32, and the result's rounding."""
+    rng = np.random.default_rng(m * 7 + n + k)
+    x = (rng.standard_normal((m, k)) * np.exp(spread * rng.standard_normal((1, k)))).astype(f32)
+    x = x / np.abs(x).max() * 100  # (within f16)
+    w = Tensor.from_numpy(exact, (rng.standard_normal((n, k)) / np.sqrt(k)).astype(f32)).convert(base.TILES)
+    x = Tensor.from_numpy(exact, x.astype(f16 if source == "f16" else f32))
+    eight = x.convert(base.F8)
+    a, b = base.stands_for(*base.parts(eight), False), base.stands_for(*base.parts(w), True)
+    out = Tensor.from_numpy(exact, np.full((m, n), np.nan, f16))
+    (eight if source == "f8" else x).matrix_mul_f8(w, out=out)
+    want = a @ b.T
+    assert (np.abs(out.to_numpy() - want) <= base.product_bound(a, b, k, "f32") + EPS16 * np.abs(want) + 2.0 ** -25).all()

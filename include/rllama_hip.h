@@ -380,7 +380,8 @@ int  rlh_rope_table_from(rlh_tensor *freqs, double theta, int first);
  * the planes may be NULL); cache planes: two tensors [n_seqs * n_kv_heads * max_seq_len x head_dim], row (b * n_kv_heads + g) * max_seq_len + t, which hold the rows' own positions
  * already; all four of one dtype, f16, f32 or Q4; head_dim 32, 64 or 128.  Query head h reads key and value head h / (n_heads / n_kv_heads).  q and out
  * [n_seqs * n x n_heads head_dim], both f16 or both f32.  f32 rows, or f32 planes: f32 arithmetic throughout; otherwise f16 operands with f32 sums,
- * where more than 32 rows of a key and value head (n n_heads / n_kv_heads n_seqs) over many positions round the softmax's weights and 4-bit values to f16 (ATTN_EXACT: they do not).
+ * where more than 32 rows of a key and value head (n n_heads / n_kv_heads n_seqs) over many positions round the softmax's weights and 4-bit values to f16 (ATTN_EXACT: they do not).  Which form a
+ * call takes goes by an estimate of its time, so a text's results may differ in their last bits when the batch around it grows.
  * The prefix is read once for the rows of all texts and not once for each.  Rows and keys outside what is seen may hold anything, NaN included.  prefix_len and max_seq_len: 2^31 - 257 at
  * most. */
 int  rlh_attn_shared(rlh_tensor *out, const rlh_tensor *q, const rlh_tensor *prefix_k, const rlh_tensor *prefix_v, int prefix_len, const rlh_tensor *cache_k,

@@ -349,8 +349,9 @@ SharedPlan plan_attn_shared(const AttnSharedParams &a, int compute_units) {
     const int64_t rows = (int64_t)a.n * (a.n_heads / a.n_kv), all = rows * a.n_seqs;
     SharedPlan c, d;
     const double us = plan_form(a, compute_units, false, c);
-    // Tiles take 128 rows of one head, of up to 16 texts where these go through tiles as well.  The estimates cost 1.2 % over the faster form on average over 160 calls of all sizes, 32 % at
+    // Tiles take 128 rows of one head, of up to 16 texts where these go through tiles as well.  The estimates cost nothing over the faster form on average over 180 calls of all sizes, 23 % at
     // worst; tiles for all of more than 32 rows took up to 2.5 times as long (245 rows of 16 heads behind 120 positions 20 us, 8; 1722 rows of 4 heads behind 8316 are 49 in tiles and 151).
+    // Working this out takes 0.04 to 4 us of host time for up to 256 texts of 8 rows, 36 for 131072 rows of a key and value head.
     if (a.form == 1 || !f16_arithmetic(a) || a.exact || all <= 2 * kAwRows || (a.prefix_len == 0 && rows < kAtRows / (kMaxTexts - 1) + 1)) return c;
     return plan_form(a, compute_units, true, d) < us || a.form == 2 ? d : c;
 }

@@ -19,7 +19,8 @@ struct EightRef {
 };
 
 // Scale and factor of a block whose largest value is `top` (finite): value = code * scale, code = e4m3(value * factor).  The bound keeps both normal numbers; below it
-// a block is all but zero.  (The factor is a reciprocal and a product, two roundings, as array libraries divide a number by an array: codes made there and here are the same.)
+// a block is all but zero.  (The factor is a reciprocal and a product, two roundings, which is what torch makes of a number divided by a tensor: codes made so there and here are the
+// same.  A division rounds once; one code in 1e5 then falls on the other side of a tie.)
 struct F8Scale {
     float scale, factor;
     __device__ explicit F8Scale(float top) {

@@ -487,6 +487,7 @@ static bool exact_products(const MatmulF8Params &p) { return !p.y_f16 || p.exact
 // and back, 8 bytes per sum and piece at 4.5 bytes per ps.  (tb of the 8-bit instruction and of the f16 one, measured in products of 32 to 2048 rows.  Of the smallest tile two workgroups
 // fit a compute unit, which take 1.7 times as long as one.)  The least sum is taken: 64 rows of 11008 x 4096 in two pieces 15.2 us (one 18.7, three 18.7), 131 of 4096 x 11008 in
 // eight pieces of 160 rows 22.7 us (four of 128 23.8, five of 64 23.9), 1024 of 11008 x 4096 in large tiles 56 us (small ones 76), 1024 of 4096 x 4096 in small ones 27 (52).
+// Over the fastest tile and number of pieces it costs 5.7 % on average with the 8-bit instruction and 1.4 % with the f16 one over 16 products each, 25 % at worst (865 x 333 x 10304).
 struct TilesPlan {
     int bm, bn, tiles_m, tiles_n, pieces;
 };
